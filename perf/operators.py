@@ -178,8 +178,10 @@ def _plain_residual_norm(s):
         u = u * s["scale_t"].float()
     if s["gate_t"] is not None:
         u = u * s["gate_t"].float()
-    r = (s["xt"].float() + u).to(TYPE[s["x"]])
-    return r, _plain_norm(r.float(), s["weight"], s["bias"], s["norm"])
+    r = s["xt"].float() + u
+    # the sum as it is stored, in 32 bits, so that its gradient is rounded once, at the end
+    r = r + (r.to(TYPE[s["x"]]).float() - r).detach()
+    return r.to(TYPE[s["x"]]), _plain_norm(r, s["weight"], s["bias"], s["norm"])
 
 
 def _plain_quantize(x):

@@ -317,6 +317,116 @@ int s3r_copy2d_async(void* dst, size_t dst_pitch, const void* src, size_t src_pi
 int s3r_ipc_export(const void* ptr, void* handle64, int64_t* offset);
 int s3r_ipc_import(const void* handle64, int64_t offset, void** ptr);
 
+/* ------------------------------------------------------------------------------------------
+ * The rest of a transformer block around the attention.  BlockRope (pi3/models/layers/block.py:310-335) leaves these steps to
+ * eager PyTorch: x + ls(branch) and the norm that follows, Linear projections, and (trainers/base_trainer_accelerate.py)
+ * gradient clipping and AdamW.
+ * ------------------------------------------------------------------------------------------ */
+#define S3R_F32 0
+#define S3R_BF16 1
+#define S3R_F16 2
+
+#define S3R_NORM_LAYER 0 /* (v - mean) / sqrt(var + eps) */
+#define S3R_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) */
+
+#define S3R_GATE_NONE 0
+#define S3R_GATE_ROW 1     /* gate[b * gate_stride_b + t * gate_stride_t]: one factor per token */
+#define S3R_GATE_CHANNEL 2 /* gate[b * gate_stride_b + c]: one factor per batch entry and channel */
+
+/* u = y, or post_norm(y);  r = x + (u * scale) * gate, rounded to x's type;  h = norm(r).  A norm is the row's, with
+ * `weight` and `bias` (each may be NULL).  x, y, r, h [batch * tokens, channels], contiguous, elements aligned to their size
+ * (vectors are used where addresses and the number of channels allow).  channels 1 to 8192. */
+typedef struct {
+  int64_t batch, tokens;
+  int channels;
+  int kind, post;          /* S3R_NORM_*; post != 0: y is normalised first */
+  float eps, post_eps;
+  int x_type, y_type, h_type, param_type, gate_type, gate_mode;
+  int64_t gate_stride_b, gate_stride_t;
+  const void *x, *y;       /* y NULL: r = x and r may be NULL */
+  const void *weight, *bias, *scale, *post_weight, *post_bias; /* [channels], param_type */
+  const void* gate;
+  void *r, *h;             /* h NULL: no norm */
+  int8_t* q;               /* instead of h: the norm's result as 8-bit tokens, rows of q_pitch bytes, ... */
+  float* q_scale;          /* ... q_scale[row] = max |h| / 127, q = h / q_scale to nearest even */
+  int64_t q_pitch;
+  float* stats;            /* NULL, or [4, batch * tokens]: mean and 1 / sqrt(..) of the norm, and of the post norm */
+} s3r_residual_norm;
+int s3r_residual_norm_fwd(const s3r_residual_norm* args_host, void* stream);
+
+/* Gradients of the above.  f: its arguments with r (x where y is NULL) and stats as the forward left them; h, q, x are not read.
+ *   dr, dh     gradients of r (x_type) and h (h_type); either may be NULL
+ *   dx, dy     [rows, channels], x_type and y_type; dy may be NULL
+ *   d_weight, d_bias, d_scale, d_post_weight, d_post_bias  [channels] param_type, each may be NULL
+ *   d_gate_row      [rows] fp32: gradient of every token's factor (S3R_GATE_ROW), may be NULL
+ *   d_gate_channel  [batch, channels] gate_type (S3R_GATE_CHANNEL), may be NULL
+ * Sums over rows are taken in fp32 in a fixed order. */
+typedef struct {
+  const void *dr, *dh;
+  void *dx, *dy;
+  void *d_weight, *d_bias, *d_scale, *d_post_weight, *d_post_bias;
+  float* d_gate_row;
+  void* d_gate_channel;
+  void* workspace;
+  size_t workspace_bytes;  /* at least s3r_residual_norm_bwd_workspace_bytes */
+} s3r_residual_norm_grad;
+size_t s3r_residual_norm_bwd_workspace_bytes(int64_t batch, int64_t tokens, int channels, int gate_mode);
+int s3r_residual_norm_bwd(const s3r_residual_norm* f_host, const s3r_residual_norm_grad* g_host, void* stream);
+
+/* q[r, c] = x[r, c] * (127 / max |x[r]|) to nearest even, scale[r] = max |x[r]| / 127.  x: rows of x_pitch elements of `type`,
+ * q: rows of q_pitch bytes; NaN in a row makes its scale NaN, rows whose largest
+ * magnitude is below 2^-119 are zeros. */
+int s3r_quantize_rows(const void* x, int type, int64_t x_pitch, int8_t* q, int64_t q_pitch, float* scale, int64_t rows, int channels,
+                      void* stream);
+
+/* out[m, n] = (sum over k of a[m, k] b[n, k]) * a_scale[m] * b_scale[n] + bias[n]: 8-bit operands, 32-bit sums, fp32 from there on.
+ *   a [M, K] rows of a_pitch bytes, b [N, K] rows of b_pitch bytes: bases and pitches multiples of 16, K <= 65536 (sums fit 32 bits)
+ *   bias [N] fp32 or NULL; out rows of N elements of `type`. */
+int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* b, int64_t b_pitch, const float* b_scale,
+                    const float* bias, void* out, int type, int64_t M, int N, int K, void* stream);
+
+/* Euclidean norm of all elements of n tensors, summed in 64 bits in a fixed order.  The arrays are HOST arrays of device pointers,
+ * element counts (0 is allowed) and types.  workspace: s3r_grad_norm_workspace_bytes(n, total elements). */
+size_t s3r_grad_norm_workspace_bytes(int n, const int64_t* counts);
+int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, const int* types, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/* One AdamW step (decoupled weight decay) over n tensors:
+ *   g = factor * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = step + 1
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * factor: 1, or min(1, max_norm / (norm + 1e-6)) where norm != NULL and max_norm > 0.  Where norm != NULL and *norm is not finite
+ * nothing changes, *step included.  *step (int64) becomes t.
+ * States: 32-bit (m, v fp32), or 8-bit where the tensor's entries of `m_exponents` and `v_exponents` are not NULL: m and v are codes, and
+ * the entries hold ceil(count / 256) bytes each, the exponent of each block of 256 codes.  A code c of m stands for
+ * (-1)^(c >> 7) * (E ? (1 + f / 8) 2^(E - 15) : f / 8 2^-14) with E = (c >> 3) & 15, f = c & 7, one of v for
+ * E ? (1 + f / 8) 2^(E - 31) : f / 8 2^-30 with E = c >> 3; both times 2^(exponent - 127), exponent 255: NaN.
+ * seed < 0: what is kept in fewer than 32 bits is rounded to nearest even, else stochastically with Philox 2x32-7, counter (pair of
+ * elements, t), key seed + index of the tensor * 0x85EBCA6B (mod 2^32).
+ * Arrays are HOST arrays; lr: a device pointer that is read on the stream, or NULL for lr_host. */
+typedef struct {
+  int n;
+  void* const* params;
+  const void* const* grads;
+  void* const* m;
+  void* const* v;
+  uint8_t* const* m_exponents; /* both NULL: all states are 32-bit */
+  uint8_t* const* v_exponents;
+  const int64_t* counts;
+  const int *param_types, *grad_types;
+  int64_t* step;
+  const float* lr;
+  double lr_host, beta1, beta2, eps, weight_decay;
+  const float* norm;
+  double max_norm;
+  int64_t seed;
+  void* workspace;            /* 256 bytes */
+} s3r_adamw;
+int s3r_adamw_step(const s3r_adamw* args_host, void* stream);
+
+/* What 8-bit states stand for: m, v (codes) -> fp32. */
+int s3r_adamw_state(int n, const void* const* m, const void* const* v, const uint8_t* const* m_exponents, const uint8_t* const* v_exponents,
+                    float* const* m_out, float* const* v_out, const int64_t* counts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,15 @@ SIGNATURES = {
     "s3r_cast_bf16": (_i, [_i, _p, _p, _p, _p]),
     "s3r_colsum_workspace_bytes": (_sz, [_i64, _i]),
     "s3r_colsum": (_i, [_p, _p, _i64, _i, _p, _sz, _p]),
+    "s3r_residual_norm_fwd": (_i, [_p, _p]),
+    "s3r_residual_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i, _i]),
+    "s3r_residual_norm_bwd": (_i, [_p, _p, _p]),
+    "s3r_quantize_rows": (_i, [_p, _i, _i64, _p, _i64, _p, _i64, _i, _p]),
+    "s3r_int8_linear": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p]),
+    "s3r_grad_norm_workspace_bytes": (_sz, [_i, _p]),
+    "s3r_grad_norm": (_i, [_i, _p, _p, _p, _p, _p, _sz, _p]),
+    "s3r_adamw_step": (_i, [_p, _p]),
+    "s3r_adamw_state": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p]),
     "s3r_copy2d_async": (_i, [_p, _sz, _p, _sz, _sz, _sz, _p]),
     "s3r_peer_pull": (_i, [_p, _p, _p, _i, _i, _p]),
     "s3r_ipc_export": (_i, [_p, _p, C.POINTER(C.c_int64)]),

@@ -69,9 +69,10 @@ def _build_torch_lib() -> None:
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     srcs = sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp")))
+    headers = glob.glob(os.path.join(CSRC, "torch", "*.h")) + glob.glob(os.path.join(PKG, "..", "include", "*.h"))
     stamp = os.path.join(OBJ, "torch_version")
     built_for = open(stamp).read() if os.path.exists(stamp) else ""
-    if built_for == torch.__version__ and not _stale(TORCH_LIB, srcs + glob.glob(os.path.join(PKG, "..", "include", "*.h"))):
+    if built_for == torch.__version__ and not _stale(TORCH_LIB, srcs + headers):
         return
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:

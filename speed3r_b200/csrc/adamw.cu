@@ -1,0 +1,509 @@
+// AdamW over many tensors in one launch, with states in 32 or in 8 bits, and the norm of their gradients.
+// Bound: HBM.  32-bit states 28 bytes per element (fp32 parameters: p, m, v read and written, g read), 8-bit states 16; the norm 4.
+//
+// 8-bit states: blocks of 256 codes share an exponent, so that a block is a warp's work: eight elements per lane, the largest
+// magnitudes by shuffles.  The shared factor is a power of two: it changes only when a block's largest magnitude crosses one, so that
+// the codes' grid stands still between steps.  Rounding a v that moves by 0.1 % a step then has a variance of step size x change
+// (with any other factor every code would be rounded anew each step, with step size^2 / 6, 30 times as much, and to nearest it
+// would hardly ever move).  All scalings are exact: the only rounding of a state is that of its code.
+#include <cmath>
+#include <initializer_list>
+
+#include "rows.cuh"
+
+namespace s3r {
+
+constexpr int kAdamBlock = 256, kAdamThreads = 256, kAdamMax = 320;
+constexpr int kAdamPerWarp = 256, kAdamPerCta = kAdamPerWarp * kAdamThreads / 32;
+
+struct AdamScalars {
+  float factor;        // of the gradients
+  float decay;         // 1 - lr * weight_decay
+  float step_size;     // lr / (1 - beta1^t)
+  float inv_root;      // 1 / sqrt(1 - beta2^t)
+  uint32_t t;
+  uint32_t skip;
+};
+
+struct AdamTensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  uint8_t *me, *ve;
+  int64_t n;
+  int64_t first;       // CTA
+  uint32_t flags;      // types (2 bits each), vectors, 8-bit states, index << 8
+};
+struct AdamParams {
+  AdamTensor t[kAdamMax];
+  int n;
+  float b1, c1, b2, c2, eps;
+  int64_t seed;
+  const AdamScalars* scalars;
+};
+constexpr uint32_t kAdamVector = 16, kAdamEight = 32;
+
+struct BeginParams {
+  int64_t* step;
+  const float* lr;
+  double lr_host, log_b1, log_b2, weight_decay, max_norm;
+  const float* norm;
+  AdamScalars* out;
+};
+
+// what all elements share; one thread
+__global__ void adamw_begin_kernel(const __grid_constant__ BeginParams p) {
+  griddep_wait();
+  griddep_launch();
+  AdamScalars s = {};
+  const float norm = p.norm ? *p.norm : 0.f;
+  s.skip = !(fabsf(norm) <= 3.4028235e38f);
+  const int64_t t = *p.step + 1;
+  if (!s.skip) *p.step = t;
+  s.factor = 1.f;
+  if (p.norm && p.max_norm > 0) s.factor = fminf(__fdiv_rn(static_cast<float>(p.max_norm), __fadd_rn(norm, 1e-6f)), 1.f);
+  const double lr = p.lr ? static_cast<double>(*p.lr) : p.lr_host;
+  s.decay = static_cast<float>(1.0 - lr * p.weight_decay);
+  // 1 - b^t = -expm1(t log b): exact to fp32 where b^t is close to 1
+  s.step_size = static_cast<float>(lr) / -expm1f(static_cast<float>(t * p.log_b1));
+  s.inv_root = 1.f / sqrtf(-expm1f(static_cast<float>(t * p.log_b2)));
+  s.t = static_cast<uint32_t>(t);
+  *p.out = s;
+}
+
+// Philox 2x32 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3), seven rounds
+__device__ __forceinline__ uint2 philox(uint32_t a, uint32_t c, uint32_t key) {
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    const uint64_t m = static_cast<uint64_t>(a) * 0xD256D193u;
+    a = static_cast<uint32_t>(m >> 32) ^ key ^ c;
+    c = static_cast<uint32_t>(m);
+    key += 0x9E3779B9u;
+  }
+  return make_uint2(a, c);
+}
+
+// The exponent of a block whose largest magnitude is `big`: 1.875 x 2^(e - 127) is the smallest such bound of it.  255: not finite, or
+// beyond 2^100.  Below 2^-100 the exponent stays.
+__device__ __forceinline__ uint32_t block_exponent(float big) {
+  const uint32_t bits = __float_as_uint(big);
+  const uint32_t e = bits >= 0x7f800000u ? 255u : (bits + 0xFFFFFu) >> 23;
+  return e > 227u ? 255u : max(e, 27u);
+}
+__device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
+// Codes: the bits of |x| scaled so that the smallest exponent field of the code is fp32's own: the code is the top of the word,
+// rounded by what `low` adds below its last bit (0x7FFFF and the last bit: to nearest even).
+template <int EXPONENT_BITS>
+__device__ __forceinline__ uint32_t code_of(float magnitude, float up, uint32_t low, bool nearest) {
+  constexpr float kDown = EXPONENT_BITS == 4 ? 1.92592994438723585e-34f : 1.26217744835361889e-29f;        // 2^-112, 2^-96
+  const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(magnitude, up), kDown));
+  const uint32_t c = (bits + (nearest ? 0x7FFFFu + (bits >> 20 & 1u) : low)) >> 20;
+  return min(c, (8u << EXPONENT_BITS) - 1u);
+}
+template <int EXPONENT_BITS>
+__device__ __forceinline__ float value_of(uint32_t code, float unit) {
+  constexpr float kUp = EXPONENT_BITS == 4 ? 5.19229685853482763e33f : 7.92281625142643376e28f;            // 2^112, 2^96
+  return __fmul_rn(__fmul_rn(__uint_as_float(code << 20), kUp), unit);
+}
+__device__ __forceinline__ float unit_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fffffffu) : power_of(e); }
+
+template <int W>
+__device__ __forceinline__ void load_some(float (&f)[8], const void* p, int type, int64_t at, int64_t n) {
+  if constexpr (W == 8) {
+    load_vector<8>(f, p, type, at);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = at + k < n ? load_one(p, type, at + k) : 0.f;
+  }
+}
+template <int W>
+__device__ __forceinline__ void store_some(const float (&f)[8], void* p, int type, int64_t at, int64_t n) {
+  if constexpr (W == 8) {
+    Raw<8> r;
+    pack<8>(r, f, type);
+    store_raw<8>(r, p, type, at);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (at + k < n) {
+        const float one[1] = {f[k]};
+        Raw<1> r;
+        pack<1>(r, one, type);
+        store_raw<1>(r, p, type, at + k);
+      }
+  }
+}
+template <int W>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int64_t at, int64_t n) {
+  if constexpr (W == 8) return *reinterpret_cast<const uint2*>(p + at);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (at + k < n) w[k / 4] |= static_cast<uint32_t>(p[at + k]) << (8 * (k & 3));
+  return make_uint2(w[0], w[1]);
+}
+template <int W>
+__device__ __forceinline__ void store_codes(uint2 c, uint8_t* p, int64_t at, int64_t n) {
+  if constexpr (W == 8) {
+    *reinterpret_cast<uint2*>(p + at) = c;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (at + k < n) p[at + k] = static_cast<uint8_t>((k < 4 ? c.x : c.y) >> (8 * (k & 3)));
+  }
+}
+
+// Eight elements per lane: a block.  W = 8: all of them exist and every array begins at a multiple of its vectors.
+template <int W>
+__device__ __forceinline__ void adamw_block(const AdamParams& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
+  const int64_t at = block * kAdamBlock + lane * 8;
+  const int p_type = x.flags & 3, g_type = x.flags >> 2 & 3;
+  const bool eight = x.flags & kAdamEight, nearest = p.seed < 0;
+  float g[8], w[8], m[8], v[8];
+  load_some<W>(g, x.g, g_type, at, x.n);
+  load_some<W>(w, x.p, p_type, at, x.n);
+  if (eight) {
+    const uint2 mc = load_codes<W>(static_cast<const uint8_t*>(x.m), at, x.n), vc = load_codes<W>(static_cast<const uint8_t*>(x.v), at, x.n);
+    const float mu = unit_of(x.me[block]), vu = unit_of(x.ve[block]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t a = (k < 4 ? mc.x : mc.y) >> (8 * (k & 3)) & 255u, b = (k < 4 ? vc.x : vc.y) >> (8 * (k & 3)) & 255u;
+      m[k] = __uint_as_float(__float_as_uint(value_of<4>(a & 127u, mu)) ^ (a & 128u) << 24);
+      v[k] = value_of<5>(b, vu);
+    }
+  } else {
+    load_some<W>(m, x.m, S3R_F32, at, x.n);
+    load_some<W>(v, x.v, S3R_F32, at, x.n);
+  }
+  // Every product and sum is rounded by itself, as in separate operations: codes do not depend on which of them the compiler
+  // would have fused.
+  float m_big = 0.f, v_big = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float gk = __fmul_rn(g[k], s.factor);
+    m[k] = __fadd_rn(__fmul_rn(m[k], p.b1), __fmul_rn(gk, p.c1));
+    v[k] = __fadd_rn(__fmul_rn(v[k], p.b2), __fmul_rn(__fmul_rn(gk, gk), p.c2));
+    w[k] = __fsub_rn(__fmul_rn(w[k], s.decay), __fmul_rn(s.step_size, __fdividef(m[k], __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), s.inv_root), p.eps))));
+    m_big = max_nan(m_big, fabsf(m[k]));
+    v_big = max_nan(v_big, v[k]);
+  }
+  uint32_t low[8];
+  if (!nearest && (eight || p_type == S3R_BF16)) {
+    const uint32_t key = static_cast<uint32_t>(p.seed) + (x.flags >> 8) * 0x85EBCA6Bu;
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const uint2 r = philox(static_cast<uint32_t>((at + k) >> 1), s.t, key);
+      low[k] = r.x;
+      low[k + 1] = r.y;
+    }
+    // 10 bits of a bf16 parameter's 16; fp16's values below 2^-14 have fewer, so it is rounded to nearest
+    if (p_type == S3R_BF16)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (fabsf(w[k]) < 3.3e38f) w[k] = __uint_as_float((__float_as_uint(w[k]) + (low[k] >> 22) * 64u + 32u) & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) low[k] = 0;
+  }
+  store_some<W>(w, x.p, p_type, at, x.n);
+  if (!eight) {
+    store_some<W>(m, x.m, S3R_F32, at, x.n);
+    store_some<W>(v, x.v, S3R_F32, at, x.n);
+    return;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    m_big = max_nan(m_big, __shfl_xor_sync(0xffffffffu, m_big, o));
+    v_big = max_nan(v_big, __shfl_xor_sync(0xffffffffu, v_big, o));
+  }
+  const uint32_t me = block_exponent(m_big), ve = block_exponent(v_big);
+  const float m_up = me == 255u ? 0.f : power_of(254u - me), v_up = ve == 255u ? 0.f : power_of(254u - ve);
+  uint32_t mc[2] = {0, 0}, vc[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    // 8 random bits of the 20 that a code of m drops, 14 of v's: v moves less in a step.  A v that is not zero keeps a code that
+    // is not: a denominator never becomes eps alone by rounding.
+    const uint32_t a = code_of<4>(fabsf(m[k]), m_up, (low[k] & 0xFFu) << 12 | 0x800u, nearest) | (m[k] < 0.f ? 128u : 0u);
+    const uint32_t b = max(code_of<5>(v[k], v_up, (low[k] >> 8 & 0x3FFFu) << 6 | 0x20u, nearest), v[k] > 0.f ? 1u : 0u);
+    mc[k / 4] |= a << (8 * (k & 3));
+    vc[k / 4] |= b << (8 * (k & 3));
+  }
+  store_codes<W>(me == 255u ? make_uint2(0, 0) : make_uint2(mc[0], mc[1]), static_cast<uint8_t*>(x.m), at, x.n);
+  store_codes<W>(ve == 255u ? make_uint2(0, 0) : make_uint2(vc[0], vc[1]), static_cast<uint8_t*>(x.v), at, x.n);
+  if (lane == 0) {
+    x.me[block] = static_cast<uint8_t>(me);
+    x.ve[block] = static_cast<uint8_t>(ve);
+  }
+}
+
+__device__ __forceinline__ int tensor_of(const AdamTensor* t, int n, int64_t cta) {
+  int lo = 0, hi = n - 1;                    // the last tensor whose first CTA is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t[mid].first <= cta) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamParams p) {
+  const int i = tensor_of(p.t, p.n, blockIdx.x);
+  const AdamTensor& x = p.t[i];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t block = (blockIdx.x - x.first) * (kAdamThreads / 32) + warp;
+  griddep_wait();
+  griddep_launch();
+  const AdamScalars s = *p.scalars;
+  if (s.skip || block * kAdamBlock >= x.n) return;
+  if ((x.flags & kAdamVector) && (block + 1) * kAdamBlock <= x.n) adamw_block<8>(p, x, s, block, lane);
+  else adamw_block<1>(p, x, s, block, lane);
+}
+
+// ---- the norm of the gradients: squares in 64 bits, where every one of them is exact ------------------------------------
+constexpr int kNormThreads = 256, kNormPerCta = 16384;
+
+struct NormTensor {
+  const void* g;
+  int64_t n;
+  int64_t first;
+  uint32_t flags;
+};
+struct GradNormParams {
+  NormTensor t[kAdamMax];
+  int n;
+  double* partial;
+};
+
+__global__ void __launch_bounds__(kNormThreads) grad_norm_kernel(const __grid_constant__ GradNormParams p) {
+  __shared__ double red[kNormThreads / 32];
+  int lo = 0, hi = p.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.t[mid].first <= blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const NormTensor& x = p.t[lo];
+  griddep_wait();
+  griddep_launch();
+  const int64_t from = (blockIdx.x - x.first) * kNormPerCta, to = min(x.n, from + kNormPerCta);
+  const int type = x.flags & 3;
+  double s[4] = {0., 0., 0., 0.};
+  int64_t at = from + threadIdx.x * 8;
+  if (x.flags & kAdamVector) {
+#pragma unroll 2
+    for (; at + 8 <= to; at += kNormThreads * 8) {
+      float f[8];
+      load_vector<8>(f, x.g, type, at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const double d = f[k];
+        s[k & 3] = fma(d, d, s[k & 3]);
+      }
+    }
+  }
+  for (; at < to; at += kNormThreads * 8)
+    for (int64_t k = at; k < min(at + 8, to); ++k) {
+      const double d = load_one(x.g, type, k);
+      s[0] = fma(d, d, s[0]);
+    }
+  double sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kNormThreads / 32; ++w) sum += red[w];
+    p.partial[blockIdx.x] = sum;
+  }
+}
+
+__global__ void __launch_bounds__(1024) grad_norm_end_kernel(const double* partial, int64_t n, float* norm) {
+  __shared__ double red[32];
+  griddep_wait();
+  griddep_launch();
+  double s = 0.;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += partial[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = red[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
+  }
+}
+
+// ---- what 8-bit states stand for -----------------------------------------------------------------------------------------
+struct StateTensor {
+  const uint8_t *m, *v, *me, *ve;
+  float *m_out, *v_out;
+  int64_t n, first;
+  uint32_t flags;
+};
+struct StateParams {
+  StateTensor t[kAdamMax];
+  int n;
+};
+__global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_constant__ StateParams p) {
+  int lo = 0, hi = p.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.t[mid].first <= blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const StateTensor& x = p.t[lo];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t block = (blockIdx.x - x.first) * (kAdamThreads / 32) + warp, at = block * kAdamBlock + lane * 8;
+  griddep_wait();
+  griddep_launch();
+  if (at >= x.n) return;
+  const bool whole = (x.flags & kAdamVector) && at + 8 <= x.n;
+  const uint2 mc = whole ? load_codes<8>(x.m, at, x.n) : load_codes<1>(x.m, at, x.n), vc = whole ? load_codes<8>(x.v, at, x.n) : load_codes<1>(x.v, at, x.n);
+  const float mu = unit_of(x.me[block]), vu = unit_of(x.ve[block]);
+  float m[8], v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t a = (k < 4 ? mc.x : mc.y) >> (8 * (k & 3)) & 255u, b = (k < 4 ? vc.x : vc.y) >> (8 * (k & 3)) & 255u;
+    m[k] = __uint_as_float(__float_as_uint(value_of<4>(a & 127u, mu)) ^ (a & 128u) << 24);
+    v[k] = value_of<5>(b, vu);
+  }
+  if (whole) {
+    store_some<8>(m, x.m_out, S3R_F32, at, x.n);
+    store_some<8>(v, x.v_out, S3R_F32, at, x.n);
+  } else {
+    store_some<1>(m, x.m_out, S3R_F32, at, x.n);
+    store_some<1>(v, x.v_out, S3R_F32, at, x.n);
+  }
+}
+
+static bool at_16(std::initializer_list<const void*> p) {
+  uintptr_t all = 0;
+  for (const void* q : p) all |= reinterpret_cast<uintptr_t>(q);
+  return (all & 15) == 0;
+}
+
+}  // namespace s3r
+
+using namespace s3r;
+
+extern "C" size_t s3r_grad_norm_workspace_bytes(int n, const int64_t* counts) {
+  size_t parts = 0;
+  for (int i = 0; counts && i < n; ++i) parts += counts[i] > 0 ? (counts[i] + kNormPerCta - 1) / kNormPerCta : 0;
+  return (parts + 1) * sizeof(double);
+}
+
+extern "C" int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, const int* types, float* norm, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  S3R_REQUIRE(n >= 0, S3R_ERR_SHAPE, "s3r_grad_norm: %d tensors", n);
+  S3R_REQUIRE(norm && workspace && (n == 0 || (tensors && counts && types)), S3R_ERR_NULL, "s3r_grad_norm: NULL pointer");
+  S3R_REQUIRE(workspace_bytes >= s3r_grad_norm_workspace_bytes(n, counts) && reinterpret_cast<uintptr_t>(workspace) % 8 == 0, S3R_ERR_TOO_LARGE,
+              "s3r_grad_norm: workspace of %zu bytes is smaller than the %zu needed", workspace_bytes, s3r_grad_norm_workspace_bytes(n, counts));
+  for (int i = 0; i < n; ++i) {
+    S3R_REQUIRE(counts[i] >= 0, S3R_ERR_SHAPE, "s3r_grad_norm: negative count");
+    S3R_REQUIRE(counts[i] == 0 || tensors[i], S3R_ERR_NULL, "s3r_grad_norm: NULL pointer");
+    S3R_REQUIRE(known_type(types[i]), S3R_ERR_UNSUPPORTED, "s3r_grad_norm: types are fp32, bf16 and fp16");
+    S3R_REQUIRE(reinterpret_cast<uintptr_t>(tensors[i]) % type_bytes(types[i]) == 0, S3R_ERR_ALIGNMENT, "s3r_grad_norm: elements must be aligned");
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GradNormParams p;
+  p.partial = static_cast<double*>(workspace);
+  p.n = 0;
+  int64_t ctas = 0, all = 0;
+  for (int i = 0; i <= n; ++i) {
+    if (p.n && (i == n || p.n == kAdamMax)) {
+      if (const int rc = launch(grad_norm_kernel, static_cast<unsigned>(ctas), kNormThreads, 0, st, p)) return rc;
+      p.partial += ctas;
+      all += ctas;
+      p.n = 0;
+      ctas = 0;
+    }
+    if (i == n || counts[i] == 0) continue;
+    p.t[p.n++] = {tensors[i], counts[i], ctas, static_cast<uint32_t>(types[i]) | (at_16({tensors[i]}) ? kAdamVector : 0u)};
+    ctas += (counts[i] + kNormPerCta - 1) / kNormPerCta;
+    S3R_REQUIRE(ctas < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_grad_norm: grid too large");
+  }
+  return launch(grad_norm_end_kernel, 1u, 1024, 0, st, static_cast<const double*>(workspace), all, norm);
+}
+
+extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
+  S3R_REQUIRE(args, S3R_ERR_NULL, "s3r_adamw_step: NULL pointer");
+  const s3r_adamw& a = *args;
+  S3R_REQUIRE(a.n >= 0, S3R_ERR_SHAPE, "s3r_adamw_step: %d tensors", a.n);
+  S3R_REQUIRE(a.step && a.workspace && (a.n == 0 || (a.params && a.grads && a.m && a.v && a.counts && a.param_types && a.grad_types)), S3R_ERR_NULL,
+              "s3r_adamw_step: NULL pointer");
+  S3R_REQUIRE(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1 && a.eps >= 0, S3R_ERR_UNSUPPORTED, "s3r_adamw_step: betas are in [0, 1), eps is not negative");
+  S3R_REQUIRE(reinterpret_cast<uintptr_t>(a.step) % 8 == 0 && reinterpret_cast<uintptr_t>(a.workspace) % 8 == 0, S3R_ERR_ALIGNMENT, "s3r_adamw_step: elements must be aligned");
+  for (int i = 0; i < a.n; ++i) {
+    S3R_REQUIRE(a.counts[i] >= 0, S3R_ERR_SHAPE, "s3r_adamw_step: negative count");
+    if (a.counts[i] == 0) continue;
+    S3R_REQUIRE(a.params[i] && a.grads[i] && a.m[i] && a.v[i], S3R_ERR_NULL, "s3r_adamw_step: NULL pointer");
+    S3R_REQUIRE(known_type(a.param_types[i]) && known_type(a.grad_types[i]), S3R_ERR_UNSUPPORTED, "s3r_adamw_step: types are fp32, bf16 and fp16");
+    const bool eight = a.m_exponents && a.m_exponents[i];
+    S3R_REQUIRE(eight == (a.v_exponents && a.v_exponents[i]), S3R_ERR_NULL, "s3r_adamw_step: exponents of m and v come together");
+    S3R_REQUIRE(reinterpret_cast<uintptr_t>(a.params[i]) % type_bytes(a.param_types[i]) == 0 && reinterpret_cast<uintptr_t>(a.grads[i]) % type_bytes(a.grad_types[i]) == 0 &&
+                    (eight || (reinterpret_cast<uintptr_t>(a.m[i]) | reinterpret_cast<uintptr_t>(a.v[i])) % 4 == 0), S3R_ERR_ALIGNMENT, "s3r_adamw_step: elements must be aligned");
+    S3R_REQUIRE(a.counts[i] < (1ll << 33), S3R_ERR_TOO_LARGE, "s3r_adamw_step: more than 2^33 elements in a tensor");
+    S3R_REQUIRE(i < (1 << 24), S3R_ERR_TOO_LARGE, "s3r_adamw_step: too many tensors");
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  AdamScalars* scalars = static_cast<AdamScalars*>(a.workspace);
+  // log 0 = -inf: 1 - 0^t = 1
+  const BeginParams b = {a.step, a.lr, a.lr_host, log(a.beta1), log(a.beta2), a.weight_decay, a.max_norm, a.norm, scalars};
+  if (const int rc = launch(adamw_begin_kernel, 1u, 1, 0, st, b)) return rc;
+  AdamParams p;
+  p.b1 = static_cast<float>(a.beta1);
+  p.c1 = static_cast<float>(1.0 - a.beta1);
+  p.b2 = static_cast<float>(a.beta2);
+  p.c2 = static_cast<float>(1.0 - a.beta2);
+  p.eps = static_cast<float>(a.eps);
+  p.seed = a.seed;
+  p.scalars = scalars;
+  p.n = 0;
+  int64_t ctas = 0;
+  for (int i = 0; i <= a.n; ++i) {
+    if (p.n && (i == a.n || p.n == kAdamMax)) {
+      if (const int rc = launch(adamw_kernel, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p)) return rc;
+      p.n = 0;
+      ctas = 0;
+    }
+    if (i == a.n || a.counts[i] == 0) continue;
+    uint8_t *me = a.m_exponents ? a.m_exponents[i] : nullptr, *ve = a.v_exponents ? a.v_exponents[i] : nullptr;
+    const uint32_t flags = static_cast<uint32_t>(a.param_types[i]) | static_cast<uint32_t>(a.grad_types[i]) << 2 |
+                           (at_16({a.params[i], a.grads[i], a.m[i], a.v[i]}) ? kAdamVector : 0u) | (me ? kAdamEight : 0u) | static_cast<uint32_t>(i) << 8;
+    p.t[p.n++] = {a.params[i], a.grads[i], a.m[i], a.v[i], me, ve, a.counts[i], ctas, flags};
+    ctas += (a.counts[i] + kAdamPerCta - 1) / kAdamPerCta;
+    S3R_REQUIRE(ctas < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_adamw_step: grid too large");
+  }
+  return 0;
+}
+
+extern "C" int s3r_adamw_state(int n, const void* const* m, const void* const* v, const uint8_t* const* m_exponents,
+                               const uint8_t* const* v_exponents, float* const* m_out, float* const* v_out, const int64_t* counts, void* stream) {
+  S3R_REQUIRE(n >= 0, S3R_ERR_SHAPE, "s3r_adamw_state: %d tensors", n);
+  S3R_REQUIRE(n == 0 || (m && v && m_exponents && v_exponents && m_out && v_out && counts), S3R_ERR_NULL, "s3r_adamw_state: NULL pointer");
+  for (int i = 0; i < n; ++i) {
+    S3R_REQUIRE(counts[i] >= 0 && counts[i] < (1ll << 33), S3R_ERR_SHAPE, "s3r_adamw_state: %lld elements", (long long)counts[i]);
+    S3R_REQUIRE(counts[i] == 0 || (m[i] && v[i] && m_exponents[i] && v_exponents[i] && m_out[i] && v_out[i]), S3R_ERR_NULL, "s3r_adamw_state: NULL pointer");
+    S3R_REQUIRE((reinterpret_cast<uintptr_t>(m_out[i]) | reinterpret_cast<uintptr_t>(v_out[i])) % 4 == 0, S3R_ERR_ALIGNMENT, "s3r_adamw_state: elements must be aligned");
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  StateParams p;
+  p.n = 0;
+  int64_t ctas = 0;
+  for (int i = 0; i <= n; ++i) {
+    if (p.n && (i == n || p.n == kAdamMax)) {
+      if (const int rc = launch(adamw_state_kernel, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p)) return rc;
+      p.n = 0;
+      ctas = 0;
+    }
+    if (i == n || counts[i] == 0) continue;
+    p.t[p.n++] = {static_cast<const uint8_t*>(m[i]), static_cast<const uint8_t*>(v[i]), m_exponents[i], v_exponents[i], m_out[i], v_out[i], counts[i], ctas,
+                  at_16({m[i], v[i], m_out[i], v_out[i]}) ? kAdamVector : 0u};
+    ctas += (counts[i] + kAdamPerCta - 1) / kAdamPerCta;
+    S3R_REQUIRE(ctas < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_adamw_state: grid too large");
+  }
+  return 0;
+}

@@ -9,65 +9,9 @@
 //     torch.compile are registered from Python (ops.py).
 //   differentiable operators (pool_tokens, flash_attn_topk, ..., sparse_attention): composite functions that
 //     call the base operators through the dispatcher, inside a C++ autograd node when a gradient is needed.
-#include <ATen/ATen.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/cuda/CUDAEvent.h>
-#include <ATen/cuda/CachingHostAllocator.h>
-#include <c10/cuda/CUDAException.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/library.h>
-
-#include <cmath>
-#include <tuple>
-#include <vector>
-
-#include "../../../include/speed3r_b200.h"
+#include "helpers.h"
 
 namespace {
-
-using at::Tensor;
-using c10::optional;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-void need(const Tensor& t, const char* name, at::ScalarType dtype = at::kBFloat16, bool contiguous = true) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor: the speed3r_b200 kernels have no CPU path");
-  TORCH_CHECK(t.scalar_type() == dtype, name, " must be ", dtype, ", got ", t.scalar_type());
-  TORCH_CHECK(!contiguous || t.is_contiguous(), name, " must be contiguous");
-}
-
-// Sizes that are divided by: a division by zero ends the process in C++, where Python raised.
-template <typename... N>
-void need_positive(const char* what, N... n) {
-  TORCH_CHECK(((n > 0) && ...), what, ": block, window and stride must be positive");
-}
-
-void check(int rc, const char* what) {
-  if (rc == 0) return;
-  char msg[512];
-  s3r_last_error(msg, sizeof(msg));
-  TORCH_CHECK(false, what, " failed with code ", rc, ": ", msg);
-}
-
-void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
-const int32_t* i32(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
-int32_t* i32m(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
-float* f32(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
-Tensor fresh(at::IntArrayRef shape, const Tensor& like, at::ScalarType dtype) {
-  return at::empty(shape, like.options().dtype(dtype));
-}
-// contiguous, whatever the strides of `t` (at::empty_like would keep a permuted layout)
-Tensor fresh_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
-// The same values at a multiple of 16 bytes: a contiguous view may begin anywhere in its storage (a slice, a flattened
-// parameter buffer), and the kernels load vectors.
-Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
-optional<Tensor> aligned(const optional<Tensor>& t) { return t.has_value() ? optional<Tensor>(aligned(*t)) : t; }
-Tensor none(const Tensor& like) { return at::empty({0}, like.options()); }
 
 // ------------------------------------------------------------------------------------------------
 // base operators
@@ -435,10 +379,6 @@ std::tuple<Tensor, Tensor> prologue_bwd(const Tensor& qkv, int64_t heads, int64_
 // the base operators as the differentiable ones call them: through the dispatcher, so that fake tensors,
 // functionalisation and dispatch modes see them
 // ------------------------------------------------------------------------------------------------
-#define S3R_DISPATCHED(fn)                                                                              \
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("speed3r_b200::" #fn, "").typed<decltype(fn)>(); \
-  return op.call
-
 Tensor call_pool_fwd(const Tensor& x, int64_t kernel, int64_t stride) { S3R_DISPATCHED(pool_fwd)(x, kernel, stride); }
 Tensor call_pool_bwd(const Tensor& g, int64_t T, int64_t kernel, int64_t stride) { S3R_DISPATCHED(pool_bwd)(g, T, kernel, stride); }
 std::tuple<Tensor, Tensor, Tensor> call_cmp_topk(const Tensor& q, const Tensor& k, const Tensor& v, int64_t topk, double scale) {
@@ -498,44 +438,6 @@ std::tuple<Tensor, Tensor> call_prologue_bwd(const Tensor& qkv, int64_t heads, i
 // ------------------------------------------------------------------------------------------------
 // differentiable operators
 // ------------------------------------------------------------------------------------------------
-// Forward-mode derivatives are refused, in every operator and whether a gradient is wanted or not: past the nodes, the base
-// operators would drop a tangent without a word.
-bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
-bool has_tangent(const optional<Tensor>& t) { return t.has_value() && has_tangent(*t); }
-template <typename... T>
-void no_tangents(const T&... t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "speed3r_b200: forward mode AD is not implemented for the operators of this package");
-}
-template <typename... T>
-bool wants_grad(const T&... t) {
-  no_tangents(t...);
-  return at::GradMode::is_enabled() && (t.requires_grad() || ...);
-}
-
-// A backward of a node.  It runs without recording; where its result is to be differentiated again (create_graph), the result
-// raises when that is tried: no operator here has a second derivative, and without this one would be missing silently.
-template <typename F>
-variable_list once(const variable_list& incoming, F&& backward) {
-  const bool again = at::GradMode::is_enabled();
-  variable_list g;
-  {
-    at::NoGradGuard no_grad;
-    g = backward();
-  }
-  if (!again) return g;
-  // the error stands between the result and all it depends on: the node's own inputs and the incoming gradients
-  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(incoming);
-  if (const auto node = torch::autograd::get_current_node()) edges.insert(edges.end(), node->next_edges().begin(), node->next_edges().end());
-  const auto error = std::make_shared<torch::autograd::Error>("the backward of speed3r_b200 operators cannot be differentiated again",
-                                                              std::move(edges));
-  for (Tensor& t : g)
-    if (t.defined()) {
-      t = t.detach();
-      torch::autograd::set_history(t, error);
-    }
-  return g;
-}
-
 struct PoolNode : torch::autograd::Function<PoolNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t kernel, int64_t stride) {
     ctx->saved_data["T"] = x.size(2);

@@ -7,7 +7,8 @@ Public functions mirror the reference's op signatures:
 * ``topk_blocksparse_attention(q, k, v, topk_idx, block_size, softmax_scale=None)`` -> ``o``
   (pi3/models/sparse_attn/topk_blocksparse_attention.py:1093-1121)
 
-plus the pieces the reference leaves to eager PyTorch (sparse_attention.py:97-102, 127-136):
+the rest of a block around them (``residual_norm``), its projections in 8 bits (``quantize_tokens``, ``int8_linear``) and the step
+that ends a training iteration (``grad_norm``, ``adamw_step``), plus the pieces the reference leaves to eager PyTorch (sparse_attention.py:97-102, 127-136):
 
 * ``pool_tokens(x, kernel, stride)``: mean pooling along the sequence
 * ``sel_attn_merge(q, k, v, idx, gate, o_c, block_size)``: selection attention with the gated
@@ -103,6 +104,42 @@ def _register_fakes() -> None:
         B, H, Tq, d = o_s.shape
         return (o_s.new_empty(o_s.shape), o_s.new_empty(B, H, Tq, 2, dtype=torch.float32), o_c.new_empty(o_c.shape),
                 o_s.new_empty(B, H, Tq, dtype=torch.float32))
+
+    @fake("speed3r_b200::residual_norm_fwd")
+    def _(x, y, weight, bias, scale, gate, post_weight, post_bias, norm, post, kind, eps, post_eps, h_type, keep):
+        return (x.new_empty(x.shape if y is not None else (0,)), x.new_empty(x.shape if norm else (0,), dtype=h_type),
+                x.new_empty(4 if keep else 0, x.shape[0] * x.shape[1], dtype=torch.float32))
+
+    @fake("speed3r_b200::residual_norm_bwd")
+    def _(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, post, kind, want, param_type):
+        if dh is None:
+            want &= ~12
+        of = lambda bit: r.new_empty(r.shape[2] if want & bit else 0, dtype=param_type)
+        return [r.new_empty(r.shape), r.new_empty(r.shape, dtype=y.dtype) if want & 2 else r.new_empty(0), of(4), of(8), of(16),
+                gate.new_empty(gate.shape) if want & 32 else r.new_empty(0), of(64), of(128)]
+
+    @fake("speed3r_b200::residual_norm_int8")
+    def _(x, y, weight, bias, scale, gate, post_weight, post_bias, post, kind, eps, post_eps):
+        B, T, C = x.shape
+        return (x.new_empty(x.shape if y is not None else (0,)), x.new_empty(B, T, -(-C // 16) * 16, dtype=torch.int8).narrow(2, 0, C),
+                x.new_empty(B, T, dtype=torch.float32))
+
+    @fake("speed3r_b200::quantize_tokens")
+    def _(x):
+        K = x.shape[-1]
+        return (x.new_empty(x.numel() // K, -(-K // 16) * 16, dtype=torch.int8).narrow(1, 0, K).view(x.shape),
+                x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+    @fake("speed3r_b200::int8_linear")
+    def _(q, q_scale, weight, weight_scale, bias, out_type):
+        return q.new_empty(*q.shape[:-1], weight.shape[0], dtype=out_type)
+
+    @fake("speed3r_b200::grad_norm")
+    def _(tensors):
+        return tensors[0].new_empty((), dtype=torch.float32)
+
+    fake("speed3r_b200::adamw_step", lambda *a: None)
+    fake("speed3r_b200::adamw_state", lambda *a: None)
 
 
 def _ops():
@@ -246,3 +283,115 @@ def sel_attn_merge_chunked(q, k_chunks, v_chunks, topk_idx, gate, o_c, block_siz
     with torch.no_grad():
         return _sel_fwd(q, k_chunks, v_chunks, topk_idx, gate, o_c, int(block_size), _scale(softmax_scale, q),
                         False, False, int(k_chunks.shape[0]))[2]
+
+
+# ------------------------------------------------------------------------------------------------
+# the rest of a block: residual, LayerScale, gate and norms; 8-bit products; the optimiser's step
+# ------------------------------------------------------------------------------------------------
+_KINDS = {"layer": 0, "rms": 1}
+NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _norm_args(norm, post_norm, kind):
+    if kind not in _KINDS:
+        raise RuntimeError(f"residual_norm: kind must be 'layer' or 'rms', got {kind!r}")
+    w, b, eps = norm if norm is not None else (None, None, 0.0)
+    pw, pb, post_eps = post_norm if post_norm is not None else (None, None, 0.0)
+    return w, b, float(eps), pw, pb, float(post_eps)
+
+
+def residual_norm(x: Tensor, y: Optional[Tensor] = None, norm=None, scale: Optional[Tensor] = None, gate: Optional[Tensor] = None,
+                  post_norm=None, kind: str = "layer", out_dtype: Optional[torch.dtype] = None):
+    """What stands between two sub-layers of a block (pi3/models/layers/block.py:310-335, LayerScale and residual, then the
+    next norm), in one pass and with gradients::
+
+        u = y, or post_norm(y)
+        r = x + u * scale * gate            (in x's type)
+        h = norm(r)                         (in ``out_dtype``, by default x's type)
+
+    ``x``, ``y`` ``[.., T, C]`` fp32, bf16 or fp16, each of its own type, C up to 8192.  ``norm`` and ``post_norm`` are
+    ``(weight, bias, eps)``, weight and bias ``[C]`` or None; ``kind`` says whether they are LayerNorms (``"layer"``) or divide by
+    the root of the mean square (``"rms"``).  ``scale [C]`` is the LayerScale, ``gate`` a factor per token ``[.., T, 1]``, per
+    sample ``[.., 1, 1]`` (stochastic depth) or per sample and channel ``[.., 1, C]`` (modulation).  Returns ``(r, h)``: ``r`` is
+    ``x`` itself where ``y`` is None, ``h`` is None where ``norm`` is None.  The norm is that of ``r`` as it is stored."""
+    w, b, eps, pw, pb, post_eps = _norm_args(norm, post_norm, kind)
+    h_type = x.dtype if out_dtype is None else out_dtype
+    if h_type not in NORM_TYPES:
+        raise RuntimeError(f"residual_norm: out_dtype must be fp32, bf16 or fp16, got {h_type}")
+    r, h = _ops().residual_norm.default(x, y, w, b, scale, gate, pw, pb, norm is not None, post_norm is not None, _KINDS[kind], eps,
+                                        post_eps, h_type)
+    return x if y is None else r, None if norm is None else h
+
+
+def residual_norm_int8(x: Tensor, y: Optional[Tensor] = None, norm=None, scale: Optional[Tensor] = None,
+                       gate: Optional[Tensor] = None, post_norm=None, kind: str = "layer"):
+    """``residual_norm`` without gradients whose ``h`` leaves as 8-bit tokens: ``(r, q, q_scale)`` as ``quantize_tokens`` makes
+    them of ``h``, without ``h`` being written."""
+    if norm is None:
+        raise RuntimeError("residual_norm_int8 needs a norm")
+    w, b, eps, pw, pb, post_eps = _norm_args(norm, post_norm, kind)
+    r, q, s = _ops().residual_norm_to_int8.default(x, y, w, b, scale, gate, pw, pb, post_norm is not None, _KINDS[kind], eps, post_eps)
+    return x if y is None else r, q, s
+
+
+def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """``x [.., K]`` fp32, bf16 or fp16 as 8-bit integers with a scale per token: ``q = round(x / q_scale)`` with
+    ``q_scale [..] = max|x| / 127``.  Rows of ``q`` lie a multiple of 16 bytes apart.  The rows of a weight ``[N, K]`` become
+    its output channels.  No gradients."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("quantize_tokens is forward-only: call it under torch.no_grad()")
+    return _ops().quantize_tokens.default(x)
+
+
+def int8_linear(q: Tensor, q_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None,
+                out_dtype: torch.dtype = _BF16) -> Tensor:
+    """``(q @ weight.T) * q_scale * weight_scale + bias`` for ``q [.., K]`` and ``weight [N, K]`` of 8-bit integers: exact sums in
+    32 bits, one fp32 scale per token and per output channel, fp32 ``bias [N]``, one rounding to ``out_dtype``.  No gradients."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q_scale, weight_scale, bias)):
+        raise RuntimeError("int8_linear is forward-only: call it under torch.no_grad()")
+    if out_dtype not in NORM_TYPES:
+        raise RuntimeError(f"int8_linear: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
+    return _ops().int8_linear.default(q, q_scale, weight, weight_scale, bias, out_dtype)
+
+
+@torch.no_grad()
+def grad_norm(tensors) -> Tensor:
+    """Euclidean norm of all elements of a list of tensors (one device; fp32, bf16, fp16), as a 0-dim fp32 tensor: squares summed
+    in 64 bits in a fixed order, without a synchronisation."""
+    return _ops().grad_norm.default(list(tensors))
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step: Tensor, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None, scales=None,
+               seed: Optional[int] = None) -> None:
+    """One AdamW step in place over lists of tensors of one device, in one pass::
+
+        g = grad * min(1, max_norm / (grad_norm + 1e-6))         (with max_norm)
+        m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+
+    ``step`` is a 0-dim int64 tensor on the device that becomes t; ``lr`` a number or a 0-dim fp32 tensor on the device.  Where
+    ``grad_norm`` is given and not finite, nothing changes.  States are fp32, or, where ``scales`` (a list, entries may be None) has a
+    uint8 ``[2, ceil(n / 256)]`` for a tensor, uint8 codes: see ``adamw_state``.  With ``seed`` (0 to 2^63 - 1) what is kept in fewer
+    bits than 32 - 8-bit states, bf16 parameters - is rounded stochastically, the same way for the same seed and step; without it to
+    nearest.  Parameters: fp32, bf16 or fp16, contiguous."""
+    if seed is not None and not 0 <= int(seed) < 1 << 63:
+        raise RuntimeError(f"adamw_step: seed {seed}")
+    if max_norm is not None and not max_norm > 0:
+        raise RuntimeError(f"adamw_step: max_norm {max_norm}")
+    if max_norm is not None and grad_norm is None:
+        raise RuntimeError("adamw_step: max_norm needs grad_norm")
+    on_device = isinstance(lr, Tensor)
+    _ops().adamw_step.default(list(params), list(grads), list(exp_avg), list(exp_avg_sq), step, [] if scales is None else list(scales),
+                              0.0 if on_device else float(lr), lr if on_device else None, float(betas[0]), float(betas[1]), float(eps),
+                              float(weight_decay), grad_norm, 0.0 if max_norm is None else float(max_norm), -1 if seed is None else int(seed))
+
+
+@torch.no_grad()
+def adamw_state(exp_avg, exp_avg_sq, scales, out=None):
+    """``(m, v)``, two lists of fp32 tensors: what 8-bit states stand for.  Blocks of 256 codes share a power of two; a code of ``m``
+    has a sign, 4 bits of exponent and 3 of mantissa, one of ``v`` 5 and 3.  ``out``: two lists to write into."""
+    m, v = out if out is not None else tuple([torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in exp_avg] for _ in range(2))
+    _ops().adamw_state.default(list(exp_avg), list(exp_avg_sq), list(scales), list(m), list(v))
+    return m, v

@@ -103,32 +103,35 @@ static int pick_quantize(const QuantParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// product on tcgen05: persistent CTAs; 128 x TN tiles, K in steps of 128 bytes through a ring of TMA copies, the sums of two
-// tiles in tensor memory so that one is written out while the next is summed.  One warp copies, one issues the products, four
-// take the sums, scale them and store through shared memory.
+// product on tcgen05: persistent CTAs, K in steps of 128 bytes through a ring of TMA copies, the sums of two tiles in tensor memory
+// so that one is written out while the next is summed.  One warp copies, one issues the products, eight take the sums (32 rows and
+// half of the columns each), scale them and store through shared memory.
+// CTAS = 2: a pair of CTAs multiplies 256 rows with TN columns; each holds 128 rows of a and half of b's rows, the products read both
+// halves.  A k-step then brings half as much of b into either CTA's shared memory, whose bandwidth bounds one CTA alone.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kI8Threads = 192, kI8Stage = 4096;       // a warp's piece of the output: 32 rows of 128 bytes
+constexpr int kI8Warps = 8, kI8Threads = 64 + 32 * kI8Warps, kI8Piece = 4096;       // a warp's piece of the output: 32 rows of 128 bytes
 
 struct I8Params {
   const float *a_scale, *b_scale, *bias;
   void* out;
   int64_t M;
-  int N, K, type;
+  int N, K;
   int m_tiles, n_tiles;
   uint32_t copy_out;             // rows of the output are a multiple of 16 bytes: TMA stores
   uint32_t* status;
 };
 
-template <int TN>
+template <int TN, int CTAS>
 struct I8Cfg {
-  static constexpr int kStages = TN == 256 ? 4 : 6;
-  static constexpr int kABytes = 128 * 128, kBBytes = TN * 128, kBytes = kABytes + kBBytes;
-  static constexpr int kOut = kStages * kBytes, kColumns = kOut + 4 * 2 * kI8Stage;
-  static constexpr int kSmem = kColumns + 4 * 32 * 8 + 1024;
+  static constexpr int kABytes = 128 * 128, kBBytes = TN / CTAS * 128, kBytes = kABytes + kBBytes;
+  static constexpr int kStages = 163840 / kBytes > 6 ? 6 : 163840 / kBytes;
+  static constexpr int kOut = kStages * kBytes, kColumns = kOut + kI8Warps * kI8Piece;
+  static constexpr int kSpan = TN / 2 < 64 ? 64 : TN / 2;       // columns of an epilogue warp: whole pieces
+  static constexpr int kSmem = kColumns + kI8Warps * kSpan * 8 + 1024;
 };
 
 struct I8Ctl {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained;
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained, pause;
   uint32_t tmem_base, abort_flag;
 };
 
@@ -137,41 +140,105 @@ __host__ __device__ constexpr uint32_t umma_idesc_i8(uint32_t M, uint32_t N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 // Four k-steps of 32 bytes.
+#define S3R_I8_K4(group)                                                     \
+  asm volatile(                                                              \
+      "{\n\t.reg .pred p, pt;\n\t.reg .b64 a, b;\n\t"                        \
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"                   \
+      "tcgen05.mma.cta_group::" group ".kind::i8 [%0], %1, %2, %3, p;\n\t"   \
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"                           \
+      "tcgen05.mma.cta_group::" group ".kind::i8 [%0], a, b, %3, pt;\n\t"    \
+      "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"                             \
+      "tcgen05.mma.cta_group::" group ".kind::i8 [%0], a, b, %3, pt;\n\t"    \
+      "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"                             \
+      "tcgen05.mma.cta_group::" group ".kind::i8 [%0], a, b, %3, pt;\n\t}"   \
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)        \
+      : "memory")
+template <int CTAS>
 __device__ __forceinline__ void umma_i8_k4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p, pt;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
-      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, pt;\n\t"
-      "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, pt;\n\t"
-      "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, pt;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
-      : "memory");
+  if constexpr (CTAS == 2) S3R_I8_K4("2");
+  else S3R_I8_K4("1");
 }
-__device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(dst_smem), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
+// arrives at this barrier of both CTAs of a pair (of this CTA's) once the products issued so far are done
+template <int CTAS>
+struct Ctas {};
+template <int CTAS>
+__device__ __forceinline__ void umma_commit(uint64_t* bar, Ctas<CTAS>) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"(static_cast<uint16_t>(3)) : "memory");
+  else
+    umma_commit(bar);
+}
+// address of `bar` in the pair's first CTA
+template <int CTAS>
+__device__ __forceinline__ uint32_t first_cta(uint64_t* bar) {
+  uint32_t at = smem_u32(bar);
+  if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(at));
+  return at;
+}
+template <int CTAS>
+__device__ __forceinline__ void arrive_first_cta(uint64_t* bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<2>(bar)) : "memory");
+  else
+    mbar_arrive(bar);
+}
+// `bar`: address of a barrier of this CTA, or of the pair's other one
+template <int CTAS>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  if constexpr (CTAS == 2)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst_smem), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst_smem), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// 32 lanes x 32 columns as four rows and eight columns per lane: register 16 h + 4 j + 2 i + e of lane l holds row 16 h + 8 i + l / 4,
+// column 8 j + 2 (l % 4) + e.
+__device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]), "=r"(r[16 * h + 5]),
+                   "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]), "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]),
+                   "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+                 : "r"(taddr + (static_cast<uint32_t>(16 * h) << 16)));
+}
+// The wait for it, tied to its registers: nothing that reads them moves in front of it.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])::"memory");
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src_smem, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(map), "r"(src_smem), "r"(c0), "r"(c1) : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+template <int CTAS>
+__device__ __forceinline__ void sync_pair() {
+  if constexpr (CTAS == 2) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+  if constexpr (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+  else tmem_dealloc(at, columns);
+}
 
-template <int TN>
+// TYPE: of the output
+template <int TN, int CTAS, int TYPE>
 __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                                                                  const __grid_constant__ CUtensorMap mo, const __grid_constant__ I8Params p) {
-  using C = I8Cfg<TN>;
+  using C = I8Cfg<TN, CTAS>;
   extern __shared__ char raw_smem[];
   __shared__ I8Ctl ctl;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? static_cast<int>(blockIdx.x & 1) : 0;          // a cluster is two consecutive CTAs
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&ctl.full[s], 1);
@@ -179,169 +246,222 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctl.acc_full[s], 1);
-      mbar_init(&ctl.acc_empty[s], 4);
+      mbar_init(&ctl.acc_empty[s], CTAS * kI8Warps);
     }
     mbar_init(&ctl.drained, 1);
+    mbar_init(&ctl.pause, 1);
     ctl.abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc(&ctl.tmem_base, 2 * TN);
-    tmem_relinquish();
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(2 * TN) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(&ctl.tmem_base, 2 * TN);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  sync_pair<CTAS>();
   tc_fence_after();
   griddep_wait();
   griddep_launch();
   const uint32_t tmem = ctl.tmem_base;
   volatile uint32_t* abort_flag = &ctl.abort_flag;
-  const int tiles = p.m_tiles * p.n_tiles, steps = (p.K + 127) / 128;
+  const int tiles = p.m_tiles * p.n_tiles, steps = (p.K + 127) / 128, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
   const uint32_t base = smem_u32(smem);
 
   if (warp == 0) {
     int n = 0;                                                     // copies so far
     bool ok = true;
     const bool leader = elect_one_sync();
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const int m0 = tile / p.n_tiles * 128, n0 = tile % p.n_tiles * TN;
+    for (int tile = first; tile < tiles && ok; tile += stride) {
+      const int m0 = (tile / p.n_tiles * CTAS + rank) * 128, n0 = tile % p.n_tiles * TN + rank * (TN / CTAS);
       for (int k = 0; k < steps; ++k, ++n) {
         const int s = n % C::kStages;
         ok = mbar_wait_warp(&ctl.empty[s], (n / C::kStages & 1) ^ 1, abort_flag);
         if (!ok) break;
         if (leader) {
-          mbar_expect_tx(&ctl.full[s], C::kBytes);
-          tma_load_2d(base + s * C::kBytes, &ma, &ctl.full[s], k * 128, m0);
-          tma_load_2d(base + s * C::kBytes + C::kABytes, &mb, &ctl.full[s], k * 128, n0);
+          const uint32_t bar = first_cta<CTAS>(&ctl.full[s]);      // both CTAs' copies complete the first one's barrier
+          if (rank == 0) mbar_expect_tx(&ctl.full[s], CTAS * C::kBytes);
+          tma_load_2d<CTAS>(base + s * C::kBytes, &ma, bar, k * 128, m0);
+          tma_load_2d<CTAS>(base + s * C::kBytes + C::kABytes, &mb, bar, k * 128, n0);
         }
         __syncwarp();
       }
     }
     if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
-      for (int i = n - C::kStages < 0 ? 0 : n - C::kStages; i < n; ++i) {
-        volatile uint32_t dummy = 0;
+      volatile uint32_t dummy = 0;
+      for (int i = n - C::kStages < 0 ? 0 : n - C::kStages; rank == 0 && i < n; ++i) {
+        dummy = 0;
         mbar_wait(&ctl.full[i % C::kStages], i / C::kStages & 1, &dummy);
       }
+      dummy = 0;
+      mbar_wait_limit(&ctl.pause, 0, &dummy, 10000000ull);         // the second CTA does not see its own land: 10 ms
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = umma_idesc_i8(128, TN);
-    const bool leader = elect_one_sync();
-    int n = 0, done = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++done) {
-      const int buf = done & 1;
-      ok = mbar_wait_warp(&ctl.acc_empty[buf], (done >> 1 & 1) ^ 1, abort_flag);
-      tc_fence_after();
-      for (int k = 0; k < steps && ok; ++k, ++n) {
-        const int s = n % C::kStages;
-        ok = mbar_wait_warp(&ctl.full[s], n / C::kStages & 1, abort_flag);
-        if (!ok) break;
+    if (rank == 0) {
+      constexpr uint32_t idesc = umma_idesc_i8(128 * CTAS, TN);
+      const bool leader = elect_one_sync();
+      int n = 0, done = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride, ++done) {
+        const int buf = done & 1;
+        ok = mbar_wait_warp(&ctl.acc_empty[buf], (done >> 1 & 1) ^ 1, abort_flag);
         tc_fence_after();
-        if (leader) {
-          umma_i8_k4(tmem + buf * TN, umma_desc_sw128(base + s * C::kBytes), umma_desc_sw128(base + s * C::kBytes + C::kABytes), idesc, k > 0);
-          umma_commit(&ctl.empty[s]);
-          if (k == steps - 1) umma_commit(&ctl.acc_full[buf]);
+        for (int k = 0; k < steps && ok; ++k, ++n) {
+          const int s = n % C::kStages;
+          ok = mbar_wait_warp(&ctl.full[s], n / C::kStages & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            umma_i8_k4<CTAS>(tmem + buf * TN, umma_desc_sw128(base + s * C::kBytes), umma_desc_sw128(base + s * C::kBytes + C::kABytes), idesc, k > 0);
+            umma_commit(&ctl.empty[s], Ctas<CTAS>());
+            if (k == steps - 1) umma_commit(&ctl.acc_full[buf], Ctas<CTAS>());
+          }
+          __syncwarp();
         }
+      }
+      if (!ok) {
+        if (leader) umma_commit(&ctl.drained, Ctas<CTAS>());
         __syncwarp();
+        volatile uint32_t dummy = 0;
+        mbar_wait(&ctl.drained, 0, &dummy);                        // let issued products drain before tensor memory is freed
       }
     }
-    if (!ok) {
-      if (leader) umma_commit(&ctl.drained);
-      __syncwarp();
-      volatile uint32_t dummy = 0;
-      mbar_wait(&ctl.drained, 0, &dummy);                          // let issued products drain before tensor memory is freed
-    }
   } else {
-    const int quarter = warp & 3;                                  // lanes 32 * quarter .. of tensor memory
-    const uint32_t stage0 = base + C::kOut + quarter * 2 * kI8Stage;
-    float2* columns = reinterpret_cast<float2*>(smem + C::kColumns) + quarter * 32;
-    const int per = p.type == S3R_F32 ? 32 : 64;                   // columns of a piece
-    int done = 0, piece = 0;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;          // lanes 32 * quarter .. of tensor memory; half of the columns
+    char* piece = smem + C::kOut + (warp - 2) * kI8Piece;
+    const uint32_t stage = smem_u32(piece);
+    float* columns = reinterpret_cast<float*>(smem + C::kColumns) + (warp - 2) * 2 * C::kSpan;        // scales, biases
+    constexpr int per = TYPE == S3R_F32 ? 32 : 64;                 // columns of a piece
+    const int from = half * C::kSpan;
+    constexpr int kMine = C::kSpan / 32;
+    // A lane's part of 32 rows x 32 columns: rows r, r + 8, r + 16, r + 24, of every eight columns two from c on.  With a row per lane
+    // every lane would need every column's factors, and reading those (a wavefront per column and warp) kept shared memory busier
+    // than the products at K = 1024 (64 512 x 4096: 248 us).
+    const int r = lane >> 2, c = 2 * (lane & 3);
+    float scale[kMine], bias[kMine], rows[4];                      // of the next tile: fetched while this one is written out
+    auto fetch = [&](int tile) {
+      const int n0 = tile % p.n_tiles * TN + from;
+      const int64_t row = (static_cast<int64_t>(tile / p.n_tiles) * CTAS + rank) * 128 + quarter * 32 + r;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int col = n0 + i * 32 + lane;
+        scale[i] = tile < tiles && col < p.N ? __ldg(p.b_scale + col) : 0.f;
+        bias[i] = tile < tiles && p.bias && col < p.N ? __ldg(p.bias + col) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = tile < tiles && row + 8 * i < p.M ? __ldg(p.a_scale + row + 8 * i) : 0.f;
+    };
+    fetch(first);
+    int done = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++done) {
+    for (int tile = first; tile < tiles && ok; tile += stride, ++done) {
       const int buf = done & 1;
-      const int64_t m0 = static_cast<int64_t>(tile / p.n_tiles) * 128 + quarter * 32;
+      const int64_t m0 = (static_cast<int64_t>(tile / p.n_tiles) * CTAS + rank) * 128 + quarter * 32;
       const int n0 = tile % p.n_tiles * TN;
-      const float row_scale = m0 + lane < p.M ? __ldg(p.a_scale + m0 + lane) : 0.f;
+      const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
+      float2 row[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) row[i] = make_float2(rows[i], rows[i]);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) columns[i * 32 + lane] = scale[i], columns[C::kSpan + i * 32 + lane] = bias[i];
+      __syncwarp();
+      fetch(tile + stride);
       ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int width = min(TN, p.N - n0);
-      for (int c0 = 0; c0 < width; c0 += per, ++piece) {
-        const uint32_t stage = stage0 + (piece & 1) * kI8Stage;
-        if (lane == 0) bulk_wait_read<1>();                        // the store before the last has left this half
-        __syncwarp();
-        for (int half = 0; half < per; half += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + c0 + half, v);
-          const int col = n0 + c0 + half + lane;
-          const bool in = col < p.N;
-          columns[lane] = make_float2(in ? __ldg(p.b_scale + col) : 0.f, in && p.bias ? __ldg(p.bias + col) : 0.f);
-          __syncwarp();
-          tmem_ld_wait();
+      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
+      uint32_t v[2][32];                                           // 32 columns' sums and the next 32
+      if (from < width) tmem_ld_32x32(sums, v[0]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float4 f = *reinterpret_cast<const float4*>(columns + i);
-            const float x = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int>(v[i])), row_scale), f.x);
-            const float y = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int>(v[i + 1])), row_scale), f.z);
-            v[i] = __float_as_uint(p.bias ? __fadd_rn(x, f.y) : x);
-            v[i + 1] = __float_as_uint(p.bias ? __fadd_rn(y, f.w) : y);
+      for (int g = 0; g < kMine; ++g) {
+        if (from + g * 32 < width) {
+          uint32_t(&now)[32] = v[g & 1];
+          tmem_ld_wait_for(now);
+          const bool last = g + 1 == kMine || from + g * 32 + 32 >= width;
+          if (!last) tmem_ld_32x32(sums + g * 32 + 32, v[(g + 1) & 1]);
+          else {                                                   // this warp's sums are in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
           }
-          auto f = [&](int i) { return __uint_as_float(v[i]); };
-          if (p.type == S3R_F32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sts128(stage + swz128(lane, i), v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          } else if (p.type == S3R_BF16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sts128(stage + swz128(lane, half / 8 + i), pack_bf16(f(8 * i), f(8 * i + 1)), pack_bf16(f(8 * i + 2), f(8 * i + 3)),
-                     pack_bf16(f(8 * i + 4), f(8 * i + 5)), pack_bf16(f(8 * i + 6), f(8 * i + 7)));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sts128(stage + swz128(lane, half / 8 + i), pack_half(f(8 * i), f(8 * i + 1)), pack_half(f(8 * i + 2), f(8 * i + 3)),
-                     pack_half(f(8 * i + 4), f(8 * i + 5)), pack_half(f(8 * i + 6), f(8 * i + 7)));
+          if (per == 32 || !(g & 1)) {
+            if (lane == 0) bulk_wait_read();                       // the store before has left this piece
+            __syncwarp();
           }
-          __syncwarp();                                            // all lanes have read the columns' factors
-        }
-        if (c0 + per >= width) {                                   // the tile's sums are in registers or stored
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.acc_empty[buf]);
-        }
-        if (p.copy_out) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (m0 < p.M) tma_store_2d(&mo, stage, n0 + c0, static_cast<int>(m0));
-            bulk_commit();
+          // all of a granule's words before the first store: a store to shared memory keeps later loads behind it
+          float2 s[4], b[4], x[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[j] = *reinterpret_cast<const float2*>(columns + g * 32 + 8 * j + c);
+            b[j] = *reinterpret_cast<const float2*>(columns + C::kSpan + g * 32 + 8 * j + c);
           }
-        } else {
-          __syncwarp();
-          const int left = min(per, width - c0);
-          for (int r = 0; r < 32 && m0 + r < p.M; ++r) {
-            const int64_t at = (m0 + r) * p.N + n0 + c0;
-            for (int c = lane; c < left; c += 32) {
-              const int byte = c * type_bytes(p.type);
-              const char* from = smem + (stage - base) + swz128(r, byte >> 4) + (byte & 15);
-              if (p.type == S3R_F32) static_cast<float*>(p.out)[at + c] = *reinterpret_cast<const float*>(from);
-              else static_cast<uint16_t*>(p.out)[at + c] = *reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
+              const float2 sum = make_float2(__int2float_rn(static_cast<int>(now[at])), __int2float_rn(static_cast<int>(now[at + 1])));
+              x[j][i] = ffma2(fmul2(sum, row[i]), s[j], b[j]);
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // row r + 8 i: 128 bytes, its 16-byte chunks swizzled by r
+            char* to = piece + r * 128 + (TYPE == S3R_F32 ? (((2 * j + (c >> 2)) ^ r) << 4) + (c & 2) * 4 : ((((g & 1) * 4 + j) ^ r) << 4) + c * 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (TYPE == S3R_F32) *reinterpret_cast<float2*>(to + i * 1024) = x[j][i];
+              else *reinterpret_cast<uint32_t*>(to + i * 1024) = TYPE == S3R_BF16 ? pack_bf16(x[j][i].x, x[j][i].y) : pack_half(x[j][i].x, x[j][i].y);
+            }
+          }
+          if (per == 32 || (g & 1) || last) {
+            const int c0 = from + (per == 32 ? g * 32 : g / 2 * 64);
+            if (p.copy_out) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (m0 < p.M) tma_store_2d(&mo, stage, n0 + c0, static_cast<int>(m0));
+                bulk_commit();
+              }
+            } else {
+              __syncwarp();
+              const int left = min(per, width - c0);
+              for (int i = 0; i < 32 && m0 + i < p.M; ++i) {
+                const int64_t at = (m0 + i) * p.N + n0 + c0;
+                for (int k = lane; k < left; k += 32) {
+                  const int byte = k * type_bytes(TYPE);
+                  const char* from_smem = piece + swz128(i, byte >> 4) + (byte & 15);
+                  if constexpr (TYPE == S3R_F32) static_cast<float*>(p.out)[at + k] = *reinterpret_cast<const float*>(from_smem);
+                  else static_cast<uint16_t*>(p.out)[at + k] = *reinterpret_cast<const uint16_t*>(from_smem);
+                }
+              }
+              __syncwarp();                                        // read before the next piece is written
             }
           }
         }
       }
+      if (from >= width) {                                         // none of this warp's columns exist
+        __syncwarp();
+        if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+      }
+      __syncwarp();                                                // its factors are read
     }
     if (lane == 0) bulk_wait_all();
     if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 2 * TN);
+  sync_pair<CTAS>();                                               // the other CTA's products and arrivals reach this one's memory
+  if (warp == 1) tmem_free<CTAS>(tmem, 2 * TN);
 }
 
-template <int TN>
-static int run_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch, I8Params p, cudaStream_t st) {
-  using C = I8Cfg<TN>;
+template <int TN, int CTAS, int TYPE>
+static int launch_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch, I8Params p, cudaStream_t st) {
+  using C = I8Cfg<TN, CTAS>;
   CUtensorMap ma, mb, mo;
   {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(a_pitch)};
@@ -350,23 +470,42 @@ static int run_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b
   }
   {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.N)}, strides[1] = {static_cast<uint64_t>(b_pitch)};
-    const uint32_t box[2] = {128, TN};
+    const uint32_t box[2] = {128, TN / CTAS};
     if (const int rc = make_tensor_map(&mb, b, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_UINT8)) return rc;
   }
   mo = ma;
   if (p.copy_out) {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)};
-    const uint64_t strides[1] = {static_cast<uint64_t>(p.N) * type_bytes(p.type)};
-    const uint32_t box[2] = {static_cast<uint32_t>(128 / type_bytes(p.type)), 32};
-    const CUtensorMapDataType type = p.type == S3R_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.type == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const uint64_t strides[1] = {static_cast<uint64_t>(p.N) * type_bytes(TYPE)};
+    const uint32_t box[2] = {128 / type_bytes(TYPE), 32};
+    const CUtensorMapDataType type = TYPE == S3R_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : TYPE == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (const int rc = make_tensor_map(&mo, p.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
   }
+  p.m_tiles = static_cast<int>((p.M + 128 * CTAS - 1) / (128 * CTAS));
   p.n_tiles = (p.N + TN - 1) / TN;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles, at_once = sm_count() / CTAS;
   S3R_REQUIRE(tiles < (1ll << 31) - 1024, S3R_ERR_TOO_LARGE, "s3r_int8_linear: too many tiles");
-  S3R_CUDA(cudaFuncSetAttribute(int8_linear_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  const unsigned grid = static_cast<unsigned>(tiles < sm_count() ? tiles : sm_count());
-  return launch(int8_linear_kernel<TN>, grid, kI8Threads, C::kSmem, st, ma, mb, mo, p);
+  S3R_CUDA(cudaFuncSetAttribute(int8_linear_kernel<TN, CTAS, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(static_cast<unsigned>((tiles < at_once ? tiles : at_once) * CTAS));
+  c.blockDim = dim3(kI8Threads);
+  c.dynamicSmemBytes = C::kSmem;
+  c.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  c.attrs = attr;
+  c.numAttrs = CTAS == 2 ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&c, int8_linear_kernel<TN, CTAS, TYPE>, ma, mb, mo, p), "kernel launch");
+}
+template <int TN, int CTAS>
+static int run_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b_pitch, int type, const I8Params& p, cudaStream_t st) {
+  if (type == S3R_F32) return launch_int8<TN, CTAS, S3R_F32>(a, a_pitch, b, b_pitch, p, st);
+  if (type == S3R_BF16) return launch_int8<TN, CTAS, S3R_BF16>(a, a_pitch, b, b_pitch, p, st);
+  return launch_int8<TN, CTAS, S3R_F16>(a, a_pitch, b, b_pitch, p, st);
 }
 
 }  // namespace s3r
@@ -407,18 +546,18 @@ extern "C" int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_
   p.M = M;
   p.N = N;
   p.K = K;
-  p.type = type;
-  p.m_tiles = static_cast<int>((M + 127) / 128);
   p.copy_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && static_cast<int64_t>(N) * type_bytes(type) % 16 == 0;
   p.status = device_status_ptr();
   S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_int8_linear: no status word");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // the tile width whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a)
-  auto cost = [&](int tn) {
-    const int64_t tiles = static_cast<int64_t>(p.m_tiles) * ((N + tn - 1) / tn);
-    return (tiles + sm_count() - 1) / sm_count() * (tn + 64);
+  // the tile whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a)
+  auto cost = [&](int tn, int ctas) {
+    const int64_t tiles = (M + 128 * ctas - 1) / (128 * ctas) * ((N + tn - 1) / tn), at_once = sm_count() / ctas;
+    return (tiles + at_once - 1) / at_once * (tn + (ctas == 2 ? 64 : 96));
   };
-  if (cost(256) <= cost(128) && cost(256) <= cost(64)) return run_int8<256>(a, a_pitch, b, b_pitch, p, st);
-  if (cost(128) <= cost(64)) return run_int8<128>(a, a_pitch, b, b_pitch, p, st);
-  return run_int8<64>(a, a_pitch, b, b_pitch, p, st);
+  const int64_t pair_256 = cost(256, 2), pair_128 = cost(128, 2), one_128 = cost(128, 1), one_64 = cost(64, 1);
+  if (M > 128 && pair_256 <= pair_128 && pair_256 <= one_128 && pair_256 <= one_64) return run_int8<256, 2>(a, a_pitch, b, b_pitch, type, p, st);
+  if (M > 128 && pair_128 <= one_128 && pair_128 <= one_64) return run_int8<128, 2>(a, a_pitch, b, b_pitch, type, p, st);
+  if (one_128 <= one_64) return run_int8<128, 1>(a, a_pitch, b, b_pitch, type, p, st);
+  return run_int8<64, 1>(a, a_pitch, b, b_pitch, type, p, st);
 }

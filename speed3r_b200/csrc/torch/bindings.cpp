@@ -999,12 +999,6 @@ void host_in_use(const Tensor& host, at::Device device) {
   at::getHostAllocator(at::kCUDA)->record_event(host.data_ptr(), host.storage().data_ptr().get_context(), c10::cuda::getCurrentCUDAStream(device.index()));
 }
 
-// a tensor with memory, not one of those that a tracer runs the backward on
-bool plain(const Tensor& t) {
-  return t.is_cuda() && !t.key_set().has(c10::DispatchKey::Python) && !t.key_set().has(c10::DispatchKey::Functionalize) &&
-         !c10::impl::dispatch_mode_enabled();
-}
-
 // The whole op.  group = 0 where compressed keys are the selection blocks.  As one node its backward adds the
 // pooled branch's gradients inside the selection kernels' stores: separate nodes write them out as [B,H,T,d] and add
 // two bf16 tensors three times (1.5 of 19.4 ms at 250 views).

@@ -84,23 +84,35 @@ s3r_residual_norm norm_args(const Tensor& x, const optional<Tensor>& y, const op
   return a;
 }
 
+struct NormInputs {
+  Tensor x;
+  optional<Tensor> y, w, b, s, g, pw, pb;
+};
+
+// (r, h, stats), undefined where there is nothing to compute or to keep
+std::tuple<Tensor, Tensor, Tensor> run_norm_fwd(const NormInputs& in, const NormShape& n, at::ScalarType h_type, bool keep) {
+  const Tensor& x = in.x;
+  s3r_residual_norm a = norm_args(x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, n);
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor r, h, stats;
+  if (in.y.has_value()) r = fresh_like(x);
+  if (n.norm) h = fresh(x.sizes(), x, h_type), a.h_type = type_of(h, "the norm's result");
+  if (keep) stats = fresh({4, a.batch * a.tokens}, x, at::kFloat);
+  if (x.numel()) {
+    a.r = pointer(r);
+    a.h = pointer(h);
+    a.stats = keep ? f32(stats) : nullptr;
+    check(s3r_residual_norm_fwd(&a, stream()), "s3r_residual_norm_fwd");
+  }
+  return {r, h, stats};
+}
 std::tuple<Tensor, Tensor, Tensor> residual_norm_fwd(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& weight,
                                                      const optional<Tensor>& bias, const optional<Tensor>& scale,
                                                      const optional<Tensor>& gate, const optional<Tensor>& post_weight,
                                                      const optional<Tensor>& post_bias, bool norm, bool post, int64_t kind, double eps,
                                                      double post_eps, at::ScalarType h_type, bool keep) {
-  s3r_residual_norm a = norm_args(x, y, weight, bias, scale, gate, post_weight, post_bias, {norm, post, kind, eps, post_eps});
-  c10::cuda::CUDAGuard guard(x.device());
-  Tensor r = y.has_value() ? fresh_like(x) : none(x), h = norm ? fresh(x.sizes(), x, h_type) : fresh({0}, x, h_type);
-  Tensor stats = fresh({keep ? 4 : 0, a.batch * a.tokens}, x, at::kFloat);
-  if (norm) a.h_type = type_of(h, "the norm's result");
-  if (x.numel()) {
-    a.r = y.has_value() ? r.data_ptr() : nullptr;
-    a.h = norm ? h.data_ptr() : nullptr;
-    a.stats = keep ? f32(stats) : nullptr;
-    check(s3r_residual_norm_fwd(&a, stream()), "s3r_residual_norm_fwd");
-  }
-  return {r, h, stats};
+  auto [r, h, stats] = run_norm_fwd({x, y, weight, bias, scale, gate, post_weight, post_bias}, {norm, post, kind, eps, post_eps}, h_type, keep);
+  return {r.defined() ? r : none(x), h.defined() ? h : fresh({0}, x, h_type), stats.defined() ? stats : fresh({0, x.size(0) * x.size(1)}, x, at::kFloat)};
 }
 
 std::tuple<Tensor, Tensor, Tensor> residual_norm_int8(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& weight,
@@ -123,12 +135,13 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm_int8(const Tensor& x, const opt
   return {r, q, s};
 }
 
-// Gradients of (x, y, weight, bias, scale, gate, post_weight, post_bias); those that `want` (a bit each) does not name have no elements.
+// Gradients of (x, y, weight, bias, scale, gate, post_weight, post_bias); those that `want` (a bit each) does not name are undefined (from the
+// operator: without elements).
 enum { kX = 1, kY = 2, kWeight = 4, kBias = 8, kScale = 16, kGate = 32, kPostWeight = 64, kPostBias = 128 };
-std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& weight,
-                                      const optional<Tensor>& scale, const optional<Tensor>& gate, const optional<Tensor>& post_weight,
-                                      const optional<Tensor>& post_bias, const Tensor& stats, const optional<Tensor>& dr,
-                                      const optional<Tensor>& dh, bool post, int64_t kind, int64_t want, at::ScalarType param_type) {
+std::vector<Tensor> run_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& weight, const optional<Tensor>& scale,
+                                 const optional<Tensor>& gate, const optional<Tensor>& post_weight, const optional<Tensor>& post_bias,
+                                 const Tensor& stats, const optional<Tensor>& dr, const optional<Tensor>& dh, bool post, int64_t kind,
+                                 int64_t want, at::ScalarType param_type) {
   s3r_residual_norm f = norm_args(r, y, weight, {}, scale, gate, post_weight, post_bias, {true, post, kind, 0., 0.});
   c10::cuda::CUDAGuard guard(r.device());
   f.r = r.data_ptr();
@@ -144,10 +157,10 @@ std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y
   TORCH_CHECK(!dr.has_value() || dr->scalar_type() == r.scalar_type(), "residual_norm: the gradient of the sum has another type than the sum");
   if (dh.has_value()) f.h_type = type_of(*dh, "the gradient of the norm");
   if (!dh.has_value()) want &= ~(kWeight | kBias);
-  auto channels = [&](int64_t bit) { return fresh({want & bit ? r.size(2) : 0}, r, param_type); };
-  Tensor dx = fresh_like(r), dy = want & kY ? fresh_like(*y) : none(r);
+  auto channels = [&](int64_t bit) { return want & bit ? fresh({r.size(2)}, r, param_type) : Tensor(); };
+  Tensor dx = fresh_like(r), dy = want & kY ? fresh_like(*y) : Tensor();
   Tensor dw = channels(kWeight), db = channels(kBias), ds = channels(kScale), dpw = channels(kPostWeight), dpb = channels(kPostBias);
-  Tensor dg = none(r), dg_row;
+  Tensor dg, dg_row;
   s3r_residual_norm_grad g = {};
   if (want & kGate) {
     if (f.gate_mode == S3R_GATE_ROW) {
@@ -159,8 +172,8 @@ std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y
     }
   }
   if (rows == 0) {
-    for (Tensor* t : {&dw, &db, &ds, &dpw, &dpb}) t->zero_();
-    if (dg.numel()) dg.zero_();
+    for (Tensor* t : {&dw, &db, &ds, &dg, &dpw, &dpb})
+      if (t->defined()) t->zero_();
   } else {
     g.dr = pointer(dr);
     g.dh = pointer(dh);
@@ -180,6 +193,16 @@ std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y
   return {dx, dy, dw, db, ds, dg, dpw, dpb};
 }
 
+std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& weight,
+                                      const optional<Tensor>& scale, const optional<Tensor>& gate, const optional<Tensor>& post_weight,
+                                      const optional<Tensor>& post_bias, const Tensor& stats, const optional<Tensor>& dr,
+                                      const optional<Tensor>& dh, bool post, int64_t kind, int64_t want, at::ScalarType param_type) {
+  auto g = run_norm_bwd(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, post, kind, want, param_type);
+  for (Tensor& t : g)
+    if (!t.defined()) t = none(r);
+  return g;
+}
+
 std::tuple<Tensor, Tensor, Tensor> call_norm_fwd(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& b,
                                                  const optional<Tensor>& s, const optional<Tensor>& g, const optional<Tensor>& pw,
                                                  const optional<Tensor>& pb, const NormShape& n, at::ScalarType h_type, bool keep) {
@@ -192,6 +215,10 @@ std::vector<Tensor> call_norm_bwd(const Tensor& r, const optional<Tensor>& y, co
   S3R_DISPATCHED(residual_norm_bwd)(r, y, w, s, g, pw, pb, stats, dr, dh, post, kind, want, param_type);
 }
 
+std::tuple<Tensor, Tensor, Tensor> call_norm_int8(const NormInputs& in, bool post, int64_t kind, double eps, double post_eps) {
+  S3R_DISPATCHED(residual_norm_int8)(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, post, kind, eps, post_eps);
+}
+
 optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 Tensor value(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
@@ -201,7 +228,9 @@ struct NormNode : torch::autograd::Function<NormNode> {
                                const optional<Tensor>& pb, bool norm, bool post, int64_t kind, double eps, double post_eps, int64_t h_type) {
     at::AutoDispatchBelowADInplaceOrView below;
     const bool branch = y.has_value();
-    auto [r, h, stats] = call_norm_fwd(x, y, w, b, s, g, pw, pb, {norm, post, kind, eps, post_eps}, static_cast<at::ScalarType>(h_type), true);
+    const NormShape shape = {norm, post, kind, eps, post_eps};
+    const auto type = static_cast<at::ScalarType>(h_type);
+    auto [r, h, stats] = plain(x) ? run_norm_fwd({x, y, w, b, s, g, pw, pb}, shape, type, true) : call_norm_fwd(x, y, w, b, s, g, pw, pb, shape, type, true);
     // the branch itself is needed for the gradients of what multiplies it
     const bool needs_y = branch && (post || (s.has_value() && s->requires_grad()) || (g.has_value() && g->requires_grad()));
     at::ScalarType param = at::kFloat;
@@ -243,10 +272,11 @@ struct NormNode : torch::autograd::Function<NormNode> {
     // a branch that nothing is multiplied with is not kept; its place is taken by a tensor of its type that is not read
     optional<Tensor> y = maybe(s[1]);
     if (branch && !y.has_value()) y = at::empty(s[0].sizes(), s[0].options().dtype(static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt())));
-    const auto g = call_norm_bwd(s[0], y, maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, post, ctx->saved_data["kind"].toInt(),
+    const auto& backward = plain(s[0]) ? run_norm_bwd : call_norm_bwd;
+    const auto g = backward(s[0], y, maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, post, ctx->saved_data["kind"].toInt(),
                                  want, static_cast<at::ScalarType>(ctx->saved_data["param"].toInt()));
     for (int i = 0; i < 8; ++i)
-      if (want >> i & 1 && (dh.has_value() || !(i == 2 || i == 3))) out[i] = g[i];
+      if (want >> i & 1 && g[i].defined() && (dh.has_value() || !(i == 2 || i == 3))) out[i] = g[i];
     return out;
   }
 };
@@ -255,6 +285,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 Tensor as_rows(const Tensor& t) {
   const int64_t d = t.dim(), tokens = d > 1 ? t.size(d - 2) : 1;
   int64_t batch = 1;
+  if (d == 3) return t.contiguous();
   for (int64_t i = 0; i + 2 < d; ++i) batch *= t.size(i);
   return t.contiguous().view({batch, tokens, t.size(d - 1)});
 }
@@ -288,10 +319,7 @@ void of_one_type(std::initializer_list<optional<Tensor>*> params) {
     if (p->has_value()) *p = (mixed ? (*p)->to(at::kFloat) : **p).contiguous();
 }
 
-struct NormInputs {
-  Tensor x;
-  optional<Tensor> y, w, b, s, g, pw, pb;
-};
+Tensor in_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 NormInputs norm_inputs(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& b, const optional<Tensor>& s,
                        const optional<Tensor>& gate, const optional<Tensor>& pw, const optional<Tensor>& pb, bool norm, bool post, int64_t kind) {
   TORCH_CHECK(x.dim() >= 1, "residual_norm: x needs a dimension");
@@ -307,7 +335,7 @@ NormInputs norm_inputs(const Tensor& x, const optional<Tensor>& y, const optiona
   return in;
 }
 
-// (r, h); without a branch r has no elements, without a norm h
+// (r, h); what is not computed - r without a branch, h without a norm - is x
 std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& b,
                                          const optional<Tensor>& s, const optional<Tensor>& gate, const optional<Tensor>& pw,
                                          const optional<Tensor>& pb, bool norm, bool post, int64_t kind, double eps, double post_eps,
@@ -316,11 +344,12 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const optional<Tensor>
   if (wants_grad(x, value(y), value(w), value(b), value(s), value(gate), value(pw), value(pb))) {
     const auto out = NormNode::apply(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, norm, post, kind, eps, post_eps,
                                      static_cast<int64_t>(h_type));
-    return {y.has_value() ? out[0].view(x.sizes()) : Tensor(at::empty({0}, x.options())),
-            norm ? out.back().view(x.sizes()) : Tensor(at::empty({0}, x.options()))};
+    return {y.has_value() ? in_shape(out[0], x.sizes()) : x, norm ? in_shape(out.back(), x.sizes()) : x};
   }
-  auto [r, h, stats] = call_norm_fwd(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, {norm, post, kind, eps, post_eps}, h_type, false);
-  return {y.has_value() ? r.view(x.sizes()) : r, norm ? h.view(x.sizes()) : h};
+  const NormShape shape = {norm, post, kind, eps, post_eps};
+  auto [r, h, stats] = plain(x) ? run_norm_fwd(in, shape, h_type, false)
+                                : call_norm_fwd(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, shape, h_type, false);
+  return {y.has_value() ? in_shape(r, x.sizes()) : x, norm ? in_shape(h, x.sizes()) : x};
 }
 
 std::tuple<Tensor, Tensor, Tensor> residual_norm_to_int8(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w,
@@ -330,15 +359,15 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm_to_int8(const Tensor& x, const 
   TORCH_CHECK(!wants_grad(x, value(y), value(w), value(b), value(s), value(gate), value(pw), value(pb)),
               "residual_norm_int8 is forward-only: call it under torch.no_grad()");
   const NormInputs in = norm_inputs(x, y, w, b, s, gate, pw, pb, true, post, kind);
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("speed3r_b200::residual_norm_int8", "").typed<decltype(residual_norm_int8)>();
-  auto [r, q, qs] = op.call(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, post, kind, eps, post_eps);
-  return {y.has_value() ? r.view(x.sizes()) : r, q.view(x.sizes()), qs.view(x.sizes().slice(0, x.dim() - 1))};
+  auto [r, q, qs] = plain(x) ? residual_norm_int8(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, post, kind, eps, post_eps)
+                             : call_norm_int8(in, post, kind, eps, post_eps);
+  return {y.has_value() ? in_shape(r, x.sizes()) : x, in_shape(q, x.sizes()), in_shape(qs, x.sizes().slice(0, x.dim() - 1))};
 }
 
 // ------------------------------------------------------------------------------------------------
 // 8-bit tokens and products
 // ------------------------------------------------------------------------------------------------
-std::tuple<Tensor, Tensor> quantize_tokens(const Tensor& x) {
+std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   need_cuda(x, "x");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "quantize_tokens: x needs channels");
   const int type = type_of(x, "x");
@@ -366,7 +395,7 @@ Tensor byte_rows(const Tensor& t, int64_t rows, int64_t K) {
   return part;
 }
 
-Tensor int8_linear(const Tensor& q, const Tensor& q_scale, const Tensor& weight, const Tensor& weight_scale, const optional<Tensor>& bias,
+Tensor int8_product(const Tensor& q, const Tensor& q_scale, const Tensor& weight, const Tensor& weight_scale, const optional<Tensor>& bias,
                    at::ScalarType out_type) {
   need_cuda(q, "q");
   TORCH_CHECK(q.scalar_type() == at::kChar && weight.scalar_type() == at::kChar, "int8_linear: q and weight must be int8");
@@ -399,7 +428,7 @@ Tensor int8_linear(const Tensor& q, const Tensor& q_scale, const Tensor& weight,
 // ------------------------------------------------------------------------------------------------
 // the optimiser
 // ------------------------------------------------------------------------------------------------
-Tensor grad_norm(at::TensorList tensors) {
+Tensor norm_of(at::TensorList tensors) {
   TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
   std::vector<Tensor> kept;
   std::vector<const void*> ptr;
@@ -432,7 +461,7 @@ void need_states(const Tensor& p, const Tensor& m, const Tensor& v, const option
                     (e->numel() == 0 || e->stride(1) == 1), "adamw: scales of ", p.numel(), " elements must be uint8 [2, ", (p.numel() + 255) / 256, "], got ", e->sizes());
 }
 
-void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
+void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
                 const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
                 double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
   const size_t n = params.size();
@@ -508,7 +537,7 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   check(s3r_adamw_step(&a, stream()), "s3r_adamw_step");
 }
 
-void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
+void adamw_values(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
   const size_t n = exp_avg.size();
   TORCH_CHECK(exp_avg_sq.size() == n && scales.size() == n && m_out.size() == n && v_out.size() == n, "adamw_state: lists of one length");
   if (n == 0) return;
@@ -535,6 +564,44 @@ void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorLi
   check(s3r_adamw_state(static_cast<int>(n), m.data(), v.data(), me.data(), ve.data(), mo.data(), vo.data(), counts.data(), stream()), "s3r_adamw_state");
 }
 
+// ------------------------------------------------------------------------------------------------
+// The operators that have no gradient, as they are called: on ordinary tensors straight into the base operator.  Through the dispatcher
+// each of them passed PyTorch's boxed autograd fallback, which looks at every tensor of every list.
+// ------------------------------------------------------------------------------------------------
+std::tuple<Tensor, Tensor> quantize_tokens(const Tensor& x) {
+  no_tangents(x);
+  if (plain(x)) return quantize_rows(x);
+  S3R_DISPATCHED(quantize_rows)(x);
+}
+Tensor int8_linear(const Tensor& q, const Tensor& q_scale, const Tensor& weight, const Tensor& weight_scale, const optional<Tensor>& bias,
+                   at::ScalarType out_type) {
+  if (plain(q)) return int8_product(q, q_scale, weight, weight_scale, bias, out_type);
+  S3R_DISPATCHED(int8_product)(q, q_scale, weight, weight_scale, bias, out_type);
+}
+Tensor grad_norm(at::TensorList tensors) {
+  TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
+  if (plain(tensors[0])) return norm_of(tensors);
+  S3R_DISPATCHED(norm_of)(tensors);
+}
+void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
+                const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
+                double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
+  TORCH_CHECK(!params.empty(), "adamw: no tensors");
+  if (plain(params[0])) {
+    adamw_update(params, grads, exp_avg, exp_avg_sq, step, scales, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+    // what autograd has saved of these tensors is not what they hold any more
+    for (const auto list : {params, exp_avg, exp_avg_sq})
+      for (const Tensor& t : list)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return;
+  }
+  S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, scales, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+}
+void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
+  if (exp_avg.empty() || plain(exp_avg[0])) return adamw_values(exp_avg, exp_avg_sq, scales, m_out, v_out);
+  S3R_DISPATCHED(adamw_values)(exp_avg, exp_avg_sq, scales, m_out, v_out);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(speed3r_b200, m) {
@@ -548,23 +615,29 @@ TORCH_LIBRARY_FRAGMENT(speed3r_b200, m) {
         "Tensor? post_bias, bool norm, bool post, int kind, float eps, float post_eps, ScalarType h_type) -> (Tensor, Tensor)", &residual_norm);
   m.def("residual_norm_to_int8(Tensor x, Tensor? y, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? gate, Tensor? post_weight, "
         "Tensor? post_bias, bool post, int kind, float eps, float post_eps) -> (Tensor, Tensor, Tensor)", &residual_norm_to_int8);
-  m.def("quantize_tokens(Tensor x) -> (Tensor, Tensor)");
-  m.def("int8_linear(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor");
-  m.def("grad_norm(Tensor[] tensors) -> Tensor");
-  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor?[] scales, float lr, "
+  m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
+  m.def("int8_product(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor");
+  m.def("norm_of(Tensor[] tensors) -> Tensor");
+  m.def("adamw_update(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor?[] scales, float lr, "
         "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()");
-  m.def("adamw_state(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()");
+  m.def("adamw_values(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()");
+  m.def("quantize_tokens(Tensor x) -> (Tensor, Tensor)", &quantize_tokens);
+  m.def("int8_linear(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor", &int8_linear);
+  m.def("grad_norm(Tensor[] tensors) -> Tensor", &grad_norm);
+  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor?[] scales, float lr, "
+        "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()", &adamw_step);
+  m.def("adamw_state(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()", &adamw_state);
 }
 
 #define S3R_BLOCK_OPS(m)                              \
   m.impl("residual_norm_fwd", &residual_norm_fwd);    \
   m.impl("residual_norm_bwd", &residual_norm_bwd);    \
   m.impl("residual_norm_int8", &residual_norm_int8);  \
-  m.impl("quantize_tokens", &quantize_tokens);        \
-  m.impl("int8_linear", &int8_linear);                \
-  m.impl("grad_norm", &grad_norm);                    \
-  m.impl("adamw_step", &adamw_step);                  \
-  m.impl("adamw_state", &adamw_state)
+  m.impl("quantize_rows", &quantize_rows);        \
+  m.impl("int8_product", &int8_product);                \
+  m.impl("norm_of", &norm_of);                    \
+  m.impl("adamw_update", &adamw_update);                  \
+  m.impl("adamw_values", &adamw_values)
 
 TORCH_LIBRARY_IMPL(speed3r_b200, CUDA, m) { S3R_BLOCK_OPS(m); }
 TORCH_LIBRARY_IMPL(speed3r_b200, CPU, m) { S3R_BLOCK_OPS(m); }      // every one of them refuses CPU tensors

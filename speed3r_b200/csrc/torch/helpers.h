@@ -99,6 +99,12 @@ variable_list once(const variable_list& incoming, F&& backward) {
   return g;
 }
 
+// a tensor with memory, not one of those that a tracer runs the backward on
+bool plain(const Tensor& t) {
+  return t.is_cuda() && !t.key_set().has(c10::DispatchKey::Python) && !t.key_set().has(c10::DispatchKey::Functionalize) &&
+         !c10::impl::dispatch_mode_enabled();
+}
+
 // Calls a base operator through the dispatcher (shape functions, tracers and modes see it).
 #define S3R_DISPATCHED(fn)                                                                              \
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("speed3r_b200::" #fn, "").typed<decltype(fn)>(); \

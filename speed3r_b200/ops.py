@@ -124,22 +124,22 @@ def _register_fakes() -> None:
         return (x.new_empty(x.shape if y is not None else (0,)), x.new_empty(B, T, -(-C // 16) * 16, dtype=torch.int8).narrow(2, 0, C),
                 x.new_empty(B, T, dtype=torch.float32))
 
-    @fake("speed3r_b200::quantize_tokens")
+    @fake("speed3r_b200::quantize_rows")
     def _(x):
         K = x.shape[-1]
         return (x.new_empty(x.numel() // K, -(-K // 16) * 16, dtype=torch.int8).narrow(1, 0, K).view(x.shape),
                 x.new_empty(x.shape[:-1], dtype=torch.float32))
 
-    @fake("speed3r_b200::int8_linear")
+    @fake("speed3r_b200::int8_product")
     def _(q, q_scale, weight, weight_scale, bias, out_type):
         return q.new_empty(*q.shape[:-1], weight.shape[0], dtype=out_type)
 
-    @fake("speed3r_b200::grad_norm")
+    @fake("speed3r_b200::norm_of")
     def _(tensors):
         return tensors[0].new_empty((), dtype=torch.float32)
 
-    fake("speed3r_b200::adamw_step", lambda *a: None)
-    fake("speed3r_b200::adamw_state", lambda *a: None)
+    fake("speed3r_b200::adamw_update", lambda *a: None)
+    fake("speed3r_b200::adamw_values", lambda *a: None)
 
 
 def _ops():
@@ -320,7 +320,7 @@ def residual_norm(x: Tensor, y: Optional[Tensor] = None, norm=None, scale: Optio
         raise RuntimeError(f"residual_norm: out_dtype must be fp32, bf16 or fp16, got {h_type}")
     r, h = _ops().residual_norm.default(x, y, w, b, scale, gate, pw, pb, norm is not None, post_norm is not None, _KINDS[kind], eps,
                                         post_eps, h_type)
-    return x if y is None else r, None if norm is None else h
+    return r if y is not None else x, h if norm is not None else None
 
 
 def residual_norm_int8(x: Tensor, y: Optional[Tensor] = None, norm=None, scale: Optional[Tensor] = None,

@@ -14,7 +14,8 @@
 namespace s3r {
 
 constexpr int kAdamBlock = 256, kAdamThreads = 256, kAdamMax = 320;
-constexpr int kAdamPerWarp = 256, kAdamPerCta = kAdamPerWarp * kAdamThreads / 32;
+constexpr int kAdamWarps = kAdamThreads / 32;
+constexpr int kAdamPerCta = kAdamBlock * kAdamWarps;
 
 struct AdamScalars {
   float factor;        // of the gradients
@@ -84,50 +85,96 @@ __device__ __forceinline__ uint2 philox(uint32_t a, uint32_t c, uint32_t key) {
   return make_uint2(a, c);
 }
 
-// The exponent of a block whose largest magnitude is `big`: 1.875 x 2^(e - 127) is the smallest such bound of it.  255: not finite, or
+// The exponent of a block whose largest magnitude has these bits: 1.875 x 2^(e - 127) is the smallest such bound.  255: not finite, or
 // beyond 2^100.  Below 2^-100 the exponent stays.
-__device__ __forceinline__ uint32_t block_exponent(float big) {
-  const uint32_t bits = __float_as_uint(big);
+__device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
   const uint32_t e = bits >= 0x7f800000u ? 255u : (bits + 0xFFFFFu) >> 23;
   return e > 227u ? 255u : max(e, 27u);
 }
 __device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
-// Codes: the bits of |x| scaled so that the smallest exponent field of the code is fp32's own: the code is the top of the word,
-// rounded by what `low` adds below its last bit (0x7FFFF and the last bit: to nearest even).
-template <int EXPONENT_BITS>
-__device__ __forceinline__ uint32_t code_of(float magnitude, float up, uint32_t low, bool nearest) {
-  constexpr float kDown = EXPONENT_BITS == 4 ? 1.92592994438723585e-34f : 1.26217744835361889e-29f;        // 2^-112, 2^-96
-  const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(magnitude, up), kDown));
-  const uint32_t c = (bits + (nearest ? 0x7FFFFu + (bits >> 20 & 1u) : low)) >> 20;
-  return min(c, (8u << EXPONENT_BITS) - 1u);
-}
-template <int EXPONENT_BITS>
-__device__ __forceinline__ float value_of(uint32_t code, float unit) {
-  constexpr float kUp = EXPONENT_BITS == 4 ? 5.19229685853482763e33f : 7.92281625142643376e28f;            // 2^112, 2^96
-  return __fmul_rn(__fmul_rn(__uint_as_float(code << 20), kUp), unit);
-}
+// Codes are the top of the bits of |x| scaled so that the code's smallest exponent field is fp32's own; what is added below the last bit
+// that is kept rounds them (0x7FFFF and that bit: to nearest even; a random number of as many bits: stochastically).  Two products, each
+// exact: by the block's power of two, then by 2^-112 (m, 4 bits of exponent) or 2^-96 (v, 5 bits).
+constexpr float kDownM = 1.92592994438723585e-34f, kDownV = 1.26217744835361889e-29f;
+constexpr float kUpM = 5.19229685853482763e33f, kUpV = 7.92281625142643376e28f;
 __device__ __forceinline__ float unit_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fffffffu) : power_of(e); }
+__device__ __forceinline__ float2 both_of(float x) { return make_float2(x, x); }
 
+// four bytes into the top of four words
+__device__ __forceinline__ void spread(uint32_t (&w)[4], uint32_t bytes) {
+  w[0] = bytes << 24;
+  w[1] = __byte_perm(bytes, 0, 0x1444);
+  w[2] = __byte_perm(bytes, 0, 0x2444);
+  w[3] = bytes & 0xff000000u;
+}
+// the top bytes of four words
+__device__ __forceinline__ uint32_t gather(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+__device__ __forceinline__ void decode_m(float2 (&m)[4], uint2 codes, float unit) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[4];
+    spread(w, h ? codes.y : codes.x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = static_cast<uint32_t>(static_cast<int32_t>(w[k]) >> 4) & 0x87f00000u;      // sign, code << 20
+    m[2 * h] = fmul2(fmul2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), both_of(kUpM)), both_of(unit));
+    m[2 * h + 1] = fmul2(fmul2(make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), both_of(kUpM)), both_of(unit));
+  }
+}
+__device__ __forceinline__ void decode_v(float2 (&v)[4], uint2 codes, float unit) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[4];
+    spread(w, h ? codes.y : codes.x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] >>= 4;
+    v[2 * h] = fmul2(fmul2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), both_of(kUpV)), both_of(unit));
+    v[2 * h + 1] = fmul2(fmul2(make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), both_of(kUpV)), both_of(unit));
+  }
+}
+__device__ __forceinline__ float sqrt_near(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_near(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Eight elements of a lane, as they come from memory.  W = 8: all of them exist and every array begins at a multiple of 16 bytes.
+template <bool EIGHT>
+struct Lane {
+  Raw<8> g, w, m, v;         // with 8-bit states m.v[0..1] and v.v[0..1] are codes
+  uint32_t me, ve;
+};
 template <int W>
-__device__ __forceinline__ void load_some(float (&f)[8], const void* p, int type, int64_t at, int64_t n) {
+__device__ __forceinline__ void load_lane(Raw<8>& r, const void* p, int type, int64_t at, int64_t n) {
   if constexpr (W == 8) {
-    load_vector<8>(f, p, type, at);
+    load_raw<8>(r, p, type, at);
   } else {
+    float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = at + k < n ? load_one(p, type, at + k) : 0.f;
+    pack<8>(r, f, type);
   }
 }
 template <int W>
-__device__ __forceinline__ void store_some(const float (&f)[8], void* p, int type, int64_t at, int64_t n) {
+__device__ __forceinline__ void store_lane(const float2 (&f)[4], void* p, int type, int64_t at, int64_t n) {
+  float e[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) e[2 * k] = f[k].x, e[2 * k + 1] = f[k].y;
   if constexpr (W == 8) {
     Raw<8> r;
-    pack<8>(r, f, type);
+    pack<8>(r, e, type);
     store_raw<8>(r, p, type, at);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (at + k < n) {
-        const float one[1] = {f[k]};
+        const float one[1] = {e[k]};
         Raw<1> r;
         pack<1>(r, one, type);
         store_raw<1>(r, p, type, at + k);
@@ -154,42 +201,56 @@ __device__ __forceinline__ void store_codes(uint2 c, uint8_t* p, int64_t at, int
   }
 }
 
-// Eight elements per lane: a block.  W = 8: all of them exist and every array begins at a multiple of its vectors.
-template <int W>
-__device__ __forceinline__ void adamw_block(const AdamParams& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
+template <int W, bool EIGHT>
+__device__ __forceinline__ void load_block(Lane<EIGHT>& l, const AdamTensor& x, int64_t block, int lane) {
+  const int64_t at = block * kAdamBlock + lane * 8;
+  load_lane<W>(l.g, x.g, x.flags >> 2 & 3, at, x.n);
+  load_lane<W>(l.w, x.p, x.flags & 3, at, x.n);
+  if constexpr (EIGHT) {
+    const uint2 mc = load_codes<W>(static_cast<const uint8_t*>(x.m), at, x.n), vc = load_codes<W>(static_cast<const uint8_t*>(x.v), at, x.n);
+    l.m.v[0] = mc.x, l.m.v[1] = mc.y, l.v.v[0] = vc.x, l.v.v[1] = vc.y;
+    l.me = x.me[block];
+    l.ve = x.ve[block];
+  } else {
+    load_lane<W>(l.m, x.m, S3R_F32, at, x.n);
+    load_lane<W>(l.v, x.v, S3R_F32, at, x.n);
+  }
+}
+
+template <int W, bool EIGHT>
+__device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamParams& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
   const int64_t at = block * kAdamBlock + lane * 8;
   const int p_type = x.flags & 3, g_type = x.flags >> 2 & 3;
-  const bool eight = x.flags & kAdamEight, nearest = p.seed < 0;
-  float g[8], w[8], m[8], v[8];
-  load_some<W>(g, x.g, g_type, at, x.n);
-  load_some<W>(w, x.p, p_type, at, x.n);
-  if (eight) {
-    const uint2 mc = load_codes<W>(static_cast<const uint8_t*>(x.m), at, x.n), vc = load_codes<W>(static_cast<const uint8_t*>(x.v), at, x.n);
-    const float mu = unit_of(x.me[block]), vu = unit_of(x.ve[block]);
+  const bool nearest = p.seed < 0;
+  float e[8];
+  float2 w[4], m[4], v[4];
+  unpack<8>(e, l.w, p_type);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t a = (k < 4 ? mc.x : mc.y) >> (8 * (k & 3)) & 255u, b = (k < 4 ? vc.x : vc.y) >> (8 * (k & 3)) & 255u;
-      m[k] = __uint_as_float(__float_as_uint(value_of<4>(a & 127u, mu)) ^ (a & 128u) << 24);
-      v[k] = value_of<5>(b, vu);
-    }
+  for (int k = 0; k < 4; ++k) w[k] = make_float2(e[2 * k], e[2 * k + 1]);
+  unpack<8>(e, l.g, g_type);
+  if constexpr (EIGHT) {
+    decode_m(m, make_uint2(l.m.v[0], l.m.v[1]), unit_of(l.me));
+    decode_v(v, make_uint2(l.v.v[0], l.v.v[1]), unit_of(l.ve));
   } else {
-    load_some<W>(m, x.m, S3R_F32, at, x.n);
-    load_some<W>(v, x.v, S3R_F32, at, x.n);
-  }
-  // Every product and sum is rounded by itself, as in separate operations: codes do not depend on which of them the compiler
-  // would have fused.
-  float m_big = 0.f, v_big = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float gk = __fmul_rn(g[k], s.factor);
-    m[k] = __fadd_rn(__fmul_rn(m[k], p.b1), __fmul_rn(gk, p.c1));
-    v[k] = __fadd_rn(__fmul_rn(v[k], p.b2), __fmul_rn(__fmul_rn(gk, gk), p.c2));
-    w[k] = __fsub_rn(__fmul_rn(w[k], s.decay), __fmul_rn(s.step_size, __fdividef(m[k], __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), s.inv_root), p.eps))));
-    m_big = max_nan(m_big, fabsf(m[k]));
-    v_big = max_nan(v_big, v[k]);
+    for (int k = 0; k < 4; ++k) {
+      m[k] = make_float2(__uint_as_float(l.m.v[2 * k]), __uint_as_float(l.m.v[2 * k + 1]));
+      v[k] = make_float2(__uint_as_float(l.v.v[2 * k]), __uint_as_float(l.v.v[2 * k + 1]));
+    }
+  }
+  // Every product and sum of the states is rounded by itself, as in separate operations: codes do not depend on which of them would
+  // have been fused.  The parameter's own arithmetic is the approximate root and reciprocal (2^-23 of the step).
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 g = fmul2(make_float2(e[2 * k], e[2 * k + 1]), both_of(s.factor));
+    m[k] = add_apart(fmul2(m[k], both_of(p.b1)), fmul2(g, both_of(p.c1)));
+    v[k] = add_apart(fmul2(v[k], both_of(p.b2)), fmul2(fmul2(g, g), both_of(p.c2)));
+    const float2 root = ffma2(make_float2(sqrt_near(v[k].x), sqrt_near(v[k].y)), both_of(s.inv_root), both_of(p.eps));
+    const float2 step = fmul2(m[k], make_float2(rcp_near(root.x), rcp_near(root.y)));
+    w[k] = ffma2(w[k], both_of(s.decay), fmul2(step, both_of(-s.step_size)));
   }
   uint32_t low[8];
-  if (!nearest && (eight || p_type == S3R_BF16)) {
+  if (!nearest && (EIGHT || p_type == S3R_BF16)) {
     const uint32_t key = static_cast<uint32_t>(p.seed) + (x.flags >> 8) * 0x85EBCA6Bu;
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
@@ -200,40 +261,67 @@ __device__ __forceinline__ void adamw_block(const AdamParams& p, const AdamTenso
     // 10 bits of a bf16 parameter's 16; fp16's values below 2^-14 have fewer, so it is rounded to nearest
     if (p_type == S3R_BF16)
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (fabsf(w[k]) < 3.3e38f) w[k] = __uint_as_float((__float_as_uint(w[k]) + (low[k] >> 22) * 64u + 32u) & 0xffff0000u);
+      for (int k = 0; k < 4; ++k) {
+        if (fabsf(w[k].x) < 3.3e38f) w[k].x = __uint_as_float((__float_as_uint(w[k].x) + (low[2 * k] >> 22) * 64u + 32u) & 0xffff0000u);
+        if (fabsf(w[k].y) < 3.3e38f) w[k].y = __uint_as_float((__float_as_uint(w[k].y) + (low[2 * k + 1] >> 22) * 64u + 32u) & 0xffff0000u);
+      }
+  }
+  store_lane<W>(w, x.p, p_type, at, x.n);
+  if constexpr (!EIGHT) {
+    store_lane<W>(m, x.m, S3R_F32, at, x.n);
+    store_lane<W>(v, x.v, S3R_F32, at, x.n);
   } else {
+    // magnitudes compare as integers, NaN above all
+    uint32_t am[8], av[8], m_big = 0, v_big = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) low[k] = 0;
-  }
-  store_some<W>(w, x.p, p_type, at, x.n);
-  if (!eight) {
-    store_some<W>(m, x.m, S3R_F32, at, x.n);
-    store_some<W>(v, x.v, S3R_F32, at, x.n);
-    return;
-  }
+    for (int k = 0; k < 4; ++k) {
+      am[2 * k] = __float_as_uint(m[k].x) & 0x7fffffffu, am[2 * k + 1] = __float_as_uint(m[k].y) & 0x7fffffffu;
+      av[2 * k] = __float_as_uint(v[k].x) & 0x7fffffffu, av[2 * k + 1] = __float_as_uint(v[k].y) & 0x7fffffffu;
+      m_big = max(m_big, max(am[2 * k], am[2 * k + 1]));
+      v_big = max(v_big, max(av[2 * k], av[2 * k + 1]));
+    }
+    m_big = __reduce_max_sync(0xffffffffu, m_big);
+    v_big = __reduce_max_sync(0xffffffffu, v_big);
+    const uint32_t me = block_exponent(m_big), ve = block_exponent(v_big);
+    const float m_up = me == 255u ? 0.f : power_of(254u - me), v_up = ve == 255u ? 0.f : power_of(254u - ve);
+    uint32_t mc[8], vc[8];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    m_big = max_nan(m_big, __shfl_xor_sync(0xffffffffu, m_big, o));
-    v_big = max_nan(v_big, __shfl_xor_sync(0xffffffffu, v_big, o));
-  }
-  const uint32_t me = block_exponent(m_big), ve = block_exponent(v_big);
-  const float m_up = me == 255u ? 0.f : power_of(254u - me), v_up = ve == 255u ? 0.f : power_of(254u - ve);
-  uint32_t mc[2] = {0, 0}, vc[2] = {0, 0};
+    for (int k = 0; k < 8; k += 2) {
+      const float2 a = fmul2(fmul2(make_float2(__uint_as_float(am[k]), __uint_as_float(am[k + 1])), both_of(m_up)), both_of(kDownM));
+      const float2 b = fmul2(fmul2(make_float2(__uint_as_float(av[k]), __uint_as_float(av[k + 1])), both_of(v_up)), both_of(kDownV));
+      mc[k] = __float_as_uint(a.x), mc[k + 1] = __float_as_uint(a.y);
+      vc[k] = __float_as_uint(b.x), vc[k + 1] = __float_as_uint(b.y);
+    }
+    // 8 random bits of the 20 that a code of m drops, 14 of v's: v moves less in a step.  No code passes its largest one: the block's
+    // exponent is such that 1.875 times the power of two is reached exactly at most.
+    if (nearest) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    // 8 random bits of the 20 that a code of m drops, 14 of v's: v moves less in a step.  A v that is not zero keeps a code that
-    // is not: a denominator never becomes eps alone by rounding.
-    const uint32_t a = code_of<4>(fabsf(m[k]), m_up, (low[k] & 0xFFu) << 12 | 0x800u, nearest) | (m[k] < 0.f ? 128u : 0u);
-    const uint32_t b = max(code_of<5>(v[k], v_up, (low[k] >> 8 & 0x3FFFu) << 6 | 0x20u, nearest), v[k] > 0.f ? 1u : 0u);
-    mc[k / 4] |= a << (8 * (k & 3));
-    vc[k / 4] |= b << (8 * (k & 3));
-  }
-  store_codes<W>(me == 255u ? make_uint2(0, 0) : make_uint2(mc[0], mc[1]), static_cast<uint8_t*>(x.m), at, x.n);
-  store_codes<W>(ve == 255u ? make_uint2(0, 0) : make_uint2(vc[0], vc[1]), static_cast<uint8_t*>(x.v), at, x.n);
-  if (lane == 0) {
-    x.me[block] = static_cast<uint8_t>(me);
-    x.ve[block] = static_cast<uint8_t>(ve);
+      for (int k = 0; k < 8; ++k) {
+        mc[k] += 0x7FFFFu + (mc[k] >> 20 & 1u);
+        vc[k] += 0x7FFFFu + (vc[k] >> 20 & 1u);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mc[k] += (low[k] << 12 & 0xFF000u) + 0x800u;
+        vc[k] += (low[k] >> 2 & 0xFFFC0u) + 0x20u;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t sign = __float_as_uint(k & 1 ? m[k / 2].y : m[k / 2].x);
+      mc[k] = (mc[k] << 4 & 0x7f000000u) | (sign & ~0x7f000000u);          // only the top byte is used
+      // a v that is not zero keeps a code that is not: a denominator never becomes eps alone by rounding
+      vc[k] = max(vc[k], av[k] ? 1u << 20 : 0u) << 4;
+    }
+    const uint2 m_codes = make_uint2(gather(mc[0], mc[1], mc[2], mc[3]), gather(mc[4], mc[5], mc[6], mc[7]));
+    const uint2 v_codes = make_uint2(gather(vc[0], vc[1], vc[2], vc[3]), gather(vc[4], vc[5], vc[6], vc[7]));
+    store_codes<W>(me == 255u ? make_uint2(0, 0) : m_codes, static_cast<uint8_t*>(x.m), at, x.n);
+    store_codes<W>(ve == 255u ? make_uint2(0, 0) : v_codes, static_cast<uint8_t*>(x.v), at, x.n);
+    if (lane == 0) {
+      x.me[block] = static_cast<uint8_t>(me);
+      x.ve[block] = static_cast<uint8_t>(ve);
+    }
   }
 }
 
@@ -247,17 +335,32 @@ __device__ __forceinline__ int tensor_of(const AdamTensor* t, int n, int64_t cta
   return lo;
 }
 
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamParams p) {
-  const int i = tensor_of(p.t, p.n, blockIdx.x);
-  const AdamTensor& x = p.t[i];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t block = (blockIdx.x - x.first) * (kAdamThreads / 32) + warp;
+// A warp has one block.  What hides the latency of its loads is other warps: with 64 registers 32 of them fit an SM (227 M elements with
+// 8-bit states 750 us; with 80 registers 830, with 94 1025), and a loop over several blocks, with or without the next one on its way in
+// registers, lost more of them than it gained (1460 to 1830).
+template <bool EIGHT>
+__device__ __forceinline__ void run_block(const AdamParams& p, const AdamTensor& x, int64_t block, int lane) {
+  Lane<EIGHT> l;
+  // whole blocks of tensors that begin at multiples of 16 bytes; what ends a tensor, and tensors that begin anywhere, element by element
+  if ((x.flags & kAdamVector) && (block + 1) * kAdamBlock <= x.n) {
+    load_block<8, EIGHT>(l, x, block, lane);
+    const AdamScalars s = *p.scalars;
+    if (!s.skip) step_block<8, EIGHT>(l, p, x, s, block, lane);
+  } else {
+    load_block<1, EIGHT>(l, x, block, lane);
+    const AdamScalars s = *p.scalars;
+    if (!s.skip) step_block<1, EIGHT>(l, p, x, s, block, lane);
+  }
+}
+
+__global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_constant__ AdamParams p) {
+  const AdamTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
+  const int64_t block = (blockIdx.x - x.first) * kAdamWarps + (threadIdx.x >> 5);
   griddep_wait();
   griddep_launch();
-  const AdamScalars s = *p.scalars;
-  if (s.skip || block * kAdamBlock >= x.n) return;
-  if ((x.flags & kAdamVector) && (block + 1) * kAdamBlock <= x.n) adamw_block<8>(p, x, s, block, lane);
-  else adamw_block<1>(p, x, s, block, lane);
+  if (block * kAdamBlock >= x.n) return;
+  if (x.flags & kAdamEight) run_block<true>(p, x, block, threadIdx.x & 31);
+  else run_block<false>(p, x, block, threadIdx.x & 31);
 }
 
 // ---- the norm of the gradients: squares in 64 bits, where every one of them is exact ------------------------------------
@@ -356,26 +459,21 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_
   }
   const StateTensor& x = p.t[lo];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t block = (blockIdx.x - x.first) * (kAdamThreads / 32) + warp, at = block * kAdamBlock + lane * 8;
+  const int64_t block = (blockIdx.x - x.first) * kAdamWarps + warp, at = block * kAdamBlock + lane * 8;
   griddep_wait();
   griddep_launch();
   if (at >= x.n) return;
   const bool whole = (x.flags & kAdamVector) && at + 8 <= x.n;
   const uint2 mc = whole ? load_codes<8>(x.m, at, x.n) : load_codes<1>(x.m, at, x.n), vc = whole ? load_codes<8>(x.v, at, x.n) : load_codes<1>(x.v, at, x.n);
-  const float mu = unit_of(x.me[block]), vu = unit_of(x.ve[block]);
-  float m[8], v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t a = (k < 4 ? mc.x : mc.y) >> (8 * (k & 3)) & 255u, b = (k < 4 ? vc.x : vc.y) >> (8 * (k & 3)) & 255u;
-    m[k] = __uint_as_float(__float_as_uint(value_of<4>(a & 127u, mu)) ^ (a & 128u) << 24);
-    v[k] = value_of<5>(b, vu);
-  }
+  float2 m[4], v[4];
+  decode_m(m, mc, unit_of(x.me[block]));
+  decode_v(v, vc, unit_of(x.ve[block]));
   if (whole) {
-    store_some<8>(m, x.m_out, S3R_F32, at, x.n);
-    store_some<8>(v, x.v_out, S3R_F32, at, x.n);
+    store_lane<8>(m, x.m_out, S3R_F32, at, x.n);
+    store_lane<8>(v, x.v_out, S3R_F32, at, x.n);
   } else {
-    store_some<1>(m, x.m_out, S3R_F32, at, x.n);
-    store_some<1>(v, x.v_out, S3R_F32, at, x.n);
+    store_lane<1>(m, x.m_out, S3R_F32, at, x.n);
+    store_lane<1>(v, x.v_out, S3R_F32, at, x.n);
   }
 }
 

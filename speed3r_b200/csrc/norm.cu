@@ -15,6 +15,7 @@ struct NormParams {
   s3r_residual_norm a;
   int64_t rows;
   float inv_n;
+  int stages;                  // rows on their way (norm_rows_kernel)
 };
 
 __device__ __forceinline__ float gate_of_row(const s3r_residual_norm& a, int64_t row) {
@@ -23,17 +24,61 @@ __device__ __forceinline__ float gate_of_row(const s3r_residual_norm& a, int64_t
   return load_one(a.gate, a.gate_type, b * a.gate_stride_b + (static_cast<uint32_t>(row) - b * tokens) * a.gate_stride_t);
 }
 
+constexpr int kNormSmem = 220 * 1024;
+
+template <int W>
+__device__ __forceinline__ void stage_vector(uint32_t dst, const void* p, int type, int64_t i) {
+  const char* src = static_cast<const char*>(p) + i * type_bytes(type);
+  if constexpr (W == 8) {
+    cp_async16(dst, src);
+    if (type == S3R_F32) cp_async16(dst + 16, src + 16);
+  } else {
+    if (type == S3R_F32) cp_async16(dst, src);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  }
+}
+template <int W>
+__device__ __forceinline__ void staged_raw(Raw<W>& r, const char* s, int type) {
+  const uint32_t at = smem_u32(s);
+  const int wide = type == S3R_F32;
+  if constexpr (W == 8)
+    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %9, 0;\n\t"
+                 "ld.shared.v4.b32 {%0, %1, %2, %3}, [%8];\n\t@b ld.shared.v4.b32 {%4, %5, %6, %7}, [%8 + 16];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7]) : "r"(at), "r"(wide) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %5, 0;\n\t"
+                 "ld.shared.v2.b32 {%0, %1}, [%4];\n\t@b ld.shared.v2.b32 {%2, %3}, [%4 + 8];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "r"(at), "r"(wide) : "memory");
+}
+
+// a vector's place in shared memory
+template <int W>
+__device__ __forceinline__ void zero_place(char* at, int bytes) {
+#pragma unroll
+  for (int k = 0; k < W; k += 2) {
+    *reinterpret_cast<uint32_t*>(at + 2 * k) = 0;
+    if (bytes == 4) *reinterpret_cast<uint32_t*>(at + 2 * W + 2 * k) = 0;
+  }
+}
+__device__ __forceinline__ void cp_async_wait_for(int pending) {
+  if (pending >= 3) cp_async_wait<3>();
+  else if (pending == 2) cp_async_wait<2>();
+  else if (pending == 1) cp_async_wait<1>();
+  else cp_async_wait<0>();
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: G threads per row, E elements per thread in registers (vectors of W); the variance from the centred values
 // ---------------------------------------------------------------------------------------------------------------------
 template <int W, int G, int E>
-__device__ __forceinline__ float2 row_statistics(const float (&v)[E], int kind, int channels, float inv_n, float eps, float* red, uint32_t& turn, int t) {
+__device__ __forceinline__ float2 row_statistics(const float (&v)[E], int kind, int channels, float inv_n, float eps, float* red, uint32_t& turn, int t,
+                                                 int bar = 0) {
   float s[1] = {0.f};
   float mean = 0.f;
   if (kind == S3R_NORM_LAYER) {
 #pragma unroll
     for (int k = 0; k < E; ++k) s[0] += v[k];            // places behind the row hold 0
-    row_sum<G>(s, red, turn, t, 0);
+    row_sum<G>(s, red, turn, t, bar);
     mean = s[0] * inv_n;
   }
   s[0] = 0.f;
@@ -45,25 +90,81 @@ __device__ __forceinline__ float2 row_statistics(const float (&v)[E], int kind, 
         const float d = v[i * W + k] - mean;
         s[0] = fmaf(d, d, s[0]);
       }
-  row_sum<G>(s, red, turn, t, 0);
+  row_sum<G>(s, red, turn, t, bar);
   return make_float2(mean, rsqrtf(fmaf(s[0], inv_n, eps)));
 }
 
+// A thread's places of `channels` elements from element `from` on, asked for.  Single elements (rows of odd width) in one branch on the
+// type: their addresses are then one register and constants, where predicates took one each.
+template <int W, int G, int N>
+__device__ __forceinline__ void request_all(Raw<W> (&r)[N], const void* p, int type, int64_t from, int channels, int t, bool there = true) {
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) load_raw<W>(r[i], p, type, from + (i * G + t) * W, there && p && (i * G + t) * W < channels);
+  } else if (there && p) {
+    if (type == S3R_F32) {
+      const uint32_t* q = static_cast<const uint32_t*>(p) + from + t;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * G + t < channels) r[i].v[0] = __ldg(q + i * G);
+    } else {
+      const uint16_t* q = static_cast<const uint16_t*>(p) + from + t;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * G + t < channels) r[i].v[0] = __ldg(q + i * G);
+    }
+  }
+}
+// [channels] parameters of a thread's places
+template <int W, int G, int N>
+__device__ __forceinline__ void load_params(float (&f)[W * N], const void* p, int type, int64_t from, int channels, int t) {
+  Raw<W> r[N];
+  request_all<W, G, N>(r, p, type, from, channels, t);
+  unpack_all<W, N>(f, r, type, [](int) { return true; });
+}
+
+template <int W, int N>
+__device__ __forceinline__ void apply_norm(float (&v)[W * N], float2 st, const void* weight, const Raw<W> (&w)[N], const void* bias, const Raw<W> (&b)[N],
+                                           int type) {
+  float p[W * N];
+  const auto all = [](int) { return true; };
+#pragma unroll
+  for (int k = 0; k < W * N; ++k) v[k] = (v[k] - st.x) * st.y;
+  if (weight) {
+    unpack_all<W, N>(p, w, type, all);
+#pragma unroll
+    for (int k = 0; k < W * N; ++k) v[k] *= p[k];
+  }
+  if (bias) {
+    unpack_all<W, N>(p, b, type, all);
+#pragma unroll
+    for (int k = 0; k < W * N; ++k) v[k] += p[k];
+  }
+}
+
+// the row as 8-bit tokens
 template <int W, int G, int E>
-__device__ __forceinline__ void apply_norm(float (&v)[E], float2 st, const void* weight, const void* bias, int type, int channels, int t) {
+__device__ __forceinline__ void store_int8(const float (&v)[E], const s3r_residual_norm& a, int64_t row, float* red, uint32_t& turn, int t, int bar) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < E / W; ++i)
+    if ((i * G + t) * W < a.channels)
+#pragma unroll
+      for (int k = 0; k < W; ++k) big = max_nan(big, fabsf(v[i * W + k]));
+  big = row_max<G>(big, red, turn, t, bar);
+  const RowScale s = row_scale(big);
+  if (t == 0) a.q_scale[row] = s.scale;
 #pragma unroll
   for (int i = 0; i < E / W; ++i) {
-    const int c = (i * G + t) * W;
-    if (c < channels) {
-      float w[W], b[W];
-      if (weight) load_vector<W>(w, weight, type, c);
-      if (bias) load_vector<W>(b, bias, type, c);
+    if ((i * G + t) * W < a.channels) {
+      int8_t* q = a.q + row * a.q_pitch + (i * G + t) * W;
+      if constexpr (W == 1) {
+        *q = static_cast<int8_t>(to_s8(v[i], s.inverse));
+      } else {
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        float x = (v[i * W + k] - st.x) * st.y;
-        if (weight) x *= w[k];
-        if (bias) x += b[k];
-        v[i * W + k] = x;
+        for (int k = 0; k < W; k += 4)
+          *reinterpret_cast<uint32_t*>(q + k) = to_s8(v[i * W + k], s.inverse) | to_s8(v[i * W + k + 1], s.inverse) << 8 |
+                                                to_s8(v[i * W + k + 2], s.inverse) << 16 | to_s8(v[i * W + k + 3], s.inverse) << 24;
       }
     }
   }
@@ -81,115 +182,224 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fwd_kernel(const __gri
   if (row >= p.rows) return;                              // whole rows leave (rows of several warps have a CTA each)
   const int64_t at = row * C;
   uint32_t turn = 0;
-  Raw<W> xr[N], yr[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * W;
-    if (c < C) {
-      load_raw<W>(xr[i], a.x, a.x_type, at + c);
-      if (a.y) load_raw<W>(yr[i], a.y, a.y_type, at + c);
-    }
-  }
-  float v[E];
+  auto in = [&](int i) { return (i * G + t) * W < C; };
+  auto place = [&](int i) { return in(i) ? at + (i * G + t) * W : int64_t{-1}; };
+  Raw<W> xr[N], yr[N], sr[N], gr[N], wr[N], br[N];
+  request_all<W, G, N>(xr, a.x, a.x_type, at, C, t);
+  request_all<W, G, N>(yr, a.y, a.y_type, at, C, t);
+  request_all<W, G, N>(sr, a.scale, a.param_type, 0, C, t);
+  float v[E], f[E];
   if (a.y) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float f[W];
-      unpack<W>(f, yr[i], a.y_type);
-#pragma unroll
-      for (int k = 0; k < W; ++k) v[i * W + k] = (i * G + t) * W < C ? f[k] : 0.f;
-    }
+    unpack_all<W, N>(v, yr, a.y_type, in);
     if (a.post) {
       const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.post_eps, red, turn, t);
       if (a.stats && t == 0) a.stats[2 * p.rows + row] = st.x, a.stats[3 * p.rows + row] = st.y;
-      apply_norm<W, G, E>(v, st, a.post_weight, a.post_bias, a.param_type, C, t);
+      request_all<W, G, N>(wr, a.post_weight, a.param_type, 0, C, t);
+      request_all<W, G, N>(br, a.post_bias, a.param_type, 0, C, t);
+      apply_norm<W, N>(v, st, a.post_weight, wr, a.post_bias, br, a.param_type);
     }
-    const float gate = gate_of_row(a, row);
-    const int64_t gate_at = a.gate_mode == S3R_GATE_CHANNEL ? row / a.tokens * a.gate_stride_b : 0;
+    if (a.scale) {
+      unpack_all<W, N>(f, sr, a.param_type, [](int) { return true; });
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * G + t) * W;
-      if (c < C) {
-        float f[W];
-        if (a.scale) {
-          load_vector<W>(f, a.scale, a.param_type, c);
-#pragma unroll
-          for (int k = 0; k < W; ++k) v[i * W + k] = __fmul_rn(v[i * W + k], f[k]);
-        }
-        if (a.gate_mode == S3R_GATE_CHANNEL) {
-          load_vector<W>(f, a.gate, a.gate_type, gate_at + c);
-#pragma unroll
-          for (int k = 0; k < W; ++k) v[i * W + k] = __fmul_rn(v[i * W + k], f[k]);
-        } else if (a.gate_mode == S3R_GATE_ROW) {
-#pragma unroll
-          for (int k = 0; k < W; ++k) v[i * W + k] = __fmul_rn(v[i * W + k], gate);
-        }
-        unpack<W>(f, xr[i], a.x_type);
-#pragma unroll
-        for (int k = 0; k < W; ++k) f[k] = __fadd_rn(f[k], v[i * W + k]);
-        // the norm is that of the stored sum, as it is for whoever reads it later, the backward among them
-        Raw<W> o;
-        pack<W>(o, f, a.x_type);
-        store_raw<W>(o, a.r, a.x_type, at + c);
-        unpack<W>(f, o, a.x_type);
-#pragma unroll
-        for (int k = 0; k < W; ++k) v[i * W + k] = f[k];
-      }
+      for (int k = 0; k < E; ++k) v[k] = __fmul_rn(v[k], f[k]);
     }
+    if (a.gate_mode == S3R_GATE_CHANNEL) {
+      request_all<W, G, N>(gr, a.gate, a.gate_type, static_cast<uint32_t>(row) / static_cast<uint32_t>(a.tokens) * a.gate_stride_b, C, t);
+      unpack_all<W, N>(f, gr, a.gate_type, [](int) { return true; });
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] = __fmul_rn(v[k], f[k]);
+    } else if (a.gate_mode == S3R_GATE_ROW) {
+      const float gate = gate_of_row(a, row);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] = __fmul_rn(v[k], gate);
+    }
+    unpack_all<W, N>(f, xr, a.x_type, in);
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] = __fadd_rn(f[k], v[k]);
+    // the norm is that of the stored sum, as it is for whoever reads it later, the backward among them
+    store_all<W, N>(v, a.r, a.x_type, place, true);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!in(i))
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[i * W + k] = 0.f;
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * G + t) * W;
-      float f[W];
-      unpack<W>(f, xr[i], a.x_type);
-#pragma unroll
-      for (int k = 0; k < W; ++k) v[i * W + k] = c < C ? f[k] : 0.f;
-      if (a.r && c < C) store_raw<W>(xr[i], a.r, a.x_type, at + c);
-    }
+    unpack_all<W, N>(v, xr, a.x_type, in);
+    if (a.r) store_all<W, N>(v, a.r, a.x_type, place);
   }
   if (!a.h && !a.q) return;
   const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.eps, red, turn, t);
   if (a.stats && t == 0) a.stats[row] = st.x, a.stats[p.rows + row] = st.y;
-  apply_norm<W, G, E>(v, st, a.weight, a.bias, a.param_type, C, t);
+  request_all<W, G, N>(wr, a.weight, a.param_type, 0, C, t);
+  request_all<W, G, N>(br, a.bias, a.param_type, 0, C, t);
+  apply_norm<W, N>(v, st, a.weight, wr, a.bias, br, a.param_type);
   if (a.h) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * G + t) * W;
-      if (c < C) {
-        float f[W];
-#pragma unroll
-        for (int k = 0; k < W; ++k) f[k] = v[i * W + k];
-        Raw<W> o;
-        pack<W>(o, f, a.h_type);
-        store_raw<W>(o, a.h, a.h_type, at + c);
-      }
-    }
+    store_all<W, N>(v, a.h, a.h_type, place);
     return;
   }
-  float big = 0.f;
+  store_int8<W, G, E>(v, a, row, red, turn, t, 0);
+}
+
+// CTAs per SM.  An fp32 sum: 512 threads and 128 registers (64 512 x 1024 122 us; 768 threads of 80 registers 149, 512 such 156).  16 bits:
+// 768 threads, a row's bytes are fewer and its arithmetic the same (94 us, with 512 101).
+__host__ __device__ constexpr int rows_resident(int G, bool full, bool wide) { return G > 256 ? 1 : (full || wide || G < 128 ? 512 : 768) / (G < 128 ? 128 : G); }
+// The same for many rows: CTAs stay, take every gridDim-th row, keep the parameters in registers and have the next rows on their way into
+// shared memory (cp.async, each thread its own bytes, so that no barrier orders them).  With a CTA per row a row cost 2 ns whatever its
+// bytes, the time it takes to start, wait for three loads one behind the other and end.
+template <int W, int G, int E, bool FULL, bool WIDE>
+__global__ void __launch_bounds__(G < 128 ? 128 : G, rows_resident(G, FULL, WIDE)) norm_rows_kernel(const __grid_constant__ NormParams p) {
+  constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, N = E / W, P = E / 2;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red_all[kRows][G > 32 ? 8 * (G / 32) : 1];
+  griddep_wait();
+  griddep_launch();
+  const s3r_residual_norm& a = p.a;
+  const int t = threadIdx.x % G, group = threadIdx.x / G, C = a.channels, rows = static_cast<int>(p.rows);
+  const int step = static_cast<int>(gridDim.x) * kRows, first = static_cast<int>(blockIdx.x) * kRows + group, bar = group + 1;
+  float* red = red_all[group];
+  uint32_t turn = 0;
+  auto in = [&](int i) { return (i * G + t) * W < C; };
+  const int xb = type_bytes(a.x_type), yb = type_bytes(a.y_type);
+  const uint32_t at_y = G * E * xb, stage_bytes = at_y + G * E * yb;
+  char* ring = smem + static_cast<size_t>(group) * p.stages * stage_bytes;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if ((i * G + t) * W < C)
+    if (!in(i))
+      for (int s = 0; s < p.stages; ++s) {
+        zero_place<W>(ring + s * stage_bytes + (i * G + t) * W * xb, xb);
+        zero_place<W>(ring + s * stage_bytes + at_y + (i * G + t) * W * yb, yb);
+      }
+  auto request = [&](int row, int stage) {
+    if (row < rows) {
+      const uint32_t to = smem_u32(ring) + stage * stage_bytes;
 #pragma unroll
-      for (int k = 0; k < W; ++k) big = max_nan(big, fabsf(v[i * W + k]));
-  big = row_max<G>(big, red, turn, t, 0);
-  const RowScale s = row_scale(big);
-  if (t == 0) a.q_scale[row] = s.scale;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * W;
-    if (c < C) {
-      int8_t* q = a.q + row * a.q_pitch + c;
-      if constexpr (W == 1) {
-        *q = static_cast<int8_t>(to_s8(v[i], s.inverse));
-      } else {
-#pragma unroll
-        for (int k = 0; k < W; k += 4)
-          *reinterpret_cast<uint32_t*>(q + k) = to_s8(v[i * W + k], s.inverse) | to_s8(v[i * W + k + 1], s.inverse) << 8 |
-                                                to_s8(v[i * W + k + 2], s.inverse) << 16 | to_s8(v[i * W + k + 3], s.inverse) << 24;
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * G + t) * W;
+        const int64_t at = static_cast<int64_t>(row) * C + c;
+        if (c < C) {
+          stage_vector<W>(to + c * xb, a.x, a.x_type, at);
+          if (a.y) stage_vector<W>(to + at_y + c * yb, a.y, a.y_type, at);
+        }
       }
     }
+    cp_async_commit();
+  };
+  float2 w[P], b[P], scale[P], pw[FULL ? P : 1], pb[FULL ? P : 1];
+  auto param = [&](float2* to, const void* from, int type, int64_t at, float other) {
+    float v[E];
+    if (from) load_params<W, G, N>(v, from, type, at, C, t);
+#pragma unroll
+    for (int k = 0; k < P; ++k) to[k] = !in(2 * k / W) ? make_float2(0.f, 0.f) : from ? make_float2(v[2 * k], v[2 * k + 1]) : make_float2(other, other);
+  };
+  for (int s = 0; s + 1 < p.stages; ++s) request(first + s * step, s);
+  param(w, a.weight, a.param_type, 0, 1.f);
+  param(b, a.bias, a.param_type, 0, 0.f);
+  param(scale, a.scale, a.param_type, 0, 1.f);
+  if constexpr (FULL) {
+    param(pw, a.post_weight, a.param_type, 0, 1.f);
+    param(pb, a.post_bias, a.param_type, 0, 0.f);
   }
+  auto both = [](float x) { return make_float2(x, x); };
+  // (mean, 1 / sqrt(..)); values behind the end of the row are 0
+  auto statistics = [&](const float2 (&v)[P], float eps) {
+    float sum[1] = {0.f};
+    float2 s = both(0.f);
+    float mean = 0.f;
+    if (a.kind == S3R_NORM_LAYER) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) s = fadd2(s, v[k]);
+      sum[0] = s.x + s.y;
+      row_sum<G>(sum, red, turn, t, bar);
+      mean = sum[0] * p.inv_n;
+      s = both(0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in(i))
+#pragma unroll
+        for (int k = 0; k < W / 2; ++k) {
+          const float2 d = fadd2(v[i * (W / 2) + k], both(-mean));
+          s = ffma2(d, d, s);
+        }
+    sum[0] = s.x + s.y;
+    row_sum<G>(sum, red, turn, t, bar);
+    return make_float2(mean, rsqrtf(fmaf(sum[0], p.inv_n, eps)));
+  };
+  int stage = 0;
+  for (int row = first; row < rows; row += step) {
+    request(row + (p.stages - 1) * step, stage + p.stages - 1 >= p.stages ? stage - 1 : p.stages - 1);
+    const float gate = gate_of_row(a, row);
+    cp_async_wait_for(p.stages - 1);
+    const char* here = ring + stage * stage_bytes;
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
+    auto place = [&](int i) { return in(i) ? static_cast<int64_t>(row) * C + (i * G + t) * W : int64_t{-1}; };
+    auto fetch = [&](float2 (&v)[P], uint32_t at, int type) {
+      Raw<W> r[N];
+      float e[E];
+#pragma unroll
+      for (int i = 0; i < N; ++i) staged_raw<W>(r[i], here + at + (i * G + t) * W * type_bytes(type), type);
+      unpack_all<W, N>(e, r, type, [](int) { return true; });
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
+    };
+    auto put = [&](float2 (&v)[P], void* to, int type, bool back) {
+      float e[E];
+#pragma unroll
+      for (int k = 0; k < P; ++k) e[2 * k] = v[k].x, e[2 * k + 1] = v[k].y;
+      store_all<W, N>(e, to, type, place, back);
+      if (back)
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
+    };
+    float2 v[P], f[P];
+    if (a.y) {
+      fetch(v, at_y, a.y_type);
+      if constexpr (FULL) {
+        if (a.post) {
+          const float2 st = statistics(v, a.post_eps);
+          if (a.stats && t == 0) a.stats[2 * p.rows + row] = st.x, a.stats[3 * p.rows + row] = st.y;
+#pragma unroll
+          for (int k = 0; k < P; ++k) v[k] = ffma2(fmul2(fadd2(v[k], both(-st.x)), both(st.y)), pw[k], pb[k]);
+        }
+      }
+      // products and sum are rounded one by one, as in separate operations (norm_fwd_kernel's r, bit for bit)
+      if (a.scale)
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[k] = fmul2(v[k], scale[k]);
+      if (a.gate_mode == S3R_GATE_ROW) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[k] = fmul2(v[k], both(gate));
+      }
+      if constexpr (FULL) {
+        if (a.gate_mode == S3R_GATE_CHANNEL) {
+          param(f, a.gate, a.gate_type, static_cast<uint32_t>(row) / static_cast<uint32_t>(a.tokens) * a.gate_stride_b, 1.f);
+#pragma unroll
+          for (int k = 0; k < P; ++k) v[k] = fmul2(v[k], f[k]);
+        }
+      }
+      fetch(f, 0, a.x_type);
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = add_apart(f[k], v[k]);
+      put(v, a.r, a.x_type, true);
+    } else {
+      fetch(v, 0, a.x_type);
+      if (a.r) put(v, a.r, a.x_type, false);
+    }
+    if (!a.h && !a.q) continue;
+    const float2 st = statistics(v, a.eps);
+    if (a.stats && t == 0) a.stats[row] = st.x, a.stats[p.rows + row] = st.y;
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = ffma2(fmul2(fadd2(v[k], both(-st.x)), both(st.y)), w[k], b[k]);
+    if (a.h) {
+      put(v, a.h, a.h_type, false);
+    } else {
+      float e[E];
+#pragma unroll
+      for (int k = 0; k < P; ++k) e[2 * k] = v[k].x, e[2 * k + 1] = v[k].y;
+      store_int8<W, G, E>(e, a, row, red, turn, t, bar);
+    }
+  }
+  cp_async_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -211,50 +421,10 @@ struct NormBwdParams {
   float* partial;              // [batch entries x slices, kSums, channels], the sums that are wanted
 };
 
-template <int W>
-__device__ __forceinline__ void stage_vector(uint32_t dst, const void* p, int type, int64_t i) {
-  const char* src = static_cast<const char*>(p) + i * type_bytes(type);
-  if constexpr (W == 8) {
-    cp_async16(dst, src);
-    if (type == S3R_F32) cp_async16(dst + 16, src + 16);
-  } else {
-    if (type == S3R_F32) cp_async16(dst, src);
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-  }
-}
-template <int W>
-__device__ __forceinline__ void staged(float (&f)[W], const char* s, int type) {
-  Raw<W> r;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(s);
-  if (type == S3R_F32) {
-#pragma unroll
-    for (int k = 0; k < W; k += 4) {
-      const uint4 u = *reinterpret_cast<const uint4*>(q + k);
-      r.v[k] = u.x, r.v[k + 1] = u.y, r.v[k + 2] = u.z, r.v[k + 3] = u.w;
-    }
-  } else if constexpr (W == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(q);
-    r.v[0] = u.x, r.v[1] = u.y, r.v[2] = u.z, r.v[3] = u.w;
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(q);
-    r.v[0] = u.x, r.v[1] = u.y;
-  }
-  unpack<W>(f, r, type);
-}
-
-__device__ __forceinline__ void cp_async_wait_for(int pending) {
-  if (pending >= 3) cp_async_wait<3>();
-  else if (pending == 2) cp_async_wait<2>();
-  else if (pending == 1) cp_async_wait<1>();
-  else cp_async_wait<0>();
-}
-
-constexpr int kNormSmem = 220 * 1024;
-
 // FULL: a post norm or a gate per channel too; without them their sums and factors take no registers
 template <int W, int G, int E, bool FULL>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
-  constexpr int kRows = G < 128 ? 128 / G : 1, N = E / W;
+  constexpr int kRows = G < 128 ? 128 / G : 1, N = E / W, P = E / 2, F = FULL ? P : 1;
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[kRows][G > 32 ? 8 * (G / 32) : 1];
   griddep_wait();
@@ -263,222 +433,252 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(const __gri
   const s3r_residual_norm_grad& g = p.g;
   const int t = threadIdx.x % G, group = threadIdx.x / G, C = f.channels;
   const int entry = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
-  const int64_t first = entry * p.span + p.span * slice / p.slices, last = entry * p.span + p.span * (slice + 1) / p.slices;
-  const bool layer = f.kind == S3R_NORM_LAYER, branch = f.y != nullptr;
-  const bool norm = g.dh != nullptr;
+  const int first = static_cast<int>(entry * p.span + p.span * slice / p.slices), last = static_cast<int>(entry * p.span + p.span * (slice + 1) / p.slices);
+  const bool layer = f.kind == S3R_NORM_LAYER, branch = f.y != nullptr, norm = g.dh != nullptr, wants_gate = g.d_gate_row != nullptr;
+  const bool reads_y = branch && (f.post || g.d_scale || g.d_gate_row || g.d_gate_channel);
   char* ring = smem + static_cast<size_t>(group) * p.stages * p.stage_bytes;
   uint32_t turn = 0;
+  auto in = [&](int i) { return (i * G + t) * W < C; };
 
-  float w[E], scale[E], gate_c[FULL ? E : 1], pw[FULL ? E : 1], pb[FULL ? E : 1];
-  float d_w[E], d_b[E], d_s[E], d_g[FULL ? E : 1], d_pw[FULL ? E : 1], d_pb[FULL ? E : 1];
+  float2 w[P], scale[P], gate_c[F], pw[F], pb[F];
+  float2 d_w[P], d_b[P], d_s[P], d_g[F], d_pw[F], d_pb[F];
+  auto param = [&](float2* to, const void* from, int type, int64_t at, float other) {
+    float v[E];
+    if (from) {
+      load_params<W, G, N>(v, from, type, at, C, t);
+    } else {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = (i * G + t) * W;
-    float one[W], zero[W];
-#pragma unroll
-    for (int k = 0; k < W; ++k) one[k] = 1.f, zero[k] = 0.f;
-    auto fetch = [&](float* to, const void* from, int type, int64_t at, const float* other) {
-      float v[W];
-      if (from && c < C) load_vector<W>(v, from, type, at + c);
-#pragma unroll
-      for (int k = 0; k < W; ++k) to[i * W + k] = from && c < C ? v[k] : other[k];
-    };
-    fetch(w, f.weight, f.param_type, 0, one);
-    fetch(scale, f.scale, f.param_type, 0, one);
-    if constexpr (FULL) {
-      fetch(gate_c, f.gate_mode == S3R_GATE_CHANNEL ? f.gate : nullptr, f.gate_type, entry * f.gate_stride_b, one);
-      fetch(pw, f.post_weight, f.param_type, 0, one);
-      fetch(pb, f.post_bias, f.param_type, 0, zero);
+      for (int k = 0; k < E; ++k) v[k] = other;
     }
-  }
 #pragma unroll
-  for (int k = 0; k < E; ++k) {
-    d_w[k] = d_b[k] = d_s[k] = 0.f;
-    if constexpr (FULL) d_g[k] = d_pw[k] = d_pb[k] = 0.f;
+    for (int k = 0; k < P; ++k) to[k] = in(2 * k / W) ? make_float2(v[2 * k], W == 1 && !in(2 * k + 1) ? 0.f : v[2 * k + 1]) : make_float2(0.f, 0.f);
+  };
+  param(w, f.weight, f.param_type, 0, 1.f);
+  param(scale, f.scale, f.param_type, 0, 1.f);
+  if constexpr (FULL) {
+    param(gate_c, f.gate_mode == S3R_GATE_CHANNEL ? f.gate : nullptr, f.gate_type, entry * f.gate_stride_b, 1.f);
+    param(pw, f.post_weight, f.param_type, 0, 1.f);
+    param(pb, f.post_bias, f.param_type, 0, 0.f);
+  }
+  const float2 nil = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    d_w[k] = d_b[k] = d_s[k] = nil;
+    if constexpr (FULL) d_g[k] = d_pw[k] = d_pb[k] = nil;
   }
 
-  const bool reads_r = norm, reads_y = branch && (f.post || g.d_scale || g.d_gate_row || g.d_gate_channel);
-  auto request = [&](int64_t row, int stage) {
+  // Places behind the end of a row: zeros that no copy overwrites, so that nothing has to be masked out further down (their
+  // factors are 0 as well).
+  const int xb = type_bytes(f.x_type), yb = type_bytes(f.y_type), hb = type_bytes(f.h_type);
+  if constexpr (W > 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!in(i))
+        for (int s = 0; s < p.stages; ++s) {
+          char* to = ring + s * p.stage_bytes;
+          const int c = (i * G + t) * W;
+          zero_place<W>(to + c * xb, xb);
+          zero_place<W>(to + p.at_y + c * yb, yb);
+          zero_place<W>(to + p.at_dr + c * xb, xb);
+          zero_place<W>(to + p.at_dh + c * hb, hb);
+        }
+
+  auto request = [&](int row, int stage) {
     if constexpr (W > 1) {
       if (row < last) {
         const uint32_t to = smem_u32(ring) + stage * p.stage_bytes;
-        const int64_t at = row * C;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int c = (i * G + t) * W;
+          const int64_t at = static_cast<int64_t>(row) * C + c;
           if (c < C) {
-            if (reads_r) stage_vector<W>(to + c * type_bytes(f.x_type), f.r, f.x_type, at + c);
-            if (reads_y) stage_vector<W>(to + p.at_y + c * type_bytes(f.y_type), f.y, f.y_type, at + c);
-            if (g.dr) stage_vector<W>(to + p.at_dr + c * type_bytes(f.x_type), g.dr, f.x_type, at + c);
-            if (g.dh) stage_vector<W>(to + p.at_dh + c * type_bytes(f.h_type), g.dh, f.h_type, at + c);
+            if (norm) stage_vector<W>(to + c * xb, f.r, f.x_type, at);
+            if (reads_y) stage_vector<W>(to + p.at_y + c * yb, f.y, f.y_type, at);
+            if (g.dr) stage_vector<W>(to + p.at_dr + c * xb, g.dr, f.x_type, at);
+            if (norm) stage_vector<W>(to + p.at_dh + c * hb, g.dh, f.h_type, at);
           }
         }
       }
       cp_async_commit();
     }
   };
-  // a vector of the present row: where it was staged, or from memory (rows of odd width)
-  auto fetch = [&](float (&v)[W], const char* stage, uint32_t at, const void* from, int type, int64_t row, int c) {
-    if constexpr (W > 1) staged<W>(v, stage + at + c * type_bytes(type), type);
-    else load_vector<W>(v, from, type, row * C + c);
+  // rows of odd width: one element at a time, a row ahead in registers
+  constexpr int M = W == 1 ? N : 1;
+  Raw<1> odd[4][M];
+  auto request_odd = [&](int row) {
+    if constexpr (W == 1) {
+      const int64_t at = static_cast<int64_t>(row) * C;
+      const bool there = row < last;
+      request_all<1, G, N>(odd[0], f.r, f.x_type, at, C, t, there && norm);
+      request_all<1, G, N>(odd[1], f.y, f.y_type, at, C, t, there && reads_y);
+      request_all<1, G, N>(odd[2], g.dr, f.x_type, at, C, t, there);
+      request_all<1, G, N>(odd[3], g.dh, f.h_type, at, C, t, there);
+    }
+  };
+  // a thread's values of the present row, in pairs
+  auto fetch = [&](float2 (&v)[P], const char* staged_at, int which, int type) {
+    float e[E];
+    if constexpr (W > 1) {
+      Raw<W> r[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) staged_raw<W>(r[i], staged_at + (i * G + t) * W * type_bytes(type), type);
+      unpack_all<W, N>(e, r, type, [](int) { return true; });
+    } else {
+      unpack_all<W, N>(e, odd[which], type, in);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
+  };
+  auto put = [&](float2 (&v)[P], void* to, int type, int row) {
+    float e[E];
+#pragma unroll
+    for (int k = 0; k < P; ++k) e[2 * k] = v[k].x, e[2 * k + 1] = v[k].y;
+    store_all<W, N>(e, to, type, [&](int i) { return in(i) ? static_cast<int64_t>(row) * C + (i * G + t) * W : int64_t{-1}; });
+  };
+  auto both = [](float x) { return make_float2(x, x); };
+  // a row's mean, 1 / sqrt(..), those of the post norm, and its gate, a row ahead
+  float ahead[5];
+  auto scalars = [&](int row) {
+    const int r = row < last ? row : last - 1;
+    ahead[0] = norm ? __ldg(f.stats + r) : 0.f;
+    ahead[1] = norm ? __ldg(f.stats + p.rows + r) : 0.f;
+    ahead[2] = FULL && f.post ? __ldg(f.stats + 2 * p.rows + r) : 0.f;
+    ahead[3] = FULL && f.post ? __ldg(f.stats + 3 * p.rows + r) : 0.f;
+    ahead[4] = gate_of_row(f, r);
   };
 
   int stage = 0;
-  for (int s = 0; s + 1 < p.stages; ++s) request(first + group + static_cast<int64_t>(s) * kRows, s);
-  for (int64_t row = first + group; row < last; row += kRows) {
-    request(row + static_cast<int64_t>(p.stages - 1) * kRows, stage + p.stages - 1 >= p.stages ? stage - 1 : p.stages - 1);
-    float mean = 0.f, inv = 0.f, p_mean = 0.f, p_inv = 0.f;
-    if (norm) mean = __ldg(f.stats + row), inv = __ldg(f.stats + p.rows + row);
-    if (FULL && f.post) p_mean = __ldg(f.stats + 2 * p.rows + row), p_inv = __ldg(f.stats + 3 * p.rows + row);
-    const float gate = gate_of_row(f, row);
+  for (int s = 0; s + 1 < p.stages; ++s) request(first + group + s * kRows, s);
+  if (first + group < last) {
+    scalars(first + group);
+    request_odd(first + group);
+  }
+  for (int row = first + group; row < last; row += kRows) {
+    request(row + (p.stages - 1) * kRows, stage + p.stages - 1 >= p.stages ? stage - 1 : p.stages - 1);
+    const float mean = ahead[0], inv = ahead[1], p_mean = ahead[2], p_inv = ahead[3], gate = ahead[4];
+    scalars(row + kRows);
     if constexpr (W > 1) cp_async_wait_for(p.stages - 1);
     const char* here = ring + stage * p.stage_bytes;
     stage = stage + 1 == p.stages ? 0 : stage + 1;
 
-    float xh[E], d[E], s[3] = {0.f, 0.f, 0.f};
+    float2 xh[P], d[P];
     if (norm) {
+      float2 dh[P], s0 = nil, s1 = nil;
+      fetch(xh, here, 0, f.x_type);
+      fetch(dh, here + p.at_dh, 3, f.h_type);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = (i * G + t) * W;
-        float a[W], b[W];
-        if (c < C) {
-          fetch(a, here, 0, f.r, f.x_type, row, c);
-          fetch(b, here, p.at_dh, g.dh, f.h_type, row, c);
-        }
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const int e = i * W + k;
-          xh[e] = c < C ? (a[k] - mean) * inv : 0.f;
-          const float dh = c < C ? b[k] : 0.f;
-          d_w[e] = fmaf(dh, xh[e], d_w[e]);
-          d_b[e] += dh;
-          d[e] = dh * w[e];
-          s[0] += d[e];
-          s[1] = fmaf(d[e], xh[e], s[1]);
-        }
+      for (int k = 0; k < P; ++k) {
+        xh[k] = fmul2(fadd2(xh[k], both(-mean)), both(inv));
+        d_w[k] = ffma2(dh[k], xh[k], d_w[k]);
+        d_b[k] = fadd2(dh[k], d_b[k]);
+        d[k] = fmul2(dh[k], w[k]);
+        s0 = fadd2(s0, d[k]);
+        s1 = ffma2(d[k], xh[k], s1);
       }
-      float both[2] = {s[0], s[1]};
-      row_sum<G>(both, red[group], turn, t, group + 1);
-      const float along = both[1] * p.inv_n, flat = layer ? both[0] * p.inv_n : 0.f;
+      float sums[2] = {s0.x + s0.y, s1.x + s1.y};
+      row_sum<G>(sums, red[group], turn, t, group + 1);
+      const float along = sums[1] * p.inv_n, flat = layer ? sums[0] * p.inv_n : 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) d[e] = inv * (d[e] - flat - xh[e] * along);
+      for (int k = 0; k < P; ++k) d[k] = fmul2(ffma2(xh[k], both(-along), fadd2(d[k], both(-flat))), both(inv));
+      if (g.dr) {
+        fetch(dh, here + p.at_dr, 2, f.x_type);
+#pragma unroll
+        for (int k = 0; k < P; ++k) d[k] = fadd2(d[k], dh[k]);
+      }
+    } else {
+      fetch(d, here + p.at_dr, 2, f.x_type);
+    }
+    put(d, g.dx, f.x_type, row);
+    if (!branch) {
+      request_odd(row + kRows);
+      continue;
+    }
+    // Where the branch is not read its place is not staged either: whatever is there is multiplied into sums that nobody wants.
+    float2 u[P], gate_sum = nil, s0 = nil, s1 = nil;
+    if (reads_y) {
+      fetch(u, here + p.at_y, 1, f.y_type);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) d[e] = 0.f;
+      for (int k = 0; k < P; ++k) u[k] = nil;
     }
+    request_odd(row + kRows);
+    if constexpr (FULL) {
+      if (f.post)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * G + t) * W;
-      if (c < C) {
-        float a[W];
-        if (g.dr) {
-          fetch(a, here, p.at_dr, g.dr, f.x_type, row, c);
-#pragma unroll
-          for (int k = 0; k < W; ++k) d[i * W + k] += a[k];
+        for (int k = 0; k < P; ++k) {
+          xh[k] = fmul2(fadd2(u[k], both(-p_mean)), both(p_inv));
+          u[k] = ffma2(xh[k], pw[k], pb[k]);
         }
+    }
+    if (FULL || wants_gate)
 #pragma unroll
-        for (int k = 0; k < W; ++k) a[k] = d[i * W + k];
-        Raw<W> o;
-        pack<W>(o, a, f.x_type);
-        store_raw<W>(o, g.dx, f.x_type, row * C + c);
-      } else {
-#pragma unroll
-        for (int k = 0; k < W; ++k) d[i * W + k] = 0.f;
+      for (int k = 0; k < P; ++k) {
+        const float2 of_gate = fmul2(fmul2(d[k], scale[k]), u[k]);
+        gate_sum = fadd2(gate_sum, of_gate);
+        if constexpr (FULL) d_g[k] = fadd2(d_g[k], of_gate);
       }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      d[k] = fmul2(d[k], both(gate));
+      if constexpr (FULL) d[k] = fmul2(d[k], gate_c[k]);
+      d_s[k] = ffma2(d[k], u[k], d_s[k]);
+      d[k] = fmul2(d[k], scale[k]);
     }
-    if (!branch) continue;
-    float gate_sum = 0.f;
-    s[0] = s[1] = 0.f;
+    if constexpr (FULL) {
+      if (f.post)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * G + t) * W;
-      float y[W];
-#pragma unroll
-      for (int k = 0; k < W; ++k) y[k] = 0.f;
-      if (reads_y && c < C) fetch(y, here, p.at_y, f.y, f.y_type, row, c);
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int e = i * W + k;
-        float u = y[k];
-        if constexpr (FULL) {
-          if (f.post) {
-            xh[e] = c < C ? (y[k] - p_mean) * p_inv : 0.f;
-            u = fmaf(xh[e], pw[e], pb[e]);
-          }
+        for (int k = 0; k < P; ++k) {
+          d_pw[k] = ffma2(d[k], xh[k], d_pw[k]);
+          d_pb[k] = fadd2(d[k], d_pb[k]);
+          d[k] = fmul2(d[k], pw[k]);
+          s0 = fadd2(s0, d[k]);
+          s1 = ffma2(d[k], xh[k], s1);
         }
-        const float of_scale = FULL ? d[e] * gate * gate_c[e] : d[e] * gate;
-        d_s[e] = fmaf(of_scale, u, d_s[e]);
-        const float of_gate = d[e] * scale[e] * u;
-        gate_sum += of_gate;
-        if constexpr (FULL) d_g[e] += of_gate;
-        const float du = of_scale * scale[e];
-        if constexpr (FULL) {
-          if (f.post) {
-            d_pw[e] = fmaf(du, xh[e], d_pw[e]);
-            d_pb[e] += du;
-            d[e] = du * pw[e];
-            s[0] += d[e];
-            s[1] = fmaf(d[e], xh[e], s[1]);
-          } else {
-            d[e] = du;
-          }
-        } else {
-          d[e] = du;
+    }
+    if ((FULL && f.post) || wants_gate) {
+      float sums[3] = {s0.x + s0.y, s1.x + s1.y, gate_sum.x + gate_sum.y};
+      row_sum<G>(sums, red[group], turn, t, group + 1);
+      if (wants_gate && t == 0) g.d_gate_row[row] = sums[2];
+      if constexpr (FULL) {
+        if (f.post) {
+          const float along = sums[1] * p.inv_n, flat = layer ? sums[0] * p.inv_n : 0.f;
+#pragma unroll
+          for (int k = 0; k < P; ++k) d[k] = fmul2(ffma2(xh[k], both(-along), fadd2(d[k], both(-flat))), both(p_inv));
         }
       }
     }
-    const bool through = FULL && f.post;
-    if (through || g.d_gate_row) {
-      s[2] = gate_sum;
-      row_sum<G>(s, red[group], turn, t, group + 1);
-      if (g.d_gate_row && t == 0) g.d_gate_row[row] = s[2];
-      if (through) {
-        const float along = s[1] * p.inv_n, flat = layer ? s[0] * p.inv_n : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) d[e] = p_inv * (d[e] - flat - xh[e] * along);
-      }
-    }
-    if (g.dy) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = (i * G + t) * W;
-        if (c < C) {
-          float a[W];
-#pragma unroll
-          for (int k = 0; k < W; ++k) a[k] = d[i * W + k];
-          Raw<W> o;
-          pack<W>(o, a, f.y_type);
-          store_raw<W>(o, g.dy, f.y_type, row * C + c);
-        }
-      }
-    }
+    if (g.dy) put(d, g.dy, f.y_type, row);
   }
 
   // this CTA's sums over rows; groups of one CTA are added in order
   float* out = p.partial + static_cast<int64_t>(blockIdx.x) * kSums * C;
-  auto leave = [&](const float* sums, int which, bool wanted) {
+  auto leave = [&](const float2* sums, int which, bool wanted) {
     if (!wanted) return;
     if constexpr (kRows > 1) {
       __syncthreads();                                  // the ring, or the sums before these
-      float* shared = reinterpret_cast<float*>(smem);
+      float2* shared = reinterpret_cast<float2*>(smem);
 #pragma unroll
-      for (int e = 0; e < E; ++e) shared[(group * E + e) * G + t] = sums[e];
+      for (int k = 0; k < P; ++k) shared[(group * P + k) * G + t] = sums[k];
       __syncthreads();
       if (group) return;
     }
+    float e[E];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      float2 s = sums[k];
+      if constexpr (kRows > 1) {
+        const float2* shared = reinterpret_cast<const float2*>(smem);
+#pragma unroll
+        for (int o = 1; o < kRows; ++o) s = fadd2(s, shared[(o * P + k) * G + t]);
+      }
+      e[2 * k] = s.x, e[2 * k + 1] = s.y;
+    }
+    // workspaces begin anywhere: one element at a time
 #pragma unroll
     for (int i = 0; i < N; ++i)
+      if (in(i))
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int e = i * W + k, c = (i * G + t) * W + k;
-        float s = sums[e];
-        if constexpr (kRows > 1) {
-          const float* shared = reinterpret_cast<const float*>(smem);
-#pragma unroll
-          for (int o = 1; o < kRows; ++o) s += shared[(o * E + e) * G + t];
-        }
-        if (c < C) out[static_cast<int64_t>(which) * C + c] = s;
-      }
+        for (int k = 0; k < W; ++k) out[static_cast<int64_t>(which) * C + (i * G + t) * W + k] = e[i * W + k];
   };
   if constexpr (W > 1) cp_async_wait<0>();
   leave(d_w, kSumWeight, g.d_weight != nullptr);
@@ -499,9 +699,9 @@ struct NormSumsParams {
   int type, gate_type;
 };
 
-// sums of the CTAs' sums: 32 columns per CTA, its 8 warps take turns at the slices
-__global__ void __launch_bounds__(256) norm_sums_kernel(const __grid_constant__ NormSumsParams p) {
-  __shared__ float red[8][32];
+// sums of the CTAs' sums: 32 columns per CTA, its 32 warps take turns at the slices
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__ NormSumsParams p) {
+  __shared__ float red[32][33];
   griddep_wait();
   griddep_launch();
   const int columns = (p.channels + 31) / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -513,17 +713,19 @@ __global__ void __launch_bounds__(256) norm_sums_kernel(const __grid_constant__ 
   const int64_t first = gate ? entry * p.slices : 0, last = gate ? first + p.slices : static_cast<int64_t>(p.entries) * p.slices;
   float s = 0.f;
   if (c < p.channels)
-#pragma unroll 4
-    for (int64_t i = first + warp; i < last; i += 8) s += __ldg(p.partial + (i * kSums + which) * p.channels + c);
+#pragma unroll 8
+    for (int64_t i = first + warp; i < last; i += 32) s += __ldg(p.partial + (i * kSums + which) * p.channels + c);
   red[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && c < p.channels) {
+  // a warp sums a column (lane: a warp's part), in a tree: the same order every time
+  float f[1] = {red[lane][warp]};
 #pragma unroll
-    for (int w = 1; w < 8; ++w) s += red[w][lane];
-    const float f[1] = {s};
+  for (int o = 16; o; o >>= 1) f[0] += __shfl_xor_sync(0xffffffffu, f[0], o);
+  const int column = static_cast<int>(blockIdx.x % columns) * 32 + warp;
+  if (lane == 0 && column < p.channels) {
     Raw<1> o;
     pack<1>(o, f, gate ? p.gate_type : p.type);
-    store_raw<1>(o, p.out[gate ? p.n : job], gate ? p.gate_type : p.type, gate ? entry * p.channels + c : c);
+    store_raw<1>(o, p.out[gate ? p.n : job], gate ? p.gate_type : p.type, gate ? entry * p.channels + column : column);
   }
 }
 
@@ -553,27 +755,39 @@ static int gate_vector(const s3r_residual_norm& a) {
   return step % 8 == 0 ? 8 : step % 4 == 0 ? 4 : 1;
 }
 
+template <int W, int G, int E, bool FULL, bool WIDE>
+static int run_rows(NormParams p, cudaStream_t st) {
+  constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kResident = rows_resident(G, FULL, WIDE);
+  const int stage = G * E * (type_bytes(p.a.x_type) + type_bytes(p.a.y_type)), room = kNormSmem / kResident / kRows / stage;
+  p.stages = room < 4 ? room : 4;
+  const int64_t want = (p.rows + kRows - 1) / kRows, most = static_cast<int64_t>(sm_count()) * kResident;
+  S3R_CUDA(cudaFuncSetAttribute(norm_rows_kernel<W, G, E, FULL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem));
+  return launch(norm_rows_kernel<W, G, E, FULL, WIDE>, static_cast<unsigned>(want < most ? want : most), kThreads,
+                static_cast<size_t>(kRows) * p.stages * stage, st, p);
+}
 template <int W, int G, int E>
 static int run_fwd(const NormParams& p, cudaStream_t st) {
-  constexpr int kRows = G < 128 ? 128 / G : 1;
-  return launch(norm_fwd_kernel<W, G, E>, static_cast<unsigned>((p.rows + kRows - 1) / kRows), G < 128 ? 128 : G, 0, st, p);
+  constexpr int kRows = G < 128 ? 128 / G : 1, kThreads = G < 128 ? 128 : G;
+  // where every CTA that fits has four rows and more
+  if constexpr (W > 1 && E == 8)
+    if (p.rows >= 4 * kRows * sm_count() * rows_resident(G, false, false)) {
+      if (p.a.post || p.a.gate_mode == S3R_GATE_CHANNEL) return run_rows<W, G, E, true, true>(p, st);
+      return p.a.x_type == S3R_F32 ? run_rows<W, G, E, false, true>(p, st) : run_rows<W, G, E, false, false>(p, st);
+    }
+  return launch(norm_fwd_kernel<W, G, E>, static_cast<unsigned>((p.rows + kRows - 1) / kRows), kThreads, 0, st, p);
 }
 template <int W>
 static int pick_fwd(const NormParams& p, cudaStream_t st) {
   const int C = p.a.channels;
+  // Eight values per thread: with 32 (a warp per row, no exchange between warps) 64 512 x 1024 took 134 us instead of 130, 12 288 33
+  // instead of 29.5.
   if (C <= 256) return run_fwd<W, 32, 8>(p, st);
-  if (C <= 1024 && p.rows <= 2 * sm_count()) return run_fwd<W, 128, 8>(p, st);
-  if (C <= 512) return run_fwd<W, 32, 16>(p, st);
-  if (C <= 1024) return run_fwd<W, 32, 32>(p, st);
-  if (C <= 2048) return run_fwd<W, 128, 16>(p, st);
-  if (C <= 4096) return run_fwd<W, 128, 32>(p, st);
-  return run_fwd<W, 256, 32>(p, st);
+  if (C <= 1024) return run_fwd<W, 128, 8>(p, st);
+  if (C <= 2048) return run_fwd<W, 256, 8>(p, st);
+  if (C <= 4096) return run_fwd<W, 512, 8>(p, st);
+  return run_fwd<W, 512, 16>(p, st);
 }
 
-struct BwdShape {
-  int threads_per_row, per_thread, ctas, stages;
-  uint32_t stage_bytes;
-};
 static void bwd_shape(int channels, int* G, int* E) {
   *G = channels <= 256 ? 32 : channels <= 512 ? 64 : channels <= 1024 ? 128 : channels <= 2048 ? 256 : 512;
   *E = channels <= 4096 ? 8 : 16;
@@ -626,7 +840,7 @@ extern "C" int s3r_residual_norm_fwd(const s3r_residual_norm* args, void* stream
   int w = row_vector(a.channels, ptr, type, 10);
   if (w > gate_vector(a)) w = gate_vector(a);
   if (a.q && (reinterpret_cast<uintptr_t>(a.q) | a.q_pitch) % 4) w = 1;
-  const NormParams p = {a, a.batch * a.tokens, 1.f / static_cast<float>(a.channels)};
+  const NormParams p = {a, a.batch * a.tokens, 1.f / static_cast<float>(a.channels), 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return w == 8 ? pick_fwd<8>(p, st) : w == 4 ? pick_fwd<4>(p, st) : pick_fwd<1>(p, st);
 }
@@ -676,7 +890,7 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
               "s3r_residual_norm_bwd: workspace of %zu bytes is smaller than the %zu needed", g.workspace ? g.workspace_bytes : 0, need);
   p.partial = static_cast<float*>(g.workspace);
   p.inv_n = 1.f / static_cast<float>(f.channels);
-  const uint32_t row = (static_cast<uint32_t>(f.channels) + 7) / 8 * 8;
+  const uint32_t row = static_cast<uint32_t>(G) * E;            // every thread has places, behind the end of a row too
   p.at_y = row * type_bytes(f.x_type);
   p.at_dr = p.at_y + row * type_bytes(f.y_type);
   p.at_dh = p.at_dr + row * type_bytes(f.x_type);
@@ -708,5 +922,5 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   s.out[s.n] = g.d_gate_channel;
   const int64_t jobs = s.n + (g.d_gate_channel ? entries : 0), blocks = jobs * ((f.channels + 31) / 32);
   S3R_REQUIRE(blocks < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_residual_norm_bwd: grid too large");
-  return launch(norm_sums_kernel, static_cast<unsigned>(blocks), 256, 0, st, s);
+  return launch(norm_sums_kernel, static_cast<unsigned>(blocks), 1024, 0, st, s);
 }

@@ -27,62 +27,76 @@ struct Raw {
   uint32_t v[W];          // 16-bit types fill half of it
 };
 
+// The vector at element i, where `in`.  Predicated, not branched around: a branch per vector, with the same registers written on
+// both sides of it, makes loads wait for one another (64 512 rows of 1024: 160 us, this way 132).
 template <int W>
-__device__ __forceinline__ void load_raw(Raw<W>& r, const void* p, int type, int64_t i) {
-  if (type == S3R_F32) {
-    const float* q = static_cast<const float*>(p) + i;
-    if constexpr (W >= 4) {
-#pragma unroll
-      for (int k = 0; k < W; k += 4) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(q + k));
-        r.v[k] = u.x, r.v[k + 1] = u.y, r.v[k + 2] = u.z, r.v[k + 3] = u.w;
-      }
-    } else {
-      r.v[0] = __ldg(reinterpret_cast<const uint32_t*>(q));
-    }
+__device__ __forceinline__ void load_raw(Raw<W>& r, const void* p, int type, int64_t i, bool in = true) {
+  const char* at = static_cast<const char*>(p) + i * type_bytes(type);
+  const int wide = in && type == S3R_F32, narrow = in && type != S3R_F32;
+  if constexpr (W == 8) {
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %9, 0;\n\tsetp.ne.s32 b, %10, 0;\n\t"
+                 "@a ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%8];\n\t@b ld.global.nc.v4.b32 {%4, %5, %6, %7}, [%8 + 16];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7])
+                 : "l"(at), "r"(static_cast<int>(in)), "r"(wide));
+  } else if constexpr (W == 4) {
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %5, 0;\n\tsetp.ne.s32 b, %6, 0;\n\t"
+                 "@a ld.global.nc.v2.b32 {%0, %1}, [%4];\n\t@b ld.global.nc.v2.b32 {%2, %3}, [%4 + 8];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "l"(at), "r"(static_cast<int>(in)), "r"(wide));
   } else {
-    const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    if constexpr (W == 8) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(q));
-      r.v[0] = u.x, r.v[1] = u.y, r.v[2] = u.z, r.v[3] = u.w;
-    } else if constexpr (W == 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(q));
-      r.v[0] = u.x, r.v[1] = u.y;
-    } else {
-      r.v[0] = __ldg(q);
-    }
+    asm volatile("{\n\t.reg .pred a, b;\n\t.reg .b16 h;\n\tsetp.ne.s32 a, %2, 0;\n\tsetp.ne.s32 b, %3, 0;\n\t"
+                 "@a ld.global.nc.b32 %0, [%1];\n\t@b ld.global.nc.b16 h, [%1];\n\t@b mov.b32 %0, {h, h};\n\t}"
+                 : "=r"(r.v[0]) : "l"(at), "r"(wide), "r"(narrow));
   }
 }
 
 __device__ __forceinline__ float half_lo(uint32_t v) { return __half2float(__ushort_as_half(static_cast<uint16_t>(v))); }
 __device__ __forceinline__ float half_hi(uint32_t v) { return __half2float(__ushort_as_half(static_cast<uint16_t>(v >> 16))); }
 
-template <int W>
-__device__ __forceinline__ void unpack(float (&f)[W], const Raw<W>& r, int type) {
-  if (type == S3R_F32) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) f[k] = __uint_as_float(r.v[k]);
-  } else if (type == S3R_BF16) {
-    if constexpr (W == 1) {
-      f[0] = bf16_lo(r.v[0]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < W; k += 2) f[k] = bf16_lo(r.v[k / 2]), f[k + 1] = bf16_hi(r.v[k / 2]);
-    }
-  } else {
-    if constexpr (W == 1) {
-      f[0] = half_lo(r.v[0]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < W; k += 2) f[k] = half_lo(r.v[k / 2]), f[k + 1] = half_hi(r.v[k / 2]);
-    }
-  }
-}
-
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+template <int W>
+__device__ __forceinline__ void unpack_as(float* f, const Raw<W>& r, int type) {       // type: a constant
+  if (type == S3R_F32) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) f[k] = __uint_as_float(r.v[k]);
+  } else if (W == 1) {
+    f[0] = type == S3R_BF16 ? bf16_lo(r.v[0]) : half_lo(r.v[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const uint32_t v = r.v[k / 2];
+      f[k] = type == S3R_BF16 ? (k & 1 ? bf16_hi(v) : bf16_lo(v)) : (k & 1 ? half_hi(v) : half_lo(v));
+    }
+  }
+}
+// all vectors of a thread in one branch; elements that are not there (`in`) are 0
+template <int W, int N, typename In>
+__device__ __forceinline__ void unpack_all(float (&f)[W * N], const Raw<W> (&r)[N], int type, In in) {
+  if (type == S3R_F32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack_as<W>(f + i * W, r[i], S3R_F32);
+  } else if (type == S3R_BF16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack_as<W>(f + i * W, r[i], S3R_BF16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack_as<W>(f + i * W, r[i], S3R_F16);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (!in(i))
+#pragma unroll
+      for (int k = 0; k < W; ++k) f[i * W + k] = 0.f;
+}
+template <int W>
+__device__ __forceinline__ void unpack(float (&f)[W], const Raw<W>& r, int type) {
+  if (type == S3R_F32) unpack_as<W>(f, r, S3R_F32);
+  else if (type == S3R_BF16) unpack_as<W>(f, r, S3R_BF16);
+  else unpack_as<W>(f, r, S3R_F16);
+}
+
 // to nearest even; what W values become in memory
 template <int W>
 __device__ __forceinline__ void pack(Raw<W>& r, const float (&f)[W], int type) {
@@ -97,20 +111,61 @@ __device__ __forceinline__ void pack(Raw<W>& r, const float (&f)[W], int type) {
   }
 }
 template <int W>
-__device__ __forceinline__ void store_raw(const Raw<W>& r, void* p, int type, int64_t i) {
-  if (type == S3R_F32) {
-    float* q = static_cast<float*>(p) + i;
-    if constexpr (W >= 4) {
-#pragma unroll
-      for (int k = 0; k < W; k += 4) *reinterpret_cast<uint4*>(q + k) = make_uint4(r.v[k], r.v[k + 1], r.v[k + 2], r.v[k + 3]);
-    } else {
-      *reinterpret_cast<uint32_t*>(q) = r.v[0];
-    }
+__device__ __forceinline__ void store_raw(const Raw<W>& r, void* p, int type, int64_t i, bool in = true) {
+  char* at = static_cast<char*>(p) + i * type_bytes(type);
+  const int wide = in && type == S3R_F32, narrow = in && type != S3R_F32;
+  if constexpr (W == 8) {
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %9, 0;\n\tsetp.ne.s32 b, %10, 0;\n\t"
+                 "@a st.global.v4.b32 [%0], {%1, %2, %3, %4};\n\t@b st.global.v4.b32 [%0 + 16], {%5, %6, %7, %8};\n\t}"
+                 ::"l"(at), "r"(r.v[0]), "r"(r.v[1]), "r"(r.v[2]), "r"(r.v[3]), "r"(r.v[4]), "r"(r.v[5]), "r"(r.v[6]), "r"(r.v[7]),
+                 "r"(static_cast<int>(in)), "r"(wide) : "memory");
+  } else if constexpr (W == 4) {
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %5, 0;\n\tsetp.ne.s32 b, %6, 0;\n\t"
+                 "@a st.global.v2.b32 [%0], {%1, %2};\n\t@b st.global.v2.b32 [%0 + 8], {%3, %4};\n\t}"
+                 ::"l"(at), "r"(r.v[0]), "r"(r.v[1]), "r"(r.v[2]), "r"(r.v[3]), "r"(static_cast<int>(in)), "r"(wide) : "memory");
   } else {
-    uint16_t* q = static_cast<uint16_t*>(p) + i;
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(q) = make_uint4(r.v[0], r.v[1], r.v[2], r.v[3]);
-    else if constexpr (W == 4) *reinterpret_cast<uint2*>(q) = make_uint2(r.v[0], r.v[1]);
-    else *q = static_cast<uint16_t>(r.v[0]);
+    asm volatile("{\n\t.reg .pred a, b;\n\t.reg .b16 h, z;\n\tsetp.ne.s32 a, %2, 0;\n\tsetp.ne.s32 b, %3, 0;\n\tmov.b32 {h, z}, %1;\n\t"
+                 "@a st.global.b32 [%0], %1;\n\t@b st.global.b16 [%0], h;\n\t}"
+                 ::"l"(at), "r"(r.v[0]), "r"(wide), "r"(narrow) : "memory");
+  }
+}
+// rounds to the type (one branch), stores all vectors of a thread, and gives back what they hold now
+template <int W, int N, typename At>
+__device__ __forceinline__ void store_all(float (&f)[W * N], void* p, int type, At at, bool back = false) {
+  Raw<W> o[N];
+  auto one = [&](int i, int t) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      if (t == S3R_F32) o[i].v[k] = __float_as_uint(f[i * W + k]);
+      else if (W == 1) o[i].v[0] = t == S3R_BF16 ? pack_bf16(f[i], 0.f) : pack_half(f[i], 0.f);
+      else if (!(k & 1)) o[i].v[k / 2] = t == S3R_BF16 ? pack_bf16(f[i * W + k], f[i * W + (k + 1) % W]) : pack_half(f[i * W + k], f[i * W + (k + 1) % W]);
+    }
+    if (back) unpack_as<W>(f + i * W, o[i], t);
+  };
+  if (type == S3R_F32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) one(i, S3R_F32);
+  } else if (type == S3R_BF16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) one(i, S3R_BF16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) one(i, S3R_F16);
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t a = at(i);
+      store_raw<W>(o[i], p, type, a, a >= 0);
+    }
+  } else if (type == S3R_F32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at(i) >= 0) static_cast<uint32_t*>(p)[at(i)] = o[i].v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at(i) >= 0) static_cast<uint16_t*>(p)[at(i)] = static_cast<uint16_t>(o[i].v[0]);
   }
 }
 
@@ -127,6 +182,10 @@ __device__ __forceinline__ void load_vector(float (&f)[W], const void* p, int ty
   load_raw<W>(r, p, type, i);
   unpack<W>(f, r, type);
 }
+
+// A sum that is not fused with the products in it: the assembler makes one instruction of a packed product and a packed sum, of a
+// packed product and scalar sums it does not.
+__device__ __forceinline__ float2 add_apart(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
 
 // max that keeps NaN
 __device__ __forceinline__ float max_nan(float a, float b) {

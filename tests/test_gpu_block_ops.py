@@ -636,3 +636,35 @@ def test_grad_norm_sizes():
     assert abs(ops.grad_norm([big]).item() - 1e30 * 1024) <= 1e-6 * 1e33
     flat = torch.randn(1000, device=DEV)
     assert abs(ops.grad_norm([flat[1:], flat.view(10, 100).t()]).item() - math.sqrt((flat[1:].double() ** 2).sum() + (flat.double() ** 2).sum())) < 1e-4
+
+
+def test_norm_sums_are_the_same_for_few_rows_and_many():
+    """r is rounded product by product, whichever kernel computes it."""
+    n = Norm((1, 20000, 1024), gate=(1, 20000, 1), seed=3)
+    r, _ = n.call()
+    assert torch.equal(r, n.x + n.y.float() * n.scale * n.gate)
+    n.x, n.y, n.gate = n.x[:, :50].contiguous(), n.y[:, :50].contiguous(), n.gate[:, :50].contiguous()
+    assert torch.equal(n.call()[0], r[:, :50])
+
+
+def test_adamw_codes_are_those_of_separate_operations():
+    """Products and sums of the states are rounded one by one: codes are the same bits as PyTorch's operations give."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    n = 1 << 22
+    g = torch.randn(n, device=DEV, generator=gen) * torch.exp(2 * torch.randn(n, device=DEV, generator=gen))
+    m, v = torch.randint(0, 256, (2, n), device=DEV, generator=gen, dtype=torch.uint8)
+    e = torch.randint(110, 130, (2, n // 256), device=DEV, generator=gen, dtype=torch.uint8)
+    m0, v0 = values(m, e[0], 4).float(), values(v, e[1], 5).float()
+    m1, v1 = m0 * 0.9 + g * (1 - 0.9), v0 * 0.999 + g * g * (1 - 0.999)
+    p, step = torch.zeros(n, device=DEV), torch.zeros((), dtype=torch.int64, device=DEV)
+    m32, v32, step32 = m0.clone(), v0.clone(), step.clone()
+    ops.adamw_step([p.clone()], [g], [m32], [v32], step32)
+    assert torch.equal(m32, m1) and torch.equal(v32, v1)
+    ops.adamw_step([p], [g], [m], [v], step, scales=[e])
+    for x, code, exponent, bits in ((m1, m, e[0], 4), (v1, v, e[1], 5)):
+        unit = torch.exp2(exponent.double() - 127).repeat_interleave(256)
+        z = x.double().abs() / unit
+        last = grid_below(z, bits)
+        want = (torch.round(z / last) * last).clamp(max=1.875)
+        want = torch.where(x > 0, want.clamp(min=2.0 ** -33), want) if bits == 5 else want
+        assert torch.equal(values(code, exponent, bits).abs() / unit, want)

@@ -22,6 +22,7 @@ import torch
 from torch import Tensor, nn
 
 from . import ops
+from .int8 import Int8Linear, Int8Tokens, tokens_of
 
 
 class _TableRows:
@@ -294,12 +295,23 @@ class SparseFlashAttentionRope(nn.Module):
         y = ops.sel_attn_merge(q, k, v, idx, gate, o_c, Bs)
         return self.proj_drop(self.proj(y))
 
+    @torch.no_grad()
+    def quantize_int8(self) -> "SparseFlashAttentionRope":
+        """Replaces the projections by 8-bit ones, for inference, in place (parameters on the GPU).  ``forward`` then takes
+        activations or ``Int8Tokens``."""
+        if self.proj.weight.dtype != torch.int8:
+            self.qkv, self.proj = Int8Linear.of(self.qkv), Int8Linear.of(self.proj)
+            self.gate[0] = Int8Linear.of(self.gate[0])
+        return self
+
     def forward(self, x: Tensor, attn_bias=None, xpos: Optional[Tensor] = None) -> Tensor:
         B, N, C = x.shape
         H = self.num_heads
         d = C // H
         Bs = self.block_size ** 2
-        op = self._native_op(x, xpos, N, Bs, d)
+        if type(self._modules["qkv"]) is Int8Linear:
+            x = tokens_of(x)                                              # once for both products that read it
+        op = self._native_op(x, xpos, N, Bs, d) if type(x) is not Int8Tokens else None
         if op is not None:
             return self._forward_native(op, x, xpos, H, d, Bs)
         qkv = self.qkv(x)

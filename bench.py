@@ -420,7 +420,9 @@ def run_train_step(args):
     mod = speed3r_b200.SparseFlashAttentionRope(dim, num_heads=H, qkv_bias=True, proj_bias=True, qk_norm=True,
                                                 rope=speed3r_b200.RoPE2D(100.0)).to(dev)
     net = torch.nn.parallel.DistributedDataParallel(mod, device_ids=[local_rank]) if world > 1 else mod
-    opt = torch.optim.AdamW(mod.parameters(), lr=1e-4)
+    opt = {"torch": lambda: torch.optim.AdamW(mod.parameters(), lr=1e-4),
+           "adamw": lambda: speed3r_b200.AdamW(mod.parameters(), lr=1e-4, max_norm=1.0),
+           "adamw8": lambda: speed3r_b200.AdamW(mod.parameters(), lr=1e-4, max_norm=1.0, state_bits=8)}[args.optimizer]()
     g = torch.Generator(device=dev).manual_seed(100 + rank)
     x = torch.randn(B, T, dim, device=dev, generator=g) * 0.5
     dy = torch.randn(B, T, dim, device=dev, generator=g) * 0.1
@@ -458,10 +460,53 @@ def run_train_step(args):
             vs_baseline=None, dtype="bf16", data="synthetic",
             config={"workload": "SparseFlashAttentionRope forward + backward + AdamW step, B=2 per GPU, 24 views of 224x224 "
                                 "(T=6144 per sample), dim 1024, 16 heads", "global_batch": world * B, "tokens_per_sample": T,
-                    "parallelism": f"ddp{world}" if world > 1 else "single"},
+                    "parallelism": f"ddp{world}" if world > 1 else "single",
+                    "optimizer": {"torch": "torch.optim.AdamW", "adamw": "this package's AdamW, gradients clipped",
+                                  "adamw8": "this package's AdamW, gradients clipped, states in 8 bits"}[args.optimizer]},
             device_status=status)))
     if world > 1:
         dist.destroy_process_group()
+
+
+def run_block(args):
+    """Forward of one transformer block around the sparse attention (1024 wide, MLP of 4096, bf16 autocast, no gradients) on `--views`
+    views: its modules one by one, with the sums and norms in one pass, and with 8-bit projections and MLP as well."""
+    import torch
+    import speed3r_b200
+    torch.cuda.set_device(0)
+    dev = torch.device("cuda", 0)
+    T = args.views * TOK_PER_VIEW
+    torch.manual_seed(0)
+    blk = speed3r_b200.BlockRope(H * D, H, qkv_bias=True, qk_norm=True, init_values=0.01, rope=speed3r_b200.RoPE2D(100.0)).to(dev).eval()
+    x = torch.randn(1, T, H * D, device=dev)
+    tok = torch.arange(T, device=dev) % TOK_PER_VIEW
+    xpos = torch.stack((tok // 36, tok % 36), -1)[None].contiguous()
+    ev = lambda: torch.cuda.Event(enable_timing=True)
+
+    def timed():
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            for _ in range(max(3, args.warmup)):
+                y = blk(x, xpos)
+            a, b = ev(), ev()
+            a.record()
+            for _ in range(args.steps):
+                y = blk(x, xpos)
+            b.record()
+            torch.cuda.synchronize()
+        return a.elapsed_time(b) / args.steps, y
+
+    blk._fuses = lambda: False
+    apart, y0 = timed()
+    del blk._fuses
+    fused, y1 = timed()
+    blk.quantize_int8()
+    int8, y2 = timed()
+    off = lambda y: ((y - x).double() - (y0 - x).double()).norm().item() / (y0 - x).double().norm().item()
+    print(json.dumps(dict(
+        metric="block_forward_tokens_per_s", value=T / (fused * 1e-3), unit="tokens/s", n_gpus=1, steps=args.steps, warmup=max(3, args.warmup),
+        ms_per_step=fused, higher_is_better=True, scaling="weak", vs_baseline=None, dtype="bf16", data="synthetic",
+        config={"workload": f"one transformer block, forward, {args.views} views of 392x504, dim 1024, 16 heads, MLP 4096", "tokens": T},
+        modules_one_by_one_ms=apart, int8_ms=int8, fused_off=off(y1), int8_off=off(y2), device_status=_lib_status())))
 
 
 def run_extension(args):
@@ -548,6 +593,11 @@ def main():
     ap.add_argument("--train-step", action="store_true",
                     help="time one data-parallel training step of the attention module at the reference's training "
                          "size (B=2 per GPU, T=6144); prints a line of its own (metric attention_module_train_tokens_per_s)")
+    ap.add_argument("--optimizer", default="torch", choices=["torch", "adamw", "adamw8"],
+                    help="--train-step: PyTorch's AdamW, or this package's with gradient clipping, states in 32 or 8 bits")
+    ap.add_argument("--block", action="store_true",
+                    help="time the forward of one transformer block on --views views: modules one by one, fused sums and norms, 8-bit "
+                         "projections; prints a line of its own (metric block_forward_tokens_per_s)")
     ap.add_argument("--setting", default="reference", choices=["reference", "extension"],
                     help="reference: pool 16/16, blocks of 16, top-32 (the reference's only setting); extension: pool 32/16, "
                          "blocks of 64, top-16 with block ranking by probability mass (1 GPU, forward; a line of its own)")
@@ -564,6 +614,9 @@ def main():
         return
     if args.train_step:
         run_train_step(args)
+        return
+    if args.block:
+        run_block(args)
         return
     if args.setting == "extension":
         run_extension(args)

@@ -335,7 +335,7 @@ int s3r_ipc_import(const void* handle64, int64_t offset, void** ptr);
 
 /* u = y, or post_norm(y);  r = x + (u * scale) * gate, rounded to x's type;  h = norm(r).  A norm is the row's, with
  * `weight` and `bias` (each may be NULL).  x, y, r, h [batch * tokens, channels], contiguous, elements aligned to their size
- * (vectors are used where addresses and the number of channels allow).  channels 1 to 8192. */
+ * (vectors are used where addresses and the number of channels allow).  channels 1 to 8192, fewer than 2^31 - 2^20 rows. */
 typedef struct {
   int64_t batch, tokens;
   int channels;
@@ -354,7 +354,8 @@ typedef struct {
 } s3r_residual_norm;
 int s3r_residual_norm_fwd(const s3r_residual_norm* args_host, void* stream);
 
-/* Gradients of the above.  f: its arguments with r (x where y is NULL) and stats as the forward left them; h, q, x are not read.
+/* Gradients of the above.  f: its arguments with r (x where y is NULL) and stats as the forward left them; h, q, x are not read, and y
+ * only for a post norm's and for the scale's and gate's gradients (else it may be any pointer that is not NULL).
  *   dr, dh     gradients of r (x_type) and h (h_type); either may be NULL
  *   dx, dy     [rows, channels], x_type and y_type; dy may be NULL
  *   d_weight, d_bias, d_scale, d_post_weight, d_post_bias  [channels] param_type, each may be NULL

@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
 static int check_args(const s3r_residual_norm& a, const char* what) {
   S3R_REQUIRE(a.batch > 0 && a.tokens > 0 && a.channels > 0, S3R_ERR_SHAPE, "%s: sizes must be positive", what);
   S3R_REQUIRE(a.channels <= kNormMaxChannels, S3R_ERR_TOO_LARGE, "%s: %d channels (at most %d)", what, a.channels, kNormMaxChannels);
-  S3R_REQUIRE(a.batch < (1ll << 31) && a.tokens < (1ll << 31) && a.batch * a.tokens < (1ll << 31), S3R_ERR_TOO_LARGE, "%s: too many rows", what);
+  S3R_REQUIRE(a.batch < (1ll << 31) && a.tokens < (1ll << 31) && a.batch * a.tokens < (1ll << 31) - (1 << 20), S3R_ERR_TOO_LARGE, "%s: too many rows", what);
   S3R_REQUIRE(a.kind == S3R_NORM_LAYER || a.kind == S3R_NORM_RMS, S3R_ERR_UNSUPPORTED, "%s: kind %d", what, a.kind);
   S3R_REQUIRE(known_type(a.x_type) && known_type(a.y_type) && known_type(a.h_type) && known_type(a.param_type) && known_type(a.gate_type),
               S3R_ERR_UNSUPPORTED, "%s: types are fp32, bf16 and fp16", what);

@@ -140,11 +140,17 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm_int8(const Tensor& x, const opt
 enum { kX = 1, kY = 2, kWeight = 4, kBias = 8, kScale = 16, kGate = 32, kPostWeight = 64, kPostBias = 128 };
 std::vector<Tensor> run_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& weight, const optional<Tensor>& scale,
                                  const optional<Tensor>& gate, const optional<Tensor>& post_weight, const optional<Tensor>& post_bias,
-                                 const Tensor& stats, const optional<Tensor>& dr, const optional<Tensor>& dh, bool post, int64_t kind,
-                                 int64_t want, at::ScalarType param_type) {
+                                 const Tensor& stats, const optional<Tensor>& dr, const optional<Tensor>& dh, optional<at::ScalarType> branch,
+                                 bool post, int64_t kind, int64_t want, at::ScalarType param_type) {
   s3r_residual_norm f = norm_args(r, y, weight, {}, scale, gate, post_weight, post_bias, {true, post, kind, 0., 0.});
+  TORCH_CHECK(y.has_value() || !post, "residual_norm: the branch of a post norm is missing");
   c10::cuda::CUDAGuard guard(r.device());
   f.r = r.data_ptr();
+  if (!y.has_value() && branch.has_value()) {                   // there was a branch, of this type, that is not read any more
+    TORCH_CHECK(!(want & (kScale | kGate)), "residual_norm: the branch is missing");
+    f.y = f.r;
+    f.y_type = type_of(at::empty({0}, at::TensorOptions().dtype(*branch)), "the branch");
+  }
   f.stats = f32(stats);
   f.param_type = type_of(at::empty({0}, at::TensorOptions().dtype(param_type)), "parameters");
   const int64_t rows = f.batch * f.tokens;
@@ -158,7 +164,7 @@ std::vector<Tensor> run_norm_bwd(const Tensor& r, const optional<Tensor>& y, con
   if (dh.has_value()) f.h_type = type_of(*dh, "the gradient of the norm");
   if (!dh.has_value()) want &= ~(kWeight | kBias);
   auto channels = [&](int64_t bit) { return want & bit ? fresh({r.size(2)}, r, param_type) : Tensor(); };
-  Tensor dx = fresh_like(r), dy = want & kY ? fresh_like(*y) : Tensor();
+  Tensor dx = fresh_like(r), dy = want & kY && branch.has_value() ? fresh(r.sizes(), r, *branch) : Tensor();
   Tensor dw = channels(kWeight), db = channels(kBias), ds = channels(kScale), dpw = channels(kPostWeight), dpb = channels(kPostBias);
   Tensor dg, dg_row;
   s3r_residual_norm_grad g = {};
@@ -196,8 +202,9 @@ std::vector<Tensor> run_norm_bwd(const Tensor& r, const optional<Tensor>& y, con
 std::vector<Tensor> residual_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& weight,
                                       const optional<Tensor>& scale, const optional<Tensor>& gate, const optional<Tensor>& post_weight,
                                       const optional<Tensor>& post_bias, const Tensor& stats, const optional<Tensor>& dr,
-                                      const optional<Tensor>& dh, bool post, int64_t kind, int64_t want, at::ScalarType param_type) {
-  auto g = run_norm_bwd(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, post, kind, want, param_type);
+                                      const optional<Tensor>& dh, optional<at::ScalarType> branch, bool post, int64_t kind, int64_t want,
+                                      at::ScalarType param_type) {
+  auto g = run_norm_bwd(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, branch, post, kind, want, param_type);
   for (Tensor& t : g)
     if (!t.defined()) t = none(r);
   return g;
@@ -210,9 +217,9 @@ std::tuple<Tensor, Tensor, Tensor> call_norm_fwd(const Tensor& x, const optional
 }
 std::vector<Tensor> call_norm_bwd(const Tensor& r, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& s,
                                   const optional<Tensor>& g, const optional<Tensor>& pw, const optional<Tensor>& pb, const Tensor& stats,
-                                  const optional<Tensor>& dr, const optional<Tensor>& dh, bool post, int64_t kind, int64_t want,
-                                  at::ScalarType param_type) {
-  S3R_DISPATCHED(residual_norm_bwd)(r, y, w, s, g, pw, pb, stats, dr, dh, post, kind, want, param_type);
+                                  const optional<Tensor>& dr, const optional<Tensor>& dh, optional<at::ScalarType> branch, bool post,
+                                  int64_t kind, int64_t want, at::ScalarType param_type) {
+  S3R_DISPATCHED(residual_norm_bwd)(r, y, w, s, g, pw, pb, stats, dr, dh, branch, post, kind, want, param_type);
 }
 
 std::tuple<Tensor, Tensor, Tensor> call_norm_int8(const NormInputs& in, bool post, int64_t kind, double eps, double post_eps) {
@@ -269,11 +276,11 @@ struct NormNode : torch::autograd::Function<NormNode> {
     for (int i = 0, edge = 0; i < 8; ++i)
       if (present >> i & 1 && ctx->needs_input_grad(edge++)) want |= int64_t{1} << i;
     if (!branch) want &= kX | kWeight | kBias;
-    // a branch that nothing is multiplied with is not kept; its place is taken by a tensor of its type that is not read
-    optional<Tensor> y = maybe(s[1]);
-    if (branch && !y.has_value()) y = at::empty(s[0].sizes(), s[0].options().dtype(static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt())));
+    // a branch that nothing is multiplied with is not kept, only its type
+    optional<at::ScalarType> branch_type;
+    if (branch) branch_type = static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt());
     const auto& backward = plain(s[0]) ? run_norm_bwd : call_norm_bwd;
-    const auto g = backward(s[0], y, maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, post, ctx->saved_data["kind"].toInt(),
+    const auto g = backward(s[0], maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, branch_type, post, ctx->saved_data["kind"].toInt(),
                                  want, static_cast<at::ScalarType>(ctx->saved_data["param"].toInt()));
     for (int i = 0; i < 8; ++i)
       if (want >> i & 1 && g[i].defined() && (dh.has_value() || !(i == 2 || i == 3))) out[i] = g[i];
@@ -608,7 +615,7 @@ TORCH_LIBRARY_FRAGMENT(speed3r_b200, m) {
   m.def("residual_norm_fwd(Tensor x, Tensor? y, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? gate, Tensor? post_weight, "
         "Tensor? post_bias, bool norm, bool post, int kind, float eps, float post_eps, ScalarType h_type, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("residual_norm_bwd(Tensor r, Tensor? y, Tensor? weight, Tensor? scale, Tensor? gate, Tensor? post_weight, Tensor? post_bias, "
-        "Tensor stats, Tensor? dr, Tensor? dh, bool post, int kind, int want, ScalarType param_type) -> Tensor[]");
+        "Tensor stats, Tensor? dr, Tensor? dh, ScalarType? branch, bool post, int kind, int want, ScalarType param_type) -> Tensor[]");
   m.def("residual_norm_int8(Tensor x, Tensor? y, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? gate, Tensor? post_weight, "
         "Tensor? post_bias, bool post, int kind, float eps, float post_eps) -> (Tensor, Tensor, Tensor)");
   m.def("residual_norm(Tensor x, Tensor? y, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? gate, Tensor? post_weight, "

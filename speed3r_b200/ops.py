@@ -111,11 +111,11 @@ def _register_fakes() -> None:
                 x.new_empty(4 if keep else 0, x.shape[0] * x.shape[1], dtype=torch.float32))
 
     @fake("speed3r_b200::residual_norm_bwd")
-    def _(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, post, kind, want, param_type):
+    def _(r, y, weight, scale, gate, post_weight, post_bias, stats, dr, dh, branch, post, kind, want, param_type):
         if dh is None:
             want &= ~12
         of = lambda bit: r.new_empty(r.shape[2] if want & bit else 0, dtype=param_type)
-        return [r.new_empty(r.shape), r.new_empty(r.shape, dtype=y.dtype) if want & 2 else r.new_empty(0), of(4), of(8), of(16),
+        return [r.new_empty(r.shape), r.new_empty(r.shape, dtype=branch) if want & 2 and branch is not None else r.new_empty(0), of(4), of(8), of(16),
                 gate.new_empty(gate.shape) if want & 32 else r.new_empty(0), of(64), of(128)]
 
     @fake("speed3r_b200::residual_norm_int8")

@@ -668,3 +668,39 @@ def test_adamw_codes_are_those_of_separate_operations():
         want = (torch.round(z / last) * last).clamp(max=1.875)
         want = torch.where(x > 0, want.clamp(min=2.0 ** -33), want) if bits == 5 else want
         assert torch.equal(values(code, exponent, bits).abs() / unit, want)
+
+
+def test_norm_keeps_no_branch_that_nothing_multiplies():
+    """Where neither scale nor gate is learnt the branch is not saved, and its gradient comes without it."""
+    n = Norm((2, 333, 512), y=torch.bfloat16, gate=(2, 1, 1), seed=13)
+    x, y = n.x.requires_grad_(True), n.y.requires_grad_(True)
+    torch.cuda.synchronize()
+    r, h = n.call()
+    dx, dy = torch.autograd.grad((r, h), (x, y), (n.dr, n.dh))
+    assert dy.dtype == torch.bfloat16
+    n.check(r.detach(), h.detach(), dict(x=dx, y=dy))
+
+
+def test_norm_beyond_four_gigabytes():
+    """Offsets pass 32 bits: the last rows of 5.4 GB are those of a small call."""
+    T, C = 1_320_000, 1024
+    x = torch.empty(1, T, C, device=DEV)
+    x.normal_()
+    w = torch.randn(C, device=DEV)
+    r, h = ops.residual_norm(x, x, (w, None, 1e-5), w, out_dtype=torch.bfloat16)
+    for part in (slice(0, 700), slice(T - 700, T)):
+        small = x[:, part].contiguous()
+        r2, h2 = ops.residual_norm(small, small, (w, None, 1e-5), w, out_dtype=torch.bfloat16)
+        assert torch.equal(r[:, part], r2)
+        # the affine part is fused there and not here
+        close(h[:, part], h2.double(), torch.bfloat16, 2 * half_step(torch.bfloat16) * h2.double().abs(), "h")
+    q, s = ops.quantize_tokens(h)
+    q2, s2 = ops.quantize_tokens(h[:, -5:].contiguous())
+    assert torch.equal(q[:, -5:], q2) and torch.equal(s[:, -5:], s2)
+    del r, x, h
+    wq = int8(40, C)
+    ws = torch.ones(40, device=DEV)
+    whole = q.repeat(1, 4, 1)                      # 5.4 GB of 8-bit tokens
+    ss = s.repeat(1, 4)
+    y = ops.int8_linear(whole, ss, wq, ws, None, torch.float32)
+    assert torch.equal(y[:, -300:], ops.int8_linear(q[:, -300:].contiguous(), s[:, -300:].contiguous(), wq, ws, None, torch.float32))

@@ -127,7 +127,7 @@ struct I8Cfg {
   static constexpr int kStages = 163840 / kBytes > 6 ? 6 : 163840 / kBytes;
   static constexpr int kOut = kStages * kBytes, kColumns = kOut + kI8Warps * kI8Piece;
   static constexpr int kSpan = TN / 2 < 64 ? 64 : TN / 2;       // columns of an epilogue warp: whole pieces
-  static constexpr int kSmem = kColumns + kI8Warps * kSpan * 8 + 1024;
+  static constexpr int kSmem = kColumns + kI8Warps * kSpan * 16 + 1024;
 };
 
 struct I8Ctl {
@@ -179,7 +179,7 @@ __device__ __forceinline__ uint32_t first_cta(uint64_t* bar) {
 template <int CTAS>
 __device__ __forceinline__ void arrive_first_cta(uint64_t* bar) {
   if constexpr (CTAS == 2)
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_cta<2>(bar)) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first_cta<2>(bar)) : "memory");
   else
     mbar_arrive(bar);
 }
@@ -271,14 +271,25 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
   const uint32_t tmem = ctl.tmem_base;
   volatile uint32_t* abort_flag = &ctl.abort_flag;
   const int tiles = p.m_tiles * p.n_tiles, steps = (p.K + 127) / 128, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
+  // tile = m * n_tiles + n, walked without a division per tile
+  struct Tile {
+    int m, n;
+  };
+  const Tile begin = {first / p.n_tiles, first % p.n_tiles}, step_by = {stride / p.n_tiles, stride % p.n_tiles};
+  auto advance = [&](Tile& t) {
+    t.m += step_by.m;
+    t.n += step_by.n;
+    if (t.n >= p.n_tiles) t.n -= p.n_tiles, ++t.m;
+  };
   const uint32_t base = smem_u32(smem);
 
   if (warp == 0) {
     int n = 0;                                                     // copies so far
     bool ok = true;
     const bool leader = elect_one_sync();
-    for (int tile = first; tile < tiles && ok; tile += stride) {
-      const int m0 = (tile / p.n_tiles * CTAS + rank) * 128, n0 = tile % p.n_tiles * TN + rank * (TN / CTAS);
+    Tile at = begin;
+    for (int tile = first; tile < tiles && ok; tile += stride, advance(at)) {
+      const int m0 = (at.m * CTAS + rank) * 128, n0 = at.n * TN + rank * (TN / CTAS);
       for (int k = 0; k < steps; ++k, ++n) {
         const int s = n % C::kStages;
         ok = mbar_wait_warp(&ctl.empty[s], (n / C::kStages & 1) ^ 1, abort_flag);
@@ -335,7 +346,8 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
     const int quarter = warp & 3, half = (warp - 2) >> 2;          // lanes 32 * quarter .. of tensor memory; half of the columns
     char* piece = smem + C::kOut + (warp - 2) * kI8Piece;
     const uint32_t stage = smem_u32(piece);
-    float* columns = reinterpret_cast<float*>(smem + C::kColumns) + (warp - 2) * 2 * C::kSpan;        // scales, biases
+    // scales and biases of its columns, of this tile and the next one
+    float* factors = reinterpret_cast<float*>(smem + C::kColumns) + (warp - 2) * 4 * C::kSpan;
     constexpr int per = TYPE == S3R_F32 ? 32 : 64;                 // columns of a piece
     const int from = half * C::kSpan;
     constexpr int kMine = C::kSpan / 32;
@@ -343,52 +355,61 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
     // every lane would need every column's factors, and reading those (a wavefront per column and warp) kept shared memory busier
     // than the products at K = 1024 (64 512 x 4096: 248 us).
     const int r = lane >> 2, c = 2 * (lane & 3);
-    float scale[kMine], bias[kMine], rows[4];                      // of the next tile: fetched while this one is written out
-    auto fetch = [&](int tile) {
-      const int n0 = tile % p.n_tiles * TN + from;
-      const int64_t row = (static_cast<int64_t>(tile / p.n_tiles) * CTAS + rank) * 128 + quarter * 32 + r;
+    float rows[4];                                                 // the next tile's row scales
+    for (int i = lane; i < 4 * C::kSpan; i += 32) factors[i] = 0.f;
+    __syncwarp();
+    auto fetch = [&](int tile, Tile at, float* to) {
+      const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + r;
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int col = n0 + i * 32 + lane;
-        scale[i] = tile < tiles && col < p.N ? __ldg(p.b_scale + col) : 0.f;
-        bias[i] = tile < tiles && p.bias && col < p.N ? __ldg(p.bias + col) : 0.f;
+        const int col = at.n * TN + from + i * 32 + lane;
+        if (tile < tiles && col < p.N) {
+          cp_async4(smem_u32(to + i * 32 + lane), p.b_scale + col);
+          if (p.bias) cp_async4(smem_u32(to + C::kSpan + i * 32 + lane), p.bias + col);
+        }
       }
+      cp_async_commit();
 #pragma unroll
       for (int i = 0; i < 4; ++i) rows[i] = tile < tiles && row + 8 * i < p.M ? __ldg(p.a_scale + row + 8 * i) : 0.f;
     };
-    fetch(first);
+    Tile at = begin, after = begin;
+    fetch(first, at, factors);
     int done = 0;
     bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += stride, ++done) {
+    for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
       const int buf = done & 1;
-      const int64_t m0 = (static_cast<int64_t>(tile / p.n_tiles) * CTAS + rank) * 128 + quarter * 32;
-      const int n0 = tile % p.n_tiles * TN;
+      const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+      const int n0 = at.n * TN;
       const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
-      float2 row[4];
+      float row[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) row[i] = make_float2(rows[i], rows[i]);
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) columns[i * 32 + lane] = scale[i], columns[C::kSpan + i * 32 + lane] = bias[i];
+      for (int i = 0; i < 4; ++i) row[i] = rows[i];
+      const float* columns = factors + buf * 2 * C::kSpan;
+      cp_async_wait<0>();
       __syncwarp();
-      fetch(tile + stride);
+      advance(after);
+      fetch(tile + stride, after, factors + (buf ^ 1) * 2 * C::kSpan);
       ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      // 32 columns' sums, and the next 32 on their way: asked for under no condition, so that their registers have no other writer to
+      // wait for (asked for where they exist, a load beside the products cost its whole latency, 900 cycles, three times per tile).
       const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t v[2][32];                                           // 32 columns' sums and the next 32
-      if (from < width) tmem_ld_32x32(sums, v[0]);
+      uint32_t v[2][32];
+      if (from < TN) tmem_ld_32x32(sums, v[0]);
 #pragma unroll
       for (int g = 0; g < kMine; ++g) {
+        uint32_t(&now)[32] = v[g & 1];
+        tmem_ld_wait_for(now);
+        if (g + 1 < kMine) {
+          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v[(g + 1) & 1]);
+        } else {                                                   // this warp's sums are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+        }
         if (from + g * 32 < width) {
-          uint32_t(&now)[32] = v[g & 1];
-          tmem_ld_wait_for(now);
           const bool last = g + 1 == kMine || from + g * 32 + 32 >= width;
-          if (!last) tmem_ld_32x32(sums + g * 32 + 32, v[(g + 1) & 1]);
-          else {                                                   // this warp's sums are in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
-          }
           if (per == 32 || !(g & 1)) {
             if (lane == 0) bulk_wait_read();                       // the store before has left this piece
             __syncwarp();
@@ -404,9 +425,9 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int at = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
-              const float2 sum = make_float2(__int2float_rn(static_cast<int>(now[at])), __int2float_rn(static_cast<int>(now[at + 1])));
-              x[j][i] = ffma2(fmul2(sum, row[i]), s[j], b[j]);
+              const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
+              const float2 sum = make_float2(__int2float_rn(static_cast<int>(now[k])), __int2float_rn(static_cast<int>(now[k + 1])));
+              x[j][i] = ffma2(fmul2(sum, make_float2(row[i], row[i])), s[j], b[j]);
             }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -431,12 +452,12 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
               __syncwarp();
               const int left = min(per, width - c0);
               for (int i = 0; i < 32 && m0 + i < p.M; ++i) {
-                const int64_t at = (m0 + i) * p.N + n0 + c0;
+                const int64_t place = (m0 + i) * p.N + n0 + c0;
                 for (int k = lane; k < left; k += 32) {
                   const int byte = k * type_bytes(TYPE);
                   const char* from_smem = piece + swz128(i, byte >> 4) + (byte & 15);
-                  if constexpr (TYPE == S3R_F32) static_cast<float*>(p.out)[at + k] = *reinterpret_cast<const float*>(from_smem);
-                  else static_cast<uint16_t*>(p.out)[at + k] = *reinterpret_cast<const uint16_t*>(from_smem);
+                  if constexpr (TYPE == S3R_F32) static_cast<float*>(p.out)[place + k] = *reinterpret_cast<const float*>(from_smem);
+                  else static_cast<uint16_t*>(p.out)[place + k] = *reinterpret_cast<const uint16_t*>(from_smem);
                 }
               }
               __syncwarp();                                        // read before the next piece is written
@@ -444,12 +465,9 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
           }
         }
       }
-      if (from >= width) {                                         // none of this warp's columns exist
-        __syncwarp();
-        if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
-      }
       __syncwarp();                                                // its factors are read
     }
+    cp_async_wait<0>();
     if (lane == 0) bulk_wait_all();
     if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
   }

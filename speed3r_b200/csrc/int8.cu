@@ -94,6 +94,8 @@ static int run_quantize(const QuantParams& p, cudaStream_t st) {
 template <int W>
 static int pick_quantize(const QuantParams& p, cudaStream_t st) {
   const int C = p.channels;
+  // 32 values per thread, all asked for at once: 64 512 x 4096 bf16 128 us (6.2 TB/s); with 16 148, with 8 204, and CTAs that stay with rows
+  // staged ahead, as the norms have them, 183
   if (C <= 256) return run_quantize<W, 32, 8>(p, st);
   if (C <= 1024 && p.rows <= 2 * sm_count()) return run_quantize<W, 128, 8>(p, st);
   if (C <= 1024) return run_quantize<W, 32, 32>(p, st);
@@ -176,6 +178,8 @@ __device__ __forceinline__ uint32_t first_cta(uint64_t* bar) {
   if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(at));
   return at;
 }
+// What it tells of - sums read from tensor memory - is complete in front of it (tcgen05.wait::ld, tcgen05.fence) and is no memory of this
+// thread, so that no release at the cluster's scope is needed: that waits for every store in flight, 2000 of a tile's 7000 cycles.
 template <int CTAS>
 __device__ __forceinline__ void arrive_first_cta(uint64_t* bar) {
   if constexpr (CTAS == 2)

@@ -24,49 +24,6 @@ __device__ __forceinline__ float gate_of_row(const s3r_residual_norm& a, int64_t
   return load_one(a.gate, a.gate_type, b * a.gate_stride_b + (static_cast<uint32_t>(row) - b * tokens) * a.gate_stride_t);
 }
 
-constexpr int kNormSmem = 220 * 1024;
-
-template <int W>
-__device__ __forceinline__ void stage_vector(uint32_t dst, const void* p, int type, int64_t i) {
-  const char* src = static_cast<const char*>(p) + i * type_bytes(type);
-  if constexpr (W == 8) {
-    cp_async16(dst, src);
-    if (type == S3R_F32) cp_async16(dst + 16, src + 16);
-  } else {
-    if (type == S3R_F32) cp_async16(dst, src);
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-  }
-}
-template <int W>
-__device__ __forceinline__ void staged_raw(Raw<W>& r, const char* s, int type) {
-  const uint32_t at = smem_u32(s);
-  const int wide = type == S3R_F32;
-  if constexpr (W == 8)
-    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %9, 0;\n\t"
-                 "ld.shared.v4.b32 {%0, %1, %2, %3}, [%8];\n\t@b ld.shared.v4.b32 {%4, %5, %6, %7}, [%8 + 16];\n\t}"
-                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7]) : "r"(at), "r"(wide) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %5, 0;\n\t"
-                 "ld.shared.v2.b32 {%0, %1}, [%4];\n\t@b ld.shared.v2.b32 {%2, %3}, [%4 + 8];\n\t}"
-                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "r"(at), "r"(wide) : "memory");
-}
-
-// a vector's place in shared memory
-template <int W>
-__device__ __forceinline__ void zero_place(char* at, int bytes) {
-#pragma unroll
-  for (int k = 0; k < W; k += 2) {
-    *reinterpret_cast<uint32_t*>(at + 2 * k) = 0;
-    if (bytes == 4) *reinterpret_cast<uint32_t*>(at + 2 * W + 2 * k) = 0;
-  }
-}
-__device__ __forceinline__ void cp_async_wait_for(int pending) {
-  if (pending >= 3) cp_async_wait<3>();
-  else if (pending == 2) cp_async_wait<2>();
-  else if (pending == 1) cp_async_wait<1>();
-  else cp_async_wait<0>();
-}
-
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: G threads per row, E elements per thread in registers (vectors of W); the variance from the centred values
 // ---------------------------------------------------------------------------------------------------------------------
@@ -758,10 +715,10 @@ static int gate_vector(const s3r_residual_norm& a) {
 template <int W, int G, int E, bool FULL, bool WIDE>
 static int run_rows(NormParams p, cudaStream_t st) {
   constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kResident = rows_resident(G, FULL, WIDE);
-  const int stage = G * E * (type_bytes(p.a.x_type) + type_bytes(p.a.y_type)), room = kNormSmem / kResident / kRows / stage;
+  const int stage = G * E * (type_bytes(p.a.x_type) + type_bytes(p.a.y_type)), room = kRowsSmem / kResident / kRows / stage;
   p.stages = room < 4 ? room : 4;
   const int64_t want = (p.rows + kRows - 1) / kRows, most = static_cast<int64_t>(sm_count()) * kResident;
-  S3R_CUDA(cudaFuncSetAttribute(norm_rows_kernel<W, G, E, FULL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem));
+  S3R_CUDA(cudaFuncSetAttribute(norm_rows_kernel<W, G, E, FULL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
   return launch(norm_rows_kernel<W, G, E, FULL, WIDE>, static_cast<unsigned>(want < most ? want : most), kThreads,
                 static_cast<size_t>(kRows) * p.stages * stage, st, p);
 }
@@ -804,8 +761,8 @@ static int bwd_slices(int64_t entries, int64_t span, int G) {
 template <int W, int G, int E, bool FULL>
 static int run_bwd(const NormBwdParams& p, unsigned ctas, cudaStream_t st) {
   constexpr int kThreads = G < 128 ? 128 : G, kGroups = kThreads / G;
-  static_assert(kGroups * E * G * 4 <= kNormSmem, "sums of the groups");
-  S3R_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<W, G, E, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem));
+  static_assert(kGroups * E * G * 4 <= kRowsSmem, "sums of the groups");
+  S3R_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<W, G, E, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
   size_t smem = W > 1 ? static_cast<size_t>(kGroups) * p.stages * p.stage_bytes : 0;
   if constexpr (kGroups > 1) {
     constexpr size_t kSumBytes = static_cast<size_t>(kGroups) * E * G * 4;
@@ -896,7 +853,7 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   p.at_dh = p.at_dr + row * type_bytes(f.x_type);
   p.stage_bytes = p.at_dh + row * type_bytes(f.h_type);
   const int threads = G < 128 ? 128 : G, resident = 512 / threads;
-  const uint32_t room = kNormSmem / resident / (threads / G);
+  const uint32_t room = kRowsSmem / resident / (threads / G);
   p.stages = static_cast<int>(room / p.stage_bytes < 4 ? room / p.stage_bytes : 4);
   S3R_REQUIRE(p.stages >= 1, S3R_ERR_TOO_LARGE, "s3r_residual_norm_bwd: rows do not fit shared memory");
 

@@ -183,6 +183,49 @@ __device__ __forceinline__ void load_vector(float (&f)[W], const void* p, int ty
   unpack<W>(f, r, type);
 }
 
+// Rows on their way into shared memory (cp.async): each thread its own vectors, so that no barrier orders them.
+constexpr int kRowsSmem = 220 * 1024;
+template <int W>
+__device__ __forceinline__ void stage_vector(uint32_t dst, const void* p, int type, int64_t i) {
+  const char* src = static_cast<const char*>(p) + i * type_bytes(type);
+  if constexpr (W == 8) {
+    cp_async16(dst, src);
+    if (type == S3R_F32) cp_async16(dst + 16, src + 16);
+  } else {
+    if (type == S3R_F32) cp_async16(dst, src);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  }
+}
+template <int W>
+__device__ __forceinline__ void staged_raw(Raw<W>& r, const char* s, int type) {
+  const uint32_t at = smem_u32(s);
+  const int wide = type == S3R_F32;
+  if constexpr (W == 8)
+    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %9, 0;\n\t"
+                 "ld.shared.v4.b32 {%0, %1, %2, %3}, [%8];\n\t@b ld.shared.v4.b32 {%4, %5, %6, %7}, [%8 + 16];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7]) : "r"(at), "r"(wide) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred b;\n\tsetp.ne.s32 b, %5, 0;\n\t"
+                 "ld.shared.v2.b32 {%0, %1}, [%4];\n\t@b ld.shared.v2.b32 {%2, %3}, [%4 + 8];\n\t}"
+                 : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "r"(at), "r"(wide) : "memory");
+}
+
+// a vector's place in shared memory
+template <int W>
+__device__ __forceinline__ void zero_place(char* at, int bytes) {
+#pragma unroll
+  for (int k = 0; k < W; k += 2) {
+    *reinterpret_cast<uint32_t*>(at + 2 * k) = 0;
+    if (bytes == 4) *reinterpret_cast<uint32_t*>(at + 2 * W + 2 * k) = 0;
+  }
+}
+__device__ __forceinline__ void cp_async_wait_for(int pending) {
+  if (pending >= 3) cp_async_wait<3>();
+  else if (pending == 2) cp_async_wait<2>();
+  else if (pending == 1) cp_async_wait<1>();
+  else cp_async_wait<0>();
+}
+
 // A sum that is not fused with the products in it: the assembler makes one instruction of a packed product and a packed sum, of a
 // packed product and scalar sums it does not.
 __device__ __forceinline__ float2 add_apart(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }

@@ -692,8 +692,11 @@ def test_norm_beyond_four_gigabytes():
         small = x[:, part].contiguous()
         r2, h2 = ops.residual_norm(small, small, (w, None, 1e-5), w, out_dtype=torch.bfloat16)
         assert torch.equal(r[:, part], r2)
-        # the affine part is fused there and not here
-        close(h[:, part], h2.double(), torch.bfloat16, 2 * half_step(torch.bfloat16) * h2.double().abs(), "h")
+        # Two kernels: each rounds to half a step, and each mean is off by a few 2^-24 of the row's largest value, which moves every
+        # centred value of the row by as much, those near zero as well (as in Norm.check)
+        r64 = r2.double()
+        row = r64.abs().amax(-1, keepdim=True) / r64.std(-1, keepdim=True)
+        close(h[:, part], h2.double(), torch.bfloat16, half_step(torch.bfloat16) * h2.double().abs() + 2 * 64 * F32 * row * w.double().abs(), "h")
     q, s = ops.quantize_tokens(h)
     q2, s2 = ops.quantize_tokens(h[:, -5:].contiguous())
     assert torch.equal(q[:, -5:], q2) and torch.equal(s[:, -5:], s2)

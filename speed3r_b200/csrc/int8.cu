@@ -530,6 +530,92 @@ static int run_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_t b
   return launch_int8<TN, CTAS, S3R_F16>(a, a_pitch, b, b_pitch, p, st);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has four output
+// channels, a lane 16 bytes of each at a time; the tokens lie in shared memory.  One token x 4096 x 1024: 6.5 us on tcgen05, this way 3.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kFewTokens = 8, kFewBytes = 48 * 1024, kFewChannels = 4, kFewWarps = 8;
+
+struct FewParams {
+  const int8_t *a, *b;
+  const float *a_scale, *b_scale, *bias;
+  void* out;
+  int64_t a_pitch, b_pitch;
+  int N, K, type, M;
+};
+
+// 16 bytes from k on; what lies behind the row's end is 0 and not read
+__device__ __forceinline__ uint4 load_16(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int i = 0; k + i < K; ++i) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int M>
+__global__ void __launch_bounds__(32 * kFewWarps) int8_few_kernel(const __grid_constant__ FewParams p) {
+  extern __shared__ __align__(16) char smem[];
+  griddep_wait();
+  griddep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (p.K + 15) / 16;
+  uint4* x = reinterpret_cast<uint4*>(smem);                       // [M][chunks]
+  const int n0 = (blockIdx.x * kFewWarps + warp) * kFewChannels;
+  // the first weights are on their way while the tokens are fetched
+  uint4 w[kFewChannels];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < kFewChannels; ++i) w[i] = n0 + i < p.N && c < chunks ? load_16(p.b + (n0 + i) * p.b_pitch, c * 16, p.K) : make_uint4(0, 0, 0, 0);
+  };
+  fetch(lane);
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+    for (int c = threadIdx.x; c < chunks; c += 32 * kFewWarps) x[m * chunks + c] = m < p.M ? load_16(p.a + m * p.a_pitch, c * 16, p.K) : make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  int sum[kFewChannels][M];
+#pragma unroll
+  for (int i = 0; i < kFewChannels; ++i)
+#pragma unroll
+    for (int m = 0; m < M; ++m) sum[i][m] = 0;
+  for (int c = lane; c < chunks; c += 32) {
+    uint4 now[kFewChannels];
+#pragma unroll
+    for (int i = 0; i < kFewChannels; ++i) now[i] = w[i];
+    fetch(c + 32);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const uint4 t = x[m * chunks + c];
+#pragma unroll
+      for (int i = 0; i < kFewChannels; ++i) {
+        int s = sum[i][m];
+        s = __dp4a(static_cast<int>(now[i].x), static_cast<int>(t.x), s);
+        s = __dp4a(static_cast<int>(now[i].y), static_cast<int>(t.y), s);
+        s = __dp4a(static_cast<int>(now[i].z), static_cast<int>(t.z), s);
+        sum[i][m] = __dp4a(static_cast<int>(now[i].w), static_cast<int>(t.w), s);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kFewChannels; ++i)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int total = __reduce_add_sync(0xffffffffu, sum[i][m]);
+      if (lane == i * M + m && m < p.M && n0 + i < p.N) {
+        const float y = __fmul_rn(__fmul_rn(__int2float_rn(total), __ldg(p.a_scale + m)), __ldg(p.b_scale + n0 + i));
+        const float v[1] = {p.bias ? __fadd_rn(y, __ldg(p.bias + n0 + i)) : y};
+        Raw<1> o;
+        pack<1>(o, v, p.type);
+        store_raw<1>(o, p.out, p.type, static_cast<int64_t>(m) * p.N + n0 + i);
+      }
+    }
+}
+
+template <int M>
+static int run_few(const FewParams& p, cudaStream_t st) {
+  static_assert(M * kFewChannels <= 32, "a lane per result");
+  const int per = kFewWarps * kFewChannels;
+  return launch(int8_few_kernel<M>, static_cast<unsigned>((p.N + per - 1) / per), 32 * kFewWarps, static_cast<size_t>(M) * ((p.K + 15) / 16) * 16, st, p);
+}
+
 }  // namespace s3r
 
 using namespace s3r;
@@ -560,6 +646,11 @@ extern "C" int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_
               "s3r_int8_linear: operands and their pitches must be multiples of 16 bytes");
   S3R_REQUIRE(((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale) | reinterpret_cast<uintptr_t>(bias)) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(out) % type_bytes(type) == 0, S3R_ERR_ALIGNMENT, "s3r_int8_linear: elements must be aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M <= kFewTokens && (M <= 2 ? M : M <= 4 ? 4 : 8) * ((static_cast<int64_t>(K) + 15) / 16 * 16) <= kFewBytes) {
+    const FewParams f = {a, b, a_scale, b_scale, bias, out, a_pitch, b_pitch, N, K, type, static_cast<int>(M)};
+    return M == 1 ? run_few<1>(f, st) : M == 2 ? run_few<2>(f, st) : M <= 4 ? run_few<4>(f, st) : run_few<8>(f, st);
+  }
   I8Params p = {};
   p.a_scale = a_scale;
   p.b_scale = b_scale;
@@ -571,7 +662,6 @@ extern "C" int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_
   p.copy_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && static_cast<int64_t>(N) * type_bytes(type) % 16 == 0;
   p.status = device_status_ptr();
   S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_int8_linear: no status word");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   // the tile whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a)
   auto cost = [&](int tn, int ctas) {
     const int64_t tiles = (M + 128 * ctas - 1) / (128 * ctas) * ((N + tn - 1) / tn), at_once = sm_count() / ctas;

@@ -355,6 +355,12 @@ def test_int8_linear_sizes(M, N, K):
     check_linear(M, N, K)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("N, K", [(1, 5), (31, 16), (33, 500), (1000, 1040), (4096, 1024), (129, 6000), (129, 6160), (40, 50000)])
+def test_int8_linear_few_tokens(M, N, K):
+    check_linear(M, N, K, torch.float32 if N % 2 else torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M, N, K", [(1, 1024, 1024), (8, 4096, 1024), (100, 1000, 500), (300, 3104, 1024), (2048, 1024, 4096), (8328, 3104, 1024), (4001, 1023, 700), (20000, 512, 256)])
 @pytest.mark.parametrize("bias", [True, False])

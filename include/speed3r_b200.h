@@ -374,11 +374,14 @@ typedef struct {
 size_t s3r_residual_norm_bwd_workspace_bytes(int64_t batch, int64_t tokens, int channels, int gate_mode);
 int s3r_residual_norm_bwd(const s3r_residual_norm* f_host, const s3r_residual_norm_grad* g_host, void* stream);
 
-/* q[r, c] = x[r, c] * (127 / max |x[r]|) to nearest even, scale[r] = max |x[r]| / 127.  x: rows of x_pitch elements of `type`,
+/* q[r, c] = x[r, c] * (127 * (1 / max |x[r]|)) to nearest even, scale[r] = max |x[r]| / 127.  x: rows of x_pitch elements of `type`,
  * q: rows of q_pitch bytes; NaN in a row makes its scale NaN, rows whose largest
  * magnitude is below 2^-119 are zeros. */
 int s3r_quantize_rows(const void* x, int type, int64_t x_pitch, int8_t* q, int64_t q_pitch, float* scale, int64_t rows, int channels,
                       void* stream);
+
+/* Rows of K bytes that begin anywhere, to rows of dst_pitch bytes (base and pitch multiples of 16) with zeros up to the next multiple of 16. */
+int s3r_pad_rows(const int8_t* src, int64_t src_pitch, int8_t* dst, int64_t dst_pitch, int64_t rows, int K, void* stream);
 
 /* out[m, n] = (sum over k of a[m, k] b[n, k]) * a_scale[m] * b_scale[n] + bias[n]: 8-bit operands, 32-bit sums, fp32 from there on.
  *   a [M, K] rows of a_pitch bytes, b [N, K] rows of b_pitch bytes: bases and pitches multiples of 16, K <= 65536 (sums fit 32 bits)

@@ -49,6 +49,7 @@ SIGNATURES = {
     "s3r_residual_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i, _i]),
     "s3r_residual_norm_bwd": (_i, [_p, _p, _p]),
     "s3r_quantize_rows": (_i, [_p, _i, _i64, _p, _i64, _p, _i64, _i, _p]),
+    "s3r_pad_rows": (_i, [_p, _i64, _p, _i64, _i64, _i, _p]),
     "s3r_int8_linear": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _p, _i, _i64, _i, _i, _p]),
     "s3r_grad_norm_workspace_bytes": (_sz, [_i, _p]),
     "s3r_grad_norm": (_i, [_i, _p, _p, _p, _p, _p, _sz, _p]),

@@ -105,6 +105,38 @@ static int pick_quantize(const QuantParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// 8-bit rows that begin anywhere, to rows at multiples of 16 bytes, as copies by TMA want them (zeros behind their end): 16 bytes per
+// thread from five aligned words.  Bound: HBM, once in and once out (PyTorch's copy moves a byte per thread).
+// ---------------------------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict__ src, int64_t src_pitch, int8_t* __restrict__ dst, int64_t dst_pitch,
+                                                       int64_t rows, int K, int chunks) {
+  griddep_wait();
+  griddep_launch();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / chunks;
+  if (row >= rows) return;
+  const int c = static_cast<int>(i - row * chunks) * 16;
+  const int8_t* from = src + row * src_pitch + c;
+  uint32_t w[4];
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 3);
+  const int8_t *first = from - off, *begin = src, *end = src + (rows - 1) * src_pitch + K;
+  if (c + 16 <= K && first >= begin && first + 20 <= end) {
+    uint32_t v[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) v[k] = __ldg(reinterpret_cast<const uint32_t*>(first) + k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], off * 8);
+  } else {                                               // the end of a row, and the first and last bytes of all
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = 0;
+      for (int b = 0; b < 4; ++b)
+        if (c + 4 * k + b < K) w[k] |= static_cast<uint32_t>(static_cast<uint8_t>(from[4 * k + b])) << (8 * b);
+    }
+  }
+  *reinterpret_cast<uint4*>(dst + row * dst_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // product on tcgen05: persistent CTAs, K in steps of 128 bytes through a ring of TMA copies, the sums of two tiles in tensor memory
 // so that one is written out while the next is summed.  One warp copies, one issues the products, eight take the sums (32 rows and
 // half of the columns each), scale them and store through shared memory.
@@ -633,6 +665,16 @@ extern "C" int s3r_quantize_rows(const void* x, int type, int64_t x_pitch, int8_
   const QuantParams p = {x, q, scale, x_pitch, q_pitch, rows, type, channels};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return w == 8 ? pick_quantize<8>(p, st) : w == 4 ? pick_quantize<4>(p, st) : pick_quantize<1>(p, st);
+}
+
+extern "C" int s3r_pad_rows(const int8_t* src, int64_t src_pitch, int8_t* dst, int64_t dst_pitch, int64_t rows, int K, void* stream) {
+  S3R_REQUIRE(src && dst, S3R_ERR_NULL, "s3r_pad_rows: NULL pointer");
+  S3R_REQUIRE(rows > 0 && K > 0 && src_pitch >= 0 && dst_pitch >= K, S3R_ERR_SHAPE, "s3r_pad_rows: sizes must be positive, rows no longer than the pitch");
+  S3R_REQUIRE(reinterpret_cast<uintptr_t>(dst) % 16 == 0 && dst_pitch % 16 == 0, S3R_ERR_ALIGNMENT, "s3r_pad_rows: rows must become multiples of 16 bytes");
+  const int chunks = static_cast<int>((static_cast<int64_t>(K) + 15) / 16);
+  const int64_t blocks = (rows * chunks + 255) / 256;
+  S3R_REQUIRE(K <= 0x7fffff00 && blocks < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_pad_rows: grid too large");
+  return launch(pad_rows_kernel, static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream), src, src_pitch, dst, dst_pitch, rows, K, chunks);
 }
 
 extern "C" int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* b, int64_t b_pitch, const float* b_scale,

@@ -243,7 +243,7 @@ struct RowScale {
   float scale, inverse;
 };
 __device__ __forceinline__ RowScale row_scale(float big) {
-  return {__fdiv_rn(big, 127.f), big < 1.5046328e-36f ? 0.f : __fdiv_rn(127.f, big)};
+  return {__fdiv_rn(big, 127.f), big < 1.5046328e-36f ? 0.f : __fmul_rn(127.f, __frcp_rn(big))};      // as PyTorch takes 127 / big
 }
 // to nearest even, NaN to 0
 __device__ __forceinline__ uint32_t to_s8(float v, float inverse) {

@@ -396,10 +396,12 @@ Tensor byte_rows(const Tensor& t, int64_t rows, int64_t K) {
   const bool fits = (K == 1 || r.stride(1) == 1) && (rows <= 1 || (r.stride(0) >= K && r.stride(0) % 16 == 0)) &&
                     reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
   if (fits) return r;                        // a single row has no pitch
-  Tensor whole = fresh({rows, (K + 15) / 16 * 16}, t, at::kChar);
-  Tensor part = whole.narrow(1, 0, K);
-  part.copy_(r);
-  return part;
+  if (K > 1 && r.stride(1) != 1) r = r.contiguous();
+  const int64_t pitch = (K + 15) / 16 * 16;
+  Tensor whole = fresh({rows, pitch}, t, at::kChar);
+  check(s3r_pad_rows(static_cast<const int8_t*>(r.data_ptr()), rows > 1 ? r.stride(0) : K, static_cast<int8_t*>(whole.data_ptr()), pitch, rows,
+                     static_cast<int>(K), stream()), "s3r_pad_rows");
+  return whole.narrow(1, 0, K);
 }
 
 Tensor int8_product(const Tensor& q, const Tensor& q_scale, const Tensor& weight, const Tensor& weight_scale, const optional<Tensor>& bias,

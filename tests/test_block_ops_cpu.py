@@ -133,6 +133,8 @@ def test_int8_arguments_are_checked_without_a_gpu(lib):
     assert q(x=None) == -4 and q(rows=0) == -1 and q(ch=17) == -1 and q(qp=8) == -1 and q(type=5) == -2 and q(x=p + 2) == -3 and q(rows=1 << 31) == -6
     f = lambda a=p, ap=32, b=p, bp=32, out=p, type=1, M=1, N=1, K=32: lib.s3r_int8_linear(a, ap, p, b, bp, p, None, out, type, M, N, K, None)
     assert f(a=None) == -4 and f(M=0) == -1 and f(K=33) == -1 and f(type=9) == -2 and f(ap=65552, bp=65552, K=65537) == -6
+    r = lambda src=p + 1, sp=5, dst=p, dp=16, rows=3, K=5: lib.s3r_pad_rows(src, sp, dst, dp, rows, K, None)
+    assert r(src=None) == -4 and r(rows=0) == -1 and r(dp=8, K=9) == -1 and r(dp=24) == -3 and r(dst=p + 8) == -3
     assert f(a=p + 1) == -3 and f(ap=40) == -3 and f(b=p + 8) == -3 and f(out=p + 1) == -3
 
 

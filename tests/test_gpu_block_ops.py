@@ -300,9 +300,8 @@ def test_norm_without_rows():
 # ---- 8 bits --------------------------------------------------------------------------------------------------------------
 def quantised(x):
     big = x.float().abs().amax(-1)
-    most = torch.full_like(big, 127)                  # a tensor: with a number PyTorch multiplies by reciprocals, and rounds twice
-    q = torch.where(big[..., None] > 0, x.float() * (most / big)[..., None], 0).round()
-    return q.to(torch.int8), big / most
+    q = torch.where(big[..., None] > 0, x.float() * (127 / big)[..., None], 0).round()        # 127 / big: big's reciprocal, times 127
+    return q.to(torch.int8), big / torch.full_like(big, 127)                                  # by a tensor: PyTorch multiplies by 1 / 127
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -390,6 +389,17 @@ def test_int8_linear_shapes_pitches_and_addresses():
         got = ops.int8_linear(a, s[: a.shape[0]], b, ws, None, torch.float32)
         assert torch.equal(got, (a.double() @ b.double().T).float())
     assert ops.int8_linear(whole[:0], s[:0], w, ws).shape == (0, 72)
+
+
+@pytest.mark.parametrize("K", [1, 5, 16, 17, 31, 33, 1001, 4095])
+def test_int8_linear_operands_that_begin_anywhere(K):
+    """Tight rows of odd length, at any byte of a buffer: nothing in front of them or behind them is read."""
+    for start in (0, 1, 2, 3, 5):
+        flat_a, flat_b = int8(start + 20 * K), int8(start + 37 * K)
+        a, b = flat_a[start:].view(20, K), flat_b[start:].view(37, K)
+        for m in (20, 3):
+            got = ops.int8_linear(a[:m], torch.ones(m, device=DEV), b, torch.ones(37, device=DEV), None, torch.float32)
+            assert torch.equal(got, (a[:m].double() @ b.double().T).float())
 
 
 def test_int8_linear_rows_of_scales_that_are_not_finite():

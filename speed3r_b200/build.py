@@ -80,7 +80,7 @@ def _build_torch_lib() -> None:
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-o", TORCH_LIB] + srcs + [
         f"-I{inc}", f"-I{inc}/torch/csrc/api/include", f"-I{cuda}/include",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-        f"-L{PKG}", "-l:libspeed3r_b200.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+        f"-L{PKG}", "-l:libspeed3r_b200.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
         f"-L{cuda}/lib64", "-lcudart"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -6,6 +6,7 @@
 // the codes' grid stands still between steps.  Rounding a v that moves by 0.1 % a step then has a variance of step size x change
 // (with any other factor every code would be rounded anew each step, with step size^2 / 6, 30 times as much, and to nearest it
 // would hardly ever move).  All scalings are exact: the only rounding of a state is that of its code.
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
@@ -13,7 +14,8 @@
 
 namespace s3r {
 
-constexpr int kAdamBlock = 256, kAdamThreads = 256, kAdamMax = 320;
+// Tensors per launch: their table is an argument of the kernel, 23 KB for 320; a launch of a few tensors copies a shorter one.
+constexpr int kAdamBlock = 256, kAdamThreads = 256, kAdamMax = 320, kAdamFew = 32;
 constexpr int kAdamWarps = kAdamThreads / 32;
 constexpr int kAdamPerCta = kAdamBlock * kAdamWarps;
 
@@ -36,14 +38,29 @@ struct AdamTensor {
   int64_t first;       // CTA
   uint32_t flags;      // types (2 bits each), vectors, 8-bit states, index << 8
 };
-struct AdamParams {
-  AdamTensor t[kAdamMax];
+struct AdamCommon {
   int n;
   float b1, c1, b2, c2, eps;
   int64_t seed;
   const AdamScalars* scalars;
 };
+template <int MAX>
+struct AdamParams {
+  AdamCommon c;
+  AdamTensor t[MAX];
+};
 constexpr uint32_t kAdamVector = 16, kAdamEight = 32;
+
+template <typename T>
+__device__ __forceinline__ int tensor_of(const T* t, int n, int64_t cta) {
+  int lo = 0, hi = n - 1;                    // the last tensor whose first CTA is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t[mid].first <= cta) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 
 struct BeginParams {
   int64_t* step;
@@ -218,7 +235,7 @@ __device__ __forceinline__ void load_block(Lane<EIGHT>& l, const AdamTensor& x, 
 }
 
 template <int W, bool EIGHT>
-__device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamParams& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
+__device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommon& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
   const int64_t at = block * kAdamBlock + lane * 8;
   const int p_type = x.flags & 3, g_type = x.flags >> 2 & 3;
   const bool nearest = p.seed < 0;
@@ -325,21 +342,11 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamParam
   }
 }
 
-__device__ __forceinline__ int tensor_of(const AdamTensor* t, int n, int64_t cta) {
-  int lo = 0, hi = n - 1;                    // the last tensor whose first CTA is not behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t[mid].first <= cta) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
 // A warp has one block.  What hides the latency of its loads is other warps: with 64 registers 32 of them fit an SM (227 M elements with
 // 8-bit states 750 us; with 80 registers 830, with 94 1025), and a loop over several blocks, with or without the next one on its way in
 // registers, lost more of them than it gained (1460 to 1830).
 template <bool EIGHT>
-__device__ __forceinline__ void run_block(const AdamParams& p, const AdamTensor& x, int64_t block, int lane) {
+__device__ __forceinline__ void run_block(const AdamCommon& p, const AdamTensor& x, int64_t block, int lane) {
   Lane<EIGHT> l;
   // whole blocks of tensors that begin at multiples of 16 bytes; what ends a tensor, and tensors that begin anywhere, element by element
   if ((x.flags & kAdamVector) && (block + 1) * kAdamBlock <= x.n) {
@@ -353,14 +360,15 @@ __device__ __forceinline__ void run_block(const AdamParams& p, const AdamTensor&
   }
 }
 
-__global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_constant__ AdamParams p) {
-  const AdamTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
+template <int MAX>
+__global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_constant__ AdamParams<MAX> p) {
+  const AdamTensor& x = p.t[tensor_of(p.t, p.c.n, blockIdx.x)];
   const int64_t block = (blockIdx.x - x.first) * kAdamWarps + (threadIdx.x >> 5);
   griddep_wait();
   griddep_launch();
   if (block * kAdamBlock >= x.n) return;
-  if (x.flags & kAdamEight) run_block<true>(p, x, block, threadIdx.x & 31);
-  else run_block<false>(p, x, block, threadIdx.x & 31);
+  if (x.flags & kAdamEight) run_block<true>(p.c, x, block, threadIdx.x & 31);
+  else run_block<false>(p.c, x, block, threadIdx.x & 31);
 }
 
 // ---- the norm of the gradients: squares in 64 bits, where every one of them is exact ------------------------------------
@@ -372,21 +380,17 @@ struct NormTensor {
   int64_t first;
   uint32_t flags;
 };
+template <int MAX>
 struct GradNormParams {
-  NormTensor t[kAdamMax];
-  int n;
   double* partial;
+  int n;
+  NormTensor t[MAX];
 };
 
-__global__ void __launch_bounds__(kNormThreads) grad_norm_kernel(const __grid_constant__ GradNormParams p) {
+template <int MAX>
+__global__ void __launch_bounds__(kNormThreads) grad_norm_kernel(const __grid_constant__ GradNormParams<MAX> p) {
   __shared__ double red[kNormThreads / 32];
-  int lo = 0, hi = p.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.t[mid].first <= blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
-  const NormTensor& x = p.t[lo];
+  const NormTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
   griddep_wait();
   griddep_launch();
   const int64_t from = (blockIdx.x - x.first) * kNormPerCta, to = min(x.n, from + kNormPerCta);
@@ -446,18 +450,14 @@ struct StateTensor {
   int64_t n, first;
   uint32_t flags;
 };
+template <int MAX>
 struct StateParams {
-  StateTensor t[kAdamMax];
   int n;
+  StateTensor t[MAX];
 };
-__global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_constant__ StateParams p) {
-  int lo = 0, hi = p.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.t[mid].first <= blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
-  const StateTensor& x = p.t[lo];
+template <int MAX>
+__global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_constant__ StateParams<MAX> p) {
+  const StateTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t block = (blockIdx.x - x.first) * kAdamWarps + warp, at = block * kAdamBlock + lane * 8;
   griddep_wait();
@@ -506,13 +506,23 @@ extern "C" int s3r_grad_norm(int n, const void* const* tensors, const int64_t* c
     S3R_REQUIRE(reinterpret_cast<uintptr_t>(tensors[i]) % type_bytes(types[i]) == 0, S3R_ERR_ALIGNMENT, "s3r_grad_norm: elements must be aligned");
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  GradNormParams p;
+  static thread_local GradNormParams<kAdamMax> p;
+  GradNormParams<kAdamFew> few;
   p.partial = static_cast<double*>(workspace);
   p.n = 0;
   int64_t ctas = 0, all = 0;
   for (int i = 0; i <= n; ++i) {
     if (p.n && (i == n || p.n == kAdamMax)) {
-      if (const int rc = launch(grad_norm_kernel, static_cast<unsigned>(ctas), kNormThreads, 0, st, p)) return rc;
+      int rc;
+      if (p.n <= kAdamFew) {
+        few.partial = p.partial;
+        few.n = p.n;
+        std::copy_n(p.t, p.n, few.t);
+        rc = launch(grad_norm_kernel<kAdamFew>, static_cast<unsigned>(ctas), kNormThreads, 0, st, few);
+      } else {
+        rc = launch(grad_norm_kernel<kAdamMax>, static_cast<unsigned>(ctas), kNormThreads, 0, st, p);
+      }
+      if (rc) return rc;
       p.partial += ctas;
       all += ctas;
       p.n = 0;
@@ -551,27 +561,36 @@ extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
   // log 0 = -inf: 1 - 0^t = 1
   const BeginParams b = {a.step, a.lr, a.lr_host, log(a.beta1), log(a.beta2), a.weight_decay, a.max_norm, a.norm, scalars};
   if (const int rc = launch(adamw_begin_kernel, 1u, 1, 0, st, b)) return rc;
-  AdamParams p;
-  p.b1 = static_cast<float>(a.beta1);
-  p.c1 = static_cast<float>(1.0 - a.beta1);
-  p.b2 = static_cast<float>(a.beta2);
-  p.c2 = static_cast<float>(1.0 - a.beta2);
-  p.eps = static_cast<float>(a.eps);
-  p.seed = a.seed;
-  p.scalars = scalars;
-  p.n = 0;
+  static thread_local AdamParams<kAdamMax> p;
+  AdamParams<kAdamFew> few;
+  p.c.b1 = static_cast<float>(a.beta1);
+  p.c.c1 = static_cast<float>(1.0 - a.beta1);
+  p.c.b2 = static_cast<float>(a.beta2);
+  p.c.c2 = static_cast<float>(1.0 - a.beta2);
+  p.c.eps = static_cast<float>(a.eps);
+  p.c.seed = a.seed;
+  p.c.scalars = scalars;
+  p.c.n = 0;
   int64_t ctas = 0;
   for (int i = 0; i <= a.n; ++i) {
-    if (p.n && (i == a.n || p.n == kAdamMax)) {
-      if (const int rc = launch(adamw_kernel, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p)) return rc;
-      p.n = 0;
+    if (p.c.n && (i == a.n || p.c.n == kAdamMax)) {
+      int rc;
+      if (p.c.n <= kAdamFew) {
+        few.c = p.c;
+        std::copy_n(p.t, p.c.n, few.t);
+        rc = launch(adamw_kernel<kAdamFew>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
+      } else {
+        rc = launch(adamw_kernel<kAdamMax>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
+      }
+      if (rc) return rc;
+      p.c.n = 0;
       ctas = 0;
     }
     if (i == a.n || a.counts[i] == 0) continue;
     uint8_t *me = a.m_exponents ? a.m_exponents[i] : nullptr, *ve = a.v_exponents ? a.v_exponents[i] : nullptr;
     const uint32_t flags = static_cast<uint32_t>(a.param_types[i]) | static_cast<uint32_t>(a.grad_types[i]) << 2 |
                            (at_16({a.params[i], a.grads[i], a.m[i], a.v[i]}) ? kAdamVector : 0u) | (me ? kAdamEight : 0u) | static_cast<uint32_t>(i) << 8;
-    p.t[p.n++] = {a.params[i], a.grads[i], a.m[i], a.v[i], me, ve, a.counts[i], ctas, flags};
+    p.t[p.c.n++] = {a.params[i], a.grads[i], a.m[i], a.v[i], me, ve, a.counts[i], ctas, flags};
     ctas += (a.counts[i] + kAdamPerCta - 1) / kAdamPerCta;
     S3R_REQUIRE(ctas < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_adamw_step: grid too large");
   }
@@ -588,12 +607,21 @@ extern "C" int s3r_adamw_state(int n, const void* const* m, const void* const* v
     S3R_REQUIRE((reinterpret_cast<uintptr_t>(m_out[i]) | reinterpret_cast<uintptr_t>(v_out[i])) % 4 == 0, S3R_ERR_ALIGNMENT, "s3r_adamw_state: elements must be aligned");
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  StateParams p;
+  static thread_local StateParams<kAdamMax> p;
+  StateParams<kAdamFew> few;
   p.n = 0;
   int64_t ctas = 0;
   for (int i = 0; i <= n; ++i) {
     if (p.n && (i == n || p.n == kAdamMax)) {
-      if (const int rc = launch(adamw_state_kernel, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p)) return rc;
+      int rc;
+      if (p.n <= kAdamFew) {
+        few.n = p.n;
+        std::copy_n(p.t, p.n, few.t);
+        rc = launch(adamw_state_kernel<kAdamFew>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
+      } else {
+        rc = launch(adamw_state_kernel<kAdamMax>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
+      }
+      if (rc) return rc;
       p.n = 0;
       ctas = 0;
     }

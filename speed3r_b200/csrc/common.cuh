@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/speed3r_b200.h"
 
 namespace s3r {
@@ -58,6 +60,18 @@ PairOrder pair_order(uint64_t a, uint64_t b);
 int make_pair_map(PairMap* out, const void* a, const void* b, int T, int BH, int chunks, int64_t chunk_stride_bytes);
 
 int sm_count();
+
+// Whether a kernel's attributes are still to be set on the current device (`done`: the kernel's own, a bit per device), and that they are.
+// Setting them on every call costs a microsecond of it.
+inline uint64_t device_bit() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? 1ull << dev : 0;
+}
+inline bool attributes_missing(const std::atomic<uint64_t>& done) {
+  const uint64_t bit = device_bit();
+  return !bit || !(done.load(std::memory_order_acquire) & bit);
+}
+inline void attributes_set(std::atomic<uint64_t>& done) { done.fetch_or(device_bit(), std::memory_order_release); }
 
 #ifdef __CUDACC__
 // Launch of a kernel whose CTAs may start while the kernel before it in the stream is still finishing (programmatic

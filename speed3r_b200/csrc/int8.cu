@@ -539,7 +539,11 @@ static int launch_int8(const int8_t* a, int64_t a_pitch, const int8_t* b, int64_
   p.n_tiles = (p.N + TN - 1) / TN;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles, at_once = sm_count() / CTAS;
   S3R_REQUIRE(tiles < (1ll << 31) - 1024, S3R_ERR_TOO_LARGE, "s3r_int8_linear: too many tiles");
-  S3R_CUDA(cudaFuncSetAttribute(int8_linear_kernel<TN, CTAS, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static std::atomic<uint64_t> ready{0};
+  if (attributes_missing(ready)) {
+    S3R_CUDA(cudaFuncSetAttribute(int8_linear_kernel<TN, CTAS, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    attributes_set(ready);
+  }
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(static_cast<unsigned>((tiles < at_once ? tiles : at_once) * CTAS));
   c.blockDim = dim3(kI8Threads);

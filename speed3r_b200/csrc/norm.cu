@@ -718,7 +718,11 @@ static int run_rows(NormParams p, cudaStream_t st) {
   const int stage = G * E * (type_bytes(p.a.x_type) + type_bytes(p.a.y_type)), room = kRowsSmem / kResident / kRows / stage;
   p.stages = room < 4 ? room : 4;
   const int64_t want = (p.rows + kRows - 1) / kRows, most = static_cast<int64_t>(sm_count()) * kResident;
-  S3R_CUDA(cudaFuncSetAttribute(norm_rows_kernel<W, G, E, FULL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+  static std::atomic<uint64_t> ready{0};
+  if (attributes_missing(ready)) {
+    S3R_CUDA(cudaFuncSetAttribute(norm_rows_kernel<W, G, E, FULL, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+    attributes_set(ready);
+  }
   return launch(norm_rows_kernel<W, G, E, FULL, WIDE>, static_cast<unsigned>(want < most ? want : most), kThreads,
                 static_cast<size_t>(kRows) * p.stages * stage, st, p);
 }
@@ -762,7 +766,11 @@ template <int W, int G, int E, bool FULL>
 static int run_bwd(const NormBwdParams& p, unsigned ctas, cudaStream_t st) {
   constexpr int kThreads = G < 128 ? 128 : G, kGroups = kThreads / G;
   static_assert(kGroups * E * G * 4 <= kRowsSmem, "sums of the groups");
-  S3R_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<W, G, E, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+  static std::atomic<uint64_t> ready{0};
+  if (attributes_missing(ready)) {
+    S3R_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<W, G, E, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem));
+    attributes_set(ready);
+  }
   size_t smem = W > 1 ? static_cast<size_t>(kGroups) * p.stages * p.stage_bytes : 0;
   if constexpr (kGroups > 1) {
     constexpr size_t kSumBytes = static_cast<size_t>(kGroups) * E * G * 4;

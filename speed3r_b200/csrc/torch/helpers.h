@@ -5,6 +5,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/CachingHostAllocator.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -50,11 +51,13 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 const int32_t* i32(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
 int32_t* i32m(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 float* f32(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+// Through the dispatcher an empty tensor takes twice as long (1.4 us), and a small call is made of such times.
 Tensor fresh(at::IntArrayRef shape, const Tensor& like, at::ScalarType dtype) {
+  if (like.is_cuda()) return at::detail::empty_cuda(shape, dtype, like.device(), c10::nullopt);
   return at::empty(shape, like.options().dtype(dtype));
 }
 // contiguous, whatever the strides of `t` (at::empty_like would keep a permuted layout)
-Tensor fresh_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
+Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t, t.scalar_type()); }
 // The same values at a multiple of 16 bytes: a contiguous view may begin anywhere in its storage (a slice, a flattened
 // parameter buffer), and the kernels load vectors.
 Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }

@@ -248,12 +248,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
       bit *= 2;
     }
     ctx->save_for_backward({branch ? r : x, needs_y ? *y : Tensor(), value(w), value(s), value(g), value(pw), value(pb), stats});
-    ctx->saved_data["present"] = present;
-    ctx->saved_data["branch"] = branch;
-    ctx->saved_data["y_type"] = static_cast<int64_t>(branch ? y->scalar_type() : x.scalar_type());
-    ctx->saved_data["post"] = post;
-    ctx->saved_data["kind"] = kind;
-    ctx->saved_data["param"] = static_cast<int64_t>(param);
+    ctx->saved_data["ints"] = std::vector<int64_t>{present, branch, static_cast<int64_t>(branch ? y->scalar_type() : x.scalar_type()), post, kind,
+                                                  static_cast<int64_t>(param)};
     ctx->set_materialize_grads(false);
     variable_list out;
     if (branch) out.push_back(r);
@@ -266,22 +262,23 @@ struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list gradients(AutogradContext* ctx, const variable_list& incoming) {
     variable_list out(14);
     const auto s = ctx->get_saved_variables();
-    const bool branch = ctx->saved_data["branch"].toBool(), post = ctx->saved_data["post"].toBool();
+    const auto ints = ctx->saved_data["ints"].toIntVector();
+    const int64_t present = ints[0];
+    const bool branch = ints[1], post = ints[3];
     auto given = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t.contiguous()) : optional<Tensor>(); };
     const optional<Tensor> dr = branch ? given(incoming[0]) : optional<Tensor>();
     const optional<Tensor> dh = incoming.size() > (branch ? 1u : 0u) ? given(incoming.back()) : optional<Tensor>();
     if (!dr.has_value() && !dh.has_value()) return out;
     int64_t want = 0;
-    const int64_t present = ctx->saved_data["present"].toInt();
     for (int i = 0, edge = 0; i < 8; ++i)
       if (present >> i & 1 && ctx->needs_input_grad(edge++)) want |= int64_t{1} << i;
     if (!branch) want &= kX | kWeight | kBias;
     // a branch that nothing is multiplied with is not kept, only its type
     optional<at::ScalarType> branch_type;
-    if (branch) branch_type = static_cast<at::ScalarType>(ctx->saved_data["y_type"].toInt());
+    if (branch) branch_type = static_cast<at::ScalarType>(ints[2]);
     const auto& backward = plain(s[0]) ? run_norm_bwd : call_norm_bwd;
-    const auto g = backward(s[0], maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, branch_type, post, ctx->saved_data["kind"].toInt(),
-                                 want, static_cast<at::ScalarType>(ctx->saved_data["param"].toInt()));
+    const auto g = backward(s[0], maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), maybe(s[5]), maybe(s[6]), s[7], dr, dh, branch_type, post, ints[4],
+                                 want, static_cast<at::ScalarType>(ints[5]));
     for (int i = 0; i < 8; ++i)
       if (want >> i & 1 && g[i].defined() && (dh.has_value() || !(i == 2 || i == 3))) out[i] = g[i];
     return out;

@@ -15,7 +15,7 @@
 namespace s3r {
 
 // Tensors per launch: their table is an argument of the kernel, 23 KB for 320; a launch of a few tensors copies a shorter one.
-constexpr int kAdamBlock = 256, kAdamThreads = 256, kAdamMax = 320, kAdamFew = 32;
+constexpr int kAdamBlock = 256, kAdamThreads = 128, kAdamMax = 320, kAdamFew = 32;
 constexpr int kAdamWarps = kAdamThreads / 32;
 constexpr int kAdamPerCta = kAdamBlock * kAdamWarps;
 
@@ -44,22 +44,40 @@ struct AdamCommon {
   int64_t seed;
   const AdamScalars* scalars;
 };
+// Which tensor the CTAs i << shift belong to: a search through all of 252 tensors was a twelfth of the time (0.9 M elements each: 645 us, this way 603).
+template <int MAX>
+struct Starts {
+  uint16_t at[MAX + 1];
+  int shift;
+};
+template <int MAX, typename T>
+static void fill_starts(Starts<MAX>& s, const T* t, int n, int64_t ctas) {
+  s.shift = 0;
+  while ((ctas - 1) >> s.shift >= MAX) ++s.shift;
+  const int last = static_cast<int>((ctas - 1) >> s.shift);
+  for (int b = 0, i = 0; b <= last; ++b) {
+    while (i + 1 < n && t[i + 1].first <= static_cast<int64_t>(b) << s.shift) ++i;
+    s.at[b] = static_cast<uint16_t>(i);
+  }
+  s.at[last + 1] = static_cast<uint16_t>(n - 1);
+}
 template <int MAX>
 struct AdamParams {
   AdamCommon c;
+  Starts<MAX> starts;
   AdamTensor t[MAX];
 };
 constexpr uint32_t kAdamVector = 16, kAdamEight = 32;
 
-template <typename T>
-__device__ __forceinline__ int tensor_of(const T* t, int n, int64_t cta) {
-  int lo = 0, hi = n - 1;                    // the last tensor whose first CTA is not behind this one
+template <typename T, int MAX>
+__device__ __forceinline__ const T& tensor_of(const T (&t)[MAX], const Starts<MAX>& s, int64_t cta) {
+  int lo = s.at[cta >> s.shift], hi = s.at[(cta >> s.shift) + 1];          // the last tensor whose first CTA is not behind this one
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (t[mid].first <= cta) lo = mid;
     else hi = mid - 1;
   }
-  return lo;
+  return t[lo];
 }
 
 struct BeginParams {
@@ -117,12 +135,12 @@ constexpr float kUpM = 5.19229685853482763e33f, kUpV = 7.92281625142643376e28f;
 __device__ __forceinline__ float unit_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fffffffu) : power_of(e); }
 __device__ __forceinline__ float2 both_of(float x) { return make_float2(x, x); }
 
-// four bytes into the top of four words
-__device__ __forceinline__ void spread(uint32_t (&w)[4], uint32_t bytes) {
-  w[0] = bytes << 24;
-  w[1] = __byte_perm(bytes, 0, 0x1444);
-  w[2] = __byte_perm(bytes, 0, 0x2444);
-  w[3] = bytes & 0xff000000u;
+// byte k of a word times 2^20; SIGN: its highest bit in all bits above
+template <bool SIGN>
+__device__ __forceinline__ uint32_t code_bits(uint32_t bytes, int k) {
+  uint32_t w;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(w) : "r"(bytes), "r"((SIGN ? 0x8044u + (k << 12) : 0x4044u) + (k << 8)));
+  return w * 16u;
 }
 // the top bytes of four words
 __device__ __forceinline__ uint32_t gather(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -132,9 +150,8 @@ __device__ __forceinline__ void decode_m(float2 (&m)[4], uint2 codes, float unit
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t w[4];
-    spread(w, h ? codes.y : codes.x);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = static_cast<uint32_t>(static_cast<int32_t>(w[k]) >> 4) & 0x87f00000u;      // sign, code << 20
+    for (int k = 0; k < 4; ++k) w[k] = code_bits<true>(h ? codes.y : codes.x, k) & 0x87f00000u;      // sign, code << 20
     m[2 * h] = fmul2(fmul2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), both_of(kUpM)), both_of(unit));
     m[2 * h + 1] = fmul2(fmul2(make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), both_of(kUpM)), both_of(unit));
   }
@@ -143,9 +160,8 @@ __device__ __forceinline__ void decode_v(float2 (&v)[4], uint2 codes, float unit
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t w[4];
-    spread(w, h ? codes.y : codes.x);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] >>= 4;
+    for (int k = 0; k < 4; ++k) w[k] = code_bits<false>(h ? codes.y : codes.x, k);
     v[2 * h] = fmul2(fmul2(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])), both_of(kUpV)), both_of(unit));
     v[2 * h + 1] = fmul2(fmul2(make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), both_of(kUpV)), both_of(unit));
   }
@@ -153,6 +169,11 @@ __device__ __forceinline__ void decode_v(float2 (&v)[4], uint2 codes, float unit
 __device__ __forceinline__ float sqrt_near(float x) {
   float y;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_abs(float a, float b, float c) {       // of the magnitudes; NaN if one is
+  float y;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ float rcp_near(float x) {
@@ -196,6 +217,17 @@ __device__ __forceinline__ void store_lane(const float2 (&f)[4], void* p, int ty
         pack<1>(r, one, type);
         store_raw<1>(r, p, type, at + k);
       }
+  }
+}
+// Eight fp32 values of a lane, the array at a multiple of 16 bytes.  One store where they fill a sector of 32 bytes: in two, each of a warp's
+// stores touches all its sectors (reading out 60 M elements: 108 us, this way 84).  The step, which reads more than it writes, gains nothing.
+__device__ __forceinline__ void store_sector(const float2 (&f)[4], float* p) {
+  if (reinterpret_cast<uintptr_t>(p) & 31) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+  } else {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "f"(f[0].x), "f"(f[0].y), "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y) : "memory");
   }
 }
 template <int W>
@@ -288,48 +320,41 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
     store_lane<W>(m, x.m, S3R_F32, at, x.n);
     store_lane<W>(v, x.v, S3R_F32, at, x.n);
   } else {
-    // magnitudes compare as integers, NaN above all
-    uint32_t am[8], av[8], m_big = 0, v_big = 0;
+    // the largest magnitudes; NaN above all, as bits too
+    float m_top = 0.f, v_top = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      am[2 * k] = __float_as_uint(m[k].x) & 0x7fffffffu, am[2 * k + 1] = __float_as_uint(m[k].y) & 0x7fffffffu;
-      av[2 * k] = __float_as_uint(v[k].x) & 0x7fffffffu, av[2 * k + 1] = __float_as_uint(v[k].y) & 0x7fffffffu;
-      m_big = max(m_big, max(am[2 * k], am[2 * k + 1]));
-      v_big = max(v_big, max(av[2 * k], av[2 * k + 1]));
-    }
-    m_big = __reduce_max_sync(0xffffffffu, m_big);
-    v_big = __reduce_max_sync(0xffffffffu, v_big);
-    const uint32_t me = block_exponent(m_big), ve = block_exponent(v_big);
+    for (int k = 0; k < 4; ++k) m_top = max_abs(m_top, m[k].x, m[k].y), v_top = max_abs(v_top, v[k].x, v[k].y);
+    const uint32_t me = block_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(m_top)));
+    const uint32_t ve = block_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v_top)));
     const float m_up = me == 255u ? 0.f : power_of(254u - me), v_up = ve == 255u ? 0.f : power_of(254u - ve);
     uint32_t mc[8], vc[8];
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
-      const float2 a = fmul2(fmul2(make_float2(__uint_as_float(am[k]), __uint_as_float(am[k + 1])), both_of(m_up)), both_of(kDownM));
-      const float2 b = fmul2(fmul2(make_float2(__uint_as_float(av[k]), __uint_as_float(av[k + 1])), both_of(v_up)), both_of(kDownV));
+      const float2 a = fmul2(fmul2(m[k / 2], both_of(m_up)), both_of(kDownM)), b = fmul2(fmul2(v[k / 2], both_of(v_up)), both_of(kDownV));
       mc[k] = __float_as_uint(a.x), mc[k + 1] = __float_as_uint(a.y);
       vc[k] = __float_as_uint(b.x), vc[k + 1] = __float_as_uint(b.y);
     }
-    // 8 random bits of the 20 that a code of m drops, 14 of v's: v moves less in a step.  No code passes its largest one: the block's
-    // exponent is such that 1.875 times the power of two is reached exactly at most.
-    if (nearest) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        mc[k] += 0x7FFFFu + (mc[k] >> 20 & 1u);
-        vc[k] += 0x7FFFFu + (vc[k] >> 20 & 1u);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        mc[k] += (low[k] << 12 & 0xFF000u) + 0x800u;
-        vc[k] += (low[k] >> 2 & 0xFFFC0u) + 0x20u;
-      }
-    }
+    // To the top byte, rounded on the way (16 x + 16 r).  8 random bits of the 20 that a code of m drops, 14 of v's: v moves less in a step.
+    // No code passes its largest one: the block's exponent is such that 1.875 times the power of two is reached exactly at most.
+    uint32_t v_least = 0xffffffffu;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t sign = __float_as_uint(k & 1 ? m[k / 2].y : m[k / 2].x);
-      mc[k] = (mc[k] << 4 & 0x7f000000u) | (sign & ~0x7f000000u);          // only the top byte is used
-      // a v that is not zero keeps a code that is not: a denominator never becomes eps alone by rounding
-      vc[k] = max(vc[k], av[k] ? 1u << 20 : 0u) << 4;
+      const uint32_t sign = mc[k];
+      if (nearest) {
+        mc[k] = (mc[k] + 0x7FFFFu + (mc[k] >> 20 & 1u)) * 16u;
+        vc[k] = (vc[k] + 0x7FFFFu + (vc[k] >> 20 & 1u)) * 16u;
+      } else {
+        mc[k] = mc[k] * 16u + __byte_perm(low[k], 0x8000u, 0x7054);                      // low[7:0] << 16, half of the last bit below
+        vc[k] = (vc[k] * 4u + ((low[k] & 0x3FFF00u) | 0x80u)) * 4u;
+      }
+      mc[k] = (mc[k] & 0x7fffffffu) | (sign & 0x80000000u);
+      v_least = min(v_least, vc[k]);
+    }
+    // a v that is not zero keeps a code that is not: a denominator never becomes eps alone by rounding
+    if (v_least < 1u << 24) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (vc[k] < 1u << 24 && (k & 1 ? v[k / 2].y : v[k / 2].x) != 0.f) vc[k] = 1u << 24;
     }
     const uint2 m_codes = make_uint2(gather(mc[0], mc[1], mc[2], mc[3]), gather(mc[4], mc[5], mc[6], mc[7]));
     const uint2 v_codes = make_uint2(gather(vc[0], vc[1], vc[2], vc[3]), gather(vc[4], vc[5], vc[6], vc[7]));
@@ -342,9 +367,10 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
   }
 }
 
-// A warp has one block.  What hides the latency of its loads is other warps: with 64 registers 32 of them fit an SM (227 M elements with
-// 8-bit states 750 us; with 80 registers 830, with 94 1025), and a loop over several blocks, with or without the next one on its way in
-// registers, lost more of them than it gained (1460 to 1830).
+// A warp has one block.  What hides the latency of its loads is other warps: with 56 registers 36 of them fit an SM (227 M elements in 252
+// tensors, 8-bit states, 601 us = 6.0 TB/s; with 64 registers 629, with 48, which spill, a hundredth more than with 56), and a loop over several
+// blocks, with or without the next one on its way in registers, lost more of them than it gained.  CTAs of 128 leave an SM in smaller
+// parts than those of 256 (640 where those take 715).
 template <bool EIGHT>
 __device__ __forceinline__ void run_block(const AdamCommon& p, const AdamTensor& x, int64_t block, int lane) {
   Lane<EIGHT> l;
@@ -361,8 +387,8 @@ __device__ __forceinline__ void run_block(const AdamCommon& p, const AdamTensor&
 }
 
 template <int MAX>
-__global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_constant__ AdamParams<MAX> p) {
-  const AdamTensor& x = p.t[tensor_of(p.t, p.c.n, blockIdx.x)];
+__global__ void __launch_bounds__(kAdamThreads, 9) adamw_kernel(const __grid_constant__ AdamParams<MAX> p) {
+  const AdamTensor& x = tensor_of(p.t, p.starts, blockIdx.x);
   const int64_t block = (blockIdx.x - x.first) * kAdamWarps + (threadIdx.x >> 5);
   griddep_wait();
   griddep_launch();
@@ -384,13 +410,14 @@ template <int MAX>
 struct GradNormParams {
   double* partial;
   int n;
+  Starts<MAX> starts;
   NormTensor t[MAX];
 };
 
 template <int MAX>
 __global__ void __launch_bounds__(kNormThreads) grad_norm_kernel(const __grid_constant__ GradNormParams<MAX> p) {
   __shared__ double red[kNormThreads / 32];
-  const NormTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
+  const NormTensor& x = tensor_of(p.t, p.starts, blockIdx.x);
   griddep_wait();
   griddep_launch();
   const int64_t from = (blockIdx.x - x.first) * kNormPerCta, to = min(x.n, from + kNormPerCta);
@@ -453,11 +480,12 @@ struct StateTensor {
 template <int MAX>
 struct StateParams {
   int n;
+  Starts<MAX> starts;
   StateTensor t[MAX];
 };
 template <int MAX>
 __global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_constant__ StateParams<MAX> p) {
-  const StateTensor& x = p.t[tensor_of(p.t, p.n, blockIdx.x)];
+  const StateTensor& x = tensor_of(p.t, p.starts, blockIdx.x);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t block = (blockIdx.x - x.first) * kAdamWarps + warp, at = block * kAdamBlock + lane * 8;
   griddep_wait();
@@ -469,8 +497,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_state_kernel(const __grid_
   decode_m(m, mc, unit_of(x.me[block]));
   decode_v(v, vc, unit_of(x.ve[block]));
   if (whole) {
-    store_lane<8>(m, x.m_out, S3R_F32, at, x.n);
-    store_lane<8>(v, x.v_out, S3R_F32, at, x.n);
+    store_sector(m, x.m_out + at);
+    store_sector(v, x.v_out + at);
   } else {
     store_lane<1>(m, x.m_out, S3R_F32, at, x.n);
     store_lane<1>(v, x.v_out, S3R_F32, at, x.n);
@@ -518,8 +546,10 @@ extern "C" int s3r_grad_norm(int n, const void* const* tensors, const int64_t* c
         few.partial = p.partial;
         few.n = p.n;
         std::copy_n(p.t, p.n, few.t);
+        fill_starts(few.starts, p.t, p.n, ctas);
         rc = launch(grad_norm_kernel<kAdamFew>, static_cast<unsigned>(ctas), kNormThreads, 0, st, few);
       } else {
+        fill_starts(p.starts, p.t, p.n, ctas);
         rc = launch(grad_norm_kernel<kAdamMax>, static_cast<unsigned>(ctas), kNormThreads, 0, st, p);
       }
       if (rc) return rc;
@@ -578,8 +608,10 @@ extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
       if (p.c.n <= kAdamFew) {
         few.c = p.c;
         std::copy_n(p.t, p.c.n, few.t);
+        fill_starts(few.starts, p.t, p.c.n, ctas);
         rc = launch(adamw_kernel<kAdamFew>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
       } else {
+        fill_starts(p.starts, p.t, p.c.n, ctas);
         rc = launch(adamw_kernel<kAdamMax>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
       }
       if (rc) return rc;
@@ -617,8 +649,10 @@ extern "C" int s3r_adamw_state(int n, const void* const* m, const void* const* v
       if (p.n <= kAdamFew) {
         few.n = p.n;
         std::copy_n(p.t, p.n, few.t);
+        fill_starts(few.starts, p.t, p.n, ctas);
         rc = launch(adamw_state_kernel<kAdamFew>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
       } else {
+        fill_starts(p.starts, p.t, p.n, ctas);
         rc = launch(adamw_state_kernel<kAdamMax>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
       }
       if (rc) return rc;

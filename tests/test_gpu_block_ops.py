@@ -609,6 +609,44 @@ def test_adamw_state_is_what_codes_stand_for():
     assert torch.equal(whole[0][1:], m) and whole[0][0] == 0
 
 
+@pytest.mark.parametrize("off", [0, 4, 1])
+def test_adamw_state_of_outputs_that_begin_anywhere(off):
+    """At a multiple of 32 bytes, of 16 and of neither; what is around them stays."""
+    n = 5000
+    codes = torch.randint(0, 256, (n,), device=DEV, dtype=torch.uint8)
+    e = torch.randint(90, 160, (2, -(-n // 256)), device=DEV, dtype=torch.uint8)
+    whole = torch.full((2, n + 9), 3.0, device=DEV)
+    m, v = whole[0][off:off + n], torch.full((n + 9,), 3.0, device=DEV)[off:off + n]
+    ops.adamw_state([codes], [codes], [e], out=([m], [v]))
+    assert torch.equal(m.double(), values(codes, e[0], 4)) and torch.equal(v.double(), values(codes, e[1], 5))
+    assert (whole[0][:off] == 3).all() and (whole[0][off + n:] == 3).all()
+
+
+@pytest.mark.parametrize("sizes", [[1, 2_000_000, 5, 256, 257, 900_000, 3], [7, 300_000, 1] * 9, [40_000, 1, 513, 90_000, 2, 2, 1025, 600_000] * 50],
+                         ids=["7", "27", "400"])
+@pytest.mark.parametrize("eight", [False, True])
+def test_adamw_finds_every_tensor(sizes, eight):
+    """All in one call and one by one: bit for bit the same."""
+    gen = torch.Generator(device=DEV).manual_seed(len(sizes))
+    p, g = ([torch.randn(n, device=DEV, generator=gen) for n in sizes] for _ in range(2))
+    m, v = ([torch.randint(0, 127, (n,), device=DEV, dtype=torch.uint8, generator=gen) if eight else torch.rand(n, device=DEV, generator=gen) for n in sizes]
+            for _ in range(2))
+    e = [torch.randint(110, 130, (2, -(-n // 256)), device=DEV, dtype=torch.uint8, generator=gen) for n in sizes] if eight else None
+    all_at_once = [[t.clone() for t in x] if x else None for x in (p, m, v, e)]
+    step = torch.zeros((), dtype=torch.int64, device=DEV)
+    ops.adamw_step(all_at_once[0], g, all_at_once[1], all_at_once[2], step, scales=all_at_once[3])
+    for i in range(len(sizes)):
+        step.zero_()
+        ops.adamw_step([p[i]], [g[i]], [m[i]], [v[i]], step, scales=[e[i]] if eight else None)
+    for x, y in zip((p, m, v, e), all_at_once):
+        assert x is None or all(torch.equal(a, b) for a, b in zip(x, y))
+    want = sum((t.double() ** 2).sum() for t in g).sqrt()
+    assert abs(ops.grad_norm(g).double() - want) <= 2.0 ** -23 * want
+    if eight:
+        for out, codes, k, bits in zip(ops.adamw_state(m, v, e), (m, v), (0, 1), (4, 5)):
+            assert all(torch.equal(o.double(), values(c, s[k], bits)) for o, c, s in zip(out, codes, e))
+
+
 def test_adamw_lr_on_the_device_and_mixed_states():
     a, b = Adam([(5000,), (10,)], seed=2), Adam([(5000,), (10,)], seed=2)
     ops.adamw_step(a.params, a.grads, a.m, a.v, a.step, lr=0.03)

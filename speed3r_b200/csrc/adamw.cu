@@ -171,11 +171,6 @@ __device__ __forceinline__ float sqrt_near(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max_abs(float a, float b, float c) {       // of the magnitudes; NaN if one is
-  float y;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 __device__ __forceinline__ float rcp_near(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -25,7 +25,7 @@ __device__ __forceinline__ void store_s8(int8_t* q, const float (&f)[W], float i
     uint32_t w[W / 4];
 #pragma unroll
     for (int k = 0; k < W; k += 4)
-      w[k / 4] = to_s8(f[k], inverse) | to_s8(f[k + 1], inverse) << 8 | to_s8(f[k + 2], inverse) << 16 | to_s8(f[k + 3], inverse) << 24;
+      w[k / 4] = to_s8x4(f + k, inverse);
     if constexpr (W == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(q) = w[0];
   }
@@ -54,8 +54,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) quantize_kernel(const __gri
       if ((i * G + t) * W < C) {
         float f[W];
         unpack<W>(f, r[i], p.type);
-#pragma unroll
-        for (int k = 0; k < W; ++k) big = max_nan(big, fabsf(f[k]));
+        big = max_abs<W>(big, f);
       }
     big = row_max<G>(big, red, turn, t, 0);
     const RowScale s = row_scale(big);
@@ -71,8 +70,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) quantize_kernel(const __gri
     for (int c = t * W; c < C; c += G * W) {
       float f[W];
       load_vector<W>(f, p.x, p.type, at + c);
-#pragma unroll
-      for (int k = 0; k < W; ++k) big = max_nan(big, fabsf(f[k]));
+      big = max_abs<W>(big, f);
     }
     big = row_max<G>(big, red, turn, t, 0);
     const RowScale s = row_scale(big);

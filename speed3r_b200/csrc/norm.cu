@@ -105,9 +105,7 @@ __device__ __forceinline__ void store_int8(const float (&v)[E], const s3r_residu
   float big = 0.f;
 #pragma unroll
   for (int i = 0; i < E / W; ++i)
-    if ((i * G + t) * W < a.channels)
-#pragma unroll
-      for (int k = 0; k < W; ++k) big = max_nan(big, fabsf(v[i * W + k]));
+    if ((i * G + t) * W < a.channels) big = max_abs<W>(big, v + i * W);
   big = row_max<G>(big, red, turn, t, bar);
   const RowScale s = row_scale(big);
   if (t == 0) a.q_scale[row] = s.scale;
@@ -119,9 +117,7 @@ __device__ __forceinline__ void store_int8(const float (&v)[E], const s3r_residu
         *q = static_cast<int8_t>(to_s8(v[i], s.inverse));
       } else {
 #pragma unroll
-        for (int k = 0; k < W; k += 4)
-          *reinterpret_cast<uint32_t*>(q + k) = to_s8(v[i * W + k], s.inverse) | to_s8(v[i * W + k + 1], s.inverse) << 8 |
-                                                to_s8(v[i * W + k + 2], s.inverse) << 16 | to_s8(v[i * W + k + 3], s.inverse) << 24;
+        for (int k = 0; k < W; k += 4) *reinterpret_cast<uint32_t*>(q + k) = to_s8x4(v + i * W + k, s.inverse);
       }
     }
   }

@@ -230,6 +230,18 @@ __device__ __forceinline__ void cp_async_wait_for(int pending) {
 // packed product and scalar sums it does not.
 __device__ __forceinline__ float2 add_apart(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
 
+// the largest magnitude; NaN if one is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float y;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+template <int W>
+__device__ __forceinline__ float max_abs(float big, const float* v) {
+#pragma unroll
+  for (int k = 0; k + 1 < W; k += 2) big = max_abs(big, v[k], v[k + 1]);
+  return W & 1 ? max_abs(big, v[W - 1], 0.f) : big;
+}
 // max that keeps NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -250,6 +262,15 @@ __device__ __forceinline__ uint32_t to_s8(float v, float inverse) {
   int q;
   asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(__fmul_rn(v, inverse)));
   return static_cast<uint32_t>(q) & 0xffu;
+}
+// four of them, the first in the lowest byte
+__device__ __forceinline__ uint32_t to_s8x4(const float* v, float inverse) {
+  const float2 lo = fmul2(make_float2(v[0], v[1]), make_float2(inverse, inverse)), hi = fmul2(make_float2(v[2], v[3]), make_float2(inverse, inverse));
+  uint32_t w;
+  asm("{\n\t.reg .s32 a, b, c, d;\n\tcvt.rni.s32.f32 a, %1;\n\tcvt.rni.s32.f32 b, %2;\n\tcvt.rni.s32.f32 c, %3;\n\tcvt.rni.s32.f32 d, %4;\n\t"
+      "cvt.pack.sat.s8.s32.b32 c, d, c, 0;\n\tcvt.pack.sat.s8.s32.b32 %0, b, a, c;\n\t}"
+      : "=r"(w) : "f"(lo.x), "f"(lo.y), "f"(hi.x), "f"(hi.y));
+  return w;
 }
 
 // Sums of N values over the G threads of a row, in a fixed order.  Rows of more than a warp exchange their warps' sums through
@@ -278,10 +299,10 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* red, uint32_t& tur
     }
   }
 }
+// the largest of values that are not negative: their bits have the same order, NaN above all
 template <int G>
 __device__ __forceinline__ float row_max(float s, float* red, uint32_t& turn, int t, int bar) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s = max_nan(s, __shfl_xor_sync(0xffffffffu, s, o));
+  s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s)));
   if constexpr (G > 32) {
     constexpr int kWarps = G / 32;
     float* half = red + turn * (4 * kWarps);

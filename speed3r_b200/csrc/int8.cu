@@ -138,6 +138,10 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict_
 // product on tcgen05: persistent CTAs, K in steps of 128 bytes through a ring of TMA copies, the sums of two tiles in tensor memory
 // so that one is written out while the next is summed.  One warp copies, one issues the products, eight take the sums (32 rows and
 // half of the columns each), scale them and store through shared memory.
+// At K = 1024 what bounds it is shared memory, written by the copies, read by the products and passed through by the results: 64 512 x 4096
+// take 155 us without the results' part, 166 without the stores at its end, 201 with them.  Tried and not kept: sixteen warps for the sums
+// (220), stores from registers by way of shared memory (211) and, with a's rows of up to 1024 bytes staying where they are, half as
+// many bytes to copy but three steps of the ring in place of five (234; 156 without the stores).
 // CTAS = 2: a pair of CTAs multiplies 256 rows with TN columns; each holds 128 rows of a and half of b's rows, the products read both
 // halves.  A k-step then brings half as much of b into either CTA's shared memory, whose bandwidth bounds one CTA alone.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -426,17 +430,30 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
       ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      // 32 columns' sums, and the next 32 on their way: asked for under no condition, so that their registers have no other writer to
-      // wait for (asked for where they exist, a load beside the products cost its whole latency, 900 cycles, three times per tile).
+      // 32 columns' sums; once they are products the next 32 are asked for, under no condition, so that their registers have no other
+      // writer to wait for, and are on their way while these are stored.
       const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t v[2][32];
-      if (from < TN) tmem_ld_32x32(sums, v[0]);
+      uint32_t v[32];
+      if (from < TN) tmem_ld_32x32(sums, v);
 #pragma unroll
       for (int g = 0; g < kMine; ++g) {
-        uint32_t(&now)[32] = v[g & 1];
-        tmem_ld_wait_for(now);
+        float2 s[4], b[4], x[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[j] = *reinterpret_cast<const float2*>(columns + g * 32 + 8 * j + c);
+          b[j] = *reinterpret_cast<const float2*>(columns + C::kSpan + g * 32 + 8 * j + c);
+        }
+        tmem_ld_wait_for(v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
+            const float2 sum = make_float2(__int2float_rn(static_cast<int>(v[k])), __int2float_rn(static_cast<int>(v[k + 1])));
+            x[j][i] = ffma2(fmul2(sum, make_float2(row[i], row[i])), s[j], b[j]);
+          }
         if (g + 1 < kMine) {
-          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v[(g + 1) & 1]);
+          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v);
         } else {                                                   // this warp's sums are in registers
           tc_fence_before();
           __syncwarp();
@@ -448,21 +465,6 @@ __global__ void __launch_bounds__(kI8Threads) int8_linear_kernel(const __grid_co
             if (lane == 0) bulk_wait_read();                       // the store before has left this piece
             __syncwarp();
           }
-          // all of a granule's words before the first store: a store to shared memory keeps later loads behind it
-          float2 s[4], b[4], x[4][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[j] = *reinterpret_cast<const float2*>(columns + g * 32 + 8 * j + c);
-            b[j] = *reinterpret_cast<const float2*>(columns + C::kSpan + g * 32 + 8 * j + c);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
-              const float2 sum = make_float2(__int2float_rn(static_cast<int>(now[k])), __int2float_rn(static_cast<int>(now[k + 1])));
-              x[j][i] = ffma2(fmul2(sum, make_float2(row[i], row[i])), s[j], b[j]);
-            }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             // row r + 8 i: 128 bytes, its 16-byte chunks swizzled by r

@@ -31,9 +31,12 @@ __device__ __forceinline__ void store_s8(int8_t* q, const float (&f)[W], float i
   }
 }
 
+// Rows of a warp: short ones in CTAs of eight, which start half as often (100 000 x 256 bf16 27 -> 16 us, x 512 28.3 -> 27.4; x 1024 31 in CTAs
+// of four, 33 in those).
+__host__ __device__ constexpr int quantize_threads(int G, int E) { return G >= 128 ? G : E <= 16 ? 256 : 128; }
 template <int W, int G, int E>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) quantize_kernel(const __grid_constant__ QuantParams p) {
-  constexpr int kRows = G < 128 ? 128 / G : 1, N = E / W;
+__global__ void __launch_bounds__(quantize_threads(G, E)) quantize_kernel(const __grid_constant__ QuantParams p) {
+  constexpr int kRows = quantize_threads(G, E) / G, N = E / W;
   __shared__ float red[G > 32 ? 8 * (G / 32) : 1];
   griddep_wait();
   griddep_launch();
@@ -85,18 +88,23 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) quantize_kernel(const __gri
 
 template <int W, int G, int E>
 static int run_quantize(const QuantParams& p, cudaStream_t st) {
-  constexpr int kRows = G < 128 ? 128 / G : 1;
+  constexpr int kRows = quantize_threads(G, E) / G;
   const int64_t grid = (p.rows + kRows - 1) / kRows;
-  return launch(quantize_kernel<W, G, E>, static_cast<unsigned>(grid), G < 128 ? 128 : G, 0, st, p);
+  return launch(quantize_kernel<W, G, E>, static_cast<unsigned>(grid), quantize_threads(G, E), 0, st, p);
 }
 template <int W>
 static int pick_quantize(const QuantParams& p, cudaStream_t st) {
   const int C = p.channels;
-  // 32 values per thread, all asked for at once: 64 512 x 4096 bf16 128 us (6.2 TB/s); with 16 148, with 8 204, and CTAs that stay with rows
-  // staged ahead, as the norms have them, 183
+  // 32 values per thread, all asked for at once: 64 512 x 4096 bf16 117 us (6.8 TB/s); with 16 135, and CTAs that stay with rows staged
+  // ahead, as the norms have them, more.  A warp per row up to 2048 values, which needs no barrier (40 000 x 2048 41 us, 128 threads 44; x 1536
+  // 35 and 44); a few rows, where latency counts, the other way round.
+  const bool few = p.rows <= 2 * sm_count();
   if (C <= 256) return run_quantize<W, 32, 8>(p, st);
-  if (C <= 1024 && p.rows <= 2 * sm_count()) return run_quantize<W, 128, 8>(p, st);
+  if (C <= 1024 && few) return run_quantize<W, 128, 8>(p, st);
+  if (C <= 512) return run_quantize<W, 32, 16>(p, st);
   if (C <= 1024) return run_quantize<W, 32, 32>(p, st);
+  if (C <= 2048 && few) return run_quantize<W, 128, 16>(p, st);
+  if (C <= 2048) return run_quantize<W, 32, 64>(p, st);
   if (C <= 4096) return run_quantize<W, 128, 32>(p, st);
   if (C <= 16384) return run_quantize<W, 512, 32>(p, st);
   return run_quantize<W, 1024, 0>(p, st);

@@ -315,6 +315,17 @@ def test_quantize_tokens(shape, dtype):
     assert x.numel() == x.shape[-1] or q.stride(-2) % 16 == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 297, 501])
+@pytest.mark.parametrize("C", [256, 260, 509, 512, 1023, 1028, 1536, 2047, 2048, 2052])
+def test_quantize_tokens_of_few_and_many_rows(rows, C, dtype):
+    x = torch.randn(rows, C, device=DEV, generator=torch.Generator(device=DEV).manual_seed(C)).to(dtype)
+    x[rows // 2, C - 1] = 50.0
+    q, s = ops.quantize_tokens(x)
+    want, scale = quantised(x)
+    assert torch.equal(q, want) and torch.equal(s, scale)
+
+
 def test_quantize_tokens_rows_of_a_slice_zeros_and_values_that_are_not_finite():
     x = torch.randn(50, 640, device=DEV)
     for part in (x[:, 3:200], x[::2, :320], x.t(), x[:1, 1:100]):

@@ -123,16 +123,19 @@ __device__ __forceinline__ void store_int8(const float (&v)[E], const s3r_residu
   }
 }
 
+// threads of a CTA that has groups of G, each a row
+__host__ __device__ constexpr int cta_threads(int G) { return G < 96 ? 128 : G; }
 template <int W, int G, int E>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fwd_kernel(const __grid_constant__ NormParams p) {
-  constexpr int kRows = G < 128 ? 128 / G : 1, N = E / W;
-  __shared__ float red[G > 32 ? 8 * (G / 32) : 1];
+__global__ void __launch_bounds__(cta_threads(G)) norm_fwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr int kRows = cta_threads(G) / G, N = E / W;
+  __shared__ float red_all[kRows][G > 32 ? 8 * (G / 32) : 1];
   griddep_wait();
   griddep_launch();
   const s3r_residual_norm& a = p.a;
-  const int t = threadIdx.x % G, C = a.channels;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / G;
-  if (row >= p.rows) return;                              // whole rows leave (rows of several warps have a CTA each)
+  const int t = threadIdx.x % G, C = a.channels, group = threadIdx.x / G, bar = group + 1;
+  float* red = red_all[group];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + group;
+  if (row >= p.rows) return;                              // whole rows leave, each with a barrier of its own
   const int64_t at = row * C;
   uint32_t turn = 0;
   auto in = [&](int i) { return (i * G + t) * W < C; };
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fwd_kernel(const __gri
   if (a.y) {
     unpack_all<W, N>(v, yr, a.y_type, in);
     if (a.post) {
-      const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.post_eps, red, turn, t);
+      const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.post_eps, red, turn, t, bar);
       if (a.stats && t == 0) a.stats[2 * p.rows + row] = st.x, a.stats[3 * p.rows + row] = st.y;
       request_all<W, G, N>(wr, a.post_weight, a.param_type, 0, C, t);
       request_all<W, G, N>(br, a.post_bias, a.param_type, 0, C, t);
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fwd_kernel(const __gri
     if (a.r) store_all<W, N>(v, a.r, a.x_type, place);
   }
   if (!a.h && !a.q) return;
-  const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.eps, red, turn, t);
+  const float2 st = row_statistics<W, G, E>(v, a.kind, C, p.inv_n, a.eps, red, turn, t, bar);
   if (a.stats && t == 0) a.stats[row] = st.x, a.stats[p.rows + row] = st.y;
   request_all<W, G, N>(wr, a.weight, a.param_type, 0, C, t);
   request_all<W, G, N>(br, a.bias, a.param_type, 0, C, t);
@@ -190,18 +193,20 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_fwd_kernel(const __gri
     store_all<W, N>(v, a.h, a.h_type, place);
     return;
   }
-  store_int8<W, G, E>(v, a, row, red, turn, t, 0);
+  store_int8<W, G, E>(v, a, row, red, turn, t, bar);
 }
 
 // CTAs per SM.  An fp32 sum: 512 threads and 128 registers (64 512 x 1024 122 us; 768 threads of 80 registers 149, 512 such 156).  16 bits:
 // 768 threads, a row's bytes are fewer and its arithmetic the same (94 us, with 512 101).
-__host__ __device__ constexpr int rows_resident(int G, bool full, bool wide) { return G > 256 ? 1 : (full || wide || G < 128 ? 512 : 768) / (G < 128 ? 128 : G); }
+__host__ __device__ constexpr int rows_resident(int G, bool full, bool wide) {
+  return G > 256 ? 1 : G == 192 && (full || wide) ? 3 : (full || wide || G < 96 ? 512 : 768) / cta_threads(G);
+}
 // The same for many rows: CTAs stay, take every gridDim-th row, keep the parameters in registers and have the next rows on their way into
 // shared memory (cp.async, each thread its own bytes, so that no barrier orders them).  With a CTA per row a row cost 2 ns whatever its
 // bytes, the time it takes to start, wait for three loads one behind the other and end.
 template <int W, int G, int E, bool FULL, bool WIDE>
-__global__ void __launch_bounds__(G < 128 ? 128 : G, rows_resident(G, FULL, WIDE)) norm_rows_kernel(const __grid_constant__ NormParams p) {
-  constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, N = E / W, P = E / 2;
+__global__ void __launch_bounds__(cta_threads(G), rows_resident(G, FULL, WIDE)) norm_rows_kernel(const __grid_constant__ NormParams p) {
+  constexpr int kThreads = cta_threads(G), kRows = kThreads / G, N = E / W, P = E / 2;
   extern __shared__ __align__(16) char smem[];
   __shared__ float red_all[kRows][G > 32 ? 8 * (G / 32) : 1];
   griddep_wait();
@@ -376,8 +381,8 @@ struct NormBwdParams {
 
 // FULL: a post norm or a gate per channel too; without them their sums and factors take no registers
 template <int W, int G, int E, bool FULL>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
-  constexpr int kRows = G < 128 ? 128 / G : 1, N = E / W, P = E / 2, F = FULL ? P : 1;
+__global__ void __launch_bounds__(cta_threads(G)) norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
+  constexpr int kRows = cta_threads(G) / G, N = E / W, P = E / 2, F = FULL ? P : 1;
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[kRows][G > 32 ? 8 * (G / 32) : 1];
   griddep_wait();
@@ -710,7 +715,7 @@ static int gate_vector(const s3r_residual_norm& a) {
 
 template <int W, int G, int E, bool FULL, bool WIDE>
 static int run_rows(NormParams p, cudaStream_t st) {
-  constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kResident = rows_resident(G, FULL, WIDE);
+  constexpr int kThreads = cta_threads(G), kRows = kThreads / G, kResident = rows_resident(G, FULL, WIDE);
   const int stage = G * E * (type_bytes(p.a.x_type) + type_bytes(p.a.y_type)), room = kRowsSmem / kResident / kRows / stage;
   p.stages = room < 4 ? room : 4;
   const int64_t want = (p.rows + kRows - 1) / kRows, most = static_cast<int64_t>(sm_count()) * kResident;
@@ -724,7 +729,7 @@ static int run_rows(NormParams p, cudaStream_t st) {
 }
 template <int W, int G, int E>
 static int run_fwd(const NormParams& p, cudaStream_t st) {
-  constexpr int kRows = G < 128 ? 128 / G : 1, kThreads = G < 128 ? 128 : G;
+  constexpr int kRows = cta_threads(G) / G, kThreads = cta_threads(G);
   // where every CTA that fits has four rows and more
   if constexpr (W > 1 && E == 8)
     if (p.rows >= 4 * kRows * sm_count() * rows_resident(G, false, false)) {
@@ -737,9 +742,13 @@ template <int W>
 static int pick_fwd(const NormParams& p, cudaStream_t st) {
   const int C = p.a.channels;
   // Eight values per thread: with 32 (a warp per row, no exchange between warps) 64 512 x 1024 took 134 us instead of 130, 12 288 33
-  // instead of 29.5.
+  // instead of 29.5.  As few threads as have them: rows of 512 by 128 threads 90 us (58 593 of them, fp32), by 64 60; 768 by 128 67, by 96 63;
+  // 1536 by 256 74, by 192 63.  (The backward gains from 96 and 192 with bf16, 89 -> 82, and loses with fp32, 105 -> 115.)
   if (C <= 256) return run_fwd<W, 32, 8>(p, st);
+  if (C <= 512) return run_fwd<W, 64, 8>(p, st);
+  if (C <= 768) return run_fwd<W, 96, 8>(p, st);
   if (C <= 1024) return run_fwd<W, 128, 8>(p, st);
+  if (C <= 1536) return run_fwd<W, 192, 8>(p, st);
   if (C <= 2048) return run_fwd<W, 256, 8>(p, st);
   if (C <= 4096) return run_fwd<W, 512, 8>(p, st);
   return run_fwd<W, 512, 16>(p, st);
@@ -751,7 +760,7 @@ static void bwd_shape(int channels, int* G, int* E) {
 }
 // slices per batch entry (of `entries`): CTAs that are resident together, each with four rows per group at least
 static int bwd_slices(int64_t entries, int64_t span, int G) {
-  const int threads = G < 128 ? 128 : G, groups = threads / G;
+  const int threads = cta_threads(G), groups = threads / G;
   const int64_t resident = static_cast<int64_t>(sm_count()) * (512 / threads > 0 ? 512 / threads : 1);
   const int64_t want = (resident + entries - 1) / entries, most = (span + 4 * groups - 1) / (4 * groups);
   const int64_t n = want < most ? want : most;
@@ -760,7 +769,7 @@ static int bwd_slices(int64_t entries, int64_t span, int G) {
 
 template <int W, int G, int E, bool FULL>
 static int run_bwd(const NormBwdParams& p, unsigned ctas, cudaStream_t st) {
-  constexpr int kThreads = G < 128 ? 128 : G, kGroups = kThreads / G;
+  constexpr int kThreads = cta_threads(G), kGroups = kThreads / G;
   static_assert(kGroups * E * G * 4 <= kRowsSmem, "sums of the groups");
   static std::atomic<uint64_t> ready{0};
   if (attributes_missing(ready)) {
@@ -856,7 +865,7 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   p.at_dr = p.at_y + row * type_bytes(f.y_type);
   p.at_dh = p.at_dr + row * type_bytes(f.x_type);
   p.stage_bytes = p.at_dh + row * type_bytes(f.h_type);
-  const int threads = G < 128 ? 128 : G, resident = 512 / threads;
+  const int threads = cta_threads(G), resident = 512 / threads;
   const uint32_t room = kRowsSmem / resident / (threads / G);
   p.stages = static_cast<int>(room / p.stage_bytes < 4 ? room / p.stage_bytes : 4);
   S3R_REQUIRE(p.stages >= 1, S3R_ERR_TOO_LARGE, "s3r_residual_norm_bwd: rows do not fit shared memory");

@@ -188,6 +188,19 @@ def test_norm_dimensions(shape, gate):
     Norm(shape, gate=gate, post=True, seed=5).train()
 
 
+@pytest.mark.parametrize("C", [260, 500, 511, 512, 516, 700, 767, 768, 772, 1100, 1540])
+@pytest.mark.parametrize("rows, x, post", [(3, torch.float32, False), (5003, torch.float32, True), (5003, torch.bfloat16, False)])
+def test_norm_rows_of_three_six_and_two_warps(C, rows, x, post):
+    n = Norm((1, rows, C), x=x, y=torch.bfloat16, post=post, seed=C, gate=(1, rows, 1))
+    n.train()
+    n.h_type = torch.float32
+    with torch.no_grad():
+        r, h = n.call()
+        r8, q, s = ops.residual_norm_int8(n.x, n.y, n.norm, n.scale, n.gate, n.post, n.kind)
+        q2, s2 = ops.quantize_tokens(h)
+    assert torch.equal(r8, r) and torch.equal(q, q2) and torch.equal(s, s2)
+
+
 def test_norm_training_size():
     Norm((2, 6144, 1024), gate=(2, 1, 1), seed=1).train()
 

@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict_
 // product on tcgen05: persistent CTAs, K in steps of 128 bytes through a ring of TMA copies, the sums of two tiles in tensor memory
 // so that one is written out while the next is summed.  One warp copies, one issues the products, eight take the sums (32 rows and
 // half of the columns each), scale them and store through shared memory.
-// At K = 1024 what bounds it is shared memory, written by the copies, read by the products and passed through by the results: 64 512 x 4096
-// take 155 us without the results' part, 166 without the stores at its end, 201 with them.  Tried and not kept: sixteen warps for the sums
+// At K = 1024 no unit is full (tensor pipe 0.72 busy, shared memory 0.55, L2 0.4, at 1.64 GHz under power), but the results' way out delays the
+// copies in: 64 512 x 4096 take 155 us without the results' part, 166 without the stores at its end, 201 with them.  Tried and not kept: sixteen warps for the sums
 // (220), stores from registers by way of shared memory (211) and, with a's rows of up to 1024 bytes staying where they are, half as
 // many bytes to copy but three steps of the ring in place of five (234; 156 without the stores).
 // CTAS = 2: a pair of CTAs multiplies 256 rows with TN columns; each holds 128 rows of a and half of b's rows, the products read both

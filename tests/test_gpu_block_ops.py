@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from speed3r_b200 import ops
+from speed3r_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -389,6 +389,23 @@ def test_int8_linear_few_tokens(M, N, K):
 @pytest.mark.parametrize("bias", [True, False])
 def test_int8_linear_types(M, N, K, dtype, bias):
     check_linear(M, N, K, dtype, bias)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 5, 7, 9, 63, 65, 67, 129, 250, 261, 517])
+@pytest.mark.parametrize("start", [0, 1, 2, 3, 5])
+def test_int8_linear_results_that_begin_anywhere(N, start, dtype):
+    """Through the library's C entry, into the middle of a buffer: what is around the result stays."""
+    M, K = 301, 144
+    q, w = int8(M, K), int8(N, K)
+    s, ws = torch.rand(M, device=DEV) + 0.5, torch.rand(N, device=DEV) + 0.5
+    whole = torch.full((start + M * N + 40,), 7.0, device=DEV, dtype=dtype)
+    code = {torch.float32: 0, torch.bfloat16: 1}[dtype]
+    rc = _lib.load().s3r_int8_linear(q.data_ptr(), K, s.data_ptr(), w.data_ptr(), K, ws.data_ptr(), None, whole.data_ptr() + start * whole.element_size(), code, M, N, K,
+                               torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert torch.equal(whole[start:start + M * N].view(M, N), ops.int8_linear(q, s, w, ws, None, dtype))
+    assert (whole[:start] == 7).all() and (whole[start + M * N:] == 7).all()
 
 
 def test_int8_linear_largest_sums_are_exact():

@@ -379,9 +379,14 @@ struct NormBwdParams {
   float* partial;              // [batch entries x slices, kSums, channels], the sums that are wanted
 };
 
+// CTAs per SM: 128 registers per thread, in a FULL backward 168.  The grid has as many as are resident: with a second, shorter round of CTAs
+// 12 288 x 1024, fp32, post norm took 75 us instead of 58, and the sums over CTAs had a third more to read.
+__host__ __device__ constexpr int bwd_resident(int G, bool full) {
+  return G > 256 ? 1 : (full ? 384 : 512) / cta_threads(G);
+}
 // FULL: a post norm or a gate per channel too; without them their sums and factors take no registers
 template <int W, int G, int E, bool FULL>
-__global__ void __launch_bounds__(cta_threads(G)) norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
+__global__ void __launch_bounds__(cta_threads(G), bwd_resident(G, FULL)) norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
   constexpr int kRows = cta_threads(G) / G, N = E / W, P = E / 2, F = FULL ? P : 1;
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[kRows][G > 32 ? 8 * (G / 32) : 1];
@@ -743,7 +748,7 @@ static int pick_fwd(const NormParams& p, cudaStream_t st) {
   const int C = p.a.channels;
   // Eight values per thread: with 32 (a warp per row, no exchange between warps) 64 512 x 1024 took 134 us instead of 130, 12 288 33
   // instead of 29.5.  As few threads as have them: rows of 512 by 128 threads 90 us (58 593 of them, fp32), by 64 60; 768 by 128 67, by 96 63;
-  // 1536 by 256 74, by 192 63.  (The backward gains from 96 and 192 with bf16, 89 -> 82, and loses with fp32, 105 -> 115.)
+  // 1536 by 256 74, by 192 63.
   if (C <= 256) return run_fwd<W, 32, 8>(p, st);
   if (C <= 512) return run_fwd<W, 64, 8>(p, st);
   if (C <= 768) return run_fwd<W, 96, 8>(p, st);
@@ -754,14 +759,16 @@ static int pick_fwd(const NormParams& p, cudaStream_t st) {
   return run_fwd<W, 512, 16>(p, st);
 }
 
-static void bwd_shape(int channels, int* G, int* E) {
-  *G = channels <= 256 ? 32 : channels <= 512 ? 64 : channels <= 1024 ? 128 : channels <= 2048 ? 256 : 512;
+// As few warps as have a row, but for fp32 rows of whole warps, where three and six warps leave too few threads on an SM: 768 channels fp32 by
+// 128 threads 101 us (39 062 rows), by 96 115, bf16 85 and 79; 1536 fp32 by 256 103, by 192 109, bf16 90 and 82; 700 fp32 124 and 110.
+static void bwd_shape(int channels, bool whole, int* G, int* E) {
+  *G = channels <= 256 ? 32 : channels <= 512 ? 64 : channels <= 768 && !whole ? 96 : channels <= 1024 ? 128 : channels <= 1536 && !whole ? 192 : channels <= 2048 ? 256 : 512;
   *E = channels <= 4096 ? 8 : 16;
 }
 // slices per batch entry (of `entries`): CTAs that are resident together, each with four rows per group at least
-static int bwd_slices(int64_t entries, int64_t span, int G) {
+static int bwd_slices(int64_t entries, int64_t span, int G, bool full) {
   const int threads = cta_threads(G), groups = threads / G;
-  const int64_t resident = static_cast<int64_t>(sm_count()) * (512 / threads > 0 ? 512 / threads : 1);
+  const int64_t resident = static_cast<int64_t>(sm_count()) * bwd_resident(G, full);
   const int64_t want = (resident + entries - 1) / entries, most = (span + 4 * groups - 1) / (4 * groups);
   const int64_t n = want < most ? want : most;
   return static_cast<int>(n < 1 ? 1 : n);
@@ -787,7 +794,9 @@ template <int W, bool FULL>
 static int pick_bwd(const NormBwdParams& p, int G, int E, unsigned ctas, cudaStream_t st) {
   if (G == 32) return run_bwd<W, 32, 8, FULL>(p, ctas, st);
   if (G == 64) return run_bwd<W, 64, 8, FULL>(p, ctas, st);
+  if (G == 96) return run_bwd<W, 96, 8, FULL>(p, ctas, st);
   if (G == 128) return run_bwd<W, 128, 8, FULL>(p, ctas, st);
+  if (G == 192) return run_bwd<W, 192, 8, FULL>(p, ctas, st);
   if (G == 256) return run_bwd<W, 256, 8, FULL>(p, ctas, st);
   if (E == 8) return run_bwd<W, 512, 8, FULL>(p, ctas, st);
   return run_bwd<W, 512, 16, FULL>(p, ctas, st);
@@ -817,10 +826,14 @@ extern "C" int s3r_residual_norm_fwd(const s3r_residual_norm* args, void* stream
 
 extern "C" size_t s3r_residual_norm_bwd_workspace_bytes(int64_t batch, int64_t tokens, int channels, int gate_mode) {
   if (batch <= 0 || tokens <= 0 || channels <= 0 || channels > kNormMaxChannels || batch > (1ll << 31) / tokens) return 0;
-  int G, E;
-  bwd_shape(channels, &G, &E);
   const int64_t entries = gate_mode == S3R_GATE_CHANNEL ? batch : 1, span = gate_mode == S3R_GATE_CHANNEL ? tokens : batch * tokens;
-  return static_cast<size_t>(entries) * bwd_slices(entries, span, G) * kSums * channels * sizeof(float);
+  int slices = 0;                                        // whatever x's type, with and without a post norm
+  for (const bool whole : {false, true}) {
+    int G, E;
+    bwd_shape(channels, whole, &G, &E);
+    slices = std::max(slices, bwd_slices(entries, span, G, false));          // not fewer than those of a full one
+  }
+  return static_cast<size_t>(entries) * slices * kSums * channels * sizeof(float);
 }
 
 extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_residual_norm_grad* g_, void* stream) {
@@ -852,8 +865,9 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   const int64_t entries = per_entry ? f.batch : 1;
   p.span = per_entry ? f.tokens : p.rows;
   int G, E;
-  bwd_shape(f.channels, &G, &E);
-  p.slices = bwd_slices(entries, p.span, G);
+  bwd_shape(f.channels, f.x_type == S3R_F32 && f.channels % 256 == 0, &G, &E);
+  const bool full = f.post || per_entry;
+  p.slices = bwd_slices(entries, p.span, G, full);
   const bool sums = g.d_weight || g.d_bias || g.d_scale || g.d_post_weight || g.d_post_bias || g.d_gate_channel;
   const size_t need = s3r_residual_norm_bwd_workspace_bytes(f.batch, f.tokens, f.channels, f.gate_mode);
   S3R_REQUIRE(!sums || (g.workspace && g.workspace_bytes >= need && reinterpret_cast<uintptr_t>(g.workspace) % 4 == 0), S3R_ERR_TOO_LARGE,
@@ -865,14 +879,13 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   p.at_dr = p.at_y + row * type_bytes(f.y_type);
   p.at_dh = p.at_dr + row * type_bytes(f.x_type);
   p.stage_bytes = p.at_dh + row * type_bytes(f.h_type);
-  const int threads = cta_threads(G), resident = 512 / threads;
+  const int threads = cta_threads(G), resident = bwd_resident(G, full);
   const uint32_t room = kRowsSmem / resident / (threads / G);
   p.stages = static_cast<int>(room / p.stage_bytes < 4 ? room / p.stage_bytes : 4);
   S3R_REQUIRE(p.stages >= 1, S3R_ERR_TOO_LARGE, "s3r_residual_norm_bwd: rows do not fit shared memory");
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const unsigned ctas = static_cast<unsigned>(entries * p.slices);
-  const bool full = f.post || per_entry;
   int rc;
   if (w == 8) rc = full ? pick_bwd<8, true>(p, G, E, ctas, st) : pick_bwd<8, false>(p, G, E, ctas, st);
   else if (w == 4) rc = full ? pick_bwd<4, true>(p, G, E, ctas, st) : pick_bwd<4, false>(p, G, E, ctas, st);

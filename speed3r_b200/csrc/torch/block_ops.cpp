@@ -467,13 +467,15 @@ void need_states(const Tensor& p, const Tensor& m, const Tensor& v, const option
                     (e->numel() == 0 || e->stride(1) == 1), "adamw: scales of ", p.numel(), " elements must be uint8 [2, ", (p.numel() + 255) / 256, "], got ", e->sizes());
 }
 
+// scales: those of the 8-bit states, one behind the other.  A list with gaps (Tensor?[]) cannot be declared as written: tracers
+// take none of its gaps, and a list that is not declared is read again from before the step.
 void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
-                const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
+                at::TensorList scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
                 double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
   const size_t n = params.size();
   TORCH_CHECK(n > 0, "adamw: no tensors");
-  TORCH_CHECK(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && (scales.empty() || scales.size() == n),
-              "adamw: ", n, " parameters, ", grads.size(), " gradients, ", exp_avg.size(), " and ", exp_avg_sq.size(), " states, ", scales.size(), " scales");
+  TORCH_CHECK(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n, "adamw: ", n, " parameters, ", grads.size(), " gradients, ",
+              exp_avg.size(), " and ", exp_avg_sq.size(), " states");
   const at::Device device = params[0].device();
   TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw: betas are in [0, 1)");
   TORCH_CHECK(eps >= 0 && weight_decay >= 0, "adamw: eps and weight_decay are not negative");
@@ -488,12 +490,17 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
   std::vector<uint8_t*> me(n, nullptr), ve(n, nullptr);
   std::vector<int64_t> counts(n);
   std::vector<int> p_types(n), g_types(n);
+  size_t scale_of = 0;
   for (size_t i = 0; i < n; ++i) {
     need_cuda(params[i], "a parameter");
     TORCH_CHECK(params[i].device() == device && grads[i].device() == device, "adamw: tensors of one device");
     TORCH_CHECK(params[i].is_contiguous(), "adamw: parameters must be contiguous");
     TORCH_CHECK(grads[i].sizes() == params[i].sizes(), "adamw: gradient ", grads[i].sizes(), " of parameter ", params[i].sizes());
-    optional<Tensor> scale = scales.empty() ? optional<Tensor>() : optional<Tensor>(scales.get(i));
+    optional<Tensor> scale;
+    if (exp_avg[i].scalar_type() == at::kByte) {
+      TORCH_CHECK(scale_of < scales.size(), "adamw: an 8-bit state has no scales");
+      scale = scales[scale_of++];
+    }
     need_states(params[i], exp_avg[i], exp_avg_sq[i], scale);
     if (scale.has_value()) {
       me[i] = static_cast<uint8_t*>(scale->data_ptr());
@@ -508,6 +515,7 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
     p_types[i] = type_of(params[i], "a parameter");
     g_types[i] = type_of(grads[i], "a gradient");
   }
+  TORCH_CHECK(scale_of == scales.size(), "adamw: scales for a state that is not in 8 bits");
   // a parameter that is listed twice would be updated by two warps at once
   for (const auto* list : {&p, &m, &v}) {
     std::vector<void*> sorted;
@@ -593,15 +601,26 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
                 const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
                 double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
   TORCH_CHECK(!params.empty(), "adamw: no tensors");
+  std::vector<Tensor> held;
+  if (!scales.empty()) {
+    TORCH_CHECK(scales.size() == params.size() && exp_avg.size() == params.size(), "adamw: ", params.size(), " parameters, ", exp_avg.size(), " states, ",
+                scales.size(), " scales");
+    for (size_t i = 0; i < exp_avg.size(); ++i) {
+      const optional<Tensor> scale = scales.get(i);
+      TORCH_CHECK(scale.has_value() == (exp_avg[i].scalar_type() == at::kByte), "adamw: scales belong to a state of uint8 codes and only to one, got ",
+                  scale.has_value() ? "scales" : "none", " for a state of ", exp_avg[i].scalar_type());
+      if (scale.has_value()) held.push_back(*scale);
+    }
+  }
   if (plain(params[0])) {
-    adamw_update(params, grads, exp_avg, exp_avg_sq, step, scales, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+    adamw_update(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
     // what autograd has saved of these tensors is not what they hold any more
     for (const auto list : {params, exp_avg, exp_avg_sq})
       for (const Tensor& t : list)
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     return;
   }
-  S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, scales, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+  S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
 }
 void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
   if (exp_avg.empty() || plain(exp_avg[0])) return adamw_values(exp_avg, exp_avg_sq, scales, m_out, v_out);
@@ -624,13 +643,13 @@ TORCH_LIBRARY_FRAGMENT(speed3r_b200, m) {
   m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
   m.def("int8_product(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor");
   m.def("norm_of(Tensor[] tensors) -> Tensor");
-  m.def("adamw_update(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor?[] scales, float lr, "
+  m.def("adamw_update(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor(e!)[] scales, float lr, "
         "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()");
   m.def("adamw_values(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()");
   m.def("quantize_tokens(Tensor x) -> (Tensor, Tensor)", &quantize_tokens);
   m.def("int8_linear(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor", &int8_linear);
   m.def("grad_norm(Tensor[] tensors) -> Tensor", &grad_norm);
-  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor?[] scales, float lr, "
+  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor(e!)?[] scales, float lr, "
         "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()", &adamw_step);
   m.def("adamw_state(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()", &adamw_state);
 }

@@ -1,0 +1,67 @@
+"""What the operators around the attention promise to tracers, to autograd and to whoever calls them, as far as no GPU is needed."""
+import pytest
+import torch
+
+from speed3r_b200 import ops
+
+U8 = torch.uint8
+
+
+def raises(text, call):
+    with pytest.raises(RuntimeError, match=text):
+        call()
+
+
+# ---- tracing ---------------------------------------------------------------------------------------------------------------
+def traced(f, *args):
+    """The graph that ahead-of-time autograd makes of f(*args).  Tracing reads shapes only; what is traced is not run."""
+    from torch._functorch.aot_autograd import aot_module_simplified
+
+    class Seen(Exception):
+        pass
+
+    graphs = []
+
+    def keep(graph, inputs):
+        graphs.append(graph.graph)
+        raise Seen
+
+    ops._ops()
+    torch._dynamo.reset()
+    with pytest.raises(Exception):                       # Seen, as the compiler passes it on
+        torch.compile(f, backend=lambda gm, ins: aot_module_simplified(gm, ins, fw_compiler=keep), fullgraph=True)(*args)
+    return graphs[0]
+
+
+def behind(node, earlier):
+    """Whether `node` depends on `earlier`."""
+    seen, todo = set(), [node]
+    while todo:
+        n = todo.pop()
+        if n is earlier:
+            return True
+        if n not in seen:
+            seen.add(n)
+            todo += n.all_input_nodes
+    return False
+
+
+def test_step_is_traced_as_writing_everything_that_it_writes():
+    n = 300
+    m, v = (torch.zeros(n, dtype=U8) for _ in range(2))
+    scales, step = torch.zeros(2, 2, dtype=U8), torch.zeros((), dtype=torch.int64)
+    names = ("p", "m", "v", "scales", "step", "p of 32-bit states", "m of 32 bits", "v of 32 bits")
+
+    def f(g, p, m, v, scales, step, q, m32, v32):
+        written = (p, m, v, scales, step, q, m32, v32)
+        before = [t + 1 for t in written]
+        ops.adamw_step([p, q], [g, g], [m, m32], [v, v32], step, scales=[scales, None])
+        return [t * 2 for t in before] + [t + 1 for t in written]
+
+    graph = traced(f, torch.ones(n), torch.zeros(n), m, v, scales, step, *(torch.zeros(n) for _ in range(3)))
+    the_step = [node for node in graph.nodes if node.op == "call_function" and "auto_functionalized" in str(node.target)]
+    assert len(the_step) == 1
+    out = next(node for node in graph.nodes if node.op == "output").args[0][-2 * len(names):]
+    for name, before, after in zip(names, out, out[len(names):]):
+        assert not behind(before, the_step[0]), name
+        assert behind(after, the_step[0]), name

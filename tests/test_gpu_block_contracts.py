@@ -1,0 +1,69 @@
+"""What the operators around the attention promise beyond their formulas: tracing, random numbers, extreme arguments, kernels chosen by size."""
+import math
+
+import pytest
+import torch
+
+from speed3r_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U8 = torch.uint8
+
+
+def compiled(f):
+    ops._ops()
+    torch._dynamo.reset()
+    return torch.compile(f, backend="aot_eager", fullgraph=True)
+
+
+def state(shapes, eight, seed=0, dtype=torch.float32):
+    """Parameters, gradients, first and second moments, scales (None: 32 bits) and the step's number."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    rand = lambda s: torch.randn(s, device=DEV, generator=g)
+    params, grads = ([rand(s).to(dtype) for s in shapes] for _ in range(2))
+    first, second, scales = [], [], []
+    for s, e in zip(shapes, eight):
+        codes = lambda: torch.randint(0, 120, s, device=DEV, dtype=U8, generator=g)
+        first.append(codes() if e else 0.1 * rand(s))
+        second.append(codes() if e else rand(s) ** 2)
+        scales.append(torch.randint(115, 125, (2, -(-math.prod(s) // 256)), device=DEV, dtype=U8, generator=g) if e else None)
+    return params, grads, first, second, scales, torch.tensor(3, device=DEV)
+
+
+# ---- tracing ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("eight", [(True, False, True), (False, False, False)])
+def test_compiled_step_is_the_step(eight):
+    shapes = [(300,), (17, 5), (1041,)]
+    some = lambda: state(shapes, eight, seed=1)
+
+    def f(params, grads, first, second, scales, step):
+        # values of before and of after, which a tracer must not take for the same
+        held = [t for t in first + second + scales if t is not None]
+        before = [t + 1 for t in held]
+        norm = ops.grad_norm(grads)
+        ops.adamw_step(params, grads, first, second, step, lr=1e-2, grad_norm=norm, max_norm=1.0, scales=scales if any(eight) else None, seed=5)
+        return before, [t + 1 for t in held], norm
+
+    a, b = some(), some()
+    want, got = f(*a), compiled(f)(*b)
+    flat = lambda x: [t for y in x for t in (flat(y) if isinstance(y, (list, tuple)) else [y]) if t is not None]
+    assert len(flat(want)) == len(flat(got)) and all(torch.equal(x, y) for x, y in zip(flat(want) + flat(a), flat(got) + flat(b)))
+
+
+def test_operators_have_the_schemas_and_shapes_that_they_say():
+    x, y, w = torch.randn(2, 3, 40, device=DEV), torch.randn(2, 3, 40, device=DEV).bfloat16(), torch.ones(40, device=DEV)
+    check = lambda op, args: torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+    ns = ops._ops()
+    args = (x, y, w, w, w, None, None, None)
+    r, h, stats = ns.residual_norm_fwd(*args, True, False, 0, 1e-5, 0.0, torch.bfloat16, True)
+    check(ns.residual_norm_fwd.default, (*args, True, False, 0, 1e-5, 0.0, torch.bfloat16, True))
+    check(ns.residual_norm_int8.default, (*args, False, 0, 1e-5, 0.0))
+    check(ns.residual_norm_bwd.default, (r, y, w, w, None, None, None, stats, x, h, torch.bfloat16, False, 0, 31, torch.float32))
+    check(ns.quantize_rows.default, (x,))
+    q, s = ops.quantize_tokens(x)
+    check(ns.int8_product.default, (q, s, q.reshape(6, 40), s.reshape(6), None, torch.float16))
+    check(ns.norm_of.default, ([x, y],))
+    p, g, m, v, e, step = state([(300,), (7,)], (True, False))
+    check(ns.adamw_update.default, (p, g, m, v, step, [e[0]], 1e-3, None, 0.9, 0.99, 1e-8, 0.1, None, 0.0, 3))
+    check(ns.adamw_values.default, (m[:1], v[:1], e[:1], [torch.zeros(300, device=DEV)], [torch.zeros(300, device=DEV)]))

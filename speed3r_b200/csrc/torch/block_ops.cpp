@@ -589,11 +589,13 @@ std::tuple<Tensor, Tensor> quantize_tokens(const Tensor& x) {
 }
 Tensor int8_linear(const Tensor& q, const Tensor& q_scale, const Tensor& weight, const Tensor& weight_scale, const optional<Tensor>& bias,
                    at::ScalarType out_type) {
+  no_tangents(q_scale, weight_scale, bias);
   if (plain(q)) return int8_product(q, q_scale, weight, weight_scale, bias, out_type);
   S3R_DISPATCHED(int8_product)(q, q_scale, weight, weight_scale, bias, out_type);
 }
 Tensor grad_norm(at::TensorList tensors) {
   TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
+  no_tangents(tensors);
   if (plain(tensors[0])) return norm_of(tensors);
   S3R_DISPATCHED(norm_of)(tensors);
 }
@@ -601,6 +603,7 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
                 const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
                 double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
   TORCH_CHECK(!params.empty(), "adamw: no tensors");
+  no_tangents(params, grads, exp_avg, exp_avg_sq, lr_tensor, norm);
   std::vector<Tensor> held;
   if (!scales.empty()) {
     TORCH_CHECK(scales.size() == params.size() && exp_avg.size() == params.size(), "adamw: ", params.size(), " parameters, ", exp_avg.size(), " states, ",
@@ -623,6 +626,7 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
 }
 void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
+  no_tangents(m_out, v_out);
   if (exp_avg.empty() || plain(exp_avg[0])) return adamw_values(exp_avg, exp_avg_sq, scales, m_out, v_out);
   S3R_DISPATCHED(adamw_values)(exp_avg, exp_avg_sq, scales, m_out, v_out);
 }

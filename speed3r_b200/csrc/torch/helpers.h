@@ -68,6 +68,11 @@ Tensor none(const Tensor& like) { return at::empty({0}, like.options()); }
 // operators would drop a tangent without a word.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const optional<Tensor>& t) { return t.has_value() && has_tangent(*t); }
+bool has_tangent(at::TensorList list) {
+  for (const Tensor& t : list)
+    if (has_tangent(t)) return true;
+  return false;
+}
 template <typename... T>
 void no_tangents(const T&... t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "speed3r_b200: forward mode AD is not implemented for the operators of this package");

@@ -65,3 +65,27 @@ def test_step_is_traced_as_writing_everything_that_it_writes():
     for name, before, after in zip(names, out, out[len(names):]):
         assert not behind(before, the_step[0]), name
         assert behind(after, the_step[0]), name
+
+
+# ---- forward mode ----------------------------------------------------------------------------------------------------------
+def test_tangents_are_refused_and_not_dropped():
+    """In every operator and every floating argument, before anything is computed."""
+    import torch.autograd.forward_ad as fwd
+
+    x, q, s = torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    codes, scales = torch.zeros(32, dtype=U8), torch.zeros(2, 1, dtype=U8)
+    step = torch.zeros((), dtype=torch.int64)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t.clone(), torch.ones_like(t))
+        d, one = dual(x), dual(torch.ones(()))
+        calls = [lambda: ops.residual_norm(d, None, (None, None, 1e-5)), lambda: ops.residual_norm(x, d), lambda: ops.residual_norm(x, x, scale=dual(torch.ones(8))),
+                 lambda: ops.residual_norm_int8(d, None, (None, None, 1e-5)), lambda: ops.quantize_tokens(d),
+                 lambda: ops.int8_linear(q, dual(s), q, s), lambda: ops.int8_linear(q, s, q, dual(s)), lambda: ops.int8_linear(q, s, q, s, dual(s)),
+                 lambda: ops.grad_norm([x, d]),
+                 lambda: ops.adamw_step([x], [x], [x], [x], step, lr=one), lambda: ops.adamw_step([x], [x], [x], [x], step, grad_norm=one)]
+        calls += [lambda i=i: ops.adamw_step(*[[x, d if k == i else x] for k in range(4)], step) for i in range(4)]
+        calls += [lambda i=i: ops.adamw_state([codes], [codes], [scales], out=[[dual(torch.zeros(32)) if k == i else torch.zeros(32)] for k in range(2)]) for i in range(2)]
+        for i, call in enumerate(calls):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call()
+                pytest.fail(f"call {i} went through")

@@ -578,6 +578,12 @@ void adamw_values(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorL
   check(s3r_adamw_state(static_cast<int>(n), m.data(), v.data(), me.data(), ve.data(), mo.data(), vo.data(), counts.data(), stream()), "s3r_adamw_state");
 }
 
+// What autograd has saved of these tensors is not what they hold any more (the dispatcher's own path counts by the schema).
+void written(at::TensorList list) {
+  for (const Tensor& t : list)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------------------------------------------------
 // The operators that have no gradient, as they are called: on ordinary tensors straight into the base operator.  Through the dispatcher
 // each of them passed PyTorch's boxed autograd fallback, which looks at every tensor of every list.
@@ -617,17 +623,18 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   }
   if (plain(params[0])) {
     adamw_update(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
-    // what autograd has saved of these tensors is not what they hold any more
-    for (const auto list : {params, exp_avg, exp_avg_sq})
-      for (const Tensor& t : list)
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    for (const auto list : {params, exp_avg, exp_avg_sq, at::TensorList(held), at::TensorList(step)}) written(list);
     return;
   }
   S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
 }
 void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
   no_tangents(m_out, v_out);
-  if (exp_avg.empty() || plain(exp_avg[0])) return adamw_values(exp_avg, exp_avg_sq, scales, m_out, v_out);
+  if (exp_avg.empty() || plain(exp_avg[0])) {
+    adamw_values(exp_avg, exp_avg_sq, scales, m_out, v_out);
+    written(m_out);
+    return written(v_out);
+  }
   S3R_DISPATCHED(adamw_values)(exp_avg, exp_avg_sq, scales, m_out, v_out);
 }
 

@@ -67,3 +67,27 @@ def test_operators_have_the_schemas_and_shapes_that_they_say():
     p, g, m, v, e, step = state([(300,), (7,)], (True, False))
     check(ns.adamw_update.default, (p, g, m, v, step, [e[0]], 1e-3, None, 0.9, 0.99, 1e-8, 0.1, None, 0.0, 3))
     check(ns.adamw_values.default, (m[:1], v[:1], e[:1], [torch.zeros(300, device=DEV)], [torch.zeros(300, device=DEV)]))
+
+
+def test_what_is_written_counts_as_changed():
+    """Autograd notices that a tensor which it has saved was written: every tensor that a call changes, and no other."""
+    p, g, m, v, e, step = state([(300,), (1041,)], (True, False))
+    norm = ops.grad_norm(g)
+    changed, read = p + m + v + e[:1] + [step], g + [norm]
+    versions = lambda ts: [t._version for t in ts]
+    before, kept = versions(changed), versions(read)
+    ops.adamw_step(p, g, m, v, step, grad_norm=norm, scales=e)
+    assert all(b > a for a, b in zip(before, versions(changed))) and versions(read) == kept
+    out = [torch.zeros(300, device=DEV)], [torch.zeros(300, device=DEV)]
+    read = m + v + e[:1]
+    before, kept = versions(out[0] + out[1]), versions(read)
+    ops.adamw_state(m[:1], v[:1], e[:1], out=out)
+    assert all(b > a for a, b in zip(before, versions(out[0] + out[1]))) and versions(read) == kept
+    w = torch.ones((), device=DEV, requires_grad=True)
+    y = (w * out[0][0]).sum()
+    ops.adamw_state(m[:1], v[:1], e[:1], out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        frozen = state([(300,)], (True,))
+        ops.adamw_step(*frozen[:4], frozen[5], scales=frozen[4])

@@ -101,19 +101,19 @@ class BlockRope(nn.Module):
         return torch.empty((x.shape[0],) + (1,) * (x.dim() - 1), dtype=torch.float32, device=x.device).bernoulli_(keep).div_(keep)
 
     def _scale(self, m: nn.Module) -> Optional[Tensor]:
-        return m.gamma if hasattr(m, "gamma") else None
+        return m.gamma if type(m) is LayerScale else None
 
     def _fuses(self) -> bool:
         """Norms and LayerScales are what they look like and nobody watches them."""
         return (_norm_args(self.norm1, self.dim) is not None and _norm_args(self.norm2, self.dim) is not None and not _global_hooks() and
-                all(type(m) is nn.Identity or (hasattr(m, "gamma") and tuple(m.gamma.shape) == (self.dim,)) for m in (self.ls1, self.ls2)) and
+                all(type(m) is nn.Identity or (type(m) is LayerScale and tuple(m.gamma.shape) == (self.dim,)) for m in (self.ls1, self.ls2)) and
                 not any(_watched(m) for m in (self.ls1, self.ls2)))
 
     def _residual(self, x: Tensor) -> Tensor:
         """x in the type that the sum with a scaled branch has."""
         kept = x.dtype
         for m in (self.ls1, self.ls2):
-            if hasattr(m, "gamma"):
+            if type(m) is LayerScale:
                 kept = torch.promote_types(kept, m.gamma.dtype)
         return x.to(kept)
 

@@ -89,3 +89,36 @@ def test_tangents_are_refused_and_not_dropped():
             with pytest.raises(NotImplementedError, match="forward mode"):
                 call()
                 pytest.fail(f"call {i} went through")
+
+
+# ---- the block -------------------------------------------------------------------------------------------------------------
+def test_a_scale_of_another_formula_is_called():
+    """What has a parameter named gamma need not multiply with it."""
+    from speed3r_b200 import BlockRope
+    from speed3r_b200.block import LayerScale
+
+    class Exponential(LayerScale):
+        def forward(self, x):
+            return x * self.gamma.exp()
+
+    class Named(torch.nn.Identity):
+        gamma = torch.full((64,), 3.0)
+
+    class Own(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gamma = torch.nn.Parameter(torch.ones(64))
+
+        def forward(self, x):
+            return x + self.gamma
+
+    b = BlockRope(64, 1, init_values=0.1)
+    assert b._fuses()
+    for name in ("ls1", "ls2"):
+        for other in (Exponential(64), Named(), Own()):
+            b = BlockRope(64, 1, init_values=0.1)
+            setattr(b, name, other)
+            assert not b._fuses(), other
+    b = BlockRope(64, 1)
+    b.ls1.gamma = torch.full((64,), 3.0)                # an Identity stays one
+    assert b._fuses() and b._scale(b.ls1) is None

@@ -91,3 +91,30 @@ def test_what_is_written_counts_as_changed():
     with torch.inference_mode():
         frozen = state([(300,)], (True,))
         ops.adamw_step(*frozen[:4], frozen[5], scales=frozen[4])
+
+
+# ---- the block -------------------------------------------------------------------------------------------------------------
+def block(dim=128, **kw):
+    from speed3r_b200 import BlockRope
+    torch.manual_seed(0)
+    return BlockRope(dim, dim // 64, **kw).to(DEV)
+
+
+def by_modules(b, x):
+    """The block's formula, every module called by itself."""
+    x = x + b.ls1(b.attn(b.norm1(x)))
+    return x + b.ls2(b.mlp(b.norm2(x)))
+
+
+def test_a_scale_of_another_formula_takes_part():
+    from speed3r_b200.block import LayerScale
+
+    class Exponential(LayerScale):
+        def forward(self, x):
+            return x * self.gamma.exp()
+
+    b = block(init_values=0.1)
+    b.ls1 = Exponential(128, 0.1).to(DEV)
+    x = torch.randn(2, 512, 128, device=DEV)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(b(x), by_modules(b, x))

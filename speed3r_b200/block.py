@@ -86,10 +86,14 @@ class BlockRope(nn.Module):
 
     @torch.no_grad()
     def quantize_int8(self) -> "BlockRope":
-        """8-bit projections and MLP for inference, in place (parameters on the GPU).  The norms then hand over 8-bit tokens."""
+        """8-bit projections and MLP for inference, in place (parameters on the GPU).  The norms then hand over 8-bit tokens.  For an
+        MLP of two Linears ``fc1`` and ``fc2``; any other ``ffn_layer`` raises, and nothing is changed."""
+        lins = [getattr(self.mlp, n, None) for n in ("fc1", "fc2")]
+        if not all(isinstance(m, (nn.Linear, Int8Linear)) for m in lins):
+            raise RuntimeError(f"quantize_int8: {type(self.mlp).__name__} is not an MLP of two Linears fc1 and fc2")
         self.attn.quantize_int8()
-        if type(self.mlp.fc1) is not Int8Linear:
-            self.mlp.fc1, self.mlp.fc2 = Int8Linear.of(self.mlp.fc1), Int8Linear.of(self.mlp.fc2)
+        if type(lins[0]) is not Int8Linear:
+            self.mlp.fc1, self.mlp.fc2 = (Int8Linear.of(m) for m in lins)
         return self
 
     # ---- pieces ----------------------------------------------------------------------------------------------------------
@@ -133,8 +137,12 @@ class BlockRope(nn.Module):
 
     def _run(self, x: Tensor, h: Union[Tensor, Int8Tokens], xpos, next_norm: Optional[nn.Module], next_int8: bool):
         a = self.attn(h, xpos=xpos)
-        x, h = self._sum_and_norm(x, a, self.norm2, self._scale(self.ls1), self._gate(x), type(self.mlp.fc1) is Int8Linear)
+        x, h = self._sum_and_norm(x, a, self.norm2, self._scale(self.ls1), self._gate(x), self._mlp_takes_int8())
         return self._sum_and_norm(x, self.mlp(h), next_norm, self._scale(self.ls2), self._gate(x), next_int8)
+
+    def _mlp_takes_int8(self) -> bool:
+        """8-bit tokens are for the MLP whose first step is that Linear; another module is given activations."""
+        return type(self.mlp) is Mlp and type(self.mlp.fc1) is Int8Linear
 
     def _takes_int8(self) -> bool:
         return type(getattr(self.attn, "qkv", None)) is Int8Linear

@@ -122,3 +122,26 @@ def test_a_scale_of_another_formula_is_called():
     b = BlockRope(64, 1)
     b.ls1.gamma = torch.full((64,), 3.0)                # an Identity stays one
     assert b._fuses() and b._scale(b.ls1) is None
+
+
+class Gated(torch.nn.Module):
+    """A feed-forward layer of three matrices."""
+
+    def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=None, drop=0.0, bias=True):
+        super().__init__()
+        hidden_features = hidden_features or in_features
+        self.w12 = torch.nn.Linear(in_features, 2 * hidden_features, bias=bias)
+        self.w3 = torch.nn.Linear(hidden_features, out_features or in_features, bias=bias)
+
+    def forward(self, x):
+        a, b = self.w12(x).chunk(2, -1)
+        return self.w3(torch.nn.functional.silu(a) * b)
+
+
+def test_a_feed_forward_layer_of_other_matrices_in_8_bits_raises_and_nothing_changes():
+    from speed3r_b200 import BlockRope
+    b = BlockRope(64, 1, ffn_layer=Gated)
+    kept = {n: type(m) for n, m in b.named_modules()}
+    raises("not an MLP of two Linears", b.quantize_int8)
+    assert {n: type(m) for n, m in b.named_modules()} == kept
+    assert not b._mlp_takes_int8()

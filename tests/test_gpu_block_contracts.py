@@ -118,3 +118,38 @@ def test_a_scale_of_another_formula_takes_part():
     x = torch.randn(2, 512, 128, device=DEV)
     with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
         assert torch.equal(b(x), by_modules(b, x))
+
+
+def test_block_with_another_feed_forward_layer():
+    from test_block_contracts_cpu import Gated
+    from speed3r_b200 import forward_blocks
+
+    b = block(ffn_layer=Gated, init_values=0.1)
+    x = torch.randn(2, 512, 128, device=DEV, requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y, z = b(x), by_modules(b, x)
+        assert torch.equal(forward_blocks([b], x), y)
+    # branches and activations are rounded to bf16 at the same places but for the LayerScales' products: 2^-9 rms each, a chain of ten
+    assert (y - z).norm() <= 0.02 * z.norm()
+    (g,) = torch.autograd.grad(y.sum(), x)
+    (h,) = torch.autograd.grad(z.sum(), x)
+    assert (g - h).norm() <= 0.02 * h.norm()
+
+
+def test_an_mlp_that_is_not_ours_is_given_activations_in_8_bits_too():
+    from speed3r_b200 import Int8Linear, Int8Tokens
+    from speed3r_b200.block import Mlp
+
+    class Other(Mlp):
+        def forward(self, x):
+            assert not isinstance(x, Int8Tokens)
+            return super().forward(x.float().clamp(-2, 2))
+
+    b = block(ffn_layer=Other).eval()
+    x = torch.randn(2, 512, 128, device=DEV)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        want = b(x)
+        got = b.quantize_int8()(x)
+        assert type(b.mlp.fc1) is Int8Linear
+        # four products in a row, about 1 % of noise each
+        assert (got - want).norm() <= 0.06 * (want - x).norm()

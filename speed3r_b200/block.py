@@ -149,7 +149,7 @@ class BlockRope(nn.Module):
 
     def forward(self, x: Tensor, xpos: Optional[Tensor] = None) -> Tensor:
         if not self._fuses():
-            drop = lambda y: y if (g := self._gate(y)) is None else y * g
+            drop = lambda y: y if (g := self._gate(y)) is None else y * g.to(y.dtype)      # the branch keeps its type
             x = x + drop(self.ls1(self.attn(self.norm1(x), xpos=xpos)))
             return x + drop(self.ls2(self.mlp(self.norm2(x))))
         x = self._residual(x)

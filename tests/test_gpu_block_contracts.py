@@ -153,3 +153,15 @@ def test_an_mlp_that_is_not_ours_is_given_activations_in_8_bits_too():
         assert type(b.mlp.fc1) is Int8Linear
         # four products in a row, about 1 % of noise each
         assert (got - want).norm() <= 0.06 * (want - x).norm()
+
+
+@pytest.mark.parametrize("watch", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_stochastic_depth_keeps_the_type(dtype, watch):
+    """With and without modules called one by one, in training and not."""
+    b = block(init_values=None, drop_path=0.4).bfloat16()
+    if watch:
+        b.norm2.register_forward_hook(lambda *a: None)
+    x = torch.randn(3, 512, 128, device=DEV).to(dtype)
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.float32):
+        assert b.train()(x).dtype == dtype and b.eval()(x).dtype == dtype

@@ -113,6 +113,12 @@ class BlockRope(nn.Module):
                 all(type(m) is nn.Identity or (type(m) is LayerScale and tuple(m.gamma.shape) == (self.dim,)) for m in (self.ls1, self.ls2)) and
                 not any(_watched(m) for m in (self.ls1, self.ls2)))
 
+    def _fits(self, x: Tensor) -> bool:
+        """``ops.residual_norm`` has a kernel for this input: not on the CPU, of its types, no wider than it reaches."""
+        params = (p for m in (self.norm1, self.norm2, self.ls1, self.ls2) for p in m._parameters.values() if p is not None)
+        return (x.device.type != "cpu" and x.dtype in ops.NORM_TYPES and 1 <= x.shape[-1] <= ops.NORM_MAX_CHANNELS and
+                all(p.dtype in ops.NORM_TYPES for p in params))
+
     def _residual(self, x: Tensor) -> Tensor:
         """x in the type that the sum with a scaled branch has."""
         kept = x.dtype
@@ -148,7 +154,7 @@ class BlockRope(nn.Module):
         return type(getattr(self.attn, "qkv", None)) is Int8Linear
 
     def forward(self, x: Tensor, xpos: Optional[Tensor] = None) -> Tensor:
-        if not self._fuses():
+        if not (self._fuses() and self._fits(x)):
             drop = lambda y: y if (g := self._gate(y)) is None else y * g.to(y.dtype)      # the branch keeps its type
             x = x + drop(self.ls1(self.attn(self.norm1(x), xpos=xpos)))
             return x + drop(self.ls2(self.mlp(self.norm2(x))))
@@ -160,7 +166,7 @@ class BlockRope(nn.Module):
 def forward_blocks(blocks: Sequence[BlockRope], x: Tensor, xpos: Optional[Tensor] = None) -> Tensor:
     """``for block in blocks: x = block(x, xpos)``, with the sum at the end of a block and the first norm of the next one in one pass."""
     blocks = list(blocks)
-    if not all(type(b) is BlockRope and not _watched(b) and b._fuses() for b in blocks):
+    if not all(type(b) is BlockRope and not _watched(b) and b._fuses() and b._fits(x) for b in blocks):
         for b in blocks:
             x = b(x, xpos=xpos)
         return x

@@ -290,6 +290,7 @@ def sel_attn_merge_chunked(q, k_chunks, v_chunks, topk_idx, gate, o_c, block_siz
 # ------------------------------------------------------------------------------------------------
 _KINDS = {"layer": 0, "rms": 1}
 NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+NORM_MAX_CHANNELS = 8192
 
 
 def _norm_args(norm, post_norm, kind):

@@ -145,3 +145,31 @@ def test_a_feed_forward_layer_of_other_matrices_in_8_bits_raises_and_nothing_cha
     raises("not an MLP of two Linears", b.quantize_int8)
     assert {n: type(m) for n, m in b.named_modules()} == kept
     assert not b._mlp_takes_int8()
+
+
+class Plain(torch.nn.Module):
+    """An attention that runs anywhere."""
+
+    def __init__(self, dim, num_heads, **kw):
+        super().__init__()
+        self.lin = torch.nn.Linear(dim, dim)
+
+    def forward(self, x, xpos=None):
+        return self.lin(x)
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, torch.float32), (64, torch.float64), (8200, torch.float32), (64, torch.bfloat16)])
+def test_a_block_that_the_kernels_do_not_reach_is_computed_by_its_modules(dim, dtype):
+    from speed3r_b200 import BlockRope, forward_blocks
+    torch.manual_seed(0)
+    b = BlockRope(dim, 1, mlp_ratio=1 / 64 if dim > 64 else 4.0, attn_class=Plain, init_values=0.3).to(dtype)
+    x = torch.randn(2, 5, dim, dtype=dtype)
+    y = x + b.ls1(b.attn(b.norm1(x)))
+    y = y + b.ls2(b.mlp(b.norm2(y)))
+    assert torch.equal(b(x), y) and torch.equal(forward_blocks([b], x), y) and y.dtype == dtype
+
+
+def test_stochastic_depth_keeps_the_type_of_the_branch():
+    from speed3r_b200 import BlockRope
+    b = BlockRope(64, 1, attn_class=Plain, drop_path=0.4).bfloat16().train()
+    assert b(torch.randn(3, 5, 64).bfloat16()).dtype == torch.bfloat16

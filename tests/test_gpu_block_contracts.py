@@ -165,3 +165,17 @@ def test_stochastic_depth_keeps_the_type(dtype, watch):
     x = torch.randn(3, 512, 128, device=DEV).to(dtype)
     with torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.float32):
         assert b.train()(x).dtype == dtype and b.eval()(x).dtype == dtype
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, torch.float64), (8200, torch.float32), (8192, torch.float32)])
+def test_a_block_that_the_norm_kernels_do_not_reach(dim, dtype):
+    from test_block_contracts_cpu import Plain
+    from speed3r_b200 import forward_blocks
+
+    b = block(dim, mlp_ratio=1 / 64 if dim > 64 else 4.0, attn_class=Plain, init_values=0.3).to(dtype)
+    x = torch.randn(2, 5, dim, device=DEV, dtype=dtype)
+    with torch.no_grad():
+        y, z = b(x), by_modules(b, x)
+        # the same PyTorch operations, or at 8192 channels fp32 sums of as many terms in another order
+        assert (y - z).norm() <= (0 if dim != 8192 else 8192 * 2.0 ** -24) * z.norm()
+        assert torch.equal(forward_blocks([b], x), y)

@@ -43,6 +43,15 @@ class Int8Linear(nn.Module):
         q, scale = ops.quantize_tokens(torch.cat([m.weight.detach().float() for m in linears]))
         return cls(q, scale, None if biases[0] is None else torch.cat([b.detach().float() for b in biases]), out_dtype)
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves as any module; scales and bias stay fp32, which ``ops.int8_linear`` takes, through ``.bfloat16()`` and the like."""
+        kept = {n: b for n, b in self._buffers.items() if n in ("weight_scale", "bias") and b is not None}
+        super()._apply(fn, recurse)
+        for n, b in kept.items():
+            if self._buffers[n].dtype != b.dtype:
+                self._buffers[n] = b.to(self._buffers[n].device)
+        return self
+
     def forward(self, x: Union[Tensor, Int8Tokens]) -> Tensor:
         if not isinstance(x, Int8Tokens):
             x = Int8Tokens(*ops.quantize_tokens(x))

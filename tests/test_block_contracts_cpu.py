@@ -173,3 +173,17 @@ def test_stochastic_depth_keeps_the_type_of_the_branch():
     from speed3r_b200 import BlockRope
     b = BlockRope(64, 1, attn_class=Plain, drop_path=0.4).bfloat16().train()
     assert b(torch.randn(3, 5, 64).bfloat16()).dtype == torch.bfloat16
+
+
+# ---- 8 bits ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("change", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.float16)])
+def test_scales_of_an_8_bit_linear_stay_fp32(change):
+    from speed3r_b200 import Int8Linear
+    scale, bias = torch.rand(5) + 0.1, torch.randn(5)
+    m = torch.nn.Sequential(Int8Linear(torch.zeros(5, 16, dtype=torch.int8), scale.clone(), bias.clone()), torch.nn.Linear(5, 5))
+    change(m)
+    assert torch.equal(m[0].weight_scale, scale) and torch.equal(m[0].bias, bias) and m[0].weight.dtype == torch.int8
+    assert m[0].weight_scale.dtype == m[0].bias.dtype == torch.float32 and m[1].weight.dtype != torch.float32
+    assert set(m.state_dict()) == {"0.weight", "0.weight_scale", "0.bias", "1.weight", "1.bias"}
+    assert Int8Linear(torch.zeros(5, 16, dtype=torch.int8), scale, None).half().bias is None
+    assert m.to("meta")[0].weight_scale.device.type == "meta"

@@ -179,3 +179,16 @@ def test_a_block_that_the_norm_kernels_do_not_reach(dim, dtype):
         # the same PyTorch operations, or at 8192 channels fp32 sums of as many terms in another order
         assert (y - z).norm() <= (0 if dim != 8192 else 8192 * 2.0 ** -24) * z.norm()
         assert torch.equal(forward_blocks([b], x), y)
+
+
+# ---- 8 bits ----------------------------------------------------------------------------------------------------------------
+def test_a_block_in_8_bits_becomes_bf16():
+    b = block(init_values=0.1).eval().quantize_int8()
+    x = torch.randn(2, 512, 128, device=DEV).bfloat16()
+    with torch.no_grad():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            want = b(x.float())
+        got = b.bfloat16()(x)
+    assert got.dtype == torch.bfloat16 and b.mlp.fc1.weight_scale.dtype == torch.float32
+    # parameters of norms and scales in bf16, sums rounded to bf16 three times
+    assert (got - want).norm() <= 0.06 * want.norm()

@@ -91,9 +91,9 @@ class BlockRope(nn.Module):
         lins = [getattr(self.mlp, n, None) for n in ("fc1", "fc2")]
         if not all(isinstance(m, (nn.Linear, Int8Linear)) for m in lins):
             raise RuntimeError(f"quantize_int8: {type(self.mlp).__name__} is not an MLP of two Linears fc1 and fc2")
+        narrow = [m if type(m) is Int8Linear else Int8Linear.of(m) for m in lins]
         self.attn.quantize_int8()
-        if type(lins[0]) is not Int8Linear:
-            self.mlp.fc1, self.mlp.fc2 = (Int8Linear.of(m) for m in lins)
+        self.mlp.fc1, self.mlp.fc2 = narrow
         return self
 
     # ---- pieces ----------------------------------------------------------------------------------------------------------

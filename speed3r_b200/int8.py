@@ -37,6 +37,9 @@ class Int8Linear(nn.Module):
     @torch.no_grad()
     def of(cls, *linears: nn.Linear, out_dtype: torch.dtype = torch.bfloat16) -> "Int8Linear":
         """The 8-bit form of a Linear on the GPU, or of several that read the same input, their outputs side by side."""
+        for m in linears:
+            if not isinstance(m, nn.Linear) or type(m).forward is not nn.Linear.forward or "forward" in m.__dict__:
+                raise RuntimeError(f"Int8Linear.of: {type(m).__name__} computes something else than a Linear")
         biases = [m.bias for m in linears]
         if any(b is None for b in biases) and any(b is not None for b in biases):
             biases = [b if b is not None else torch.zeros(m.out_features, device=m.weight.device) for b, m in zip(biases, linears)]

@@ -300,8 +300,7 @@ class SparseFlashAttentionRope(nn.Module):
         """Replaces the projections by 8-bit ones, for inference, in place (parameters on the GPU).  ``forward`` then takes
         activations or ``Int8Tokens``."""
         if self.proj.weight.dtype != torch.int8:
-            self.qkv, self.proj = Int8Linear.of(self.qkv), Int8Linear.of(self.proj)
-            self.gate[0] = Int8Linear.of(self.gate[0])
+            self.qkv, self.proj, self.gate[0] = (Int8Linear.of(m) for m in (self.qkv, self.proj, self.gate[0]))
         return self
 
     def forward(self, x: Tensor, attn_bias=None, xpos: Optional[Tensor] = None) -> Tensor:

@@ -187,3 +187,19 @@ def test_scales_of_an_8_bit_linear_stay_fp32(change):
     assert set(m.state_dict()) == {"0.weight", "0.weight_scale", "0.bias", "1.weight", "1.bias"}
     assert Int8Linear(torch.zeros(5, 16, dtype=torch.int8), scale, None).half().bias is None
     assert m.to("meta")[0].weight_scale.device.type == "meta"
+
+
+class Adapted(torch.nn.Linear):
+    """A Linear with something beside it, as fine-tuning adds."""
+
+    def forward(self, x):
+        return super().forward(x) + x.sum(-1, keepdim=True)
+
+
+def test_what_is_more_than_a_linear_does_not_become_an_8_bit_one():
+    from speed3r_b200 import BlockRope, Int8Linear
+    raises("something else than a Linear", lambda: Int8Linear.of(Adapted(16, 5)))
+    raises("something else than a Linear", lambda: Int8Linear.of(torch.nn.Identity()))
+    wrapped = torch.nn.Linear(16, 5)
+    wrapped.forward = lambda x: x
+    raises("something else than a Linear", lambda: Int8Linear.of(wrapped))

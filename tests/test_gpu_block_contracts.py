@@ -192,3 +192,16 @@ def test_a_block_in_8_bits_becomes_bf16():
     assert got.dtype == torch.bfloat16 and b.mlp.fc1.weight_scale.dtype == torch.float32
     # parameters of norms and scales in bf16, sums rounded to bf16 three times
     assert (got - want).norm() <= 0.06 * want.norm()
+
+
+@pytest.mark.parametrize("where", ["attn.qkv", "attn.proj", "attn.gate.0", "mlp.fc1", "mlp.fc2"])
+def test_a_block_that_cannot_become_8_bit_stays_as_it_is(where):
+    from test_block_contracts_cpu import Adapted
+
+    b = block()
+    old = b.get_submodule(where)
+    b.set_submodule(where, Adapted(old.in_features, old.out_features).to(DEV))
+    kept = {n: type(m) for n, m in b.named_modules()}
+    with pytest.raises(RuntimeError, match="something else than a Linear"):
+        b.quantize_int8()
+    assert {n: type(m) for n, m in b.named_modules()} == kept

@@ -93,16 +93,34 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As PyTorch's, but a state keeps its own type (PyTorch casts it to its parameter's), and counts that were shared are again."""
+        """A state dict of this class or of ``torch.optim.AdamW`` (whose states become fp32; ``maximize`` and ``amsgrad`` raise).  States keep
+        their own type where PyTorch casts them to their parameter's; what a group does not say stays as it is; counts that were shared
+        are again."""
+        for g in state_dict["param_groups"]:
+            for name in ("maximize", "amsgrad"):
+                if g.get(name):
+                    raise RuntimeError(f"AdamW: a state dict with {name} belongs to another optimiser")
+        mine = [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)
+        for old, g in zip(mine, self.param_groups):
+            for name, value in old.items():
+                g.setdefault(name, value)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(device=p.device, copy=True) if isinstance(v, Tensor) else v for k, v in state_dict["state"][i].items()}
+                self.state[p] = self._loaded(p, state_dict["state"][i])
         for g in self.param_groups:
             shared: dict = {}
             for p in g["params"]:
                 st = self.state.get(p)
                 if st:
                     st["step"] = shared.setdefault((p.device, int(st["step"])), st["step"])
+
+    @staticmethod
+    def _loaded(p: Tensor, st: dict) -> dict:
+        if not st:
+            return {}
+        types = dict(step=torch.int64, scales=torch.uint8)
+        types["exp_avg"] = types["exp_avg_sq"] = torch.uint8 if st.get("scales") is not None else torch.float32
+        return {k: torch.as_tensor(st[k]).detach().to(device=p.device, dtype=t, copy=True).contiguous() for k, t in types.items() if st.get(k) is not None}

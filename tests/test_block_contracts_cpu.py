@@ -203,3 +203,48 @@ def test_what_is_more_than_a_linear_does_not_become_an_8_bit_one():
     wrapped = torch.nn.Linear(16, 5)
     wrapped.forward = lambda x: x
     raises("something else than a Linear", lambda: Int8Linear.of(wrapped))
+
+
+# ---- optimiser -------------------------------------------------------------------------------------------------------------
+def stepped(params, steps=3, **kw):
+    """torch.optim.AdamW after some steps, some parameters from the second on."""
+    opt = torch.optim.AdamW(params, **kw)
+    for i in range(steps):
+        for k, p in enumerate(params):
+            p.grad = torch.full_like(p, 0.1 * (k + 1)) if i or k else None
+        opt.step()
+    return opt
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_state_dict_of_pytorchs_adamw_loads(dtype):
+    from speed3r_b200 import AdamW
+    make = lambda: [torch.nn.Parameter(torch.ones(3, 4, dtype=dtype)), torch.nn.Parameter(torch.ones(5, dtype=dtype))]
+    theirs = stepped(make(), lr=2e-3, betas=(0.8, 0.9), weight_decay=0.3)
+    saved = theirs.state_dict()
+    params = make()
+    opt = AdamW(params, lr=1.0, state_bits=8, seed=7)
+    opt.load_state_dict(saved)
+    (group,) = opt.param_groups
+    assert (group["lr"], group["betas"], group["weight_decay"]) == (2e-3, (0.8, 0.9), 0.3)
+    assert (group["state_bits"], group["min_8bit_size"], group["seed"]) == (8, 4096, 7)
+    for p, i in zip(params, range(2)):
+        st, want = opt.state[p], saved["state"][i]
+        assert st["step"].dtype == torch.int64 and int(st["step"]) == int(want["step"]) == 2 + i
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert st[name].dtype == torch.float32 and torch.equal(st[name], want[name].float()) and st[name].data_ptr() != want[name].data_ptr()
+    # as older versions save it: the count as a number
+    old = {"state": {i: {**st, "step": int(st["step"])} for i, st in saved["state"].items()}, "param_groups": saved["param_groups"]}
+    opt.load_state_dict(old)
+    assert [int(opt.state[p]["step"]) for p in params] == [2, 3] and opt.state[params[0]]["step"].dtype == torch.int64
+
+
+@pytest.mark.parametrize("name", ["maximize", "amsgrad"])
+def test_a_state_dict_of_another_formula_is_refused(name):
+    from speed3r_b200 import AdamW
+    make = lambda: [torch.nn.Parameter(torch.ones(3))]
+    saved = stepped(make(), **{name: True}).state_dict()
+    params = make()
+    opt = AdamW(params, lr=0.5)
+    raises(name, lambda: opt.load_state_dict(saved))
+    assert opt.param_groups[0]["lr"] == 0.5 and not opt.state

@@ -205,3 +205,32 @@ def test_a_block_that_cannot_become_8_bit_stays_as_it_is(where):
     with pytest.raises(RuntimeError, match="something else than a Linear"):
         b.quantize_int8()
     assert {n: type(m) for n, m in b.named_modules()} == kept
+
+
+# ---- optimiser -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fused", [False, True])
+def test_a_run_of_pytorchs_adamw_goes_on(fused):
+    from speed3r_b200 import AdamW
+
+    make = lambda: [torch.nn.Parameter(torch.linspace(-1, 1, n, device=DEV)) for n in (300, 5000)]
+    a, b = make(), make()
+    theirs = torch.optim.AdamW(a, lr=1e-2, betas=(0.8, 0.95), fused=fused)
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    grads = [[torch.randn(p.shape, device=DEV, generator=gen) for p in a] for _ in range(6)]
+
+    def go(params, opt, rounds):
+        for gs in rounds:
+            for p, g in zip(params, gs):
+                p.grad = g.clone()
+            opt.step()
+
+    go(a, theirs, grads[:3])
+    ours = AdamW(b, lr=1.0)
+    ours.load_state_dict(theirs.state_dict())
+    for p, q in zip(a, b):
+        q.data.copy_(p.data)
+    go(a, theirs, grads[3:])
+    go(b, ours, grads[3:])
+    for p, q in zip(a, b):
+        # three steps of lr, each off by a few 2^-23 of itself, and the parameter's own rounding
+        assert ((p - q).abs() <= 8 * 2.0 ** -24 * p.abs() + 3 * 1e-2 * 40 * 2.0 ** -24).all()

@@ -405,7 +405,7 @@ int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, cons
  * (-1)^(c >> 7) * (E ? (1 + f / 8) 2^(E - 15) : f / 8 2^-14) with E = (c >> 3) & 15, f = c & 7, one of v for
  * E ? (1 + f / 8) 2^(E - 31) : f / 8 2^-30 with E = c >> 3; both times 2^(exponent - 127), exponent 255: NaN.
  * seed < 0: what is kept in fewer than 32 bits is rounded to nearest even, else stochastically with Philox 2x32-7, counter (pair of
- * elements, t), key seed + index of the tensor * 0x85EBCA6B (mod 2^32).
+ * elements, t), key (seed mod 2^32) + (seed >> 32) * 0xC2B2AE35 + number of the tensor * 0x85EBCA6B (mod 2^32).
  * Arrays are HOST arrays; lr: a device pointer that is read on the stream, or NULL for lr_host. */
 typedef struct {
   int n;
@@ -426,6 +426,9 @@ typedef struct {
   void* workspace;            /* 256 bytes */
 } s3r_adamw;
 int s3r_adamw_step(const s3r_adamw* args_host, void* stream);
+/* The same with the tensors' numbers (HOST array, each below 2^24), by which their random numbers go; NULL, and above: their index.  A program
+ * whose lists change from step to step, or that makes several calls per step, gives every tensor a number of its own. */
+int s3r_adamw_step_numbered(const s3r_adamw* args_host, const uint32_t* numbers, void* stream);
 
 /* What 8-bit states stand for: m, v (codes) -> fp32. */
 int s3r_adamw_state(int n, const void* const* m, const void* const* v, const uint8_t* const* m_exponents, const uint8_t* const* v_exponents,

@@ -54,6 +54,7 @@ SIGNATURES = {
     "s3r_grad_norm_workspace_bytes": (_sz, [_i, _p]),
     "s3r_grad_norm": (_i, [_i, _p, _p, _p, _p, _p, _sz, _p]),
     "s3r_adamw_step": (_i, [_p, _p]),
+    "s3r_adamw_step_numbered": (_i, [_p, _p, _p]),
     "s3r_adamw_state": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p]),
     "s3r_copy2d_async": (_i, [_p, _sz, _p, _sz, _sz, _sz, _p]),
     "s3r_peer_pull": (_i, [_p, _p, _p, _i, _i, _p]),

@@ -36,7 +36,7 @@ struct AdamTensor {
   uint8_t *me, *ve;
   int64_t n;
   int64_t first;       // CTA
-  uint32_t flags;      // types (2 bits each), vectors, 8-bit states, index << 8
+  uint32_t flags;      // types (2 bits each), vectors, 8-bit states, number << 8
 };
 struct AdamCommon {
   int n;
@@ -561,7 +561,9 @@ extern "C" int s3r_grad_norm(int n, const void* const* tensors, const int64_t* c
   return launch(grad_norm_end_kernel, 1u, 1024, 0, st, static_cast<const double*>(workspace), all, norm);
 }
 
-extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
+extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) { return s3r_adamw_step_numbered(args, nullptr, stream); }
+
+extern "C" int s3r_adamw_step_numbered(const s3r_adamw* args, const uint32_t* numbers, void* stream) {
   S3R_REQUIRE(args, S3R_ERR_NULL, "s3r_adamw_step: NULL pointer");
   const s3r_adamw& a = *args;
   S3R_REQUIRE(a.n >= 0, S3R_ERR_SHAPE, "s3r_adamw_step: %d tensors", a.n);
@@ -579,7 +581,7 @@ extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
     S3R_REQUIRE(reinterpret_cast<uintptr_t>(a.params[i]) % type_bytes(a.param_types[i]) == 0 && reinterpret_cast<uintptr_t>(a.grads[i]) % type_bytes(a.grad_types[i]) == 0 &&
                     (eight || (reinterpret_cast<uintptr_t>(a.m[i]) | reinterpret_cast<uintptr_t>(a.v[i])) % 4 == 0), S3R_ERR_ALIGNMENT, "s3r_adamw_step: elements must be aligned");
     S3R_REQUIRE(a.counts[i] < (1ll << 33), S3R_ERR_TOO_LARGE, "s3r_adamw_step: more than 2^33 elements in a tensor");
-    S3R_REQUIRE(i < (1 << 24), S3R_ERR_TOO_LARGE, "s3r_adamw_step: too many tensors");
+    S3R_REQUIRE((numbers ? numbers[i] : static_cast<uint32_t>(i)) < 1u << 24, S3R_ERR_TOO_LARGE, "s3r_adamw_step: tensors are numbered below 2^24");
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   AdamScalars* scalars = static_cast<AdamScalars*>(a.workspace);
@@ -593,7 +595,8 @@ extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
   p.c.b2 = static_cast<float>(a.beta2);
   p.c.c2 = static_cast<float>(1.0 - a.beta2);
   p.c.eps = static_cast<float>(a.eps);
-  p.c.seed = a.seed;
+  p.c.seed = static_cast<uint32_t>(a.seed) + static_cast<uint32_t>(a.seed >> 32) * 0xC2B2AE35u;
+  if (a.seed < 0) p.c.seed = -1;
   p.c.scalars = scalars;
   p.c.n = 0;
   int64_t ctas = 0;
@@ -616,7 +619,7 @@ extern "C" int s3r_adamw_step(const s3r_adamw* args, void* stream) {
     if (i == a.n || a.counts[i] == 0) continue;
     uint8_t *me = a.m_exponents ? a.m_exponents[i] : nullptr, *ve = a.v_exponents ? a.v_exponents[i] : nullptr;
     const uint32_t flags = static_cast<uint32_t>(a.param_types[i]) | static_cast<uint32_t>(a.grad_types[i]) << 2 |
-                           (at_16({a.params[i], a.grads[i], a.m[i], a.v[i]}) ? kAdamVector : 0u) | (me ? kAdamEight : 0u) | static_cast<uint32_t>(i) << 8;
+                           (at_16({a.params[i], a.grads[i], a.m[i], a.v[i]}) ? kAdamVector : 0u) | (me ? kAdamEight : 0u) | (numbers ? numbers[i] : static_cast<uint32_t>(i)) << 8;
     p.t[p.c.n++] = {a.params[i], a.grads[i], a.m[i], a.v[i], me, ve, a.counts[i], ctas, flags};
     ctas += (a.counts[i] + kAdamPerCta - 1) / kAdamPerCta;
     S3R_REQUIRE(ctas < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_adamw_step: grid too large");

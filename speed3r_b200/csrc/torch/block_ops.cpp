@@ -471,7 +471,7 @@ void need_states(const Tensor& p, const Tensor& m, const Tensor& v, const option
 // take none of its gaps, and a list that is not declared is read again from before the step.
 void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
                 at::TensorList scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
-                double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
+                double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed, at::OptionalIntArrayRef numbers) {
   const size_t n = params.size();
   TORCH_CHECK(n > 0, "adamw: no tensors");
   TORCH_CHECK(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n, "adamw: ", n, " parameters, ", grads.size(), " gradients, ",
@@ -484,6 +484,14 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
     TORCH_CHECK(!t->has_value() || ((*t)->device() == device && (*t)->scalar_type() == at::kFloat && (*t)->numel() == 1),
                 "adamw: grad_norm and lr as tensors must be one fp32 on the parameters' device");
   TORCH_CHECK(max_norm <= 0 || norm.has_value(), "adamw: max_norm needs grad_norm");
+  std::vector<uint32_t> number_of;
+  if (numbers.has_value()) {
+    TORCH_CHECK(numbers->size() == n, "adamw: ", n, " parameters, ", numbers->size(), " numbers");
+    for (const int64_t i : *numbers) {
+      TORCH_CHECK(i >= 0 && i < (1 << 24), "adamw: numbers are 0 to 2^24 - 1, got ", i);
+      number_of.push_back(static_cast<uint32_t>(i));
+    }
+  }
   std::vector<Tensor> kept;
   std::vector<void*> p(n), m(n), v(n);
   std::vector<const void*> g(n);
@@ -548,7 +556,7 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
   a.max_norm = max_norm;
   a.seed = seed;
   a.workspace = ws.data_ptr();
-  check(s3r_adamw_step(&a, stream()), "s3r_adamw_step");
+  check(s3r_adamw_step_numbered(&a, number_of.empty() ? nullptr : number_of.data(), stream()), "s3r_adamw_step");
 }
 
 void adamw_values(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
@@ -607,7 +615,7 @@ Tensor grad_norm(at::TensorList tensors) {
 }
 void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, const Tensor& step,
                 const c10::List<optional<Tensor>>& scales, double lr, const optional<Tensor>& lr_tensor, double beta1, double beta2, double eps,
-                double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed) {
+                double weight_decay, const optional<Tensor>& norm, double max_norm, int64_t seed, at::OptionalIntArrayRef numbers) {
   TORCH_CHECK(!params.empty(), "adamw: no tensors");
   no_tangents(params, grads, exp_avg, exp_avg_sq, lr_tensor, norm);
   std::vector<Tensor> held;
@@ -622,11 +630,11 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
     }
   }
   if (plain(params[0])) {
-    adamw_update(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+    adamw_update(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed, numbers);
     for (const auto list : {params, exp_avg, exp_avg_sq, at::TensorList(held), at::TensorList(step)}) written(list);
     return;
   }
-  S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed);
+  S3R_DISPATCHED(adamw_update)(params, grads, exp_avg, exp_avg_sq, step, held, lr, lr_tensor, beta1, beta2, eps, weight_decay, norm, max_norm, seed, numbers);
 }
 void adamw_state(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList scales, at::TensorList m_out, at::TensorList v_out) {
   no_tangents(m_out, v_out);
@@ -655,13 +663,13 @@ TORCH_LIBRARY_FRAGMENT(speed3r_b200, m) {
   m.def("int8_product(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor");
   m.def("norm_of(Tensor[] tensors) -> Tensor");
   m.def("adamw_update(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor(e!)[] scales, float lr, "
-        "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()");
+        "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed, int[]? numbers=None) -> ()");
   m.def("adamw_values(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()");
   m.def("quantize_tokens(Tensor x) -> (Tensor, Tensor)", &quantize_tokens);
   m.def("int8_linear(Tensor q, Tensor q_scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_type) -> Tensor", &int8_linear);
   m.def("grad_norm(Tensor[] tensors) -> Tensor", &grad_norm);
   m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!) step, Tensor(e!)?[] scales, float lr, "
-        "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed) -> ()", &adamw_step);
+        "Tensor? lr_tensor, float beta1, float beta2, float eps, float weight_decay, Tensor? norm, float max_norm, int seed, int[]? numbers=None) -> ()", &adamw_step);
   m.def("adamw_state(Tensor[] exp_avg, Tensor[] exp_avg_sq, Tensor[] scales, Tensor(a!)[] m_out, Tensor(b!)[] v_out) -> ()", &adamw_state);
 }
 

@@ -365,7 +365,7 @@ def grad_norm(tensors) -> Tensor:
 @torch.no_grad()
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step: Tensor, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, grad_norm: Optional[Tensor] = None, max_norm: Optional[float] = None, scales=None,
-               seed: Optional[int] = None) -> None:
+               seed: Optional[int] = None, numbers=None) -> None:
     """One AdamW step in place over lists of tensors of one device, in one pass::
 
         g = grad * min(1, max_norm / (grad_norm + 1e-6))         (with max_norm)
@@ -376,7 +376,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: Tensor, lr=1e-3, betas=
     ``grad_norm`` is given and not finite, nothing changes.  States are fp32, or, where ``scales`` (a list, entries may be None) has a
     uint8 ``[2, ceil(n / 256)]`` for a tensor, uint8 codes: see ``adamw_state``.  With ``seed`` (0 to 2^63 - 1) what is kept in fewer
     bits than 32 - 8-bit states, bf16 parameters - is rounded stochastically, the same way for the same seed and step; without it to
-    nearest.  Parameters: fp32, bf16 or fp16, contiguous."""
+    nearest.  A tensor's random numbers go by its index in the lists, or by its entry in ``numbers`` (one integer below 2^24 per
+    tensor): give every tensor its own where several calls make up a step.  Parameters: fp32, bf16 or fp16, contiguous."""
     if seed is not None and not 0 <= int(seed) < 1 << 63:
         raise RuntimeError(f"adamw_step: seed {seed}")
     if max_norm is not None and not max_norm > 0:
@@ -386,7 +387,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: Tensor, lr=1e-3, betas=
     on_device = isinstance(lr, Tensor)
     _ops().adamw_step.default(list(params), list(grads), list(exp_avg), list(exp_avg_sq), step, [] if scales is None else list(scales),
                               0.0 if on_device else float(lr), lr if on_device else None, float(betas[0]), float(betas[1]), float(eps),
-                              float(weight_decay), grad_norm, 0.0 if max_norm is None else float(max_norm), -1 if seed is None else int(seed))
+                              float(weight_decay), grad_norm, 0.0 if max_norm is None else float(max_norm), -1 if seed is None else int(seed),
+                              None if numbers is None else list(numbers))
 
 
 @torch.no_grad()

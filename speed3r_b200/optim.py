@@ -55,7 +55,13 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
+        # a parameter's number over all groups: its random numbers do not depend on which others have a gradient
+        first, work, numbers = 0, [], {}
+        for g in self.param_groups:
+            work.append((g, [p for p in g["params"] if p.grad is not None]))
+            if g["seed"] is not None:
+                numbers.update((id(p), first + i) for i, p in enumerate(g["params"]))
+            first += len(g["params"])
         for _, params in work:
             for p in params:
                 if p.grad.is_sparse:
@@ -89,7 +95,8 @@ class AdamW(torch.optim.Optimizer):
                 states = [self.state[p] for p in together]
                 ops.adamw_step(together, [p.grad for p in together], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step,
                                lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_norm=norm,
-                               max_norm=self.max_norm, scales=[s.get("scales") for s in states], seed=group["seed"])
+                               max_norm=self.max_norm, scales=[s.get("scales") for s in states], seed=group["seed"],
+                               numbers=None if group["seed"] is None else [numbers[id(p)] for p in together])
         return loss
 
     def load_state_dict(self, state_dict):

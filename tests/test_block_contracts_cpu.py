@@ -248,3 +248,36 @@ def test_a_state_dict_of_another_formula_is_refused(name):
     opt = AdamW(params, lr=0.5)
     raises(name, lambda: opt.load_state_dict(saved))
     assert opt.param_groups[0]["lr"] == 0.5 and not opt.state
+
+
+def test_numbers_of_a_step_are_checked_without_a_gpu(lib):
+    import ctypes as C
+    from test_block_ops_cpu import AdamArgs
+
+    buf = C.create_string_buffer(4096)
+    p = (C.addressof(buf) + 255) & ~255
+    one, count, types = (C.c_void_p * 1)(p), (C.c_int64 * 1)(4), (C.c_int * 1)(0)
+    at = lambda x: C.cast(x, C.c_void_p)
+    a = AdamArgs(n=1, params=at(one), grads=at(one), m=at(one), v=at(one), counts=at(count), param_types=at(types), grad_types=at(types), step=p,
+                 lr_host=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, seed=1, workspace=p)
+    assert lib.s3r_adamw_step_numbered(None, None, None) == -4
+    assert lib.s3r_adamw_step_numbered(C.byref(a), at((C.c_uint32 * 1)(1 << 24)), None) == -6
+
+
+def test_the_optimiser_numbers_its_parameters(monkeypatch):
+    """Over all groups, whichever of them have a gradient and however many calls a step makes."""
+    from speed3r_b200 import AdamW
+    seen = []
+    monkeypatch.setattr(ops, "adamw_step", lambda params, *a, numbers=None, **kw: seen.extend(zip([id(p) for p in params], numbers or [None] * len(params))))
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(5)]
+    opt = AdamW([dict(params=ps[:3]), dict(params=ps[3:], weight_decay=0.0)])
+    for missing in ((), (0,), (1, 3), ()):
+        for i, p in enumerate(ps):
+            p.grad = None if i in missing else torch.ones(3)
+        seen.clear()
+        opt.step()
+        assert sorted(seen) == sorted((id(p), i) for i, p in enumerate(ps) if i not in missing)
+    opt = AdamW(ps, seed=None)
+    seen.clear()
+    opt.step()
+    assert [n for _, n in seen] == [None] * 5

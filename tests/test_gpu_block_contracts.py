@@ -234,3 +234,37 @@ def test_a_run_of_pytorchs_adamw_goes_on(fused):
     for p, q in zip(a, b):
         # three steps of lr, each off by a few 2^-23 of itself, and the parameter's own rounding
         assert ((p - q).abs() <= 8 * 2.0 ** -24 * p.abs() + 3 * 1e-2 * 40 * 2.0 ** -24).all()
+
+
+def test_random_numbers_go_by_seed_and_number():
+    def codes(numbers=None, seed=5, count=2):
+        p, g, m, v, e, step = state([(2000,)], (True,), seed=3)
+        p, g, m, v, e = ([ts[0].clone() for _ in range(count)] for ts in (p, g, m, v, e))       # the same tensor over and over
+        ops.adamw_step(p, g, m, v, step, scales=e, seed=seed, numbers=numbers)
+        return m
+
+    by_index = codes()
+    assert not torch.equal(*by_index) and not torch.equal(*codes([9, 8])) and torch.equal(*codes([7, 7]))
+    assert all(torch.equal(a, b) for a, b in zip(by_index, codes([0, 1])))
+    assert torch.equal(codes([1, 0])[0], by_index[1]) and torch.equal(codes([1], count=1)[0], by_index[1])
+    assert not torch.equal(codes(seed=5 + (1 << 32))[0], by_index[0]) and not torch.equal(codes(seed=5 + (1 << 62))[0], by_index[0])
+    for bad in ([0], [0, -1], [0, 1 << 24]):
+        with pytest.raises(RuntimeError, match="numbers"):
+            codes(bad)
+
+
+def test_groups_round_by_themselves_and_a_missing_gradient_changes_nothing_else():
+    from speed3r_b200 import AdamW
+
+    def run(missing=()):
+        ps = [torch.nn.Parameter(torch.linspace(1, 2, 8192, device=DEV).bfloat16()) for _ in range(4)]
+        opt = AdamW([dict(params=ps[:2]), dict(params=ps[2:])], lr=1e-3, weight_decay=0.0, state_bits=8)
+        for k in range(3):
+            for i, p in enumerate(ps):
+                p.grad = None if i in missing and k else torch.full_like(p, 0.1)
+            opt.step()
+        return ps, [opt.state[p]["exp_avg"] for p in ps]
+
+    (ps, ms), (qs, ns) = run(), run(missing=(0, 3))
+    assert not torch.equal(ps[0], ps[2]) and not torch.equal(ms[0], ms[2]) and not torch.equal(ms[1], ms[3])
+    assert torch.equal(ps[1], qs[1]) and torch.equal(ms[1], ns[1]) and torch.equal(ps[2], qs[2]) and torch.equal(ms[2], ns[2])

@@ -55,20 +55,18 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # a parameter's number over all groups: its random numbers do not depend on which others have a gradient
-        first, work, numbers = 0, [], {}
+        # with a number over all groups, so that its random numbers do not depend on which others have a gradient
+        first, work = 0, []
         for g in self.param_groups:
-            work.append((g, [p for p in g["params"] if p.grad is not None]))
-            if g["seed"] is not None:
-                numbers.update((id(p), first + i) for i, p in enumerate(g["params"]))
+            work.append((g, [(i, p) for i, p in enumerate(g["params"], first) if p.grad is not None]))
             first += len(g["params"])
         for _, params in work:
-            for p in params:
+            for _, p in params:
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
         norm = None
         if self.max_norm is not None:
-            grads = [p.grad for _, params in work for p in params]
+            grads = [p.grad for _, params in work for _, p in params]
             if grads:
                 norm = self.grad_norm = ops.grad_norm(grads)
         for group, params in work:
@@ -76,27 +74,29 @@ class AdamW(torch.optim.Optimizer):
             # where some of a count's parameters have no gradient this time, the others go on with a count of their own.
             counts: dict = {}
             fresh = None
-            for p in params:
+            for i, p in params:
                 st = self.state[p]
                 if not st:
                     if fresh is None or fresh.device != p.device:
                         fresh = torch.zeros((), dtype=torch.int64, device=p.device)
                     st.update(self._new_state(group, p, fresh))
-                counts.setdefault(id(st["step"]), (st["step"], []))[1].append(p)
+                _, together, numbers = counts.setdefault(id(st["step"]), (st["step"], [], []))
+                together.append(p)
+                numbers.append(i)
             if counts and len(params) < len(group["params"]):
-                present = set(map(id, params))
+                present = {id(p) for _, p in params}
                 for key in {id(self.state[p]["step"]) for p in group["params"] if id(p) not in present and self.state.get(p)} & counts.keys():
-                    step, together = counts[key]
+                    step, together, numbers = counts[key]
                     step = step.clone()
                     for p in together:
                         self.state[p]["step"] = step
-                    counts[key] = (step, together)
-            for step, together in counts.values():
+                    counts[key] = (step, together, numbers)
+            for step, together, numbers in counts.values():
                 states = [self.state[p] for p in together]
                 ops.adamw_step(together, [p.grad for p in together], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step,
                                lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_norm=norm,
                                max_norm=self.max_norm, scales=[s.get("scales") for s in states], seed=group["seed"],
-                               numbers=None if group["seed"] is None else [numbers[id(p)] for p in together])
+                               numbers=None if group["seed"] is None else numbers)
         return loss
 
     def load_state_dict(self, state_dict):

@@ -399,7 +399,7 @@ int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, cons
  *   g = factor * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  t = step + 1
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * factor: 1, or min(1, max_norm / (norm + 1e-6)) where norm != NULL and max_norm > 0.  Where norm != NULL and *norm is not finite
- * nothing changes, *step included.  *step (int64) becomes t.
+ * nothing changes, *step included.  *step (int64) becomes t.  eps: 0, or 2^-126 and more.
  * States: 32-bit (m, v fp32), or 8-bit where the tensor's entries of `m_exponents` and `v_exponents` are not NULL: m and v are codes, and
  * the entries hold ceil(count / 256) bytes each, the exponent of each block of 256 codes.  A code c of m stands for
  * (-1)^(c >> 7) * (E ? (1 + f / 8) 2^(E - 15) : f / 8 2^-14) with E = (c >> 3) & 15, f = c & 7, one of v for

@@ -166,9 +166,11 @@ __device__ __forceinline__ void decode_v(float2 (&v)[4], uint2 codes, float unit
     v[2 * h + 1] = fmul2(fmul2(make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), both_of(kUpV)), both_of(unit));
   }
 }
+template <bool SUBNORMAL>
 __device__ __forceinline__ float sqrt_near(float x) {
   float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  if constexpr (SUBNORMAL) asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));            // 0 below 2^-126
   return y;
 }
 __device__ __forceinline__ float rcp_near(float x) {
@@ -261,7 +263,7 @@ __device__ __forceinline__ void load_block(Lane<EIGHT>& l, const AdamTensor& x, 
   }
 }
 
-template <int W, bool EIGHT>
+template <int W, bool EIGHT, bool SUBNORMAL>
 __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommon& p, const AdamTensor& x, const AdamScalars& s, int64_t block, int lane) {
   const int64_t at = block * kAdamBlock + lane * 8;
   const int p_type = x.flags & 3, g_type = x.flags >> 2 & 3;
@@ -289,7 +291,7 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
     const float2 g = fmul2(make_float2(e[2 * k], e[2 * k + 1]), both_of(s.factor));
     m[k] = add_apart(fmul2(m[k], both_of(p.b1)), fmul2(g, both_of(p.c1)));
     v[k] = add_apart(fmul2(v[k], both_of(p.b2)), fmul2(fmul2(g, g), both_of(p.c2)));
-    const float2 root = ffma2(make_float2(sqrt_near(v[k].x), sqrt_near(v[k].y)), both_of(s.inv_root), both_of(p.eps));
+    const float2 root = ffma2(make_float2(sqrt_near<SUBNORMAL>(v[k].x), sqrt_near<SUBNORMAL>(v[k].y)), both_of(s.inv_root), both_of(p.eps));
     const float2 step = fmul2(m[k], make_float2(rcp_near(root.x), rcp_near(root.y)));
     w[k] = ffma2(w[k], both_of(s.decay), fmul2(step, both_of(-s.step_size)));
   }
@@ -366,30 +368,30 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
 // tensors, 8-bit states, 601 us = 6.0 TB/s; with 64 registers 629, with 48, which spill, a hundredth more than with 56), and a loop over several
 // blocks, with or without the next one on its way in registers, lost more of them than it gained.  CTAs of 128 leave an SM in smaller
 // parts than those of 256 (640 where those take 715).
-template <bool EIGHT>
+template <bool EIGHT, bool SUBNORMAL>
 __device__ __forceinline__ void run_block(const AdamCommon& p, const AdamTensor& x, int64_t block, int lane) {
   Lane<EIGHT> l;
   // whole blocks of tensors that begin at multiples of 16 bytes; what ends a tensor, and tensors that begin anywhere, element by element
   if ((x.flags & kAdamVector) && (block + 1) * kAdamBlock <= x.n) {
     load_block<8, EIGHT>(l, x, block, lane);
     const AdamScalars s = *p.scalars;
-    if (!s.skip) step_block<8, EIGHT>(l, p, x, s, block, lane);
+    if (!s.skip) step_block<8, EIGHT, SUBNORMAL>(l, p, x, s, block, lane);
   } else {
     load_block<1, EIGHT>(l, x, block, lane);
     const AdamScalars s = *p.scalars;
-    if (!s.skip) step_block<1, EIGHT>(l, p, x, s, block, lane);
+    if (!s.skip) step_block<1, EIGHT, SUBNORMAL>(l, p, x, s, block, lane);
   }
 }
 
-template <int MAX>
+template <int MAX, bool SUBNORMAL>
 __global__ void __launch_bounds__(kAdamThreads, 9) adamw_kernel(const __grid_constant__ AdamParams<MAX> p) {
   const AdamTensor& x = tensor_of(p.t, p.starts, blockIdx.x);
   const int64_t block = (blockIdx.x - x.first) * kAdamWarps + (threadIdx.x >> 5);
   griddep_wait();
   griddep_launch();
   if (block * kAdamBlock >= x.n) return;
-  if (x.flags & kAdamEight) run_block<true>(p.c, x, block, threadIdx.x & 31);
-  else run_block<false>(p.c, x, block, threadIdx.x & 31);
+  if (x.flags & kAdamEight) run_block<true, SUBNORMAL>(p.c, x, block, threadIdx.x & 31);
+  else run_block<false, SUBNORMAL>(p.c, x, block, threadIdx.x & 31);
 }
 
 // ---- the norm of the gradients: squares in 64 bits, where every one of them is exact ------------------------------------
@@ -570,6 +572,7 @@ extern "C" int s3r_adamw_step_numbered(const s3r_adamw* args, const uint32_t* nu
   S3R_REQUIRE(a.step && a.workspace && (a.n == 0 || (a.params && a.grads && a.m && a.v && a.counts && a.param_types && a.grad_types)), S3R_ERR_NULL,
               "s3r_adamw_step: NULL pointer");
   S3R_REQUIRE(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1 && a.eps >= 0, S3R_ERR_UNSUPPORTED, "s3r_adamw_step: betas are in [0, 1), eps is not negative");
+  S3R_REQUIRE(a.eps == 0 || a.eps >= 0x1p-126, S3R_ERR_UNSUPPORTED, "s3r_adamw_step: eps is 0 or a normal number of fp32, got %g", a.eps);
   S3R_REQUIRE(reinterpret_cast<uintptr_t>(a.step) % 8 == 0 && reinterpret_cast<uintptr_t>(a.workspace) % 8 == 0, S3R_ERR_ALIGNMENT, "s3r_adamw_step: elements must be aligned");
   for (int i = 0; i < a.n; ++i) {
     S3R_REQUIRE(a.counts[i] >= 0, S3R_ERR_SHAPE, "s3r_adamw_step: negative count");
@@ -599,6 +602,9 @@ extern "C" int s3r_adamw_step_numbered(const s3r_adamw* args, const uint32_t* nu
   if (a.seed < 0) p.c.seed = -1;
   p.c.scalars = scalars;
   p.c.n = 0;
+  // A v below 2^-126 has a root below 2^-63, times 1 / sqrt(1 - beta2) at most.  Where that is 2^-24 of eps and less it may be taken as 0 (the
+  // cheaper root: the other one costs 8-bit states 1 to 3 %); with a smaller eps it is what the step is divided by.
+  const bool subnormal = a.eps * sqrt(1.0 - a.beta2) < 0x1p-39;
   int64_t ctas = 0;
   for (int i = 0; i <= a.n; ++i) {
     if (p.c.n && (i == a.n || p.c.n == kAdamMax)) {
@@ -607,10 +613,10 @@ extern "C" int s3r_adamw_step_numbered(const s3r_adamw* args, const uint32_t* nu
         few.c = p.c;
         std::copy_n(p.t, p.c.n, few.t);
         fill_starts(few.starts, p.t, p.c.n, ctas);
-        rc = launch(adamw_kernel<kAdamFew>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
+        rc = launch(subnormal ? adamw_kernel<kAdamFew, true> : adamw_kernel<kAdamFew, false>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, few);
       } else {
         fill_starts(p.starts, p.t, p.c.n, ctas);
-        rc = launch(adamw_kernel<kAdamMax>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
+        rc = launch(subnormal ? adamw_kernel<kAdamMax, true> : adamw_kernel<kAdamMax, false>, static_cast<unsigned>(ctas), kAdamThreads, 0, st, p);
       }
       if (rc) return rc;
       p.c.n = 0;

@@ -372,8 +372,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: Tensor, lr=1e-3, betas=
         m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
         p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
 
-    ``step`` is a 0-dim int64 tensor on the device that becomes t; ``lr`` a number or a 0-dim fp32 tensor on the device.  Where
-    ``grad_norm`` is given and not finite, nothing changes.  States are fp32, or, where ``scales`` (a list, entries may be None) has a
+    ``step`` is a 0-dim int64 tensor on the device that becomes t; ``lr`` a number or a 0-dim fp32 tensor on the device.  ``eps`` is
+    0 or at least 2^-126.  Where ``grad_norm`` is given and not finite, nothing changes.  States are fp32, or, where ``scales`` (a list, entries may be None) has a
     uint8 ``[2, ceil(n / 256)]`` for a tensor, uint8 codes: see ``adamw_state``.  With ``seed`` (0 to 2^63 - 1) what is kept in fewer
     bits than 32 - 8-bit states, bf16 parameters - is rounded stochastically, the same way for the same seed and step; without it to
     nearest.  A tensor's random numbers go by its index in the lists, or by its entry in ``numbers`` (one integer below 2^24 per

@@ -281,3 +281,15 @@ def test_the_optimiser_numbers_its_parameters(monkeypatch):
     seen.clear()
     opt.step()
     assert [n for _, n in seen] == [None] * 5
+
+
+def test_an_eps_that_fp32_does_not_hold_is_refused(lib):
+    import ctypes as C
+    from test_block_ops_cpu import AdamArgs
+
+    buf = C.create_string_buffer(4096)
+    p = (C.addressof(buf) + 255) & ~255
+    a = AdamArgs(n=-1, step=p, lr_host=1e-3, beta1=0.9, beta2=0.999, workspace=p)
+    for eps, code in ((0.0, -1), (2.0 ** -126, -1), (1e-8, -1), (1e-38, -2), (1e-60, -2), (-1.0, -2), (float("nan"), -2)):
+        a.eps, a.n = eps, 0 if code == -2 else -1
+        assert lib.s3r_adamw_step(C.byref(a), None) == code, eps

@@ -268,3 +268,30 @@ def test_groups_round_by_themselves_and_a_missing_gradient_changes_nothing_else(
     (ps, ms), (qs, ns) = run(), run(missing=(0, 3))
     assert not torch.equal(ps[0], ps[2]) and not torch.equal(ms[0], ms[2]) and not torch.equal(ms[1], ms[3])
     assert torch.equal(ps[1], qs[1]) and torch.equal(ms[1], ns[1]) and torch.equal(ps[2], qs[2]) and torch.equal(ms[2], ns[2])
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-20, 1e-18, 1e-15, 1e-8])
+@pytest.mark.parametrize("eight", [False, True])
+def test_second_moments_below_the_normal_numbers(eight, eps):
+    """Gradients of 1e-19: v is a subnormal number, and its root is what the step is divided by where eps is no larger."""
+    from test_gpu_block_ops import values
+
+    n, b1, b2, lr = 5000, 0.9, 0.999, 1e-2
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    p = torch.randn(n, device=DEV, generator=gen)
+    zeros = lambda: torch.zeros(n, device=DEV, dtype=U8 if eight else torch.float32)
+    m, v, e, step = zeros(), zeros(), torch.full((2, -(-n // 256)), 27, device=DEV, dtype=U8), torch.zeros((), dtype=torch.int64, device=DEV)
+    for t in (1, 2):
+        g = (0.5 + 1.5 * torch.rand(n, device=DEV, generator=gen)) * 1e-19
+        m0, v0 = (values(m, e[0], 4), values(v, e[1], 5)) if eight else (m.double(), v.double())
+        p0, d = p.double(), g.double()
+        ops.adamw_step([p], [g], [m], [v], step, lr=lr, betas=(b1, b2), eps=eps, weight_decay=0.0, scales=[e] if eight else None)
+        m1, v1 = b1 * m0 + (1 - b1) * d, b2 * v0 + (1 - b2) * d * d
+        inv_root = 1 / math.sqrt(1 - b2 ** t)
+        root = torch.sqrt(v1) * inv_root + eps
+        moved = lr / (1 - b1 ** t) * m1 / root
+        # In fp32: b2 v and (1 - b2) g^2 are rounded to multiples of 2^-149, by half a one each, and the square by as little; their sum is
+        # exact.  That moves the root by half its share of v, which is within the share itself.  The rest: 2^-24, a few of them.
+        share = 2.0 ** -149 * 1.01 / v1
+        close = moved.abs() * (40 * 2.0 ** -24 + share) + 8 * 2.0 ** -24 * p0.abs()
+        assert p.isfinite().all() and ((p.double() - (p0 - moved)).abs() <= close).all(), (t, eps)

@@ -405,7 +405,8 @@ int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, cons
  * (-1)^(c >> 7) * (E ? (1 + f / 8) 2^(E - 15) : f / 8 2^-14) with E = (c >> 3) & 15, f = c & 7, one of v for
  * E ? (1 + f / 8) 2^(E - 31) : f / 8 2^-30 with E = c >> 3; both times 2^(exponent - 127), exponent 255: NaN.
  * seed < 0: what is kept in fewer than 32 bits is rounded to nearest even, else stochastically with Philox 2x32-7, counter (pair of
- * elements, t), key (seed mod 2^32) + (seed >> 32) * 0xC2B2AE35 + number of the tensor * 0x85EBCA6B (mod 2^32).
+ * elements, t), key (seed mod 2^32) + (seed >> 32) * 0xC2B2AE35 + number of the tensor * 0x85EBCA6B (mod 2^32): of the
+ * element's 32 bits the lowest 8 round m, the next 14 v, and the upper 16 a bf16 parameter, all that it drops.  fp16: to nearest even.
  * Arrays are HOST arrays; lr: a device pointer that is read on the stream, or NULL for lr_host. */
 typedef struct {
   int n;

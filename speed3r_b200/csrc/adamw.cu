@@ -304,12 +304,14 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
       low[k] = r.x;
       low[k + 1] = r.y;
     }
-    // 10 bits of a bf16 parameter's 16; fp16's values below 2^-14 have fewer, so it is rounded to nearest
+    // All 16 bits that a bf16 parameter drops, so that an update of any size happens as often as it should; the lower 6 of them are the upper 6
+    // of those that round v, of which a parameter's rounding hardly ever depends.  fp16's values below 2^-14 have fewer, so it is rounded to
+    // nearest.
     if (p_type == S3R_BF16)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (fabsf(w[k].x) < 3.3e38f) w[k].x = __uint_as_float((__float_as_uint(w[k].x) + (low[2 * k] >> 22) * 64u + 32u) & 0xffff0000u);
-        if (fabsf(w[k].y) < 3.3e38f) w[k].y = __uint_as_float((__float_as_uint(w[k].y) + (low[2 * k + 1] >> 22) * 64u + 32u) & 0xffff0000u);
+        if (fabsf(w[k].x) < 3.3e38f) w[k].x = __uint_as_float((__float_as_uint(w[k].x) + (low[2 * k] >> 16)) & 0xffff0000u);
+        if (fabsf(w[k].y) < 3.3e38f) w[k].y = __uint_as_float((__float_as_uint(w[k].y) + (low[2 * k + 1] >> 16)) & 0xffff0000u);
       }
   }
   store_lane<W>(w, x.p, p_type, at, x.n);

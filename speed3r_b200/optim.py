@@ -19,7 +19,8 @@ class AdamW(torch.optim.Optimizer):
     ``max_norm``: gradients are scaled by ``min(1, max_norm / (norm + 1e-6))``, norm taken over all parameters; a step whose norm is
     not finite is left out.  ``state_bits=8``: tensors of at least ``min_8bit_size`` elements keep their moments in 8 bits
     (``ops.adamw_state`` says what the codes stand for), rounded stochastically with ``seed``; ``seed=None`` rounds to nearest, with
-    which a second moment hardly follows gradients that shrink.  bf16 parameters are rounded the same way.  ``lr`` may be a 0-dim
+    which a second moment hardly follows gradients that shrink.  bf16 parameters are rounded the same way, by all bits that they
+    drop; fp16 parameters to nearest.  ``lr`` may be a 0-dim
     fp32 tensor on the device, which a captured step reads anew each time.
 
     Parameters are counted from the first step in which they had a gradient, as PyTorch does."""

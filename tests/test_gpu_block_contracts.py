@@ -295,3 +295,36 @@ def test_second_moments_below_the_normal_numbers(eight, eps):
         share = 2.0 ** -149 * 1.01 / v1
         close = moved.abs() * (40 * 2.0 ** -24 + share) + 8 * 2.0 ** -24 * p0.abs()
         assert p.isfinite().all() and ((p.double() - (p0 - moved)).abs() <= close).all(), (t, eps)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_bf16_parameters_are_rounded_by_all_bits_that_they_drop(eight):
+    """Against the same step of fp32 parameters, rounded here."""
+    from test_gpu_block_ops import philox
+
+    n, seed = 100_003, 21
+    p, g, m, v, e, step = state([(n,)], (eight,), seed=6, dtype=torch.bfloat16)
+    wide, m2, v2, e2, step2 = [p[0].float()], [m[0].clone()], [v[0].clone()], [e[0].clone() if eight else None], step.clone()
+    ops.adamw_step(wide, g, m2, v2, step2, lr=1e-2, scales=e2)
+    ops.adamw_step(p, g, m, v, step, lr=1e-2, scales=e, seed=seed)
+    pair = torch.arange((n + 1) // 2, device=DEV)
+    low = philox(pair, step.expand(pair.shape), seed)[:n]
+    want = ((wide[0].view(torch.int32).long() & 0xFFFFFFFF) + (low >> 16)) >> 16
+    assert torch.equal(p[0].view(torch.int16).long() & 0xFFFF, want)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_updates_far_below_a_bf16_step_happen_on_average(eight, sign):
+    """An update of a 8192nd of a step moves one parameter in 8192."""
+    n = 1 << 22
+    p, g = torch.full((n,), 1.5, device=DEV).bfloat16(), torch.full((n,), sign, device=DEV).bfloat16()
+    zeros = lambda: torch.zeros(n, device=DEV, dtype=U8 if eight else torch.float32)
+    e = [torch.full((2, n // 256), 27, device=DEV, dtype=U8)] if eight else None
+    # the first step is lr in size whatever the gradient
+    ops.adamw_step([p], [g], [zeros()], [zeros()], torch.zeros((), dtype=torch.int64, device=DEV), lr=2.0 ** -20, eps=0.0, weight_decay=0.0, scales=e, seed=9)
+    step = p.float() - 1.5
+    moved = int((step != 0).sum())
+    assert ((step == 0) | (step == -sign * 2.0 ** -7)).all()
+    # binomial: 512 expected, 22.6 its deviation
+    assert abs(moved - n / 8192) <= 6 * math.sqrt(n / 8192)

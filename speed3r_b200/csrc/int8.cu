@@ -682,8 +682,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) int8_few_kernel(const __grid_c
     for (int m = 0; m < M; ++m) {
       const int total = __reduce_add_sync(0xffffffffu, sum[i][m]);
       if (lane == i * M + m && m < p.M && n0 + i < p.N) {
-        const float y = __fmul_rn(__fmul_rn(__int2float_rn(total), __ldg(p.a_scale + m)), __ldg(p.b_scale + n0 + i));
-        const float v[1] = {p.bias ? __fadd_rn(y, __ldg(p.bias + n0 + i)) : y};
+        // the larger kernel's operations, so that a token's results do not depend on how many it comes with
+        const float v[1] = {__fmaf_rn(__fmul_rn(__int2float_rn(total), __ldg(p.a_scale + m)), __ldg(p.b_scale + n0 + i), p.bias ? __ldg(p.bias + n0 + i) : 0.f)};
         Raw<1> o;
         pack<1>(o, v, p.type);
         store_raw<1>(o, p.out, p.type, static_cast<int64_t>(m) * p.N + n0 + i);

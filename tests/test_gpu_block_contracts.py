@@ -328,3 +328,18 @@ def test_updates_far_below_a_bf16_step_happen_on_average(eight, sign):
     assert ((step == 0) | (step == -sign * 2.0 ** -7)).all()
     # binomial: 512 expected, 22.6 its deviation
     assert abs(moved - n / 8192) <= 6 * math.sqrt(n / 8192)
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N, K", [(1000, 1024), (257, 500)])
+def test_a_token_has_the_same_results_in_every_batch(N, K, dtype, bias):
+    """Whichever kernel and tile computes them: bit for bit."""
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    q, w = (torch.randint(-127, 128, s, device=DEV, dtype=torch.int8, generator=gen) for s in ((9000, K), (N, K)))
+    s, ws = (torch.rand(n, device=DEV, generator=gen) + 0.1 for n in (9000, N))
+    ws *= 0.01
+    b = torch.randn(N, device=DEV, generator=gen) if bias else None
+    whole = ops.int8_linear(q, s, w, ws, b, dtype)
+    for M in (1, 2, 3, 4, 5, 8, 9, 64, 129, 700):
+        assert torch.equal(ops.int8_linear(q[:M], s[:M], w, ws, b, dtype), whole[:M]), M

@@ -375,7 +375,7 @@ size_t s3r_residual_norm_bwd_workspace_bytes(int64_t batch, int64_t tokens, int 
 int s3r_residual_norm_bwd(const s3r_residual_norm* f_host, const s3r_residual_norm_grad* g_host, void* stream);
 
 /* q[r, c] = x[r, c] * (127 * (1 / max |x[r]|)) to nearest even, scale[r] = max |x[r]| / 127.  x: rows of x_pitch elements of `type`,
- * q: rows of q_pitch bytes; NaN in a row makes its scale NaN, rows whose largest
+ * q: rows of q_pitch bytes; at most 2^31 - 8193 channels; NaN in a row makes its scale NaN, rows whose largest
  * magnitude is below 2^-119 are zeros. */
 int s3r_quantize_rows(const void* x, int type, int64_t x_pitch, int8_t* q, int64_t q_pitch, float* scale, int64_t rows, int channels,
                       void* stream);

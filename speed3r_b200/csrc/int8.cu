@@ -2,6 +2,7 @@
 //   quantise  scale[r] = max |x[r]| / 127, q = x / scale to nearest even.  Bound: HBM, a row is read once and kept in registers.
 //   product   out[m, n] = (sum_k a[m, k] b[n, k]) a_scale[m] b_scale[n] + bias[n].  The sums are exact (32-bit integers), so that
 //             no order of the k-steps changes a result.
+#include <climits>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -708,6 +709,8 @@ extern "C" int s3r_quantize_rows(const void* x, int type, int64_t x_pitch, int8_
   S3R_REQUIRE(rows > 0 && channels > 0 && x_pitch >= channels && q_pitch >= channels, S3R_ERR_SHAPE, "s3r_quantize_rows: sizes must be positive, pitches no shorter than rows");
   S3R_REQUIRE(known_type(type), S3R_ERR_UNSUPPORTED, "s3r_quantize_rows: types are fp32, bf16 and fp16");
   S3R_REQUIRE(rows < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_quantize_rows: too many rows");
+  // a thread's next column, up to 1024 x 8 behind the last one, is an int too
+  S3R_REQUIRE(channels <= INT_MAX - 8192, S3R_ERR_TOO_LARGE, "s3r_quantize_rows: %d channels (at most 2^31 - 8193)", channels);
   S3R_REQUIRE(reinterpret_cast<uintptr_t>(x) % type_bytes(type) == 0 && reinterpret_cast<uintptr_t>(scale) % 4 == 0, S3R_ERR_ALIGNMENT, "s3r_quantize_rows: elements must be aligned");
   const void* ptr[] = {x};
   int w = row_vector(channels, ptr, &type, 1);

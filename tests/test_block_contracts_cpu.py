@@ -293,3 +293,10 @@ def test_an_eps_that_fp32_does_not_hold_is_refused(lib):
     for eps, code in ((0.0, -1), (2.0 ** -126, -1), (1e-8, -1), (1e-38, -2), (1e-60, -2), (-1.0, -2), (float("nan"), -2)):
         a.eps, a.n = eps, 0 if code == -2 else -1
         assert lib.s3r_adamw_step(C.byref(a), None) == code, eps
+
+
+def test_rows_whose_columns_an_int_does_not_reach_are_refused(lib):
+    """The last column's successor in a thread's walk has to be a column number too."""
+    p = 1 << 12
+    rc = lambda channels: lib.s3r_quantize_rows(p, 0, 1 << 31, p, 1 << 31, p, 1, channels, None)
+    assert rc(2 ** 31 - 1) == -6 and rc(2 ** 31 - 8192) == -6

@@ -369,7 +369,8 @@ typedef struct {
   float* d_gate_row;
   void* d_gate_channel;
   void* workspace;
-  size_t workspace_bytes;  /* at least s3r_residual_norm_bwd_workspace_bytes */
+  size_t workspace_bytes;  /* at least s3r_residual_norm_bwd_workspace_bytes; a sixth of it for each of the six sums over rows (d_weight to
+                              d_post_bias, d_gate_channel) that is wanted is enough, and none at all where none is */
 } s3r_residual_norm_grad;
 size_t s3r_residual_norm_bwd_workspace_bytes(int64_t batch, int64_t tokens, int channels, int gate_mode);
 int s3r_residual_norm_bwd(const s3r_residual_norm* f_host, const s3r_residual_norm_grad* g_host, void* stream);

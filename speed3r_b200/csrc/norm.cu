@@ -376,7 +376,9 @@ struct NormBwdParams {
   uint32_t stage_bytes;
   uint32_t at_y, at_dr, at_dh; // of a stage, behind r
   float inv_n;
-  float* partial;              // [batch entries x slices, kSums, channels], the sums that are wanted
+  int sums;                    // that are wanted, and the place of each among them
+  int place[kSums];
+  float* partial;              // [batch entries x slices, sums, channels]
 };
 
 // CTAs per SM: 128 registers per thread, in a FULL backward 168.  The grid has as many as are resident: with a second, shorter round of CTAs
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(cta_threads(G), bwd_resident(G, FULL)) norm_bw
   }
 
   // this CTA's sums over rows; groups of one CTA are added in order
-  float* out = p.partial + static_cast<int64_t>(blockIdx.x) * kSums * C;
+  float* out = p.partial + static_cast<int64_t>(blockIdx.x) * p.sums * C;
   auto leave = [&](const float2* sums, int which, bool wanted) {
     if (!wanted) return;
     if constexpr (kRows > 1) {
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(cta_threads(G), bwd_resident(G, FULL)) norm_bw
     for (int i = 0; i < N; ++i)
       if (in(i))
 #pragma unroll
-        for (int k = 0; k < W; ++k) out[static_cast<int64_t>(which) * C + (i * G + t) * W + k] = e[i * W + k];
+        for (int k = 0; k < W; ++k) out[p.place[which] * C + (i * G + t) * W + k] = e[i * W + k];
   };
   if constexpr (W > 1) cp_async_wait<0>();
   leave(d_w, kSumWeight, g.d_weight != nullptr);
@@ -658,7 +660,7 @@ struct NormSumsParams {
   const float* partial;
   void* out[kSums + 1];
   int n, channels, slices, entries;    // entries: batch entries of the gate (its slices are summed apart)
-  int which[kSums + 1];
+  int sums, place[kSums + 1];          // of a slice; the gate's place stands last
   int type, gate_type;
 };
 
@@ -671,13 +673,13 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__
   const int64_t job = blockIdx.x / columns;
   const int c = static_cast<int>(blockIdx.x % columns) * 32 + lane;
   const bool gate = job >= p.n;
-  const int which = gate ? kSumGate : p.which[job];
+  const int place = p.place[gate ? p.n : job];
   const int64_t entry = gate ? job - p.n : 0;
   const int64_t first = gate ? entry * p.slices : 0, last = gate ? first + p.slices : static_cast<int64_t>(p.entries) * p.slices;
   float s = 0.f;
   if (c < p.channels)
 #pragma unroll 8
-    for (int64_t i = first + warp; i < last; i += 32) s += __ldg(p.partial + (i * kSums + which) * p.channels + c);
+    for (int64_t i = first + warp; i < last; i += 32) s += __ldg(p.partial + (i * p.sums + place) * p.channels + c);
   red[warp][lane] = s;
   __syncthreads();
   // a warp sums a column (lane: a warp's part), in a tree: the same order every time
@@ -869,8 +871,10 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   bwd_shape(f.channels, f.x_type == S3R_F32 && f.channels % 256 == 0, &G, &E);
   const bool full = f.post || per_entry;
   p.slices = bwd_slices(entries, p.span, G, full);
-  const bool sums = g.d_weight || g.d_bias || g.d_scale || g.d_post_weight || g.d_post_bias || g.d_gate_channel;
-  const size_t need = s3r_residual_norm_bwd_workspace_bytes(f.batch, f.tokens, f.channels, f.gate_mode);
+  void* const out[kSums] = {g.d_weight, g.d_bias, g.d_scale, g.d_post_weight, g.d_post_bias, g.d_gate_channel};
+  for (int i = 0; i < kSums; ++i) p.place[i] = out[i] ? p.sums++ : 0;
+  const bool sums = p.sums > 0;
+  const size_t need = s3r_residual_norm_bwd_workspace_bytes(f.batch, f.tokens, f.channels, f.gate_mode) / kSums * p.sums;
   S3R_REQUIRE(!sums || (g.workspace && g.workspace_bytes >= need && reinterpret_cast<uintptr_t>(g.workspace) % 4 == 0), S3R_ERR_TOO_LARGE,
               "s3r_residual_norm_bwd: workspace of %zu bytes is smaller than the %zu needed", g.workspace ? g.workspace_bytes : 0, need);
   p.partial = static_cast<float*>(g.workspace);
@@ -900,9 +904,10 @@ extern "C" int s3r_residual_norm_bwd(const s3r_residual_norm* f_, const s3r_resi
   s.entries = static_cast<int>(entries);
   s.type = f.param_type;
   s.gate_type = f.gate_type;
-  void* out[] = {g.d_weight, g.d_bias, g.d_scale, g.d_post_weight, g.d_post_bias};
-  for (int i = 0; i < 5; ++i)
-    if (out[i]) s.which[s.n] = i, s.out[s.n++] = out[i];
+  s.sums = p.sums;
+  for (int i = 0; i < kSumGate; ++i)
+    if (out[i]) s.place[s.n] = p.place[i], s.out[s.n++] = out[i];
+  s.place[s.n] = p.place[kSumGate];
   s.out[s.n] = g.d_gate_channel;
   const int64_t jobs = s.n + (g.d_gate_channel ? entries : 0), blocks = jobs * ((f.channels + 31) / 32);
   S3R_REQUIRE(blocks < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_residual_norm_bwd: grid too large");

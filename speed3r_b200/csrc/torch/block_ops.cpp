@@ -190,9 +190,14 @@ std::vector<Tensor> run_norm_bwd(const Tensor& r, const optional<Tensor>& y, con
     g.d_scale = pointer(ds);
     g.d_post_weight = pointer(dpw);
     g.d_post_bias = pointer(dpb);
-    g.workspace_bytes = s3r_residual_norm_bwd_workspace_bytes(f.batch, f.tokens, f.channels, f.gate_mode);
-    const Tensor ws = fresh({static_cast<int64_t>(g.workspace_bytes)}, r, at::kByte);
-    g.workspace = ws.data_ptr();
+    int sums = 0;
+    for (const Tensor* t : {&dw, &db, &ds, &dpw, &dpb, &dg}) sums += t->defined();
+    Tensor ws;
+    if (sums) {
+      g.workspace_bytes = s3r_residual_norm_bwd_workspace_bytes(f.batch, f.tokens, f.channels, f.gate_mode) / 6 * sums;
+      ws = fresh({static_cast<int64_t>(g.workspace_bytes)}, r, at::kByte);
+      g.workspace = ws.data_ptr();
+    }
     check(s3r_residual_norm_bwd(&f, &g, stream()), "s3r_residual_norm_bwd");
   }
   if (dg_row.defined()) dg = (gate->size(1) == 1 ? dg_row.sum(1, true) : dg_row).to(gate->scalar_type());

@@ -300,3 +300,32 @@ def test_rows_whose_columns_an_int_does_not_reach_are_refused(lib):
     p = 1 << 12
     rc = lambda channels: lib.s3r_quantize_rows(p, 0, 1 << 31, p, 1 << 31, p, 1, channels, None)
     assert rc(2 ** 31 - 1) == -6 and rc(2 ** 31 - 8192) == -6
+
+
+def norm_backward_args(p, wanted, **kw):
+    """Arguments of a backward whose tensors all lie at `p`, with the named sums wanted."""
+    import ctypes as C
+    from test_block_ops_cpu import NormArgs
+
+    class Grad(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("dr", "dh", "dx", "dy", "d_weight", "d_bias", "d_scale", "d_post_weight", "d_post_bias", "d_gate_row", "d_gate_channel",
+                                              "workspace")] + [("workspace_bytes", C.c_size_t)]
+
+    f = NormArgs(batch=3, tokens=50, channels=64, post=1, x=p, y=p, r=p, stats=p, weight=p, bias=p, scale=p, post_weight=p, post_bias=p, gate=p, gate_mode=2,
+                 gate_stride_b=64)
+    for k, v in kw.items():
+        setattr(f, k, v)
+    return f, Grad(dr=p, dh=p, dx=p, workspace=p, **{n: p for n in wanted})
+
+
+SUMS = ("d_weight", "d_bias", "d_scale", "d_post_weight", "d_post_bias", "d_gate_channel")
+
+
+@pytest.mark.parametrize("count", range(1, 7))
+def test_a_workspace_that_is_too_small_for_the_sums_is_refused(lib, count):
+    import ctypes as C
+    f, g = norm_backward_args(1 << 12, SUMS[:count])
+    whole = lib.s3r_residual_norm_bwd_workspace_bytes(3, 50, 64, 2)
+    assert whole > 0 and whole % 6 == 0
+    g.workspace_bytes = whole // 6 * count - 1
+    assert lib.s3r_residual_norm_bwd(C.byref(f), C.byref(g), None) == -6

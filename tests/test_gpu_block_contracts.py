@@ -343,3 +343,59 @@ def test_a_token_has_the_same_results_in_every_batch(N, K, dtype, bias):
     whole = ops.int8_linear(q, s, w, ws, b, dtype)
     for M in (1, 2, 3, 4, 5, 8, 9, 64, 129, 700):
         assert torch.equal(ops.int8_linear(q[:M], s[:M], w, ws, b, dtype), whole[:M]), M
+
+
+# ---- norms -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [(3, 50), (40, 1), (2, 5000)])
+@pytest.mark.parametrize("wanted", [("d_weight",), ("d_bias", "d_gate_channel"), ("d_scale", "d_post_weight", "d_post_bias"), ("d_gate_channel",),
+                                    ("d_weight", "d_bias", "d_scale", "d_post_weight", "d_post_bias", "d_gate_channel")])
+def test_sums_that_are_wanted_need_their_own_workspace_and_no_more(rows, wanted):
+    """Through the library's C entry, with just the workspace that the header asks for: the same sums, nothing behind it written."""
+    import ctypes as C
+    from speed3r_b200 import _lib
+    from test_block_contracts_cpu import SUMS, norm_backward_args
+
+    B, T, Ch = *rows, 64
+    gen = torch.Generator(device=DEV).manual_seed(B)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+    t = {n: rand(B * T, Ch) for n in ("r", "y", "dr", "dh", "dx")}
+    t |= {n: rand(Ch) for n in ("weight", "bias", "scale", "post_weight", "post_bias")} | dict(gate=rand(B, Ch), stats=rand(4, B * T))
+    lib = _lib.load()
+    whole = lib.s3r_residual_norm_bwd_workspace_bytes(B, T, Ch, 2)
+
+    def sums(names):
+        need = whole // 6 * len(names)
+        space = torch.full((need + 4096,), 7, dtype=U8, device=DEV)
+        out = {n: torch.zeros(B, Ch, device=DEV) if n == "d_gate_channel" else torch.zeros(Ch, device=DEV) for n in names}
+        f, g = norm_backward_args(0, (), batch=B, tokens=T, **{n: t[n].data_ptr() for n in ("r", "y", "weight", "bias", "scale", "post_weight", "post_bias", "gate", "stats")},
+                                  x=t["r"].data_ptr())
+        g.dr, g.dh, g.dx, g.workspace, g.workspace_bytes = (*(t[n].data_ptr() for n in ("dr", "dh", "dx")), space.data_ptr(), need)
+        for n, o in out.items():
+            setattr(g, n, o.data_ptr())
+        assert lib.s3r_residual_norm_bwd(C.byref(f), C.byref(g), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert (space[need:] == 7).all()
+        return out
+
+    every = sums(SUMS)
+    assert all(o.isfinite().all() and (o != 0).any() for o in every.values())
+    got = sums(wanted)
+    assert all(torch.equal(got[n], every[n]) for n in wanted)
+
+
+@pytest.mark.parametrize("learn", [(), ("gate",)])
+def test_backward_takes_no_memory_for_sums_that_nobody_wants(learn):
+    B, Ch = 8192, 1024
+    x, y = (torch.randn(B, 1, Ch, device=DEV).requires_grad_(True) for _ in range(2))
+    gate = torch.randn(B, 1, Ch, device=DEV).requires_grad_("gate" in learn)
+    r, h = ops.residual_norm(x, y, (torch.ones(Ch, device=DEV), None, 1e-5), gate=gate)
+    leaves = [x, y] + [gate] * len(learn)
+    grads = [torch.ones_like(t) for t in (r, h)]
+    one = B * Ch * 4
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    torch.autograd.grad((r, h), leaves, grads)
+    torch.cuda.synchronize()
+    # dx and dy; with the gate its gradient, and a sum per entry of it
+    assert torch.cuda.max_memory_allocated() - before <= (2 + 2 * len(learn)) * one + (8 << 20)

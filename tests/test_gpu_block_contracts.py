@@ -399,3 +399,42 @@ def test_backward_takes_no_memory_for_sums_that_nobody_wants(learn):
     torch.cuda.synchronize()
     # dx and dy; with the gate its gradient, and a sum per entry of it
     assert torch.cuda.max_memory_allocated() - before <= (2 + 2 * len(learn)) * one + (8 << 20)
+
+
+def saved_by(call):
+    """Addresses of the tensors that autograd keeps of a call."""
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.data_ptr()) or t, lambda t: t):
+        out = call()
+    return set(kept), out
+
+
+@pytest.mark.parametrize("learn", ["", "scale", "gate", "post"])
+def test_the_branch_is_kept_where_it_is_needed_and_only_there(learn):
+    x, y = (torch.randn(2, 33, 256, device=DEV).to(t).requires_grad_(True) for t in (torch.float32, torch.bfloat16))
+    w, scale, gate = (torch.randn(s, device=DEV).requires_grad_(n == learn) for n, s in (("w", 256), ("scale", 256), ("gate", (2, 33, 1))))
+    kept, (r, h) = saved_by(lambda: ops.residual_norm(x, y, (w, None, 1e-5), scale, gate, (None, None, 1e-5) if learn == "post" else None))
+    assert (y.data_ptr() in kept) == bool(learn)
+    assert r.data_ptr() in kept and x.data_ptr() not in kept and h.data_ptr() not in kept
+
+
+@pytest.mark.parametrize("C, rows", [(64, 9500), (100, 9473), (132, 9999), (256, 9472), (320, 5000), (1024, 2371), (2056, 601), (3000, 592), (4096, 777)])
+@pytest.mark.parametrize("kw", [dict(kind="rms"), dict(gate="channel"), dict(gate="channel", kind="rms", post=True), dict(branch=False), dict(branch=False, kind="rms"),
+                                dict(half=True), dict(half=True, gate="token", post=True), dict(norm=False)], ids=str)
+def test_norms_of_many_rows(C, rows, kw):
+    """As many as the kernel whose CTAs stay is for (four rows and more for each group that is resident), in every form."""
+    from test_gpu_block_ops import Norm
+
+    kw = dict(kw)
+    gate = {None: None, "channel": (2, 1, C), "token": (2, -(-rows // 2), 1)}[kw.pop("gate", None)]
+    types = dict.fromkeys("xyhw", torch.float16) if kw.pop("half", False) else {}
+    n = Norm((2, -(-rows // 2), C), gate=gate, seed=C, **types, **kw)
+    n.train()
+    if not kw.get("norm", True):
+        return
+    n.h_type = torch.float32
+    with torch.no_grad():
+        r, h = n.call()
+        r8, q, s = ops.residual_norm_int8(n.x, n.y, n.norm, n.scale, n.gate, n.post, n.kind)
+        q2, s2 = ops.quantize_tokens(h)
+    assert torch.equal(r8, r) and torch.equal(q, q2) and torch.equal(s, s2)

@@ -42,6 +42,12 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = max_norm
         self.grad_norm: Optional[Tensor] = None       # of the last step with max_norm, 0-dim on the device
 
+    @staticmethod
+    def _outside_of_a_graph(what: str) -> None:
+        """What makes states once would make them anew in every replay."""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"AdamW: {what} cannot be captured: take a step with the same gradients outside of the graph first")
+
     def _new_state(self, group, p, step):
         if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:
             codes = lambda: torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
@@ -78,6 +84,7 @@ class AdamW(torch.optim.Optimizer):
             for i, p in params:
                 st = self.state[p]
                 if not st:
+                    self._outside_of_a_graph("a parameter's first step")
                     if fresh is None or fresh.device != p.device:
                         fresh = torch.zeros((), dtype=torch.int64, device=p.device)
                     st.update(self._new_state(group, p, fresh))
@@ -87,6 +94,7 @@ class AdamW(torch.optim.Optimizer):
             if counts and len(params) < len(group["params"]):
                 present = {id(p) for _, p in params}
                 for key in {id(self.state[p]["step"]) for p in group["params"] if id(p) not in present and self.state.get(p)} & counts.keys():
+                    self._outside_of_a_graph("a step from which a parameter is left out for the first time")
                     step, together, numbers = counts[key]
                     step = step.clone()
                     for p in together:

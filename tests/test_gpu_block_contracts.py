@@ -438,3 +438,32 @@ def test_norms_of_many_rows(C, rows, kw):
         r8, q, s = ops.residual_norm_int8(n.x, n.y, n.norm, n.scale, n.gate, n.post, n.kind)
         q2, s2 = ops.quantize_tokens(h)
     assert torch.equal(r8, r) and torch.equal(q, q2) and torch.equal(s, s2)
+
+
+def test_a_step_that_makes_states_is_not_captured():
+    """Its replays would begin anew each time."""
+    from speed3r_b200 import AdamW
+
+    def captured(opt):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        return graph
+
+    ps = [torch.nn.Parameter(torch.ones(300, device=DEV)) for _ in range(2)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = AdamW(ps, lr=0.1)
+    with pytest.raises(RuntimeError, match="first step cannot be captured"):
+        captured(opt)
+    opt = AdamW(ps, lr=0.1)
+    opt.step()
+    grad, ps[1].grad = ps[1].grad, None
+    with pytest.raises(RuntimeError, match="left out for the first time"):
+        captured(opt)
+    opt.step()                                          # outside of the graph it is taken
+    captured(opt).replay()
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 1]
+    ps[1].grad = grad
+    captured(opt).replay()
+    assert [int(opt.state[p]["step"]) for p in ps] == [4, 2]

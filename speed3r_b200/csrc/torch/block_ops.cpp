@@ -529,14 +529,19 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
     g_types[i] = type_of(grads[i], "a gradient");
   }
   TORCH_CHECK(scale_of == scales.size(), "adamw: scales for a state that is not in 8 bits");
-  // a parameter that is listed twice would be updated by two warps at once
-  for (const auto* list : {&p, &m, &v}) {
-    std::vector<void*> sorted;
+  // memory that is listed twice, as a whole or in part, would be updated by two warps at once
+  std::vector<std::pair<const char*, const char*>> ranges;
+  auto apart = [&](const auto& list, auto&& bytes) {
+    ranges.clear();
     for (size_t i = 0; i < n; ++i)
-      if (counts[i]) sorted.push_back((*list)[i]);
-    std::sort(sorted.begin(), sorted.end());
-    TORCH_CHECK(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(), "adamw: a parameter or state is listed twice");
-  }
+      if (counts[i] && list[i]) ranges.emplace_back(reinterpret_cast<const char*>(list[i]), reinterpret_cast<const char*>(list[i]) + bytes(i));
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+      TORCH_CHECK(ranges[i - 1].second <= ranges[i].first, "adamw: a parameter or state is listed twice, as a whole or in part");
+  };
+  apart(p, [&](size_t i) { return counts[i] * params[i].element_size(); });
+  for (const auto* list : {&m, &v}) apart(*list, [&](size_t i) { return counts[i] * exp_avg[i].element_size(); });
+  for (const auto* list : {&me, &ve}) apart(*list, [&](size_t i) { return (counts[i] + 255) / 256; });
   c10::cuda::CUDAGuard guard(device);
   const Tensor ws = fresh({256}, params[0], at::kByte);
   s3r_adamw a = {};

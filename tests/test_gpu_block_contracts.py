@@ -467,3 +467,24 @@ def test_a_step_that_makes_states_is_not_captured():
     ps[1].grad = grad
     captured(opt).replay()
     assert [int(opt.state[p]["step"]) for p in ps] == [4, 2]
+
+
+@pytest.mark.parametrize("what", ["params", "exp_avg", "exp_avg_sq", "scales", "scales of m and v"])
+def test_memory_that_is_listed_twice_in_part_is_refused(what):
+    p, g, m, v, e, step = state([(512,), (512,)], (True, True))
+    flat = torch.zeros(4096, device=DEV)
+    if what == "params":
+        p = [flat[:512], flat[511:1023]]
+    elif what == "scales":
+        e = [e[0], e[0]]
+    elif what == "scales of m and v":
+        whole = torch.zeros(2, 4, device=DEV, dtype=U8)
+        e = [whole[:, :2], whole[:, 1:3]]
+    else:
+        codes = flat.view(U8)
+        (m if what == "exp_avg" else v)[:] = [codes[:512], codes[100:612]]
+    with pytest.raises(RuntimeError, match="listed twice"):
+        ops.adamw_step(p, g, m, v, step, scales=e)
+    assert int(step) == 3
+    if what == "params":                                 # side by side they may lie
+        ops.adamw_step([flat[:512], flat[512:1024]], g, m, v, step, scales=e)

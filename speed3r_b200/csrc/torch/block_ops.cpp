@@ -462,12 +462,12 @@ Tensor norm_of(at::TensorList tensors) {
   return norm;
 }
 
-void need_states(const Tensor& p, const Tensor& m, const Tensor& v, const optional<Tensor>& e) {
-  const at::ScalarType type = e.has_value() ? at::kByte : at::kFloat;
+void need_states(const Tensor& p, const Tensor& m, const Tensor& v, const Tensor* e) {
+  const at::ScalarType type = e ? at::kByte : at::kFloat;
   for (const Tensor* t : {&m, &v})
     TORCH_CHECK(t->device() == p.device() && t->scalar_type() == type && t->sizes() == p.sizes() && t->is_contiguous(),
                 "adamw: a state must be contiguous ", type, " of its parameter's shape ", p.sizes(), ", got ", t->scalar_type(), " ", t->sizes());
-  if (e.has_value())
+  if (e)
     TORCH_CHECK(e->device() == p.device() && e->scalar_type() == at::kByte && e->dim() == 2 && e->size(0) == 2 && e->size(1) == (p.numel() + 255) / 256 &&
                     (e->numel() == 0 || e->stride(1) == 1), "adamw: scales of ", p.numel(), " elements must be uint8 [2, ", (p.numel() + 255) / 256, "], got ", e->sizes());
 }
@@ -509,13 +509,13 @@ void adamw_update(at::TensorList params, at::TensorList grads, at::TensorList ex
     TORCH_CHECK(params[i].device() == device && grads[i].device() == device, "adamw: tensors of one device");
     TORCH_CHECK(params[i].is_contiguous(), "adamw: parameters must be contiguous");
     TORCH_CHECK(grads[i].sizes() == params[i].sizes(), "adamw: gradient ", grads[i].sizes(), " of parameter ", params[i].sizes());
-    optional<Tensor> scale;
+    const Tensor* scale = nullptr;
     if (exp_avg[i].scalar_type() == at::kByte) {
       TORCH_CHECK(scale_of < scales.size(), "adamw: an 8-bit state has no scales");
-      scale = scales[scale_of++];
+      scale = &scales[scale_of++];
     }
     need_states(params[i], exp_avg[i], exp_avg_sq[i], scale);
-    if (scale.has_value()) {
+    if (scale) {
       me[i] = static_cast<uint8_t*>(scale->data_ptr());
       ve[i] = me[i] + scale->stride(0);
     }
@@ -580,7 +580,7 @@ void adamw_values(at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorL
   for (size_t i = 0; i < n; ++i) {
     need_cuda(exp_avg[i], "a state");
     TORCH_CHECK(exp_avg[i].device() == exp_avg[0].device(), "adamw_state: tensors of one device");
-    need_states(exp_avg[i], exp_avg[i], exp_avg_sq[i], scales[i]);
+    need_states(exp_avg[i], exp_avg[i], exp_avg_sq[i], &scales[i]);
     for (const Tensor* t : {&m_out[i], &v_out[i]})
       TORCH_CHECK(t->device() == exp_avg[i].device() && t->scalar_type() == at::kFloat && t->sizes() == exp_avg[i].sizes() && t->is_contiguous(),
                   "adamw_state: results must be contiguous fp32 of the states' shapes");
@@ -632,11 +632,12 @@ void adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_
   if (!scales.empty()) {
     TORCH_CHECK(scales.size() == params.size() && exp_avg.size() == params.size(), "adamw: ", params.size(), " parameters, ", exp_avg.size(), " states, ",
                 scales.size(), " scales");
+    held.reserve(scales.size());
     for (size_t i = 0; i < exp_avg.size(); ++i) {
-      const optional<Tensor> scale = scales.get(i);
+      optional<Tensor> scale = scales.get(i);
       TORCH_CHECK(scale.has_value() == (exp_avg[i].scalar_type() == at::kByte), "adamw: scales belong to a state of uint8 codes and only to one, got ",
                   scale.has_value() ? "scales" : "none", " for a state of ", exp_avg[i].scalar_type());
-      if (scale.has_value()) held.push_back(*scale);
+      if (scale.has_value()) held.push_back(*std::move(scale));
     }
   }
   if (plain(params[0])) {

@@ -391,7 +391,7 @@ int s3r_int8_linear(const int8_t* a, int64_t a_pitch, const float* a_scale, cons
                     const float* bias, void* out, int type, int64_t M, int N, int K, void* stream);
 
 /* Euclidean norm of all elements of n tensors, summed in 64 bits in a fixed order.  The arrays are HOST arrays of device pointers,
- * element counts (0 is allowed) and types.  workspace: s3r_grad_norm_workspace_bytes(n, total elements). */
+ * element counts (0 is allowed) and types.  workspace: s3r_grad_norm_workspace_bytes(n, counts). */
 size_t s3r_grad_norm_workspace_bytes(int n, const int64_t* counts);
 int s3r_grad_norm(int n, const void* const* tensors, const int64_t* counts, const int* types, float* norm, void* workspace,
                   size_t workspace_bytes, void* stream);

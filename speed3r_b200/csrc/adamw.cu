@@ -5,7 +5,8 @@
 // magnitudes by shuffles.  The shared factor is a power of two: it changes only when a block's largest magnitude crosses one, so that
 // the codes' grid stands still between steps.  Rounding a v that moves by 0.1 % a step then has a variance of step size x change
 // (with any other factor every code would be rounded anew each step, with step size^2 / 6, 30 times as much, and to nearest it
-// would hardly ever move).  All scalings are exact: the only rounding of a state is that of its code.
+// would hardly ever move).  All scalings are by powers of two and exact, but for values below a code's normal numbers (exponent field 0): these
+// are fp32 subnormals once scaled, rounded to 2^-20 of a code's step before they are rounded to the code.  There is no other rounding of a state.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -128,8 +129,8 @@ __device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
 }
 __device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
 // Codes are the top of the bits of |x| scaled so that the code's smallest exponent field is fp32's own; what is added below the last bit
-// that is kept rounds them (0x7FFFF and that bit: to nearest even; a random number of as many bits: stochastically).  Two products, each
-// exact: by the block's power of two, then by 2^-112 (m, 4 bits of exponent) or 2^-96 (v, 5 bits).
+// that is kept rounds them (0x7FFFF and that bit: to nearest even; a random number of as many bits: stochastically).  Two products, by
+// powers of two: by the block's power of two, then by 2^-112 (m, 4 bits of exponent) or 2^-96 (v, 5 bits).
 constexpr float kDownM = 1.92592994438723585e-34f, kDownV = 1.26217744835361889e-29f;
 constexpr float kUpM = 5.19229685853482763e33f, kUpV = 7.92281625142643376e28f;
 __device__ __forceinline__ float unit_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fffffffu) : power_of(e); }
@@ -367,7 +368,7 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
 }
 
 // A warp has one block.  What hides the latency of its loads is other warps: with 56 registers 36 of them fit an SM (227 M elements in 252
-// tensors, 8-bit states, 601 us = 6.0 TB/s; with 64 registers 629, with 48, which spill, a hundredth more than with 56), and a loop over several
+// tensors, 8-bit states, 601 us = 6.0 TB/s; though they spill 172 bytes; with 64 registers 629, with 48 a hundredth more than with 56), and a loop over several
 // blocks, with or without the next one on its way in registers, lost more of them than it gained.  CTAs of 128 leave an SM in smaller
 // parts than those of 256 (640 where those take 715).
 template <bool EIGHT, bool SUBNORMAL>

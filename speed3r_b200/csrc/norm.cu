@@ -768,7 +768,7 @@ static void bwd_shape(int channels, bool whole, int* G, int* E) {
   *E = channels <= 4096 ? 8 : 16;
 }
 // slices per batch entry (of `entries`): CTAs that are resident together and no more (3 x 1041 rows of 1540, a gate per channel: 150 of them on
-// 148 SMs took 61 us, 147 take 35), each with four rows per group at least
+// 148 SMs took 61 us, 147 take 35), each with two rows per group or more where there are as many
 static int bwd_slices(int64_t entries, int64_t span, int G, bool full) {
   const int threads = cta_threads(G), groups = threads / G;
   const int64_t resident = static_cast<int64_t>(sm_count()) * bwd_resident(G, full);

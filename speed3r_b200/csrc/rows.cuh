@@ -250,7 +250,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // A quotient of 8 bits per element and one scale per row: what 127 is worth, and its inverse.  Rows whose largest magnitude is
-// below 2^-119 (127 / big would be infinite) become zeros.
+// below 2^-119 become zeros (below 2^-121 the inverse, 127 / big, would be infinite); their scale is what it is.
 struct RowScale {
   float scale, inverse;
 };

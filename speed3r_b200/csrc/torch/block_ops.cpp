@@ -290,7 +290,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 };
 
-// [.., tokens, channels] as [batch, tokens, channels], at a multiple of 16 bytes
+// [.., tokens, channels] as a contiguous [batch, tokens, channels], which begins anywhere: the kernels look at addresses themselves
 Tensor as_rows(const Tensor& t) {
   const int64_t d = t.dim(), tokens = d > 1 ? t.size(d - 2) : 1;
   int64_t batch = 1;

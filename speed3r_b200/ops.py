@@ -16,7 +16,8 @@ that ends a training iteration (``grad_norm``, ``adamw_step``), plus the pieces 
 
 Allocation, argument checks and autograd wiring are native (``csrc/torch/bindings.cpp``, a ``torch.library``
 namespace over the C ABI); this file holds the Python signatures and the shape functions for
-``torch.compile``.  CPU tensors, fp32/fp16 inputs and a missing library raise: there is no fallback.
+``torch.compile``.  CPU tensors, types that an operator does not take (the attention's take bf16, the operators around it fp32 and
+fp16 too) and a missing library raise: there is no fallback.
 """
 from __future__ import annotations
 

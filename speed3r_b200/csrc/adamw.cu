@@ -306,7 +306,7 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
       low[k + 1] = r.y;
     }
     // All 16 bits that a bf16 parameter drops, so that an update of any size happens as often as it should; the lower 6 of them are the upper 6
-    // of those that round v, of which a parameter's rounding hardly ever depends.  fp16's values below 2^-14 have fewer, so it is rounded to
+    // of those that round v, on which a parameter's rounding hardly ever depends.  fp16's values below 2^-14 have fewer, so it is rounded to
     // nearest.
     if (p_type == S3R_BF16)
 #pragma unroll
@@ -368,8 +368,8 @@ __device__ __forceinline__ void step_block(const Lane<EIGHT>& l, const AdamCommo
 }
 
 // A warp has one block.  What hides the latency of its loads is other warps: with 56 registers 36 of them fit an SM (227 M elements in 252
-// tensors, 8-bit states, 601 us = 6.0 TB/s; though they spill 172 bytes; with 64 registers 629, with 48 a hundredth more than with 56), and a loop over several
-// blocks, with or without the next one on its way in registers, lost more of them than it gained.  CTAs of 128 leave an SM in smaller
+// tensors, 8-bit states, 601 us = 6.0 TB/s, 172 bytes of spills and all; with 64 registers 629, with 48 a hundredth more than with 56), and a
+// loop over several blocks, with or without the next one on its way in registers, lost more of them than it gained.  CTAs of 128 leave an SM in smaller
 // parts than those of 256 (640 where those take 715).
 template <bool EIGHT, bool SUBNORMAL>
 __device__ __forceinline__ void run_block(const AdamCommon& p, const AdamTensor& x, int64_t block, int lane) {

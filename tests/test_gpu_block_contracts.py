@@ -51,6 +51,39 @@ def test_compiled_step_is_the_step(eight):
     assert len(flat(want)) == len(flat(got)) and all(torch.equal(x, y) for x, y in zip(flat(want) + flat(a), flat(got) + flat(b)))
 
 
+@pytest.mark.parametrize("post", [False, True])
+def test_compiled_norms_are_the_norms(post):
+    """Forward and backward, through the nodes that a tracer sees."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+    inputs = [rand(2, 33, 136), rand(2, 33, 136).bfloat16(), rand(136), rand(136), rand(136), rand(2, 33, 1), rand(136)]
+
+    def f(x, y, w, b, scale, gate, pw):
+        r, h = ops.residual_norm(x, y, (w, b, 1e-5), scale, gate, (pw, None, 1e-6) if post else None, "rms" if post else "layer", torch.bfloat16)
+        return (r * 2).sum() + (h.float() ** 2).sum(), r, h
+
+    results = []
+    for call in (f, compiled(f)):
+        leaves = [t.clone().requires_grad_(True) for t in inputs]
+        loss, r, h = call(*leaves)
+        loss.backward()
+        results.append([r.detach(), h.detach()] + [t.grad for t in leaves[:6 + post]])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and len(results[0]) == 8 + post
+
+
+def test_compiled_8_bit_products_are_the_products():
+    x, w = torch.randn(3, 7, 72, device=DEV).bfloat16(), torch.randn(40, 72, device=DEV)
+    wq, ws = ops.quantize_tokens(w)
+    bias, one = torch.randn(40, device=DEV), torch.ones(72, device=DEV)
+
+    def f(x):
+        r, q, s = ops.residual_norm_int8(x, x, (one, None, 1e-5))
+        return r, ops.int8_linear(q, s, wq, ws, bias), ops.int8_linear(*ops.quantize_tokens(x), wq, ws, None, torch.float32)
+
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(f(x), compiled(f)(x)))
+
+
 def test_operators_have_the_schemas_and_shapes_that_they_say():
     x, y, w = torch.randn(2, 3, 40, device=DEV), torch.randn(2, 3, 40, device=DEV).bfloat16(), torch.ones(40, device=DEV)
     check = lambda op, args: torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))

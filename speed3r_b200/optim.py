@@ -42,6 +42,10 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = max_norm
         self.grad_norm: Optional[Tensor] = None       # of the last step with max_norm, 0-dim on the device
 
+    def __getstate__(self):
+        """PyTorch's keeps three attributes; copies and pickles clip as well."""
+        return {**super().__getstate__(), "max_norm": self.max_norm, "grad_norm": None}
+
     @staticmethod
     def _outside_of_a_graph(what: str) -> None:
         """What makes states once would make them anew in every replay."""

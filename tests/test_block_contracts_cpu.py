@@ -329,3 +329,20 @@ def test_a_workspace_that_is_too_small_for_the_sums_is_refused(lib, count):
     assert whole > 0 and whole % 6 == 0
     g.workspace_bytes = whole // 6 * count - 1
     assert lib.s3r_residual_norm_bwd(C.byref(f), C.byref(g), None) == -6
+
+
+def test_copies_of_the_optimiser_clip_too(monkeypatch):
+    import copy
+    import pickle
+    from speed3r_b200 import AdamW
+
+    seen = []
+    monkeypatch.setattr(ops, "grad_norm", lambda grads: torch.tensor(3.0))
+    monkeypatch.setattr(ops, "adamw_step", lambda *a, grad_norm=None, max_norm=None, **kw: seen.append((float(grad_norm), max_norm)))
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = AdamW([p], max_norm=2.0)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        (q,) = other.param_groups[0]["params"]
+        q.grad = torch.ones(3)
+        other.step()
+    assert seen == [(3.0, 2.0)] * 2

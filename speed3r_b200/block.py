@@ -151,7 +151,7 @@ class BlockRope(nn.Module):
         return type(self.mlp) is Mlp and type(self.mlp.fc1) is Int8Linear
 
     def _takes_int8(self) -> bool:
-        return type(getattr(self.attn, "qkv", None)) is Int8Linear
+        return type(self.attn).forward is SparseFlashAttentionRope.forward and type(self.attn.qkv) is Int8Linear
 
     def forward(self, x: Tensor, xpos: Optional[Tensor] = None) -> Tensor:
         if not (self._fuses() and self._fits(x)):

@@ -346,3 +346,17 @@ def test_copies_of_the_optimiser_clip_too(monkeypatch):
         q.grad = torch.ones(3)
         other.step()
     assert seen == [(3.0, 2.0)] * 2
+
+
+def test_another_attention_is_given_activations_in_8_bits_too():
+    from speed3r_b200 import BlockRope, Int8Linear, SparseFlashAttentionRope
+
+    class Other(SparseFlashAttentionRope):
+        def forward(self, x, attn_bias=None, xpos=None):
+            return super().forward(x * 1.0, attn_bias, xpos)
+
+    for cls in (Other, Plain, SparseFlashAttentionRope):
+        b = BlockRope(64, 1, attn_class=cls)
+        assert not b._takes_int8()
+        b.attn.qkv = Int8Linear(torch.zeros(192, 64, dtype=torch.int8), torch.ones(192), None)
+        assert b._takes_int8() == (cls is SparseFlashAttentionRope)

@@ -40,6 +40,8 @@ class Int8Linear(nn.Module):
         for m in linears:
             if not isinstance(m, nn.Linear) or type(m).forward is not nn.Linear.forward or "forward" in m.__dict__:
                 raise RuntimeError(f"Int8Linear.of: {type(m).__name__} computes something else than a Linear")
+            if m._forward_hooks or m._forward_pre_hooks:              # they may change what goes in and out, or make the weight
+                raise RuntimeError("Int8Linear.of: this Linear has hooks, which its 8-bit form would lose: remove them first")
         biases = [m.bias for m in linears]
         if any(b is None for b in biases) and any(b is not None for b in biases):
             biases = [b if b is not None else torch.zeros(m.out_features, device=m.weight.device) for b, m in zip(biases, linears)]

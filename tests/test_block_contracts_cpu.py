@@ -360,3 +360,18 @@ def test_another_attention_is_given_activations_in_8_bits_too():
         assert not b._takes_int8()
         b.attn.qkv = Int8Linear(torch.zeros(192, 64, dtype=torch.int8), torch.ones(192), None)
         assert b._takes_int8() == (cls is SparseFlashAttentionRope)
+
+
+@pytest.mark.filterwarnings("ignore::FutureWarning")
+def test_a_linear_with_hooks_does_not_become_an_8_bit_one():
+    """One whose weight a hook makes of others has, until it is called, the weight of before."""
+    from speed3r_b200 import Int8Linear
+    normed = torch.nn.utils.weight_norm(torch.nn.Linear(16, 5))
+    with torch.no_grad():
+        normed.weight_g.mul_(3)
+    raises("has hooks", lambda: Int8Linear.of(normed))
+    watched = torch.nn.Linear(16, 5)
+    handle = watched.register_forward_hook(lambda m, i, o: o * 2)
+    raises("has hooks", lambda: Int8Linear.of(torch.nn.Linear(16, 5), watched))
+    handle.remove()
+    raises("no CPU path", lambda: Int8Linear.of(watched))

@@ -436,6 +436,90 @@ int s3r_adamw_step_numbered(const s3r_adamw* args_host, const uint32_t* numbers,
 int s3r_adamw_state(int n, const void* const* m, const void* const* v, const uint8_t* const* m_exponents, const uint8_t* const* v_exponents,
                     float* const* m_out, float* const* v_out, const int64_t* counts, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The dense half of a block: Linear layers with what follows them, and what stands between the qkv projection and dense attention
+ * (pi3/models/layers/attention.py:324-348, block.py:310-335), which the reference leaves to eager PyTorch.
+ * ------------------------------------------------------------------------------------------ */
+#define S3R_ACT_NONE 0
+#define S3R_ACT_GELU 1      /* z Phi(z) */
+#define S3R_ACT_GELU_TANH 2 /* z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define S3R_ACT_SILU 3      /* z / (1 + exp(-z)) */
+
+/* z = x W^T + bias;  out = residual + act(z) * scale, in fp32, rounded once.  x [M, K], weight [N, K]: both of `type` (S3R_BF16 or S3R_F16), base
+ * and rows at multiples of 16 bytes (pitches in elements).  bias, scale [N], residual [M, N]: each may be NULL and has a type of its own.
+ * residual, out [M, N] contiguous.  Fewer than 2^31 - 512 rows and columns. */
+typedef struct {
+  int64_t M;
+  int N, K, type;
+  const void* x;
+  int64_t x_pitch;
+  const void* weight;
+  int64_t w_pitch;
+  const void *bias, *scale, *residual;
+  int bias_type, scale_type, residual_type, act;
+  void* out;
+  int out_type;
+} s3r_linear;
+int s3r_linear_fwd(const s3r_linear* args_host, void* stream);
+
+/* The elementwise part of its backward; f: the forward's arguments (residual and out are not read).  dy [M, N] contiguous, of f's out_type.
+ *   dz       [M, N] of f's type, rows of dz_pitch elements at multiples of 16 bytes: dy * scale * act'(z); may be NULL
+ *   d_bias   [N] of bias_type: sum of dz over rows; d_scale [N] of scale_type: sum of dy * act(z); each may be NULL
+ * z is computed again where act or d_scale needs it.  workspace: s3r_linear_bwd_workspace_bytes for each of d_bias and d_scale that is wanted. */
+typedef struct {
+  const void* dy;
+  void* dz;
+  int64_t dz_pitch;
+  void *d_bias, *d_scale;
+  void* workspace;
+  size_t workspace_bytes;
+} s3r_linear_grad;
+size_t s3r_linear_bwd_workspace_bytes(int64_t M, int N);
+int s3r_linear_bwd(const s3r_linear* f_host, const s3r_linear_grad* g_host, void* stream);
+
+/* out [M, N] contiguous = sum over k of a(m, k) b(n, k), fp32 sums: a lies as [M, K] or, turned, as [K, M], b as [N, K] or [K, N].  All of `type`
+ * (S3R_BF16 or S3R_F16); operands' bases and rows at multiples of 16 bytes.  dx = product(dz, weight turned), dW = product(dz turned, x turned). */
+int s3r_product(const void* a, int64_t a_pitch, int a_turned, const void* b, int64_t b_pitch, int b_turned, int type, void* out, int64_t M, int N,
+                int64_t K, void* stream);
+
+/* The packed projection qkv [batch, tokens, (heads + 2 * kv_heads) * head_dim], heads of q, k and v one behind the other, as q, k and v
+ * [batch, heads | kv_heads, tokens, head_dim] contiguous:  n = norm(x) * weight + bias per head of q and k (S3R_NORM_*, q_normed / k_normed == 0:
+ * n = x), then the rotation: axis a (of `axes`, 0: none) turns columns 2 * pairs * a + i and 2 * pairs * a + pairs + i, i < pairs, by
+ *   (n1 cos - n2 sin, n2 cos + n1 sin),  cos and sin of row pos[b, t, a], column i.
+ * Columns from 2 * pairs * axes on are not turned.  fp32 inside, one rounding.
+ *   head_dim even, 2 to 256; qkv, q, k, v of `type`, strides in elements (a token's columns are contiguous)
+ *   pos int64 [batch, tokens, axes], last stride 1; a position outside [0, rows) is clamped and sets S3R_STATUS_BAD_INDEX
+ *   cos, sin [rows, pairs] of table_type, rows of *_pitch elements;  weights and biases [head_dim] of param_type, each may be NULL */
+typedef struct {
+  int64_t batch, tokens;
+  int heads, kv_heads, head_dim;
+  int kind, q_normed, k_normed;
+  float q_eps, k_eps;
+  int type, param_type, table_type;
+  int axes, pairs, rows;
+  int64_t stride_b, stride_t, pos_stride_b, pos_stride_t, cos_pitch, sin_pitch;
+  const void* qkv;
+  const int64_t* pos;
+  const void *cos, *sin;
+  const void *q_weight, *q_bias, *k_weight, *k_bias;
+  void *q, *k, *v;
+} s3r_qkv_norm_rope;
+int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* args_host, void* stream);
+
+/* Gradients: d_qkv [batch, tokens, (heads + 2 * kv_heads) * head_dim] contiguous from dq, dk, dv (any of them NULL: zeros), whose strides of a batch
+ * entry, a head and a token are given in elements.  d_* [head_dim] of param_type, each may be NULL: sums in fp32 in a fixed order.  f's q, k, v are
+ * not read.  workspace: s3r_qkv_norm_rope_bwd_workspace_bytes where a d_* is wanted. */
+typedef struct {
+  const void *dq, *dk, *dv;
+  int64_t dq_strides[3], dk_strides[3], dv_strides[3];
+  void* d_qkv;
+  void *d_q_weight, *d_q_bias, *d_k_weight, *d_k_bias;
+  void* workspace;
+  size_t workspace_bytes;
+} s3r_qkv_norm_rope_grad;
+size_t s3r_qkv_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim);
+int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f_host, const s3r_qkv_norm_rope_grad* g_host, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,6 +56,13 @@ SIGNATURES = {
     "s3r_adamw_step": (_i, [_p, _p]),
     "s3r_adamw_step_numbered": (_i, [_p, _p, _p]),
     "s3r_adamw_state": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "s3r_linear_fwd": (_i, [_p, _p]),
+    "s3r_linear_bwd_workspace_bytes": (_sz, [_i64, _i]),
+    "s3r_linear_bwd": (_i, [_p, _p, _p]),
+    "s3r_product": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _p, _i64, _i, _i64, _p]),
+    "s3r_qkv_norm_rope_fwd": (_i, [_p, _p]),
+    "s3r_qkv_norm_rope_bwd_workspace_bytes": (_sz, [_i64, _i64, _i, _i, _i]),
+    "s3r_qkv_norm_rope_bwd": (_i, [_p, _p, _p]),
     "s3r_copy2d_async": (_i, [_p, _sz, _p, _sz, _sz, _sz, _p]),
     "s3r_peer_pull": (_i, [_p, _p, _p, _i, _i, _p]),
     "s3r_ipc_export": (_i, [_p, _p, C.POINTER(C.c_int64)]),

@@ -1,0 +1,650 @@
+// The packed projection [batch, tokens, heads of q, k and v] as q, k and v [batch, heads, tokens, head_dim]: every head of q and k normalised
+// (LayerNorm or by the root of its mean square) and turned by the rotary embedding, in one pass, and the gradient of that.
+// Bound: HBM, every element is read once and written once (backward: x and its gradient read, one gradient written).
+//
+// A head's columns are pairs (i, i + pairs) that rotation turns, so a thread takes both members: V columns of the first kind and the V columns
+// `pairs` further, two vectors, and needs nobody else's for the rotation.  G threads share a head; sums over it are log2 G shuffles.
+// Columns that are not turned are taken as two neighbouring vectors.  A group of G threads stays with one token and walks over heads, so that the
+// token's sines and cosines, the parameters and the sums over rows stay in registers; the groups of a warp have neighbouring tokens, whose
+// results lie one behind the other.
+#include <type_traits>
+
+#include "rows.cuh"
+
+namespace s3r {
+
+struct NrParams {
+  const void *qkv, *cos, *sin;
+  const int64_t* pos;
+  const void *weight[2], *bias[2];     // of q and k
+  void* out[3];                        // q, k, v
+  const void* d_out[3];                // backward: their gradients
+  int64_t d_strides[3][3];
+  void* d_qkv;
+  float* sums;                         // [head chunks of q, then of k][CTAs of a chunk][weight, bias][head_dim]
+  int64_t stride_b, stride_t, pos_stride_b, pos_stride_t, cos_pitch, sin_pitch, rows_of_tokens;
+  int tokens, heads, kv_heads, head_dim, kind, type, param_type, table_type, axes, pairs, rows;
+  int normed[2];
+  float eps[2], inverse_dim;
+  int per_chunk, q_chunks, kv_chunks;
+  uint32_t* status;
+};
+
+// A vector of V elements of 16 or 32 bits, as it lies in memory.
+template <int V, int BYTES>
+struct Vec {
+  static constexpr int kWords = V * BYTES / 4 < 1 ? 1 : V * BYTES / 4;
+  uint32_t w[kWords];
+};
+template <int V, int BYTES>
+__device__ __forceinline__ void load_vec(Vec<V, BYTES>& v, const void* p, int64_t at) {
+  const char* from = static_cast<const char*>(p) + at * BYTES;
+  if constexpr (V * BYTES == 2) {
+    v.w[0] = __ldg(reinterpret_cast<const uint16_t*>(from));
+  } else if constexpr (V * BYTES == 4) {
+    v.w[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+  } else if constexpr (V * BYTES == 8) {
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(from));
+    v.w[0] = u.x, v.w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V * BYTES / 16; ++i) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(from) + i);
+      v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+    }
+  }
+}
+template <int V, int BYTES>
+__device__ __forceinline__ void store_vec(const Vec<V, BYTES>& v, void* p, int64_t at) {
+  char* to = static_cast<char*>(p) + at * BYTES;
+  if constexpr (V * BYTES == 2) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(v.w[0]);
+  else if constexpr (V * BYTES == 4) *reinterpret_cast<uint32_t*>(to) = v.w[0];
+  else if constexpr (V * BYTES == 8) *reinterpret_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < V * BYTES / 16; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
+}
+template <int V, int BYTES>
+__device__ __forceinline__ void values(float* f, const Vec<V, BYTES>& v, int type) {
+  if constexpr (BYTES == 4) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(v.w[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const uint32_t w = v.w[k / 2];
+      f[k] = type == S3R_BF16 ? (k & 1 ? bf16_hi(w) : bf16_lo(w)) : (k & 1 ? half_hi(w) : half_lo(w));
+    }
+  }
+}
+template <int V, int BYTES>
+__device__ __forceinline__ void rounded(Vec<V, BYTES>& v, const float* f, int type) {
+  if constexpr (BYTES == 4) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v.w[k] = __float_as_uint(f[k]);
+  } else if constexpr (V == 1) {
+    v.w[0] = (type == S3R_BF16 ? pack_bf16(f[0], 0.f) : pack_half(f[0], 0.f)) & 0xffffu;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) v.w[k / 2] = type == S3R_BF16 ? pack_bf16(f[k], f[k + 1]) : pack_half(f[k], f[k + 1]);
+  }
+}
+
+constexpr int kNrThreads = 256;
+
+// Where a thread's E slots lie: columns c0 .. c0 + V and c1 .. c1 + V, the axis that turns them (-1: none), column of the tables.
+struct Slot {
+  int c0, c1, axis, column;
+};
+template <int V>
+__device__ __forceinline__ Slot slot_of(int s, const NrParams& p) {
+  const int per = p.axes ? p.pairs / V : 1, turned = p.axes * per;
+  if (s < turned) {
+    const int a = s / per, j = (s - a * per) * V;
+    return {2 * p.pairs * a + j, 2 * p.pairs * a + p.pairs + j, a, j};
+  }
+  const int c = 2 * p.pairs * p.axes + (s - turned) * 2 * V;
+  return {c, c + V, -1, 0};
+}
+
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&s)[N]) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+}
+
+// What a thread keeps of its token and of its columns
+template <int V, int E>
+struct Lane {
+  Slot slot[E];
+  bool on[E];
+  float cos[E][V], sin[E][V], weight[E][2 * V], bias[E][2 * V];
+};
+template <int V, int E>
+__device__ __forceinline__ void parameters(Lane<V, E>& l, const NrParams& p, int part, bool bias) {
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) {
+      const int col = (k < V ? l.slot[e].c0 : l.slot[e].c1 - V) + k;
+      l.weight[e][k] = part < 2 && l.on[e] && p.weight[part] ? load_one(p.weight[part], p.param_type, col) : 1.f;
+      l.bias[e][k] = bias && part < 2 && l.on[e] && p.bias[part] ? load_one(p.bias[part], p.param_type, col) : 0.f;
+    }
+}
+template <int V, int E>
+__device__ __forceinline__ void angles(Lane<V, E>& l, const NrParams& p, int64_t b, int t, bool in) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool turned = in && l.on[e] && l.slot[e].axis >= 0;
+    int64_t row = turned ? __ldg(p.pos + b * p.pos_stride_b + t * p.pos_stride_t + l.slot[e].axis) : 0;
+    if (row < 0 || row >= p.rows) {
+      if (turned) atomicOr(p.status, kStatusBadIndex);
+      row = row < 0 ? 0 : p.rows - 1;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      l.cos[e][k] = turned ? load_one(p.cos, p.table_type, row * p.cos_pitch + l.slot[e].column + k) : 1.f;
+      l.sin[e][k] = turned ? load_one(p.sin, p.table_type, row * p.sin_pitch + l.slot[e].column + k) : 0.f;
+    }
+  }
+}
+
+// Heads of a CTA: part 0 q, 1 k, 2 v; heads first .. first + count of it.
+struct Heads {
+  int part, first, count;
+};
+__device__ __forceinline__ Heads heads_of(int chunk, const NrParams& p) {
+  int part = 0, n = p.heads;
+  if (chunk >= p.q_chunks) {
+    chunk -= p.q_chunks;
+    part = 1;
+    n = p.kv_heads;
+    if (chunk >= p.kv_chunks) chunk -= p.kv_chunks, part = 2;
+  }
+  const int first = chunk * p.per_chunk;
+  return {part, first, min(p.per_chunk, n - first)};
+}
+__device__ __forceinline__ int packed_head(const Heads& h, const NrParams& p) { return h.first + (h.part > 0 ? p.heads : 0) + (h.part > 1 ? p.kv_heads : 0); }
+
+// (x - mean) * inverse in place; returns the inverse
+template <int V, int G, int E>
+__device__ __forceinline__ float normalise(float (&x)[E][2 * V], const Lane<V, E>& l, const NrParams& p, int part) {
+  float s[1];
+  if (p.kind == S3R_NORM_LAYER) {
+    s[0] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 0; k < 2 * V; ++k) s[0] += x[e][k];
+    group_sum<G>(s);
+    const float mean = s[0] * p.inverse_dim;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 0; k < 2 * V; ++k) x[e][k] = l.on[e] ? x[e][k] - mean : 0.f;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) s[0] = fmaf(x[e][k], x[e][k], s[0]);
+  group_sum<G>(s);
+  const float inverse = 1.f / sqrtf(s[0] * p.inverse_dim + p.eps[part]);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) x[e][k] *= inverse;
+  return inverse;
+}
+
+template <int V, int G, int E, int BYTES>
+__global__ void __launch_bounds__(kNrThreads) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
+  constexpr int kTokens = kNrThreads / G, U = V * BYTES * E >= 32 ? 2 : 4;       // heads whose loads are in flight
+  griddep_wait();
+  griddep_launch();
+  const int t = threadIdx.x % G;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / G, b = token / p.tokens;
+  const bool in = token < p.rows_of_tokens;
+  const int at = static_cast<int>(token - b * p.tokens);
+  const Heads h = heads_of(blockIdx.y, p);
+  const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
+  Lane<V, E> l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    l.slot[e] = slot_of<V>(t + e * G, p);
+    l.on[e] = (t + e * G) * 2 * V < p.head_dim;
+  }
+  const int64_t from = b * p.stride_b + at * p.stride_t + static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
+  const int64_t plane = static_cast<int64_t>(p.tokens) * p.head_dim;
+  const int64_t to = (b * (h.part == 0 ? p.heads : p.kv_heads) + h.first) * plane + static_cast<int64_t>(at) * p.head_dim;
+  void* out = p.out[h.part];
+  Vec<V, BYTES> raw[U][E][2];
+  auto fetch = [&](int i, int u) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (in && l.on[e] && i < h.count) {
+        load_vec<V, BYTES>(raw[u][e][0], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
+        load_vec<V, BYTES>(raw[u][e][1], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
+      }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) fetch(u, u);
+  if (h.part < 2) {
+    angles<V, E>(l, p, b, at, in);
+    parameters<V, E>(l, p, h.part, true);
+  }
+  for (int i0 = 0; i0 < h.count; i0 += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= h.count) break;
+      if (h.part == 2) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (in && l.on[e]) {
+            store_vec<V, BYTES>(raw[u][e][0], out, to + i * plane + l.slot[e].c0);
+            store_vec<V, BYTES>(raw[u][e][1], out, to + i * plane + l.slot[e].c1);
+          }
+        fetch(i + U, u);
+        continue;
+      }
+      float x[E][2 * V];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        values<V, BYTES>(x[e], raw[u][e][0], p.type);
+        values<V, BYTES>(x[e] + V, raw[u][e][1], p.type);
+        if (!(in && l.on[e]))
+#pragma unroll
+          for (int k = 0; k < 2 * V; ++k) x[e][k] = 0.f;
+      }
+      fetch(i + U, u);
+      if (normed) {
+        normalise<V, G, E>(x, l, p, h.part);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int k = 0; k < 2 * V; ++k) x[e][k] = fmaf(x[e][k], l.weight[e][k], l.bias[e][k]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (in && l.on[e]) {
+          if (l.slot[e].axis >= 0)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const float x1 = x[e][k], x2 = x[e][V + k];
+              x[e][k] = x1 * l.cos[e][k] - x2 * l.sin[e][k];
+              x[e][V + k] = x2 * l.cos[e][k] + x1 * l.sin[e][k];
+            }
+          Vec<V, BYTES> o;
+          rounded<V, BYTES>(o, x[e], p.type);
+          store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c0);
+          rounded<V, BYTES>(o, x[e] + V, p.type);
+          store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c1);
+        }
+    }
+  }
+}
+
+// The gradient of a head: turned back, then through the norm as computed again from x.  Sums for weight and bias: over the CTA's tokens and heads in
+// registers, over the warp's groups by shuffles, over warps in shared memory, over CTAs by norm_rope_sums_kernel.
+template <int V, int G, int E, int BYTES>
+__global__ void __launch_bounds__(kNrThreads) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
+  constexpr int kTokens = kNrThreads / G;
+  __shared__ float red[2][kNrThreads / 32][2 * V * G * E];
+  griddep_wait();
+  griddep_launch();
+  const int t = threadIdx.x % G;
+  const Heads h = heads_of(blockIdx.y, p);
+  const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
+  Lane<V, E> l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    l.slot[e] = slot_of<V>(t + e * G, p);
+    l.on[e] = (t + e * G) * 2 * V < p.head_dim;
+  }
+  if (normed) parameters<V, E>(l, p, h.part, false);
+  float dw[E][2 * V], db[E][2 * V];
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) dw[e][k] = db[e][k] = 0.f;
+  const void* d_out = p.d_out[h.part];
+  const int64_t width = static_cast<int64_t>(p.heads + 2 * p.kv_heads) * p.head_dim;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens; first < p.rows_of_tokens; first += static_cast<int64_t>(gridDim.x) * kTokens) {
+    const int64_t token = first + threadIdx.x / G, b = token / p.tokens;
+    const bool in = token < p.rows_of_tokens;
+    const int at = static_cast<int>(token - b * p.tokens);
+    const int64_t column = static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
+    const int64_t from = b * p.stride_b + at * p.stride_t + column, to = token * width + column;
+    const int64_t d_from = b * p.d_strides[h.part][0] + h.first * p.d_strides[h.part][1] + at * p.d_strides[h.part][2], d_head = p.d_strides[h.part][1];
+    if (h.part < 2) angles<V, E>(l, p, b, at, in);
+    for (int i = 0; i < h.count; ++i) {
+      Vec<V, BYTES> raw[E][2], d_raw[E][2];
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (in && l.on[e]) {
+          if (d_out) {
+            load_vec<V, BYTES>(d_raw[e][0], d_out, d_from + i * d_head + l.slot[e].c0);
+            load_vec<V, BYTES>(d_raw[e][1], d_out, d_from + i * d_head + l.slot[e].c1);
+          }
+          if (normed) {
+            load_vec<V, BYTES>(raw[e][0], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
+            load_vec<V, BYTES>(raw[e][1], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
+          }
+        }
+      float d[E][2 * V];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        values<V, BYTES>(d[e], d_raw[e][0], p.type);
+        values<V, BYTES>(d[e] + V, d_raw[e][1], p.type);
+        if (!(in && l.on[e] && d_out))
+#pragma unroll
+          for (int k = 0; k < 2 * V; ++k) d[e][k] = 0.f;
+        if (h.part < 2 && l.slot[e].axis >= 0)
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float d1 = d[e][k], d2 = d[e][V + k];
+            d[e][k] = d1 * l.cos[e][k] + d2 * l.sin[e][k];
+            d[e][V + k] = d2 * l.cos[e][k] - d1 * l.sin[e][k];
+          }
+      }
+      if (normed) {
+        float x[E][2 * V];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          values<V, BYTES>(x[e], raw[e][0], p.type);
+          values<V, BYTES>(x[e] + V, raw[e][1], p.type);
+          if (!(in && l.on[e]))
+#pragma unroll
+            for (int k = 0; k < 2 * V; ++k) x[e][k] = 0.f;
+        }
+        const float inverse = normalise<V, G, E>(x, l, p, h.part);
+        float s[2] = {0.f, 0.f};                             // sums of e and e * n, e = d * weight
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int k = 0; k < 2 * V; ++k) {
+            if (in) dw[e][k] = fmaf(d[e][k], x[e][k], dw[e][k]);      // a token that is not there has d = 0, x whatever eps makes of zeros
+            db[e][k] += d[e][k];
+            d[e][k] *= l.weight[e][k];
+            s[0] += d[e][k];
+            s[1] = fmaf(d[e][k], x[e][k], s[1]);
+          }
+        group_sum<G>(s);
+        const float mean = p.kind == S3R_NORM_LAYER ? s[0] * p.inverse_dim : 0.f, along = s[1] * p.inverse_dim;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int k = 0; k < 2 * V; ++k) d[e][k] = inverse * (d[e][k] - mean - x[e][k] * along);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (in && l.on[e]) {
+          Vec<V, BYTES> o;
+          rounded<V, BYTES>(o, d[e], p.type);
+          store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
+          rounded<V, BYTES>(o, d[e] + V, p.type);
+          store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
+        }
+    }
+  }
+  if (!p.sums || !normed) return;                            // the same for the whole CTA
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k)
+#pragma unroll
+      for (int o = 16; o >= G; o >>= 1) {
+        dw[e][k] += __shfl_xor_sync(0xffffffffu, dw[e][k], o);
+        db[e][k] += __shfl_xor_sync(0xffffffffu, db[e][k], o);
+      }
+  if ((threadIdx.x & 31) < G)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (l.on[e])
+#pragma unroll
+        for (int k = 0; k < 2 * V; ++k) {
+          const int col = (k < V ? l.slot[e].c0 : l.slot[e].c1 - V) + k;
+          red[0][threadIdx.x >> 5][col] = dw[e][k];
+          red[1][threadIdx.x >> 5][col] = db[e][k];
+        }
+  __syncthreads();
+  float* to = p.sums + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.head_dim;
+  for (int c = threadIdx.x; c < 2 * p.head_dim; c += kNrThreads) {
+    const int which = c >= p.head_dim, col = c - which * p.head_dim;
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNrThreads / 32; ++w) total += red[which][w][col];
+    to[c] = total;
+  }
+}
+
+// The CTAs' sums, in a fixed order: a CTA has 32 of a part's 2 * head_dim columns, a warp every 32nd row.
+struct NrSums {
+  const float* sums;
+  void* out[2][2];                   // of q and k: weight, bias
+  int64_t first[2], rows[2];
+  int head_dim, type;
+};
+__global__ void __launch_bounds__(1024) norm_rope_sums_kernel(const __grid_constant__ NrSums p) {
+  __shared__ float red[32][33];
+  griddep_wait();
+  griddep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = blockIdx.y, col = blockIdx.x * 32 + lane;
+  const bool in = col < 2 * p.head_dim;
+  float total = 0.f;
+  if (in)
+    for (int64_t i = warp; i < p.rows[part]; i += 32) total += __ldg(p.sums + (p.first[part] + i) * 2 * p.head_dim + col);
+  red[warp][lane] = total;
+  __syncthreads();
+  const int which = col >= p.head_dim;
+  void* out = p.out[part][which];
+  if (warp == 0 && in && out) {
+    float v[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[0] += red[i][lane];
+    Raw<1> o;
+    pack<1>(o, v, p.type);
+    store_raw<1>(o, out, p.type, col - which * p.head_dim);
+  }
+}
+
+template <int V, int G, int E, int BYTES>
+static int run_norm_rope(const NrParams& p, bool backward, unsigned ctas, cudaStream_t st) {
+  const dim3 grid(ctas, static_cast<unsigned>(p.q_chunks + 2 * p.kv_chunks));
+  if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+  return launch(norm_rope_fwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+}
+// Threads of a head: as many as it has pairs of vectors, a power of two.
+struct NrShape {
+  int vector, group;
+};
+static NrShape norm_rope_shape(int vector, int head_dim) {
+  const int slots = head_dim / (2 * vector);
+  if (vector == 8) return {8, slots <= 2 ? 2 : slots <= 4 ? 4 : slots <= 8 ? 8 : 16};
+  if (vector == 4) return {4, slots <= 8 ? 8 : 32};
+  return {1, 32};
+}
+template <int BYTES>
+static int pick_norm_rope(const NrParams& p, NrShape s, bool backward, unsigned ctas, cudaStream_t st) {
+  if (s.vector == 8 && s.group == 2) return run_norm_rope<8, 2, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 8 && s.group == 4) return run_norm_rope<8, 4, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 8 && s.group == 8) return run_norm_rope<8, 8, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 8) return run_norm_rope<8, 16, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 4 && s.group == 8) return run_norm_rope<4, 8, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 4) return run_norm_rope<4, 32, 1, BYTES>(p, backward, ctas, st);
+  return run_norm_rope<1, 32, 4, BYTES>(p, backward, ctas, st);
+}
+
+// Heads are split over CTAs until there are some for every SM; no further than that, a token's angles are found once per CTA.
+static void norm_rope_chunks(int64_t token_ctas, int heads, int kv_heads, int* per_chunk, int* q_chunks, int* kv_chunks) {
+  int per = heads;
+  while (per > 1) {
+    const int64_t chunks = (heads + per - 1) / per + 2 * ((kv_heads + per - 1) / per);
+    if (chunks * token_ctas >= 4 * sm_count()) break;
+    per = (per + 1) / 2;
+  }
+  *per_chunk = per;
+  *q_chunks = (heads + per - 1) / per;
+  *kv_chunks = (kv_heads + per - 1) / per;
+}
+// CTAs of the backward along the tokens: those that are resident together, so that each leaves one row of sums.
+static unsigned norm_rope_bwd_ctas(int64_t token_ctas, int chunks) {
+  const int64_t most = (4 * static_cast<int64_t>(sm_count()) + chunks - 1) / chunks;
+  return static_cast<unsigned>(token_ctas < most ? token_ctas : most < 1 ? 1 : most);
+}
+
+static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
+  S3R_REQUIRE(f && f->qkv, S3R_ERR_NULL, "%s: NULL pointer", what);
+  S3R_REQUIRE(f->batch > 0 && f->tokens > 0 && f->heads > 0 && f->kv_heads > 0, S3R_ERR_SHAPE, "%s: sizes must be positive", what);
+  S3R_REQUIRE(f->head_dim >= 2 && f->head_dim <= 256 && f->head_dim % 2 == 0, S3R_ERR_UNSUPPORTED, "%s: head_dim %d (even, 2 to 256)", what, f->head_dim);
+  S3R_REQUIRE(f->heads <= 4096 && f->kv_heads <= 4096 && f->tokens < (1ll << 31) - 1024 && f->batch < (1ll << 31) - 1024 && f->batch * f->tokens < (1ll << 31) - 1024,
+              S3R_ERR_TOO_LARGE, "%s: too many heads or tokens", what);
+  S3R_REQUIRE(known_type(f->type), S3R_ERR_UNSUPPORTED, "%s: types are fp32, bf16 and fp16", what);
+  S3R_REQUIRE(f->kind == S3R_NORM_LAYER || f->kind == S3R_NORM_RMS, S3R_ERR_UNSUPPORTED, "%s: kind %d", what, f->kind);
+  S3R_REQUIRE((f->q_normed || (!f->q_weight && !f->q_bias)) && (f->k_normed || (!f->k_weight && !f->k_bias)), S3R_ERR_SHAPE, "%s: weight and bias belong to a norm", what);
+  S3R_REQUIRE(!(f->q_weight || f->q_bias || f->k_weight || f->k_bias) || known_type(f->param_type), S3R_ERR_UNSUPPORTED, "%s: types are fp32, bf16 and fp16", what);
+  S3R_REQUIRE(f->axes >= 0 && (f->axes == 0 || (f->pairs > 0 && f->rows > 0 && f->pos && f->cos && f->sin)), S3R_ERR_SHAPE, "%s: a rotation needs positions and tables", what);
+  S3R_REQUIRE(f->axes == 0 || (f->axes <= 128 && f->pairs <= 128 && 2 * f->axes * f->pairs <= f->head_dim), S3R_ERR_SHAPE, "%s: %d axes of %d pairs in %d columns", what,
+              f->axes, f->pairs, f->head_dim);
+  S3R_REQUIRE(f->axes == 0 || known_type(f->table_type), S3R_ERR_UNSUPPORTED, "%s: types are fp32, bf16 and fp16", what);
+  const void* params[] = {f->q_weight, f->q_bias, f->k_weight, f->k_bias};
+  for (const void* t : params) S3R_REQUIRE(!t || reinterpret_cast<uintptr_t>(t) % type_bytes(f->param_type) == 0, S3R_ERR_ALIGNMENT, "%s: elements must be aligned", what);
+  S3R_REQUIRE(reinterpret_cast<uintptr_t>(f->qkv) % type_bytes(f->type) == 0 &&
+                  (f->axes == 0 || ((reinterpret_cast<uintptr_t>(f->cos) | reinterpret_cast<uintptr_t>(f->sin)) % type_bytes(f->table_type) == 0 &&
+                                    reinterpret_cast<uintptr_t>(f->pos) % 8 == 0)), S3R_ERR_ALIGNMENT, "%s: elements must be aligned", what);
+  return 0;
+}
+
+// The largest vector that divides pairs, what is not turned, addresses and strides
+static int norm_rope_vector(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
+  const int turned = 2 * f->axes * f->pairs;
+  for (const int v : {8, 4}) {
+    const int bytes = v * type_bytes(f->type) < 16 ? v * type_bytes(f->type) : 16;
+    bool fits = (f->axes == 0 || f->pairs % v == 0) && (f->head_dim - turned) % (2 * v) == 0;
+    for (int i = 0; i < n_pointers; ++i) fits = fits && reinterpret_cast<uintptr_t>(pointers[i]) % bytes == 0;
+    for (int i = 0; i < n_strides; ++i) fits = fits && strides[i] * type_bytes(f->type) % bytes == 0;
+    if (fits) return v;
+  }
+  return 1;
+}
+
+static NrParams norm_rope_params(const s3r_qkv_norm_rope* f) {
+  NrParams p = {};
+  p.qkv = f->qkv;
+  p.cos = f->cos;
+  p.sin = f->sin;
+  p.pos = f->pos;
+  p.weight[0] = f->q_weight;
+  p.weight[1] = f->k_weight;
+  p.bias[0] = f->q_bias;
+  p.bias[1] = f->k_bias;
+  p.stride_b = f->stride_b;
+  p.stride_t = f->stride_t;
+  p.pos_stride_b = f->pos_stride_b;
+  p.pos_stride_t = f->pos_stride_t;
+  p.cos_pitch = f->cos_pitch;
+  p.sin_pitch = f->sin_pitch;
+  p.rows_of_tokens = f->batch * f->tokens;
+  p.tokens = static_cast<int>(f->tokens);
+  p.heads = f->heads;
+  p.kv_heads = f->kv_heads;
+  p.head_dim = f->head_dim;
+  p.kind = f->kind;
+  p.type = f->type;
+  p.param_type = f->param_type;
+  p.table_type = f->table_type;
+  p.axes = f->axes;
+  p.pairs = f->axes ? f->pairs : 0;
+  p.rows = f->rows;
+  p.normed[0] = f->q_normed;
+  p.normed[1] = f->k_normed;
+  p.eps[0] = f->q_eps;
+  p.eps[1] = f->k_eps;
+  p.inverse_dim = 1.f / static_cast<float>(f->head_dim);
+  p.status = device_status_ptr();
+  return p;
+}
+
+}  // namespace s3r
+
+using namespace s3r;
+
+extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
+  if (const int rc = check_norm_rope(f, "s3r_qkv_norm_rope_fwd")) return rc;
+  S3R_REQUIRE(f->q && f->k && f->v, S3R_ERR_NULL, "s3r_qkv_norm_rope_fwd: NULL pointer");
+  for (const void* t : {f->q, f->k, f->v}) S3R_REQUIRE(reinterpret_cast<uintptr_t>(t) % type_bytes(f->type) == 0, S3R_ERR_ALIGNMENT, "s3r_qkv_norm_rope_fwd: elements must be aligned");
+  NrParams p = norm_rope_params(f);
+  S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_qkv_norm_rope_fwd: no status word");
+  p.out[0] = f->q;
+  p.out[1] = f->k;
+  p.out[2] = f->v;
+  const void* pointers[] = {f->qkv, f->q, f->k, f->v};
+  const int64_t strides[] = {f->batch > 1 ? f->stride_b : 0, f->tokens > 1 ? f->stride_t : 0};
+  const NrShape s = norm_rope_shape(norm_rope_vector(f, pointers, 4, strides, 2), f->head_dim);
+  const int64_t per = kNrThreads / s.group, ctas = (p.rows_of_tokens + per - 1) / per;
+  norm_rope_chunks(ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return f->type == S3R_F32 ? pick_norm_rope<4>(p, s, false, static_cast<unsigned>(ctas), st) : pick_norm_rope<2>(p, s, false, static_cast<unsigned>(ctas), st);
+}
+
+// Room for either shape of the grid: the chunks of heads depend on the vectors that addresses allow.
+extern "C" size_t s3r_qkv_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  // chunks of q and k times CTAs along the tokens: at most one more CTA per chunk than 4 per SM in all, and no chunk without a head
+  return static_cast<size_t>(4 * sm_count() + heads + 2 * kv_heads) * 2 * head_dim * sizeof(float);
+}
+
+extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_norm_rope_grad* g, void* stream) {
+  if (const int rc = check_norm_rope(f, "s3r_qkv_norm_rope_bwd")) return rc;
+  S3R_REQUIRE(g && g->d_qkv, S3R_ERR_NULL, "s3r_qkv_norm_rope_bwd: NULL pointer");
+  for (const void* t : {g->dq, g->dk, g->dv, static_cast<const void*>(g->d_qkv)})
+    S3R_REQUIRE(reinterpret_cast<uintptr_t>(t) % type_bytes(f->type) == 0, S3R_ERR_ALIGNMENT, "s3r_qkv_norm_rope_bwd: elements must be aligned");
+  S3R_REQUIRE((f->q_normed || (!g->d_q_weight && !g->d_q_bias)) && (f->k_normed || (!g->d_k_weight && !g->d_k_bias)), S3R_ERR_SHAPE,
+              "s3r_qkv_norm_rope_bwd: weight and bias belong to a norm");
+  const bool sums = g->d_q_weight || g->d_q_bias || g->d_k_weight || g->d_k_bias;
+  const size_t need = s3r_qkv_norm_rope_bwd_workspace_bytes(f->batch, f->tokens, f->heads, f->kv_heads, f->head_dim);
+  S3R_REQUIRE(!sums || known_type(f->param_type), S3R_ERR_UNSUPPORTED, "s3r_qkv_norm_rope_bwd: types are fp32, bf16 and fp16");
+  S3R_REQUIRE(!sums || (g->workspace && g->workspace_bytes >= need && reinterpret_cast<uintptr_t>(g->workspace) % 4 == 0), S3R_ERR_TOO_LARGE,
+              "s3r_qkv_norm_rope_bwd: workspace too small");
+  NrParams p = norm_rope_params(f);
+  S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_qkv_norm_rope_bwd: no status word");
+  const void* d_out[] = {g->dq, g->dk, g->dv};
+  const int64_t* d_strides[] = {g->dq_strides, g->dk_strides, g->dv_strides};
+  const void* pointers[5] = {f->qkv, g->d_qkv};
+  int64_t strides[11] = {f->batch > 1 ? f->stride_b : 0, f->tokens > 1 ? f->stride_t : 0};
+  int np = 2, ns = 2;
+  for (int i = 0; i < 3; ++i) {
+    p.d_out[i] = d_out[i];
+    if (!d_out[i]) continue;
+    pointers[np++] = d_out[i];
+    const int64_t sizes[3] = {f->batch, i == 0 ? f->heads : f->kv_heads, f->tokens};
+    for (int k = 0; k < 3; ++k) p.d_strides[i][k] = strides[ns++] = sizes[k] > 1 ? d_strides[i][k] : 0;
+  }
+  p.d_qkv = g->d_qkv;
+  p.sums = sums ? static_cast<float*>(g->workspace) : nullptr;
+  const NrShape s = norm_rope_shape(norm_rope_vector(f, pointers, np, strides, ns), f->head_dim);
+  const int64_t per = kNrThreads / s.group, token_ctas = (p.rows_of_tokens + per - 1) / per;
+  norm_rope_chunks(token_ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
+  const int chunks = p.q_chunks + 2 * p.kv_chunks;
+  const unsigned ctas = norm_rope_bwd_ctas(token_ctas, chunks);
+  S3R_REQUIRE(!sums || static_cast<size_t>(p.q_chunks + p.kv_chunks) * ctas * 2 * f->head_dim * sizeof(float) <= need, S3R_ERR_TOO_LARGE,
+              "s3r_qkv_norm_rope_bwd: workspace too small");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = f->type == S3R_F32 ? pick_norm_rope<4>(p, s, true, ctas, st) : pick_norm_rope<2>(p, s, true, ctas, st);
+  if (rc || !sums) return rc;
+  NrSums n = {};
+  n.sums = p.sums;
+  n.out[0][0] = g->d_q_weight;
+  n.out[0][1] = g->d_q_bias;
+  n.out[1][0] = g->d_k_weight;
+  n.out[1][1] = g->d_k_bias;
+  n.rows[0] = static_cast<int64_t>(p.q_chunks) * ctas;
+  n.first[1] = n.rows[0];
+  n.rows[1] = static_cast<int64_t>(p.kv_chunks) * ctas;
+  n.head_dim = f->head_dim;
+  n.type = f->param_type;
+  return launch(norm_rope_sums_kernel, dim3(static_cast<unsigned>((2 * f->head_dim + 31) / 32), 2), 1024, 0, st, n);
+}

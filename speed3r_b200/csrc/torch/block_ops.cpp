@@ -5,20 +5,6 @@
 
 namespace {
 
-int type_of(const Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return S3R_F32;
-    case at::kBFloat16: return S3R_BF16;
-    case at::kHalf: return S3R_F16;
-    default: TORCH_CHECK(false, name, " must be fp32, bf16 or fp16, got ", t.scalar_type());
-  }
-}
-void need_cuda(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor: the speed3r_b200 kernels have no CPU path");
-}
-const void* pointer(const optional<Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
-void* pointer(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
-
 // ------------------------------------------------------------------------------------------------
 // residual and norms.  x, y [batch, tokens, channels] contiguous; gate [batch, 1 | tokens, 1] or [batch, 1, channels]
 // ------------------------------------------------------------------------------------------------
@@ -231,9 +217,6 @@ std::tuple<Tensor, Tensor, Tensor> call_norm_int8(const NormInputs& in, bool pos
   S3R_DISPATCHED(residual_norm_int8)(in.x, in.y, in.w, in.b, in.s, in.g, in.pw, in.pb, post, kind, eps, post_eps);
 }
 
-optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
-Tensor value(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
-
 struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w,
                                const optional<Tensor>& b, const optional<Tensor>& s, const optional<Tensor>& g, const optional<Tensor>& pw,
@@ -315,19 +298,6 @@ optional<Tensor> gate_of(const optional<Tensor>& gate, const Tensor& x) {
   const Tensor rows = g.expand(whole).reshape({batch, tokens, channels});
   return channels > 1 && rows.stride(2) != 1 ? rows.contiguous() : rows;
 }
-// parameters of several types are taken in fp32
-void of_one_type(std::initializer_list<optional<Tensor>*> params) {
-  bool mixed = false;
-  const Tensor* first = nullptr;
-  for (const auto* p : params)
-    if (p->has_value()) {
-      if (first && first->scalar_type() != (*p)->scalar_type()) mixed = true;
-      first = &**p;
-    }
-  for (auto* p : params)
-    if (p->has_value()) *p = (mixed ? (*p)->to(at::kFloat) : **p).contiguous();
-}
-
 Tensor in_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 NormInputs norm_inputs(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& b, const optional<Tensor>& s,
                        const optional<Tensor>& gate, const optional<Tensor>& pw, const optional<Tensor>& pb, bool norm, bool post, int64_t kind) {

@@ -17,6 +17,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <tuple>
 #include <vector>
 
@@ -113,6 +114,34 @@ variable_list once(const variable_list& incoming, F&& backward) {
 bool plain(const Tensor& t) {
   return t.is_cuda() && !t.key_set().has(c10::DispatchKey::Python) && !t.key_set().has(c10::DispatchKey::Functionalize) &&
          !c10::impl::dispatch_mode_enabled();
+}
+
+int type_of(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return S3R_F32;
+    case at::kBFloat16: return S3R_BF16;
+    case at::kHalf: return S3R_F16;
+    default: TORCH_CHECK(false, name, " must be fp32, bf16 or fp16, got ", t.scalar_type());
+  }
+}
+void need_cuda(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor: the speed3r_b200 kernels have no CPU path");
+}
+const void* pointer(const optional<Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
+void* pointer(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
+Tensor value(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+// parameters of several types are taken in fp32
+void of_one_type(std::initializer_list<optional<Tensor>*> params) {
+  bool mixed = false;
+  const Tensor* first = nullptr;
+  for (const auto* p : params)
+    if (p->has_value()) {
+      if (first && first->scalar_type() != (*p)->scalar_type()) mixed = true;
+      first = &**p;
+    }
+  for (auto* p : params)
+    if (p->has_value()) *p = (mixed ? (*p)->to(at::kFloat) : **p).contiguous();
 }
 
 // Calls a base operator through the dispatcher (shape functions, tracers and modes see it).

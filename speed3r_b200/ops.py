@@ -135,6 +135,24 @@ def _register_fakes() -> None:
     def _(q, q_scale, weight, weight_scale, bias, out_type):
         return q.new_empty(*q.shape[:-1], weight.shape[0], dtype=out_type)
 
+    @fake("speed3r_b200::linear_fwd")
+    def _(x, weight, bias, scale, residual, act, out_type):
+        return x.new_empty(*x.shape[:-1], weight.shape[0], dtype=out_type)
+
+    @fake("speed3r_b200::linear_bwd")
+    def _(x, weight, bias, scale, dy, act, want):
+        return [t.new_empty(t.shape) if want >> i & 1 else x.new_empty(0) for i, t in enumerate((x, weight, bias, scale))]
+
+    @fake("speed3r_b200::qkv_norm_rope_fwd")
+    def _(qkv, pos, cos, sin, qw, qb, kw, kb, heads, kv_heads, q_normed, k_normed, kind, q_eps, k_eps):
+        B, T, C = qkv.shape
+        return tuple(qkv.new_empty(B, h, T, C // (heads + 2 * kv_heads)) for h in (heads, kv_heads, kv_heads))
+
+    @fake("speed3r_b200::qkv_norm_rope_bwd")
+    def _(qkv, pos, cos, sin, qw, kw, dq, dk, dv, heads, kv_heads, q_normed, k_normed, kind, q_eps, k_eps, want, param_type):
+        d = qkv.shape[2] // (heads + 2 * kv_heads)
+        return [qkv.new_empty(qkv.shape)] + [qkv.new_empty(d if want >> i & 1 else 0, dtype=param_type) for i in range(1, 5)]
+
     @fake("speed3r_b200::norm_of")
     def _(tensors):
         return tensors[0].new_empty((), dtype=torch.float32)
@@ -354,6 +372,47 @@ def int8_linear(q: Tensor, q_scale: Tensor, weight: Tensor, weight_scale: Tensor
     if out_dtype not in NORM_TYPES:
         raise RuntimeError(f"int8_linear: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
     return _ops().int8_linear.default(q, q_scale, weight, weight_scale, bias, out_dtype)
+
+
+_ACTS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
+
+
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Optional[str] = None, residual: Optional[Tensor] = None,
+           scale: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tensor:
+    """A Linear and what follows it (pi3/models/layers/block.py:310-335: activation; LayerScale and residual), in one pass and with gradients::
+
+        residual + act(x @ weight.T + bias) * scale
+
+    ``x [.., K]`` and ``weight [N, K]`` both bf16 or both fp16; sums and all that follows them in fp32, one rounding to ``out_dtype`` (by default
+    ``residual``'s type, else x's).  ``act``: None, ``"gelu"``, ``"gelu_tanh"`` or ``"silu"``.  ``bias`` and ``scale [N]`` and ``residual [.., N]`` are fp32,
+    bf16 or fp16, each of its own type.  The backward computes the sums again rather than keeping them.  Operands whose rows do not begin at
+    multiples of 16 bytes are laid out anew on every call."""
+    if act not in _ACTS:
+        raise RuntimeError(f"linear: act must be None, 'gelu', 'gelu_tanh' or 'silu', got {act!r}")
+    if out_dtype is None:
+        out_dtype = x.dtype if residual is None else residual.dtype
+    if out_dtype not in NORM_TYPES:
+        raise RuntimeError(f"linear: out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
+    return _ops().linear.default(x, weight, bias, scale, residual, _ACTS[act], out_dtype)
+
+
+def qkv_norm_rope(qkv: Tensor, num_heads: int, kv_heads: Optional[int] = None, pos: Optional[Tensor] = None, cos: Optional[Tensor] = None,
+                  sin: Optional[Tensor] = None, q_norm=None, k_norm=None, kind: str = "layer") -> Tuple[Tensor, Tensor, Tensor]:
+    """What stands between the qkv projection and dense attention (pi3/models/layers/attention.py:324-348: split, norm of every head of q and k,
+    rotary embedding), in one pass and with gradients: ``qkv [B, T, (num_heads + 2 * kv_heads) * d]`` -> ``q [B, num_heads, T, d]``, ``k`` and
+    ``v [B, kv_heads, T, d]``, contiguous.  fp32, bf16 or fp16, fp32 inside, one rounding; d even, up to 256.
+
+    ``q_norm`` and ``k_norm`` are ``(weight, bias, eps)``, weight and bias ``[d]`` or None, or None for no norm; ``kind`` as in ``residual_norm``.
+    ``pos [B or 1, T, axes]`` (or ``[T, axes]``) are a token's integer positions, ``cos`` and ``sin [rows, W]`` the tables of sines and cosines: axis
+    a turns the columns ``2 * W * a + i`` and ``2 * W * a + W + i``, i < W, by the angle of table row ``pos[.., a]`` and column i; columns from
+    ``2 * W * axes`` on are not turned.  (Of tables whose halves repeat, as ``RoPE2D`` makes them, hand over the first half.)  A position outside of
+    the tables is clamped and sets a bit of the device's status word."""
+    if kind not in _KINDS:
+        raise RuntimeError(f"qkv_norm_rope: kind must be 'layer' or 'rms', got {kind!r}")
+    qw, qb, q_eps = q_norm if q_norm is not None else (None, None, 0.0)
+    kw, kb, k_eps = k_norm if k_norm is not None else (None, None, 0.0)
+    return _ops().qkv_norm_rope.default(qkv, pos, cos, sin, qw, qb, kw, kb, int(num_heads), int(num_heads if kv_heads is None else kv_heads),
+                                        q_norm is not None, k_norm is not None, _KINDS[kind], float(q_eps), float(k_eps))
 
 
 @torch.no_grad()

@@ -3,488 +3,9 @@
 //   backward  du = dy * scale,  dz = du * act'(z),  d_bias = sum of dz over rows,  d_scale = sum of dy * u over rows;  dx = dz W,  dW = dz^T x
 // z is not kept: where it is needed (an activation's slope, the scale's gradient) the backward makes it again, and dz is the epilogue of that product.
 // The forward then writes nothing but its result, and both sums over rows see z as it was, not rounded to 16 bits.
-#include <climits>
-
-#include "pairs.cuh"
+#include "linear.cuh"
 
 namespace s3r {
-
-// ---------------------------------------------------------------------------------------------------------------------
-// activations
-// ---------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float fast_rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float2 fast_rcp2(float2 x) { return make_float2(fast_rcp(x.x), fast_rcp(x.y)); }
-__device__ __forceinline__ float2 exp2_2(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
-// u = act(z), and its slope.
-// GELU: z Phi(z) with Phi from erfc as Abramowitz and Stegun give it (7.1.26: a polynomial of degree 5 in t = 1 / (1 + p |x|), times exp(-x^2),
-// off by 1.5e-7 at most, so Phi by 7.5e-8): one exponential, which the slope's density shares, one reciprocal and seven packed operations per pair.
-// erff takes about three times as many, and at K = 1024 a tile's products leave 32 issue slots per value.
-// GELU by tanh: z sigmoid(2 sqrt(2 / pi) (z + 0.044715 z^3)), the same function.
-template <bool SLOPE>
-__device__ __forceinline__ float2 activate(float2 z, int act, float2& slope) {
-  if (act == S3R_ACT_GELU) {
-    const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
-    const float2 t = fast_rcp2(ffma2(a, both(0.23164190f), both(1.f)));             // 0.3275911 / sqrt(2)
-    const float2 e = exp2_2(fmul2(fmul2(z, z), both(-0.72134752f)));                // exp(-z^2 / 2)
-    float2 h = both(0.530702715f);                                                  // the halved coefficients
-    h = ffma2(h, t, both(-0.726576014f));
-    h = ffma2(h, t, both(0.710706868f));
-    h = ffma2(h, t, both(-0.142248368f));
-    h = ffma2(h, t, both(0.127414796f));
-    h = fmul2(fmul2(h, t), e);                                                      // Phi(-|z|)
-    const float2 below = make_float2(z.x < 0.f ? h.x : 1.f - h.x, z.y < 0.f ? h.y : 1.f - h.y);
-    if (SLOPE) slope = ffma2(fmul2(z, both(0.398942280f)), e, below);
-    return fmul2(z, below);
-  }
-  if (act == S3R_ACT_NONE) {
-    if (SLOPE) slope = both(1.f);
-    return z;
-  }
-  const float2 q = fmul2(z, z);
-  const float2 arg = act == S3R_ACT_SILU ? fmul2(z, both(-1.44269504f)) : fmul2(z, ffma2(q, both(-0.102943240f), both(-2.30220819f)));
-  const float2 p = fast_rcp2(fadd2(exp2_2(arg), both(1.f)));
-  const float2 u = fmul2(z, p);
-  if (SLOPE) {
-    // the argument's own slope: 1, or 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2)
-    const float2 inner = act == S3R_ACT_SILU ? both(1.f) : ffma2(q, both(0.214064488f), both(1.59576912f));
-    slope = ffma2(fmul2(u, inner), fadd2(both(1.f), make_float2(-p.x, -p.y)), p);
-  }
-  return u;
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// product on tcgen05: persistent CTAs (pairs of them), the contraction in steps of 64 through a ring of TMA copies, the sums of two tiles in
-// tensor memory so that one is written out while the next is summed.  One warp copies, one issues the products, eight take the sums: 32 rows
-// and half of the columns each, four rows and eight columns of every 32 x 32 per lane.
-// Either operand lies with the contraction contiguous ([rows][k]: x, W of the forward, dz of dx) or turned ([k][rows]: W of dx, dz and x of dW);
-// a turned one comes in boxes of 64 rows x 64 steps and is read through the other form of the matrix descriptor.
-// ---------------------------------------------------------------------------------------------------------------------
-constexpr int kLinWarps = 8, kLinThreads = 64 + 32 * kLinWarps, kLinPiece = 4096;       // a warp's piece of the output: 32 rows of 128 bytes
-constexpr int kLinStep = 64;                                                            // elements of the contraction per stage: 128 bytes
-
-struct LinParams {
-  const void *bias, *scale, *residual, *dy;
-  void* out;
-  float *bias_sums, *scale_sums;       // [32-row blocks, N]: sums of dz and of dy * u
-  int64_t M, out_pitch;
-  int N, steps, m_tiles, n_tiles;
-  int bias_type, scale_type, residual_type, dy_type, out_type, act;
-  uint32_t idesc, a_turned, b_turned, copy_out, residual_pairs;      // rows of the residual | of dy in pairs of elements
-  uint32_t* status;
-};
-
-template <int TN, int CTAS>
-struct LinCfg {
-  static constexpr int kABytes = 128 * 128, kBBytes = TN / CTAS * 128, kBytes = kABytes + kBBytes;
-  static constexpr int kStages = 163840 / kBytes > 6 ? 6 : 163840 / kBytes;
-  static constexpr int kOut = kStages * kBytes, kColumns = kOut + kLinWarps * kLinPiece;
-  static constexpr int kSpan = TN / 2 < 64 ? 64 : TN / 2;       // columns of an epilogue warp: whole pieces
-  static constexpr int kSmem = kColumns + kLinWarps * kSpan * 16 + 1024;
-};
-
-struct LinCtl {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained, pause;
-  uint32_t tmem_base, abort_flag;
-};
-
-// kind::f16 with fp32 sums; a_type, b_type: 0 fp16, 1 bf16
-constexpr uint32_t umma_idesc_half(uint32_t M, uint32_t N, uint32_t bf16, uint32_t a_turned, uint32_t b_turned) {
-  return (1u << 4) | (bf16 << 7) | (bf16 << 10) | (a_turned << 15) | (b_turned << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
-}
-// Four k-steps of 16.
-#define S3R_LIN_K4(group)                                                    \
-  asm volatile(                                                              \
-      "{\n\t.reg .pred p, pt;\n\t.reg .b64 a, b;\n\t"                        \
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"                   \
-      "tcgen05.mma.cta_group::" group ".kind::f16 [%0], %1, %2, %3, p;\n\t"  \
-      "add.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t"                         \
-      "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, pt;\n\t"   \
-      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"                           \
-      "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, pt;\n\t"   \
-      "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"                           \
-      "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, pt;\n\t}"  \
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum), "l"(a_step), "l"(b_step) \
-      : "memory")
-template <int CTAS>
-__device__ __forceinline__ void umma_half_k4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accum, uint64_t a_step, uint64_t b_step) {
-  if constexpr (CTAS == 2) S3R_LIN_K4("2");
-  else S3R_LIN_K4("1");
-}
-
-// Two neighbours of a row, of which `n` are there; `pairs`: they begin at a multiple of both.
-__device__ __forceinline__ float2 load_pair(const void* p, int type, int64_t at, int n, bool pairs) {
-  float2 v = make_float2(0.f, 0.f);
-  if (type == S3R_F32) {
-    const float* f = static_cast<const float*>(p) + at;
-    if (pairs && n == 2) return __ldg(reinterpret_cast<const float2*>(f));
-    if (n > 0) v.x = __ldg(f);
-    if (n > 1) v.y = __ldg(f + 1);
-    return v;
-  }
-  const uint16_t* h = static_cast<const uint16_t*>(p) + at;
-  uint32_t w = 0;
-  if (pairs && n == 2) {
-    w = __ldg(reinterpret_cast<const uint32_t*>(h));
-  } else {
-    if (n > 0) w = __ldg(h);
-    if (n > 1) w |= static_cast<uint32_t>(__ldg(h + 1)) << 16;
-  }
-  return type == S3R_BF16 ? make_float2(bf16_lo(w), bf16_hi(w)) : make_float2(half_lo(w), half_hi(w));
-}
-
-// WIDE: the result is fp32.  DZ: out = dz from dy, and sums over rows, in place of the forward's result
-template <int TN, int CTAS, bool WIDE, bool DZ>
-__global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
-                                                             const __grid_constant__ CUtensorMap mo, const __grid_constant__ LinParams p) {
-  using C = LinCfg<TN, CTAS>;
-  extern __shared__ char raw_smem[];
-  __shared__ LinCtl ctl;
-  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = CTAS == 2 ? static_cast<int>(blockIdx.x & 1) : 0;          // a cluster is two consecutive CTAs
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&ctl.full[s], 1);
-      mbar_init(&ctl.empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&ctl.acc_full[s], 1);
-      mbar_init(&ctl.acc_empty[s], CTAS * kLinWarps);
-    }
-    mbar_init(&ctl.drained, 1);
-    mbar_init(&ctl.pause, 1);
-    ctl.abort_flag = 0;
-    mbar_fence_init();
-  }
-  if (warp == 1) {
-    if constexpr (CTAS == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(2 * TN) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      tmem_alloc(&ctl.tmem_base, 2 * TN);
-      tmem_relinquish();
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  sync_pair<CTAS>();
-  tc_fence_after();
-  griddep_wait();
-  griddep_launch();
-  const uint32_t tmem = ctl.tmem_base;
-  volatile uint32_t* abort_flag = &ctl.abort_flag;
-  const int tiles = p.m_tiles * p.n_tiles, steps = p.steps, first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
-  // tile = m * n_tiles + n, walked without a division per tile
-  struct Tile {
-    int m, n;
-  };
-  const Tile begin = {first / p.n_tiles, first % p.n_tiles}, step_by = {stride / p.n_tiles, stride % p.n_tiles};
-  auto advance = [&](Tile& t) {
-    t.m += step_by.m;
-    t.n += step_by.n;
-    if (t.n >= p.n_tiles) t.n -= p.n_tiles, ++t.m;
-  };
-  const uint32_t base = smem_u32(smem);
-
-  if (warp == 0) {
-    int n = 0;                                                     // copies so far
-    bool ok = true;
-    const bool leader = elect_one_sync();
-    Tile at = begin;
-    for (int tile = first; tile < tiles && ok; tile += stride, advance(at)) {
-      const int m0 = (at.m * CTAS + rank) * 128, n0 = at.n * TN + rank * (TN / CTAS);
-      for (int k = 0; k < steps; ++k, ++n) {
-        const int s = n % C::kStages;
-        ok = mbar_wait_warp(&ctl.empty[s], (n / C::kStages & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        if (leader) {
-          const uint32_t bar = first_cta<CTAS>(&ctl.full[s]);      // both CTAs' copies complete the first one's barrier
-          if (rank == 0) mbar_expect_tx(&ctl.full[s], CTAS * C::kBytes);
-          const uint32_t a = base + s * C::kBytes, b = a + C::kABytes;
-          if (!p.a_turned) {
-            tma_load_2d<CTAS>(a, &ma, bar, k * kLinStep, m0);
-          } else {
-            tma_load_2d<CTAS>(a, &ma, bar, m0, k * kLinStep);
-            tma_load_2d<CTAS>(a + 8192, &ma, bar, m0 + 64, k * kLinStep);
-          }
-          if (!p.b_turned) {
-            tma_load_2d<CTAS>(b, &mb, bar, k * kLinStep, n0);
-          } else {
-            tma_load_2d<CTAS>(b, &mb, bar, n0, k * kLinStep);
-            if constexpr (TN / CTAS == 128) tma_load_2d<CTAS>(b + 8192, &mb, bar, n0 + 64, k * kLinStep);
-          }
-        }
-        __syncwarp();
-      }
-    }
-    if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
-      volatile uint32_t dummy = 0;
-      for (int i = n - C::kStages < 0 ? 0 : n - C::kStages; rank == 0 && i < n; ++i) {
-        dummy = 0;
-        mbar_wait(&ctl.full[i % C::kStages], i / C::kStages & 1, &dummy);
-      }
-      dummy = 0;
-      mbar_wait_limit(&ctl.pause, 0, &dummy, 10000000ull);         // the second CTA does not see its own land: 10 ms
-    }
-  } else if (warp == 1) {
-    if (rank == 0) {
-      const bool leader = elect_one_sync();
-      // along a row 32 bytes per k-step; turned: 16 rows of 128 bytes, and the next 64 rows of the operand 8 KB further
-      const uint64_t a_step = p.a_turned ? 128 : 2, b_step = p.b_turned ? 128 : 2;
-      const uint32_t a_far = p.a_turned ? 8192 : 16, b_far = p.b_turned ? 8192 : 16;
-      int n = 0, done = 0;
-      bool ok = true;
-      for (int tile = first; tile < tiles && ok; tile += stride, ++done) {
-        const int buf = done & 1;
-        ok = mbar_wait_warp(&ctl.acc_empty[buf], (done >> 1 & 1) ^ 1, abort_flag);
-        tc_fence_after();
-        for (int k = 0; k < steps && ok; ++k, ++n) {
-          const int s = n % C::kStages;
-          ok = mbar_wait_warp(&ctl.full[s], n / C::kStages & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-            umma_half_k4<CTAS>(tmem + buf * TN, umma_desc_sw128(base + s * C::kBytes, 1024, a_far),
-                               umma_desc_sw128(base + s * C::kBytes + C::kABytes, 1024, b_far), p.idesc, k > 0, a_step, b_step);
-            umma_commit(&ctl.empty[s], Ctas<CTAS>());
-            if (k == steps - 1) umma_commit(&ctl.acc_full[buf], Ctas<CTAS>());
-          }
-          __syncwarp();
-        }
-      }
-      if (!ok) {
-        if (leader) umma_commit(&ctl.drained, Ctas<CTAS>());
-        __syncwarp();
-        volatile uint32_t dummy = 0;
-        mbar_wait(&ctl.drained, 0, &dummy);                        // let issued products drain before tensor memory is freed
-      }
-    }
-  } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;          // lanes 32 * quarter .. of tensor memory; half of the columns
-    char* piece = smem + C::kOut + (warp - 2) * kLinPiece;
-    const uint32_t stage = smem_u32(piece);
-    // scales and biases of its columns, of this tile and the next one
-    float* factors = reinterpret_cast<float*>(smem + C::kColumns) + (warp - 2) * 4 * C::kSpan;
-    constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
-    const int from = half * C::kSpan;
-    constexpr int kMine = C::kSpan / 32;
-    const int r = lane >> 2, c = 2 * (lane & 3);                   // rows r, r + 8, r + 16, r + 24, of every eight columns two from c on
-    const void* other = DZ ? p.dy : p.residual;
-    const int other_type = DZ ? p.dy_type : p.residual_type;
-    auto fetch = [&](int tile, Tile at, float* to) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int col = at.n * TN + from + i * 32 + lane;
-        const bool in = tile < tiles && col < p.N;
-        to[i * 32 + lane] = in && p.scale ? load_one(p.scale, p.scale_type, col) : 1.f;
-        to[C::kSpan + i * 32 + lane] = in && p.bias ? load_one(p.bias, p.bias_type, col) : 0.f;
-      }
-    };
-    Tile at = begin, after = begin;
-    fetch(first, at, factors);
-    int done = 0;
-    bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
-      const int buf = done & 1;
-      const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
-      const int n0 = at.n * TN;
-      const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
-      const float* columns = factors + buf * 2 * C::kSpan;
-      __syncwarp();
-      advance(after);
-      fetch(tile + stride, after, factors + (buf ^ 1) * 2 * C::kSpan);
-      ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      // 32 columns' sums; once they are taken the next 32 are asked for, under no condition, so that their registers have no other writer to
-      // wait for, and are on their way while these are stored.
-      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t v[32];
-      if (from < TN) tmem_ld_32x32(sums, v);
-#pragma unroll
-      for (int g = 0; g < kMine; ++g) {
-        float2 x[4][4], o[4][4];
-        if (other) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int64_t row = m0 + r + 8 * i;
-              const int col = from + g * 32 + 8 * j + c, n = row < p.M && col < width ? min(2, width - col) : 0;
-              o[j][i] = load_pair(other, other_type, row * p.N + n0 + col, n, p.residual_pairs);
-            }
-        }
-        tmem_ld_wait_for(v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 s = *reinterpret_cast<const float2*>(columns + g * 32 + 8 * j + c);
-          const float2 b = *reinterpret_cast<const float2*>(columns + C::kSpan + g * 32 + 8 * j + c);
-          float2 db = both(0.f), ds = both(0.f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
-            const float2 z = fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), b);
-            float2 slope;
-            const float2 u = activate<DZ>(z, p.act, slope);
-            if constexpr (DZ) {
-              x[j][i] = fmul2(fmul2(o[j][i], s), slope);
-              if (m0 + r + 8 * i < p.M) {                          // a row that is not there has dy = 0, but may have any z
-                db = fadd2(db, x[j][i]);
-                ds = ffma2(o[j][i], u, ds);
-              }
-            } else {
-              x[j][i] = other ? ffma2(u, s, o[j][i]) : fmul2(u, s);
-            }
-          }
-          if constexpr (DZ) {
-            if (p.bias_sums || p.scale_sums) {
-#pragma unroll
-              for (int step = 4; step < 32; step *= 2) {
-                db = fadd2(db, make_float2(__shfl_xor_sync(0xffffffffu, db.x, step), __shfl_xor_sync(0xffffffffu, db.y, step)));
-                ds = fadd2(ds, make_float2(__shfl_xor_sync(0xffffffffu, ds.x, step), __shfl_xor_sync(0xffffffffu, ds.y, step)));
-              }
-              const int col = from + g * 32 + 8 * j + c;
-              const int64_t to = (m0 >> 5) * p.N + n0 + col;
-              if (r == 0 && m0 < p.M && col < width) {
-                if (p.bias_sums) p.bias_sums[to] = db.x;
-                if (p.scale_sums) p.scale_sums[to] = ds.x;
-                if (col + 1 < width) {
-                  if (p.bias_sums) p.bias_sums[to + 1] = db.y;
-                  if (p.scale_sums) p.scale_sums[to + 1] = ds.y;
-                }
-              }
-            }
-          }
-        }
-        if (g + 1 < kMine) {
-          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v);
-        } else {                                                   // this warp's sums are in registers
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
-        }
-        if (from + g * 32 < width && p.out) {
-          const bool last = g + 1 == kMine || from + g * 32 + 32 >= width;
-          if (per == 32 || !(g & 1)) {
-            if (lane == 0) bulk_wait_read();                       // the store before has left this piece
-            __syncwarp();
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // row r + 8 i: 128 bytes, its 16-byte chunks swizzled by r
-            char* to = piece + r * 128 + (WIDE ? (((2 * j + (c >> 2)) ^ r) << 4) + (c & 2) * 4 : ((((g & 1) * 4 + j) ^ r) << 4) + c * 2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (WIDE) *reinterpret_cast<float2*>(to + i * 1024) = x[j][i];
-              else *reinterpret_cast<uint32_t*>(to + i * 1024) = p.out_type == S3R_BF16 ? pack_bf16(x[j][i].x, x[j][i].y) : pack_half(x[j][i].x, x[j][i].y);
-            }
-          }
-          if (per == 32 || (g & 1) || last) {
-            const int c0 = from + (per == 32 ? g * 32 : g / 2 * 64);
-            if (p.copy_out) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                if (m0 < p.M) tma_store_2d(&mo, stage, n0 + c0, static_cast<int>(m0));
-                bulk_commit();
-              }
-            } else {
-              __syncwarp();
-              constexpr int kSize = WIDE ? 4 : 2;
-              store_lines<WIDE ? S3R_F32 : S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * kSize, p.out_pitch * kSize, piece,
-                                                     min(per, width - c0), static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
-              __syncwarp();                                        // read before the next piece is written
-            }
-          }
-        }
-      }
-      __syncwarp();                                                // its factors are read
-    }
-    if (lane == 0) bulk_wait_all();
-    if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
-  }
-  tc_fence_before();
-  __syncthreads();
-  sync_pair<CTAS>();                                               // the other CTA's products and arrivals reach this one's memory
-  if (warp == 1) tmem_free<CTAS>(tmem, 2 * TN);
-}
-
-// An operand: `rows` of the result's rows or columns, `k` steps of the contraction; pitch in elements.
-struct LinOperand {
-  const void* data;
-  int64_t pitch;
-  bool turned;
-};
-static int operand_map(CUtensorMap* map, const LinOperand& o, int64_t rows, int64_t k, uint32_t box_rows, bool bf16) {
-  const uint64_t dims[2] = {static_cast<uint64_t>(o.turned ? rows : k), static_cast<uint64_t>(o.turned ? k : rows)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(o.pitch) * 2};
-  const uint32_t box[2] = {64, o.turned ? 64 : box_rows};
-  return make_tensor_map(map, o.data, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
-}
-
-template <int TN, int CTAS, bool WIDE, bool DZ>
-static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, LinParams p, cudaStream_t st) {
-  using C = LinCfg<TN, CTAS>;
-  CUtensorMap ma, mb, mo;
-  if (const int rc = operand_map(&ma, a, p.M, k, 128, bf16)) return rc;
-  if (const int rc = operand_map(&mb, b, p.N, k, TN / CTAS, bf16)) return rc;
-  mo = ma;
-  constexpr int kSize = WIDE ? 4 : 2;
-  p.copy_out = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_pitch * kSize % 16 == 0;
-  if (p.copy_out && p.out) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(p.out_pitch) * kSize};
-    const uint32_t box[2] = {128 / kSize, 32};
-    const CUtensorMapDataType type = WIDE ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.out_type == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (const int rc = make_tensor_map(&mo, p.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
-  }
-  p.idesc = umma_idesc_half(128 * CTAS, TN, bf16, a.turned, b.turned);
-  p.a_turned = a.turned;
-  p.b_turned = b.turned;
-  p.steps = static_cast<int>((k + kLinStep - 1) / kLinStep);
-  p.m_tiles = static_cast<int>((p.M + 128 * CTAS - 1) / (128 * CTAS));
-  p.n_tiles = (p.N + TN - 1) / TN;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles, at_once = sm_count() / CTAS;
-  S3R_REQUIRE(tiles < (1ll << 31) - 1024, S3R_ERR_TOO_LARGE, "s3r_linear: too many tiles");
-  static std::atomic<uint64_t> ready{0};
-  if (attributes_missing(ready)) {
-    S3R_CUDA(cudaFuncSetAttribute(linear_kernel<TN, CTAS, WIDE, DZ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-    attributes_set(ready);
-  }
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(static_cast<unsigned>((tiles < at_once ? tiles : at_once) * CTAS));
-  c.blockDim = dim3(kLinThreads);
-  c.dynamicSmemBytes = C::kSmem;
-  c.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CTAS;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  c.attrs = attr;
-  c.numAttrs = CTAS == 2 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&c, linear_kernel<TN, CTAS, WIDE, DZ>, ma, mb, mo, p), "kernel launch");
-}
-
-// The tile whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a).
-template <bool WIDE, bool DZ>
-static int run_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st) {
-  auto cost = [&](int tn, int ctas) {
-    const int64_t tiles = (p.M + 128 * ctas - 1) / (128 * ctas) * ((p.N + tn - 1) / tn), at_once = sm_count() / ctas;
-    return (tiles + at_once - 1) / at_once * (tn + (ctas == 2 ? 64 : 96));
-  };
-  const int64_t pair_256 = cost(256, 2), pair_128 = cost(128, 2), one_128 = cost(128, 1), one_64 = cost(64, 1);
-  if (p.M > 128 && pair_256 <= pair_128 && pair_256 <= one_128 && pair_256 <= one_64) return launch_linear<256, 2, WIDE, DZ>(a, b, k, bf16, p, st);
-  if (p.M > 128 && pair_128 <= one_128 && pair_128 <= one_64) return launch_linear<128, 2, WIDE, DZ>(a, b, k, bf16, p, st);
-  if (one_128 <= one_64) return launch_linear<128, 1, WIDE, DZ>(a, b, k, bf16, p, st);
-  return launch_linear<64, 1, WIDE, DZ>(a, b, k, bf16, p, st);
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has four output
@@ -567,8 +88,12 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
         const int n = n0 + i;
         const int64_t at = static_cast<int64_t>(m) * p.N + n;
         if (p.bias) total += load_one(p.bias, p.bias_type, n);
-        float2 slope;
-        float v[1] = {activate<false>(both(total), p.act, slope).x};
+        float v[1];
+        with_act(p.act, [&](auto act) {
+          float2 slope;
+          v[0] = activate<decltype(act)::value, false>(both(total), slope).x;
+          return 0;
+        });
         const float s = p.scale ? load_one(p.scale, p.scale_type, n) : 1.f;
         v[0] = p.residual ? __fmaf_rn(v[0], s, load_one(p.residual, p.residual_type, at)) : v[0] * s;
         Raw<1> o;
@@ -702,7 +227,8 @@ static int check_linear(const s3r_linear* f, const char* what) {
                   (!f->residual || at_multiple(f->residual, f->residual_type)), S3R_ERR_ALIGNMENT, "%s: elements must be aligned", what);
   return 0;
 }
-static bool in_pairs(const void* p, int type, int N) { return N % 2 == 0 && reinterpret_cast<uintptr_t>(p) % (2 * type_bytes(type)) == 0; }
+// rows of N elements all begin at multiples of `bytes`
+static bool in_vectors(const void* p, int type, int N, int bytes) { return static_cast<int64_t>(N) * type_bytes(type) % bytes == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 static LinParams linear_params(const s3r_linear* f) {
   LinParams p = {};
@@ -733,15 +259,15 @@ extern "C" int s3r_linear_fwd(const s3r_linear* f, void* stream) {
   }
   LinParams p = linear_params(f);
   S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_linear_fwd: no status word");
-  p.residual = f->residual;
-  p.residual_type = f->residual_type;
-  p.residual_pairs = f->residual && in_pairs(f->residual, f->residual_type, f->N);
+  p.other = f->residual;
+  p.other_type = f->residual_type;
+  p.other_vectors = f->residual && in_vectors(f->residual, f->residual_type, f->N, 16);
   p.out = f->out;
   p.out_pitch = f->N;
   p.out_type = f->out_type;
   const LinOperand a = {f->x, f->x_pitch, false}, b = {f->weight, f->w_pitch, false};
   const bool bf16 = f->type == S3R_BF16;
-  return f->out_type == S3R_F32 ? run_linear<true, false>(a, b, f->K, bf16, p, st) : run_linear<false, false>(a, b, f->K, bf16, p, st);
+  return f->residual ? linear_added(a, b, f->K, bf16, p, st) : f->out_type == S3R_F32 ? linear_wide(a, b, f->K, bf16, p, st) : linear_narrow(a, b, f->K, bf16, p, st);
 }
 
 static int64_t sum_blocks(int64_t M) { return (M + 31) / 32; }
@@ -780,15 +306,15 @@ extern "C" int s3r_linear_bwd(const s3r_linear* f, const s3r_linear_grad* g, voi
   } else {
     LinParams p = linear_params(f);
     S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_linear_bwd: no status word");
-    p.dy = g->dy;
-    p.dy_type = f->out_type;
-    p.residual_pairs = in_pairs(g->dy, f->out_type, f->N);
+    p.other = g->dy;
+    p.other_type = f->out_type;
+    p.other_vectors = in_vectors(g->dy, f->out_type, f->N, 2 * type_bytes(f->out_type));
     p.out = g->dz;
     p.out_pitch = g->dz ? g->dz_pitch : 8;
     p.out_type = f->type;
     p.bias_sums = bias_sums;
     p.scale_sums = scale_sums;
-    rc = run_linear<false, true>({f->x, f->x_pitch, false}, {f->weight, f->w_pitch, false}, f->K, f->type == S3R_BF16, p, st);
+    rc = linear_dz({f->x, f->x_pitch, false}, {f->weight, f->w_pitch, false}, f->K, f->type == S3R_BF16, p, st);
     s.blocks = sum_blocks(f->M);
   }
   if (rc || !sums) return rc;
@@ -815,5 +341,5 @@ extern "C" int s3r_product(const void* a, int64_t a_pitch, int a_turned, const v
   p.out_type = type;
   p.status = device_status_ptr();
   S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_product: no status word");
-  return run_linear<false, false>({a, a_pitch, a_turned != 0}, {b, b_pitch, b_turned != 0}, K, type == S3R_BF16, p, static_cast<cudaStream_t>(stream));
+  return linear_narrow({a, a_pitch, a_turned != 0}, {b, b_pitch, b_turned != 0}, K, type == S3R_BF16, p, static_cast<cudaStream_t>(stream));
 }

@@ -99,20 +99,22 @@ struct LinParams {
   int N, steps, m_tiles, n_tiles;
   int bias_type, scale_type, other_type, out_type, act;
   uint32_t idesc, a_turned, b_turned, copy_out, other_vectors;         // other's rows: in vectors of 16 bytes (the residual), in pairs (dy)
+  uint32_t other_copied;               // dy by TMA
   uint32_t* status;
 };
 
-template <int TN, int CTAS>
+// PIECES: per summing warp
+template <int TN, int CTAS, int PIECES>
 struct LinCfg {
   static constexpr int kABytes = 128 * 128, kBBytes = TN / CTAS * 128, kBytes = kABytes + kBBytes;
-  static constexpr int kStages = 163840 / kBytes > 6 ? 6 : 163840 / kBytes;
-  static constexpr int kOut = kStages * kBytes, kColumns = kOut + kLinWarps * kLinPiece;
+  static constexpr int kRing = 196608 - kLinWarps * PIECES * kLinPiece, kStages = kRing / kBytes > 6 ? 6 : kRing / kBytes;
+  static constexpr int kOut = kStages * kBytes, kColumns = kOut + kLinWarps * PIECES * kLinPiece;
   static constexpr int kSpan = TN / 2 < 64 ? 64 : TN / 2;       // columns of an epilogue warp: whole pieces
   static constexpr int kSmem = kColumns + kLinWarps * kSpan * 8 + 1024;
 };
 
 struct LinCtl {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained, pause;
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drained, pause, piece_full[kLinWarps][2];
   uint32_t tmem_base, abort_flag;
 };
 
@@ -229,6 +231,12 @@ __device__ __forceinline__ void pack_pairs(uint32_t (&x)[WORDS], const float2 (&
   }
 }
 
+// four 8 x 8 matrices of 16-bit elements: lane l has elements 2 (l % 4) and the next of row l / 4, and gives the address of row l % 8 of matrix l / 8
+__device__ __forceinline__ void stsm_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
 // Sums over the eight lanes that share columns, of eight columns each: halves change hands, so that every lane ends with one column, number
 // 8 (lane >> 3) + 2 (lane & 3) + (lane >> 2 & 1) of 32.
 __device__ __forceinline__ float column_sum(const float2 (&d)[4], int lane) {
@@ -245,11 +253,11 @@ __device__ __forceinline__ float column_sum(const float2 (&d)[4], int lane) {
 }
 
 // ACT: the activation, kAnyAct: p.act.  OTHER: type of the residual | of dy, kNoOther: there is none.  WIDE: the result is fp32.
-// DZ: out = dz from dy, and sums over rows, in place of the forward's result
-template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, bool DZ>
+// DZ: 1 out = dz from dy, and its sums over rows, in place of the forward's result; 2 the same with a scale, and the sums for that
+template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
-                                                             const __grid_constant__ CUtensorMap mo, const __grid_constant__ LinParams p) {
-  using C = LinCfg<TN, CTAS>;
+                                                             const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap md, const __grid_constant__ LinParams p) {
+  using C = LinCfg<TN, CTAS, DZ ? 2 : 1>;
   extern __shared__ char raw_smem[];
   __shared__ LinCtl ctl;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -264,6 +272,8 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       mbar_init(&ctl.acc_full[s], 1);
       mbar_init(&ctl.acc_empty[s], CTAS * kLinWarps);
     }
+    if (DZ)
+      for (int s = 0; s < 2 * kLinWarps; ++s) mbar_init(&ctl.piece_full[s / 2][s % 2], 1);
     mbar_init(&ctl.drained, 1);
     mbar_init(&ctl.pause, 1);
     ctl.abort_flag = 0;
@@ -376,13 +386,13 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       }
     }
   } else if (warp >= kLinFirst) {
+   if constexpr (!DZ) {
     const int quarter = warp & 3, half = (warp - kLinFirst) >> 2;  // lanes 32 * quarter .. of tensor memory; half of the columns
     char* piece = smem + C::kOut + (warp - kLinFirst) * kLinPiece;
     float* factors = reinterpret_cast<float*>(smem + C::kColumns) + (warp - kLinFirst) * 2 * C::kSpan;     // scales and biases of its columns
     constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
     const int from = half * C::kSpan;
     constexpr int kMine = C::kSpan / 32;
-    const int r = lane >> 2, c = 2 * (lane & 3);                   // backward: rows r, r + 8, r + 16, r + 24, of every eight columns two from c on
     // What the next tile needs is asked for a tile ahead, and its first part of the residual | of dy; the other parts 32 columns ahead.
     Raw<1> scales[kMine], biases[kMine];
     uint32_t o[OTHER == kNoOther ? 1 : OTHER == S3R_F32 ? 32 : 16];
@@ -400,12 +410,24 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
         if (tile >= tiles) return;
         const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
         const int col = at.n * TN + from + g * 32, end = min(p.N, at.n * TN + min(from + C::kSpan, TN));
-        if constexpr (DZ) load_square<OTHER>(o, p.other, row + r, p.M, p.N, col + c, end, p.other_vectors);
-        else load_row<OTHER>(o, p.other, (row + lane) * p.N + col, row + lane < p.M ? end - col : 0, p.other_vectors);
+        load_row<OTHER>(o, p.other, (row + lane) * p.N + col, row + lane < p.M ? end - col : 0, p.other_vectors);
+      }
+    };
+    // its rows, a lane each, into L2: what is asked for 32 columns ahead would wait for memory longer than those columns take
+    auto soon = [&](int tile, Tile at) {
+      if constexpr (OTHER != kNoOther) {
+        const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + lane;
+        const int col = at.n * TN + from, n = min(p.N, at.n * TN + min(from + C::kSpan, TN)) - col;
+        if (tile >= tiles || row >= p.M) return;
+        const char* first_byte = static_cast<const char*>(p.other) + (row * p.N + col) * type_bytes(OTHER);
+#pragma unroll
+        for (int i = 0; i < C::kSpan * type_bytes(OTHER) / 128; ++i)
+          if (i * (128 / type_bytes(OTHER)) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(first_byte + 128 * i));
       }
     };
     Tile at = begin, after = begin;
     fetch(first, at);
+    soon(first, at);
     ahead(first, at, 0);
     int done = 0;
     bool ok = true;
@@ -426,23 +448,32 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       __syncwarp();
       advance(after);
       fetch(tile + stride, after);
+      soon(tile + stride, after);
       ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      // 32 columns' sums; once they are taken the next 32 are asked for, under no condition, so that their registers have no other writer to
-      // wait for, and are on their way while these are stored.
+      // 32 columns' sums; when they are there the next 32 are asked for, into the other registers, and the last ones free the tile's columns
       const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t v[32];
-      if (from < TN) {
-        if constexpr (DZ) tmem_ld_32x32(sums, v);
-        else tmem_ld32(sums, v);
-      }
-#pragma unroll 1
+      uint32_t two[2][32];
+      auto take = [&](int g) {
+        if (from >= TN) return;
+        tmem_ld32(sums + g * 32, two[g & 1]);
+      };
+      take(0);
+#pragma unroll
       for (int g = 0; g < kMine; ++g) {
         uint32_t x[WIDE ? 32 : 16];                                // as it is stored
         const float *s = factors + g * 32, *b = s + C::kSpan;
+        uint32_t (&v)[32] = two[g & 1];
         tmem_ld_wait_for(v);
-        if constexpr (!DZ) {
+        if (g + 1 < kMine) {
+          take(g + 1);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+        }
+        {
           float2 y[16];
           auto columns = [&](auto act) {
 #pragma unroll
@@ -466,49 +497,9 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
             }
           }
           pack_pairs<WIDE>(x, y, p.out_type);
-        } else {
-          float2 y[16], db[4], ds[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = *reinterpret_cast<const float2*>(s + 8 * j + c), add = *reinterpret_cast<const float2*>(b + 8 * j + c);
-            db[j] = ds[j] = both(0.f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
-              float2 slope;
-              const float2 u = activate<ACT, true>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), add), slope);
-              const float2 dy = other_pair<OTHER>(o, (i * 4 + j) * 2);
-              y[j * 4 + i] = fmul2(fmul2(dy, f), slope);
-              const bool there = m0 + r + 8 * i < p.M;             // a row that is not there has dy = 0, but may have any z
-              db[j] = fadd2(db[j], there ? y[j * 4 + i] : both(0.f));
-              ds[j] = ffma2(dy, there ? u : both(0.f), ds[j]);
-            }
-          }
-          const int col = from + g * 32 + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
-          const int64_t to = (m0 >> 5) * p.N + n0 + col;
-          const bool there = m0 < p.M && col < width;
-          if (p.bias_sums) {
-            const float sum = column_sum(db, lane);
-            if (there) p.bias_sums[to] = sum;
-          }
-          if (p.scale_sums) {
-            const float sum = column_sum(ds, lane);
-            if (there) p.scale_sums[to] = sum;
-          }
-          pack_pairs<WIDE>(x, y, p.out_type);
         }
-        if (g + 1 < kMine) {
-          if (from < TN) {
-            if constexpr (DZ) tmem_ld_32x32(sums + g * 32 + 32, v);
-            else tmem_ld32(sums + g * 32 + 32, v);
-          }
-          ahead(tile, at, g + 1);
-        } else {                                                   // this warp's sums are in registers
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
-          ahead(tile + stride, after, 0);
-        }
+        if (g + 1 < kMine) ahead(tile, at, g + 1);
+        else ahead(tile + stride, after, 0);
         if (from + g * 32 < width && p.out) {
           const int half_piece = WIDE ? 0 : g & 1;
           if (!half_piece) {
@@ -516,17 +507,9 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
             __syncwarp();
           }
           // rows of 128 bytes, their 16-byte chunks swizzled by the row
-          if constexpr (!DZ) {
 #pragma unroll
-            for (int k = 0; k < (WIDE ? 8 : 4); ++k)
-              *reinterpret_cast<uint4*>(piece + swz128(lane, half_piece * 4 + k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-          } else {
-            static_assert(!DZ || !WIDE, "dz has the operands' type");
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(piece + swz128(r + 8 * i, half_piece * 4 + j) + c * 2) = x[j * 4 + i];
-          }
+          for (int k = 0; k < (WIDE ? 8 : 4); ++k)
+            *reinterpret_cast<uint4*>(piece + swz128(lane, half_piece * 4 + k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
           if (WIDE || half_piece || g + 1 == kMine || from + g * 32 + 32 >= width) {
             const int c0 = from + (g - half_piece) * 32;
             if (p.copy_out) {
@@ -549,6 +532,206 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
     }
     if (lane == 0) bulk_wait_all();
     if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
+   } else {
+    const int me = warp - kLinFirst, quarter = warp & 3, from = (me >> 2) * C::kSpan;
+    float* factors = reinterpret_cast<float*>(smem + C::kColumns) + me * 2 * C::kSpan;
+    constexpr int kMine = C::kSpan / 32, kPerTile = C::kSpan / 64;
+    const int r = lane >> 2, c = 2 * (lane & 3);                   // rows r, r + 8, r + 16, r + 24, of every eight columns two from c on
+    // dy of 16 bits comes by TMA, 32 rows x 64 columns into one of two pieces, where dz takes its place and leaves by TMA as well; half a piece
+    // ahead.  In the layout of tensor memory's 16 x 256 bits a lane's elements are those of 8 x 8 matrices.  Other dy is read from memory, fp32
+    // 32 columns ahead.
+    const bool by_copy = OTHER != S3R_F32 && p.other_copied;
+    Raw<1> scales[kMine], biases[kMine];
+    uint32_t o[OTHER == S3R_F32 ? 32 : 16];
+    auto fetch = [&](int tile, Tile at) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int col = at.n * TN + from + i * 32 + lane;
+        const bool in = tile < tiles && col < p.N;
+        if (DZ == 2) load_raw<1>(scales[i], p.scale, p.scale_type, col, in);
+        load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
+      }
+    };
+    auto ahead = [&](int tile, Tile at, int g) {
+      if (OTHER != S3R_F32 || tile >= tiles) return;
+      const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+      load_square<OTHER>(o, p.other, row + r, p.M, p.N, at.n * TN + from + g * 32 + c, min(p.N, at.n * TN + min(from + C::kSpan, TN)), p.other_vectors);
+    };
+    auto soon = [&](int tile, Tile at) {                           // its rows, a lane each, into L2
+      const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + lane;
+      const int col = at.n * TN + from, n = min(p.N, at.n * TN + min(from + C::kSpan, TN)) - col;
+      if (tile >= tiles || row >= p.M) return;
+      const char* first_byte = static_cast<const char*>(p.other) + (row * p.N + col) * type_bytes(OTHER);
+#pragma unroll
+      for (int i = 0; i < C::kSpan * type_bytes(OTHER) / 128; ++i)
+        if (i * (128 / type_bytes(OTHER)) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(first_byte + 128 * i));
+    };
+    auto piece_at = [&](uint32_t q) { return smem + C::kOut + (me * 2 + (q & 1)) * kLinPiece; };
+    // piece h of a tile, number q of this warp's: asked for; pieces without columns are left out everywhere
+    auto has = [&](Tile at, int h) { return from + h * 64 < TN && at.n * TN + from + h * 64 < p.N; };
+    auto ask = [&](Tile at, int h, uint32_t q) {
+      if (lane == 0) {
+        mbar_expect_tx(&ctl.piece_full[me][q & 1], kLinPiece);
+        tma_load_2d<1>(smem_u32(piece_at(q)), &md, smem_u32(&ctl.piece_full[me][q & 1]), at.n * TN + from + h * 64, (at.m * CTAS + rank) * 128 + quarter * 32);
+      }
+    };
+    Tile at = begin, after = begin, asked = begin;                 // asked, asked_tile, asked_piece: the next piece to ask for
+    int asked_tile = first, asked_piece = 0;
+    uint32_t asks = 0, q = 0;
+    auto ask_next = [&] {
+      while (asked_tile < tiles) {
+        const bool there = has(asked, asked_piece);
+        if (there) ask(asked, asked_piece, asks++);
+        if (++asked_piece == kPerTile) {
+          asked_piece = 0;
+          asked_tile += stride;
+          advance(asked);
+        }
+        if (there) return;
+      }
+    };
+    fetch(first, at);
+    soon(first, at);
+    if (by_copy) {
+      ask_next();
+      ask_next();
+    }
+    ahead(first, at, 0);
+    int done = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
+      const int buf = done & 1;
+      const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+      const int n0 = at.n * TN;
+      const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
+      __syncwarp();                                                // the last tile's factors are read
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        float f[1];
+        if (DZ == 2) {
+          unpack<1>(f, scales[i], p.scale_type);
+          factors[i * 32 + lane] = f[0];
+        }
+        unpack<1>(f, biases[i], p.bias_type);
+        factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
+      }
+      __syncwarp();
+      advance(after);
+      fetch(tile + stride, after);
+      soon(tile + stride, after);
+      ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
+      uint32_t v[32];
+      if (from < TN) tmem_ld_32x32(sums, v);
+      const bool whole = m0 + 32 <= p.M;
+#pragma unroll
+      for (int g = 0; g < kMine; ++g) {
+        const bool some = from + g * 32 < width;
+        char* piece = piece_at(q);
+        // matrices (i, j): rows 8 i .. of columns 8 j ..; lane l gives the address of row l % 8 of matrix l / 8
+        auto matrix_row = [&](int j) { return smem_u32(piece + swz128(lane, (g & 1) * 4 + j)); };
+        tmem_ld_wait_for(v);
+        if (OTHER != S3R_F32 && some) {
+          if (by_copy) {
+            if (!(g & 1)) ok = mbar_wait_warp(&ctl.piece_full[me][q & 1], q >> 1 & 1, abort_flag);
+            if (!ok) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ldsm_x4(o[j], o[4 + j], o[8 + j], o[12 + j], matrix_row(j));
+          } else {
+            load_square<OTHER>(o, p.other, m0 + r, p.M, p.N, n0 + from + g * 32 + c, n0 + width, p.other_vectors);
+          }
+        }
+        float2 y[16], db[4], ds[4];
+        const float *s = factors + g * 32, *b = s + C::kSpan;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = *reinterpret_cast<const float2*>(s + 8 * j + c), add = *reinterpret_cast<const float2*>(b + 8 * j + c);
+          ds[j] = both(0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
+            float2 slope;
+            const float2 u = activate<ACT, true>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), add), slope);
+            const float2 dy = other_pair<OTHER>(o, (i * 4 + j) * 2);
+            y[i * 4 + j] = fmul2(DZ == 2 ? fmul2(dy, f) : dy, slope);
+            if (DZ == 2) ds[j] = ffma2(dy, whole || m0 + r + 8 * i < p.M ? u : both(0.f), ds[j]);
+          }
+        }
+        if (!whole) {                                              // a row that is not there has dy = 0, but may have any z
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (m0 + r + 8 * (k >> 2) >= p.M) y[k] = both(0.f);
+        }
+        if (g + 1 < kMine) {
+          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v);
+          ahead(tile, at, g + 1);
+        } else {                                                   // this warp's sums are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+          ahead(tile + stride, after, 0);
+        }
+        const int col = from + g * 32 + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
+        const int64_t to = (m0 >> 5) * p.N + n0 + col;
+        const bool there = m0 < p.M && col < width;
+        if (p.bias_sums) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) db[j] = fadd2(fadd2(y[j], y[4 + j]), fadd2(y[8 + j], y[12 + j]));
+          const float sum = column_sum(db, lane);
+          if (there) p.bias_sums[to] = sum;
+        }
+        if (DZ == 2 && p.scale_sums) {
+          const float sum = column_sum(ds, lane);
+          if (there) p.scale_sums[to] = sum;
+        }
+        if (!some) continue;
+        if (p.out) {
+          if (!(g & 1) && !by_copy) {
+            if (lane == 0) bulk_wait_read_but_one();               // the store before the last has left this piece
+            __syncwarp();
+          }
+          uint32_t x[16];
+          pack_pairs<false>(x, y, p.out_type);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) stsm_x4(matrix_row(j), x[j], x[4 + j], x[8 + j], x[12 + j]);
+        }
+        const bool last = (g & 1) || from + g * 32 + 32 >= width;
+        if (by_copy && (!(g & 1)) && q > 0) {                      // the piece before has left its place: the one behind this one comes there
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+          ask_next();
+        }
+        if (!last) continue;
+        if (p.out) {
+          const int c0 = from + (g & ~1) * 32;
+          if (p.copy_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (m0 < p.M) tma_store_2d(&mo, smem_u32(piece), n0 + c0, static_cast<int>(m0));
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            store_lines<S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * 2, p.out_pitch * 2, piece, min(64, width - c0),
+                                  static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
+          }
+        }
+        ++q;
+      }
+    }
+    if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
+      volatile uint32_t dummy;
+      for (uint32_t i = asks > 2 ? asks - 2 : 0; i < asks; ++i) {
+        dummy = 0;
+        mbar_wait(&ctl.piece_full[me][i & 1], i >> 1 & 1, &dummy);
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
+   }
   }
   tc_fence_before();
   __syncthreads();
@@ -563,13 +746,13 @@ static int operand_map(CUtensorMap* map, const LinOperand& o, int64_t rows, int6
   return make_tensor_map(map, o.data, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
 }
 
-template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, bool DZ>
+template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, LinParams p, cudaStream_t st) {
-  using C = LinCfg<TN, CTAS>;
-  CUtensorMap ma, mb, mo;
+  using C = LinCfg<TN, CTAS, DZ ? 2 : 1>;
+  CUtensorMap ma, mb, mo, md;
   if (const int rc = operand_map(&ma, a, p.M, k, 128, bf16)) return rc;
   if (const int rc = operand_map(&mb, b, p.N, k, TN / CTAS, bf16)) return rc;
-  mo = ma;
+  mo = md = ma;
   constexpr int kSize = WIDE ? 4 : 2;
   p.copy_out = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_pitch * kSize % 16 == 0;
   if (p.copy_out && p.out) {
@@ -577,6 +760,13 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
     const uint32_t box[2] = {128 / kSize, 32};
     const CUtensorMapDataType type = WIDE ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.out_type == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (const int rc = make_tensor_map(&mo, p.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
+  }
+  p.other_copied = DZ && OTHER != S3R_F32 && (reinterpret_cast<uintptr_t>(p.other) & 15) == 0 && p.N % 8 == 0 && (p.copy_out || !p.out);
+  if (p.other_copied) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(p.N) * 2};
+    const uint32_t box[2] = {64, 32};
+    if (const int rc = make_tensor_map(&md, p.other, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       OTHER == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16)) return rc;
   }
   p.idesc = umma_idesc_half(128 * CTAS, TN, bf16, a.turned, b.turned);
   p.a_turned = a.turned;
@@ -604,11 +794,11 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   c.attrs = attr;
   c.numAttrs = CTAS == 2 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&c, linear_kernel<TN, CTAS, ACT, OTHER, WIDE, DZ>, ma, mb, mo, p), "kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&c, linear_kernel<TN, CTAS, ACT, OTHER, WIDE, DZ>, ma, mb, mo, md, p), "kernel launch");
 }
 
 // The tile whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a).
-template <int ACT, int OTHER, bool WIDE, bool DZ>
+template <int ACT, int OTHER, bool WIDE, int DZ>
 static int run_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st) {
   auto cost = [&](int tn, int ctas) {
     const int64_t tiles = (p.M + 128 * ctas - 1) / (128 * ctas) * ((p.N + tn - 1) / tn), at_once = sm_count() / ctas;

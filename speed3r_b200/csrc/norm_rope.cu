@@ -64,32 +64,6 @@ __device__ __forceinline__ void store_vec(const Vec<V, BYTES>& v, void* p, int64
 #pragma unroll
     for (int i = 0; i < V * BYTES / 16; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
 }
-template <int V, int BYTES>
-__device__ __forceinline__ void values(float* f, const Vec<V, BYTES>& v, int type) {
-  if constexpr (BYTES == 4) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(v.w[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const uint32_t w = v.w[k / 2];
-      f[k] = type == S3R_BF16 ? (k & 1 ? bf16_hi(w) : bf16_lo(w)) : (k & 1 ? half_hi(w) : half_lo(w));
-    }
-  }
-}
-template <int V, int BYTES>
-__device__ __forceinline__ void rounded(Vec<V, BYTES>& v, const float* f, int type) {
-  if constexpr (BYTES == 4) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) v.w[k] = __float_as_uint(f[k]);
-  } else if constexpr (V == 1) {
-    v.w[0] = (type == S3R_BF16 ? pack_bf16(f[0], 0.f) : pack_half(f[0], 0.f)) & 0xffffu;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k += 2) v.w[k / 2] = type == S3R_BF16 ? pack_bf16(f[k], f[k + 1]) : pack_half(f[k], f[k + 1]);
-  }
-}
-
 constexpr int kNrThreads = 256;
 
 // Where a thread's E slots lie: columns c0 .. c0 + V and c1 .. c1 + V, the axis that turns them (-1: none), column of the tables.
@@ -115,26 +89,65 @@ __device__ __forceinline__ void group_sum(float (&s)[N]) {
     for (int k = 0; k < N; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
 }
 
-// What a thread keeps of its token and of its columns
+// Values of a slot in packed pairs: H of the first member, H of the second (V = 1: one value each, beside a zero).
+template <int V>
+constexpr int kHalf = V == 1 ? 1 : V / 2;
+template <int V, int BYTES>
+__device__ __forceinline__ void values(float2* f, const Vec<V, BYTES>& v, int type) {
+  if constexpr (V == 1) {
+    f[0] = make_float2(BYTES == 4 ? __uint_as_float(v.w[0]) : type == S3R_BF16 ? bf16_lo(v.w[0]) : half_lo(v.w[0]), 0.f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if constexpr (BYTES == 4) f[k] = make_float2(__uint_as_float(v.w[2 * k]), __uint_as_float(v.w[2 * k + 1]));
+      else f[k] = type == S3R_BF16 ? make_float2(bf16_lo(v.w[k]), bf16_hi(v.w[k])) : make_float2(half_lo(v.w[k]), half_hi(v.w[k]));
+    }
+  }
+}
+template <int V, int BYTES>
+__device__ __forceinline__ void rounded(Vec<V, BYTES>& v, const float2* f, int type) {
+  if constexpr (V == 1) {
+    v.w[0] = BYTES == 4 ? __float_as_uint(f[0].x) : (type == S3R_BF16 ? pack_bf16(f[0].x, 0.f) : pack_half(f[0].x, 0.f)) & 0xffffu;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if constexpr (BYTES == 4) v.w[2 * k] = __float_as_uint(f[k].x), v.w[2 * k + 1] = __float_as_uint(f[k].y);
+      else v.w[k] = type == S3R_BF16 ? pack_bf16(f[k].x, f[k].y) : pack_half(f[k].x, f[k].y);
+    }
+  }
+}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
+
+// What a thread keeps of its columns, in the order of values(): member m of slot e in [e][m]
 template <int V, int E>
 struct Lane {
   Slot slot[E];
   bool on[E];
-  float cos[E][V], sin[E][V], weight[E][2 * V], bias[E][2 * V];
 };
+template <int V, int G, int E>
+__device__ __forceinline__ void place(Lane<V, E>& l, const NrParams& p, int t) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    l.slot[e] = slot_of<V>(t + e * G, p);
+    l.on[e] = (t + e * G) * 2 * V < p.head_dim;
+  }
+}
 template <int V, int E>
-__device__ __forceinline__ void parameters(Lane<V, E>& l, const NrParams& p, int part, bool bias) {
+__device__ __forceinline__ void parameter(float2 (&f)[E][2][kHalf<V>], const Lane<V, E>& l, const void* from, int type, float other) {
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int k = 0; k < 2 * V; ++k) {
-      const int col = (k < V ? l.slot[e].c0 : l.slot[e].c1 - V) + k;
-      l.weight[e][k] = part < 2 && l.on[e] && p.weight[part] ? load_one(p.weight[part], p.param_type, col) : 1.f;
-      l.bias[e][k] = bias && part < 2 && l.on[e] && p.bias[part] ? load_one(p.bias[part], p.param_type, col) : 0.f;
-    }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < kHalf<V>; ++k) {
+        const int col = (m ? l.slot[e].c1 : l.slot[e].c0) + 2 * k;
+        f[e][m][k].x = from && l.on[e] ? load_one(from, type, col) : other;
+        f[e][m][k].y = V > 1 && from && l.on[e] ? load_one(from, type, col + 1) : other;
+      }
 }
 template <int V, int E>
-__device__ __forceinline__ void angles(Lane<V, E>& l, const NrParams& p, int64_t b, int t, bool in) {
+__device__ __forceinline__ void angles(float2 (&c)[E][kHalf<V>], float2 (&s)[E][kHalf<V>], const Lane<V, E>& l, const NrParams& p, int64_t b, int t, bool in) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const bool turned = in && l.on[e] && l.slot[e].axis >= 0;
@@ -144,9 +157,12 @@ __device__ __forceinline__ void angles(Lane<V, E>& l, const NrParams& p, int64_t
       row = row < 0 ? 0 : p.rows - 1;
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      l.cos[e][k] = turned ? load_one(p.cos, p.table_type, row * p.cos_pitch + l.slot[e].column + k) : 1.f;
-      l.sin[e][k] = turned ? load_one(p.sin, p.table_type, row * p.sin_pitch + l.slot[e].column + k) : 0.f;
+    for (int k = 0; k < kHalf<V>; ++k) {
+      const int64_t ci = row * p.cos_pitch + l.slot[e].column + 2 * k, si = row * p.sin_pitch + l.slot[e].column + 2 * k;
+      c[e][k].x = turned ? load_one(p.cos, p.table_type, ci) : 1.f;
+      s[e][k].x = turned ? load_one(p.sin, p.table_type, si) : 0.f;
+      c[e][k].y = V > 1 && turned ? load_one(p.cos, p.table_type, ci + 1) : 1.f;
+      s[e][k].y = V > 1 && turned ? load_one(p.sin, p.table_type, si + 1) : 0.f;
     }
   }
 }
@@ -168,56 +184,64 @@ __device__ __forceinline__ Heads heads_of(int chunk, const NrParams& p) {
 }
 __device__ __forceinline__ int packed_head(const Heads& h, const NrParams& p) { return h.first + (h.part > 0 ? p.heads : 0) + (h.part > 1 ? p.kv_heads : 0); }
 
-// (x - mean) * inverse in place; returns the inverse
+// (x - mean) * inverse in place; returns the inverse.  The variance is that of centred values.
 template <int V, int G, int E>
-__device__ __forceinline__ float normalise(float (&x)[E][2 * V], const Lane<V, E>& l, const NrParams& p, int part) {
+__device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const Lane<V, E>& l, const NrParams& p, float eps) {
   float s[1];
+  float2 t;
   if (p.kind == S3R_NORM_LAYER) {
-    s[0] = 0.f;
+    t = twice(0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int k = 0; k < 2 * V; ++k) s[0] += x[e][k];
+      for (int k = 0; k < kHalf<V>; ++k) t = fadd2(t, fadd2(x[e][0][k], x[e][1][k]));
+    s[0] = t.x + t.y;
     group_sum<G>(s);
     const float mean = s[0] * p.inverse_dim;
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int k = 0; k < 2 * V; ++k) x[e][k] = l.on[e] ? x[e][k] - mean : 0.f;
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int k = 0; k < kHalf<V>; ++k) {
+          const float centre = l.on[e] ? -mean : 0.f;              // columns that are not there stay 0
+          x[e][m][k] = fadd2(x[e][m][k], make_float2(centre, V > 1 ? centre : 0.f));
+        }
   }
-  s[0] = 0.f;
+  t = twice(0.f);
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int k = 0; k < 2 * V; ++k) s[0] = fmaf(x[e][k], x[e][k], s[0]);
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < kHalf<V>; ++k) t = ffma2(x[e][m][k], x[e][m][k], t);
+  s[0] = t.x + t.y;
   group_sum<G>(s);
-  const float inverse = 1.f / sqrtf(s[0] * p.inverse_dim + p.eps[part]);
+  const float inverse = rsqrtf(fmaf(s[0], p.inverse_dim, eps));
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int k = 0; k < 2 * V; ++k) x[e][k] *= inverse;
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < kHalf<V>; ++k) x[e][m][k] = fmul2(x[e][m][k], twice(inverse));
   return inverse;
 }
 
+// Rotation and the norm's weight and bias are one linear map of a pair of normalised values, of which a thread keeps six numbers per token:
+//   out1 = n1 (w1 c) - n2 (w2 s) + (b1 c - b2 s),  out2 = n2 (w2 c) + n1 (w1 s) + (b2 c + b1 s)
 template <int V, int G, int E, int BYTES>
-__global__ void __launch_bounds__(kNrThreads) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
-  constexpr int kTokens = kNrThreads / G, U = V * BYTES * E >= 32 ? 2 : 4;       // heads whose loads are in flight
+__global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
+  constexpr int kTokens = kNrThreads / G, H = kHalf<V>, U = V * BYTES * E >= 32 ? 2 : 4;       // U: heads whose loads are in flight
   griddep_wait();
   griddep_launch();
-  const int t = threadIdx.x % G;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / G, b = token / p.tokens;
   const bool in = token < p.rows_of_tokens;
   const int at = static_cast<int>(token - b * p.tokens);
   const Heads h = heads_of(blockIdx.y, p);
-  const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
   Lane<V, E> l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    l.slot[e] = slot_of<V>(t + e * G, p);
-    l.on[e] = (t + e * G) * 2 * V < p.head_dim;
-  }
-  const int64_t from = b * p.stride_b + at * p.stride_t + static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
+  place<V, G, E>(l, p, threadIdx.x % G);
   const int64_t plane = static_cast<int64_t>(p.tokens) * p.head_dim;
+  const int64_t from = b * p.stride_b + at * p.stride_t + static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
   const int64_t to = (b * (h.part == 0 ? p.heads : p.kv_heads) + h.first) * plane + static_cast<int64_t>(at) * p.head_dim;
   void* out = p.out[h.part];
   Vec<V, BYTES> raw[U][E][2];
@@ -231,58 +255,72 @@ __global__ void __launch_bounds__(kNrThreads) norm_rope_fwd_kernel(const __grid_
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) fetch(u, u);
-  if (h.part < 2) {
-    angles<V, E>(l, p, b, at, in);
-    parameters<V, E>(l, p, h.part, true);
+  if (h.part == 2) {
+    for (int i0 = 0; i0 < h.count; i0 += U)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (in && l.on[e] && i < h.count) {
+            store_vec<V, BYTES>(raw[u][e][0], out, to + i * plane + l.slot[e].c0);
+            store_vec<V, BYTES>(raw[u][e][1], out, to + i * plane + l.slot[e].c1);
+          }
+        fetch(i + U, u);
+      }
+    return;
+  }
+  const bool normed = p.normed[h.part];
+  float2 own[E][2][H], other[E][2][H], add[E][2][H];               // what multiplies a member, its partner, and what is added
+  {
+    float2 c[E][H], s[E][H], w[E][2][H], bias[E][2][H];
+    angles<V, E>(c, s, l, p, b, at, in);
+    parameter<V, E>(w, l, p.weight[h.part], p.param_type, 1.f);
+    parameter<V, E>(bias, l, p.bias[h.part], p.param_type, 0.f);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        own[e][0][k] = fmul2(w[e][0][k], c[e][k]);
+        own[e][1][k] = fmul2(w[e][1][k], c[e][k]);
+        other[e][0][k] = minus(fmul2(w[e][1][k], s[e][k]));
+        other[e][1][k] = fmul2(w[e][0][k], s[e][k]);
+        add[e][0][k] = ffma2(bias[e][0][k], c[e][k], minus(fmul2(bias[e][1][k], s[e][k])));
+        add[e][1][k] = ffma2(bias[e][1][k], c[e][k], fmul2(bias[e][0][k], s[e][k]));
+      }
   }
   for (int i0 = 0; i0 < h.count; i0 += U) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u;
-      if (i >= h.count) break;
-      if (h.part == 2) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (in && l.on[e]) {
-            store_vec<V, BYTES>(raw[u][e][0], out, to + i * plane + l.slot[e].c0);
-            store_vec<V, BYTES>(raw[u][e][1], out, to + i * plane + l.slot[e].c1);
-          }
-        fetch(i + U, u);
-        continue;
-      }
-      float x[E][2 * V];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        values<V, BYTES>(x[e], raw[u][e][0], p.type);
-        values<V, BYTES>(x[e] + V, raw[u][e][1], p.type);
-        if (!(in && l.on[e]))
-#pragma unroll
-          for (int k = 0; k < 2 * V; ++k) x[e][k] = 0.f;
-      }
-      fetch(i + U, u);
-      if (normed) {
-        normalise<V, G, E>(x, l, p, h.part);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-          for (int k = 0; k < 2 * V; ++k) x[e][k] = fmaf(x[e][k], l.weight[e][k], l.bias[e][k]);
-      }
+      float2 x[E][2][H];
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (in && l.on[e]) {
-          if (l.slot[e].axis >= 0)
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-              const float x1 = x[e][k], x2 = x[e][V + k];
-              x[e][k] = x1 * l.cos[e][k] - x2 * l.sin[e][k];
-              x[e][V + k] = x2 * l.cos[e][k] + x1 * l.sin[e][k];
-            }
+        for (int m = 0; m < 2; ++m) {
+          values<V, BYTES>(x[e][m], raw[u][e][m], p.type);
+          if (!l.on[e])
+#pragma unroll
+            for (int k = 0; k < H; ++k) x[e][m][k] = twice(0.f);
+        }
+      fetch(i + U, u);
+      if (normed) normalise<V, G, E>(x, l, p, p.eps[h.part]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float2 y[2][H];
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          y[0][k] = ffma2(x[e][0][k], own[e][0][k], ffma2(x[e][1][k], other[e][0][k], add[e][0][k]));
+          y[1][k] = ffma2(x[e][1][k], own[e][1][k], ffma2(x[e][0][k], other[e][1][k], add[e][1][k]));
+        }
+        if (in && l.on[e] && i < h.count) {
           Vec<V, BYTES> o;
-          rounded<V, BYTES>(o, x[e], p.type);
+          rounded<V, BYTES>(o, y[0], p.type);
           store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c0);
-          rounded<V, BYTES>(o, x[e] + V, p.type);
+          rounded<V, BYTES>(o, y[1], p.type);
           store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c1);
         }
+      }
     }
   }
 }
@@ -290,41 +328,37 @@ __global__ void __launch_bounds__(kNrThreads) norm_rope_fwd_kernel(const __grid_
 // The gradient of a head: turned back, then through the norm as computed again from x.  Sums for weight and bias: over the CTA's tokens and heads in
 // registers, over the warp's groups by shuffles, over warps in shared memory, over CTAs by norm_rope_sums_kernel.
 template <int V, int G, int E, int BYTES>
-__global__ void __launch_bounds__(kNrThreads) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
-  constexpr int kTokens = kNrThreads / G;
+__global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
+  constexpr int kTokens = kNrThreads / G, H = kHalf<V>;
   __shared__ float red[2][kNrThreads / 32][2 * V * G * E];
   griddep_wait();
   griddep_launch();
-  const int t = threadIdx.x % G;
   const Heads h = heads_of(blockIdx.y, p);
   const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
   Lane<V, E> l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    l.slot[e] = slot_of<V>(t + e * G, p);
-    l.on[e] = (t + e * G) * 2 * V < p.head_dim;
-  }
-  if (normed) parameters<V, E>(l, p, h.part, false);
-  float dw[E][2 * V], db[E][2 * V];
+  place<V, G, E>(l, p, threadIdx.x % G);
+  float2 w[E][2][H], dw[E][2][H], db[E][2][H];
+  if (normed) parameter<V, E>(w, l, p.weight[h.part], p.param_type, 1.f);
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int k = 0; k < 2 * V; ++k) dw[e][k] = db[e][k] = 0.f;
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < H; ++k) dw[e][m][k] = db[e][m][k] = twice(0.f);
   const void* d_out = p.d_out[h.part];
-  const int64_t width = static_cast<int64_t>(p.heads + 2 * p.kv_heads) * p.head_dim;
+  const int64_t width = static_cast<int64_t>(p.heads + 2 * p.kv_heads) * p.head_dim, column = static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
+  const int64_t d_head = p.d_strides[h.part][1];
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens; first < p.rows_of_tokens; first += static_cast<int64_t>(gridDim.x) * kTokens) {
     const int64_t token = first + threadIdx.x / G, b = token / p.tokens;
     const bool in = token < p.rows_of_tokens;
     const int at = static_cast<int>(token - b * p.tokens);
-    const int64_t column = static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
     const int64_t from = b * p.stride_b + at * p.stride_t + column, to = token * width + column;
-    const int64_t d_from = b * p.d_strides[h.part][0] + h.first * p.d_strides[h.part][1] + at * p.d_strides[h.part][2], d_head = p.d_strides[h.part][1];
-    if (h.part < 2) angles<V, E>(l, p, b, at, in);
-    for (int i = 0; i < h.count; ++i) {
-      Vec<V, BYTES> raw[E][2], d_raw[E][2];
+    const int64_t d_from = b * p.d_strides[h.part][0] + h.first * d_head + at * p.d_strides[h.part][2];
+    Vec<V, BYTES> raw[E][2], d_raw[E][2];                          // of the next head
+    auto fetch = [&](int i) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (in && l.on[e]) {
+        if (in && l.on[e] && i < h.count) {
           if (d_out) {
             load_vec<V, BYTES>(d_raw[e][0], d_out, d_from + i * d_head + l.slot[e].c0);
             load_vec<V, BYTES>(d_raw[e][1], d_out, d_from + i * d_head + l.slot[e].c1);
@@ -334,58 +368,73 @@ __global__ void __launch_bounds__(kNrThreads) norm_rope_bwd_kernel(const __grid_
             load_vec<V, BYTES>(raw[e][1], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
           }
         }
-      float d[E][2 * V];
+    };
+    fetch(0);
+    float2 c[E][H], s[E][H];
+    if (h.part < 2) angles<V, E>(c, s, l, p, b, at, in);
+    for (int i = 0; i < h.count; ++i) {
+      float2 d[E][2][H], x[E][2][H];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        values<V, BYTES>(d[e], d_raw[e][0], p.type);
-        values<V, BYTES>(d[e] + V, d_raw[e][1], p.type);
-        if (!(in && l.on[e] && d_out))
+      for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int k = 0; k < 2 * V; ++k) d[e][k] = 0.f;
-        if (h.part < 2 && l.slot[e].axis >= 0)
+        for (int m = 0; m < 2; ++m) {
+          values<V, BYTES>(d[e][m], d_raw[e][m], p.type);
+          values<V, BYTES>(x[e][m], raw[e][m], p.type);
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float d1 = d[e][k], d2 = d[e][V + k];
-            d[e][k] = d1 * l.cos[e][k] + d2 * l.sin[e][k];
-            d[e][V + k] = d2 * l.cos[e][k] - d1 * l.sin[e][k];
+          for (int k = 0; k < H; ++k) {
+            if (!(in && l.on[e] && d_out)) d[e][m][k] = twice(0.f);
+            if (!l.on[e]) x[e][m][k] = twice(0.f);
           }
-      }
-      if (normed) {
-        float x[E][2 * V];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          values<V, BYTES>(x[e], raw[e][0], p.type);
-          values<V, BYTES>(x[e] + V, raw[e][1], p.type);
-          if (!(in && l.on[e]))
-#pragma unroll
-            for (int k = 0; k < 2 * V; ++k) x[e][k] = 0.f;
         }
-        const float inverse = normalise<V, G, E>(x, l, p, h.part);
-        float s[2] = {0.f, 0.f};                             // sums of e and e * n, e = d * weight
+      fetch(i + 1);
+      if (h.part < 2)
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int k = 0; k < 2 * V; ++k) {
-            if (in) dw[e][k] = fmaf(d[e][k], x[e][k], dw[e][k]);      // a token that is not there has d = 0, x whatever eps makes of zeros
-            db[e][k] += d[e][k];
-            d[e][k] *= l.weight[e][k];
-            s[0] += d[e][k];
-            s[1] = fmaf(d[e][k], x[e][k], s[1]);
+          for (int k = 0; k < H; ++k) {
+            const float2 d1 = d[e][0][k], d2 = d[e][1][k];
+            d[e][0][k] = ffma2(d1, c[e][k], fmul2(d2, s[e][k]));
+            d[e][1][k] = ffma2(d2, c[e][k], minus(fmul2(d1, s[e][k])));
           }
-        group_sum<G>(s);
-        const float mean = p.kind == S3R_NORM_LAYER ? s[0] * p.inverse_dim : 0.f, along = s[1] * p.inverse_dim;
+      if (normed) {
+        if (!in)                                                   // a token that is not there has d = 0; x is whatever was in the registers
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int k = 0; k < H; ++k) x[e][m][k] = twice(0.f);
+        const float inverse = normalise<V, G, E>(x, l, p, in ? p.eps[h.part] : 1.f);
+        float2 t0 = twice(0.f), t1 = twice(0.f);                   // sums of e and of e n, e = d * weight
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int k = 0; k < 2 * V; ++k) d[e][k] = inverse * (d[e][k] - mean - x[e][k] * along);
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+              dw[e][m][k] = ffma2(d[e][m][k], x[e][m][k], dw[e][m][k]);
+              db[e][m][k] = fadd2(db[e][m][k], d[e][m][k]);
+              d[e][m][k] = fmul2(d[e][m][k], w[e][m][k]);
+              t0 = fadd2(t0, d[e][m][k]);
+              t1 = ffma2(d[e][m][k], x[e][m][k], t1);
+            }
+        float sums[2] = {t0.x + t0.y, t1.x + t1.y};
+        group_sum<G>(sums);
+        const float mean = p.kind == S3R_NORM_LAYER ? -sums[0] * p.inverse_dim * inverse : 0.f, along = -sums[1] * p.inverse_dim * inverse;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < H; ++k) d[e][m][k] = ffma2(d[e][m][k], twice(inverse), ffma2(x[e][m][k], twice(along), twice(mean)));
       }
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (in && l.on[e]) {
           Vec<V, BYTES> o;
-          rounded<V, BYTES>(o, d[e], p.type);
+          rounded<V, BYTES>(o, d[e][0], p.type);
           store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
-          rounded<V, BYTES>(o, d[e] + V, p.type);
+          rounded<V, BYTES>(o, d[e][1], p.type);
           store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
         }
     }
@@ -394,22 +443,24 @@ __global__ void __launch_bounds__(kNrThreads) norm_rope_bwd_kernel(const __grid_
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int k = 0; k < 2 * V; ++k)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int o = 16; o >= G; o >>= 1) {
-        dw[e][k] += __shfl_xor_sync(0xffffffffu, dw[e][k], o);
-        db[e][k] += __shfl_xor_sync(0xffffffffu, db[e][k], o);
-      }
-  if ((threadIdx.x & 31) < G)
+      for (int k = 0; k < H; ++k) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (l.on[e])
-#pragma unroll
-        for (int k = 0; k < 2 * V; ++k) {
-          const int col = (k < V ? l.slot[e].c0 : l.slot[e].c1 - V) + k;
-          red[0][threadIdx.x >> 5][col] = dw[e][k];
-          red[1][threadIdx.x >> 5][col] = db[e][k];
+        for (int o = 16; o >= G; o >>= 1) {
+          dw[e][m][k] = fadd2(dw[e][m][k], make_float2(__shfl_xor_sync(0xffffffffu, dw[e][m][k].x, o), __shfl_xor_sync(0xffffffffu, dw[e][m][k].y, o)));
+          db[e][m][k] = fadd2(db[e][m][k], make_float2(__shfl_xor_sync(0xffffffffu, db[e][m][k].x, o), __shfl_xor_sync(0xffffffffu, db[e][m][k].y, o)));
         }
+        if ((threadIdx.x & 31) < G && l.on[e]) {
+          const int col = (m ? l.slot[e].c1 : l.slot[e].c0) + 2 * k;
+          red[0][threadIdx.x >> 5][col] = dw[e][m][k].x;
+          red[1][threadIdx.x >> 5][col] = db[e][m][k].x;
+          if (V > 1) {
+            red[0][threadIdx.x >> 5][col + 1] = dw[e][m][k].y;
+            red[1][threadIdx.x >> 5][col + 1] = db[e][m][k].y;
+          }
+        }
+      }
   __syncthreads();
   float* to = p.sums + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * p.head_dim;
   for (int c = threadIdx.x; c < 2 * p.head_dim; c += kNrThreads) {
@@ -454,7 +505,9 @@ __global__ void __launch_bounds__(1024) norm_rope_sums_kernel(const __grid_const
 template <int V, int G, int E, int BYTES>
 static int run_norm_rope(const NrParams& p, bool backward, unsigned ctas, cudaStream_t st) {
   const dim3 grid(ctas, static_cast<unsigned>(p.q_chunks + 2 * p.kv_chunks));
-  if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+  if constexpr (V < 8) {
+    if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+  }
   return launch(norm_rope_fwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
 }
 // Threads of a head: as many as it has pairs of vectors, a power of two.
@@ -464,7 +517,7 @@ struct NrShape {
 static NrShape norm_rope_shape(int vector, int head_dim) {
   const int slots = head_dim / (2 * vector);
   if (vector == 8) return {8, slots <= 2 ? 2 : slots <= 4 ? 4 : slots <= 8 ? 8 : 16};
-  if (vector == 4) return {4, slots <= 8 ? 8 : 32};
+  if (vector == 4) return {4, slots <= 8 ? 8 : slots <= 16 ? 16 : 32};
   return {1, 32};
 }
 template <int BYTES>
@@ -474,6 +527,7 @@ static int pick_norm_rope(const NrParams& p, NrShape s, bool backward, unsigned 
   if (s.vector == 8 && s.group == 8) return run_norm_rope<8, 8, 1, BYTES>(p, backward, ctas, st);
   if (s.vector == 8) return run_norm_rope<8, 16, 1, BYTES>(p, backward, ctas, st);
   if (s.vector == 4 && s.group == 8) return run_norm_rope<4, 8, 1, BYTES>(p, backward, ctas, st);
+  if (s.vector == 4 && s.group == 16) return run_norm_rope<4, 16, 1, BYTES>(p, backward, ctas, st);
   if (s.vector == 4) return run_norm_rope<4, 32, 1, BYTES>(p, backward, ctas, st);
   return run_norm_rope<1, 32, 4, BYTES>(p, backward, ctas, st);
 }
@@ -518,10 +572,10 @@ static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
   return 0;
 }
 
-// The largest vector that divides pairs, what is not turned, addresses and strides
-static int norm_rope_vector(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
+// The largest vector, up to `most`, that divides pairs, what is not turned, addresses and strides
+static int norm_rope_vector(const s3r_qkv_norm_rope* f, int most, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
   const int turned = 2 * f->axes * f->pairs;
-  for (const int v : {8, 4}) {
+  for (int v = most; v >= 4; v /= 2) {
     const int bytes = v * type_bytes(f->type) < 16 ? v * type_bytes(f->type) : 16;
     bool fits = (f->axes == 0 || f->pairs % v == 0) && (f->head_dim - turned) % (2 * v) == 0;
     for (int i = 0; i < n_pointers; ++i) fits = fits && reinterpret_cast<uintptr_t>(pointers[i]) % bytes == 0;
@@ -583,7 +637,7 @@ extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
   p.out[2] = f->v;
   const void* pointers[] = {f->qkv, f->q, f->k, f->v};
   const int64_t strides[] = {f->batch > 1 ? f->stride_b : 0, f->tokens > 1 ? f->stride_t : 0};
-  const NrShape s = norm_rope_shape(norm_rope_vector(f, pointers, 4, strides, 2), f->head_dim);
+  const NrShape s = norm_rope_shape(norm_rope_vector(f, 8, pointers, 4, strides, 2), f->head_dim);
   const int64_t per = kNrThreads / s.group, ctas = (p.rows_of_tokens + per - 1) / per;
   norm_rope_chunks(ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -625,7 +679,7 @@ extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_n
   }
   p.d_qkv = g->d_qkv;
   p.sums = sums ? static_cast<float*>(g->workspace) : nullptr;
-  const NrShape s = norm_rope_shape(norm_rope_vector(f, pointers, np, strides, ns), f->head_dim);
+  const NrShape s = norm_rope_shape(norm_rope_vector(f, 4, pointers, np, strides, ns), f->head_dim);
   const int64_t per = kNrThreads / s.group, token_ctas = (p.rows_of_tokens + per - 1) / per;
   norm_rope_chunks(token_ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   const int chunks = p.q_chunks + 2 * p.kv_chunks;

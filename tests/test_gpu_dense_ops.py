@@ -438,7 +438,9 @@ def test_qkv_that_lies_elsewhere():
         view.copy_(c.qkv)
         view.requires_grad_(False)
         got = ops.qkv_norm_rope(view, 4, 2, c.pos, c.cos, c.sin, *c.norms)
-        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        c.check(got)
+        # at multiples of 16 bytes in the same vectors, whose sums have the same order; elsewhere in another, within the bounds of check()
+        assert first == 5 or all(torch.equal(a, b) for a, b in zip(got, want))
     turned = c.qkv.permute(2, 1, 0).contiguous().permute(2, 1, 0)
     assert all(torch.equal(a, b) for a, b in zip(ops.qkv_norm_rope(turned, 4, 2, c.pos, c.cos, c.sin, *c.norms), want))
     twice = torch.cat((c.cos, c.cos), 1), torch.cat((c.sin, c.sin), 1)          # as RoPE2D keeps them

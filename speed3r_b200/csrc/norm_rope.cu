@@ -7,6 +7,9 @@
 // Columns that are not turned are taken as two neighbouring vectors.  A group of G threads stays with one token and walks over heads, so that the
 // token's sines and cosines, the parameters and the sums over rows stay in registers; the groups of a warp have neighbouring tokens, whose
 // results lie one behind the other.
+// Memory is read and written by whole rows: the heads of a warp's tokens come by cp.async, neighbouring lanes neighbouring chunks, several heads
+// ahead, and results leave the same way through shared memory.  A thread's own vectors copied by itself are pieces of 32 bytes, and took 150 us
+// where rows take less; in registers, four heads ahead, 173 (64 512 tokens of 16 heads of 64 in bf16).
 #include <type_traits>
 
 #include "rows.cuh"
@@ -23,7 +26,8 @@ struct NrParams {
   void* d_qkv;
   float* sums;                         // [head chunks of q, then of k][CTAs of a chunk][weight, bias][head_dim]
   int64_t stride_b, stride_t, pos_stride_b, pos_stride_t, cos_pitch, sin_pitch, rows_of_tokens;
-  int tokens, heads, kv_heads, head_dim, kind, type, param_type, table_type, axes, pairs, rows;
+  uint32_t tokens;
+  int heads, kv_heads, head_dim, kind, type, param_type, table_type, axes, pairs, rows;
   int normed[2];
   float eps[2], inverse_dim;
   int per_chunk, q_chunks, kv_chunks;
@@ -37,34 +41,72 @@ struct Vec {
   uint32_t w[kWords];
 };
 template <int V, int BYTES>
-__device__ __forceinline__ void load_vec(Vec<V, BYTES>& v, const void* p, int64_t at) {
-  const char* from = static_cast<const char*>(p) + at * BYTES;
+__device__ __forceinline__ void take_vec(Vec<V, BYTES>& v, uint32_t at) {
   if constexpr (V * BYTES == 2) {
-    v.w[0] = __ldg(reinterpret_cast<const uint16_t*>(from));
+    uint16_t h;
+    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
+    v.w[0] = h;
   } else if constexpr (V * BYTES == 4) {
-    v.w[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v.w[0]) : "r"(at) : "memory");
   } else if constexpr (V * BYTES == 8) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(from));
-    v.w[0] = u.x, v.w[1] = u.y;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.w[0]), "=r"(v.w[1]) : "r"(at) : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < V * BYTES / 16; ++i) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(from) + i);
-      v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+    for (int k = 0; k < V * BYTES / 16; ++k) {
+      const uint4 u = lds128(at + 16 * k);
+      v.w[4 * k] = u.x, v.w[4 * k + 1] = u.y, v.w[4 * k + 2] = u.z, v.w[4 * k + 3] = u.w;
     }
   }
 }
 template <int V, int BYTES>
-__device__ __forceinline__ void store_vec(const Vec<V, BYTES>& v, void* p, int64_t at) {
-  char* to = static_cast<char*>(p) + at * BYTES;
-  if constexpr (V * BYTES == 2) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(v.w[0]);
-  else if constexpr (V * BYTES == 4) *reinterpret_cast<uint32_t*>(to) = v.w[0];
-  else if constexpr (V * BYTES == 8) *reinterpret_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
+__device__ __forceinline__ void put_vec(const Vec<V, BYTES>& v, uint32_t at) {
+  if constexpr (V * BYTES == 2) asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(v.w[0])) : "memory");
+  else if constexpr (V * BYTES == 4) sts32(at, v.w[0]);
+  else if constexpr (V * BYTES == 8) sts64(at, v.w[0], v.w[1]);
   else
 #pragma unroll
-    for (int i = 0; i < V * BYTES / 16; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
+    for (int k = 0; k < V * BYTES / 16; ++k) sts128(at + 16 * k, v.w[4 * k], v.w[4 * k + 1], v.w[4 * k + 2], v.w[4 * k + 3]);
 }
-constexpr int kNrThreads = 256;
+
+constexpr int kNrThreads = 128, kNrWarps = kNrThreads / 32;
+
+// One head of a warp's tokens: rows of a constant pitch, 16 bytes longer than the longest, so that rows begin in different banks.
+// CB: bytes that a lane copies at a time; chunk n of a lane is number 32 n + lane, row by row.
+template <int V, int G, int E, int BYTES, int CB, int INPUTS>
+struct Tile {
+  static constexpr int kZeros = V * BYTES < 16 ? 16 : V * BYTES;       // behind the tiles: what lanes without columns read
+  static constexpr int kRows = 32 / G, kPitch = 2 * V * G * E * BYTES + 16, kBytes = kRows * kPitch;
+  static constexpr int kChunks = kRows * (kPitch - 16) / (32 * CB) < 1 ? 1 : kRows * (kPitch - 16) / (32 * CB);
+  static constexpr int kAhead = 4, kSmem = kNrWarps * kBytes * (kAhead * INPUTS + 1) + kZeros;
+  struct Chunk {
+    int row, byte;           // byte: in the row
+    uint32_t at;             // in the tile
+    bool in;
+  };
+  static __device__ __forceinline__ Chunk chunk(int n, int lane, int row_bytes) {
+    const int per = row_bytes / CB, i = 32 * n + lane, row = i / per, byte = (i - row * per) * CB;
+    return {row, byte, static_cast<uint32_t>(row * kPitch + byte), row < kRows};
+  }
+  static __device__ __forceinline__ void ask(uint32_t to, const char* from) {
+    if constexpr (CB == 16) {
+      cp_async16(to, from);
+    } else if constexpr (CB == 8) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+    } else if constexpr (CB == 4) {
+      cp_async4(to, from);
+    } else {
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(__ldg(reinterpret_cast<const uint16_t*>(from))) : "memory");
+    }
+  }
+  static __device__ __forceinline__ void leave(char* to, uint32_t from) {
+    Vec<CB / 2, 2> v;
+    take_vec<CB / 2, 2>(v, from);
+    if constexpr (CB == 16) *reinterpret_cast<uint4*>(to) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    else if constexpr (CB == 8) *reinterpret_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
+    else if constexpr (CB == 4) *reinterpret_cast<uint32_t*>(to) = v.w[0];
+    else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(v.w[0]);
+  }
+};
 
 // Where a thread's E slots lie: columns c0 .. c0 + V and c1 .. c1 + V, the axis that turns them (-1: none), column of the tables.
 struct Slot {
@@ -124,6 +166,7 @@ template <int V, int E>
 struct Lane {
   Slot slot[E];
   bool on[E];
+  float share[E];        // -1 / head_dim, 0 for columns that are not there, which stay 0 when the mean is taken off
 };
 template <int V, int G, int E>
 __device__ __forceinline__ void place(Lane<V, E>& l, const NrParams& p, int t) {
@@ -131,6 +174,7 @@ __device__ __forceinline__ void place(Lane<V, E>& l, const NrParams& p, int t) {
   for (int e = 0; e < E; ++e) {
     l.slot[e] = slot_of<V>(t + e * G, p);
     l.on[e] = (t + e * G) * 2 * V < p.head_dim;
+    l.share[e] = l.on[e] ? -p.inverse_dim : 0.f;
   }
 }
 template <int V, int E>
@@ -197,15 +241,16 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
       for (int k = 0; k < kHalf<V>; ++k) t = fadd2(t, fadd2(x[e][0][k], x[e][1][k]));
     s[0] = t.x + t.y;
     group_sum<G>(s);
-    const float mean = s[0] * p.inverse_dim;
+    float minus_mean[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) minus_mean[e] = s[0] * l.share[e];
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int k = 0; k < kHalf<V>; ++k) {
-          const float centre = l.on[e] ? -mean : 0.f;              // columns that are not there stay 0
-          x[e][m][k] = fadd2(x[e][m][k], make_float2(centre, V > 1 ? centre : 0.f));
+          x[e][m][k] = fadd2(x[e][m][k], make_float2(minus_mean[e], V > 1 ? minus_mean[e] : 0.f));
         }
   }
   t = twice(0.f);
@@ -229,45 +274,67 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
 
 // Rotation and the norm's weight and bias are one linear map of a pair of normalised values, of which a thread keeps six numbers per token:
 //   out1 = n1 (w1 c) - n2 (w2 s) + (b1 c - b2 s),  out2 = n2 (w2 c) + n1 (w1 s) + (b2 c + b1 s)
-template <int V, int G, int E, int BYTES>
-__global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
-  constexpr int kTokens = kNrThreads / G, H = kHalf<V>, U = V * BYTES * E >= 32 ? 2 : 4;       // U: heads whose loads are in flight
+template <int V, int G, int E, int BYTES, int CB>
+__global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 6) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
+  using T = Tile<V, G, E, BYTES, CB, 1>;
+  constexpr int H = kHalf<V>, kChunks = T::kChunks;
+  extern __shared__ __align__(16) char smem[];
   griddep_wait();
   griddep_launch();
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / G, b = token / p.tokens;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kNrWarps + warp) * T::kRows;       // token of the warp's first row
+  const int64_t token = first + lane / G, b = static_cast<uint32_t>(token) / p.tokens;
   const bool in = token < p.rows_of_tokens;
   const int at = static_cast<int>(token - b * p.tokens);
   const Heads h = heads_of(blockIdx.y, p);
   Lane<V, E> l;
-  place<V, G, E>(l, p, threadIdx.x % G);
-  const int64_t plane = static_cast<int64_t>(p.tokens) * p.head_dim;
-  const int64_t from = b * p.stride_b + at * p.stride_t + static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
-  const int64_t to = (b * (h.part == 0 ? p.heads : p.kv_heads) + h.first) * plane + static_cast<int64_t>(at) * p.head_dim;
-  void* out = p.out[h.part];
-  Vec<V, BYTES> raw[U][E][2];
-  auto fetch = [&](int i, int u) {
+  place<V, G, E>(l, p, lane % G);
+  const int64_t row_bytes = p.head_dim * BYTES, plane = p.tokens * row_bytes;
+  const uint32_t ring = smem_u32(smem) + warp * T::kBytes * (T::kAhead + 1), last = ring + T::kAhead * T::kBytes;
+  const char* from[kChunks];
+  char* to[kChunks];
+  uint32_t place_of[kChunks];
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (in && l.on[e] && i < h.count) {
-        load_vec<V, BYTES>(raw[u][e][0], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
-        load_vec<V, BYTES>(raw[u][e][1], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
+  for (int n = 0; n < kChunks; ++n) {
+    const auto c = T::chunk(n, lane, static_cast<int>(row_bytes));
+    const uint32_t tok = static_cast<uint32_t>(first) + c.row, cb = tok / p.tokens, ct = tok - cb * p.tokens;       // fewer than 2^31
+    const bool there = c.in && tok < p.rows_of_tokens;
+    from[n] = there ? static_cast<const char*>(p.qkv) + (static_cast<int64_t>(cb) * p.stride_b + static_cast<int64_t>(ct) * p.stride_t) * BYTES + packed_head(h, p) * row_bytes + c.byte : nullptr;
+    to[n] = static_cast<char*>(p.out[h.part]) + (static_cast<int64_t>(cb) * (h.part == 0 ? p.heads : p.kv_heads) + h.first) * plane + ct * row_bytes + c.byte;
+    place_of[n] = c.at;
+  }
+  int left = h.count;                                              // heads that are still to be asked for
+  uint32_t free = 0, full = 0;                                     // places in the ring
+  auto next = [&](uint32_t& place) { place = place == (T::kAhead - 1) * T::kBytes ? 0 : place + T::kBytes; };
+  auto fetch = [&] {
+    if (left > 0)
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n)
+        if (from[n]) {
+          T::ask(ring + free + place_of[n], from[n]);
+          from[n] += row_bytes;
+        }
+    --left;
+    next(free);
+    cp_async_commit();
+  };
+  auto leave = [&](uint32_t tile) {
+#pragma unroll
+    for (int n = 0; n < kChunks; ++n)
+      if (from[n]) {
+        T::leave(to[n], tile + place_of[n]);
+        to[n] += plane;
       }
   };
 #pragma unroll
-  for (int u = 0; u < U; ++u) fetch(u, u);
+  for (int u = 0; u < T::kAhead; ++u) fetch();
   if (h.part == 2) {
-    for (int i0 = 0; i0 < h.count; i0 += U)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (in && l.on[e] && i < h.count) {
-            store_vec<V, BYTES>(raw[u][e][0], out, to + i * plane + l.slot[e].c0);
-            store_vec<V, BYTES>(raw[u][e][1], out, to + i * plane + l.slot[e].c1);
-          }
-        fetch(i + U, u);
-      }
+    for (int i = 0; i < h.count; ++i) {
+      cp_async_wait<T::kAhead - 1>();
+      leave(ring + full);
+      next(full);
+      fetch();
+    }
     return;
   }
   const bool normed = p.normed[h.part];
@@ -289,54 +356,68 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_fwd_kern
         add[e][1][k] = ffma2(bias[e][1][k], c[e][k], fmul2(bias[e][0][k], s[e][k]));
       }
   }
-  for (int i0 = 0; i0 < h.count; i0 += U) {
+  const uint32_t mine = lane / G * T::kPitch, zeros = smem_u32(smem) + T::kSmem - T::kZeros;
+  uint32_t in_tile[E][2];                                          // its vectors in the first place; without columns: the zeros, whatever the place
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      float2 x[E][2][H];
+  for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int e = 0; e < E; ++e)
+    for (int m = 0; m < 2; ++m) in_tile[e][m] = l.on[e] ? ring + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES : zeros;
+  if (threadIdx.x < T::kZeros / 4) sts32(zeros + 4 * threadIdx.x, 0);
+  __syncthreads();
+  const float eps = p.eps[h.part];
+#pragma unroll 1
+  for (int i = 0; i < h.count; ++i) {
+    cp_async_wait<T::kAhead - 1>();
+    __syncwarp();                                                  // every lane's copies are there, and the last head's results have left
+    float2 x[E][2][H];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        Vec<V, BYTES> raw;
+        take_vec<V, BYTES>(raw, in_tile[e][m] + (l.on[e] ? full : 0));
+        values<V, BYTES>(x[e][m], raw, p.type);
+      }
+    next(full);
+    __syncwarp();
+    fetch();
+    if (normed) normalise<V, G, E>(x, l, p, eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float2 y[2][H];
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        y[0][k] = ffma2(x[e][0][k], own[e][0][k], ffma2(x[e][1][k], other[e][0][k], add[e][0][k]));
+        y[1][k] = ffma2(x[e][1][k], own[e][1][k], ffma2(x[e][0][k], other[e][1][k], add[e][1][k]));
+      }
+      if (l.on[e])
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          values<V, BYTES>(x[e][m], raw[u][e][m], p.type);
-          if (!l.on[e])
-#pragma unroll
-            for (int k = 0; k < H; ++k) x[e][m][k] = twice(0.f);
-        }
-      fetch(i + U, u);
-      if (normed) normalise<V, G, E>(x, l, p, p.eps[h.part]);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float2 y[2][H];
-#pragma unroll
-        for (int k = 0; k < H; ++k) {
-          y[0][k] = ffma2(x[e][0][k], own[e][0][k], ffma2(x[e][1][k], other[e][0][k], add[e][0][k]));
-          y[1][k] = ffma2(x[e][1][k], own[e][1][k], ffma2(x[e][0][k], other[e][1][k], add[e][1][k]));
-        }
-        if (in && l.on[e] && i < h.count) {
           Vec<V, BYTES> o;
-          rounded<V, BYTES>(o, y[0], p.type);
-          store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c0);
-          rounded<V, BYTES>(o, y[1], p.type);
-          store_vec<V, BYTES>(o, out, to + i * plane + l.slot[e].c1);
+          rounded<V, BYTES>(o, y[m], p.type);
+          put_vec<V, BYTES>(o, last + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES);
         }
-      }
     }
+    __syncwarp();
+    leave(last);
   }
 }
 
 // The gradient of a head: turned back, then through the norm as computed again from x.  Sums for weight and bias: over the CTA's tokens and heads in
 // registers, over the warp's groups by shuffles, over warps in shared memory, over CTAs by norm_rope_sums_kernel.
-template <int V, int G, int E, int BYTES>
-__global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
-  constexpr int kTokens = kNrThreads / G, H = kHalf<V>;
-  __shared__ float red[2][kNrThreads / 32][2 * V * G * E];
+template <int V, int G, int E, int BYTES, int CB>
+__global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
+  using T = Tile<V, G, E, BYTES, CB, 2>;
+  constexpr int H = kHalf<V>, kChunks = T::kChunks;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[2][kNrWarps][2 * V * G * E];
   griddep_wait();
   griddep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Heads h = heads_of(blockIdx.y, p);
   const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
   Lane<V, E> l;
-  place<V, G, E>(l, p, threadIdx.x % G);
+  place<V, G, E>(l, p, lane % G);
   float2 w[E][2][H], dw[E][2][H], db[E][2][H];
   if (normed) parameter<V, E>(w, l, p.weight[h.part], p.param_type, 1.f);
 #pragma unroll
@@ -345,65 +426,108 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_bwd_kern
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int k = 0; k < H; ++k) dw[e][m][k] = db[e][m][k] = twice(0.f);
-  const void* d_out = p.d_out[h.part];
-  const int64_t width = static_cast<int64_t>(p.heads + 2 * p.kv_heads) * p.head_dim, column = static_cast<int64_t>(packed_head(h, p)) * p.head_dim;
-  const int64_t d_head = p.d_strides[h.part][1];
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens; first < p.rows_of_tokens; first += static_cast<int64_t>(gridDim.x) * kTokens) {
-    const int64_t token = first + threadIdx.x / G, b = token / p.tokens;
+  const char* d_out = static_cast<const char*>(p.d_out[h.part]);
+  const int64_t row_bytes = p.head_dim * BYTES, width = (p.heads + 2 * p.kv_heads) * row_bytes, column = packed_head(h, p) * row_bytes;
+  const int64_t d_head = p.d_strides[h.part][1] * BYTES;
+  const uint32_t ring = smem_u32(smem) + warp * T::kBytes * (2 * T::kAhead + 1), last = ring + 2 * T::kAhead * T::kBytes, mine = lane / G * T::kPitch;
+  const uint32_t zeros = smem_u32(smem) + T::kSmem - T::kZeros;
+  uint32_t in_tile[E][2];                                          // its vectors in the first place; without columns: the zeros, whatever the place
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) in_tile[e][m] = l.on[e] ? ring + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES : zeros;
+  if (threadIdx.x < T::kZeros / 4) sts32(zeros + 4 * threadIdx.x, 0);
+  __syncthreads();
+  for (int64_t begin = static_cast<int64_t>(blockIdx.x) * kNrWarps * T::kRows; begin < p.rows_of_tokens; begin += static_cast<int64_t>(gridDim.x) * kNrWarps * T::kRows) {
+    const int64_t first = begin + warp * T::kRows, token = first + lane / G, b = static_cast<uint32_t>(token) / p.tokens;
     const bool in = token < p.rows_of_tokens;
     const int at = static_cast<int>(token - b * p.tokens);
-    const int64_t from = b * p.stride_b + at * p.stride_t + column, to = token * width + column;
-    const int64_t d_from = b * p.d_strides[h.part][0] + h.first * d_head + at * p.d_strides[h.part][2];
-    Vec<V, BYTES> raw[E][2], d_raw[E][2];                          // of the next head
-    auto fetch = [&](int i) {
+    const char *from[kChunks], *d_from[kChunks];
+    char* to[kChunks];                                             // NULL: not there
+    uint32_t place_of[kChunks];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (in && l.on[e] && i < h.count) {
-          if (d_out) {
-            load_vec<V, BYTES>(d_raw[e][0], d_out, d_from + i * d_head + l.slot[e].c0);
-            load_vec<V, BYTES>(d_raw[e][1], d_out, d_from + i * d_head + l.slot[e].c1);
+    for (int n = 0; n < kChunks; ++n) {
+      const auto c = T::chunk(n, lane, static_cast<int>(row_bytes));
+      const uint32_t tok = static_cast<uint32_t>(first) + c.row, cb = tok / p.tokens, ct = tok - cb * p.tokens;       // fewer than 2^31
+      from[n] = static_cast<const char*>(p.qkv) + (static_cast<int64_t>(cb) * p.stride_b + static_cast<int64_t>(ct) * p.stride_t) * BYTES + column + c.byte;
+      d_from[n] = d_out + (static_cast<int64_t>(cb) * p.d_strides[h.part][0] + static_cast<int64_t>(ct) * p.d_strides[h.part][2]) * BYTES + h.first * d_head + c.byte;
+      to[n] = c.in && tok < p.rows_of_tokens ? static_cast<char*>(p.d_qkv) + tok * width + column + c.byte : nullptr;
+      place_of[n] = c.at;
+    }
+    int left = h.count;                                            // heads that are still to be asked for
+    uint32_t free = 0, full = 0;                                   // places in the ring
+    auto next = [&](uint32_t& place) { place = place == (T::kAhead - 1) * 2 * T::kBytes ? 0 : place + 2 * T::kBytes; };
+    auto fetch = [&] {
+      if (left > 0)
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n)
+          if (to[n]) {
+            if (d_out) T::ask(ring + free + place_of[n], d_from[n]);
+            if (normed) T::ask(ring + free + T::kBytes + place_of[n], from[n]);
+            d_from[n] += d_head;
+            from[n] += row_bytes;
           }
-          if (normed) {
-            load_vec<V, BYTES>(raw[e][0], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
-            load_vec<V, BYTES>(raw[e][1], p.qkv, from + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
-          }
+      --left;
+      next(free);
+      cp_async_commit();
+    };
+    auto leave = [&](uint32_t tile) {
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n)
+        if (to[n]) {
+          T::leave(to[n], tile + place_of[n]);
+          to[n] += row_bytes;
         }
     };
-    fetch(0);
+    __syncwarp();                                                  // the last tokens' tiles are read
+#pragma unroll
+    for (int u = 0; u < T::kAhead; ++u) fetch();
     float2 c[E][H], s[E][H];
     if (h.part < 2) angles<V, E>(c, s, l, p, b, at, in);
+#pragma unroll 1
     for (int i = 0; i < h.count; ++i) {
+      cp_async_wait<T::kAhead - 1>();
+      if (h.part == 2) {
+        if (!d_out)                                                // zeros, by way of the results' tile
+#pragma unroll
+          for (int n = 0; n < kChunks; ++n) {
+            Vec<CB / 2, 2> zero;
+#pragma unroll
+            for (int k = 0; k < Vec<CB / 2, 2>::kWords; ++k) zero.w[k] = 0;
+            if (to[n]) put_vec<CB / 2, 2>(zero, last + place_of[n]);
+          }
+        leave(d_out ? ring + full : last);
+        next(full);
+        fetch();
+        continue;
+      }
+      __syncwarp();                                                // every lane's copies are there, and the last head's results have left
       float2 d[E][2][H], x[E][2][H];
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          values<V, BYTES>(d[e][m], d_raw[e][m], p.type);
-          values<V, BYTES>(x[e][m], raw[e][m], p.type);
-#pragma unroll
-          for (int k = 0; k < H; ++k) {
-            if (!(in && l.on[e] && d_out)) d[e][m][k] = twice(0.f);
-            if (!l.on[e]) x[e][m][k] = twice(0.f);
+          Vec<V, BYTES> raw, d_raw;
+          // a token that is not there has whatever was in the tile
+          take_vec<V, BYTES>(d_raw, in && d_out ? in_tile[e][m] + (l.on[e] ? full : 0) : zeros);
+          values<V, BYTES>(d[e][m], d_raw, p.type);
+          if (normed) {
+            take_vec<V, BYTES>(raw, in ? in_tile[e][m] + (l.on[e] ? full + T::kBytes : 0) : zeros);
+            values<V, BYTES>(x[e][m], raw, p.type);
           }
         }
-      fetch(i + 1);
-      if (h.part < 2)
+      next(full);
+      __syncwarp();
+      fetch();
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+      for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int k = 0; k < H; ++k) {
-            const float2 d1 = d[e][0][k], d2 = d[e][1][k];
-            d[e][0][k] = ffma2(d1, c[e][k], fmul2(d2, s[e][k]));
-            d[e][1][k] = ffma2(d2, c[e][k], minus(fmul2(d1, s[e][k])));
-          }
+        for (int k = 0; k < H; ++k) {
+          const float2 d1 = d[e][0][k], d2 = d[e][1][k];
+          d[e][0][k] = ffma2(d1, c[e][k], fmul2(d2, s[e][k]));
+          d[e][1][k] = ffma2(d2, c[e][k], minus(fmul2(d1, s[e][k])));
+        }
       if (normed) {
-        if (!in)                                                   // a token that is not there has d = 0; x is whatever was in the registers
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-              for (int k = 0; k < H; ++k) x[e][m][k] = twice(0.f);
         const float inverse = normalise<V, G, E>(x, l, p, in ? p.eps[h.part] : 1.f);
         float2 t0 = twice(0.f), t1 = twice(0.f);                   // sums of e and of e n, e = d * weight
 #pragma unroll
@@ -430,13 +554,15 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_bwd_kern
       }
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (in && l.on[e]) {
-          Vec<V, BYTES> o;
-          rounded<V, BYTES>(o, d[e][0], p.type);
-          store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c0);
-          rounded<V, BYTES>(o, d[e][1], p.type);
-          store_vec<V, BYTES>(o, p.d_qkv, to + static_cast<int64_t>(i) * p.head_dim + l.slot[e].c1);
-        }
+        if (l.on[e])
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            Vec<V, BYTES> o;
+            rounded<V, BYTES>(o, d[e][m], p.type);
+            put_vec<V, BYTES>(o, last + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES);
+          }
+      __syncwarp();
+      leave(last);
     }
   }
   if (!p.sums || !normed) return;                            // the same for the whole CTA
@@ -467,7 +593,7 @@ __global__ void __launch_bounds__(kNrThreads, V == 1 ? 1 : 2) norm_rope_bwd_kern
     const int which = c >= p.head_dim, col = c - which * p.head_dim;
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kNrThreads / 32; ++w) total += red[which][w][col];
+    for (int k = 0; k < kNrWarps; ++k) total += red[which][k][col];
     to[c] = total;
   }
 }
@@ -502,34 +628,47 @@ __global__ void __launch_bounds__(1024) norm_rope_sums_kernel(const __grid_const
   }
 }
 
-template <int V, int G, int E, int BYTES>
+template <int V, int G, int E, int BYTES, int CB>
 static int run_norm_rope(const NrParams& p, bool backward, unsigned ctas, cudaStream_t st) {
   const dim3 grid(ctas, static_cast<unsigned>(p.q_chunks + 2 * p.kv_chunks));
-  if constexpr (V < 8) {
-    if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+  auto run = [&](void (*kernel)(NrParams), int smem) {
+    static std::atomic<uint64_t> ready[2];
+    if (attributes_missing(ready[backward])) {
+      S3R_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      attributes_set(ready[backward]);
+    }
+    return launch(kernel, grid, kNrThreads, smem, st, p);
+  };
+  if (backward) return run(norm_rope_bwd_kernel<V, G, E, BYTES, CB>, Tile<V, G, E, BYTES, CB, 2>::kSmem);
+  return run(norm_rope_fwd_kernel<V, G, E, BYTES, CB>, Tile<V, G, E, BYTES, CB, 1>::kSmem);
+}
+// The widest copy of at most 16 bytes that divides rows, addresses and strides, and no narrower than a vector; in between only what V = 1 has.
+template <int V, int G, int E, int BYTES>
+static int by_chunk(const NrParams& p, int bytes, bool backward, unsigned ctas, cudaStream_t st) {
+  constexpr int kVector = V * BYTES > 16 ? 16 : V * BYTES;
+  if (bytes >= 16) return run_norm_rope<V, G, E, BYTES, 16>(p, backward, ctas, st);
+  if constexpr (kVector == 2) {
+    if (bytes >= 4) return run_norm_rope<V, G, E, BYTES, 4>(p, backward, ctas, st);
   }
-  return launch(norm_rope_fwd_kernel<V, G, E, BYTES>, grid, kNrThreads, 0, st, p);
+  return run_norm_rope<V, G, E, BYTES, kVector>(p, backward, ctas, st);
 }
-// Threads of a head: as many as it has pairs of vectors, a power of two.
+// Elements of a thread's vectors, threads of a head (a power of two), pairs of vectors of each, bytes of a copy.
 struct NrShape {
-  int vector, group;
+  int vector, group, each, bytes;
 };
-static NrShape norm_rope_shape(int vector, int head_dim) {
-  const int slots = head_dim / (2 * vector);
-  if (vector == 8) return {8, slots <= 2 ? 2 : slots <= 4 ? 4 : slots <= 8 ? 8 : 16};
-  if (vector == 4) return {4, slots <= 8 ? 8 : slots <= 16 ? 16 : 32};
-  return {1, 32};
-}
 template <int BYTES>
 static int pick_norm_rope(const NrParams& p, NrShape s, bool backward, unsigned ctas, cudaStream_t st) {
-  if (s.vector == 8 && s.group == 2) return run_norm_rope<8, 2, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 8 && s.group == 4) return run_norm_rope<8, 4, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 8 && s.group == 8) return run_norm_rope<8, 8, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 8) return run_norm_rope<8, 16, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 4 && s.group == 8) return run_norm_rope<4, 8, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 4 && s.group == 16) return run_norm_rope<4, 16, 1, BYTES>(p, backward, ctas, st);
-  if (s.vector == 4) return run_norm_rope<4, 32, 1, BYTES>(p, backward, ctas, st);
-  return run_norm_rope<1, 32, 4, BYTES>(p, backward, ctas, st);
+  switch (s.vector * 100 + s.group + s.each - 1) {
+    case 408: return by_chunk<4, 8, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 416: return by_chunk<4, 16, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 432: return by_chunk<4, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 216: return by_chunk<2, 16, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 232: return by_chunk<2, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 233: return by_chunk<2, 32, 2, BYTES>(p, s.bytes, backward, ctas, st);
+    case 132: return by_chunk<1, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 133: return by_chunk<1, 32, 2, BYTES>(p, s.bytes, backward, ctas, st);
+    default: return by_chunk<1, 32, 4, BYTES>(p, s.bytes, backward, ctas, st);
+  }
 }
 
 // Heads are split over CTAs until there are some for every SM; no further than that, a token's angles are found once per CTA.
@@ -546,7 +685,7 @@ static void norm_rope_chunks(int64_t token_ctas, int heads, int kv_heads, int* p
 }
 // CTAs of the backward along the tokens: those that are resident together, so that each leaves one row of sums.
 static unsigned norm_rope_bwd_ctas(int64_t token_ctas, int chunks) {
-  const int64_t most = (4 * static_cast<int64_t>(sm_count()) + chunks - 1) / chunks;
+  const int64_t most = (8 * static_cast<int64_t>(sm_count()) + chunks - 1) / chunks;
   return static_cast<unsigned>(token_ctas < most ? token_ctas : most < 1 ? 1 : most);
 }
 
@@ -572,17 +711,19 @@ static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
   return 0;
 }
 
-// The largest vector, up to `most`, that divides pairs, what is not turned, addresses and strides
-static int norm_rope_vector(const s3r_qkv_norm_rope* f, int most, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
-  const int turned = 2 * f->axes * f->pairs;
-  for (int v = most; v >= 4; v /= 2) {
-    const int bytes = v * type_bytes(f->type) < 16 ? v * type_bytes(f->type) : 16;
-    bool fits = (f->axes == 0 || f->pairs % v == 0) && (f->head_dim - turned) % (2 * v) == 0;
-    for (int i = 0; i < n_pointers; ++i) fits = fits && reinterpret_cast<uintptr_t>(pointers[i]) % bytes == 0;
-    for (int i = 0; i < n_strides; ++i) fits = fits && strides[i] * type_bytes(f->type) % bytes == 0;
-    if (fits) return v;
-  }
-  return 1;
+// The largest vector, up to four elements, that divides pairs, what is not turned, addresses and strides
+static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
+  const int turned = 2 * f->axes * f->pairs, size = type_bytes(f->type);
+  uint64_t grid = 16 | static_cast<uint64_t>(f->head_dim) * size;      // its lowest bit: what rows, addresses and strides are multiples of
+  for (int i = 0; i < n_pointers; ++i) grid |= reinterpret_cast<uintptr_t>(pointers[i]);
+  for (int i = 0; i < n_strides; ++i) grid |= static_cast<uint64_t>(strides[i]) * size;
+  const int bytes = static_cast<int>(grid & (~grid + 1));
+  int v = 4;
+  while (v > 1 && ((f->axes && f->pairs % v) || (f->head_dim - turned) % (2 * v) || (v * size < 16 ? v * size : 16) > bytes)) v /= 2;
+  const int slots = f->head_dim / (2 * v);
+  if (v == 4) return {4, slots <= 8 ? 8 : slots <= 16 ? 16 : 32, 1, bytes};
+  if (v == 2) return {2, slots <= 16 ? 16 : 32, slots <= 32 ? 1 : 2, bytes};
+  return {1, 32, slots <= 32 ? 1 : slots <= 64 ? 2 : 4, bytes};
 }
 
 static NrParams norm_rope_params(const s3r_qkv_norm_rope* f) {
@@ -602,7 +743,7 @@ static NrParams norm_rope_params(const s3r_qkv_norm_rope* f) {
   p.cos_pitch = f->cos_pitch;
   p.sin_pitch = f->sin_pitch;
   p.rows_of_tokens = f->batch * f->tokens;
-  p.tokens = static_cast<int>(f->tokens);
+  p.tokens = static_cast<uint32_t>(f->tokens);
   p.heads = f->heads;
   p.kv_heads = f->kv_heads;
   p.head_dim = f->head_dim;
@@ -637,7 +778,7 @@ extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
   p.out[2] = f->v;
   const void* pointers[] = {f->qkv, f->q, f->k, f->v};
   const int64_t strides[] = {f->batch > 1 ? f->stride_b : 0, f->tokens > 1 ? f->stride_t : 0};
-  const NrShape s = norm_rope_shape(norm_rope_vector(f, 8, pointers, 4, strides, 2), f->head_dim);
+  const NrShape s = norm_rope_shape(f, pointers, 4, strides, 2);
   const int64_t per = kNrThreads / s.group, ctas = (p.rows_of_tokens + per - 1) / per;
   norm_rope_chunks(ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -647,8 +788,8 @@ extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
 // Room for either shape of the grid: the chunks of heads depend on the vectors that addresses allow.
 extern "C" size_t s3r_qkv_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim) {
   if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  // chunks of q and k times CTAs along the tokens: at most one more CTA per chunk than 4 per SM in all, and no chunk without a head
-  return static_cast<size_t>(4 * sm_count() + heads + 2 * kv_heads) * 2 * head_dim * sizeof(float);
+  // chunks of q and k times CTAs along the tokens: at most one more CTA per chunk than 8 per SM in all, and no chunk without a head
+  return static_cast<size_t>(8 * sm_count() + heads + 2 * kv_heads) * 2 * head_dim * sizeof(float);
 }
 
 extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_norm_rope_grad* g, void* stream) {
@@ -679,7 +820,7 @@ extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_n
   }
   p.d_qkv = g->d_qkv;
   p.sums = sums ? static_cast<float*>(g->workspace) : nullptr;
-  const NrShape s = norm_rope_shape(norm_rope_vector(f, 4, pointers, np, strides, ns), f->head_dim);
+  const NrShape s = norm_rope_shape(f, pointers, np, strides, ns);
   const int64_t per = kNrThreads / s.group, token_ctas = (p.rows_of_tokens + per - 1) / per;
   norm_rope_chunks(token_ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   const int chunks = p.q_chunks + 2 * p.kv_chunks;

@@ -459,7 +459,10 @@ typedef struct {
   int bias_type, scale_type, residual_type, act;
   void* out;
   int out_type;
+  void* workspace;          /* s3r_linear_workspace_bytes, 16-byte aligned; with less, or none, a long sum of few rows is not cut into parts */
+  size_t workspace_bytes;
 } s3r_linear;
+size_t s3r_linear_workspace_bytes(int64_t M, int64_t N, int64_t K); /* 0: none is used; of a product out [M, N] over K, too */
 int s3r_linear_fwd(const s3r_linear* args_host, void* stream);
 
 /* The elementwise part of its backward; f: the forward's arguments (residual and out are not read).  dy [M, N] contiguous, of f's out_type.
@@ -480,7 +483,7 @@ int s3r_linear_bwd(const s3r_linear* f_host, const s3r_linear_grad* g_host, void
 /* out [M, N] contiguous = sum over k of a(m, k) b(n, k), fp32 sums: a lies as [M, K] or, turned, as [K, M], b as [N, K] or [K, N].  All of `type`
  * (S3R_BF16 or S3R_F16); operands' bases and rows at multiples of 16 bytes.  dx = product(dz, weight turned), dW = product(dz turned, x turned). */
 int s3r_product(const void* a, int64_t a_pitch, int a_turned, const void* b, int64_t b_pitch, int b_turned, int type, void* out, int64_t M, int N,
-                int64_t K, void* stream);
+                int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The packed projection qkv [batch, tokens, (heads + 2 * kv_heads) * head_dim], heads of q, k and v one behind the other, as q, k and v
  * [batch, heads | kv_heads, tokens, head_dim] contiguous:  n = norm(x) * weight + bias per head of q and k (S3R_NORM_*, q_normed / k_normed == 0:

@@ -59,7 +59,8 @@ SIGNATURES = {
     "s3r_linear_fwd": (_i, [_p, _p]),
     "s3r_linear_bwd_workspace_bytes": (_sz, [_i64, _i]),
     "s3r_linear_bwd": (_i, [_p, _p, _p]),
-    "s3r_product": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _p, _i64, _i, _i64, _p]),
+    "s3r_linear_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "s3r_product": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _p, _i64, _i, _i64, _p, _sz, _p]),
     "s3r_qkv_norm_rope_fwd": (_i, [_p, _p]),
     "s3r_qkv_norm_rope_bwd_workspace_bytes": (_sz, [_i64, _i64, _i, _i, _i]),
     "s3r_qkv_norm_rope_bwd": (_i, [_p, _p, _p]),

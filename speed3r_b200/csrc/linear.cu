@@ -8,10 +8,11 @@
 namespace s3r {
 
 // ---------------------------------------------------------------------------------------------------------------------
-// a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has four output
-// channels, a lane 16 bytes of each at a time; the tokens lie in shared memory.
+// a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has two output channels,
+// a lane 16 bytes of each at a time and four of those in flight; the tokens lie in shared memory.  One token x 4096 x 1024, weights not in L2:
+// {FEW}; with four channels and one ahead 8.0.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kLinFew = 8, kLinFewBytes = 48 * 1024, kLinFewChannels = 4, kLinFewWarps = 8;
+constexpr int kLinFew = 8, kLinFewBytes = 48 * 1024, kLinFewChannels = 2, kLinFewWarps = 8, kLinFewAhead = 4;
 
 struct LinFewParams {
   const uint16_t *x, *w;
@@ -42,12 +43,13 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
   uint4* x = reinterpret_cast<uint4*>(smem);                       // [M][chunks]
   const int n0 = (blockIdx.x * kLinFewWarps + warp) * kLinFewChannels;
   // the first weights are on their way while the tokens are fetched
-  uint4 w[kLinFewChannels];
-  auto fetch = [&](int c) {
+  uint4 w[kLinFewAhead][kLinFewChannels];
+  auto fetch = [&](int c, int at) {
 #pragma unroll
-    for (int i = 0; i < kLinFewChannels; ++i) w[i] = n0 + i < p.N && c < chunks ? load_8(p.w + (n0 + i) * p.w_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kLinFewChannels; ++i) w[at][i] = n0 + i < p.N && c < chunks ? load_8(p.w + (n0 + i) * p.w_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
   };
-  fetch(lane);
+#pragma unroll
+  for (int k = 0; k < kLinFewAhead; ++k) fetch(lane + 32 * k, k);
 #pragma unroll
   for (int m = 0; m < M; ++m)
     for (int c = threadIdx.x; c < chunks; c += 32 * kLinFewWarps) x[m * chunks + c] = m < p.M ? load_8(p.x + m * p.x_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
@@ -57,24 +59,29 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
   for (int i = 0; i < kLinFewChannels; ++i)
 #pragma unroll
     for (int m = 0; m < M; ++m) sum[i][m] = both(0.f);
-  for (int c = lane; c < chunks; c += 32) {
-    float2 now[kLinFewChannels][4];
+  for (int c0 = lane; c0 < chunks; c0 += 32 * kLinFewAhead) {
 #pragma unroll
-    for (int i = 0; i < kLinFewChannels; ++i) {
-      now[i][0] = pair_of<BF16>(w[i].x);
-      now[i][1] = pair_of<BF16>(w[i].y);
-      now[i][2] = pair_of<BF16>(w[i].z);
-      now[i][3] = pair_of<BF16>(w[i].w);
-    }
-    fetch(c + 32);
+    for (int k = 0; k < kLinFewAhead; ++k) {
+      const int c = c0 + 32 * k;
+      float2 now[kLinFewChannels][4];
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const uint4 t = x[m * chunks + c];
-      const float2 v[4] = {pair_of<BF16>(t.x), pair_of<BF16>(t.y), pair_of<BF16>(t.z), pair_of<BF16>(t.w)};
+      for (int i = 0; i < kLinFewChannels; ++i) {
+        now[i][0] = pair_of<BF16>(w[k][i].x);
+        now[i][1] = pair_of<BF16>(w[k][i].y);
+        now[i][2] = pair_of<BF16>(w[k][i].z);
+        now[i][3] = pair_of<BF16>(w[k][i].w);
+      }
+      fetch(c + 32 * kLinFewAhead, k);
+      if (c >= chunks) continue;
 #pragma unroll
-      for (int i = 0; i < kLinFewChannels; ++i)
+      for (int m = 0; m < M; ++m) {
+        const uint4 t = x[m * chunks + c];
+        const float2 v[4] = {pair_of<BF16>(t.x), pair_of<BF16>(t.y), pair_of<BF16>(t.z), pair_of<BF16>(t.w)};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[i][m] = ffma2(now[i][k], v[k], sum[i][m]);
+        for (int i = 0; i < kLinFewChannels; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[i][m] = ffma2(now[i][j], v[j], sum[i][m]);
+      }
     }
   }
 #pragma unroll
@@ -111,6 +118,104 @@ static int run_linear_few(const LinFewParams& p, cudaStream_t st) {
   const size_t smem = static_cast<size_t>(M) * ((p.K + 7) / 8) * 16;
   return p.type == S3R_BF16 ? launch(linear_few_kernel<M, true>, grid, 32 * kLinFewWarps, smem, st, p)
                             : launch(linear_few_kernel<M, false>, grid, 32 * kLinFewWarps, smem, st, p);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// the sums of a contraction's parts, in their order, and what follows them: a thread has four columns of a row
+// ---------------------------------------------------------------------------------------------------------------------
+struct JoinParams {
+  const float* sums;                    // [parts][part_rows][pitch]
+  const void *bias, *scale, *residual;
+  void* out;
+  int64_t M, part_rows;
+  int N, pitch, parts, quads;
+  int bias_type, scale_type, residual_type, out_type, act, vectors;
+};
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ JoinParams p) {
+  griddep_wait();
+  griddep_launch();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / p.quads;
+  if (row >= p.M) return;
+  const int col = static_cast<int>(i - row * p.quads) * 4;
+  const float* from = p.sums + row * p.pitch + col;
+  const int64_t part = p.part_rows * p.pitch;
+  float4 v[16];
+#pragma unroll
+  for (int s = 0; s < 16; ++s)
+    if (s < p.parts) v[s] = __ldg(reinterpret_cast<const float4*>(from + s * part));
+  float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+  for (int s = 1; s < 16; ++s)
+    if (s < p.parts) f[0] += v[s].x, f[1] += v[s].y, f[2] += v[s].z, f[3] += v[s].w;
+  const int64_t at = row * p.N + col;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (p.bias && col + k < p.N) f[k] += load_one(p.bias, p.bias_type, col + k);
+  with_act(p.act, [&](auto act) {
+    float2 slope;
+    const float2 a = activate<decltype(act)::value, false>(make_float2(f[0], f[1]), slope), b = activate<decltype(act)::value, false>(make_float2(f[2], f[3]), slope);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+    return 0;
+  });
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (col + k < p.N) {
+      const float s = p.scale ? load_one(p.scale, p.scale_type, col + k) : 1.f;
+      f[k] = p.residual ? __fmaf_rn(f[k], s, load_one(p.residual, p.residual_type, at + k)) : f[k] * s;
+    }
+  if (p.vectors) {
+    Raw<4> o;
+    pack<4>(o, f, p.out_type);
+    store_raw<4>(o, p.out, p.out_type, at);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < p.N) {
+        const float one[1] = {f[k]};
+        Raw<1> o;
+        pack<1>(o, one, p.out_type);
+        store_raw<1>(o, p.out, p.out_type, at + k);
+      }
+  }
+}
+
+// Bytes of the parts' sums, 0 where there is one part
+static size_t part_bytes(const LinPlan& t, int64_t M, int64_t N) {
+  return t.parts > 1 ? static_cast<size_t>(part_rows(M, t.ctas)) * t.parts * ((N + 3) / 4 * 4) * sizeof(float) : 0;
+}
+// The product with its epilogue (p: everything but its result) in parts
+static int run_parts(const LinPlan& t, const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, void* workspace, cudaStream_t st) {
+  LinParams part = {};
+  part.rows = p.M;
+  part.N = p.N;
+  part.parts = t.parts;
+  part.out = workspace;
+  part.out_pitch = (p.N + 3) / 4 * 4;
+  part.out_type = S3R_F32;
+  part.status = p.status;
+  if (const int rc = linear_partial(a, b, k, bf16, part, st)) return rc;
+  JoinParams j = {};
+  j.sums = static_cast<const float*>(workspace);
+  j.bias = p.bias;
+  j.scale = p.scale;
+  j.residual = p.other;
+  j.out = p.out;
+  j.M = p.M;
+  j.part_rows = part_rows(p.M, t.ctas);
+  j.N = p.N;
+  j.pitch = static_cast<int>(part.out_pitch);
+  j.parts = t.parts;
+  j.quads = (p.N + 3) / 4;
+  j.bias_type = p.bias_type;
+  j.scale_type = p.scale_type;
+  j.residual_type = p.other_type;
+  j.out_type = p.out_type;
+  j.act = p.act;
+  const void* ptr[] = {p.out};
+  j.vectors = row_vector(p.N, ptr, &p.out_type, 1) >= 4;
+  const int64_t blocks = (p.M * j.quads + 255) / 256;
+  S3R_REQUIRE(blocks < (1ll << 31), S3R_ERR_TOO_LARGE, "s3r_linear: too many rows");
+  return launch(linear_join_kernel, static_cast<unsigned>(blocks), 256, 0, st, j);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -190,7 +295,13 @@ __global__ void __launch_bounds__(1024) linear_sums_kernel(const __grid_constant
   const int type = blockIdx.y ? p.types[1] : p.types[0];
   float total = 0.f;
   if (col < p.N)
-    for (int64_t i = warp; i < p.blocks; i += 32) total += __ldg(sums + i * p.N + col);
+    for (int64_t i = warp; i < p.blocks; i += 32 * 8) {            // eight on their way at a time
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < p.blocks ? __ldg(sums + (i + 32 * k) * p.N + col) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) total += v[k];
+    }
   red[warp][lane] = total;
   __syncthreads();
   if (warp == 0) {
@@ -230,6 +341,10 @@ static int check_linear(const s3r_linear* f, const char* what) {
 // rows of N elements all begin at multiples of `bytes`
 static bool in_vectors(const void* p, int type, int N, int bytes) { return static_cast<int64_t>(N) * type_bytes(type) % bytes == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+static bool is_few(int64_t M, int64_t K) { return M <= kLinFew && (M <= 2 ? M : M <= 4 ? 4 : 8) * ((K + 7) / 8 * 16) <= kLinFewBytes; }
+// A workspace is used where it is given and large enough: without one the contraction stays in one part.
+static bool has_room(const void* workspace, size_t bytes, size_t need) { return workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0; }
+
 static LinParams linear_params(const s3r_linear* f) {
   LinParams p = {};
   p.M = f->M;
@@ -247,12 +362,16 @@ static LinParams linear_params(const s3r_linear* f) {
 
 using namespace s3r;
 
+extern "C" size_t s3r_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  return M > 0 && N > 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31) && !is_few(M, K) ? part_bytes(linear_plan(M, N, K, true), M, N) : 0;
+}
+
 extern "C" int s3r_linear_fwd(const s3r_linear* f, void* stream) {
   if (const int rc = check_linear(f, "s3r_linear_fwd")) return rc;
   S3R_REQUIRE(f->out, S3R_ERR_NULL, "s3r_linear_fwd: NULL pointer");
   S3R_REQUIRE(at_multiple(f->out, f->out_type), S3R_ERR_ALIGNMENT, "s3r_linear_fwd: elements must be aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (f->M <= kLinFew && (f->M <= 2 ? f->M : f->M <= 4 ? 4 : 8) * ((static_cast<int64_t>(f->K) + 7) / 8 * 16) <= kLinFewBytes) {
+  if (is_few(f->M, f->K)) {
     const LinFewParams p = {static_cast<const uint16_t*>(f->x), static_cast<const uint16_t*>(f->weight), f->bias, f->scale, f->residual, f->out, f->x_pitch, f->w_pitch,
                             f->N, f->K, static_cast<int>(f->M), f->type, f->bias_type, f->scale_type, f->residual_type, f->out_type, f->act};
     return f->M == 1 ? run_linear_few<1>(p, st) : f->M == 2 ? run_linear_few<2>(p, st) : f->M <= 4 ? run_linear_few<4>(p, st) : run_linear_few<8>(p, st);
@@ -267,6 +386,8 @@ extern "C" int s3r_linear_fwd(const s3r_linear* f, void* stream) {
   p.out_type = f->out_type;
   const LinOperand a = {f->x, f->x_pitch, false}, b = {f->weight, f->w_pitch, false};
   const bool bf16 = f->type == S3R_BF16;
+  const LinPlan t = linear_plan(f->M, f->N, f->K, true);
+  if (t.parts > 1 && has_room(f->workspace, f->workspace_bytes, part_bytes(t, f->M, f->N))) return run_parts(t, a, b, f->K, bf16, p, f->workspace, st);
   return f->residual ? linear_added(a, b, f->K, bf16, p, st) : f->out_type == S3R_F32 ? linear_wide(a, b, f->K, bf16, p, st) : linear_narrow(a, b, f->K, bf16, p, st);
 }
 
@@ -325,7 +446,7 @@ extern "C" int s3r_linear_bwd(const s3r_linear* f, const s3r_linear_grad* g, voi
 }
 
 extern "C" int s3r_product(const void* a, int64_t a_pitch, int a_turned, const void* b, int64_t b_pitch, int b_turned, int type, void* out, int64_t M, int N,
-                           int64_t K, void* stream) {
+                           int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
   S3R_REQUIRE(a && b && out, S3R_ERR_NULL, "s3r_product: NULL pointer");
   S3R_REQUIRE(M > 0 && N > 0 && K > 0 && a_pitch >= (a_turned ? M : K) && b_pitch >= (b_turned ? N : K), S3R_ERR_SHAPE,
               "s3r_product: sizes must be positive, pitches no shorter than rows");
@@ -341,5 +462,9 @@ extern "C" int s3r_product(const void* a, int64_t a_pitch, int a_turned, const v
   p.out_type = type;
   p.status = device_status_ptr();
   S3R_REQUIRE(p.status, S3R_ERR_DRIVER, "s3r_product: no status word");
-  return linear_narrow({a, a_pitch, a_turned != 0}, {b, b_pitch, b_turned != 0}, K, type == S3R_BF16, p, static_cast<cudaStream_t>(stream));
+  const LinOperand left = {a, a_pitch, a_turned != 0}, right = {b, b_pitch, b_turned != 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const LinPlan t = linear_plan(M, N, K, true);
+  if (t.parts > 1 && has_room(workspace, workspace_bytes, part_bytes(t, M, N))) return run_parts(t, left, right, K, type == S3R_BF16, p, workspace, st);
+  return linear_narrow(left, right, K, type == S3R_BF16, p, st);
 }

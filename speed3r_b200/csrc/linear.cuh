@@ -78,6 +78,7 @@ int linear_narrow(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16
 int linear_wide(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st);            // fp32 result, nothing added
 int linear_added(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st);           // with a residual
 int linear_dz(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st);
+int linear_partial(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st);         // parts of the contraction, fp32
 
 // ---------------------------------------------------------------------------------------------------------------------
 // product on tcgen05: persistent CTAs (pairs of them), the contraction in steps of 64 through a ring of TMA copies, the sums of two tiles in
@@ -89,14 +90,15 @@ int linear_dz(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, co
 constexpr int kLinFirst = 4, kLinWarps = 8, kLinThreads = 32 * (kLinFirst + kLinWarps);      // warps 0 and 1 feed, the last eight take the sums
 constexpr int kLinPiece = 4096;                                    // a warp's piece of the output: 32 rows of 128 bytes
 constexpr int kLinStep = 64;                                       // elements of the contraction per stage: 128 bytes
-constexpr int kNoOther = -1, kAnyAct = -1;
+constexpr int kNoOther = -1, kAnyAct = -1, kPartial = -2;
 
 struct LinParams {
   const void *bias, *scale, *other;    // other: the residual | dy
   void* out;
   float *bias_sums, *scale_sums;       // [32-row blocks, N]: sums of dz and of dy * u
-  int64_t M, out_pitch;
+  int64_t M, rows, out_pitch;          // rows: kPartial's, of a
   int N, steps, m_tiles, n_tiles;
+  int parts, row_tiles, part_steps;           // kPartial: tiles of a's rows, steps of a part; m_tiles is that of all parts, M their rows
   int bias_type, scale_type, other_type, out_type, act;
   uint32_t idesc, a_turned, b_turned, copy_out, other_vectors;         // other's rows: in vectors of 16 bytes (the residual), in pairs (dy)
   uint32_t other_copied;               // dy by TMA
@@ -252,7 +254,7 @@ __device__ __forceinline__ float column_sum(const float2 (&d)[4], int lane) {
   return (odd ? b.y : b.x) + __shfl_xor_sync(0xffffffffu, odd ? b.x : b.y, 4);
 }
 
-// ACT: the activation, kAnyAct: p.act.  OTHER: type of the residual | of dy, kNoOther: there is none.  WIDE: the result is fp32.
+// ACT: the activation, kAnyAct: p.act, kPartial: none, and tile m of part s is number s * row_tiles + m.  OTHER: type of the residual | of dy, kNoOther: there is none.  WIDE: the result is fp32.
 // DZ: 1 out = dz from dy, and its sums over rows, in place of the forward's result; 2 the same with a scale, and the sums for that
 template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
@@ -318,8 +320,10 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
     const bool leader = elect_one_sync();
     Tile at = begin;
     for (int tile = first; tile < tiles && ok; tile += stride, advance(at)) {
-      const int m0 = (at.m * CTAS + rank) * 128, n0 = at.n * TN + rank * (TN / CTAS);
-      for (int k = 0; k < steps; ++k, ++n) {
+      const int part = ACT == kPartial ? at.m / p.row_tiles : 0;
+      const int m0 = ((at.m - part * p.row_tiles) * CTAS + rank) * 128, n0 = at.n * TN + rank * (TN / CTAS);
+      const int k0 = part * p.part_steps, k1 = ACT == kPartial ? min(steps, k0 + p.part_steps) : steps;
+      for (int k = k0; k < k1; ++k, ++n) {
         const int s = n % C::kStages;
         ok = mbar_wait_warp(&ctl.empty[s], (n / C::kStages & 1) ^ 1, abort_flag);
         if (!ok) break;
@@ -360,11 +364,12 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       const uint32_t a_far = p.a_turned ? 8192 : 16, b_far = p.b_turned ? 8192 : 16;
       int n = 0, done = 0;
       bool ok = true;
-      for (int tile = first; tile < tiles && ok; tile += stride, ++done) {
-        const int buf = done & 1;
+      Tile at = begin;
+      for (int tile = first; tile < tiles && ok; tile += stride, ++done, advance(at)) {
+        const int buf = done & 1, k0 = ACT == kPartial ? at.m / p.row_tiles * p.part_steps : 0, count = ACT == kPartial ? min(steps - k0, p.part_steps) : steps;
         ok = mbar_wait_warp(&ctl.acc_empty[buf], (done >> 1 & 1) ^ 1, abort_flag);
         tc_fence_after();
-        for (int k = 0; k < steps && ok; ++k, ++n) {
+        for (int k = 0; k < count && ok; ++k, ++n) {
           const int s = n % C::kStages;
           ok = mbar_wait_warp(&ctl.full[s], n / C::kStages & 1, abort_flag);
           if (!ok) break;
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
             umma_half_k4<CTAS>(tmem + buf * TN, umma_desc_sw128(base + s * C::kBytes, 1024, a_far),
                                umma_desc_sw128(base + s * C::kBytes + C::kABytes, 1024, b_far), p.idesc, k > 0, a_step, b_step);
             umma_commit(&ctl.empty[s], Ctas<CTAS>());
-            if (k == steps - 1) umma_commit(&ctl.acc_full[buf], Ctas<CTAS>());
+            if (k == count - 1) umma_commit(&ctl.acc_full[buf], Ctas<CTAS>());
           }
           __syncwarp();
         }
@@ -486,6 +491,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
             return 0;
           };
           if constexpr (ACT == kAnyAct) with_act(p.act, columns);
+          else if constexpr (ACT == kPartial) columns(std::integral_constant<int, S3R_ACT_NONE>());
           else columns(std::integral_constant<int, ACT>());
           if (OTHER != kNoOther || p.scale) {
 #pragma unroll
@@ -746,13 +752,18 @@ static int operand_map(CUtensorMap* map, const LinOperand& o, int64_t rows, int6
   return make_tensor_map(map, o.data, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
 }
 
+// rows of a part, which are whole tiles
+inline int64_t part_rows(int64_t rows, int ctas) { return (rows + 128 * ctas - 1) / (128 * ctas) * (128 * ctas); }
+
 template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, LinParams p, cudaStream_t st) {
   using C = LinCfg<TN, CTAS, DZ ? 2 : 1>;
   CUtensorMap ma, mb, mo, md;
-  if (const int rc = operand_map(&ma, a, p.M, k, 128, bf16)) return rc;
+  const int64_t rows = ACT == kPartial ? p.rows : p.M;
+  if (const int rc = operand_map(&ma, a, rows, k, 128, bf16)) return rc;
   if (const int rc = operand_map(&mb, b, p.N, k, TN / CTAS, bf16)) return rc;
   mo = md = ma;
+  if (ACT == kPartial) p.M = part_rows(rows, CTAS) * p.parts;
   constexpr int kSize = WIDE ? 4 : 2;
   p.copy_out = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_pitch * kSize % 16 == 0;
   if (p.copy_out && p.out) {
@@ -772,7 +783,12 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
   p.a_turned = a.turned;
   p.b_turned = b.turned;
   p.steps = static_cast<int>((k + kLinStep - 1) / kLinStep);
-  p.m_tiles = static_cast<int>((p.M + 128 * CTAS - 1) / (128 * CTAS));
+  p.m_tiles = static_cast<int>((rows + 128 * CTAS - 1) / (128 * CTAS));
+  if (ACT == kPartial) {
+    p.row_tiles = p.m_tiles;
+    p.part_steps = (p.steps + p.parts - 1) / p.parts;
+    p.m_tiles *= p.parts;
+  }
   p.n_tiles = (p.N + TN - 1) / TN;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles, at_once = sm_count() / CTAS;
   S3R_REQUIRE(tiles < (1ll << 31) - 1024, S3R_ERR_TOO_LARGE, "s3r_linear: too many tiles");
@@ -797,17 +813,34 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
   return check_cuda(cudaLaunchKernelEx(&c, linear_kernel<TN, CTAS, ACT, OTHER, WIDE, DZ>, ma, mb, mo, md, p), "kernel launch");
 }
 
-// The tile whose waves cost least: a wave of narrower tiles takes less, but not in proportion (the same rows of a).
+// The tile and the number of parts of the contraction whose waves cost least.  A wave of narrower tiles takes less, but not in proportion (the same
+// rows of a).  Parts - each a tile of its own, whose sums are joined by a second kernel - pay where there are few tiles and many steps:
+// 64 x 1024 x 4096 in eight parts {PARTS_64}, in one 20; the weight gradient 1024 x 1024 of 12 288 tokens {PARTS_DW}.
+struct LinPlan {
+  int width, ctas, parts;
+};
+inline LinPlan linear_plan(int64_t M, int64_t N, int64_t K, bool parts) {
+  const LinPlan tiles[] = {{256, 2, 1}, {128, 2, 1}, {128, 1, 1}, {64, 1, 1}};
+  const int64_t steps = (K + kLinStep - 1) / kLinStep;
+  LinPlan best = {};
+  int64_t least = INT64_MAX;
+  for (const LinPlan& t : tiles)
+    for (int n = 1; n <= 16; n *= 2) {
+      if ((t.ctas == 2 && M <= 128) || (n > 1 && (!parts || steps < 4 * n))) continue;
+      const int64_t part = (steps + n - 1) / n, used = (steps + part - 1) / part;      // parts that have steps
+      const int64_t all = (M + 128 * t.ctas - 1) / (128 * t.ctas) * ((N + t.width - 1) / t.width) * used, at_once = sm_count() / t.ctas;
+      // cycles: of a step, of a tile's start and end; of the second kernel and its traffic
+      const int64_t cost = (all + at_once - 1) / at_once * (part * (t.width + (t.ctas == 2 ? 64 : 96)) * 8 / 5 + 1500) + (n > 1 ? 6000 + used * M * N / 275 : 0);
+      if (cost < least) least = cost, best = {t.width, t.ctas, static_cast<int>(used)};
+    }
+  return best;
+}
 template <int ACT, int OTHER, bool WIDE, int DZ>
 static int run_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, const LinParams& p, cudaStream_t st) {
-  auto cost = [&](int tn, int ctas) {
-    const int64_t tiles = (p.M + 128 * ctas - 1) / (128 * ctas) * ((p.N + tn - 1) / tn), at_once = sm_count() / ctas;
-    return (tiles + at_once - 1) / at_once * (tn + (ctas == 2 ? 64 : 96));
-  };
-  const int64_t pair_256 = cost(256, 2), pair_128 = cost(128, 2), one_128 = cost(128, 1), one_64 = cost(64, 1);
-  if (p.M > 128 && pair_256 <= pair_128 && pair_256 <= one_128 && pair_256 <= one_64) return launch_linear<256, 2, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
-  if (p.M > 128 && pair_128 <= one_128 && pair_128 <= one_64) return launch_linear<128, 2, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
-  if (one_128 <= one_64) return launch_linear<128, 1, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
+  const LinPlan t = ACT == kPartial ? linear_plan(p.rows, p.N, k, true) : linear_plan(p.M, p.N, k, false);
+  if (t.ctas == 2 && t.width == 256) return launch_linear<256, 2, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
+  if (t.ctas == 2) return launch_linear<128, 2, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
+  if (t.width == 128) return launch_linear<128, 1, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
   return launch_linear<64, 1, ACT, OTHER, WIDE, DZ>(a, b, k, bf16, p, st);
 }
 

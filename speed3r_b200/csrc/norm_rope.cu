@@ -613,7 +613,13 @@ __global__ void __launch_bounds__(1024) norm_rope_sums_kernel(const __grid_const
   const bool in = col < 2 * p.head_dim;
   float total = 0.f;
   if (in)
-    for (int64_t i = warp; i < p.rows[part]; i += 32) total += __ldg(p.sums + (p.first[part] + i) * 2 * p.head_dim + col);
+    for (int64_t i = warp; i < p.rows[part]; i += 32 * 8) {        // eight on their way at a time
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < p.rows[part] ? __ldg(p.sums + (p.first[part] + i + 32 * k) * 2 * p.head_dim + col) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) total += v[k];
+    }
   red[warp][lane] = total;
   __syncthreads();
   const int which = col >= p.head_dim;
@@ -631,16 +637,15 @@ __global__ void __launch_bounds__(1024) norm_rope_sums_kernel(const __grid_const
 template <int V, int G, int E, int BYTES, int CB>
 static int run_norm_rope(const NrParams& p, bool backward, unsigned ctas, cudaStream_t st) {
   const dim3 grid(ctas, static_cast<unsigned>(p.q_chunks + 2 * p.kv_chunks));
-  auto run = [&](void (*kernel)(NrParams), int smem) {
-    static std::atomic<uint64_t> ready[2];
-    if (attributes_missing(ready[backward])) {
-      S3R_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      attributes_set(ready[backward]);
-    }
-    return launch(kernel, grid, kNrThreads, smem, st, p);
-  };
-  if (backward) return run(norm_rope_bwd_kernel<V, G, E, BYTES, CB>, Tile<V, G, E, BYTES, CB, 2>::kSmem);
-  return run(norm_rope_fwd_kernel<V, G, E, BYTES, CB>, Tile<V, G, E, BYTES, CB, 1>::kSmem);
+  constexpr int kForward = Tile<V, G, E, BYTES, CB, 1>::kSmem, kBackward = Tile<V, G, E, BYTES, CB, 2>::kSmem;
+  static std::atomic<uint64_t> ready[2];
+  if (attributes_missing(ready[backward])) {
+    if (backward) S3R_CUDA(cudaFuncSetAttribute(norm_rope_bwd_kernel<V, G, E, BYTES, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBackward));
+    else S3R_CUDA(cudaFuncSetAttribute(norm_rope_fwd_kernel<V, G, E, BYTES, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kForward));
+    attributes_set(ready[backward]);
+  }
+  if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES, CB>, grid, kNrThreads, kBackward, st, p);
+  return launch(norm_rope_fwd_kernel<V, G, E, BYTES, CB>, grid, kNrThreads, kForward, st, p);
 }
 // The widest copy of at most 16 bytes that divides rows, addresses and strides, and no narrower than a vector; in between only what V = 1 has.
 template <int V, int G, int E, int BYTES>

@@ -298,7 +298,6 @@ optional<Tensor> gate_of(const optional<Tensor>& gate, const Tensor& x) {
   const Tensor rows = g.expand(whole).reshape({batch, tokens, channels});
   return channels > 1 && rows.stride(2) != 1 ? rows.contiguous() : rows;
 }
-Tensor in_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 NormInputs norm_inputs(const Tensor& x, const optional<Tensor>& y, const optional<Tensor>& w, const optional<Tensor>& b, const optional<Tensor>& s,
                        const optional<Tensor>& gate, const optional<Tensor>& pw, const optional<Tensor>& pb, bool norm, bool post, int64_t kind) {
   TORCH_CHECK(x.dim() >= 1, "residual_norm: x needs a dimension");

@@ -58,6 +58,11 @@ s3r_linear linear_args(const Tensor& x, const Tensor& weight, const Tensor& bias
   TORCH_CHECK(out_type == at::kFloat || out_type == at::kBFloat16 || out_type == at::kHalf, "linear: the result must be fp32, bf16 or fp16, got ", out_type);
   return a;
 }
+// for the parts of a long sum of few rows
+Tensor workspace(const Tensor& like, int64_t M, int64_t N, int64_t K) {
+  const size_t bytes = s3r_linear_workspace_bytes(M, N, K);
+  return bytes ? fresh({static_cast<int64_t>(bytes)}, like, at::kByte) : Tensor();
+}
 Tensor dense(const optional<Tensor>& t) { return t.has_value() ? t->contiguous() : Tensor(); }
 
 Tensor linear_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& scale, const optional<Tensor>& residual,
@@ -77,6 +82,9 @@ Tensor linear_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>&
   s3r_linear f = linear_args(a, w, b, s, n, act, out_type);
   if (r.defined()) f.residual = r.data_ptr(), f.residual_type = type_of(r, "residual");
   f.out = out.data_ptr();
+  const Tensor ws = workspace(x, n.M, n.N, n.K);
+  f.workspace = pointer(ws);
+  f.workspace_bytes = ws.defined() ? ws.numel() : 0;
   check(s3r_linear_fwd(&f, stream()), "s3r_linear_fwd");
   return out;
 }
@@ -118,10 +126,13 @@ std::vector<Tensor> run_linear_bwd(const Tensor& x, const Tensor& weight, const 
     g.workspace = ws.data_ptr();
   }
   check(s3r_linear_bwd(&f, &g, stream()), "s3r_linear_bwd");
-  if (dx.defined())
-    check(s3r_product(dz.data_ptr(), pitch, 0, w.data_ptr(), pitch_of(w), 1, f.type, dx.data_ptr(), n.M, static_cast<int>(n.K), n.N, stream()), "s3r_product");
-  if (dw.defined())
-    check(s3r_product(dz.data_ptr(), pitch, 1, a.data_ptr(), pitch_of(a), 1, f.type, dw.data_ptr(), n.N, static_cast<int>(n.K), n.M, stream()), "s3r_product");
+  auto product = [&](bool turned, const Tensor& other, Tensor& out, int64_t rows, int64_t sum) {
+    const Tensor parts = workspace(x, rows, n.K, sum);
+    check(s3r_product(dz.data_ptr(), pitch, turned, other.data_ptr(), pitch_of(other), 1, f.type, out.data_ptr(), rows, static_cast<int>(n.K), sum, pointer(parts),
+                      parts.defined() ? parts.numel() : 0, stream()), "s3r_product");
+  };
+  if (dx.defined()) product(false, w, dx, n.M, n.N);
+  if (dw.defined()) product(true, a, dw, n.N, n.M);
   return {dx, dw, db, ds};
 }
 std::vector<Tensor> linear_bwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& scale, const Tensor& dy, int64_t act,
@@ -143,6 +154,14 @@ std::vector<Tensor> call_linear_bwd(const Tensor& x, const Tensor& weight, const
   S3R_DISPATCHED(linear_bwd)(x, weight, bias, scale, dy, act, want);
 }
 
+// a residual of x's leading dimensions as rows
+Tensor as_result(const Tensor& residual, const Tensor& x, const LinearSizes& n) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = n.N;
+  TORCH_CHECK(residual.device() == x.device() && residual.sizes() == at::IntArrayRef(shape), "linear: residual must be ", at::IntArrayRef(shape), " on x's device, got ", residual.sizes());
+  return residual.reshape({n.M, n.N});
+}
+
 struct LinearNode : torch::autograd::Function<LinearNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& scale,
                         const optional<Tensor>& residual, int64_t act, int64_t out_type) {
@@ -152,10 +171,22 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (scale.has_value()) present |= 8;
     if (residual.has_value()) present |= 16;
     const int64_t kept = residual.has_value() ? static_cast<int64_t>(residual->scalar_type()) : 0;
-    ctx->save_for_backward({x, weight, value(bias), value(scale)});
     ctx->saved_data["ints"] = std::vector<int64_t>{present, act, kept};
     ctx->set_materialize_grads(false);
-    return call_linear_fwd(x, weight, bias, scale, residual, act, static_cast<at::ScalarType>(out_type));
+    if (!plain(x)) {
+      ctx->save_for_backward({x, weight, value(bias), value(scale)});
+      return call_linear_fwd(x, weight, bias, scale, residual, act, static_cast<at::ScalarType>(out_type));
+    }
+    // what is laid out anew is kept that way
+    const LinearSizes n = linear_sizes(x, weight, bias, scale);
+    c10::cuda::CUDAGuard guard(x.device());
+    const Tensor a = n.M ? half_rows(x, n.M, n.K) : x, w = n.M ? half_rows(weight, n.N, n.K) : weight;
+    ctx->save_for_backward({a, w, value(bias), value(scale)});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    Tensor out = linear_fwd(a, w, bias, scale, residual.has_value() && n.M ? optional<Tensor>(as_result(*residual, x, n)) : residual, act, static_cast<at::ScalarType>(out_type));
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n.N;
+    return in_shape(out, shape);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     return once(g, [&] { return gradients(ctx, g); });
@@ -173,6 +204,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const auto g = call_linear_bwd(s[0], s[1], maybe(s[2]), maybe(s[3]), incoming[0].contiguous(), ints[1], want & 15);
       for (int i = 0; i < 4; ++i)
         if (want >> i & 1) out[i] = g[i];
+      if (out[0].defined() && ctx->saved_data.count("shape")) out[0] = in_shape(out[0], ctx->saved_data["shape"].toIntVector());
     }
     return out;
   }

@@ -131,6 +131,7 @@ const void* pointer(const optional<Tensor>& t) { return t.has_value() && t->defi
 void* pointer(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 Tensor value(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+Tensor in_shape(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.view(shape); }
 // parameters of several types are taken in fp32
 void of_one_type(std::initializer_list<optional<Tensor>*> params) {
   bool mixed = false;

@@ -111,7 +111,7 @@ def test_operators_are_traced():
 class LinearArgs(C.Structure):
     _fields_ = [("M", C.c_int64), ("N", C.c_int), ("K", C.c_int), ("type", C.c_int), ("x", C.c_void_p), ("x_pitch", C.c_int64), ("weight", C.c_void_p),
                 ("w_pitch", C.c_int64), ("bias", C.c_void_p), ("scale", C.c_void_p), ("residual", C.c_void_p), ("bias_type", C.c_int), ("scale_type", C.c_int),
-                ("residual_type", C.c_int), ("act", C.c_int), ("out", C.c_void_p), ("out_type", C.c_int)]
+                ("residual_type", C.c_int), ("act", C.c_int), ("out", C.c_void_p), ("out_type", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class LinearGrad(C.Structure):
@@ -163,7 +163,7 @@ def test_c_abi_refuses_linear_gradients(lib):
 
 
 def test_c_abi_refuses_products(lib):
-    ok = dict(a=P, a_pitch=40, at=0, b=P, b_pitch=40, bt=0, type=1, out=P, M=64, N=32, K=40)
+    ok = dict(a=P, a_pitch=40, at=0, b=P, b_pitch=40, bt=0, type=1, out=P, M=64, N=32, K=40, workspace=None, bytes=0)
     call = lambda **more: lib.s3r_product(*{**ok, **more}.values(), None)
     assert call(a=None) == call(b=None) == call(out=None) == NULL
     assert call(M=0) == call(N=0) == call(K=0) == call(a_pitch=39) == call(at=1) == call(b_pitch=24) == SHAPE

@@ -248,8 +248,11 @@ def test_linear_beyond_32_bits():
     for rows in (slice(0, 3), slice(M - 300, M)):
         assert torch.equal(y[rows], ops.linear(x[rows].repeat(1 + 16 // x[rows].shape[0], 1), w, act="gelu")[:x[rows].shape[0]])
     dx = torch.autograd.grad(ops.linear(x.requires_grad_(True), w, act="gelu"), x, y)[0]
+    # few rows take their sums in parts: N products in another order, each addition off by at most 2^-23 of the magnitudes, and two roundings
     tail = x.detach()[-300:].requires_grad_(True)
-    assert torch.equal(dx[-300:], torch.autograd.grad(ops.linear(tail, w, act="gelu"), tail, y[-300:])[0])
+    want = torch.autograd.grad(ops.linear(tail, w, act="gelu"), tail, y[-300:])[0].double()
+    size = 1.13 * y[-300:].double().abs() @ w.double().abs()
+    assert ((dx[-300:].double() - want).abs() <= 4 * F32 * (N + 2) * size + 2 * half_step(BF16) * want.abs()).all()
     del y, dx, x
     x = torch.zeros(N, M, device=DEV, dtype=BF16)                                          # as an operand
     x[-1], x[-2, ::2] = 1.0, 1.0

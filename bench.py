@@ -470,7 +470,8 @@ def run_train_step(args):
 
 def run_block(args):
     """Forward of one transformer block around the sparse attention (1024 wide, MLP of 4096, bf16 autocast, no gradients) on `--views`
-    views: its modules one by one, with the sums and norms in one pass, and with 8-bit projections and MLP as well."""
+    views: its modules one by one, with the sums and norms in one pass, with the MLP's matrices, GELU and last sum as well, and with 8-bit
+    projections and MLP."""
     import torch
     import speed3r_b200
     torch.cuda.set_device(0)
@@ -499,6 +500,10 @@ def run_block(args):
     apart, y0 = timed()
     del blk._fuses
     fused, y1 = timed()
+    mlp, blk.mlp = blk.mlp, speed3r_b200.FusedMlp(H * D, 4 * H * D).to(dev).eval()
+    blk.mlp.load_state_dict(mlp.state_dict())
+    fused_mlp, y3 = timed()
+    blk.mlp = mlp
     blk.quantize_int8()
     int8, y2 = timed()
     off = lambda y: ((y - x).double() - (y0 - x).double()).norm().item() / (y0 - x).double().norm().item()
@@ -506,7 +511,7 @@ def run_block(args):
         metric="block_forward_tokens_per_s", value=T / (fused * 1e-3), unit="tokens/s", n_gpus=1, steps=args.steps, warmup=max(3, args.warmup),
         ms_per_step=fused, higher_is_better=True, scaling="weak", vs_baseline=None, dtype="bf16", data="synthetic",
         config={"workload": f"one transformer block, forward, {args.views} views of 392x504, dim 1024, 16 heads, MLP 4096", "tokens": T},
-        modules_one_by_one_ms=apart, int8_ms=int8, fused_off=off(y1), int8_off=off(y2), device_status=_lib_status())))
+        modules_one_by_one_ms=apart, fused_mlp_ms=fused_mlp, int8_ms=int8, fused_off=off(y1), fused_mlp_off=off(y3), int8_off=off(y2), device_status=_lib_status())))
 
 
 def run_extension(args):

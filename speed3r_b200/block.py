@@ -40,6 +40,52 @@ class Mlp(nn.Module):
         return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
 
 
+def product_type(x, *linears: nn.Module) -> Optional[torch.dtype]:
+    """The type in which ``ops.linear`` computes these Linears on x as autocast, or else x, wants them; None where they are to be called instead:
+    something else than plain Linears, hooks, other types or devices."""
+    if not isinstance(x, Tensor) or not x.is_cuda or _global_hooks() or any(type(m) is not nn.Linear or _watched(m) for m in linears):
+        return None
+    autocast = torch.is_autocast_enabled("cuda")
+    t = torch.get_autocast_dtype("cuda") if autocast else x.dtype
+    params = [p for m in linears for p in m._parameters.values() if p is not None]
+    if t not in (torch.bfloat16, torch.float16) or any(p.device != x.device for p in params):
+        return None
+    if autocast:
+        return t if x.dtype in ops.NORM_TYPES and all(p.dtype in ops.NORM_TYPES for p in params) else None
+    return t if all(p.dtype == t for p in params) else None
+
+
+class FusedMlp(Mlp):
+    """``Mlp`` whose matrices come with what follows them (``ops.linear``): the activation, and on request a LayerScale and the residual.  For
+    ``BlockRope(ffn_layer=FusedMlp)``; parameters and results are ``Mlp``'s, but that nothing is rounded between a matrix and its activation.  Where
+    the kernel does not reach - other types than bf16 and fp16, active dropout, hooks, an activation other than GELU and SiLU - modules are called
+    one by one."""
+
+    def _act(self) -> Optional[str]:
+        m = self.act
+        if _watched(m):
+            return None
+        if type(m) is nn.GELU:
+            return "gelu" if m.approximate == "none" else "gelu_tanh"
+        return "silu" if type(m) is nn.SiLU else None
+
+    def _type(self, x) -> Optional[torch.dtype]:
+        if self._act() is None or _watched(self.drop) or (self.drop.p and self.drop.training):
+            return None
+        return product_type(x, self.fc1, self.fc2)
+
+    def forward(self, x, residual: Optional[Tensor] = None, scale: Optional[Tensor] = None) -> Tensor:
+        """``residual + mlp(x) * scale``, in the residual's type, or the MLP alone"""
+        t = self._type(x)
+        if t is None:
+            y = super().forward(x)
+            y = y if scale is None else y * scale
+            return y if residual is None else residual + y
+        of = lambda p: None if p is None else p.to(t)
+        h = ops.linear(x.to(t), of(self.fc1.weight), self.fc1.bias, self._act())
+        return ops.linear(h, of(self.fc2.weight), self.fc2.bias, None, residual, scale, t if residual is None else residual.dtype)
+
+
 def _norm_args(m: nn.Module, dim: int) -> Optional[Tuple[str, tuple]]:
     """(kind, (weight, bias, eps)) of a norm that ``ops.residual_norm`` computes, None for any other module."""
     if _watched(m):
@@ -144,6 +190,8 @@ class BlockRope(nn.Module):
     def _run(self, x: Tensor, h: Union[Tensor, Int8Tokens], xpos, next_norm: Optional[nn.Module], next_int8: bool):
         a = self.attn(h, xpos=xpos)
         x, h = self._sum_and_norm(x, a, self.norm2, self._scale(self.ls1), self._gate(x), self._mlp_takes_int8())
+        if next_norm is None and type(self.mlp) is FusedMlp and not _watched(self.mlp) and not (self.training and self.drop_path) and self.mlp._type(h) is not None:
+            return self.mlp(h, residual=x, scale=self._scale(self.ls2)), None            # nothing comes behind the sum: it leaves with the product
         return self._sum_and_norm(x, self.mlp(h), next_norm, self._scale(self.ls2), self._gate(x), next_int8)
 
     def _mlp_takes_int8(self) -> bool:

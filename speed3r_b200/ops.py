@@ -8,7 +8,7 @@ Public functions mirror the reference's op signatures:
   (pi3/models/sparse_attn/topk_blocksparse_attention.py:1093-1121)
 
 the rest of a block around them (``residual_norm``), its projections in 8 bits (``quantize_tokens``, ``int8_linear``) and the step
-that ends a training iteration (``grad_norm``, ``adamw_step``), plus the pieces the reference leaves to eager PyTorch (sparse_attention.py:97-102, 127-136):
+that ends a training iteration (``grad_norm``, ``adamw_step``), the dense half of a block (``linear``, ``qkv_norm_rope``), plus the pieces the reference leaves to eager PyTorch (sparse_attention.py:97-102, 127-136):
 
 * ``pool_tokens(x, kernel, stride)``: mean pooling along the sequence
 * ``sel_attn_merge(q, k, v, idx, gate, o_c, block_size)``: selection attention with the gated
@@ -17,7 +17,7 @@ that ends a training iteration (``grad_norm``, ``adamw_step``), plus the pieces 
 Allocation, argument checks and autograd wiring are native (``csrc/torch/bindings.cpp``, a ``torch.library``
 namespace over the C ABI); this file holds the Python signatures and the shape functions for
 ``torch.compile``.  CPU tensors, types that an operator does not take (the attention's take bf16, the operators around it fp32 and
-fp16 too) and a missing library raise: there is no fallback.
+fp16 too, matrix products bf16 and fp16) and a missing library raise: there is no fallback.
 """
 from __future__ import annotations
 

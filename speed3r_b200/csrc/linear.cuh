@@ -87,7 +87,8 @@ int linear_partial(const LinOperand& a, const LinOperand& b, int64_t k, bool bf1
 // Either operand lies with the contraction contiguous ([rows][k]: x, W of the forward, dz of dx) or turned ([k][rows]: W of dx, dz and x of dW);
 // a turned one comes in boxes of 64 rows x 64 steps and is read through the other form of the matrix descriptor.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kLinFirst = 4, kLinWarps = 8, kLinThreads = 32 * (kLinFirst + kLinWarps);      // warps 0 and 1 feed, the last eight take the sums
+// Warps 0 and 1 feed, the last eight take the sums.  Two in between do nothing: without them every kind of epilogue took 4 to 10 % longer.
+constexpr int kLinFirst = 4, kLinWarps = 8, kLinThreads = 32 * (kLinFirst + kLinWarps);
 constexpr int kLinPiece = 4096;                                    // a warp's piece of the output: 32 rows of 128 bytes
 constexpr int kLinStep = 64;                                       // elements of the contraction per stage: 128 bytes
 constexpr int kNoOther = -1, kAnyAct = -1, kPartial = -2;
@@ -101,7 +102,7 @@ struct LinParams {
   int parts, row_tiles, part_steps;           // kPartial: tiles of a's rows, steps of a part; m_tiles is that of all parts, M their rows
   int bias_type, scale_type, other_type, out_type, act;
   uint32_t idesc, a_turned, b_turned, copy_out, other_vectors;         // other's rows: in vectors of 16 bytes (the residual), in pairs (dy)
-  uint32_t other_copied;               // dy by TMA
+  uint32_t other_copied;               // dy | the residual by TMA
   uint32_t* status;
 };
 
@@ -259,7 +260,7 @@ __device__ __forceinline__ float column_sum(const float2 (&d)[4], int lane) {
 template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
                                                              const __grid_constant__ CUtensorMap mo, const __grid_constant__ CUtensorMap md, const __grid_constant__ LinParams p) {
-  using C = LinCfg<TN, CTAS, DZ ? 2 : 1>;
+  using C = LinCfg<TN, CTAS, DZ || OTHER != kNoOther ? 2 : 1>;
   extern __shared__ char raw_smem[];
   __shared__ LinCtl ctl;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       mbar_init(&ctl.acc_full[s], 1);
       mbar_init(&ctl.acc_empty[s], CTAS * kLinWarps);
     }
-    if (DZ)
+    if (OTHER != kNoOther)
       for (int s = 0; s < 2 * kLinWarps; ++s) mbar_init(&ctl.piece_full[s / 2][s % 2], 1);
     mbar_init(&ctl.drained, 1);
     mbar_init(&ctl.pause, 1);
@@ -310,9 +311,6 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
     if (t.n >= p.n_tiles) t.n -= p.n_tiles, ++t.m;
   };
   const uint32_t base = smem_u32(smem);
-
-  if (warp < kLinFirst) reg_dealloc<40>();
-  else reg_alloc<232>();
 
   if (warp == 0) {
     int n = 0;                                                     // copies so far
@@ -391,36 +389,239 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       }
     }
   } else if (warp >= kLinFirst) {
-   if constexpr (!DZ) {
-    const int quarter = warp & 3, half = (warp - kLinFirst) >> 2;  // lanes 32 * quarter .. of tensor memory; half of the columns
-    char* piece = smem + C::kOut + (warp - kLinFirst) * kLinPiece;
-    float* factors = reinterpret_cast<float*>(smem + C::kColumns) + (warp - kLinFirst) * 2 * C::kSpan;     // scales and biases of its columns
-    constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
-    const int from = half * C::kSpan;
-    constexpr int kMine = C::kSpan / 32;
-    // What the next tile needs is asked for a tile ahead, and its first part of the residual | of dy; the other parts 32 columns ahead.
-    Raw<1> scales[kMine], biases[kMine];
-    uint32_t o[OTHER == kNoOther ? 1 : OTHER == S3R_F32 ? 32 : 16];
-    auto fetch = [&](int tile, Tile at) {
+    if constexpr (!DZ) {
+      const int me = warp - kLinFirst, quarter = warp & 3, from = (me >> 2) * C::kSpan;      // lanes 32 * quarter .. of tensor memory; its first column
+      float* factors = reinterpret_cast<float*>(smem + C::kColumns) + me * 2 * C::kSpan;     // scales and biases of its columns
+      constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
+      constexpr int kMine = C::kSpan / 32, kPieces = OTHER == kNoOther ? 1 : 2;
+      // A residual of the result's size comes by TMA into the piece that the sum leaves from, a piece ahead; rows that a lane reads from memory itself,
+      // 16 bytes of 32 lines at a time, took 1092 us for 64 512 x 4096 in fp32 where this way takes {RES}.  Other residuals are read 32 columns ahead.
+      constexpr bool kInPlace = OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
+      const bool by_copy = kInPlace && p.other_copied;
+      // What the next tile needs is asked for a tile ahead.
+      Raw<1> scales[kMine], biases[kMine];
+      uint32_t o[OTHER == kNoOther ? 1 : OTHER == S3R_F32 ? 32 : 16];
+      auto fetch = [&](int tile, Tile at) {
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int col = at.n * TN + from + i * 32 + lane;
-        const bool in = tile < tiles && col < p.N;
-        load_raw<1>(scales[i], p.scale, p.scale_type, col, in && p.scale);
-        load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
+        for (int i = 0; i < kMine; ++i) {
+          const int col = at.n * TN + from + i * 32 + lane;
+          const bool in = tile < tiles && col < p.N;
+          load_raw<1>(scales[i], p.scale, p.scale_type, col, in && p.scale);
+          load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
+        }
+      };
+      auto ahead = [&](int tile, Tile at, int g) {
+        if constexpr (OTHER != kNoOther) {
+          if (by_copy || tile >= tiles) return;
+          const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+          const int col = at.n * TN + from + g * 32, end = min(p.N, at.n * TN + min(from + C::kSpan, TN));
+          load_row<OTHER>(o, p.other, (row + lane) * p.N + col, row + lane < p.M ? end - col : 0, p.other_vectors);
+        }
+      };
+      // its rows, a lane each, into L2: what is asked for 32 columns ahead would wait for memory longer than those columns take
+      auto soon = [&](int tile, Tile at) {
+        if constexpr (OTHER != kNoOther) {
+          const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + lane;
+          const int col = at.n * TN + from, n = min(p.N, at.n * TN + min(from + C::kSpan, TN)) - col;
+          if (tile >= tiles || row >= p.M) return;
+          const char* first_byte = static_cast<const char*>(p.other) + (row * p.N + col) * type_bytes(OTHER);
+#pragma unroll
+          for (int i = 0; i < C::kSpan * type_bytes(OTHER) / 128; ++i)
+            if (i * (128 / type_bytes(OTHER)) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(first_byte + 128 * i));
+        }
+      };
+      auto piece_at = [&](uint32_t q) { return smem + C::kOut + (me * kPieces + q % kPieces) * kLinPiece; };
+      // The next piece to ask for; pieces without columns are left out everywhere.
+      Tile at = begin, after = begin, asked = begin;
+      int asked_tile = first, asked_piece = 0;
+      uint32_t asks = 0, q = 0;
+      auto ask_next = [&] {
+        while (asked_tile < tiles) {
+          const int c0 = from + asked_piece * per, n0 = asked.n * TN;
+          const bool there = c0 < TN && n0 + c0 < p.N;
+          if (there && lane == 0) {
+            mbar_expect_tx(&ctl.piece_full[me][asks & 1], kLinPiece);
+            tma_load_2d<1>(smem_u32(piece_at(asks)), &md, smem_u32(&ctl.piece_full[me][asks & 1]), n0 + c0, (asked.m * CTAS + rank) * 128 + quarter * 32);
+          }
+          asks += there;
+          if (++asked_piece == C::kSpan / per) {
+            asked_piece = 0;
+            asked_tile += stride;
+            advance(asked);
+          }
+          if (there) return;
+        }
+      };
+      fetch(first, at);
+      soon(first, at);
+      if (by_copy) {
+        ask_next();
+        ask_next();
       }
-    };
-    auto ahead = [&](int tile, Tile at, int g) {
-      if constexpr (OTHER != kNoOther) {
-        if (tile >= tiles) return;
+      ahead(first, at, 0);
+      int done = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
+        const int buf = done & 1;
+        const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+        const int n0 = at.n * TN;
+        const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
+        __syncwarp();                                                // the last tile's factors are read
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          float f[1];
+          unpack<1>(f, scales[i], p.scale_type);
+          factors[i * 32 + lane] = p.scale ? f[0] : 1.f;
+          unpack<1>(f, biases[i], p.bias_type);
+          factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
+        }
+        __syncwarp();
+        advance(after);
+        fetch(tile + stride, after);
+        soon(tile + stride, after);
+        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        // 32 columns' sums; when they are there, or have been used, the next 32 are asked for; the last ones free the tile's columns
+        const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
+        constexpr int kSets = OTHER == kNoOther ? 2 : 1;               // what is added takes the other set's place
+        uint32_t two[kSets][32];
+        auto take = [&](int g) {
+          if (from >= TN) return;
+          tmem_ld32(sums + g * 32, two[g % kSets]);
+        };
+        auto taken = [&](int g) {
+          if (g + 1 < kMine) {
+            take(g + 1);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+          }
+        };
+        take(0);
+#pragma unroll
+        for (int g = 0; g < kMine; ++g) {
+          uint32_t x[WIDE ? 32 : 16];                                // as it is stored
+          const bool some = from + g * 32 < width;
+          const int half_piece = WIDE ? 0 : g & 1;
+          char* piece = piece_at(q);
+          const float *s = factors + g * 32, *b = s + C::kSpan;
+          uint32_t (&v)[32] = two[g % kSets];
+          tmem_ld_wait_for(v);
+          if (kSets == 2) taken(g);
+          if constexpr (kInPlace) {
+            if (by_copy && some) {
+              if (!half_piece) {
+                ok = mbar_wait_warp(&ctl.piece_full[me][q & 1], q >> 1 & 1, abort_flag);
+                if (!ok) break;
+              }
+#pragma unroll
+              for (int k = 0; k < (WIDE ? 8 : 4); ++k) {
+                const uint4 w = lds128(smem_u32(piece + swz128(lane, half_piece * 4 + k)));
+                o[4 * k] = w.x, o[4 * k + 1] = w.y, o[4 * k + 2] = w.z, o[4 * k + 3] = w.w;
+              }
+              if (!half_piece && asks - q < 2) {                     // the piece before has left its place: the one behind this one comes there
+                if (lane == 0) bulk_wait_read();
+                __syncwarp();
+                ask_next();
+              }
+            }
+          }
+          {
+            float2 y[16];
+            auto columns = [&](auto act) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const float4 add = *reinterpret_cast<const float4*>(b + k);
+                float2 slope;
+                y[k / 2] = activate<decltype(act)::value, false>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), make_float2(add.x, add.y)), slope);
+                y[k / 2 + 1] = activate<decltype(act)::value, false>(fadd2(make_float2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])), make_float2(add.z, add.w)), slope);
+              }
+              return 0;
+            };
+            if constexpr (ACT == kAnyAct) with_act(p.act, columns);
+            else if constexpr (ACT == kPartial) columns(std::integral_constant<int, S3R_ACT_NONE>());
+            else columns(std::integral_constant<int, ACT>());
+            if (OTHER != kNoOther || p.scale) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(s + k);
+                const float2 lo = make_float2(f.x, f.y), hi = make_float2(f.z, f.w);
+                y[k / 2] = OTHER == kNoOther ? fmul2(y[k / 2], lo) : ffma2(y[k / 2], lo, other_pair<OTHER>(o, k));
+                y[k / 2 + 1] = OTHER == kNoOther ? fmul2(y[k / 2 + 1], hi) : ffma2(y[k / 2 + 1], hi, other_pair<OTHER>(o, k + 2));
+              }
+            }
+            pack_pairs<WIDE>(x, y, p.out_type);
+          }
+          if (kSets == 1) taken(g);
+          if (g + 1 < kMine) ahead(tile, at, g + 1);
+          else ahead(tile + stride, after, 0);
+          if (some) {
+            if (!half_piece && !by_copy) {
+              if (lane == 0) kPieces == 2 ? bulk_wait_read_but_one() : bulk_wait_read();     // the store before has left this piece
+              __syncwarp();
+            }
+            // rows of 128 bytes, their 16-byte chunks swizzled by the row
+#pragma unroll
+            for (int k = 0; k < (WIDE ? 8 : 4); ++k)
+              *reinterpret_cast<uint4*>(piece + swz128(lane, half_piece * 4 + k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+            if (WIDE || half_piece || from + g * 32 + 32 >= width) {
+              ++q;
+              const int c0 = from + (g - half_piece) * 32;
+              if (p.copy_out) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  if (m0 < p.M) tma_store_2d(&mo, smem_u32(piece), n0 + c0, static_cast<int>(m0));
+                  bulk_commit();
+                }
+              } else {
+                __syncwarp();
+                constexpr int kSize = WIDE ? 4 : 2;
+                store_lines<WIDE ? S3R_F32 : S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * kSize, p.out_pitch * kSize, piece,
+                                                       min(per, width - c0), static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
+                __syncwarp();                                        // read before the next piece is written
+              }
+            }
+          }
+        }
+      }
+      if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
+        volatile uint32_t dummy;
+        for (uint32_t k = asks > 2 ? asks - 2 : 0; k < asks; ++k) {
+          dummy = 0;
+          mbar_wait(&ctl.piece_full[me][k & 1], k >> 1 & 1, &dummy);
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+      if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
+    } else {
+      const int me = warp - kLinFirst, quarter = warp & 3, from = (me >> 2) * C::kSpan;
+      float* factors = reinterpret_cast<float*>(smem + C::kColumns) + me * 2 * C::kSpan;
+      constexpr int kMine = C::kSpan / 32, kPerTile = C::kSpan / 64;
+      const int r = lane >> 2, c = 2 * (lane & 3);                   // rows r, r + 8, r + 16, r + 24, of every eight columns two from c on
+      // dy of 16 bits comes by TMA, 32 rows x 64 columns into one of two pieces, where dz takes its place and leaves by TMA as well; half a piece
+      // ahead.  In the layout of tensor memory's 16 x 256 bits a lane's elements are those of 8 x 8 matrices.  Other dy is read from memory, fp32
+      // 32 columns ahead.
+      const bool by_copy = OTHER != S3R_F32 && p.other_copied;
+      Raw<1> scales[kMine], biases[kMine];
+      uint32_t o[OTHER == S3R_F32 ? 32 : 16];
+      auto fetch = [&](int tile, Tile at) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int col = at.n * TN + from + i * 32 + lane;
+          const bool in = tile < tiles && col < p.N;
+          if (DZ == 2) load_raw<1>(scales[i], p.scale, p.scale_type, col, in);
+          load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
+        }
+      };
+      auto ahead = [&](int tile, Tile at, int g) {
+        if (OTHER != S3R_F32 || tile >= tiles) return;
         const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
-        const int col = at.n * TN + from + g * 32, end = min(p.N, at.n * TN + min(from + C::kSpan, TN));
-        load_row<OTHER>(o, p.other, (row + lane) * p.N + col, row + lane < p.M ? end - col : 0, p.other_vectors);
-      }
-    };
-    // its rows, a lane each, into L2: what is asked for 32 columns ahead would wait for memory longer than those columns take
-    auto soon = [&](int tile, Tile at) {
-      if constexpr (OTHER != kNoOther) {
+        load_square<OTHER>(o, p.other, row + r, p.M, p.N, at.n * TN + from + g * 32 + c, min(p.N, at.n * TN + min(from + C::kSpan, TN)), p.other_vectors);
+      };
+      auto soon = [&](int tile, Tile at) {                           // its rows, a lane each, into L2
         const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + lane;
         const int col = at.n * TN + from, n = min(p.N, at.n * TN + min(from + C::kSpan, TN)) - col;
         if (tile >= tiles || row >= p.M) return;
@@ -428,96 +629,147 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < C::kSpan * type_bytes(OTHER) / 128; ++i)
           if (i * (128 / type_bytes(OTHER)) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(first_byte + 128 * i));
-      }
-    };
-    Tile at = begin, after = begin;
-    fetch(first, at);
-    soon(first, at);
-    ahead(first, at, 0);
-    int done = 0;
-    bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
-      const int buf = done & 1;
-      const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
-      const int n0 = at.n * TN;
-      const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
-      __syncwarp();                                                // the last tile's factors are read
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        float f[1];
-        unpack<1>(f, scales[i], p.scale_type);
-        factors[i * 32 + lane] = p.scale ? f[0] : 1.f;
-        unpack<1>(f, biases[i], p.bias_type);
-        factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
-      }
-      __syncwarp();
-      advance(after);
-      fetch(tile + stride, after);
-      soon(tile + stride, after);
-      ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      // 32 columns' sums; when they are there the next 32 are asked for, into the other registers, and the last ones free the tile's columns
-      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t two[2][32];
-      auto take = [&](int g) {
-        if (from >= TN) return;
-        tmem_ld32(sums + g * 32, two[g & 1]);
       };
-      take(0);
-#pragma unroll
-      for (int g = 0; g < kMine; ++g) {
-        uint32_t x[WIDE ? 32 : 16];                                // as it is stored
-        const float *s = factors + g * 32, *b = s + C::kSpan;
-        uint32_t (&v)[32] = two[g & 1];
-        tmem_ld_wait_for(v);
-        if (g + 1 < kMine) {
-          take(g + 1);
-        } else {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+      auto piece_at = [&](uint32_t q) { return smem + C::kOut + (me * 2 + (q & 1)) * kLinPiece; };
+      // piece h of a tile, number q of this warp's: asked for; pieces without columns are left out everywhere
+      auto has = [&](Tile at, int h) { return from + h * 64 < TN && at.n * TN + from + h * 64 < p.N; };
+      auto ask = [&](Tile at, int h, uint32_t q) {
+        if (lane == 0) {
+          mbar_expect_tx(&ctl.piece_full[me][q & 1], kLinPiece);
+          tma_load_2d<1>(smem_u32(piece_at(q)), &md, smem_u32(&ctl.piece_full[me][q & 1]), at.n * TN + from + h * 64, (at.m * CTAS + rank) * 128 + quarter * 32);
         }
-        {
-          float2 y[16];
-          auto columns = [&](auto act) {
+      };
+      Tile at = begin, after = begin, asked = begin;                 // asked, asked_tile, asked_piece: the next piece to ask for
+      int asked_tile = first, asked_piece = 0;
+      uint32_t asks = 0, q = 0;
+      auto ask_next = [&] {
+        while (asked_tile < tiles) {
+          const bool there = has(asked, asked_piece);
+          if (there) ask(asked, asked_piece, asks++);
+          if (++asked_piece == kPerTile) {
+            asked_piece = 0;
+            asked_tile += stride;
+            advance(asked);
+          }
+          if (there) return;
+        }
+      };
+      fetch(first, at);
+      soon(first, at);
+      if (by_copy) {
+        ask_next();
+        ask_next();
+      }
+      ahead(first, at, 0);
+      int done = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
+        const int buf = done & 1;
+        const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
+        const int n0 = at.n * TN;
+        const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
+        __syncwarp();                                                // the last tile's factors are read
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 add = *reinterpret_cast<const float4*>(b + k);
+        for (int i = 0; i < kMine; ++i) {
+          float f[1];
+          if (DZ == 2) {
+            unpack<1>(f, scales[i], p.scale_type);
+            factors[i * 32 + lane] = f[0];
+          }
+          unpack<1>(f, biases[i], p.bias_type);
+          factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
+        }
+        __syncwarp();
+        advance(after);
+        fetch(tile + stride, after);
+        soon(tile + stride, after);
+        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
+        uint32_t v[32];
+        if (from < TN) tmem_ld_32x32(sums, v);
+        const bool whole = m0 + 32 <= p.M;
+#pragma unroll
+        for (int g = 0; g < kMine; ++g) {
+          const bool some = from + g * 32 < width;
+          char* piece = piece_at(q);
+          // matrices (i, j): rows 8 i .. of columns 8 j ..; lane l gives the address of row l % 8 of matrix l / 8
+          auto matrix_row = [&](int j) { return smem_u32(piece + swz128(lane, (g & 1) * 4 + j)); };
+          tmem_ld_wait_for(v);
+          if (OTHER != S3R_F32 && some) {
+            if (by_copy) {
+              if (!(g & 1)) ok = mbar_wait_warp(&ctl.piece_full[me][q & 1], q >> 1 & 1, abort_flag);
+              if (!ok) break;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) ldsm_x4(o[j], o[4 + j], o[8 + j], o[12 + j], matrix_row(j));
+            } else {
+              load_square<OTHER>(o, p.other, m0 + r, p.M, p.N, n0 + from + g * 32 + c, n0 + width, p.other_vectors);
+            }
+          }
+          float2 y[16], db[4], ds[4];
+          const float *s = factors + g * 32, *b = s + C::kSpan;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = *reinterpret_cast<const float2*>(s + 8 * j + c), add = *reinterpret_cast<const float2*>(b + 8 * j + c);
+            ds[j] = both(0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
               float2 slope;
-              y[k / 2] = activate<decltype(act)::value, false>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), make_float2(add.x, add.y)), slope);
-              y[k / 2 + 1] = activate<decltype(act)::value, false>(fadd2(make_float2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])), make_float2(add.z, add.w)), slope);
-            }
-            return 0;
-          };
-          if constexpr (ACT == kAnyAct) with_act(p.act, columns);
-          else if constexpr (ACT == kPartial) columns(std::integral_constant<int, S3R_ACT_NONE>());
-          else columns(std::integral_constant<int, ACT>());
-          if (OTHER != kNoOther || p.scale) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(s + k);
-              const float2 lo = make_float2(f.x, f.y), hi = make_float2(f.z, f.w);
-              y[k / 2] = OTHER == kNoOther ? fmul2(y[k / 2], lo) : ffma2(y[k / 2], lo, other_pair<OTHER>(o, k));
-              y[k / 2 + 1] = OTHER == kNoOther ? fmul2(y[k / 2 + 1], hi) : ffma2(y[k / 2 + 1], hi, other_pair<OTHER>(o, k + 2));
+              const float2 u = activate<ACT, true>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), add), slope);
+              const float2 dy = other_pair<OTHER>(o, (i * 4 + j) * 2);
+              y[i * 4 + j] = fmul2(DZ == 2 ? fmul2(dy, f) : dy, slope);
+              if (DZ == 2) ds[j] = ffma2(dy, whole || m0 + r + 8 * i < p.M ? u : both(0.f), ds[j]);
             }
           }
-          pack_pairs<WIDE>(x, y, p.out_type);
-        }
-        if (g + 1 < kMine) ahead(tile, at, g + 1);
-        else ahead(tile + stride, after, 0);
-        if (from + g * 32 < width && p.out) {
-          const int half_piece = WIDE ? 0 : g & 1;
-          if (!half_piece) {
-            if (lane == 0) bulk_wait_read();                       // the store before has left this piece
+          if (!whole) {                                              // a row that is not there has dy = 0, but may have any z
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (m0 + r + 8 * (k >> 2) >= p.M) y[k] = both(0.f);
+          }
+          if (g + 1 < kMine) {
+            if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v);
+            ahead(tile, at, g + 1);
+          } else {                                                   // this warp's sums are in registers
+            tc_fence_before();
             __syncwarp();
+            if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
+            ahead(tile + stride, after, 0);
           }
-          // rows of 128 bytes, their 16-byte chunks swizzled by the row
+          const int col = from + g * 32 + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
+          const int64_t to = (m0 >> 5) * p.N + n0 + col;
+          const bool there = m0 < p.M && col < width;
+          if (p.bias_sums) {
 #pragma unroll
-          for (int k = 0; k < (WIDE ? 8 : 4); ++k)
-            *reinterpret_cast<uint4*>(piece + swz128(lane, half_piece * 4 + k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-          if (WIDE || half_piece || g + 1 == kMine || from + g * 32 + 32 >= width) {
-            const int c0 = from + (g - half_piece) * 32;
+            for (int j = 0; j < 4; ++j) db[j] = fadd2(fadd2(y[j], y[4 + j]), fadd2(y[8 + j], y[12 + j]));
+            const float sum = column_sum(db, lane);
+            if (there) p.bias_sums[to] = sum;
+          }
+          if (DZ == 2 && p.scale_sums) {
+            const float sum = column_sum(ds, lane);
+            if (there) p.scale_sums[to] = sum;
+          }
+          if (!some) continue;
+          if (p.out) {
+            if (!(g & 1) && !by_copy) {
+              if (lane == 0) bulk_wait_read_but_one();               // the store before the last has left this piece
+              __syncwarp();
+            }
+            uint32_t x[16];
+            pack_pairs<false>(x, y, p.out_type);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) stsm_x4(matrix_row(j), x[j], x[4 + j], x[8 + j], x[12 + j]);
+          }
+          const bool last = (g & 1) || from + g * 32 + 32 >= width;
+          if (by_copy && (!(g & 1)) && q > 0) {                      // the piece before has left its place: the one behind this one comes there
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
+            ask_next();
+          }
+          if (!last) continue;
+          if (p.out) {
+            const int c0 = from + (g & ~1) * 32;
             if (p.copy_out) {
               fence_proxy_async_smem();
               __syncwarp();
@@ -527,217 +779,23 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
               }
             } else {
               __syncwarp();
-              constexpr int kSize = WIDE ? 4 : 2;
-              store_lines<WIDE ? S3R_F32 : S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * kSize, p.out_pitch * kSize, piece,
-                                                     min(per, width - c0), static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
-              __syncwarp();                                        // read before the next piece is written
+              store_lines<S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * 2, p.out_pitch * 2, piece, min(64, width - c0),
+                                    static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
             }
           }
+          ++q;
         }
       }
+      if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
+        volatile uint32_t dummy;
+        for (uint32_t i = asks > 2 ? asks - 2 : 0; i < asks; ++i) {
+          dummy = 0;
+          mbar_wait(&ctl.piece_full[me][i & 1], i >> 1 & 1, &dummy);
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+      if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
     }
-    if (lane == 0) bulk_wait_all();
-    if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
-   } else {
-    const int me = warp - kLinFirst, quarter = warp & 3, from = (me >> 2) * C::kSpan;
-    float* factors = reinterpret_cast<float*>(smem + C::kColumns) + me * 2 * C::kSpan;
-    constexpr int kMine = C::kSpan / 32, kPerTile = C::kSpan / 64;
-    const int r = lane >> 2, c = 2 * (lane & 3);                   // rows r, r + 8, r + 16, r + 24, of every eight columns two from c on
-    // dy of 16 bits comes by TMA, 32 rows x 64 columns into one of two pieces, where dz takes its place and leaves by TMA as well; half a piece
-    // ahead.  In the layout of tensor memory's 16 x 256 bits a lane's elements are those of 8 x 8 matrices.  Other dy is read from memory, fp32
-    // 32 columns ahead.
-    const bool by_copy = OTHER != S3R_F32 && p.other_copied;
-    Raw<1> scales[kMine], biases[kMine];
-    uint32_t o[OTHER == S3R_F32 ? 32 : 16];
-    auto fetch = [&](int tile, Tile at) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int col = at.n * TN + from + i * 32 + lane;
-        const bool in = tile < tiles && col < p.N;
-        if (DZ == 2) load_raw<1>(scales[i], p.scale, p.scale_type, col, in);
-        load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
-      }
-    };
-    auto ahead = [&](int tile, Tile at, int g) {
-      if (OTHER != S3R_F32 || tile >= tiles) return;
-      const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
-      load_square<OTHER>(o, p.other, row + r, p.M, p.N, at.n * TN + from + g * 32 + c, min(p.N, at.n * TN + min(from + C::kSpan, TN)), p.other_vectors);
-    };
-    auto soon = [&](int tile, Tile at) {                           // its rows, a lane each, into L2
-      const int64_t row = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32 + lane;
-      const int col = at.n * TN + from, n = min(p.N, at.n * TN + min(from + C::kSpan, TN)) - col;
-      if (tile >= tiles || row >= p.M) return;
-      const char* first_byte = static_cast<const char*>(p.other) + (row * p.N + col) * type_bytes(OTHER);
-#pragma unroll
-      for (int i = 0; i < C::kSpan * type_bytes(OTHER) / 128; ++i)
-        if (i * (128 / type_bytes(OTHER)) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(first_byte + 128 * i));
-    };
-    auto piece_at = [&](uint32_t q) { return smem + C::kOut + (me * 2 + (q & 1)) * kLinPiece; };
-    // piece h of a tile, number q of this warp's: asked for; pieces without columns are left out everywhere
-    auto has = [&](Tile at, int h) { return from + h * 64 < TN && at.n * TN + from + h * 64 < p.N; };
-    auto ask = [&](Tile at, int h, uint32_t q) {
-      if (lane == 0) {
-        mbar_expect_tx(&ctl.piece_full[me][q & 1], kLinPiece);
-        tma_load_2d<1>(smem_u32(piece_at(q)), &md, smem_u32(&ctl.piece_full[me][q & 1]), at.n * TN + from + h * 64, (at.m * CTAS + rank) * 128 + quarter * 32);
-      }
-    };
-    Tile at = begin, after = begin, asked = begin;                 // asked, asked_tile, asked_piece: the next piece to ask for
-    int asked_tile = first, asked_piece = 0;
-    uint32_t asks = 0, q = 0;
-    auto ask_next = [&] {
-      while (asked_tile < tiles) {
-        const bool there = has(asked, asked_piece);
-        if (there) ask(asked, asked_piece, asks++);
-        if (++asked_piece == kPerTile) {
-          asked_piece = 0;
-          asked_tile += stride;
-          advance(asked);
-        }
-        if (there) return;
-      }
-    };
-    fetch(first, at);
-    soon(first, at);
-    if (by_copy) {
-      ask_next();
-      ask_next();
-    }
-    ahead(first, at, 0);
-    int done = 0;
-    bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += stride, at = after, ++done) {
-      const int buf = done & 1;
-      const int64_t m0 = (static_cast<int64_t>(at.m) * CTAS + rank) * 128 + quarter * 32;
-      const int n0 = at.n * TN;
-      const int width = min(min(from + C::kSpan, TN), p.N - n0);   // columns from .. width
-      __syncwarp();                                                // the last tile's factors are read
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        float f[1];
-        if (DZ == 2) {
-          unpack<1>(f, scales[i], p.scale_type);
-          factors[i * 32 + lane] = f[0];
-        }
-        unpack<1>(f, biases[i], p.bias_type);
-        factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
-      }
-      __syncwarp();
-      advance(after);
-      fetch(tile + stride, after);
-      soon(tile + stride, after);
-      ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;
-      uint32_t v[32];
-      if (from < TN) tmem_ld_32x32(sums, v);
-      const bool whole = m0 + 32 <= p.M;
-#pragma unroll
-      for (int g = 0; g < kMine; ++g) {
-        const bool some = from + g * 32 < width;
-        char* piece = piece_at(q);
-        // matrices (i, j): rows 8 i .. of columns 8 j ..; lane l gives the address of row l % 8 of matrix l / 8
-        auto matrix_row = [&](int j) { return smem_u32(piece + swz128(lane, (g & 1) * 4 + j)); };
-        tmem_ld_wait_for(v);
-        if (OTHER != S3R_F32 && some) {
-          if (by_copy) {
-            if (!(g & 1)) ok = mbar_wait_warp(&ctl.piece_full[me][q & 1], q >> 1 & 1, abort_flag);
-            if (!ok) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ldsm_x4(o[j], o[4 + j], o[8 + j], o[12 + j], matrix_row(j));
-          } else {
-            load_square<OTHER>(o, p.other, m0 + r, p.M, p.N, n0 + from + g * 32 + c, n0 + width, p.other_vectors);
-          }
-        }
-        float2 y[16], db[4], ds[4];
-        const float *s = factors + g * 32, *b = s + C::kSpan;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = *reinterpret_cast<const float2*>(s + 8 * j + c), add = *reinterpret_cast<const float2*>(b + 8 * j + c);
-          ds[j] = both(0.f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = (i >> 1) * 16 + j * 4 + (i & 1) * 2;
-            float2 slope;
-            const float2 u = activate<ACT, true>(fadd2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), add), slope);
-            const float2 dy = other_pair<OTHER>(o, (i * 4 + j) * 2);
-            y[i * 4 + j] = fmul2(DZ == 2 ? fmul2(dy, f) : dy, slope);
-            if (DZ == 2) ds[j] = ffma2(dy, whole || m0 + r + 8 * i < p.M ? u : both(0.f), ds[j]);
-          }
-        }
-        if (!whole) {                                              // a row that is not there has dy = 0, but may have any z
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (m0 + r + 8 * (k >> 2) >= p.M) y[k] = both(0.f);
-        }
-        if (g + 1 < kMine) {
-          if (from < TN) tmem_ld_32x32(sums + g * 32 + 32, v);
-          ahead(tile, at, g + 1);
-        } else {                                                   // this warp's sums are in registers
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_first_cta<CTAS>(&ctl.acc_empty[buf]);
-          ahead(tile + stride, after, 0);
-        }
-        const int col = from + g * 32 + (lane & 24) + 2 * (lane & 3) + (lane >> 2 & 1);
-        const int64_t to = (m0 >> 5) * p.N + n0 + col;
-        const bool there = m0 < p.M && col < width;
-        if (p.bias_sums) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) db[j] = fadd2(fadd2(y[j], y[4 + j]), fadd2(y[8 + j], y[12 + j]));
-          const float sum = column_sum(db, lane);
-          if (there) p.bias_sums[to] = sum;
-        }
-        if (DZ == 2 && p.scale_sums) {
-          const float sum = column_sum(ds, lane);
-          if (there) p.scale_sums[to] = sum;
-        }
-        if (!some) continue;
-        if (p.out) {
-          if (!(g & 1) && !by_copy) {
-            if (lane == 0) bulk_wait_read_but_one();               // the store before the last has left this piece
-            __syncwarp();
-          }
-          uint32_t x[16];
-          pack_pairs<false>(x, y, p.out_type);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) stsm_x4(matrix_row(j), x[j], x[4 + j], x[8 + j], x[12 + j]);
-        }
-        const bool last = (g & 1) || from + g * 32 + 32 >= width;
-        if (by_copy && (!(g & 1)) && q > 0) {                      // the piece before has left its place: the one behind this one comes there
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-          ask_next();
-        }
-        if (!last) continue;
-        if (p.out) {
-          const int c0 = from + (g & ~1) * 32;
-          if (p.copy_out) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (m0 < p.M) tma_store_2d(&mo, smem_u32(piece), n0 + c0, static_cast<int>(m0));
-              bulk_commit();
-            }
-          } else {
-            __syncwarp();
-            store_lines<S3R_BF16>(static_cast<char*>(p.out) + (m0 * p.out_pitch + n0 + c0) * 2, p.out_pitch * 2, piece, min(64, width - c0),
-                                  static_cast<int>(min(static_cast<int64_t>(32), p.M - m0)), lane);
-          }
-        }
-        ++q;
-      }
-    }
-    if (!ok) {                                                     // copies in flight land before the CTA's memory is given away
-      volatile uint32_t dummy;
-      for (uint32_t i = asks > 2 ? asks - 2 : 0; i < asks; ++i) {
-        dummy = 0;
-        mbar_wait(&ctl.piece_full[me][i & 1], i >> 1 & 1, &dummy);
-      }
-    }
-    if (lane == 0) bulk_wait_all();
-    if (!ok && lane == 0) atomicOr(p.status, kStatusWaitTimeout);
-   }
   }
   tc_fence_before();
   __syncthreads();
@@ -757,7 +815,7 @@ inline int64_t part_rows(int64_t rows, int ctas) { return (rows + 128 * ctas - 1
 
 template <int TN, int CTAS, int ACT, int OTHER, bool WIDE, int DZ>
 static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bool bf16, LinParams p, cudaStream_t st) {
-  using C = LinCfg<TN, CTAS, DZ ? 2 : 1>;
+  using C = LinCfg<TN, CTAS, DZ || OTHER != kNoOther ? 2 : 1>;
   CUtensorMap ma, mb, mo, md;
   const int64_t rows = ACT == kPartial ? p.rows : p.M;
   if (const int rc = operand_map(&ma, a, rows, k, 128, bf16)) return rc;
@@ -772,12 +830,13 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
     const CUtensorMapDataType type = WIDE ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.out_type == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (const int rc = make_tensor_map(&mo, p.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
   }
-  p.other_copied = DZ && OTHER != S3R_F32 && (reinterpret_cast<uintptr_t>(p.other) & 15) == 0 && p.N % 8 == 0 && (p.copy_out || !p.out);
+  constexpr bool kCopied = DZ ? OTHER != S3R_F32 : OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
+  p.other_copied = kCopied && (reinterpret_cast<uintptr_t>(p.other) & 15) == 0 && p.N * kSize % 16 == 0 && (p.copy_out || !p.out);
   if (p.other_copied) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(p.N) * 2};
-    const uint32_t box[2] = {64, 32};
-    if (const int rc = make_tensor_map(&md, p.other, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                                       OTHER == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16)) return rc;
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(p.N) * kSize};
+    const uint32_t box[2] = {128 / kSize, 32};
+    const CUtensorMapDataType type = OTHER == S3R_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : OTHER == S3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (const int rc = make_tensor_map(&md, p.other, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
   }
   p.idesc = umma_idesc_half(128 * CTAS, TN, bf16, a.turned, b.turned);
   p.a_turned = a.turned;
@@ -817,10 +876,10 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
 // rows of a).  Parts - each a tile of its own, whose sums are joined by a second kernel - pay where there are few tiles and many steps:
 // 64 x 1024 x 4096 in eight parts {PARTS_64}, in one 20; the weight gradient 1024 x 1024 of 12 288 tokens {PARTS_DW}.
 struct LinPlan {
-  int width, ctas, parts;
+  int width, ctas, parts, step;
 };
 inline LinPlan linear_plan(int64_t M, int64_t N, int64_t K, bool parts) {
-  const LinPlan tiles[] = {{256, 2, 1}, {128, 2, 1}, {128, 1, 1}, {64, 1, 1}};
+  const LinPlan tiles[] = {{256, 2, 1, 640}, {128, 2, 1, 460}, {128, 1, 1, 500}, {64, 1, 1, 440}};
   const int64_t steps = (K + kLinStep - 1) / kLinStep;
   LinPlan best = {};
   int64_t least = INT64_MAX;
@@ -829,9 +888,9 @@ inline LinPlan linear_plan(int64_t M, int64_t N, int64_t K, bool parts) {
       if ((t.ctas == 2 && M <= 128) || (n > 1 && (!parts || steps < 4 * n))) continue;
       const int64_t part = (steps + n - 1) / n, used = (steps + part - 1) / part;      // parts that have steps
       const int64_t all = (M + 128 * t.ctas - 1) / (128 * t.ctas) * ((N + t.width - 1) / t.width) * used, at_once = sm_count() / t.ctas;
-      // cycles: of a step, of a tile's start and end; of the second kernel and its traffic
-      const int64_t cost = (all + at_once - 1) / at_once * (part * (t.width + (t.ctas == 2 ? 64 : 96)) * 8 / 5 + 1500) + (n > 1 ? 6000 + used * M * N / 275 : 0);
-      if (cost < least) least = cost, best = {t.width, t.ctas, static_cast<int>(used)};
+      // cycles: of a step (a full GPU, L2 behind it), of a tile's start and end; of the second kernel and its traffic
+      const int64_t cost = (all + at_once - 1) / at_once * (part * t.step + 1500) + (n > 1 ? 6000 + used * M * N / 275 : 0);
+      if (cost < least) least = cost, best = {t.width, t.ctas, static_cast<int>(used), t.step};
     }
   return best;
 }

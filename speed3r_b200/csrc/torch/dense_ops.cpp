@@ -6,8 +6,10 @@ namespace {
 // ------------------------------------------------------------------------------------------------
 // residual + act(x W^T + bias) * scale
 // ------------------------------------------------------------------------------------------------
-// [rows, K] of 16-bit elements whose base and rows begin at multiples of 16 bytes
+// The tensor itself where its rows of K 16-bit elements lie one behind the other at multiples of 16 bytes (a view takes a microsecond), else [rows, K]
+// whose base and rows begin at such
 Tensor half_rows(const Tensor& t, int64_t rows, int64_t K) {
+  if (K % 8 == 0 && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
   Tensor r = t.reshape({rows, K});
   const bool fits = (K == 1 || r.stride(1) == 1) && (rows <= 1 || (r.stride(0) >= K && r.stride(0) % 8 == 0)) &&
                     reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
@@ -19,7 +21,7 @@ Tensor half_rows(const Tensor& t, int64_t rows, int64_t K) {
                      static_cast<int>(2 * K), stream()), "s3r_pad_rows");
   return whole.narrow(1, 0, K);
 }
-int64_t pitch_of(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : (rows.size(1) + 7) / 8 * 8; }
+int64_t pitch_of(const Tensor& t, int64_t K) { return t.dim() == 2 && t.size(0) > 1 ? t.stride(0) : (K + 7) / 8 * 8; }
 
 struct LinearSizes {
   int64_t M, N, K;
@@ -48,9 +50,9 @@ s3r_linear linear_args(const Tensor& x, const Tensor& weight, const Tensor& bias
   a.K = static_cast<int>(n.K);
   a.type = type_of(x, "x");
   a.x = x.data_ptr();
-  a.x_pitch = pitch_of(x);
+  a.x_pitch = pitch_of(x, n.K);
   a.weight = weight.data_ptr();
-  a.w_pitch = pitch_of(weight);
+  a.w_pitch = pitch_of(weight, n.K);
   if (bias.defined()) a.bias = bias.data_ptr(), a.bias_type = type_of(bias, "bias");
   if (scale.defined()) a.scale = scale.data_ptr(), a.scale_type = type_of(scale, "scale");
   a.act = static_cast<int>(act);
@@ -128,7 +130,7 @@ std::vector<Tensor> run_linear_bwd(const Tensor& x, const Tensor& weight, const 
   check(s3r_linear_bwd(&f, &g, stream()), "s3r_linear_bwd");
   auto product = [&](bool turned, const Tensor& other, Tensor& out, int64_t rows, int64_t sum) {
     const Tensor parts = workspace(x, rows, n.K, sum);
-    check(s3r_product(dz.data_ptr(), pitch, turned, other.data_ptr(), pitch_of(other), 1, f.type, out.data_ptr(), rows, static_cast<int>(n.K), sum, pointer(parts),
+    check(s3r_product(dz.data_ptr(), pitch, turned, other.data_ptr(), pitch_of(other, n.K), 1, f.type, out.data_ptr(), rows, static_cast<int>(n.K), sum, pointer(parts),
                       parts.defined() ? parts.numel() : 0, stream()), "s3r_product");
   };
   if (dx.defined()) product(false, w, dx, n.M, n.N);
@@ -183,7 +185,9 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     const Tensor a = n.M ? half_rows(x, n.M, n.K) : x, w = n.M ? half_rows(weight, n.N, n.K) : weight;
     ctx->save_for_backward({a, w, value(bias), value(scale)});
     ctx->saved_data["shape"] = x.sizes().vec();
-    Tensor out = linear_fwd(a, w, bias, scale, residual.has_value() && n.M ? optional<Tensor>(as_result(*residual, x, n)) : residual, act, static_cast<at::ScalarType>(out_type));
+    const bool rows = a.sizes() != x.sizes();
+    Tensor out = linear_fwd(a, w, bias, scale, rows && residual.has_value() ? optional<Tensor>(as_result(*residual, x, n)) : residual, act, static_cast<at::ScalarType>(out_type));
+    if (!rows) return out;
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = n.N;
     return in_shape(out, shape);
@@ -427,12 +431,13 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, const option
     TORCH_CHECK(pos->scalar_type() == at::kLong || pos->scalar_type() == at::kInt, "qkv_norm_rope: pos must be int64 or int32, got ", pos->scalar_type());
     TORCH_CHECK((pos->dim() == 3 || pos->dim() == 2) && pos->size(pos->dim() - 2) == qkv.size(1) && (pos->dim() == 2 || pos->size(0) == 1 || pos->size(0) == qkv.size(0)),
                 "qkv_norm_rope: pos must be [batch or 1, tokens, axes] or [tokens, axes], got ", pos->sizes(), " for ", qkv.sizes());
-    Tensor p = pos->to(at::kLong);
+    // calls that would change nothing are left out: each takes up to a microsecond
+    Tensor p = pos->scalar_type() == at::kLong ? *pos : pos->to(at::kLong);
     if (p.size(-1) > 1 && p.stride(-1) != 1) p = p.contiguous();
-    in.pos = p.expand({qkv.size(0), qkv.size(1), p.size(-1)});
-    const at::ScalarType type = cos->scalar_type() == sin->scalar_type() ? cos->scalar_type() : at::kFloat;
+    in.pos = p.dim() == 3 && p.size(0) == qkv.size(0) ? p : p.expand({qkv.size(0), qkv.size(1), p.size(-1)});
+    const bool mixed = cos->scalar_type() != sin->scalar_type();
     for (optional<Tensor>* t : {&in.cos, &in.sin}) {
-      **t = (*t)->to(type);
+      if (mixed) **t = (*t)->to(at::kFloat);
       if ((*t)->dim() == 2 && (*t)->size(1) > 1 && (*t)->stride(1) != 1) **t = (*t)->contiguous();
     }
   }

@@ -9,8 +9,8 @@ namespace s3r {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has two output channels,
-// a lane 16 bytes of each at a time and four of those in flight; the tokens lie in shared memory.  One token x 4096 x 1024, weights not in L2:
-// {FEW}; with four channels and one ahead 8.0.
+// a lane 16 bytes of each at a time and four of those in flight; the tokens lie in shared memory.  One token x 4096 x 1024, weights in HBM: 7 us, of
+// which 1.3 are the weights' bytes, and the rest the start of the kernel and one trip to memory.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kLinFew = 8, kLinFewBytes = 48 * 1024, kLinFewChannels = 2, kLinFewWarps = 8, kLinFewAhead = 4;
 
@@ -121,7 +121,8 @@ static int run_linear_few(const LinFewParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the sums of a contraction's parts, in their order, and what follows them: a thread has four columns of a row
+// the sums of a contraction's parts, in their order, and what follows them: a thread has four columns of a row, and all parts' loads in flight.
+// Bound: the latency of those loads, from L2, where the parts have just been written (64 x 1024 in sixteen parts: 4 MB).
 // ---------------------------------------------------------------------------------------------------------------------
 struct JoinParams {
   const float* sums;                    // [parts][part_rows][pitch]
@@ -219,8 +220,8 @@ static int run_parts(const LinPlan& t, const LinOperand& a, const LinOperand& b,
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dz = dy * scale where no z is needed, with its sums over rows.  Bound: HBM.  A CTA has 64 rows and 256 columns, a thread eight columns of
-// every eighth row.
+// dz = dy * scale where no z is needed, with its sums over rows.  Bound: HBM, dy read and dz written once.  A CTA has 64 rows and 256 columns, a
+// thread eight columns of every eighth row.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kDzRows = 64, kDzColumns = 256;
 

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <climits>
+#include <cmath>
 
 #include "pairs.cuh"
 
@@ -50,9 +51,9 @@ __device__ __forceinline__ float2 activate(float2 z, float2& slope) {
     const float2 p = fast_rcp2(fadd2(exp2_2(arg), both(1.f)));
     const float2 u = fmul2(z, p);
     if (SLOPE) {
-      // the argument's own slope: 1, or 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2)
-      const float2 inner = ACT == S3R_ACT_SILU ? both(1.f) : ffma2(q, both(0.214064488f), both(1.59576912f));
-      slope = ffma2(fmul2(u, inner), fadd2(both(1.f), make_float2(-p.x, -p.y)), p);
+      // p + u (1 - p) times the argument's own slope: 1, or 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2), last, for it may be huge where 1 - p is 0
+      const float2 rest = fadd2(both(1.f), make_float2(-p.x, -p.y));
+      slope = ACT == S3R_ACT_SILU ? ffma2(u, rest, p) : ffma2(fmul2(u, rest), ffma2(q, both(0.214064488f), both(1.59576912f)), p);
     }
     return u;
   }
@@ -86,6 +87,14 @@ int linear_partial(const LinOperand& a, const LinOperand& b, int64_t k, bool bf1
 // and half of the columns each.
 // Either operand lies with the contraction contiguous ([rows][k]: x, W of the forward, dz of dx) or turned ([k][rows]: W of dx, dz and x of dW);
 // a turned one comes in boxes of 64 rows x 64 steps and is read through the other form of the matrix descriptor.
+//
+// Bound: the tensor cores, and at full size the power they take.  64 512 x 4096 x 1024 in bf16: the products alone 322 us (1680 TFLOP/s), with GELU
+// 360 to 400 by the clock that power leaves.  What the epilogue takes must stay below the products' time: alone (K = 64) it is 109 us for a sum that
+// is only rounded, 185 with SiLU, 231 with GELU, 376 with an fp32 residual, 380 for dz with GELU's slope and a sum over rows, of which the memory
+// traffic is 80, 80, 80, 320 and 161 (dz: dy read, dz written).  dz is the one that issues most: 41 % of all cycles, the tensor cores busy in 65 %
+// (forward with GELU 83 %).
+// Tried, and slower: sixteen summing warps, which spill (166 -> 237, dz 375 -> 494); two pieces of output per warp where nothing is read beside the
+// sums (166 -> 172); two sets of dz's sums in registers (373 -> 395).
 // ---------------------------------------------------------------------------------------------------------------------
 // Warps 0 and 1 feed, the last eight take the sums.  Two in between do nothing: without them every kind of epilogue took 4 to 10 % longer.
 constexpr int kLinFirst = 4, kLinWarps = 8, kLinThreads = 32 * (kLinFirst + kLinWarps);
@@ -395,7 +404,8 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
       constexpr int kMine = C::kSpan / 32, kPieces = OTHER == kNoOther ? 1 : 2;
       // A residual of the result's size comes by TMA into the piece that the sum leaves from, a piece ahead; rows that a lane reads from memory itself,
-      // 16 bytes of 32 lines at a time, took 1092 us for 64 512 x 4096 in fp32 where this way takes {RES}.  Other residuals are read 32 columns ahead.
+      // 16 bytes of 32 lines at a time, took 1092 us for 64 512 x 4096 x 1024 in fp32 where this way takes 566.  Other residuals are
+      // read 32 columns ahead.
       constexpr bool kInPlace = OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
       const bool by_copy = kInPlace && p.other_copied;
       // What the next tile needs is asked for a tile ahead.
@@ -831,7 +841,7 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
     if (const int rc = make_tensor_map(&mo, p.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, type)) return rc;
   }
   constexpr bool kCopied = DZ ? OTHER != S3R_F32 : OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
-  p.other_copied = kCopied && (reinterpret_cast<uintptr_t>(p.other) & 15) == 0 && p.N * kSize % 16 == 0 && (p.copy_out || !p.out);
+  p.other_copied = kCopied && (reinterpret_cast<uintptr_t>(p.other) & 15) == 0 && static_cast<int64_t>(p.N) * kSize % 16 == 0 && (p.copy_out || !p.out);
   if (p.other_copied) {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)}, strides[1] = {static_cast<uint64_t>(p.N) * kSize};
     const uint32_t box[2] = {128 / kSize, 32};
@@ -873,8 +883,8 @@ static int launch_linear(const LinOperand& a, const LinOperand& b, int64_t k, bo
 }
 
 // The tile and the number of parts of the contraction whose waves cost least.  A wave of narrower tiles takes less, but not in proportion (the same
-// rows of a).  Parts - each a tile of its own, whose sums are joined by a second kernel - pay where there are few tiles and many steps:
-// 64 x 1024 x 4096 in eight parts {PARTS_64}, in one 20; the weight gradient 1024 x 1024 of 12 288 tokens {PARTS_DW}.
+// rows of a).  Parts - each a tile of its own, whose sums are joined by a second kernel - pay where there are few tiles and many steps (inputs in
+// HBM): 64 x 1024 x 4096 in sixteen parts 13 us, in one 21; the weight gradient 1024 x 1024 of 12 288 tokens in four 36, in one 60.
 struct LinPlan {
   int width, ctas, parts, step;
 };
@@ -882,14 +892,14 @@ inline LinPlan linear_plan(int64_t M, int64_t N, int64_t K, bool parts) {
   const LinPlan tiles[] = {{256, 2, 1, 640}, {128, 2, 1, 460}, {128, 1, 1, 500}, {64, 1, 1, 440}};
   const int64_t steps = (K + kLinStep - 1) / kLinStep;
   LinPlan best = {};
-  int64_t least = INT64_MAX;
+  double least = HUGE_VAL;
   for (const LinPlan& t : tiles)
     for (int n = 1; n <= 16; n *= 2) {
       if ((t.ctas == 2 && M <= 128) || (n > 1 && (!parts || steps < 4 * n))) continue;
       const int64_t part = (steps + n - 1) / n, used = (steps + part - 1) / part;      // parts that have steps
       const int64_t all = (M + 128 * t.ctas - 1) / (128 * t.ctas) * ((N + t.width - 1) / t.width) * used, at_once = sm_count() / t.ctas;
       // cycles: of a step (a full GPU, L2 behind it), of a tile's start and end; of the second kernel and its traffic
-      const int64_t cost = (all + at_once - 1) / at_once * (part * t.step + 1500) + (n > 1 ? 6000 + used * M * N / 275 : 0);
+      const double cost = static_cast<double>((all + at_once - 1) / at_once) * (part * t.step + 1500) + (n > 1 ? 6000 + static_cast<double>(used * M) * N / 275 : 0);
       if (cost < least) least = cost, best = {t.width, t.ctas, static_cast<int>(used), t.step};
     }
   return best;

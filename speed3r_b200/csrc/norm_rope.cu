@@ -7,9 +7,15 @@
 // Columns that are not turned are taken as two neighbouring vectors.  A group of G threads stays with one token and walks over heads, so that the
 // token's sines and cosines, the parameters and the sums over rows stay in registers; the groups of a warp have neighbouring tokens, whose
 // results lie one behind the other.
-// Memory is read and written by whole rows: the heads of a warp's tokens come by cp.async, neighbouring lanes neighbouring chunks, several heads
-// ahead, and results leave the same way through shared memory.  A thread's own vectors copied by itself are pieces of 32 bytes, and took 150 us
-// where rows take less; in registers, four heads ahead, 173 (64 512 tokens of 16 heads of 64 in bf16).
+// Memory is read and written by whole rows: the heads of a warp's tokens come by cp.async, neighbouring lanes neighbouring chunks, four heads
+// ahead, and results leave the same way through shared memory.
+//
+// 64 512 tokens of 16 heads of 64 in bf16, LayerNorm with weight and bias, two axes: forward 139 us (793 MB, 5.7 TB/s; a copy with the same pattern
+// 123.5), 61 % of the issue slots taken; backward 231 us (1.19 GB read and written with the gradients of q, k and v, 5.1 TB/s), 55 % taken at 22 % of
+// the warps: it waits for its own shuffles and loads in turn.
+// Tried there, and slower: a thread's own vectors, pieces of 32 bytes, by cp.async 150 to 156, and in registers four heads ahead 173; vectors of
+// eight elements 153; a CTA that walks over q, k and v 155 to 191; three heads ahead 141, eight 143.  Backward: two heads ahead 271; vectors of
+// eight 235, but the same time as these at 48 x 256 tokens, at 168 registers in every variant.
 #include <type_traits>
 
 #include "rows.cuh"
@@ -676,21 +682,27 @@ static int pick_norm_rope(const NrParams& p, NrShape s, bool backward, unsigned 
   }
 }
 
-// Heads are split over CTAs until there are some for every SM; no further than that, a token's angles are found once per CTA.
-static void norm_rope_chunks(int64_t token_ctas, int heads, int kv_heads, int* per_chunk, int* q_chunks, int* kv_chunks) {
+// Heads are split over CTAs until there are `per_sm` for every SM; no further than that, a token's angles are found once per CTA, and the backward has
+// a row of sums for each.  Forward / backward: 3 x 1041 tokens of 12 + 4 heads of 80, four per SM 13.8 / 19, eight 10.2 / 22.5, twelve 14 / 26; 1041 of
+// 16 heads of 64, four 8.2 / 11.3, eight 7.2 / 15; 300 of them backward, two or three 7.9, four 11.1; 2 x 1041 backward, two 15.5, three 14.4, six 18.1.
+constexpr int kNrForwardSplit = 8, kNrBackwardSplit = 3;
+static void norm_rope_chunks(int64_t token_ctas, int heads, int kv_heads, int per_sm, int* per_chunk, int* q_chunks, int* kv_chunks) {
   int per = heads;
   while (per > 1) {
     const int64_t chunks = (heads + per - 1) / per + 2 * ((kv_heads + per - 1) / per);
-    if (chunks * token_ctas >= 4 * sm_count()) break;
+    if (chunks * token_ctas >= static_cast<int64_t>(per_sm) * sm_count()) break;
     per = (per + 1) / 2;
   }
   *per_chunk = per;
   *q_chunks = (heads + per - 1) / per;
   *kv_chunks = (kv_heads + per - 1) / per;
 }
-// CTAs of the backward along the tokens: those that are resident together, so that each leaves one row of sums.
+// CTAs of the backward along the tokens: each walks over its share of them and leaves one row of sums.  Three times what is resident, so that v's,
+// which do least and come last, fill the gaps of the others: 64 x 1008 tokens 231 us, all resident 270, twice 250, four times 231 to 238; 48 x 256
+// 53.7, 59.4, 56.9, 55.3.
+constexpr int kNrBackwardCtas = 12;      // per SM
 static unsigned norm_rope_bwd_ctas(int64_t token_ctas, int chunks) {
-  const int64_t most = (8 * static_cast<int64_t>(sm_count()) + chunks - 1) / chunks;
+  const int64_t most = kNrBackwardCtas * static_cast<int64_t>(sm_count()) / chunks;
   return static_cast<unsigned>(token_ctas < most ? token_ctas : most < 1 ? 1 : most);
 }
 
@@ -785,7 +797,7 @@ extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
   const int64_t strides[] = {f->batch > 1 ? f->stride_b : 0, f->tokens > 1 ? f->stride_t : 0};
   const NrShape s = norm_rope_shape(f, pointers, 4, strides, 2);
   const int64_t per = kNrThreads / s.group, ctas = (p.rows_of_tokens + per - 1) / per;
-  norm_rope_chunks(ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
+  norm_rope_chunks(ctas, f->heads, f->kv_heads, kNrForwardSplit, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return f->type == S3R_F32 ? pick_norm_rope<4>(p, s, false, static_cast<unsigned>(ctas), st) : pick_norm_rope<2>(p, s, false, static_cast<unsigned>(ctas), st);
 }
@@ -793,8 +805,8 @@ extern "C" int s3r_qkv_norm_rope_fwd(const s3r_qkv_norm_rope* f, void* stream) {
 // Room for either shape of the grid: the chunks of heads depend on the vectors that addresses allow.
 extern "C" size_t s3r_qkv_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim) {
   if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  // chunks of q and k times CTAs along the tokens: at most one more CTA per chunk than 8 per SM in all, and no chunk without a head
-  return static_cast<size_t>(8 * sm_count() + heads + 2 * kv_heads) * 2 * head_dim * sizeof(float);
+  // chunks of q and k times CTAs along the tokens: all of them together as many as there are, or one for each chunk of a head at least
+  return static_cast<size_t>(kNrBackwardCtas * sm_count() + heads + 2 * kv_heads) * 2 * head_dim * sizeof(float);
 }
 
 extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_norm_rope_grad* g, void* stream) {
@@ -827,7 +839,7 @@ extern "C" int s3r_qkv_norm_rope_bwd(const s3r_qkv_norm_rope* f, const s3r_qkv_n
   p.sums = sums ? static_cast<float*>(g->workspace) : nullptr;
   const NrShape s = norm_rope_shape(f, pointers, np, strides, ns);
   const int64_t per = kNrThreads / s.group, token_ctas = (p.rows_of_tokens + per - 1) / per;
-  norm_rope_chunks(token_ctas, f->heads, f->kv_heads, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
+  norm_rope_chunks(token_ctas, f->heads, f->kv_heads, kNrBackwardSplit, &p.per_chunk, &p.q_chunks, &p.kv_chunks);
   const int chunks = p.q_chunks + 2 * p.kv_chunks;
   const unsigned ctas = norm_rope_bwd_ctas(token_ctas, chunks);
   S3R_REQUIRE(!sums || static_cast<size_t>(p.q_chunks + p.kv_chunks) * ctas * 2 * f->head_dim * sizeof(float) <= need, S3R_ERR_TOO_LARGE,

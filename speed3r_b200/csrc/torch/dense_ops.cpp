@@ -179,11 +179,11 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       ctx->save_for_backward({x, weight, value(bias), value(scale)});
       return call_linear_fwd(x, weight, bias, scale, residual, act, static_cast<at::ScalarType>(out_type));
     }
-    // what is laid out anew is kept that way
+    // what is laid out anew is kept that way; a view made here does not count its owner's changes, so the owner is kept in its place
     const LinearSizes n = linear_sizes(x, weight, bias, scale);
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor a = n.M ? half_rows(x, n.M, n.K) : x, w = n.M ? half_rows(weight, n.N, n.K) : weight;
-    ctx->save_for_backward({a, w, value(bias), value(scale)});
+    ctx->save_for_backward({a.is_alias_of(x) ? x : a, w.is_alias_of(weight) ? weight : w, value(bias), value(scale)});
     ctx->saved_data["shape"] = x.sizes().vec();
     const bool rows = a.sizes() != x.sizes();
     Tensor out = linear_fwd(a, w, bias, scale, rows && residual.has_value() ? optional<Tensor>(as_result(*residual, x, n)) : residual, act, static_cast<at::ScalarType>(out_type));

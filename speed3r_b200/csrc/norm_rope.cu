@@ -10,12 +10,10 @@
 // Memory is read and written by whole rows: the heads of a warp's tokens come by cp.async, neighbouring lanes neighbouring chunks, four heads
 // ahead, and results leave the same way through shared memory.
 //
-// 64 512 tokens of 16 heads of 64 in bf16, LayerNorm with weight and bias, two axes: forward 139 us (793 MB, 5.7 TB/s; a copy with the same pattern
-// 123.5), 61 % of the issue slots taken; backward 231 us (1.19 GB read and written with the gradients of q, k and v, 5.1 TB/s), 55 % taken at 22 % of
-// the warps: it waits for its own shuffles and loads in turn.
-// Tried there, and slower: a thread's own vectors, pieces of 32 bytes, by cp.async 150 to 156, and in registers four heads ahead 173; vectors of
-// eight elements 153; a CTA that walks over q, k and v 155 to 191; three heads ahead 141, eight 143.  Backward: two heads ahead 271; vectors of
-// eight 235, but the same time as these at 48 x 256 tokens, at 168 registers in every variant.
+// 64 512 tokens of 16 heads of 64 in bf16, LayerNorm with weight and bias, two axes: forward 132 us (793 MB, 6.0 TB/s; a copy by the same route 123);
+// backward 215 us (1.19 GB read and written with the gradients of q, k and v, 5.5 TB/s; the rest is latency, at 16 warps per SM).
+// Tried there, and slower: a thread's own vectors, pieces of 32 bytes, by cp.async 150 to 156 (where these took 139), and in registers four heads ahead
+// 173; vectors of eight elements 153; a CTA that walks over q, k and v 155 to 191; three heads ahead 141, eight 143; backward two heads ahead 271 for 252.
 #include <type_traits>
 
 #include "rows.cuh"
@@ -137,35 +135,62 @@ __device__ __forceinline__ void group_sum(float (&s)[N]) {
     for (int k = 0; k < N; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
 }
 
-// Values of a slot in packed pairs: H of the first member, H of the second (V = 1: one value each, beside a zero).
+// Values of a slot in packed pairs: H of the first member, H of the second; V = 1: the two members are the one pair.
 template <int V>
 constexpr int kHalf = V == 1 ? 1 : V / 2;
+template <int V>
+constexpr int kSides = V == 1 ? 1 : 2;
+template <int BYTES>
+__device__ __forceinline__ float one_value(uint32_t w, int type) {
+  return BYTES == 4 ? __uint_as_float(w) : type == S3R_BF16 ? bf16_lo(w) : half_lo(w);
+}
 template <int V, int BYTES>
-__device__ __forceinline__ void values(float2* f, const Vec<V, BYTES>& v, int type) {
+__device__ __forceinline__ void take_slot(float2 (&x)[kSides<V>][kHalf<V>], uint32_t at0, uint32_t at1, int type) {
+  Vec<V, BYTES> v[2];
+  take_vec<V, BYTES>(v[0], at0);
+  take_vec<V, BYTES>(v[1], at1);
   if constexpr (V == 1) {
-    f[0] = make_float2(BYTES == 4 ? __uint_as_float(v.w[0]) : type == S3R_BF16 ? bf16_lo(v.w[0]) : half_lo(v.w[0]), 0.f);
+    x[0][0] = make_float2(one_value<BYTES>(v[0].w[0], type), one_value<BYTES>(v[1].w[0], type));
   } else {
 #pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      if constexpr (BYTES == 4) f[k] = make_float2(__uint_as_float(v.w[2 * k]), __uint_as_float(v.w[2 * k + 1]));
-      else f[k] = type == S3R_BF16 ? make_float2(bf16_lo(v.w[k]), bf16_hi(v.w[k])) : make_float2(half_lo(v.w[k]), half_hi(v.w[k]));
-    }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        if constexpr (BYTES == 4) x[m][k] = make_float2(__uint_as_float(v[m].w[2 * k]), __uint_as_float(v[m].w[2 * k + 1]));
+        else x[m][k] = type == S3R_BF16 ? make_float2(bf16_lo(v[m].w[k]), bf16_hi(v[m].w[k])) : make_float2(half_lo(v[m].w[k]), half_hi(v[m].w[k]));
+      }
   }
 }
 template <int V, int BYTES>
-__device__ __forceinline__ void rounded(Vec<V, BYTES>& v, const float2* f, int type) {
+__device__ __forceinline__ void put_slot(const float2 (&x)[kSides<V>][kHalf<V>], uint32_t at0, uint32_t at1, int type) {
+  Vec<V, BYTES> v[2];
   if constexpr (V == 1) {
-    v.w[0] = BYTES == 4 ? __float_as_uint(f[0].x) : (type == S3R_BF16 ? pack_bf16(f[0].x, 0.f) : pack_half(f[0].x, 0.f)) & 0xffffu;
+    if constexpr (BYTES == 4) {
+      v[0].w[0] = __float_as_uint(x[0][0].x), v[1].w[0] = __float_as_uint(x[0][0].y);
+    } else {
+      const uint32_t w = type == S3R_BF16 ? pack_bf16(x[0][0].x, x[0][0].y) : pack_half(x[0][0].x, x[0][0].y);
+      v[0].w[0] = w & 0xffffu, v[1].w[0] = w >> 16;
+    }
   } else {
 #pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      if constexpr (BYTES == 4) v.w[2 * k] = __float_as_uint(f[k].x), v.w[2 * k + 1] = __float_as_uint(f[k].y);
-      else v.w[k] = type == S3R_BF16 ? pack_bf16(f[k].x, f[k].y) : pack_half(f[k].x, f[k].y);
-    }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        if constexpr (BYTES == 4) v[m].w[2 * k] = __float_as_uint(x[m][k].x), v[m].w[2 * k + 1] = __float_as_uint(x[m][k].y);
+        else v[m].w[k] = type == S3R_BF16 ? pack_bf16(x[m][k].x, x[m][k].y) : pack_half(x[m][k].x, x[m][k].y);
+      }
   }
+  put_vec<V, BYTES>(v[0], at0);
+  put_vec<V, BYTES>(v[1], at1);
 }
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
+// What a quarter turn makes of a slot, (a, b) -> (-b, a), and with `back` of its gradient, (a, b) -> (b, -a)
+template <int V>
+__device__ __forceinline__ float2 quarter(const float2 (&x)[kSides<V>][kHalf<V>], int m, int k, bool back) {
+  if constexpr (V == 1) return back ? make_float2(x[0][0].y, -x[0][0].x) : make_float2(-x[0][0].y, x[0][0].x);
+  else return (m == 0) != back ? minus(x[1 - m][k]) : x[1 - m][k];
+}
 
 // What a thread keeps of its columns, in the order of values(): member m of slot e in [e][m]
 template <int V, int E>
@@ -183,38 +208,78 @@ __device__ __forceinline__ void place(Lane<V, E>& l, const NrParams& p, int t) {
     l.share[e] = l.on[e] ? -p.inverse_dim : 0.f;
   }
 }
+// columns of the two values of pair [m][k] of a slot
+template <int V>
+__device__ __forceinline__ int column_x(const Slot& s, int m, int k) { return (m ? s.c1 : s.c0) + 2 * k; }
+template <int V>
+__device__ __forceinline__ int column_y(const Slot& s, int m, int k) { return V == 1 ? s.c1 : column_x<V>(s, m, k) + 1; }
+// f(an element's width): decided once in front of all loads, which then are on their way together; a load that decides for itself is waited for
+// before the next (forward 139 us where this takes 132, one token of 16 heads 3.8 and 3.0)
+template <typename F>
+__device__ __forceinline__ void with_width(int type, F f) {
+  if (type == S3R_F32) f(uint32_t());
+  else f(uint16_t());
+}
+__device__ __forceinline__ float any_value(uint32_t w, int type) { return type == S3R_F32 ? __uint_as_float(w) : type == S3R_BF16 ? bf16_lo(w) : half_lo(w); }
 template <int V, int E>
-__device__ __forceinline__ void parameter(float2 (&f)[E][2][kHalf<V>], const Lane<V, E>& l, const void* from, int type, float other) {
+__device__ __forceinline__ void parameter(float2 (&f)[E][kSides<V>][kHalf<V>], const Lane<V, E>& l, const void* from, int type, float other) {
+  uint32_t raw[E][kSides<V>][kHalf<V>][2];
+  with_width(type, [&](auto width) {
+    const auto* at = static_cast<const decltype(width)*>(from);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int m = 0; m < kSides<V>; ++m)
+#pragma unroll
+        for (int k = 0; k < kHalf<V>; ++k) {
+          raw[e][m][k][0] = from && l.on[e] ? __ldg(at + column_x<V>(l.slot[e], m, k)) : 0;
+          raw[e][m][k][1] = from && l.on[e] ? __ldg(at + column_y<V>(l.slot[e], m, k)) : 0;
+        }
+  });
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < kSides<V>; ++m)
 #pragma unroll
-      for (int k = 0; k < kHalf<V>; ++k) {
-        const int col = (m ? l.slot[e].c1 : l.slot[e].c0) + 2 * k;
-        f[e][m][k].x = from && l.on[e] ? load_one(from, type, col) : other;
-        f[e][m][k].y = V > 1 && from && l.on[e] ? load_one(from, type, col + 1) : other;
-      }
+      for (int k = 0; k < kHalf<V>; ++k)
+        f[e][m][k] = from && l.on[e] ? make_float2(any_value(raw[e][m][k][0], type), any_value(raw[e][m][k][1], type)) : make_float2(other, other);
 }
 template <int V, int E>
 __device__ __forceinline__ void angles(float2 (&c)[E][kHalf<V>], float2 (&s)[E][kHalf<V>], const Lane<V, E>& l, const NrParams& p, int64_t b, int t, bool in) {
+  constexpr int N = V == 1 ? 1 : 2;                                // values of a pair that differ
+  int64_t row[E];
+  bool turned[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool turned = in && l.on[e] && l.slot[e].axis >= 0;
-    int64_t row = turned ? __ldg(p.pos + b * p.pos_stride_b + t * p.pos_stride_t + l.slot[e].axis) : 0;
-    if (row < 0 || row >= p.rows) {
-      if (turned) atomicOr(p.status, kStatusBadIndex);
-      row = row < 0 ? 0 : p.rows - 1;
+    turned[e] = in && l.on[e] && l.slot[e].axis >= 0;
+    row[e] = turned[e] ? __ldg(p.pos + b * p.pos_stride_b + t * p.pos_stride_t + l.slot[e].axis) : 0;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (row[e] < 0 || row[e] >= p.rows) {
+      if (turned[e]) atomicOr(p.status, kStatusBadIndex);
+      row[e] = row[e] < 0 ? 0 : p.rows - 1;
     }
+  uint32_t cr[E][kHalf<V>][N], sr[E][kHalf<V>][N];
+  with_width(p.table_type, [&](auto width) {
+    const auto *cos = static_cast<const decltype(width)*>(p.cos), *sin = static_cast<const decltype(width)*>(p.sin);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int k = 0; k < kHalf<V>; ++k)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          cr[e][k][n] = turned[e] ? __ldg(cos + row[e] * p.cos_pitch + l.slot[e].column + 2 * k + n) : 0;
+          sr[e][k][n] = turned[e] ? __ldg(sin + row[e] * p.sin_pitch + l.slot[e].column + 2 * k + n) : 0;
+        }
+  });
+#pragma unroll
+  for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int k = 0; k < kHalf<V>; ++k) {
-      const int64_t ci = row * p.cos_pitch + l.slot[e].column + 2 * k, si = row * p.sin_pitch + l.slot[e].column + 2 * k;
-      c[e][k].x = turned ? load_one(p.cos, p.table_type, ci) : 1.f;
-      s[e][k].x = turned ? load_one(p.sin, p.table_type, si) : 0.f;
-      c[e][k].y = V > 1 && turned ? load_one(p.cos, p.table_type, ci + 1) : 1.f;
-      s[e][k].y = V > 1 && turned ? load_one(p.sin, p.table_type, si + 1) : 0.f;
+      c[e][k] = turned[e] ? make_float2(any_value(cr[e][k][0], p.table_type), any_value(cr[e][k][N - 1], p.table_type)) : twice(1.f);
+      s[e][k] = turned[e] ? make_float2(any_value(sr[e][k][0], p.table_type), any_value(sr[e][k][N - 1], p.table_type)) : twice(0.f);
     }
-  }
 }
 
 // Heads of a CTA: part 0 q, 1 k, 2 v; heads first .. first + count of it.
@@ -236,7 +301,7 @@ __device__ __forceinline__ int packed_head(const Heads& h, const NrParams& p) { 
 
 // (x - mean) * inverse in place; returns the inverse.  The variance is that of centred values.
 template <int V, int G, int E>
-__device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const Lane<V, E>& l, const NrParams& p, float eps) {
+__device__ __forceinline__ float normalise(float2 (&x)[E][kSides<V>][kHalf<V>], const Lane<V, E>& l, const NrParams& p, float eps) {
   float s[1];
   float2 t;
   if (p.kind == S3R_NORM_LAYER) {
@@ -244,7 +309,7 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int k = 0; k < kHalf<V>; ++k) t = fadd2(t, fadd2(x[e][0][k], x[e][1][k]));
+      for (int k = 0; k < kHalf<V>; ++k) t = fadd2(t, V == 1 ? x[e][0][k] : fadd2(x[e][0][k], x[e][kSides<V> - 1][k]));
     s[0] = t.x + t.y;
     group_sum<G>(s);
     float minus_mean[E];
@@ -253,17 +318,15 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < kSides<V>; ++m)
 #pragma unroll
-        for (int k = 0; k < kHalf<V>; ++k) {
-          x[e][m][k] = fadd2(x[e][m][k], make_float2(minus_mean[e], V > 1 ? minus_mean[e] : 0.f));
-        }
+        for (int k = 0; k < kHalf<V>; ++k) x[e][m][k] = fadd2(x[e][m][k], twice(minus_mean[e]));
   }
   t = twice(0.f);
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < kSides<V>; ++m)
 #pragma unroll
       for (int k = 0; k < kHalf<V>; ++k) t = ffma2(x[e][m][k], x[e][m][k], t);
   s[0] = t.x + t.y;
@@ -272,7 +335,7 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < kSides<V>; ++m)
 #pragma unroll
       for (int k = 0; k < kHalf<V>; ++k) x[e][m][k] = fmul2(x[e][m][k], twice(inverse));
   return inverse;
@@ -281,9 +344,9 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][2][kHalf<V>], const La
 // Rotation and the norm's weight and bias are one linear map of a pair of normalised values, of which a thread keeps six numbers per token:
 //   out1 = n1 (w1 c) - n2 (w2 s) + (b1 c - b2 s),  out2 = n2 (w2 c) + n1 (w1 s) + (b2 c + b1 s)
 template <int V, int G, int E, int BYTES, int CB>
-__global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 6) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
+__global__ void __launch_bounds__(kNrThreads, E * V > 4 || Tile<V, G, E, BYTES, CB, 1>::kChunks > 4 ? 4 : 6) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
   using T = Tile<V, G, E, BYTES, CB, 1>;
-  constexpr int H = kHalf<V>, kChunks = T::kChunks;
+  constexpr int H = kHalf<V>, S = kSides<V>, kChunks = T::kChunks;
   extern __shared__ __align__(16) char smem[];
   griddep_wait();
   griddep_launch();
@@ -344,23 +407,22 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 6) norm_r
     return;
   }
   const bool normed = p.normed[h.part];
-  float2 own[E][2][H], other[E][2][H], add[E][2][H];               // what multiplies a member, its partner, and what is added
+  float2 own[E][S][H], other[E][S][H], add[E][S][H];               // what multiplies a member, its partner, and what is added
   {
-    float2 c[E][H], s[E][H], w[E][2][H], bias[E][2][H];
+    float2 c[E][H], s[E][H], w[E][S][H], bias[E][S][H];
     angles<V, E>(c, s, l, p, b, at, in);
     parameter<V, E>(w, l, p.weight[h.part], p.param_type, 1.f);
     parameter<V, E>(bias, l, p.bias[h.part], p.param_type, 0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int k = 0; k < H; ++k) {
-        own[e][0][k] = fmul2(w[e][0][k], c[e][k]);
-        own[e][1][k] = fmul2(w[e][1][k], c[e][k]);
-        other[e][0][k] = minus(fmul2(w[e][1][k], s[e][k]));
-        other[e][1][k] = fmul2(w[e][0][k], s[e][k]);
-        add[e][0][k] = ffma2(bias[e][0][k], c[e][k], minus(fmul2(bias[e][1][k], s[e][k])));
-        add[e][1][k] = ffma2(bias[e][1][k], c[e][k], fmul2(bias[e][0][k], s[e][k]));
-      }
+      for (int m = 0; m < S; ++m)
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          own[e][m][k] = fmul2(w[e][m][k], c[e][k]);
+          other[e][m][k] = fmul2(quarter<V>(w[e], m, k, false), s[e][k]);
+          add[e][m][k] = ffma2(bias[e][m][k], c[e][k], fmul2(quarter<V>(bias[e], m, k, false), s[e][k]));
+        }
   }
   const uint32_t mine = lane / G * T::kPitch, zeros = smem_u32(smem) + T::kSmem - T::kZeros;
   uint32_t in_tile[E][2];                                          // its vectors in the first place; without columns: the zeros, whatever the place
@@ -375,34 +437,24 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 6) norm_r
   for (int i = 0; i < h.count; ++i) {
     cp_async_wait<T::kAhead - 1>();
     __syncwarp();                                                  // every lane's copies are there, and the last head's results have left
-    float2 x[E][2][H];
+    float2 x[E][S][H];
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        Vec<V, BYTES> raw;
-        take_vec<V, BYTES>(raw, in_tile[e][m] + (l.on[e] ? full : 0));
-        values<V, BYTES>(x[e][m], raw, p.type);
-      }
+    for (int e = 0; e < E; ++e) take_slot<V, BYTES>(x[e], in_tile[e][0] + (l.on[e] ? full : 0), in_tile[e][1] + (l.on[e] ? full : 0), p.type);
     next(full);
     __syncwarp();
     fetch();
     if (normed) normalise<V, G, E>(x, l, p, eps);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float2 y[2][H];
+      float2 y[S][H];
 #pragma unroll
-      for (int k = 0; k < H; ++k) {
-        y[0][k] = ffma2(x[e][0][k], own[e][0][k], ffma2(x[e][1][k], other[e][0][k], add[e][0][k]));
-        y[1][k] = ffma2(x[e][1][k], own[e][1][k], ffma2(x[e][0][k], other[e][1][k], add[e][1][k]));
-      }
-      if (l.on[e])
+      for (int m = 0; m < S; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          Vec<V, BYTES> o;
-          rounded<V, BYTES>(o, y[m], p.type);
-          put_vec<V, BYTES>(o, last + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES);
+        for (int k = 0; k < H; ++k) {
+          const float2 partner = V == 1 ? make_float2(x[e][m][k].y, x[e][m][k].x) : x[e][S - 1 - m][k];
+          y[m][k] = ffma2(x[e][m][k], own[e][m][k], ffma2(partner, other[e][m][k], add[e][m][k]));
         }
+      if (l.on[e]) put_slot<V, BYTES>(y, last + mine + l.slot[e].c0 * BYTES, last + mine + l.slot[e].c1 * BYTES, p.type);
     }
     __syncwarp();
     leave(last);
@@ -412,9 +464,9 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 6) norm_r
 // The gradient of a head: turned back, then through the norm as computed again from x.  Sums for weight and bias: over the CTA's tokens and heads in
 // registers, over the warp's groups by shuffles, over warps in shared memory, over CTAs by norm_rope_sums_kernel.
 template <int V, int G, int E, int BYTES, int CB>
-__global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
+__global__ void __launch_bounds__(kNrThreads, E * V > 4 || (V == 1 && E == 4) || Tile<V, G, E, BYTES, CB, 2>::kChunks > 4 ? 3 : 4) norm_rope_bwd_kernel(const __grid_constant__ NrParams p) {
   using T = Tile<V, G, E, BYTES, CB, 2>;
-  constexpr int H = kHalf<V>, kChunks = T::kChunks;
+  constexpr int H = kHalf<V>, S = kSides<V>, kChunks = T::kChunks;
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[2][kNrWarps][2 * V * G * E];
   griddep_wait();
@@ -424,12 +476,12 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_r
   const bool normed = h.part < 2 && p.normed[h.part < 2 ? h.part : 0];
   Lane<V, E> l;
   place<V, G, E>(l, p, lane % G);
-  float2 w[E][2][H], dw[E][2][H], db[E][2][H];
+  float2 w[E][S][H], dw[E][S][H], db[E][S][H];
   if (normed) parameter<V, E>(w, l, p.weight[h.part], p.param_type, 1.f);
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < S; ++m)
 #pragma unroll
       for (int k = 0; k < H; ++k) dw[e][m][k] = db[e][m][k] = twice(0.f);
   const char* d_out = static_cast<const char*>(p.d_out[h.part]);
@@ -508,38 +560,36 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_r
         continue;
       }
       __syncwarp();                                                // every lane's copies are there, and the last head's results have left
-      float2 d[E][2][H], x[E][2][H];
+      float2 d[E][S][H], x[E][S][H];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          Vec<V, BYTES> raw, d_raw;
-          // a token that is not there has whatever was in the tile
-          take_vec<V, BYTES>(d_raw, in && d_out ? in_tile[e][m] + (l.on[e] ? full : 0) : zeros);
-          values<V, BYTES>(d[e][m], d_raw, p.type);
-          if (normed) {
-            take_vec<V, BYTES>(raw, in ? in_tile[e][m] + (l.on[e] ? full + T::kBytes : 0) : zeros);
-            values<V, BYTES>(x[e][m], raw, p.type);
-          }
-        }
+      for (int e = 0; e < E; ++e) {
+        // a token that is not there has whatever was in the tile
+        const uint32_t of = l.on[e] ? full : 0, there = in ? l.on[e] ? full + T::kBytes : 0 : 0;
+        take_slot<V, BYTES>(d[e], in && d_out ? in_tile[e][0] + of : zeros, in && d_out ? in_tile[e][1] + of : zeros, p.type);
+        if (normed) take_slot<V, BYTES>(x[e], in ? in_tile[e][0] + there : zeros, in ? in_tile[e][1] + there : zeros, p.type);
+      }
       next(full);
       __syncwarp();
       fetch();
 #pragma unroll
-      for (int e = 0; e < E; ++e)
+      for (int e = 0; e < E; ++e) {
+        float2 turned[S][H];
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-          const float2 d1 = d[e][0][k], d2 = d[e][1][k];
-          d[e][0][k] = ffma2(d1, c[e][k], fmul2(d2, s[e][k]));
-          d[e][1][k] = ffma2(d2, c[e][k], minus(fmul2(d1, s[e][k])));
-        }
+        for (int m = 0; m < S; ++m)
+#pragma unroll
+          for (int k = 0; k < H; ++k) turned[m][k] = ffma2(d[e][m][k], c[e][k], fmul2(quarter<V>(d[e], m, k, true), s[e][k]));
+#pragma unroll
+        for (int m = 0; m < S; ++m)
+#pragma unroll
+          for (int k = 0; k < H; ++k) d[e][m][k] = turned[m][k];
+      }
       if (normed) {
         const float inverse = normalise<V, G, E>(x, l, p, in ? p.eps[h.part] : 1.f);
         float2 t0 = twice(0.f), t1 = twice(0.f);                   // sums of e and of e n, e = d * weight
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < S; ++m)
 #pragma unroll
             for (int k = 0; k < H; ++k) {
               dw[e][m][k] = ffma2(d[e][m][k], x[e][m][k], dw[e][m][k]);
@@ -554,19 +604,13 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_r
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < S; ++m)
 #pragma unroll
             for (int k = 0; k < H; ++k) d[e][m][k] = ffma2(d[e][m][k], twice(inverse), ffma2(x[e][m][k], twice(along), twice(mean)));
       }
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (l.on[e])
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            Vec<V, BYTES> o;
-            rounded<V, BYTES>(o, d[e][m], p.type);
-            put_vec<V, BYTES>(o, last + mine + (m ? l.slot[e].c1 : l.slot[e].c0) * BYTES);
-          }
+        if (l.on[e]) put_slot<V, BYTES>(d[e], last + mine + l.slot[e].c0 * BYTES, last + mine + l.slot[e].c1 * BYTES, p.type);
       __syncwarp();
       leave(last);
     }
@@ -575,7 +619,7 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_r
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < S; ++m)
 #pragma unroll
       for (int k = 0; k < H; ++k) {
 #pragma unroll
@@ -584,13 +628,11 @@ __global__ void __launch_bounds__(kNrThreads, E * V < 2 || E > 1 ? 2 : 4) norm_r
           db[e][m][k] = fadd2(db[e][m][k], make_float2(__shfl_xor_sync(0xffffffffu, db[e][m][k].x, o), __shfl_xor_sync(0xffffffffu, db[e][m][k].y, o)));
         }
         if ((threadIdx.x & 31) < G && l.on[e]) {
-          const int col = (m ? l.slot[e].c1 : l.slot[e].c0) + 2 * k;
-          red[0][threadIdx.x >> 5][col] = dw[e][m][k].x;
-          red[1][threadIdx.x >> 5][col] = db[e][m][k].x;
-          if (V > 1) {
-            red[0][threadIdx.x >> 5][col + 1] = dw[e][m][k].y;
-            red[1][threadIdx.x >> 5][col + 1] = db[e][m][k].y;
-          }
+          const int x = column_x<V>(l.slot[e], m, k), y = column_y<V>(l.slot[e], m, k);
+          red[0][threadIdx.x >> 5][x] = dw[e][m][k].x;
+          red[1][threadIdx.x >> 5][x] = db[e][m][k].x;
+          red[0][threadIdx.x >> 5][y] = dw[e][m][k].y;
+          red[1][threadIdx.x >> 5][y] = db[e][m][k].y;
         }
       }
   __syncthreads();
@@ -653,13 +695,16 @@ static int run_norm_rope(const NrParams& p, bool backward, unsigned ctas, cudaSt
   if (backward) return launch(norm_rope_bwd_kernel<V, G, E, BYTES, CB>, grid, kNrThreads, kBackward, st, p);
   return launch(norm_rope_fwd_kernel<V, G, E, BYTES, CB>, grid, kNrThreads, kForward, st, p);
 }
-// The widest copy of at most 16 bytes that divides rows, addresses and strides, and no narrower than a vector; in between only what V = 1 has.
+// The widest copy of at most 16 bytes that divides rows, addresses and strides, and no narrower than a vector
 template <int V, int G, int E, int BYTES>
 static int by_chunk(const NrParams& p, int bytes, bool backward, unsigned ctas, cudaStream_t st) {
   constexpr int kVector = V * BYTES > 16 ? 16 : V * BYTES;
   if (bytes >= 16) return run_norm_rope<V, G, E, BYTES, 16>(p, backward, ctas, st);
-  if constexpr (kVector == 2) {
-    if (bytes >= 4) return run_norm_rope<V, G, E, BYTES, 4>(p, backward, ctas, st);
+  if constexpr (kVector <= 8) {
+    if (bytes == 8) return run_norm_rope<V, G, E, BYTES, 8>(p, backward, ctas, st);
+  }
+  if constexpr (kVector <= 4) {
+    if (bytes == 4) return run_norm_rope<V, G, E, BYTES, 4>(p, backward, ctas, st);
   }
   return run_norm_rope<V, G, E, BYTES, kVector>(p, backward, ctas, st);
 }
@@ -669,15 +714,20 @@ struct NrShape {
 };
 template <int BYTES>
 static int pick_norm_rope(const NrParams& p, NrShape s, bool backward, unsigned ctas, cudaStream_t st) {
-  switch (s.vector * 100 + s.group + s.each - 1) {
-    case 408: return by_chunk<4, 8, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 416: return by_chunk<4, 16, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 432: return by_chunk<4, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 216: return by_chunk<2, 16, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 232: return by_chunk<2, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 233: return by_chunk<2, 32, 2, BYTES>(p, s.bytes, backward, ctas, st);
-    case 132: return by_chunk<1, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
-    case 133: return by_chunk<1, 32, 2, BYTES>(p, s.bytes, backward, ctas, st);
+  switch (s.vector * 1000 + s.group * 10 + s.each) {
+    case 4081: return by_chunk<4, 8, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 4161: return by_chunk<4, 16, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 4321: return by_chunk<4, 32, 1, BYTES>(p, s.bytes, backward, ctas, st);
+    case 2082: return by_chunk<2, 8, 2, BYTES>(p, s.bytes, backward, ctas, st);
+    case 2083: return by_chunk<2, 8, 3, BYTES>(p, s.bytes, backward, ctas, st);
+    case 2162: return by_chunk<2, 16, 2, BYTES>(p, s.bytes, backward, ctas, st);
+    case 2163: return by_chunk<2, 16, 3, BYTES>(p, s.bytes, backward, ctas, st);
+    case 2322: return by_chunk<2, 32, 2, BYTES>(p, s.bytes, backward, ctas, st);
+    case 1083: return by_chunk<1, 8, 3, BYTES>(p, s.bytes, backward, ctas, st);
+    case 1084: return by_chunk<1, 8, 4, BYTES>(p, s.bytes, backward, ctas, st);
+    case 1163: return by_chunk<1, 16, 3, BYTES>(p, s.bytes, backward, ctas, st);
+    case 1164: return by_chunk<1, 16, 4, BYTES>(p, s.bytes, backward, ctas, st);
+    case 1323: return by_chunk<1, 32, 3, BYTES>(p, s.bytes, backward, ctas, st);
     default: return by_chunk<1, 32, 4, BYTES>(p, s.bytes, backward, ctas, st);
   }
 }
@@ -728,7 +778,9 @@ static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
   return 0;
 }
 
-// The largest vector, up to four elements, that divides pairs, what is not turned, addresses and strides
+// The largest vector, up to four elements, that divides pairs, what is not turned, addresses and strides, and groups of threads that hold a head with
+// eight to sixteen values each: a thread with less repeats the sums' shuffles for little (16 128 tokens of 16 heads, forward / backward: 50 channels, one
+// pair for each of 32 threads 73 / 156, four for each of 8 64 / 135; 72 channels 87 / 188 and 52 / 98).
 static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
   const int turned = 2 * f->axes * f->pairs, size = type_bytes(f->type);
   uint64_t grid = 16 | static_cast<uint64_t>(f->head_dim) * size;      // its lowest bit: what rows, addresses and strides are multiples of
@@ -737,10 +789,19 @@ static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* po
   const int bytes = static_cast<int>(grid & (~grid + 1));
   int v = 4;
   while (v > 1 && ((f->axes && f->pairs % v) || (f->head_dim - turned) % (2 * v) || (v * size < 16 ? v * size : 16) > bytes)) v /= 2;
-  const int slots = f->head_dim / (2 * v);
-  if (v == 4) return {4, slots <= 8 ? 8 : slots <= 16 ? 16 : 32, 1, bytes};
-  if (v == 2) return {2, slots <= 16 ? 16 : 32, slots <= 32 ? 1 : 2, bytes};
-  return {1, 32, slots <= 32 ? 1 : slots <= 64 ? 2 : 4, bytes};
+  int slots = f->head_dim / (2 * v);
+  if (v == 4) {
+    // A quarter of the threads or more without columns: three vectors of two for half as many threads, where those still fill the GPU (96 channels,
+    // 16 128 tokens 67 / 120 and 50 / 96; 2082 tokens 11.6 / 21 and 16.9 / 25)
+    const int group = slots <= 8 ? 8 : slots <= 16 ? 16 : 32;
+    const int64_t halved = (f->batch * f->tokens * (group / 2) + kNrThreads - 1) / kNrThreads;      // CTAs of groups of half as many threads
+    if (group == 8 || 4 * slots > 3 * group || halved < 2 * static_cast<int64_t>(sm_count())) return {4, group, 1, bytes};
+    v = 2, slots *= 2;
+  }
+  int group = 8;
+  const int most = v == 2 ? 3 : 4, least = most - 1;
+  while (group < 32 && slots > group * most) group *= 2;
+  return {v, group, slots <= group * least ? least : most, bytes};
 }
 
 static NrParams norm_rope_params(const s3r_qkv_norm_rope* f) {

@@ -34,6 +34,17 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {
   return BF16 ? make_float2(bf16_lo(w), bf16_hi(w)) : make_float2(half_lo(w), half_hi(w));
 }
 
+// An element that is asked for long before it is used: a register for either width, so that nothing waits for the load in front of its use.
+struct Early {
+  uint32_t wide, narrow;
+  Early() = default;
+  __device__ __forceinline__ Early(const void* p, int type, int64_t i, bool in) {
+    wide = p && in && type == S3R_F32 ? __ldg(static_cast<const uint32_t*>(p) + i) : 0;
+    narrow = p && in && type != S3R_F32 ? __ldg(static_cast<const uint16_t*>(p) + i) : 0;
+  }
+  __device__ __forceinline__ float value(int type) const { return type == S3R_F32 ? __uint_as_float(wide) : type == S3R_BF16 ? bf16_lo(narrow) : half_lo(narrow); }
+};
+
 template <int M, bool BF16>
 __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __grid_constant__ LinFewParams p) {
   extern __shared__ __align__(16) char smem[];
@@ -54,6 +65,11 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
   for (int m = 0; m < M; ++m)
     for (int c = threadIdx.x; c < chunks; c += 32 * kLinFewWarps) x[m * chunks + c] = m < p.M ? load_8(p.x + m * p.x_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
   __syncthreads();
+  // what a lane needs for its one result comes beside the weights
+  const int n = n0 + lane / M, row = lane % M;
+  const bool mine = lane < kLinFewChannels * M && row < p.M && n < p.N;
+  const int64_t at = static_cast<int64_t>(row) * p.N + n;
+  const Early bias(p.bias, p.bias_type, n, mine), scale(p.scale, p.scale_type, n, mine), residual(p.residual, p.residual_type, at, mine);
   float2 sum[kLinFewChannels][M];
 #pragma unroll
   for (int i = 0; i < kLinFewChannels; ++i)
@@ -84,6 +100,7 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
       }
     }
   }
+  float result = 0.f;
 #pragma unroll
   for (int i = 0; i < kLinFewChannels; ++i)
 #pragma unroll
@@ -91,23 +108,21 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
       float total = sum[i][m].x + sum[i][m].y;
 #pragma unroll
       for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      if (lane == i * M + m && m < p.M && n0 + i < p.N) {
-        const int n = n0 + i;
-        const int64_t at = static_cast<int64_t>(m) * p.N + n;
-        if (p.bias) total += load_one(p.bias, p.bias_type, n);
-        float v[1];
-        with_act(p.act, [&](auto act) {
-          float2 slope;
-          v[0] = activate<decltype(act)::value, false>(both(total), slope).x;
-          return 0;
-        });
-        const float s = p.scale ? load_one(p.scale, p.scale_type, n) : 1.f;
-        v[0] = p.residual ? __fmaf_rn(v[0], s, load_one(p.residual, p.residual_type, at)) : v[0] * s;
-        Raw<1> o;
-        pack<1>(o, v, p.out_type);
-        store_raw<1>(o, p.out, p.out_type, at);
-      }
+      if (lane == i * M + m) result = total;
     }
+  if (!mine) return;
+  if (p.bias) result += bias.value(p.bias_type);
+  float v[1];
+  with_act(p.act, [&](auto act) {
+    float2 slope;
+    v[0] = activate<decltype(act)::value, false>(both(result), slope).x;
+    return 0;
+  });
+  const float s = p.scale ? scale.value(p.scale_type) : 1.f;
+  v[0] = p.residual ? __fmaf_rn(v[0], s, residual.value(p.residual_type)) : v[0] * s;
+  Raw<1> o;
+  pack<1>(o, v, p.out_type);
+  store_raw<1>(o, p.out, p.out_type, at);
 }
 
 template <int M>
@@ -140,6 +155,14 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   const int col = static_cast<int>(i - row * p.quads) * 4;
   const float* from = p.sums + row * p.pitch + col;
   const int64_t part = p.part_rows * p.pitch;
+  const int64_t at = row * p.N + col;
+  Early bias[4], scale[4], residual[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    bias[k] = Early(p.bias, p.bias_type, col + k, col + k < p.N);
+    scale[k] = Early(p.scale, p.scale_type, col + k, col + k < p.N);
+    residual[k] = Early(p.residual, p.residual_type, at + k, col + k < p.N);
+  }
   float4 v[16];
 #pragma unroll
   for (int s = 0; s < 16; ++s)
@@ -148,10 +171,9 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
 #pragma unroll
   for (int s = 1; s < 16; ++s)
     if (s < p.parts) f[0] += v[s].x, f[1] += v[s].y, f[2] += v[s].z, f[3] += v[s].w;
-  const int64_t at = row * p.N + col;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (p.bias && col + k < p.N) f[k] += load_one(p.bias, p.bias_type, col + k);
+    if (p.bias) f[k] += bias[k].value(p.bias_type);
   with_act(p.act, [&](auto act) {
     float2 slope;
     const float2 a = activate<decltype(act)::value, false>(make_float2(f[0], f[1]), slope), b = activate<decltype(act)::value, false>(make_float2(f[2], f[3]), slope);
@@ -159,11 +181,10 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
     return 0;
   });
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (col + k < p.N) {
-      const float s = p.scale ? load_one(p.scale, p.scale_type, col + k) : 1.f;
-      f[k] = p.residual ? __fmaf_rn(f[k], s, load_one(p.residual, p.residual_type, at + k)) : f[k] * s;
-    }
+  for (int k = 0; k < 4; ++k) {
+    const float s = p.scale ? scale[k].value(p.scale_type) : 1.f;
+    f[k] = p.residual ? __fmaf_rn(f[k], s, residual[k].value(p.residual_type)) : f[k] * s;
+  }
   if (p.vectors) {
     Raw<4> o;
     pack<4>(o, f, p.out_type);

@@ -243,6 +243,16 @@ __device__ __forceinline__ void pack_pairs(uint32_t (&x)[WORDS], const float2 (&
   }
 }
 
+// every 32nd element from `col` on, as it lies in memory, 0 from element `end` on
+template <int N>
+__device__ __forceinline__ void load_factors(uint32_t (&f)[N], const void* p, int type, int end, int col) {
+  with_width(type, [&](auto width) {
+    const auto* from = static_cast<const decltype(width)*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = col + 32 * i < end ? __ldg(from + col + 32 * i) : 0;
+  });
+}
+
 // four 8 x 8 matrices of 16-bit elements: lane l has elements 2 (l % 4) and the next of row l / 4, and gives the address of row l % 8 of matrix l / 8
 __device__ __forceinline__ void stsm_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
@@ -409,16 +419,11 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       constexpr bool kInPlace = OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
       const bool by_copy = kInPlace && p.other_copied;
       // What the next tile needs is asked for a tile ahead.
-      Raw<1> scales[kMine], biases[kMine];
+      uint32_t scales[kMine], biases[kMine];
       uint32_t o[OTHER == kNoOther ? 1 : OTHER == S3R_F32 ? 32 : 16];
       auto fetch = [&](int tile, Tile at) {
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int col = at.n * TN + from + i * 32 + lane;
-          const bool in = tile < tiles && col < p.N;
-          load_raw<1>(scales[i], p.scale, p.scale_type, col, in && p.scale);
-          load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
-        }
+        if (p.scale) load_factors(scales, p.scale, p.scale_type, tile < tiles ? p.N : 0, at.n * TN + from + lane);
+        if (p.bias) load_factors(biases, p.bias, p.bias_type, tile < tiles ? p.N : 0, at.n * TN + from + lane);
       };
       auto ahead = [&](int tile, Tile at, int g) {
         if constexpr (OTHER != kNoOther) {
@@ -479,11 +484,8 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
         __syncwarp();                                                // the last tile's factors are read
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-          float f[1];
-          unpack<1>(f, scales[i], p.scale_type);
-          factors[i * 32 + lane] = p.scale ? f[0] : 1.f;
-          unpack<1>(f, biases[i], p.bias_type);
-          factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
+          factors[i * 32 + lane] = p.scale ? any_value(scales[i], p.scale_type) : 1.f;
+          factors[C::kSpan + i * 32 + lane] = p.bias ? any_value(biases[i], p.bias_type) : 0.f;
         }
         __syncwarp();
         advance(after);
@@ -615,16 +617,11 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       // ahead.  In the layout of tensor memory's 16 x 256 bits a lane's elements are those of 8 x 8 matrices.  Other dy is read from memory, fp32
       // 32 columns ahead.
       const bool by_copy = OTHER != S3R_F32 && p.other_copied;
-      Raw<1> scales[kMine], biases[kMine];
+      uint32_t scales[kMine], biases[kMine];
       uint32_t o[OTHER == S3R_F32 ? 32 : 16];
       auto fetch = [&](int tile, Tile at) {
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int col = at.n * TN + from + i * 32 + lane;
-          const bool in = tile < tiles && col < p.N;
-          if (DZ == 2) load_raw<1>(scales[i], p.scale, p.scale_type, col, in);
-          load_raw<1>(biases[i], p.bias, p.bias_type, col, in && p.bias);
-        }
+        if (DZ == 2) load_factors(scales, p.scale, p.scale_type, tile < tiles ? p.N : 0, at.n * TN + from + lane);
+        if (p.bias) load_factors(biases, p.bias, p.bias_type, tile < tiles ? p.N : 0, at.n * TN + from + lane);
       };
       auto ahead = [&](int tile, Tile at, int g) {
         if (OTHER != S3R_F32 || tile >= tiles) return;
@@ -681,13 +678,8 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
         __syncwarp();                                                // the last tile's factors are read
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-          float f[1];
-          if (DZ == 2) {
-            unpack<1>(f, scales[i], p.scale_type);
-            factors[i * 32 + lane] = f[0];
-          }
-          unpack<1>(f, biases[i], p.bias_type);
-          factors[C::kSpan + i * 32 + lane] = p.bias ? f[0] : 0.f;
+          if (DZ == 2) factors[i * 32 + lane] = any_value(scales[i], p.scale_type);
+          factors[C::kSpan + i * 32 + lane] = p.bias ? any_value(biases[i], p.bias_type) : 0.f;
         }
         __syncwarp();
         advance(after);

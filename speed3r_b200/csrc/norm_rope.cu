@@ -213,14 +213,6 @@ template <int V>
 __device__ __forceinline__ int column_x(const Slot& s, int m, int k) { return (m ? s.c1 : s.c0) + 2 * k; }
 template <int V>
 __device__ __forceinline__ int column_y(const Slot& s, int m, int k) { return V == 1 ? s.c1 : column_x<V>(s, m, k) + 1; }
-// f(an element's width): decided once in front of all loads, which then are on their way together; a load that decides for itself is waited for
-// before the next (forward 139 us where this takes 132, one token of 16 heads 3.8 and 3.0)
-template <typename F>
-__device__ __forceinline__ void with_width(int type, F f) {
-  if (type == S3R_F32) f(uint32_t());
-  else f(uint16_t());
-}
-__device__ __forceinline__ float any_value(uint32_t w, int type) { return type == S3R_F32 ? __uint_as_float(w) : type == S3R_BF16 ? bf16_lo(w) : half_lo(w); }
 template <int V, int E>
 __device__ __forceinline__ void parameter(float2 (&f)[E][kSides<V>][kHalf<V>], const Lane<V, E>& l, const void* from, int type, float other) {
   uint32_t raw[E][kSides<V>][kHalf<V>][2];

@@ -176,6 +176,14 @@ __device__ __forceinline__ float load_one(const void* p, int type, int64_t i) {
   unpack<1>(f, r, type);
   return f[0];
 }
+// f(an element's width): decided once in front of all loads, which then are on their way together; a load that decides for itself is waited for
+// before the next, as load_one does (norms and rotation of 64 512 x 16 heads of 64: 139 us, this way 132; of one token 3.8 and 3.0)
+template <typename F>
+__device__ __forceinline__ void with_width(int type, F f) {
+  if (type == S3R_F32) f(uint32_t());
+  else f(uint16_t());
+}
+__device__ __forceinline__ float any_value(uint32_t w, int type) { return type == S3R_F32 ? __uint_as_float(w) : type == S3R_BF16 ? bf16_lo(w) : half_lo(w); }
 template <int W>
 __device__ __forceinline__ void load_vector(float (&f)[W], const void* p, int type, int64_t i) {
   Raw<W> r;

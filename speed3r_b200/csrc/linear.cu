@@ -8,11 +8,12 @@
 namespace s3r {
 
 // ---------------------------------------------------------------------------------------------------------------------
-// a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has two output channels,
-// a lane 16 bytes of each at a time and four of those in flight; the tokens lie in shared memory.  One token x 4096 x 1024, weights in HBM: 7 us, of
-// which 1.3 are the weights' bytes, and the rest the start of the kernel and one trip to memory.
+// a few tokens: the weights are read once, at the rate of memory, and tensor cores would wait for tiles of them.  A warp has two output channels
+// (one where that still leaves an SM no more than a CTA), a lane 16 bytes at a time and eight of those in flight; the tokens lie in shared memory.
+// Bound: the start of the kernel and its trips to memory, one for each 4 KB of a channel's weights.  One token x 4096 x 1024, one call behind the other in
+// a graph, weights in HBM: 4.3 us, of which 1.3 are the weights' bytes; eight tokens x 1024 x 1024 6.0.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kLinFew = 8, kLinFewBytes = 48 * 1024, kLinFewChannels = 2, kLinFewWarps = 8, kLinFewAhead = 4;
+constexpr int kLinFew = 8, kLinFewBytes = 48 * 1024, kLinFewWarps = 8;
 
 struct LinFewParams {
   const uint16_t *x, *w;
@@ -45,56 +46,57 @@ struct Early {
   __device__ __forceinline__ float value(int type) const { return type == S3R_F32 ? __uint_as_float(wide) : type == S3R_BF16 ? bf16_lo(narrow) : half_lo(narrow); }
 };
 
-template <int M, bool BF16>
+template <int M, bool BF16, int CHANNELS>
 __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __grid_constant__ LinFewParams p) {
+  constexpr int kAhead = 8 / CHANNELS;
   extern __shared__ __align__(16) char smem[];
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (p.K + 7) / 8;
   uint4* x = reinterpret_cast<uint4*>(smem);                       // [M][chunks]
-  const int n0 = (blockIdx.x * kLinFewWarps + warp) * kLinFewChannels;
+  const int n0 = (blockIdx.x * kLinFewWarps + warp) * CHANNELS;
   // the first weights are on their way while the tokens are fetched
-  uint4 w[kLinFewAhead][kLinFewChannels];
+  uint4 w[kAhead][CHANNELS];
   auto fetch = [&](int c, int at) {
 #pragma unroll
-    for (int i = 0; i < kLinFewChannels; ++i) w[at][i] = n0 + i < p.N && c < chunks ? load_8(p.w + (n0 + i) * p.w_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < CHANNELS; ++i) w[at][i] = n0 + i < p.N && c < chunks ? load_8(p.w + (n0 + i) * p.w_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
   };
 #pragma unroll
-  for (int k = 0; k < kLinFewAhead; ++k) fetch(lane + 32 * k, k);
+  for (int k = 0; k < kAhead; ++k) fetch(lane + 32 * k, k);
 #pragma unroll
   for (int m = 0; m < M; ++m)
     for (int c = threadIdx.x; c < chunks; c += 32 * kLinFewWarps) x[m * chunks + c] = m < p.M ? load_8(p.x + m * p.x_pitch, c * 8, p.K) : make_uint4(0, 0, 0, 0);
   __syncthreads();
   // what a lane needs for its one result comes beside the weights
   const int n = n0 + lane / M, row = lane % M;
-  const bool mine = lane < kLinFewChannels * M && row < p.M && n < p.N;
+  const bool mine = lane < CHANNELS * M && row < p.M && n < p.N;
   const int64_t at = static_cast<int64_t>(row) * p.N + n;
   const Early bias(p.bias, p.bias_type, n, mine), scale(p.scale, p.scale_type, n, mine), residual(p.residual, p.residual_type, at, mine);
-  float2 sum[kLinFewChannels][M];
+  float2 sum[CHANNELS][M];
 #pragma unroll
-  for (int i = 0; i < kLinFewChannels; ++i)
+  for (int i = 0; i < CHANNELS; ++i)
 #pragma unroll
     for (int m = 0; m < M; ++m) sum[i][m] = both(0.f);
-  for (int c0 = lane; c0 < chunks; c0 += 32 * kLinFewAhead) {
+  for (int c0 = lane; c0 < chunks; c0 += 32 * kAhead) {
 #pragma unroll
-    for (int k = 0; k < kLinFewAhead; ++k) {
+    for (int k = 0; k < kAhead; ++k) {
       const int c = c0 + 32 * k;
-      float2 now[kLinFewChannels][4];
+      float2 now[CHANNELS][4];
 #pragma unroll
-      for (int i = 0; i < kLinFewChannels; ++i) {
+      for (int i = 0; i < CHANNELS; ++i) {
         now[i][0] = pair_of<BF16>(w[k][i].x);
         now[i][1] = pair_of<BF16>(w[k][i].y);
         now[i][2] = pair_of<BF16>(w[k][i].z);
         now[i][3] = pair_of<BF16>(w[k][i].w);
       }
-      fetch(c + 32 * kLinFewAhead, k);
+      fetch(c + 32 * kAhead, k);
       if (c >= chunks) continue;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const uint4 t = x[m * chunks + c];
         const float2 v[4] = {pair_of<BF16>(t.x), pair_of<BF16>(t.y), pair_of<BF16>(t.z), pair_of<BF16>(t.w)};
 #pragma unroll
-        for (int i = 0; i < kLinFewChannels; ++i)
+        for (int i = 0; i < CHANNELS; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) sum[i][m] = ffma2(now[i][j], v[j], sum[i][m]);
       }
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
   }
   float result = 0.f;
 #pragma unroll
-  for (int i = 0; i < kLinFewChannels; ++i)
+  for (int i = 0; i < CHANNELS; ++i)
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       float total = sum[i][m].x + sum[i][m].y;
@@ -125,14 +127,19 @@ __global__ void __launch_bounds__(32 * kLinFewWarps) linear_few_kernel(const __g
   store_raw<1>(o, p.out, p.out_type, at);
 }
 
-template <int M>
-static int run_linear_few(const LinFewParams& p, cudaStream_t st) {
-  static_assert(M * kLinFewChannels <= 32, "a lane per result");
-  const int per = kLinFewWarps * kLinFewChannels;
+template <int M, int CHANNELS>
+static int run_few_channels(const LinFewParams& p, cudaStream_t st) {
+  static_assert(M * CHANNELS <= 32, "a lane per result");
+  const int per = kLinFewWarps * CHANNELS;
   const unsigned grid = static_cast<unsigned>((p.N + per - 1) / per);
   const size_t smem = static_cast<size_t>(M) * ((p.K + 7) / 8) * 16;
-  return p.type == S3R_BF16 ? launch(linear_few_kernel<M, true>, grid, 32 * kLinFewWarps, smem, st, p)
-                            : launch(linear_few_kernel<M, false>, grid, 32 * kLinFewWarps, smem, st, p);
+  return p.type == S3R_BF16 ? launch(linear_few_kernel<M, true, CHANNELS>, grid, 32 * kLinFewWarps, smem, st, p)
+                            : launch(linear_few_kernel<M, false, CHANNELS>, grid, 32 * kLinFewWarps, smem, st, p);
+}
+// One channel of 1024, a token: 2.9 us, two 3.2; of 4096 5.9 and 9.2.  4096 channels fill the SMs either way.
+template <int M>
+static int run_linear_few(const LinFewParams& p, cudaStream_t st) {
+  return p.N <= kLinFewWarps * sm_count() ? run_few_channels<M, 1>(p, st) : run_few_channels<M, 2>(p, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

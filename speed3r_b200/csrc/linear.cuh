@@ -89,9 +89,9 @@ int linear_partial(const LinOperand& a, const LinOperand& b, int64_t k, bool bf1
 // a turned one comes in boxes of 64 rows x 64 steps and is read through the other form of the matrix descriptor.
 //
 // Bound: the tensor cores, and at full size the power they take.  64 512 x 4096 x 1024 in bf16: the products alone 322 us (1680 TFLOP/s), with GELU
-// 360 to 400 by the clock that power leaves.  What the epilogue takes must stay below the products' time: alone (K = 64) it is 109 us for a sum that
-// is only rounded, 185 with SiLU, 231 with GELU, 376 with an fp32 residual, 380 for dz with GELU's slope and a sum over rows, of which the memory
-// traffic is 80, 80, 80, 320 and 161 (dz: dy read, dz written).  dz is the one that issues most: 41 % of all cycles, the tensor cores busy in 65 %
+// 384 at first and 435 at the clock that power leaves.  What the epilogue takes must stay below the products' time: alone (K = 64) it is 103 us for a sum that
+// is only rounded, 186 with SiLU, 234 with GELU, 376 with an fp32 residual, 391 for dz with GELU's slope and a sum over rows, of which the memory
+// traffic is 80, 80, 80, 320 and 161 (dz: dy read, dz written).  dz is the one that issues most: 40 % of all cycles, the tensor cores busy in 65 %
 // (forward with GELU 83 %).
 // Tried, and slower: sixteen summing warps, which spill (166 -> 237, dz 375 -> 494); two pieces of output per warp where nothing is read beside the
 // sums (166 -> 172); two sets of dz's sums in registers (373 -> 395).

@@ -772,7 +772,7 @@ static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
 
 // The largest vector, up to four elements, that divides pairs, what is not turned, addresses and strides, and groups of threads that hold a head with
 // eight to sixteen values each: a thread with less repeats the sums' shuffles for little (16 128 tokens of 16 heads, forward / backward: 50 channels, one
-// pair for each of 32 threads 73 / 156, four for each of 8 64 / 135; 72 channels 87 / 188 and 52 / 98).
+// pair for each of 32 threads 73 / 156, four for each of 8 64 / 135; 72 channels 87 / 188 and 52 / 98).  In a few tokens' work it costs a microsecond.
 static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
   const int turned = 2 * f->axes * f->pairs, size = type_bytes(f->type);
   uint64_t grid = 16 | static_cast<uint64_t>(f->head_dim) * size;      // its lowest bit: what rows, addresses and strides are multiples of

@@ -80,7 +80,7 @@ template <int V, int G, int E, int BYTES, int CB, int INPUTS>
 struct Tile {
   static constexpr int kZeros = V * BYTES < 16 ? 16 : V * BYTES;       // behind the tiles: what lanes without columns read
   static constexpr int kRows = 32 / G, kPitch = 2 * V * G * E * BYTES + 16, kBytes = kRows * kPitch;
-  static constexpr int kChunks = kRows * (kPitch - 16) / (32 * CB) < 1 ? 1 : kRows * (kPitch - 16) / (32 * CB);
+  static constexpr int kChunks = (kRows * (kPitch - 16) + 32 * CB - 1) / (32 * CB);
   static constexpr int kAhead = 4, kSmem = kNrWarps * kBytes * (kAhead * INPUTS + 1) + kZeros;
   struct Chunk {
     int row, byte;           // byte: in the row
@@ -772,7 +772,7 @@ static int check_norm_rope(const s3r_qkv_norm_rope* f, const char* what) {
 
 // The largest vector, up to four elements, that divides pairs, what is not turned, addresses and strides, and groups of threads that hold a head with
 // eight to sixteen values each: a thread with less repeats the sums' shuffles for little (16 128 tokens of 16 heads, forward / backward: 50 channels, one
-// pair for each of 32 threads 73 / 156, four for each of 8 64 / 135; 72 channels 87 / 188 and 52 / 98).  In a few tokens' work it costs a microsecond.
+// pair for each of 32 threads 73 / 156, four for each of 8 64 / 135; 72 channels 87 / 188 and 53 / 104).  In a few tokens' work it costs a microsecond.
 static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* pointers, int n_pointers, const int64_t* strides, int n_strides) {
   const int turned = 2 * f->axes * f->pairs, size = type_bytes(f->type);
   uint64_t grid = 16 | static_cast<uint64_t>(f->head_dim) * size;      // its lowest bit: what rows, addresses and strides are multiples of
@@ -784,7 +784,7 @@ static NrShape norm_rope_shape(const s3r_qkv_norm_rope* f, const void* const* po
   int slots = f->head_dim / (2 * v);
   if (v == 4) {
     // A quarter of the threads or more without columns: three vectors of two for half as many threads, where those still fill the GPU (96 channels,
-    // 16 128 tokens 67 / 120 and 50 / 96; 2082 tokens 11.6 / 21 and 16.9 / 25)
+    // 16 128 tokens 63 / 117 and 58 / 107; 6246 tokens 27.3 / 51.7 and 27.9 / 48.2)
     const int group = slots <= 8 ? 8 : slots <= 16 ? 16 : 32;
     const int64_t halved = (f->batch * f->tokens * (group / 2) + kNrThreads - 1) / kNrThreads;      // CTAs of groups of half as many threads
     if (group == 8 || 4 * slots > 3 * group || halved < 2 * static_cast<int64_t>(sm_count())) return {4, group, 1, bytes};

@@ -335,6 +335,8 @@ __device__ __forceinline__ float normalise(float2 (&x)[E][kSides<V>][kHalf<V>], 
 
 // Rotation and the norm's weight and bias are one linear map of a pair of normalised values, of which a thread keeps six numbers per token:
 //   out1 = n1 (w1 c) - n2 (w2 s) + (b1 c - b2 s),  out2 = n2 (w2 c) + n1 (w1 s) + (b2 c + b1 s)
+// Columns that no axis turns have no partner, not one times 0: 0 * infinity would be NaN.  What is added to them without a bias is -0, which leaves
+// every value as it is, -0 too.
 template <int V, int G, int E, int BYTES, int CB>
 __global__ void __launch_bounds__(kNrThreads, E * V > 4 || Tile<V, G, E, BYTES, CB, 1>::kChunks > 4 ? 4 : 6) norm_rope_fwd_kernel(const __grid_constant__ NrParams p) {
   using T = Tile<V, G, E, BYTES, CB, 1>;
@@ -411,9 +413,10 @@ __global__ void __launch_bounds__(kNrThreads, E * V > 4 || Tile<V, G, E, BYTES, 
       for (int m = 0; m < S; ++m)
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          own[e][m][k] = fmul2(w[e][m][k], c[e][k]);
+          const bool turned = l.slot[e].axis >= 0;
+          own[e][m][k] = turned ? fmul2(w[e][m][k], c[e][k]) : w[e][m][k];
           other[e][m][k] = fmul2(quarter<V>(w[e], m, k, false), s[e][k]);
-          add[e][m][k] = ffma2(bias[e][m][k], c[e][k], fmul2(quarter<V>(bias[e], m, k, false), s[e][k]));
+          add[e][m][k] = turned ? ffma2(bias[e][m][k], c[e][k], fmul2(quarter<V>(bias[e], m, k, false), s[e][k])) : p.bias[h.part] ? bias[e][m][k] : twice(-0.f);
         }
   }
   const uint32_t mine = lane / G * T::kPitch, zeros = smem_u32(smem) + T::kSmem - T::kZeros;
@@ -425,6 +428,7 @@ __global__ void __launch_bounds__(kNrThreads, E * V > 4 || Tile<V, G, E, BYTES, 
   if (threadIdx.x < T::kZeros / 4) sts32(zeros + 4 * threadIdx.x, 0);
   __syncthreads();
   const float eps = p.eps[h.part];
+  const int turned_slots = p.axes * (p.pairs / V);                 // a slot's number tells whether an axis turns it: no register for each
 #pragma unroll 1
   for (int i = 0; i < h.count; ++i) {
     cp_async_wait<T::kAhead - 1>();
@@ -445,6 +449,7 @@ __global__ void __launch_bounds__(kNrThreads, E * V > 4 || Tile<V, G, E, BYTES, 
         for (int k = 0; k < H; ++k) {
           const float2 partner = V == 1 ? make_float2(x[e][m][k].y, x[e][m][k].x) : x[e][S - 1 - m][k];
           y[m][k] = ffma2(x[e][m][k], own[e][m][k], ffma2(partner, other[e][m][k], add[e][m][k]));
+          if (lane % G + e * G >= turned_slots) y[m][k] = ffma2(x[e][m][k], own[e][m][k], add[e][m][k]);
         }
       if (l.on[e]) put_slot<V, BYTES>(y, last + mine + l.slot[e].c0 * BYTES, last + mine + l.slot[e].c1 * BYTES, p.type);
     }
@@ -479,6 +484,7 @@ __global__ void __launch_bounds__(kNrThreads, E * V > 4 || (V == 1 && E == 4) ||
   const char* d_out = static_cast<const char*>(p.d_out[h.part]);
   const int64_t row_bytes = p.head_dim * BYTES, width = (p.heads + 2 * p.kv_heads) * row_bytes, column = packed_head(h, p) * row_bytes;
   const int64_t d_head = p.d_strides[h.part][1] * BYTES;
+  const int turned_slots = p.axes * (p.pairs / V);
   const uint32_t ring = smem_u32(smem) + warp * T::kBytes * (2 * T::kAhead + 1), last = ring + 2 * T::kAhead * T::kBytes, mine = lane / G * T::kPitch;
   const uint32_t zeros = smem_u32(smem) + T::kSmem - T::kZeros;
   uint32_t in_tile[E][2];                                          // its vectors in the first place; without columns: the zeros, whatever the place
@@ -565,15 +571,16 @@ __global__ void __launch_bounds__(kNrThreads, E * V > 4 || (V == 1 && E == 4) ||
       fetch();
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        float2 turned[S][H];
+        float2 partner[S][H];
 #pragma unroll
         for (int m = 0; m < S; ++m)
 #pragma unroll
-          for (int k = 0; k < H; ++k) turned[m][k] = ffma2(d[e][m][k], c[e][k], fmul2(quarter<V>(d[e], m, k, true), s[e][k]));
+          for (int k = 0; k < H; ++k) partner[m][k] = fmul2(quarter<V>(d[e], m, k, true), s[e][k]);
+        if (lane % G + e * G >= turned_slots) continue;            // no partner where nothing turns, as in the forward
 #pragma unroll
         for (int m = 0; m < S; ++m)
 #pragma unroll
-          for (int k = 0; k < H; ++k) d[e][m][k] = turned[m][k];
+          for (int k = 0; k < H; ++k) d[e][m][k] = ffma2(d[e][m][k], c[e][k], partner[m][k]);
       }
       if (normed) {
         const float inverse = normalise<V, G, E>(x, l, p, in ? p.eps[h.part] : 1.f);

@@ -1,0 +1,74 @@
+"""Values that linear and qkv_norm_rope have to leave alone or carry through: infinities, NaN and -0 next to other columns, huge arguments."""
+import math
+
+import pytest
+import torch
+
+from speed3r_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def no_status():
+    _lib.device_status()
+    yield
+    assert _lib.device_status() == 0
+
+
+def same_bits(a, b):
+    whole = torch.int32 if a.dtype == FP32 else torch.int16
+    nan = torch.isnan(a)
+    assert torch.equal(nan, torch.isnan(b))
+    assert torch.equal(a.contiguous().view(whole)[~nan], b.contiguous().view(whole)[~nan])
+
+
+# channels, axes, pairs: vectors of 4, 2 and 1 elements without a rotation, and with one of a part of the columns
+STILL = [(64, 0, 0), (36, 0, 0), (50, 0, 0), (250, 0, 0), (80, 1, 20), (100, 1, 10), (66, 1, 15), (128, 2, 16), (254, 3, 5)]
+
+
+@pytest.mark.parametrize("x", (BF16, F16, FP32))
+@pytest.mark.parametrize("d, axes, pairs", STILL)
+def test_columns_that_are_not_turned_are_their_own(d, axes, pairs, x):
+    """Without a norm they leave as they came, forward and backward, whatever stands next to them; one special value per token."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    first, T = 2 * axes * pairs, 4 * (d - 2 * axes * pairs)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=g).to(x)
+    pos = torch.randint(0, 20, (1, T, axes), device=DEV, generator=g) if axes else None
+    cos, sin = (rand(20, pairs), rand(20, pairs)) if axes else (None, None)
+    clean = [rand(1, T, d) for _ in range(6)]                    # q, k, v and their gradients
+    special = torch.tensor([math.inf, -math.inf, math.nan, -0.0], device=DEV).to(x).repeat(d - first)
+    planted = [t.clone() for t in clean]
+    for t in planted:
+        t[0, torch.arange(T), first + torch.arange(T) // 4] = special
+    results = []
+    for q, k, v, dq, dk, dv in (clean, planted):
+        qkv = torch.cat((q, k, v), -1).requires_grad_(True)
+        out = ops.qkv_norm_rope(qkv, 1, 1, pos, cos, sin)
+        back = torch.autograd.grad(out, qkv, [t[:, None] for t in (dq, dk, dv)])[0]
+        results.append([o.detach()[:, 0] for o in out] + list(back.split(d, -1)))
+    for i, (was, now) in enumerate(zip(*results)):
+        still = slice(0 if i % 3 == 2 else first, d)             # v is never turned
+        same_bits(now[..., still], planted[i][..., still])
+        assert torch.equal(now[..., :first], was[..., :first])
+
+
+@pytest.mark.parametrize("d, axes, pairs", STILL)
+def test_parameters_of_columns_that_are_not_turned_are_their_own(d, axes, pairs):
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    first, T = 2 * axes * pairs, 9
+    qkv, w, b = rand(1, T, 3 * d).to(BF16), rand(d), rand(d)
+    pos = torch.randint(0, 20, (1, T, axes), device=DEV, generator=g) if axes else None
+    cos, sin = (rand(20, pairs), rand(20, pairs)) if axes else (None, None)
+    call = lambda w, b: ops.qkv_norm_rope(qkv, 1, 1, pos, cos, sin, (w, b, 1e-5), (w, b, 1e-5))[:2]
+    clean = call(w, b)
+    for column in (first, first + 1, first + 3, (first + d) // 2, d - 1):
+        for which in range(2):
+            params = [w.clone(), b.clone()]
+            params[which][column] = math.inf
+            rest = torch.arange(d, device=DEV) != column
+            for was, now in zip(clean, call(*params)):
+                assert torch.isinf(now[..., column]).all() and torch.equal(now[..., rest], was[..., rest])

@@ -51,9 +51,10 @@ __device__ __forceinline__ float2 activate(float2 z, float2& slope) {
     const float2 p = fast_rcp2(fadd2(exp2_2(arg), both(1.f)));
     const float2 u = fmul2(z, p);
     if (SLOPE) {
-      // p + u (1 - p) times the argument's own slope: 1, or 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2), last, for it may be huge where 1 - p is 0
-      const float2 rest = fadd2(both(1.f), make_float2(-p.x, -p.y));
-      slope = ACT == S3R_ACT_SILU ? ffma2(u, rest, p) : ffma2(fmul2(u, rest), ffma2(q, both(0.214064488f), both(1.59576912f)), p);
+      // p + u (1 - p) times the argument's own slope: 1, or 2 sqrt(2 / pi) (1 + 3 * 0.044715 z^2), last, for it may be huge where 1 - p is 0.  z^2
+      // is infinite from |z| = 2^64 on, and 0 times that NaN: it stays at 2^100, from where on u (1 - p) has long been 0 on either side.
+      const float2 rest = fadd2(both(1.f), make_float2(-p.x, -p.y)), finite = make_float2(fminf(q.x, 0x1p100f), fminf(q.y, 0x1p100f));
+      slope = ACT == S3R_ACT_SILU ? ffma2(u, rest, p) : ffma2(fmul2(u, rest), ffma2(finite, both(0.214064488f), both(1.59576912f)), p);
     }
     return u;
   }

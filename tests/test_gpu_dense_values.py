@@ -72,3 +72,24 @@ def test_parameters_of_columns_that_are_not_turned_are_their_own(d, axes, pairs)
             rest = torch.arange(d, device=DEV) != column
             for was, now in zip(clean, call(*params)):
                 assert torch.isinf(now[..., column]).all() and torch.equal(now[..., rest], was[..., rest])
+
+
+@pytest.mark.parametrize("scale", (False, True))
+@pytest.mark.parametrize("act", ("gelu", "gelu_tanh", "silu"))
+def test_slopes_as_far_out_as_bf16_reaches(act, scale):
+    """z^2 is infinite in fp32 from 2^64 on: the activations are still z and 0 there, their slopes 1 and 0, exactly."""
+    powers = [p for p in range(10, 124, 2)]
+    M = 2 * len(powers)
+    x = torch.zeros(M, 16, device=DEV, dtype=BF16)
+    x[:, 0] = torch.tensor([sign * 2.0 ** p for p in powers for sign in (1, -1)], device=DEV)
+    x.requires_grad_(True)
+    w = torch.zeros(24, 16, device=DEV, dtype=BF16)
+    w[:, 0] = 1
+    s = torch.full((24,), 2.0, device=DEV, requires_grad=True) if scale else None
+    y = ops.linear(x, w, torch.zeros(24, device=DEV), act=act, scale=s)
+    factor = 2.0 if scale else 1.0
+    assert torch.equal(y, factor * torch.relu(x[:, :1]).expand(M, 24))
+    grads = torch.autograd.grad(y, [x] + ([s] if scale else []), torch.ones_like(y))
+    assert torch.equal(grads[0][:, 0], 24.0 * factor * (x[:, 0] > 0)) and not grads[0][:, 1:].any()
+    if scale:
+        assert torch.allclose(grads[1].double(), torch.relu(x.double()[:, 0]).sum().expand(24), rtol=2.0 ** -20, atol=0)     # 57 additions of 2^-24

@@ -131,6 +131,9 @@ struct LinCtl {
   uint32_t tmem_base, abort_flag;
 };
 
+// How long a tile's sums are waited for: a step takes about 0.25 us, and a contraction may have 33 million of them.
+__device__ __forceinline__ uint64_t tile_limit_ns(int steps) { return 1000000000ull + 1000ull * static_cast<uint32_t>(steps); }
+
 // kind::f16 with fp32 sums; a_type, b_type: 0 fp16, 1 bf16
 constexpr uint32_t umma_idesc_half(uint32_t M, uint32_t N, uint32_t bf16, uint32_t a_turned, uint32_t b_turned) {
   return (1u << 4) | (bf16 << 7) | (bf16 << 10) | (a_turned << 15) | (b_turned << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
         advance(after);
         fetch(tile + stride, after);
         soon(tile + stride, after);
-        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
+        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag, tile_limit_ns(steps));
         if (!ok) break;
         tc_fence_after();
         // 32 columns' sums; when they are there, or have been used, the next 32 are asked for; the last ones free the tile's columns
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
         advance(after);
         fetch(tile + stride, after);
         soon(tile + stride, after);
-        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag);
+        ok = mbar_wait_warp(&ctl.acc_full[buf], done >> 1 & 1, abort_flag, tile_limit_ns(steps));
         if (!ok) break;
         tc_fence_after();
         const uint32_t sums = tmem + (static_cast<uint32_t>(quarter) << 21) + buf * TN + from;

@@ -93,3 +93,16 @@ def test_slopes_as_far_out_as_bf16_reaches(act, scale):
     assert torch.equal(grads[0][:, 0], 24.0 * factor * (x[:, 0] > 0)) and not grads[0][:, 1:].any()
     if scale:
         assert torch.allclose(grads[1].double(), torch.relu(x.double()[:, 0]).sum().expand(24), rtol=2.0 ** -20, atol=0)     # 57 additions of 2^-24
+
+
+def test_a_sum_that_takes_seconds():
+    """The longest that linear takes, made again in one part by the backward: no wait gives up on it (the status word is looked at)."""
+    K = 2 ** 30 - 8
+    x, w = torch.zeros(1, K, device=DEV, dtype=BF16), torch.zeros(1, K, device=DEV, dtype=BF16)
+    x[0, 0], x[0, K // 2], x[0, -1] = 1.0, 2.0, -0.5
+    w[0, 0], w[0, K // 2], w[0, -1] = 0.5, 0.25, 1.0
+    b = torch.zeros(1, device=DEV, requires_grad=True)
+    y = ops.linear(x, w, b, act="silu", out_dtype=FP32)
+    db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
+    p = 1 / (1 + math.exp(-0.5))                                 # z = 0.5; the sigmoid within 2^-21
+    assert abs(y.item() - 0.5 * p) <= 2.0 ** -20 and abs(db.item() - p * (1 + 0.5 * (1 - p))) <= 2.0 ** -19

@@ -74,13 +74,20 @@ class FusedMlp(Mlp):
             return None
         return product_type(x, self.fc1, self.fc2)
 
+    def _sums(self, x: Tensor, residual: Optional[Tensor], scale: Optional[Tensor]) -> bool:
+        """The second product takes this residual and this scale: no types beyond the kernel's, nothing that is broadcast."""
+        N = self.fc2.out_features
+        return all(v is None or (v.dtype in ops.NORM_TYPES and v.device == x.device and v.shape == shape)
+                   for v, shape in ((residual, (*x.shape[:-1], N)), (scale, (N,))))
+
     def forward(self, x, residual: Optional[Tensor] = None, scale: Optional[Tensor] = None) -> Tensor:
-        """``residual + mlp(x) * scale``, in the residual's type, or the MLP alone"""
+        """``residual + mlp(x) * scale``, in the residual's type, or without one in the MLP's own"""
         t = self._type(x)
-        if t is None:
+        if t is None or not self._sums(x, residual, scale):
             y = super().forward(x)
+            kept = y.dtype if residual is None else residual.dtype
             y = y if scale is None else y * scale
-            return y if residual is None else residual + y
+            return (y if residual is None else residual + y).to(kept)
         of = lambda p: None if p is None else p.to(t)
         h = ops.linear(x.to(t), of(self.fc1.weight), self.fc1.bias, self._act())
         return ops.linear(h, of(self.fc2.weight), self.fc2.bias, None, residual, scale, t if residual is None else residual.dtype)

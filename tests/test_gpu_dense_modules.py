@@ -1,0 +1,54 @@
+"""FusedMlp and FlashAttentionRope where their modules are replaced, watched or given what the kernels do not take."""
+import itertools
+
+import pytest
+import torch
+
+from speed3r_b200 import _lib
+from test_gpu_block import DEV, DIM, near
+from test_gpu_dense_block import launched, mlps
+
+pytestmark = pytest.mark.gpu
+BF16, F16, FP32, FP64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+
+
+@pytest.fixture(autouse=True)
+def no_status():
+    _lib.device_status()
+    yield
+    assert _lib.device_status() == 0
+
+
+def fused(f):
+    return sum("linear_kernel" in n or "linear_few" in n for n in launched(f)) == 2
+
+
+@pytest.mark.parametrize("residual, scale", list(itertools.product((None, BF16, F16, FP32, FP64), repeat=2)))
+def test_the_type_of_the_sum(residual, scale):
+    """The residual's, or the MLP's own, whichever way the modules are called."""
+    a, _ = mlps(dtype=BF16)
+    torch.manual_seed(3)
+    x = torch.randn(2, 9, DIM, device=DEV).to(BF16)
+    r = None if residual is None else torch.randn(2, 9, DIM, device=DEV).to(residual)
+    s = None if scale is None else torch.randn(DIM, device=DEV).to(scale)
+    with torch.no_grad():
+        assert fused(lambda: a(x, r, s)) == (FP64 not in (residual, scale))
+        y = a(x, r, s)
+        hook = a.fc1.register_forward_hook(lambda m, i, o: None)
+        z = a(x, r, s)
+        hook.remove()
+    assert y.dtype == z.dtype == (residual or BF16)
+    near(y, z, 0.02)                                             # four roundings of 2^-9 in the modules, half as many in the products
+
+
+def test_a_sum_that_is_broadcast():
+    a, b = mlps(dtype=BF16)
+    x = torch.randn(2, 9, DIM, device=DEV).to(BF16)
+    row, s = torch.randn(DIM, device=DEV), torch.randn(DIM, device=DEV)
+    with torch.no_grad():
+        want = b(x)
+        for r, f in ((row, s), (row[None, None], None), (None, s[0]), (None, s[None, None]), (torch.randn(3, 2, 9, DIM, device=DEV), s), (torch.randn(2, 1, DIM, device=DEV), s[:1])):
+            y = a(x, r, f)
+            z = want.float() * (1 if f is None else f) + (0 if r is None else r)
+            assert y.shape == z.shape and y.dtype == (BF16 if r is None else FP32)
+            near(y, z, 0.01)

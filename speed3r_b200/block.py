@@ -70,7 +70,8 @@ class FusedMlp(Mlp):
         return "silu" if type(m) is nn.SiLU else None
 
     def _type(self, x) -> Optional[torch.dtype]:
-        if self._act() is None or _watched(self.drop) or (self.drop.p and self.drop.training):
+        d = self.drop
+        if self._act() is None or _watched(d) or not (type(d) is nn.Identity or (type(d) is nn.Dropout and not (d.p and d.training))):
             return None
         return product_type(x, self.fc1, self.fc2)
 

@@ -3,6 +3,7 @@ import itertools
 
 import pytest
 import torch
+from torch import nn
 
 from speed3r_b200 import _lib
 from test_gpu_block import DEV, DIM, near
@@ -52,3 +53,17 @@ def test_a_sum_that_is_broadcast():
             z = want.float() * (1 if f is None else f) + (0 if r is None else r)
             assert y.shape == z.shape and y.dtype == (BF16 if r is None else FP32)
             near(y, z, 0.01)
+
+
+def test_a_dropout_that_was_replaced():
+    class Half(nn.Module):
+        def forward(self, x):
+            return x * 0.5
+
+    x = torch.randn(3, DIM, device=DEV).to(BF16)
+    for drop, takes in ((nn.Identity(), True), (Half(), False), (nn.AlphaDropout(0.0), False), (nn.Dropout(0.5).eval(), True)):
+        a, b = mlps(dtype=BF16)
+        a.drop = b.drop = drop
+        with torch.no_grad():
+            assert fused(lambda: a(x)) == takes
+            near(a(x), b(x), 0.01)

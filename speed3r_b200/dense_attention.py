@@ -82,5 +82,6 @@ class FlashAttentionRope(nn.Module):
     def forward(self, x: Tensor, attn_bias=None, xpos: Optional[Tensor] = None) -> Tensor:
         B, N, C = x.shape
         q, k, v = self._heads(self._linear(self.qkv, x), xpos, B, N, C // self.num_heads)
-        y = nn.functional.scaled_dot_product_attention(q, k, v, attn_mask=attn_bias, dropout_p=self.attn_drop.p if self.training else 0.0)
+        drop = self.attn_drop                           # its own mode decides; an Identity has no p
+        y = nn.functional.scaled_dot_product_attention(q, k, v, attn_mask=attn_bias, dropout_p=getattr(drop, "p", 0.0) if drop.training else 0.0)
         return self.proj_drop(self._linear(self.proj, y.transpose(1, 2).reshape(B, N, C)))

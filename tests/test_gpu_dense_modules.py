@@ -7,7 +7,7 @@ from torch import nn
 
 from speed3r_b200 import _lib
 from test_gpu_block import DEV, DIM, near
-from test_gpu_dense_block import launched, mlps
+from test_gpu_dense_block import attention, launched, mlps
 
 pytestmark = pytest.mark.gpu
 BF16, F16, FP32, FP64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
@@ -67,3 +67,14 @@ def test_a_dropout_that_was_replaced():
         with torch.no_grad():
             assert fused(lambda: a(x)) == takes
             near(a(x), b(x), 0.01)
+
+
+def test_attention_goes_by_its_own_dropout():
+    m = attention(1, dtype=BF16, rope=None, attn_drop=0.5).train()
+    x = torch.randn(2, 50, DIM, device=DEV).to(BF16)
+    assert not torch.equal(m(x), m(x))
+    m.attn_drop.eval()
+    y = m(x)
+    assert torch.equal(y, m(x))
+    m.attn_drop = nn.Identity()
+    assert torch.equal(y, m.train()(x)) and torch.equal(y, m.eval()(x))

@@ -141,7 +141,10 @@ class BlockRope(nn.Module):
     @torch.no_grad()
     def quantize_int8(self) -> "BlockRope":
         """8-bit projections and MLP for inference, in place (parameters on the GPU).  The norms then hand over 8-bit tokens.  For an
-        MLP of two Linears ``fc1`` and ``fc2``; any other ``ffn_layer`` raises, and nothing is changed."""
+        MLP of two Linears ``fc1`` and ``fc2`` and an attention with an 8-bit form (``SparseFlashAttentionRope``); any other ``ffn_layer`` or
+        ``attn_class`` raises, and nothing is changed."""
+        if not callable(getattr(self.attn, "quantize_int8", None)):
+            raise RuntimeError(f"quantize_int8: {type(self.attn).__name__} has no 8-bit form")
         lins = [getattr(self.mlp, n, None) for n in ("fc1", "fc2")]
         if not all(isinstance(m, (nn.Linear, Int8Linear)) for m in lins):
             raise RuntimeError(f"quantize_int8: {type(self.mlp).__name__} is not an MLP of two Linears fc1 and fc2")

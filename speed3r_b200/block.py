@@ -207,7 +207,7 @@ class BlockRope(nn.Module):
 
     def _mlp_takes_int8(self) -> bool:
         """8-bit tokens are for the MLP whose first step is that Linear; another module is given activations."""
-        return type(self.mlp) is Mlp and type(self.mlp.fc1) is Int8Linear
+        return type(self.mlp) in (Mlp, FusedMlp) and type(self.mlp.fc1) is Int8Linear
 
     def _takes_int8(self) -> bool:
         return type(self.attn).forward is SparseFlashAttentionRope.forward and type(self.attn.qkv) is Int8Linear

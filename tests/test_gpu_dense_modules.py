@@ -5,8 +5,8 @@ import pytest
 import torch
 from torch import nn
 
-from speed3r_b200 import _lib
-from test_gpu_block import DEV, DIM, near
+from speed3r_b200 import FusedMlp, _lib, forward_blocks
+from test_gpu_block import DEV, DIM, block, near, positions
 from test_gpu_dense_block import attention, launched, mlps
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +78,15 @@ def test_attention_goes_by_its_own_dropout():
     assert torch.equal(y, m(x))
     m.attn_drop = nn.Identity()
     assert torch.equal(y, m.train()(x)) and torch.equal(y, m.eval()(x))
+
+
+def test_8_bit_blocks_with_either_mlp_are_one():
+    """Their norms hand over 8-bit tokens to both: the same kernels, the same bits."""
+    x, pos = torch.randn(2, 512, DIM, device=DEV), positions(2, 512)
+    kinds = [[block(i, **kw).eval().quantize_int8() for i in range(2)] for kw in ({}, dict(ffn_layer=FusedMlp))]
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        for blocks in kinds:
+            forward_blocks(blocks, x, pos)                       # what is set up once has been
+        names = [launched(lambda: forward_blocks(blocks, x, pos)) for blocks in kinds]
+        assert names[0] == names[1] and any("int8" in n for n in names[0])
+        assert torch.equal(*(forward_blocks(blocks, x, pos) for blocks in kinds))

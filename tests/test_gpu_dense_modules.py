@@ -80,6 +80,36 @@ def test_attention_goes_by_its_own_dropout():
     assert torch.equal(y, m.train()(x)) and torch.equal(y, m.eval()(x))
 
 
+@pytest.mark.parametrize("kw", [{}, dict(qk_norm=False), dict(rope=None), dict(norm_layer=lambda d: nn.RMSNorm(d, eps=1e-6)), dict(dim=4 * 48), dict(dim=4 * 128)])
+def test_gradient_of_the_projections_bias(kw):
+    """Of q, k and v: the sum over tokens of the projection's own gradient, in 32 bits; and for q and v the modules' (for k the sum nearly cancels
+    where rotation is slow: what is added to all keys alike changes no softmax)."""
+    C = kw.get("dim", DIM)
+    torch.manual_seed(2)
+    x, dy = torch.randn(3, 200, C, device=DEV), torch.randn(3, 200, C, device=DEV)
+    grads = []
+    for plain in (False, True):
+        m, kept = attention(1, plain=plain, **kw), []
+        heads = m._heads
+
+        def watched(qkv, *args):
+            qkv.retain_grad()
+            kept.append(qkv)
+            return heads(qkv, *args)
+
+        m._heads = watched
+        with torch.autocast("cuda", dtype=BF16):
+            y = m(x, xpos=positions(3, 200))
+        y.float().backward(dy)
+        grads.append(m.qkv.bias.grad)
+        if not plain:
+            d = kept[0].grad.double().flatten(0, 1)
+            # 600 terms, each addition off by at most 2^-24 of the magnitudes so far
+            assert ((grads[0].double() - d.sum(0)).abs() <= 600 * 2.0 ** -24 * d.abs().sum(0)).all() and (grads[0] != 0).any()
+    for i in (0, 2):
+        near(grads[0].view(3, C)[i], grads[1].view(3, C)[i], 0.04)           # as every other parameter's: about sixteen roundings of 2^-9
+
+
 def test_8_bit_blocks_with_either_mlp_are_one():
     """Their norms hand over 8-bit tokens to both: the same kernels, the same bits."""
     x, pos = torch.randn(2, 512, DIM, device=DEV), positions(2, 512)

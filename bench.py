@@ -471,7 +471,8 @@ def run_train_step(args):
 def run_block(args):
     """Forward of one transformer block around the sparse attention (1024 wide, MLP of 4096, bf16 autocast, no gradients) on `--views`
     views: its modules one by one, with the sums and norms in one pass, with the MLP's matrices, GELU and last sum as well, and with 8-bit
-    projections and MLP."""
+    projections and MLP.  The four are timed in turn, call by call."""
+    import copy
     import torch
     import speed3r_b200
     torch.cuda.set_device(0)
@@ -484,28 +485,29 @@ def run_block(args):
     xpos = torch.stack((tok // 36, tok % 36), -1)[None].contiguous()
     ev = lambda: torch.cuda.Event(enable_timing=True)
 
-    def timed():
-        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
-            for _ in range(max(3, args.warmup)):
-                y = blk(x, xpos)
-            a, b = ev(), ev()
-            a.record()
-            for _ in range(args.steps):
-                y = blk(x, xpos)
-            b.record()
-            torch.cuda.synchronize()
-        return a.elapsed_time(b) / args.steps, y
-
-    blk._fuses = lambda: False
-    apart, y0 = timed()
-    del blk._fuses
-    fused, y1 = timed()
-    mlp, blk.mlp = blk.mlp, speed3r_b200.FusedMlp(H * D, 4 * H * D).to(dev).eval()
-    blk.mlp.load_state_dict(mlp.state_dict())
-    fused_mlp, y3 = timed()
-    blk.mlp = mlp
-    blk.quantize_int8()
-    int8, y2 = timed()
+    # one block per form, called in turn: what a GPU at its power limit loses, all of them lose
+    apart, mlp, narrow = (copy.deepcopy(blk) for _ in range(3))
+    apart._fuses = lambda: False
+    mlp.mlp = speed3r_b200.FusedMlp(H * D, 4 * H * D).to(dev).eval()
+    mlp.mlp.load_state_dict(blk.mlp.state_dict())
+    narrow.quantize_int8()
+    forms = [apart, blk, mlp, narrow]
+    ends = []
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        outs = [f(x, xpos) for f in forms]
+        for _ in range(max(3, args.warmup) - 1):
+            for f in forms:
+                f(x, xpos)
+        for _ in range(args.steps):
+            ends.append([])
+            for f in forms:
+                ends[-1].append((ev(), ev()))
+                ends[-1][-1][0].record()
+                f(x, xpos)
+                ends[-1][-1][1].record()
+        torch.cuda.synchronize()
+    apart, fused, fused_mlp, int8 = (sum(r[i][0].elapsed_time(r[i][1]) for r in ends) / args.steps for i in range(len(forms)))
+    y0, y1, y3, y2 = outs
     off = lambda y: ((y - x).double() - (y0 - x).double()).norm().item() / (y0 - x).double().norm().item()
     print(json.dumps(dict(
         metric="block_forward_tokens_per_s", value=T / (fused * 1e-3), unit="tokens/s", n_gpus=1, steps=args.steps, warmup=max(3, args.warmup),

@@ -3,7 +3,7 @@
 ``BlockRope`` keeps the constructor keywords, sub-module names (``norm1``, ``attn``, ``ls1``, ``norm2``, ``mlp.fc1``, ``mlp.fc2``, ``ls2``) and
 ``forward(x, xpos=None)`` of pi3/models/layers/block.py:259-335, so that a checkpoint loads unchanged.  What stands between its
 sub-layers - LayerScale, stochastic depth, residual and the next norm - is ``ops.residual_norm``, one pass with gradients; the MLP's
-matrices stay PyTorch (cuBLAS) code, or become 8-bit products for inference (``quantize_int8``).  ``forward_blocks`` runs a list of blocks and
+matrices stay PyTorch (cuBLAS) code with ``Mlp``, are ``ops.linear`` with ``FusedMlp``, or become 8-bit products for inference (``quantize_int8``).  ``forward_blocks`` runs a list of blocks and
 takes the sum that ends a block and the norm that begins the next one in one pass as well.
 """
 from __future__ import annotations
@@ -58,8 +58,8 @@ def product_type(x, *linears: nn.Module) -> Optional[torch.dtype]:
 class FusedMlp(Mlp):
     """``Mlp`` whose matrices come with what follows them (``ops.linear``): the activation, and on request a LayerScale and the residual.  For
     ``BlockRope(ffn_layer=FusedMlp)``; parameters and results are ``Mlp``'s, but that nothing is rounded between a matrix and its activation.  Where
-    the kernel does not reach - other types than bf16 and fp16, active dropout, hooks, an activation other than GELU and SiLU - modules are called
-    one by one."""
+    the kernel does not reach - other types than bf16 and fp16, active dropout, hooks, an activation other than GELU and SiLU, a residual or scale
+    that is broadcast or has 64 bits - modules are called one by one.  Under autocast the weights are cast on every call."""
 
     def _act(self) -> Optional[str]:
         m = self.act

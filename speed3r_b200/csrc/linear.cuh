@@ -90,10 +90,13 @@ int linear_partial(const LinOperand& a, const LinOperand& b, int64_t k, bool bf1
 // a turned one comes in boxes of 64 rows x 64 steps and is read through the other form of the matrix descriptor.
 //
 // Bound: the tensor cores, and at full size the power they take.  64 512 x 4096 x 1024 in bf16: the products alone 322 us (1680 TFLOP/s), with GELU
-// 384 at first and 435 at the clock that power leaves.  What the epilogue takes must stay below the products' time: alone (K = 64) it is 103 us for a sum that
+// 388 at first and 458 at the clock that power leaves.  What the epilogue takes must stay below the products' time: alone (K = 64) it is 103 us for a sum that
 // is only rounded, 186 with SiLU, 234 with GELU, 376 with an fp32 residual, 391 for dz with GELU's slope and a sum over rows, of which the memory
 // traffic is 80, 80, 80, 320 and 161 (dz: dy read, dz written).  dz is the one that issues most: 40 % of all cycles, the tensor cores busy in 65 %
 // (forward with GELU 83 %).
+// Roundings: the tensor cores cut every addition to an fp32 sum off towards zero, so that over K = 4096 terms z is 4.4e-6 too small (a library's fp32
+// result of the same product, too), and d_scale with it.  dz is rounded to the operands' type, as its two products take it: half a step more in
+// dx and dW; two halves of 16 bits would keep it, for twice both products.
 // Tried, and slower: sixteen summing warps, which spill (166 -> 237, dz 375 -> 494); two pieces of output per warp where nothing is read beside the
 // sums (166 -> 172); two sets of dz's sums in registers (373 -> 395).
 // ---------------------------------------------------------------------------------------------------------------------
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const __grid_consta
       constexpr int per = WIDE ? 32 : 64;                            // columns of a piece
       constexpr int kMine = C::kSpan / 32, kPieces = OTHER == kNoOther ? 1 : 2;
       // A residual of the result's size comes by TMA into the piece that the sum leaves from, a piece ahead; rows that a lane reads from memory itself,
-      // 16 bytes of 32 lines at a time, took 1092 us for 64 512 x 4096 x 1024 in fp32 where this way takes 566.  Other residuals are
+      // 16 bytes of 32 lines at a time, took 1092 us for 64 512 x 4096 x 1024 in fp32 where this way takes 575.  Other residuals are
       // read 32 columns ahead.
       constexpr bool kInPlace = OTHER != kNoOther && (OTHER == S3R_F32) == WIDE;
       const bool by_copy = kInPlace && p.other_copied;

@@ -385,7 +385,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: Option
 
     ``x [.., K]`` and ``weight [N, K]`` both bf16 or both fp16; sums and all that follows them in fp32, one rounding to ``out_dtype`` (by default
     ``residual``'s type, else x's).  ``act``: None, ``"gelu"``, ``"gelu_tanh"`` or ``"silu"``.  ``bias`` and ``scale [N]`` and ``residual [.., N]`` are fp32,
-    bf16 or fp16, each of its own type.  The backward computes the sums again rather than keeping them.  Operands whose rows do not begin at
+    bf16 or fp16, each of its own type.  The backward computes the sums again rather than keeping them; the gradient in front of ``act``, of which those
+    of x and weight are products, is rounded to their type.  Operands whose rows do not begin at
     multiples of 16 bytes are laid out anew on every call."""
     if act not in _ACTS:
         raise RuntimeError(f"linear: act must be None, 'gelu', 'gelu_tanh' or 'silu', got {act!r}")
@@ -405,7 +406,7 @@ def qkv_norm_rope(qkv: Tensor, num_heads: int, kv_heads: Optional[int] = None, p
     ``q_norm`` and ``k_norm`` are ``(weight, bias, eps)``, weight and bias ``[d]`` or None, or None for no norm; ``kind`` as in ``residual_norm``.
     ``pos [B or 1, T, axes]`` (or ``[T, axes]``) are a token's integer positions, ``cos`` and ``sin [rows, W]`` the tables of sines and cosines: axis
     a turns the columns ``2 * W * a + i`` and ``2 * W * a + W + i``, i < W, by the angle of table row ``pos[.., a]`` and column i; columns from
-    ``2 * W * axes`` on are not turned.  (Of tables whose halves repeat, as ``RoPE2D`` makes them, hand over the first half.)  A position outside of
+    ``2 * W * axes`` on are not turned, and without a norm leave as they came.  (Of tables whose halves repeat, as ``RoPE2D`` makes them, hand over the first half.)  A position outside of
     the tables is clamped and sets a bit of the device's status word."""
     if kind not in _KINDS:
         raise RuntimeError(f"qkv_norm_rope: kind must be 'layer' or 'rms', got {kind!r}")
